@@ -361,17 +361,16 @@ def work(case):
         flops = 2 * m * k * n
         if not train:
             return {"bytes": size * (m * k + m * n) + n * k, "flops": flops}
-        return {"bytes": size * (3 * m * k + 2 * m * n + 3 * n * k), "flops": 3 * flops}
+        return {"bytes": 2 * size * (m * k + m * n + n * k), "flops": 3 * flops}
     if op in ("dropout", "norm"):
         e = case["tokens"] * case["dim"]
-        passes = 2 if not train else 4 if op == "dropout" else 5
-        return {"bytes": passes * e * size, "flops": (8 if op == "norm" else 2) * e * (3 if train else 1)}
+        return {"bytes": (4 if train else 2) * e * size, "flops": (8 if op == "norm" else 2) * e * (3 if train else 1)}
     rows = case["batch"] * case["tokens"]
     e = rows * case["dim"]
     gate = {"none": 0, "element": e, "sample": case["batch"] * case["dim"], "token": rows}[case["gate"]]
     words = 3 * e + (e if case["next"] else 0) + gate
-    if train:   # x, h, dout, dy and the gate again; dx, dh and the gate's gradient
-        words += 5 * e + (e if case["next"] else 0) + 2 * gate
+    if train:   # dout and dy; dx, dh and the gate's gradient
+        words += 3 * e + (e if case["next"] else 0) + gate
     return {"bytes": words * size, "flops": 16 * e * (3 if train else 1)}
 
 
