@@ -416,6 +416,61 @@ P3D_API int p3d_attn_bwd(const p3d_operator *op, const void *dy, const void *sk,
                  float *dglobal_scale, void *workspace, size_t workspace_bytes, void *stream);
 P3D_API size_t p3d_attn_bwd_workspace(const p3d_operator *op);
 
+/*
+ * The feed-forward half of a transformer block (pack3d_b200.residual).  No counterpart in the
+ * reference, whose layer ends at its own residual.
+ *
+ * p3d_dropout: y[r, c] = keep(r, c) * x[r, c] / (1 - p), p = threshold / 65536.  keep(r, c) is
+ *   whether 16-bit field c % 8 of the Philox-4x32-10 block at counter
+ *   (r * ceil(dim / 8) + c / 8, offset) under the key `seed` is at least threshold (0 .. 65536).
+ *   (seed, offset) are rng[0], rng[1] in device memory when rng is not NULL, else the two
+ *   arguments.  The gradient is the same call on dy.  x may equal y.
+ *
+ * p3d_residual: one row of dim columns at a time, in fp32,
+ *     u   = N_post(h) * post_weight + post_bias   (post_kind P3D_NORM_NONE: u = h)
+ *     d   = keep * u * act(gate) / (1 - p)        (gate_mode P3D_GATE_NONE: act = 1)
+ *     out = x + s * d                             (s: scale[dim], or scale_value when NULL)
+ *     y   = N_next(out) * next_weight + next_bias (of out before its rounding)
+ *   N: (z - mean) / sqrt(var + eps) for P3D_NORM_LAYER, z / sqrt(mean(z^2) + eps) for P3D_NORM_RMS.
+ *   h NULL: out = x and y = N_next(x); out is not written.  Biases may be NULL.  gate: [rows, dim]
+ *   (ELEMENT), [rows / rows_per_sample, dim] (SAMPLE) or [rows] (TOKEN).  x, h, gate, out, y in
+ *   dtype, the parameters in param_dtype (dtype or P3D_F32).  dim 1 .. 16384.
+ * p3d_residual_fwd: out, y [rows, dim]; stats [rows, 4] fp32 (mean and 1/deviation of h, then of
+ *   out) or NULL.
+ * p3d_residual_bwd: from dout and dy (either may be NULL: zero) and the stats: dx, dh [rows, dim],
+ *   dgate in dtype, and the parameters' gradients in param_dtype, each summed over its rows in a
+ *   fixed order (bitwise repeatable).  Outputs that are NULL are not written.  out is made again
+ *   from x and h.  workspace: p3d_residual_bwd_workspace() bytes.
+ */
+#define P3D_NORM_NONE 0
+#define P3D_NORM_RMS 1
+#define P3D_NORM_LAYER 2
+#define P3D_GATE_NONE 0
+#define P3D_GATE_ELEMENT 1
+#define P3D_GATE_SAMPLE 2
+#define P3D_GATE_TOKEN 3
+#define P3D_ACT_IDENTITY 0
+#define P3D_ACT_SIGMOID 1
+#define P3D_ACT_TANH 2
+typedef struct {
+  int64_t rows, rows_per_sample;
+  const void *x, *h, *gate;
+  const void *post_weight, *post_bias, *scale, *next_weight, *next_bias;
+  const uint64_t *rng;
+  uint64_t seed, offset;
+  int32_t dim, dtype, param_dtype, post_kind, next_kind, gate_mode, gate_act;
+  uint32_t threshold; /* dropout: p * 65536 */
+  float post_eps, next_eps, scale_value;
+} p3d_residual;
+P3D_API int p3d_dropout(const void *x, void *y, int dtype, int64_t rows, int64_t dim, uint32_t threshold,
+                const uint64_t *rng, uint64_t seed, uint64_t offset, void *stream);
+P3D_API int p3d_residual_fwd(const p3d_residual *args, void *out, void *y, float *stats, void *stream);
+P3D_API size_t p3d_residual_bwd_workspace(const p3d_residual *args);
+P3D_API int p3d_residual_bwd(const p3d_residual *args, const void *dout, const void *dy, const float *stats, void *dx,
+                     void *dh, void *dgate, void *dscale, void *dpost_weight, void *dpost_bias,
+                     void *dnext_weight, void *dnext_bias, void *workspace, size_t workspace_bytes,
+                     void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -6,6 +6,7 @@ has not been built (``python -m pack3d_b200.build``); there is no fallback.
 from __future__ import annotations
 
 import ctypes
+import struct
 import threading
 from pathlib import Path
 
@@ -61,6 +62,10 @@ class PeerCopy(ctypes.Structure):
                 ("src_stride", ctypes.c_int64), ("dst_stride", ctypes.c_int64)]
 
 
+#: ``p3d_residual`` of ``include/pack3d_b200.h``, packed by :mod:`pack3d_b200.residual` for each call (packing the
+#: bytes takes a fraction of the time of filling a ctypes structure field by field)
+RESIDUAL = struct.Struct("@2q9P2Q7iI3f4x")
+
 PEER_HANDLE_BYTES = 64
 PEER_MAX_COPIES = 32
 PEER_MAX_TARGETS = 16
@@ -110,6 +115,11 @@ _SIGNATURES = {
     "p3d_attn_bwd": (_c_int, [ctypes.POINTER(Operator), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
                               _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, ctypes.c_size_t, _vp]),
     "p3d_attn_bwd_workspace": (ctypes.c_size_t, [ctypes.POINTER(Operator)]),
+    "p3d_dropout": (_c_int, [_vp, _vp, _c_int, _c_i64, _c_i64, ctypes.c_uint32, _vp, ctypes.c_uint64,
+                             ctypes.c_uint64, _vp]),
+    "p3d_residual_fwd": (_c_int, [_vp] * 5),
+    "p3d_residual_bwd_workspace": (ctypes.c_size_t, [_vp]),
+    "p3d_residual_bwd": (_c_int, [_vp] * 13 + [ctypes.c_size_t, _vp]),
     "p3d_peer_alloc": (_c_int, [ctypes.c_size_t, ctypes.POINTER(_vp), _vp]),
     "p3d_peer_free": (_c_int, [_vp]),
     "p3d_peer_open": (_c_int, [_vp, ctypes.POINTER(_vp)]),

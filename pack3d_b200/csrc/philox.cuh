@@ -1,0 +1,62 @@
+// Counter-based random bits for dropout: Philox-4x32 with ten rounds (Salmon, Moraes, Dror,
+// Shaw, "Parallel random numbers: as easy as 1, 2, 3", SC 2011).  A 128-bit counter under a
+// 64-bit key gives 128 bits, so any element's bits can be made again from its position alone
+// and no mask is ever stored.
+#pragma once
+
+#include <stdint.h>
+
+namespace p3d {
+
+struct PhiloxKey {
+  uint64_t seed, offset;
+};
+
+// Seed and offset of a call: by value, or from device memory when `rng` is not null (a captured
+// graph then draws new bits at each replay that advances it).
+__device__ __forceinline__ PhiloxKey philox_key(const uint64_t *rng, uint64_t seed, uint64_t offset) {
+  if (rng != nullptr) return PhiloxKey{rng[0], rng[1]};
+  return PhiloxKey{seed, offset};
+}
+
+__device__ __forceinline__ uint4 philox(PhiloxKey key, uint64_t block) {
+  uint32_t c0 = (uint32_t)block, c1 = (uint32_t)(block >> 32);
+  uint32_t c2 = (uint32_t)key.offset, c3 = (uint32_t)(key.offset >> 32);
+  uint32_t k0 = (uint32_t)key.seed, k1 = (uint32_t)(key.seed >> 32);
+#pragma unroll
+  for (int round = 0; round < 10; ++round) {
+    const uint64_t p0 = (uint64_t)0xD2511F53u * c0, p1 = (uint64_t)0xCD9E8D57u * c2;
+    c0 = (uint32_t)(p1 >> 32) ^ c1 ^ k0;
+    c2 = (uint32_t)(p0 >> 32) ^ c3 ^ k1;
+    c1 = (uint32_t)p1;
+    c3 = (uint32_t)p0;
+    k0 += 0x9E3779B9u;
+    k1 += 0xBB67AE85u;
+  }
+  return make_uint4(c0, c1, c2, c3);
+}
+
+// The eight keep decisions of a block as bits: element j is kept when its 16-bit field (field
+// j % 2 of word j / 2, low half first) is at least `threshold`, so the drop probability is
+// threshold / 65536.  Sixteen bits an element instead of 32 halve the rounds; the probability
+// asked for is met within 2^-17.
+__device__ __forceinline__ uint32_t keep_bits(PhiloxKey key, uint64_t block, uint32_t threshold) {
+  const uint4 r = philox(key, block);
+  uint32_t bits = 0;
+  bits |= (r.x & 0xffffu) >= threshold ? 1u : 0u;
+  bits |= (r.x >> 16) >= threshold ? 2u : 0u;
+  bits |= (r.y & 0xffffu) >= threshold ? 4u : 0u;
+  bits |= (r.y >> 16) >= threshold ? 8u : 0u;
+  bits |= (r.z & 0xffffu) >= threshold ? 16u : 0u;
+  bits |= (r.z >> 16) >= threshold ? 32u : 0u;
+  bits |= (r.w & 0xffffu) >= threshold ? 64u : 0u;
+  bits |= (r.w >> 16) >= threshold ? 128u : 0u;
+  return bits;
+}
+
+// 1 / (1 - p) of the probability actually used; 0 when everything is dropped.
+__host__ __device__ inline float keep_scale(uint32_t threshold) {
+  return threshold >= 65536u ? 0.f : 65536.f / (float)(65536u - threshold);
+}
+
+}  // namespace p3d

@@ -1,0 +1,374 @@
+"""norm, residual_norm and dropout against plain implementations in 64 bits.
+
+Tolerances: the kernels compute in fp32 and round each output once to its type, so an element may be off by half an
+ulp of its type (2^-8 of the value in bf16, with its 8-bit significand, 2^-11 in fp16, 2^-24 in fp32) plus fp32's own
+error, a few ulps of the terms that make it up: the terms here are of order one, up to eight, and 64 ulps of that
+(2^-18 * 8) cover the ten or so operations and the row sums.  Sums over R rows of fp32 terms add independent
+roundings: sqrt(R) * 2^-22 of the terms' norm, which is sqrt(R) times their size (four).
+"""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+ULP = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+LOW = 0xFFFFFFFF
+
+
+def philox_fields(block, rng):
+    """The eight 16-bit fields of one block, in Python integers."""
+    seed, offset = rng
+    c = [block & LOW, block >> 32, offset & LOW, (offset >> 32) & LOW]
+    k = [seed & LOW, (seed >> 32) & LOW]
+    for _ in range(10):
+        p0, p1 = 0xD2511F53 * c[0], 0xCD9E8D57 * c[2]
+        c = [(p1 >> 32) ^ c[1] ^ k[0], p1 & LOW, (p0 >> 32) ^ c[3] ^ k[1], p0 & LOW]
+        k = [(k[0] + 0x9E3779B9) & LOW, (k[1] + 0xBB67AE85) & LOW]
+    return [f for w in c for f in (w & 0xFFFF, w >> 16)]
+
+
+def keep_mask(rows, dim, p, rng):
+    blocks = -(-dim // 8)
+    t = round(65536 * p)
+    m = torch.empty(rows, dim, dtype=torch.bool)
+    for r in range(rows):
+        fields = [f for b in range(blocks) for f in philox_fields(r * blocks + b, rng)]
+        m[r] = torch.tensor(fields[:dim]) >= t
+    return m
+
+
+def test_philox_known_answers():
+    """The published known-answer vectors of philox4x32-10 (counter and key all zeros, all ones)."""
+    def words(fields):
+        return [fields[2 * i] | fields[2 * i + 1] << 16 for i in range(4)]
+    assert words(philox_fields(0, (0, 0))) == [0x6627E8D5, 0xE169C58D, 0xBC57AC4C, 0x9B00DBD8]
+    ones = 0xFFFFFFFFFFFFFFFF
+    assert words(philox_fields(ones, (ones, ones))) == [0x408F276D, 0x41C83B0E, 0xA20BC7C6, 0x6D5451FD]
+
+
+@pytest.mark.parametrize("shape", [(1,), (7,), (3, 5), (2, 3, 8), (33, 64), (5, 195), (4, 1000), (1, 8192 + 3)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("p", [0.0, 0.1, 0.5, 1.0])
+def test_dropout_matches_its_definition(cuda_device, shape, dtype, p):
+    from pack3d_b200 import dropout
+    rng = (0x123456789ABCDEF, (1 << 40) + 5)
+    x = torch.randn(shape, generator=torch.Generator().manual_seed(1)).to(dtype)
+    keep = keep_mask(x.numel() // shape[-1], shape[-1], p, rng).view(shape)
+    t = round(65536 * p)
+    want = torch.where(keep, x.double() * (65536 / (65536 - t) if t < 65536 else 0.0), 0.0)
+    xd = x.to(cuda_device).requires_grad_()
+    y = dropout(xd, p, rng)
+    assert y.dtype == dtype and y.shape == shape
+    assert torch.equal(y.cpu() != 0, (want != 0))
+    subnormal = 2.0 ** -25 if dtype == torch.float16 else 0.0      # half a step of fp16 below 2^-14
+    assert ((y.cpu().double() - want).abs() <= want.abs() * (ULP[dtype] + 2.0 ** -23) + subnormal).all()
+    dy = torch.randn(shape, generator=torch.Generator().manual_seed(2)).to(dtype)
+    dx, = torch.autograd.grad(y, [xd], dy.to(cuda_device))
+    back = torch.where(keep, dy.double() * (65536 / (65536 - t) if t < 65536 else 0.0), 0.0)
+    assert ((dx.cpu().double() - back).abs() <= back.abs() * (ULP[dtype] + 2.0 ** -23) + subnormal).all()
+    device_rng = torch.tensor(rng, dtype=torch.int64, device=cuda_device)
+    assert torch.equal(dropout(xd, p, device_rng), y)
+
+
+def test_dropout_drops_what_is_not_finite(cuda_device):
+    from pack3d_b200 import dropout
+    x = torch.full((64, 96), float("nan"), device=cuda_device)
+    x[::2] = float("inf")
+    rng = (3, 4)
+    keep = keep_mask(64, 96, 0.5, rng).to(cuda_device)
+    y = dropout(x, 0.5, rng)
+    assert (y[~keep] == 0).all() and not torch.isfinite(y[keep]).any()
+
+
+def test_dropout_strides_alignment_and_streams(cuda_device):
+    from pack3d_b200 import dropout
+    rng = (9, 1)
+    base = torch.randn(40, 65, device=cuda_device, dtype=torch.bfloat16)
+    want = dropout(base[:, 1:].contiguous(), 0.3, rng)
+    assert torch.equal(dropout(base[:, 1:], 0.3, rng), want)
+    odd = torch.empty(40 * 64 + 1, device=cuda_device, dtype=torch.bfloat16)[1:].view(40, 64)
+    odd.copy_(base[:, 1:])
+    assert odd.data_ptr() % 16 and torch.equal(dropout(odd, 0.3, rng), want)
+    t = torch.randn(64, 40, device=cuda_device, dtype=torch.bfloat16)
+    assert torch.equal(dropout(t.t(), 0.3, rng), dropout(t.t().contiguous(), 0.3, rng))
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        other = dropout(odd, 0.3, rng)
+    torch.cuda.current_stream().wait_stream(stream)
+    assert torch.equal(other, want)
+    assert dropout(base[:0], 0.3, rng).shape == (0, 65)
+
+
+def test_dropout_rate(cuda_device):
+    from pack3d_b200 import dropout
+    n = 1 << 20
+    y = dropout(torch.ones(n, device=cuda_device), 0.1, (11, 12))
+    dropped = (y == 0).double().mean().item()
+    assert abs(dropped - 0.1) < 6 * (0.1 * 0.9 / n) ** 0.5 + 2.0 ** -17
+    again = dropout(torch.ones(n, device=cuda_device), 0.1, (11, 13))
+    both = ((y == 0) & (again == 0)).double().mean().item()     # another offset: independent bits
+    assert abs(both - 0.01) < 6 * (0.01 * 0.99 / n) ** 0.5 + 2.0 ** -17
+
+
+# ------------------------------------------------------------------------------- norms
+def plain_norm(z, spec):
+    if spec is None:
+        return z
+    w, b, kind, eps = spec
+    if kind == "layer":
+        z = z - z.mean(-1, keepdim=True)
+    z = z / torch.sqrt(z.square().mean(-1, keepdim=True) + eps)
+    z = z if w is None else z * w
+    return z if b is None else z + b
+
+
+ACT = {"identity": lambda t: t, "sigmoid": torch.sigmoid, "tanh": torch.tanh}
+
+
+def plain_residual(x, h, post, gate, act, scale, nxt, keep, keep_scale):
+    u = plain_norm(h, post)
+    if gate is not None:
+        u = u * ACT[act](gate)
+    if keep is not None:
+        u = torch.where(keep, u * keep_scale, torch.zeros_like(u))
+    out = x + (u if scale is None else scale * u)
+    return out, (None if nxt is None else plain_norm(out, nxt))
+
+
+def close(got, want, dtype, summed=1):
+    """Whether got is want rounded to dtype after fp32 arithmetic; `summed`: how many rows or columns were added up."""
+    got, want = got.detach().double().cpu(), want.detach().double().cpu()
+    slack = 2.0 ** -18 * 8 + (summed * 2.0 ** -22 * 4 if summed > 1 else 0) + (2.0 ** -25 if dtype == torch.float16 else 0)
+    worst = ((got - want).abs() - want.abs() * (ULP[dtype] * 1.01 + 2.0 ** -20) - slack).max().item() if got.numel() else 0
+    assert worst <= 0, worst
+
+
+def make(shape, dtype, device, seed, mean=0.0, std=1.0):
+    return (torch.randn(shape, generator=torch.Generator().manual_seed(seed)) * std + mean).to(dtype).to(device)
+
+
+def check_residual(device, shape, dtype, kind="rms", gate=None, act="identity", p=0.0, post=True, nxt=True, scale=True,
+                   bias=True, pdtype=None, seed=0, use_y=True, use_out=True):
+    from pack3d_b200 import NormSpec, residual_norm
+    pdtype = pdtype or dtype
+    dim = shape[-1]
+    x, h = make(shape, dtype, device, seed, 0.3, 1.5), make(shape, dtype, device, seed + 1, -0.2, 0.7)
+    gate_shape = {None: None, "element": shape, "token": (*shape[:-1], 1), "sample": (shape[0], *(1,) * (len(shape) - 2), dim),
+                  "all": (dim,)}[gate]
+    leaves = {"x": x, "h": h}
+    if gate_shape is not None:
+        leaves["gate"] = make(gate_shape, dtype, device, seed + 2)
+    if post:
+        leaves["pw"] = make((dim,), pdtype, device, seed + 3, 1.0, 0.2)
+        if bias:
+            leaves["pb"] = make((dim,), pdtype, device, seed + 4, 0.0, 0.2)
+    if scale is True:
+        leaves["scale"] = make((dim,), pdtype, device, seed + 5, 0.5, 0.2)
+    if nxt:
+        leaves["nw"] = make((dim,), pdtype, device, seed + 6, 1.0, 0.2)
+        if bias:
+            leaves["nb"] = make((dim,), pdtype, device, seed + 7, 0.0, 0.2)
+    for t in leaves.values():
+        t.requires_grad_()
+    exact = {k: t.detach().double().requires_grad_() for k, t in leaves.items()}
+    rng = (seed + 77, seed + 5)
+    t = round(65536 * p)
+    rows = x.numel() // dim
+    keep = keep_mask(rows, dim, p, rng).view(shape).to(device) if t else None
+    eps = 1e-5
+
+    def spec(w, b, of, cls):
+        return cls((of.get(w), of.get(b), kind, eps)) if cls is tuple else cls(of.get(w), of.get(b), kind, eps)
+
+    value = scale if not isinstance(scale, bool) else None
+    out, y = residual_norm(x, h, post_norm=spec("pw", "pb", leaves, NormSpec) if post else None, gate=leaves.get("gate"),
+                           gate_activation=act, scale=leaves.get("scale", value),
+                           next_norm=spec("nw", "nb", leaves, NormSpec) if nxt else None, p=p, rng=rng)
+    want_out, want_y = plain_residual(exact["x"], exact["h"], spec("pw", "pb", exact, tuple) if post else None,
+                                      exact.get("gate"), act, exact.get("scale", value),
+                                      spec("nw", "nb", exact, tuple) if nxt else None, keep,
+                                      65536 / (65536 - t) if t < 65536 else 0.0)
+    close(out, want_out, dtype)
+    if nxt:
+        close(y, want_y, dtype)
+    else:
+        assert y is None
+    dout, dy = make(shape, dtype, device, seed + 8), make(shape, dtype, device, seed + 9)
+    got_of, want_of, up = [], [], []
+    if use_out:
+        got_of, want_of, up = [out], [want_out], [dout]
+    if nxt and use_y:
+        got_of, want_of, up = got_of + [y], want_of + [want_y], up + [dy]
+    names = [n for n in leaves if nxt and use_y or n not in ("nw", "nb")]
+    got = torch.autograd.grad(got_of, [leaves[n] for n in names], up)
+    want = torch.autograd.grad(want_of, [exact[n] for n in names], [u.double() for u in up])
+    for name, a, b in zip(names, got, want):
+        assert a.dtype == leaves[name].dtype and a.shape == leaves[name].shape, name
+        summed = rows if name in ("pw", "pb", "scale", "nw", "nb") else dim if gate == "token" and name == "gate" else \
+            rows // shape[0] if gate == "sample" and name == "gate" else rows if name == "gate" and gate == "all" else 1
+        close(a, b, a.dtype, summed)
+    again = torch.autograd.grad(
+        [v for v, u in zip(residual_norm(x, h, post_norm=spec("pw", "pb", leaves, NormSpec) if post else None,
+                                         gate=leaves.get("gate"), gate_activation=act, scale=leaves.get("scale", value),
+                                         next_norm=spec("nw", "nb", leaves, NormSpec) if nxt else None, p=p, rng=rng),
+                           (use_out, nxt and use_y)) if u], [leaves[n] for n in names], up)
+    assert all(torch.equal(a, b) for a, b in zip(got, again))    # bitwise repeatable
+
+
+SHAPES = [(1, 1), (1, 2048), (3, 7), (2, 5, 8), (2, 9, 192), (5, 33, 200), (37, 255), (3, 1001), (2, 3, 4096), (3, 4104),
+          (2, 8193), (2, 16384), (2, 16383)]
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+def test_residual_shapes(cuda_device, shape, dtype, kind):
+    check_residual(cuda_device, shape, dtype, kind, gate="element", act="sigmoid", p=0.25 if shape[-1] < 300 else 0.0)
+
+
+@pytest.mark.parametrize("gate,act", [(None, "identity"), ("element", "tanh"), ("token", "sigmoid"), ("sample", "identity"),
+                                      ("all", "tanh")])
+@pytest.mark.parametrize("post", [True, False])
+@pytest.mark.parametrize("nxt", [True, False])
+@pytest.mark.parametrize("scale", [True, False, 0.5])
+@pytest.mark.parametrize("dim", [96, 101])
+def test_residual_forms(cuda_device, gate, act, post, nxt, scale, dim):
+    check_residual(cuda_device, (3, 50, dim), torch.bfloat16, "layer", gate, act, 0.1, post, nxt, scale, seed=dim)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("bias", [True, False])
+def test_residual_fp32_parameters(cuda_device, dtype, bias):
+    check_residual(cuda_device, (4, 130, 320), dtype, "layer", "sample", "sigmoid", bias=bias, pdtype=torch.float32)
+    check_residual(cuda_device, (4, 130, 321), dtype, "rms", "token", "tanh", bias=bias, pdtype=torch.float32)
+
+
+@pytest.mark.parametrize("use_out,use_y", [(True, False), (False, True)])
+def test_residual_one_output_used(cuda_device, use_out, use_y):
+    check_residual(cuda_device, (7, 11, 136), torch.bfloat16, "layer", "element", "sigmoid", 0.2, use_out=use_out,
+                   use_y=use_y)
+
+
+@pytest.mark.parametrize("batch,tokens", [(1, 5000), (700, 3), (40, 130), (1300, 1)])
+def test_residual_many_rows_and_samples(cuda_device, batch, tokens):
+    check_residual(cuda_device, (batch, tokens, 40), torch.float32, "layer", "sample", "identity", seed=batch)
+
+
+def test_residual_large_offset_mean(cuda_device):
+    """A mean a thousand deviations away: squares about the mean, not a difference of squares."""
+    from pack3d_b200 import NormSpec, norm
+    z = 1000 + torch.randn(9, 512, generator=torch.Generator().manual_seed(3))
+    y = norm(z.to(cuda_device), NormSpec(kind="layer", eps=0.0)).cpu().double()
+    want = plain_norm(z.double(), (None, None, "layer", 0.0))
+    assert (y - want).abs().max() < 1000 * 2.0 ** -23 * 8      # the mean's own rounding, over a deviation of one
+
+
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+def test_rows_of_zeros_infinity_and_nan(cuda_device, kind):
+    """A row of zeros norms to its bias; a row with NaN or infinities touches no other row."""
+    from pack3d_b200 import NormSpec, norm, residual_norm
+    x = torch.randn(6, 72, device=cuda_device)
+    x[1] = 0
+    w, b = torch.rand(72, device=cuda_device), torch.rand(72, device=cuda_device)
+    spec = NormSpec(w, b, kind)
+    clean = norm(x, spec)
+    assert torch.equal(clean[1], b)
+    bad = x.clone()
+    bad[2, 5], bad[4, 70] = float("nan"), float("inf")
+    y = norm(bad, spec)
+    good = [0, 1, 3, 5]
+    assert torch.equal(y[good], clean[good]) and y[2].isnan().all() and not y[4].isfinite().all()
+    out, y2 = residual_norm(x, bad, post_norm=spec, next_norm=spec)
+    ref, ref2 = residual_norm(x, x, post_norm=spec, next_norm=spec)
+    assert torch.equal(out[good], ref[good]) and torch.equal(y2[good], ref2[good])
+
+
+def test_residual_dropout_is_dropout(cuda_device):
+    """With nothing else asked for, the fused call adds exactly what dropout() gives."""
+    from pack3d_b200 import dropout, residual_norm
+    for dim in (64, 77):
+        h = torch.randn(21, dim, device=cuda_device)
+        out, _ = residual_norm(torch.zeros_like(h), h, p=0.4, rng=(5, 6))
+        assert torch.equal(out, dropout(h, 0.4, (5, 6)))
+
+
+def test_residual_strides_alignment_and_empty(cuda_device):
+    from pack3d_b200 import NormSpec, residual_norm
+    big = torch.randn(12, 2 * 80 + 2, device=cuda_device, dtype=torch.bfloat16)
+    x, h = big[:, :80], big[:, 81:161]
+    w = torch.rand(81, device=cuda_device, dtype=torch.bfloat16)[1:]
+    spec = NormSpec(w)
+    want = residual_norm(x.contiguous(), h.contiguous(), post_norm=NormSpec(w.clone()), next_norm=NormSpec(w.clone()))
+    got = residual_norm(x, h, post_norm=spec, next_norm=spec)
+    for a, b in zip(got, want):
+        assert (a.float() - b.float()).abs().max() <= 2.0 ** -8 * b.float().abs().max()   # other summation order
+    e = torch.empty(0, 3, 80, device=cuda_device, requires_grad=True)
+    w32 = torch.ones(80, device=cuda_device, requires_grad=True)
+    out, y = residual_norm(e, e * 1, post_norm=NormSpec(w32), next_norm=NormSpec(w32))
+    g = torch.autograd.grad(out.sum() + y.sum(), [e, w32])
+    assert out.shape == y.shape == (0, 3, 80) and g[0].shape == (0, 3, 80) and (g[1] == 0).all()
+
+
+def test_norm_matches_residual_and_gradient_by_differences(cuda_device):
+    """norm() by itself, and its gradient against central differences in 64 bits of the plain form."""
+    from pack3d_b200 import NormSpec, norm
+    for kind in ("rms", "layer"):
+        x = make((5, 40), torch.float32, cuda_device, 4).requires_grad_()
+        w = make((40,), torch.float32, cuda_device, 5, 1.0, 0.3).requires_grad_()
+        dy = make((5, 40), torch.float32, cuda_device, 6)
+        y = norm(x, NormSpec(w, None, kind))
+        close(y, plain_norm(x.double(), (w.double(), None, kind, 1e-6)), torch.float32)
+        dx, dw = torch.autograd.grad(y, [x, w], dy)
+
+        def loss(xd, wd):
+            return (plain_norm(xd, (wd, None, kind, 1e-6)) * dy.double()).sum()
+
+        for t, d in ((x, dx), (w, dw)):
+            probe = torch.randn(t.shape, generator=torch.Generator().manual_seed(8)).double().to(cuda_device)
+            step = 1e-5
+            xs, ws = x.detach().double(), w.detach().double()
+            at = [(xs + s * probe, ws) if t is x else (xs, ws + s * probe) for s in (step, -step)]
+            numeric = (loss(*at[0]) - loss(*at[1])) / (2 * step)
+            analytic = (d.double() * probe).sum()
+            # central differences err by step^2, the gradient by fp32 roundings of 200 terms of order one
+            assert abs(numeric - analytic) < 1e-3
+
+
+def test_refusals(cuda_device):
+    from pack3d_b200 import NormSpec, dropout, norm, residual_norm
+    x = torch.randn(4, 6, 32, device=cuda_device)
+    w = torch.ones(32, device=cuda_device)
+    with pytest.raises(ValueError, match="between 0 and 1"):
+        dropout(x, 1.5, (1, 2))
+    with pytest.raises(ValueError, match="between 0 and 1"):
+        dropout(x, float("nan"), (1, 2))
+    for rng in (None, 3, (1,), torch.zeros(2, device=cuda_device), torch.zeros(2, dtype=torch.int64)):
+        with pytest.raises(ValueError, match="rng"):
+            dropout(x, 0.5, rng)
+    with pytest.raises(ValueError, match="CUDA"):
+        dropout(x.double(), 0.5, (1, 2))
+    with pytest.raises(ValueError, match="shape"):
+        norm(x, NormSpec(w[:16]))
+    with pytest.raises(ValueError, match="kind"):
+        norm(x, NormSpec(w, None, "batch"))
+    with pytest.raises(ValueError, match="eps"):
+        norm(x, NormSpec(w, None, "rms", -1.0))
+    with pytest.raises(ValueError, match="parameters must be"):
+        norm(x, NormSpec(w.half()))
+    with pytest.raises(ValueError, match="same device"):
+        norm(x, NormSpec(w.cpu()))
+    with pytest.raises(ValueError, match="last dimension"):
+        norm(torch.randn(2, 16385, device=cuda_device), NormSpec())
+    with pytest.raises(ValueError, match="NormSpec"):
+        norm(x, w)
+    with pytest.raises(ValueError, match="h must"):
+        residual_norm(x, x[:2])
+    with pytest.raises(ValueError, match="gate must"):
+        residual_norm(x, x, gate=torch.ones(4, 6, 16, device=cuda_device))
+    with pytest.raises(ValueError, match="gate must"):
+        residual_norm(x, x, gate=torch.ones(2, 1, 32, device=cuda_device))
+    with pytest.raises(ValueError, match="gate_activation"):
+        residual_norm(x, x, gate=x, gate_activation="relu")
+    with pytest.raises(ValueError, match="rng"):
+        residual_norm(x, x, p=0.5)
