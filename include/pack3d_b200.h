@@ -471,6 +471,35 @@ P3D_API int p3d_residual_bwd(const p3d_residual *args, const void *dout, const v
                      void *dnext_weight, void *dnext_bias, void *workspace, size_t workspace_bytes,
                      void *stream);
 
+/*
+ * 8-bit matrices with one power-of-two scale for each block of 128 (pack3d_b200.fp8).  No
+ * counterpart in the reference.  A matrix is e4m3 values [rows, pitch] (pitch a multiple of 16
+ * bytes, at least cols) and scale bytes e + 127: the value is v * 2^e.  Blocks run along the
+ * columns: block b of a row is columns [128 b, 128 b + 128).  The scales of 128 rows and four blocks
+ * are 512 consecutive bytes, row r's block b at (r % 32) * 16 + (r % 128) / 32 * 4 + b % 4;
+ * p3d_fp8_scale_bytes(rows, cols) in all.  e is the smallest integer with amax / 2^e <= 448, amax the
+ * largest finite magnitude of the block, at least -126, and 0 for a block of zeros; values are
+ * rounded to nearest even; NaN and infinities become NaN.
+ *
+ * p3d_fp8_quantize: x [rows, cols] of dtype, contiguous.  Any of: q and scales (1 x 128 blocks, or 128 x
+ *   128 blocks with square, the scale written for each row), the transposed qt [cols, t_pitch]
+ *   and t_scales (blocks of 128 rows of x, or the same square ones), col_sum [cols] of
+ *   col_sum_dtype (sums of x over its rows in fp32, fixed order; workspace of
+ *   p3d_fp8_quantize_workspace() bytes).
+ * p3d_fp8_matmul: out [rows, cols] of out_dtype = a [rows, k] b [cols, k]^T (+ bias [cols]), both with their
+ *   scales, fp32 accumulation on the tensor cores.  The sum over k is cut in a fixed way where there
+ *   are few tiles: bitwise repeatable.  workspace: p3d_fp8_matmul_workspace() bytes (may be 0).
+ */
+P3D_API int64_t p3d_fp8_scale_bytes(int64_t rows, int64_t cols);
+P3D_API size_t p3d_fp8_quantize_workspace(int64_t rows, int64_t cols);
+P3D_API int p3d_fp8_quantize(const void *x, int dtype, int64_t rows, int64_t cols, int square, void *q, int64_t pitch,
+                     void *scales, void *qt, int64_t t_pitch, void *t_scales, void *col_sum, int col_sum_dtype,
+                     void *workspace, size_t workspace_bytes, void *stream);
+P3D_API size_t p3d_fp8_matmul_workspace(int64_t rows, int64_t cols, int64_t k);
+P3D_API int p3d_fp8_matmul(const void *a, int64_t a_pitch, const void *a_scales, const void *b, int64_t b_pitch,
+                   const void *b_scales, int64_t rows, int64_t cols, int64_t k, const void *bias, int bias_dtype,
+                   void *out, int out_dtype, void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

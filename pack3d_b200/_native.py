@@ -120,6 +120,13 @@ _SIGNATURES = {
     "p3d_residual_fwd": (_c_int, [_vp] * 5),
     "p3d_residual_bwd_workspace": (ctypes.c_size_t, [_vp]),
     "p3d_residual_bwd": (_c_int, [_vp] * 13 + [ctypes.c_size_t, _vp]),
+    "p3d_fp8_scale_bytes": (_c_i64, [_c_i64, _c_i64]),
+    "p3d_fp8_quantize_workspace": (ctypes.c_size_t, [_c_i64, _c_i64]),
+    "p3d_fp8_quantize": (_c_int, [_vp, _c_int, _c_i64, _c_i64, _c_int, _vp, _c_i64, _vp, _vp, _c_i64, _vp, _vp, _c_int,
+                                  _vp, ctypes.c_size_t, _vp]),
+    "p3d_fp8_matmul_workspace": (ctypes.c_size_t, [_c_i64] * 3),
+    "p3d_fp8_matmul": (_c_int, [_vp, _c_i64, _vp, _vp, _c_i64, _vp, _c_i64, _c_i64, _c_i64, _vp, _c_int, _vp, _c_int,
+                                _vp, ctypes.c_size_t, _vp]),
     "p3d_peer_alloc": (_c_int, [ctypes.c_size_t, ctypes.POINTER(_vp), _vp]),
     "p3d_peer_free": (_c_int, [_vp]),
     "p3d_peer_open": (_c_int, [_vp, ctypes.POINTER(_vp)]),

@@ -1,0 +1,459 @@
+// Product of two e4m3 matrices with power-of-two scales for each block of 128 (see fp8.cu):
+//     out[m, n] = sum over k of a[m, k] 2^ea[m, k / 128] b[n, k] 2^eb[n, k / 128]  (+ bias[n])
+// Both operands lie along k.  The tensor cores take the scales themselves (tcgen05.mma, block-scaled 8-bit
+// kind): products of e4m3 and their powers of two are exact in fp32, so nothing but the fp32
+// accumulation and the last rounding is inexact, and no accumulator leaves TMEM before its tile is done.
+//
+// Work unit: a 128 x BN tile of the output, or a slice of its k (split) when there are fewer tiles than
+// SMs; CTAs walk units persistently.  Roles: warp 0 TMA producer (a ring of 128-column slices of both
+// operands, 128-byte rows, SWIZZLE_128B, with the scale bytes of four slices when a new four
+// begin), warp 1 MMA issuer (copies those bytes to TMEM, where one byte of a row's word scales one
+// slice, and issues the products into one of two accumulators), warps 2-5 epilogue (one row a
+// thread).  Few rows of `a` (tokens of a decode step) are taken as the N side (SWAP): the weight's rows
+// then fill the 128 lanes and the token count only sets N.
+// Slices of k go to fp32 partials that a second kernel adds in slice order.
+//
+// Every wait is bounded (2 s): on a timeout the kernel records an error bit (p3d_device_errors), drains its
+// copies and MMAs and frees TMEM.
+#include <algorithm>
+
+#include "common.cuh"
+#include "kernels.cuh"
+#include "sm100.cuh"
+#include "tma_host.cuh"
+
+namespace p3d {
+namespace {
+
+using namespace sm100;
+
+__device__ unsigned g_fp8_errors = 0;
+
+constexpr int kTileM = 128, kSlice = 128;
+constexpr int kThreads = 192;
+constexpr int kProducerWarp = 0, kMmaWarp = 1;
+constexpr uint64_t kWaitNs = 2000000000ull;
+constexpr int kMaxStages = 12;
+
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int c0, int c1) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(
+          dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1)
+      : "memory");
+}
+
+// D[tmem] (+)= A[smem desc] * B[smem desc]^T, e4m3, each row of A and of B times the power of two in its
+// byte of the scale words in TMEM; K = 32.
+__device__ __forceinline__ void mma_scaled(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb,
+                                           uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
+      : "memory");
+}
+
+// 32 rows of 16 bytes from shared memory to four columns of TMEM, repeated in every quarter of its lanes.
+__device__ __forceinline__ void copy_scales(uint32_t tmem, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+}
+
+// Unswizzled descriptor of 512 scale bytes: 8-row groups of 16-byte rows, 128 bytes apart.
+__device__ __forceinline__ uint64_t desc_scales(uint32_t smem) {
+  return (uint64_t)((smem >> 4) & 0x3FFFu) | (uint64_t)(128 >> 4) << 32 | (uint64_t)1 << 46;
+}
+
+// Instruction descriptor: e4m3 operands along k, power-of-two scales; the byte of the scale words
+// that a slice uses is or-ed in.
+__host__ __device__ constexpr uint32_t idesc_scaled(int m, int n) {
+  return (uint32_t)(n >> 3) << 17 | 1u << 23 | (uint32_t)(m >> 7) << 27;
+}
+__device__ __forceinline__ uint32_t scale_ids(int byte) { return (uint32_t)byte << 4 | (uint32_t)byte << 29; }
+
+struct GemmParams {
+  int rows, cols;          // of the tile space: rows of the 128-lane operand, of the N operand
+  int slices;              // ceil(k / 128)
+  int tiles_m, tiles_n, splits;
+  const uint8_t *scales_a, *scales_b;   // of the 128-lane operand, of the N operand
+  void *out;               // [rows, cols] (SWAP: [cols, rows]) of out_type, or the partials [splits][..] fp32
+  int64_t pitch;           // elements between out's rows
+  int64_t split_stride;    // elements between partials
+  const void *bias;        // over out's columns, of bias_type, or null
+  int out_type, bias_type, vector;   // vector: 16-byte stores are aligned
+  int stages;
+};
+
+// Which tile and slices a unit is: units of one tile follow each other, tiles go down groups of eight
+// tile rows so that the operands of CTAs at work together stay in L2.
+struct Unit {
+  int tm, tn, split, begin, end;
+};
+__device__ __forceinline__ Unit unit_of(const GemmParams &p, int u) {
+  Unit r;
+  r.split = u % p.splits;
+  const int t = u / p.splits, group = 8 * p.tiles_n, g = t / group, in = t - g * group;
+  const int height = min(8, p.tiles_m - 8 * g);
+  r.tm = 8 * g + in % height;
+  r.tn = in / height;
+  r.begin = (int)((int64_t)p.slices * r.split / p.splits);
+  r.end = (int)((int64_t)p.slices * (r.split + 1) / p.splits);
+  return r;
+}
+
+template <typename T>
+__device__ __forceinline__ void store_row(T *dst, const float (&v)[32], int valid, bool vector) {
+  if (vector && valid >= 32) {
+    constexpr int n = 16 / sizeof(T);
+#pragma unroll
+    for (int i = 0; i < 32 / n; ++i) {
+      T t[n];
+#pragma unroll
+      for (int j = 0; j < n; ++j) t[j] = from_f32<T>(v[i * n + j]);
+      uint4 w;
+      memcpy(&w, t, 16);
+      reinterpret_cast<uint4 *>(dst)[i] = w;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (j < valid) dst[j] = from_f32<T>(v[j]);
+  }
+}
+
+// BN: columns of a tile; SWAP: out is written transposed (its rows are this kernel's columns).
+template <int BN, bool SWAP>
+__global__ void __launch_bounds__(kThreads, 1)
+    fp8_gemm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb, const GemmParams p) {
+  constexpr int kChunksB = (BN + 127) / 128;            // 512-byte scale chunks of the N operand
+  constexpr uint32_t kBytesA = kTileM * kSlice, kBytesB = BN * kSlice, kBytesS = 512u * (1 + kChunksB);
+  constexpr uint32_t kStageBytes = kBytesA + (kBytesB + 1023u) / 1024u * 1024u + 2048u;
+  constexpr int kAccCols = BN < 32 ? 32 : BN;
+  constexpr int kScaleCols = 4 + 4 * kChunksB;           // per buffer; two buffers
+  constexpr int kUsed = 2 * kAccCols + 2 * kScaleCols;
+  constexpr int kTmemCols = kUsed <= 128 ? 128 : kUsed <= 256 ? 256 : 512;
+  static_assert(kUsed <= 512, "TMEM");
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  __shared__ __align__(8) uint64_t s_bars[2 * kMaxStages + 5];
+  __shared__ uint32_t tmem_holder;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t bars = smem_u32(s_bars);
+  const int S = p.stages;
+  auto full = [&](int s) { return bars + 8u * s; };
+  auto empty = [&](int s) { return bars + 8u * (kMaxStages + s); };
+  auto acc_full = [&](int a) { return bars + 8u * (2 * kMaxStages + a); };
+  auto acc_empty = [&](int a) { return bars + 8u * (2 * kMaxStages + 2 + a); };
+  const uint32_t drain = bars + 8u * (2 * kMaxStages + 4);
+  const int units = p.tiles_m * p.tiles_n * p.splits;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(full(s), 1);
+      mbar_init(empty(s), 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(acc_full(a), 1);
+      mbar_init(acc_empty(a), 4);
+    }
+    mbar_init(drain, 1);
+    fence_mbar_init();
+  }
+  if (warp == kMmaWarp) {
+    tmem_alloc(smem_u32(&tmem_holder), kTmemCols);
+    tmem_relinquish();
+  }
+  if (warp == kProducerWarp && lane == 0) {
+    prefetch_tmap(&ta);
+    prefetch_tmap(&tb);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_holder;
+
+  if (warp == kProducerWarp) {
+    // ------------------------------------------------------------------ TMA producer
+    if (lane == 0) {
+      const int groups = (p.slices + 3) / 4;
+      int it = 0;
+      bool ok = true;
+      for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
+        const Unit w = unit_of(p, u);
+        const uint8_t *sa = p.scales_a + (int64_t)w.tm * groups * 512;
+        const uint8_t *sb = p.scales_b + (int64_t)(w.tn * BN / 128) * groups * 512;
+        for (int kb = w.begin; kb < w.end; ++kb, ++it) {
+          const int s = it % S;
+          if (it >= S && !mbar_wait(empty(s), (it / S - 1) & 1, &g_fp8_errors, kWaitNs, kErrProducer)) {
+            ok = false;
+            break;
+          }
+          const uint32_t st = base + s * kStageBytes;
+          const bool scales = kb == w.begin || kb % 4 == 0;
+          // the last tile of the N operand may have one chunk of 128 rows fewer than BN
+          const int chunks_b = min(kChunksB, (p.cols - w.tn * BN + 127) / 128);
+          mbar_expect_tx(full(s), kBytesA + kBytesB + (scales ? 512u * (1 + chunks_b) : 0u));
+          tma_load_2d(st, &ta, full(s), kb * kSlice, w.tm * kTileM);
+          tma_load_2d(st + kBytesA, &tb, full(s), kb * kSlice, w.tn * BN);
+          if (scales) {
+            const uint32_t at = st + kStageBytes - 2048u;
+            bulk_load(at, sa + (int64_t)(kb / 4) * 512, 512u, full(s));
+            for (int c = 0; c < chunks_b; ++c)
+              bulk_load(at + 512u * (1 + c), sb + ((int64_t)c * groups + kb / 4) * 512, 512u, full(s));
+          }
+        }
+      }
+      // no copies in flight into shared memory this CTA gives up
+      for (int i = it > S ? it - S : 0; i < it; ++i)
+        mbar_wait(full(i % S), (i / S) & 1, &g_fp8_errors, kWaitNs, kErrTeardown);
+    }
+  } else if (warp == kMmaWarp) {
+    // ------------------------------------------------------------------ MMA issuer
+    if (lane == 0) {
+      constexpr uint32_t idesc = idesc_scaled(kTileM, BN);
+      const uint32_t scale_cols = tmem + 2 * kAccCols;
+      const uint64_t desc_a = desc_sw128(base, 1024), desc_b = desc_sw128(base + kBytesA, 1024);
+      const uint64_t desc_s = desc_scales(base + kStageBytes - 2048u);
+      int it = 0, n = 0, groups = 0;
+      bool ok = true;
+      for (int u = blockIdx.x; ok && u < units; u += gridDim.x, ++n) {
+        const Unit w = unit_of(p, u);
+        const int a = n & 1;
+        if (n >= 2 && !mbar_wait(acc_empty(a), (n / 2 - 1) & 1, &g_fp8_errors, kWaitNs, kErrMma)) break;
+        for (int kb = w.begin; kb < w.end; ++kb, ++it) {
+          const int s = it % S;
+          if (!mbar_wait(full(s), (it / S) & 1, &g_fp8_errors, kWaitNs, kErrMma)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint64_t off = (uint64_t)(s * kStageBytes >> 4);
+          if (kb == w.begin || kb % 4 == 0) {
+            // the other buffer: products of the four slices before may still read theirs
+            const uint32_t to = scale_cols + (groups & 1) * kScaleCols;
+#pragma unroll
+            for (int c = 0; c < 1 + kChunksB; ++c) copy_scales(to + 4 * c, desc_s + off + 32u * c);
+            ++groups;
+          }
+          const uint32_t sc = scale_cols + ((groups - 1) & 1) * kScaleCols;
+          const uint32_t id = idesc | scale_ids(kb % 4);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)   // 32 columns: 32 bytes along the 128-byte rows
+            mma_scaled(tmem + a * kAccCols, desc_a + off + 2 * k, desc_b + off + 2 * k, id, sc, sc + 4,
+                       kb > w.begin || k > 0 ? 1u : 0u);
+          mma_commit(empty(s));
+        }
+        if (!ok) break;
+        mma_commit(acc_full(a));
+      }
+      // drain: every commit of this CTA before its barriers and TMEM go away
+      mma_commit(drain);
+      mbar_wait(drain, 0, &g_fp8_errors, kWaitNs, kErrTeardown);
+      for (int i = it > S ? it - S : 0; i < it; ++i)
+        mbar_wait(empty(i % S), (i / S) & 1, &g_fp8_errors, kWaitNs, kErrTeardown);
+      for (int i = n > 2 ? n - 2 : 0; i < n; ++i)
+        mbar_wait(acc_full(i & 1), (i / 2) & 1, &g_fp8_errors, kWaitNs, kErrTeardown);
+    }
+  } else {
+    // ------------------------------------------------------------------ epilogue
+    const int quarter = warp & 3;   // TMEM lanes this warp may read
+    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
+    int n = 0;
+    for (int u = blockIdx.x; u < units; u += gridDim.x, ++n) {
+      const Unit w = unit_of(p, u);
+      const int a = n & 1;
+      const bool ready = mbar_wait(acc_full(a), (n / 2) & 1, &g_fp8_errors, kWaitNs, kErrSoftmax);
+      if (!__all_sync(0xffffffffu, ready)) break;
+      tc_fence_after();
+      const int row = w.tm * kTileM + quarter * 32 + lane;
+      constexpr int kWide = BN < 32 ? BN : 32;
+#pragma unroll 1
+      for (int c0 = 0; c0 < BN; c0 += 32) {
+        const int col = w.tn * BN + c0, valid = min(kWide, p.cols - col);
+        if (valid <= 0) break;
+        uint32_t raw[32];
+        tmem_ld32(lanes + a * kAccCols + c0, raw);
+        tmem_wait_ld();
+        float v[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(raw[j]);
+        if (row < p.rows) {
+          if constexpr (!SWAP) {
+            if (p.bias) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (j < valid) v[j] += load_any(p.bias, p.bias_type, col + j);
+            }
+            const int64_t at = (int64_t)row * p.pitch + col + (int64_t)w.split * p.split_stride;
+            switch (p.out_type) {
+              case P3D_F16: store_row(static_cast<__half *>(p.out) + at, v, valid, p.vector); break;
+              case P3D_BF16: store_row(static_cast<__nv_bfloat16 *>(p.out) + at, v, valid, p.vector); break;
+              default: store_row(static_cast<float *>(p.out) + at, v, valid, p.vector);
+            }
+          } else {
+            // lanes hold consecutive columns of out: each store is one run of its row
+            const float add = p.bias ? load_any(p.bias, p.bias_type, row) : 0.f;
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (j < valid)
+                store_any(p.out, p.out_type, (int64_t)(col + j) * p.pitch + row + (int64_t)w.split * p.split_stride,
+                          v[j] + add);
+          }
+        }
+        __syncwarp();   // the TMEM loads take the whole warp
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(acc_empty(a));
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+// out = the partials added in slice order, plus the bias.
+__global__ void __launch_bounds__(256) add_splits_kernel(const float *part, int splits, int64_t rows, int64_t cols,
+                                                         const void *bias, int bias_type, void *out, int out_type,
+                                                         int64_t pitch) {
+  const int64_t total = rows * cols, step = (int64_t)gridDim.x * blockDim.x;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += step) {
+    const int64_t r = i / cols, c = i - r * cols;
+    float v = part[i];
+    for (int s = 1; s < splits; ++s) v += part[s * total + i];
+    if (bias) v += load_any(bias, bias_type, c);
+    store_any(out, out_type, r * pitch + c, v);
+  }
+}
+
+struct Plan {
+  int bn;
+  bool swap;
+  int tiles_m, tiles_n, splits;
+  int64_t rows, cols;   // tile space
+};
+
+// Tokens up to 64 become the N side.  Splits: as many slices of k as fill the SMs, each of at least two
+// 128-column slices.
+Plan plan_of(int64_t rows, int64_t cols, int64_t k, int sms) {
+  Plan p;
+  p.swap = rows <= 64;
+  p.rows = p.swap ? cols : rows;
+  p.cols = p.swap ? rows : cols;
+  p.bn = !p.swap ? 128 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+  p.tiles_m = (int)((p.rows + kTileM - 1) / kTileM);
+  p.tiles_n = (int)((p.cols + p.bn - 1) / p.bn);
+  const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n, slices = (k + kSlice - 1) / kSlice;
+  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({sms / std::max<int64_t>(1, tiles), slices / 2, 64}));
+  return p;
+}
+
+template <int BN, bool SWAP>
+int launch_gemm(const CUtensorMap &ta, const CUtensorMap &tb, GemmParams g, int sms, cudaStream_t s) {
+  constexpr size_t stage = kTileM * kSlice + (BN * kSlice + 1023) / 1024 * 1024 + 2048;
+  g.stages = (int)std::min<size_t>(kMaxStages, (220 * 1024) / stage);
+  const size_t smem = g.stages * stage + 1024;
+  static size_t seen[kMaxDevices] = {};
+  if (int st = smem_optin(fp8_gemm_kernel<BN, SWAP>, smem, seen)) return st;
+  const int64_t units = (int64_t)g.tiles_m * g.tiles_n * g.splits;
+  fp8_gemm_kernel<BN, SWAP><<<(unsigned)std::min<int64_t>(units, sms), kThreads, smem, s>>>(ta, tb, g);
+  P3D_LAUNCH_CHECK();
+  return P3D_OK;
+}
+
+int check_extents(int64_t rows, int64_t cols, int64_t k, const char *what) {
+  P3D_CHECK_ARG(rows >= 1 && cols >= 1 && k >= 1, "%s: extents must be positive", what);
+  const int64_t most = (int64_t)1 << 30;
+  if (rows > most || cols > most || k > most || ((rows + 127) / 128) * ((cols + 127) / 128) > most)
+    return fail(P3D_ERR_UNSUPPORTED, "%s: extents too large", what);
+  return P3D_OK;
+}
+
+}  // namespace
+
+int take_fp8_errors(unsigned *flags) {
+  unsigned v = 0, zero = 0;
+  P3D_CUDA_TRY(cudaMemcpyFromSymbol(&v, g_fp8_errors, sizeof(v)));
+  P3D_CUDA_TRY(cudaMemcpyToSymbol(g_fp8_errors, &zero, sizeof(zero)));
+  *flags |= v;
+  return P3D_OK;
+}
+
+}  // namespace p3d
+
+using namespace p3d;
+
+extern "C" size_t p3d_fp8_matmul_workspace(int64_t rows, int64_t cols, int64_t k) {
+  DeviceInfo info;
+  if (check_extents(rows, cols, k, "p3d_fp8_matmul_workspace") || device_info(&info)) return 0;
+  const Plan p = plan_of(rows, cols, k, info.sm_count);
+  return p.splits > 1 ? (size_t)p.splits * rows * cols * sizeof(float) : 0;
+}
+
+extern "C" int p3d_fp8_matmul(const void *a, int64_t a_pitch, const void *a_scales, const void *b, int64_t b_pitch,
+                              const void *b_scales, int64_t rows, int64_t cols, int64_t k, const void *bias,
+                              int bias_dtype, void *out, int out_dtype, void *workspace, size_t workspace_bytes,
+                              void *stream) {
+  if (int st = check_extents(rows, cols, k, "p3d_fp8_matmul")) return st;
+  P3D_CHECK_ARG(a && a_scales && b && b_scales && out, "p3d_fp8_matmul: null pointer");
+  P3D_CHECK_ARG(dtype_ok(out_dtype) && (!bias || dtype_ok(bias_dtype)), "p3d_fp8_matmul: unknown dtype");
+  P3D_CHECK_ARG(a_pitch >= k && b_pitch >= k && a_pitch % 16 == 0 && b_pitch % 16 == 0,
+                "p3d_fp8_matmul: pitches must be multiples of 16 and hold k columns");
+  P3D_CHECK_ARG((((uintptr_t)a | (uintptr_t)b | (uintptr_t)a_scales | (uintptr_t)b_scales | (uintptr_t)workspace) & 15) == 0,
+                "p3d_fp8_matmul: operands, scales and workspace must be 16-byte aligned");
+  DeviceInfo info;
+  if (int st = device_info(&info)) return st;
+  if (info.major != 10) return fail(P3D_ERR_DEVICE, "p3d_fp8_matmul needs an sm_100 device");
+  const Plan p = plan_of(rows, cols, k, info.sm_count);
+  const size_t need = p.splits > 1 ? (size_t)p.splits * rows * cols * sizeof(float) : 0;
+  if (need && (!workspace || workspace_bytes < need))
+    return fail(P3D_ERR_WORKSPACE, "p3d_fp8_matmul: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+  const void *wide = p.swap ? b : a, *narrow = p.swap ? a : b;
+  const int64_t wide_pitch = p.swap ? b_pitch : a_pitch, narrow_pitch = p.swap ? a_pitch : b_pitch;
+  CUtensorMap ta, tb;
+  {
+    const uint64_t dims[2] = {(uint64_t)k, (uint64_t)p.rows}, strides[1] = {(uint64_t)wide_pitch};
+    const uint32_t box[2] = {kSlice, kTileM};
+    if (int st = encode_tiled(&ta, CU_TENSOR_MAP_DATA_TYPE_UINT8, wide, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B))
+      return st;
+  }
+  {
+    const uint64_t dims[2] = {(uint64_t)k, (uint64_t)p.cols}, strides[1] = {(uint64_t)narrow_pitch};
+    const uint32_t box[2] = {kSlice, (uint32_t)p.bn};
+    if (int st = encode_tiled(&tb, CU_TENSOR_MAP_DATA_TYPE_UINT8, narrow, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B))
+      return st;
+  }
+  GemmParams g = {};
+  g.rows = (int)p.rows;
+  g.cols = (int)p.cols;
+  g.slices = (int)((k + kSlice - 1) / kSlice);
+  g.tiles_m = p.tiles_m;
+  g.tiles_n = p.tiles_n;
+  g.splits = p.splits;
+  g.scales_a = static_cast<const uint8_t *>(p.swap ? b_scales : a_scales);
+  g.scales_b = static_cast<const uint8_t *>(p.swap ? a_scales : b_scales);
+  g.out = p.splits > 1 ? workspace : out;
+  g.out_type = p.splits > 1 ? (int)P3D_F32 : out_dtype;
+  g.pitch = cols;
+  g.split_stride = p.splits > 1 ? rows * cols : 0;
+  g.bias = p.splits > 1 ? nullptr : bias;
+  g.bias_type = bias_dtype;
+  g.vector = (cols * dtype_size(g.out_type)) % 16 == 0 && ((uintptr_t)g.out & 15) == 0;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  int st;
+  if (!p.swap) st = launch_gemm<128, false>(ta, tb, g, info.sm_count, s);
+  else if (p.bn == 16) st = launch_gemm<16, true>(ta, tb, g, info.sm_count, s);
+  else if (p.bn == 32) st = launch_gemm<32, true>(ta, tb, g, info.sm_count, s);
+  else st = launch_gemm<64, true>(ta, tb, g, info.sm_count, s);
+  if (st != P3D_OK || p.splits == 1) return st;
+  const unsigned grid = (unsigned)std::min<int64_t>((rows * cols + 255) / 256, (int64_t)info.sm_count * 8);
+  add_splits_kernel<<<grid, 256, 0, s>>>(static_cast<const float *>(workspace), p.splits, rows, cols, bias, bias_dtype,
+                                         out, out_dtype, cols);
+  P3D_LAUNCH_CHECK();
+  return P3D_OK;
+}

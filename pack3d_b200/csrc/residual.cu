@@ -661,6 +661,19 @@ size_t partial_floats(const p3d_residual &p, const Split &c) {
 }
 
 }  // namespace
+
+int launch_column_join(const float *partials, void *out, int dtype, int64_t count, int dim, cudaStream_t s) {
+  const dim3 grid((unsigned)((dim + 31) / 32)), block(32, 8);
+  const Joins none = {};
+  if (dtype == P3D_F32) join_kernel<float><<<grid, block, 0, s>>>(partials, static_cast<float *>(out), none, count, dim);
+  else if (dtype == P3D_F16)
+    join_kernel<__half><<<grid, block, 0, s>>>(partials, static_cast<__half *>(out), none, count, dim);
+  else
+    join_kernel<__nv_bfloat16><<<grid, block, 0, s>>>(partials, static_cast<__nv_bfloat16 *>(out), none, count, dim);
+  P3D_LAUNCH_CHECK();
+  return P3D_OK;
+}
+
 }  // namespace p3d
 
 using namespace p3d;

@@ -1,0 +1,205 @@
+"""Linear layers in 8-bit floating point with one power-of-two scale for each block of 128.
+
+* :class:`Fp8Matrix` -- e4m3 values and their scales as the tensor cores read them.
+* :func:`quantize` / :func:`quantize_weight` -- blocks of 1 x 128 (activations) and 128 x 128 (weights).
+* :func:`fp8_matmul` -- ``a b^T`` of two such matrices, fp32 accumulation, one rounding at the end.
+* :func:`fp8_linear` -- ``x W^T + bias`` for training (both gradients in the same products) or from a kept weight.
+
+No counterpart in the reference, whose projections are 16- or 32-bit (``attention.py:37-51``).  A block's scale is the
+smallest power of two that brings its largest finite magnitude to at most 448, so scaling is exact and e4m3's rounding
+to nearest even is the only one; products are exact in fp32.  NaN and infinities become NaN and set no scale.
+"""
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _native
+from ._validation import check_cuda
+from .residual import _Guard
+
+BLOCK = 128
+
+
+class Fp8Matrix:
+    """``values`` [rows, pitch] (``torch.float8_e4m3fn``, pitch a multiple of 16, columns from ``cols`` on unused) and
+    ``scales`` (bytes e + 127 of 2^e, one for each row and block of 128 columns, in the order of
+    ``p3d_fp8_quantize``)."""
+
+    __slots__ = ("values", "scales", "rows", "cols")
+
+    def __init__(self, values, scales, rows, cols):
+        self.values, self.scales, self.rows, self.cols = values, scales, int(rows), int(cols)
+
+    @property
+    def shape(self):
+        return torch.Size((self.rows, self.cols))
+
+    @property
+    def device(self):
+        return self.values.device
+
+    def exponents(self):
+        """int32 [rows, ceil(cols / 128)]: the e of each block's scale 2^e."""
+        blocks = -(-self.cols // BLOCK)
+        tiles, groups = -(-self.rows // BLOCK), -(-blocks // 4)
+        t = self.scales.view(tiles, groups, 32, 4, 4).permute(0, 3, 2, 1, 4).reshape(tiles * BLOCK, groups * 4)
+        return t[:self.rows, :blocks].to(torch.int32) - 127
+
+    def dequantize(self, dtype=torch.float32):
+        """The values that the bytes stand for, [rows, cols], rounded to ``dtype`` (infinite where it cannot hold
+        them: a block's largest value may round up past fp32's range)."""
+        scale = ((self.exponents() + 127) << 23).view(torch.float32).to(torch.float64)   # 2^e from its bits
+        scale = scale.repeat_interleave(BLOCK, 1)[:, :self.cols]
+        return (self.values[:, :self.cols].to(torch.float64) * scale).to(dtype)
+
+    @staticmethod
+    def _empty(rows, cols, device):
+        pitch = -(-cols // 16) * 16
+        return Fp8Matrix(torch.empty((rows, pitch), dtype=torch.float8_e4m3fn, device=device),
+                         torch.empty(_native.lib().p3d_fp8_scale_bytes(rows, cols), dtype=torch.uint8, device=device),
+                         rows, cols)
+
+
+def _check_matrix(x, what):
+    check_cuda(x)
+    if x.ndim != 2 or x.shape[0] < 1 or x.shape[1] < 1:
+        raise ValueError(f"{what} needs a matrix with at least one row and one column, got {list(x.shape)}")
+
+
+def _quantize(x, square=False, rows=True, transposed=False, sums=None):
+    """(q or None, qt or None) of a contiguous matrix; `sums`: a vector for the sums over its rows."""
+    m, n = x.shape
+    q = Fp8Matrix._empty(m, n, x.device) if rows else None
+    qt = Fp8Matrix._empty(n, m, x.device) if transposed else None
+    lib = _native.lib()
+    with _Guard(x.device):
+        ws = None
+        if sums is not None:
+            ws = torch.empty(max(16, lib.p3d_fp8_quantize_workspace(m, n)), dtype=torch.uint8, device=x.device)
+        _native.check(lib.p3d_fp8_quantize(
+            x.data_ptr(), _native.DTYPE_CODE[x.dtype], m, n, 1 if square else 0,
+            q.values.data_ptr() if q else None, q.values.shape[1] if q else 0, q.scales.data_ptr() if q else None,
+            qt.values.data_ptr() if qt else None, qt.values.shape[1] if qt else 0, qt.scales.data_ptr() if qt else None,
+            None if sums is None else sums.data_ptr(), 0 if sums is None else _native.DTYPE_CODE[sums.dtype],
+            None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(),
+            _native.stream_of(x.device)), "p3d_fp8_quantize")
+    return q, qt
+
+
+def quantize(x):
+    """:class:`Fp8Matrix` of a matrix with one scale for each row and block of 128 columns."""
+    _check_matrix(x, "quantize")
+    return _quantize(x.detach().contiguous())[0]
+
+
+def quantize_weight(weight):
+    """:class:`Fp8Matrix` of a weight [out, in] with one scale for each 128 x 128 block (repeated for its rows), as
+    :func:`fp8_linear` quantises it: keep it to serve from 8-bit weights."""
+    _check_matrix(weight, "quantize_weight")
+    return _quantize(weight.detach().contiguous(), square=True)[0]
+
+
+def _matmul(a, b, bias, dtype):
+    out = torch.empty((a.rows, b.rows), dtype=dtype, device=a.device)
+    lib = _native.lib()
+    with _Guard(a.device):
+        need = lib.p3d_fp8_matmul_workspace(a.rows, b.rows, a.cols)
+        ws = torch.empty(need, dtype=torch.uint8, device=a.device) if need else None
+        _native.check(lib.p3d_fp8_matmul(
+            a.values.data_ptr(), a.values.shape[1], a.scales.data_ptr(), b.values.data_ptr(), b.values.shape[1],
+            b.scales.data_ptr(), a.rows, b.rows, a.cols, None if bias is None else bias.data_ptr(),
+            0 if bias is None else _native.DTYPE_CODE[bias.dtype], out.data_ptr(), _native.DTYPE_CODE[dtype],
+            None if ws is None else ws.data_ptr(), need, _native.stream_of(a.device)), "p3d_fp8_matmul")
+    return out
+
+
+def _check_bias(bias, n, device):
+    if bias is None:
+        return None
+    if bias.shape != (n,) or bias.device != device or bias.dtype not in _native.DTYPE_CODE:
+        raise ValueError(f"bias must be {n} fp32, fp16 or bf16 values on the input's device")
+    return bias.contiguous()
+
+
+def fp8_matmul(a, b, *, bias=None, dtype=torch.bfloat16):
+    """``a b^T`` (``+ bias``) as [a.rows, b.rows] of ``dtype`` (fp32, fp16, bf16) for two :class:`Fp8Matrix` of the same
+    number of columns.  Products and sums in fp32; the order of the sum depends on the extents alone."""
+    if not (isinstance(a, Fp8Matrix) and isinstance(b, Fp8Matrix)):
+        raise ValueError("fp8_matmul takes two Fp8Matrix")
+    if a.cols != b.cols or a.device != b.device:
+        raise ValueError(f"operands must have the same columns and device, got {list(a.shape)} and {list(b.shape)}")
+    if dtype not in _native.DTYPE_CODE:
+        raise ValueError("dtype must be fp32, fp16 or bf16")
+    return _matmul(a, b, _check_bias(bias, b.rows, a.device), dtype)
+
+
+class _Fp8Linear(torch.autograd.Function):
+    """Forward keeps x and the weight in 8 bits only: x with blocks along its rows for dW, the weight transposed for
+    dx (its 128 x 128 blocks serve both directions)."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias):
+        need_x, need_w = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
+        xq, xt = _quantize(x, transposed=need_w)
+        wq, wt = _quantize(weight, square=True, transposed=need_x)
+        ctx.meta = (x.shape, weight.shape, x.dtype, weight.dtype, None if bias is None else bias.dtype)
+        ctx.save_for_backward(*(t for q in (xt, wt) for t in ((None, None) if q is None else (q.values, q.scales))))
+        return _matmul(xq, wq, bias, x.dtype)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        (m, k), (n, _), x_type, w_type, b_type = ctx.meta
+        need_x, need_w, need_b = ctx.needs_input_grad
+        xtv, xts, wtv, wts = ctx.saved_tensors
+        dy = dy.contiguous()
+        db = torch.empty(n, dtype=b_type, device=dy.device) if need_b else None
+        dyq, dyt = _quantize(dy, rows=need_x, transposed=need_w, sums=db)
+        dx = _matmul(dyq, Fp8Matrix(wtv, wts, k, n), None, x_type) if need_x else None
+        dw = _matmul(dyt, Fp8Matrix(xtv, xts, k, m), None, w_type) if need_w else None
+        return dx, dw, db
+
+
+def fp8_linear(x, weight, bias=None):
+    """``x weight^T + bias`` over the last dimension of ``x`` with both operands in 8-bit blocks.
+
+    ``x`` [..., in] fp32, fp16 or bf16.  ``weight`` [out, in] is a tensor, quantised in the call (training: its gradient
+    and x's are products of 8-bit blocks too), or an :class:`Fp8Matrix` from :func:`quantize_weight` (serving; no
+    gradients).  Blocks: x and dy 1 x 128 along the dimension that is summed over (for the weight's gradient that
+    is the tokens), the weight 128 x 128.  The result has x's dtype, gradients their inputs'; the bias's gradient is
+    summed in fp32.
+    """
+    check_cuda(x)
+    if x.ndim < 1:
+        raise ValueError("fp8_linear needs at least one dimension")
+    kept = isinstance(weight, Fp8Matrix)
+    shape = weight.shape
+    if len(shape) != 2 or x.shape[-1] != shape[1] or shape[0] < 1 or shape[1] < 1:
+        raise ValueError(f"weight must be [out, {x.shape[-1]}], got {list(shape)}")
+    if weight.device != x.device:
+        raise ValueError("x and weight must be on the same device")
+    bias = _check_bias(bias, shape[0], x.device)
+    rows = x.reshape(-1, shape[1]).contiguous()
+    grad = torch.is_grad_enabled()
+    if kept:
+        if grad and (x.requires_grad or bias is not None and bias.requires_grad):
+            raise ValueError("an 8-bit weight has no gradients: pass the weight itself, or call under torch.no_grad()")
+    elif weight.dtype not in _native.DTYPE_CODE:
+        raise ValueError("weight must be fp32, fp16 or bf16")
+    else:
+        weight = weight.contiguous()
+    if rows.shape[0] == 0:
+        y = x.new_empty(0, shape[0])
+        if not kept and grad:   # zero gradients for the weight and bias, as of an empty sum
+            y = rows @ weight.t().to(x.dtype) + (0 if bias is None else bias.to(x.dtype))
+    elif kept:
+        y = _matmul(_quantize(rows.detach())[0], weight, bias, x.dtype)
+    elif grad and (x.requires_grad or weight.requires_grad or bias is not None and bias.requires_grad):
+        y = _Fp8Linear.apply(rows, weight, bias)
+    else:
+        y = _matmul(_quantize(rows)[0], _quantize(weight, square=True)[0], bias, x.dtype)
+    return y.view(*x.shape[:-1], shape[0])
+
+
+__all__ = ["BLOCK", "Fp8Matrix", "fp8_linear", "fp8_matmul", "quantize", "quantize_weight"]
