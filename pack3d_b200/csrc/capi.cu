@@ -338,6 +338,7 @@ int p3d_device_errors(unsigned *flags) {
   if (int st = take_proj_errors(flags)) return st;
   if (int st = take_peer_errors(flags)) return st;
   if (int st = take_fp8_errors(flags)) return st;
+  if (int st = take_row_errors(flags)) return st;
   return take_bwd_errors(flags);
 }
 

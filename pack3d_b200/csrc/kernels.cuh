@@ -86,6 +86,7 @@ int launch_proj_split(const ProjArgs &a, cudaStream_t stream);
 int take_proj_errors(unsigned *flags);
 int take_peer_errors(unsigned *flags);  // peer.cu
 int take_fp8_errors(unsigned *flags);   // fp8_gemm.cu
+int take_row_errors(unsigned *flags);   // residual.cu
 // out[c] (of dtype) = sum over i < count of partials[i, c], in a fixed order (residual.cu)
 int launch_column_join(const float *partials, void *out, int dtype, int64_t count, int dim, cudaStream_t s);
 

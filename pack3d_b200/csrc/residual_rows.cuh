@@ -1,0 +1,1058 @@
+// Row kernels of the norms around a block (norm, gate, dropout, residual scale, residual, next norm) and
+// of their backward; instantiated for each type in residual_{f32,f16,bf16}.cu.
+//
+// One pass over the data in each direction, bound by HBM: forward 4 (x, h, out, y) and backward 6 (x, h,
+// dout, dy, dx, dh) values an element, plus the gate's.  A row is held by 32 to 512 threads, eight
+// columns each (up to eight CTAs of a cluster for the widest rows), so the row statistics cost shuffles
+// and no second read.  Row groups of a CTA work independently: each has a ring of row batches in shared
+// memory that bulk copies fill ahead of it, so the bytes in flight do not depend on how many
+// warps fit beside the column sums' registers.
+//
+// The backward makes out = x + s d again from x and h instead of reading the stored out: the same
+// bytes, and the normalised row keeps its 32 bits (the stored one is rounded to 16).  Every
+// thread keeps the column sums of its eight columns over all rows of its CTA in registers; they
+// are joined over the CTA's row groups in shared memory, written once per CTA and summed over the
+// CTAs by a second small kernel, all in a fixed order.
+//
+// What a call does not have (a norm, a bias, a gate) is a neutral value in the same formula.  Only what
+// costs registers or many instructions is a variant of its own: whether there is a block at all,
+// a gate, dropout, and centring (layer norm or a bias).
+#pragma once
+
+#include <algorithm>
+
+#include "common.cuh"
+#include "kernels.cuh"
+#include "philox.cuh"
+#include "sm100.cuh"
+
+namespace p3d {
+namespace rows {
+
+using sm100::add2;
+using sm100::fma2;
+using sm100::mul2;
+
+constexpr int kUnit = 8;             // columns of a unit; a thread owns one or two (NU)
+constexpr int kMaxRowThreads = 512;  // threads a row of one CTA
+constexpr int kMaxCluster = 8;
+constexpr int kMaxStages = 4;
+constexpr int kMaxGroups = 8;
+constexpr uint64_t kWaitNs = 2000000000ull;
+
+static __device__ unsigned g_row_errors = 0;
+
+enum : int { kX = 0, kH = 1, kGate = 2, kDout = 3, kDy = 4, kArrays = 5 };
+enum : int { kPostW = 0, kScale = 1, kNextW = 2, kPostB = 3, kNextB = 4, kParams = 5 };
+// Vectors that a variant keeps in shared memory, and the place of each.
+__host__ __device__ constexpr int param_count(bool block, bool center) {
+  return block ? (center ? 5 : 3) : (center ? 2 : 1);
+}
+__host__ __device__ constexpr int param_slot(bool block, int k) { return block ? k : k == kNextW ? 0 : 1; }
+enum : int { kGateAny = -1 };   // a variant that reads the gate's mode from its arguments
+
+struct Args {
+  p3d_residual p;
+  const void *in[kArrays];   // streamed rows; null: not read
+  const void *params[kParams];   // null: the neutral value
+  void *out, *y;
+  float *stats;              // [rows][4]; the backward streams them too
+  void *dx, *dh, *dgate;
+  float *partials;  // [kSums - 1][CTA slots][dim], then the sample gate's [samples][slices][dim]
+  int row_threads, groups, members;
+  int batch_rows, stages;
+  uint32_t slot_bytes;       // of one array's batch in the ring
+  uint32_t stage_bytes;      // of all arrays and the statistics
+  int slots[kArrays];        // ring slot of each array
+  int slot_count;
+  int segments, slices, segment_rows;   // the rows are `segments` runs, each cut into slices
+};
+
+__device__ __forceinline__ float2 splat(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float2 sub2(float2 a, float2 b) { return fma2(b, splat(-1.f), a); }
+
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// ------------------------------------------------------------------------ a thread's columns of a row
+// Aligned: units of eight consecutive columns that move in 16-byte pieces, a thread's second unit
+// row_threads units after its first.  Threads past the row's end read its last unit and neither
+// add to a sum nor store.  Otherwise (odd dim, or a pointer off 16 bytes) column j of the thread
+// is j * row_threads columns after its first, so that the lanes of a warp stay on consecutive
+// elements; columns past the end read as zero.
+struct Place {
+  int group, t, warps, warp, lane;
+  int rank, first;         // CTA of the cluster, its first column
+  int threads, dim, end;   // threads of the row here; columns in all; columns from `first` on
+  bool live[2];            // aligned: whether the unit is inside the row
+  int at[2];               // aligned: the unit's first column from `first` on, inside the row
+
+  __device__ __forceinline__ void barrier() const {   // of the row group
+    if (warps > 1) asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(warps * 32) : "memory");
+    else __syncwarp();
+  }
+  // Column j of the thread (from `first` on).
+  template <bool ALIGNED>
+  __device__ __forceinline__ int col(int j) const {
+    return ALIGNED ? (t + j / kUnit * threads) * kUnit + j % kUnit : t + j * threads;
+  }
+  template <bool ALIGNED>
+  __device__ __forceinline__ bool has(int j) const { return col<ALIGNED>(j) < end; }
+};
+
+template <bool ALIGNED>
+__device__ __forceinline__ Place place_of(const Args &a) {
+  Place q;
+  q.threads = a.row_threads;
+  q.group = threadIdx.x / a.row_threads;
+  q.t = threadIdx.x - q.group * a.row_threads;
+  q.warps = a.row_threads / 32;
+  q.warp = q.t / 32;
+  q.lane = q.t % 32;
+  q.rank = 0;
+  if (a.members > 1) asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(q.rank));
+  q.dim = a.p.dim;
+  return q;
+}
+template <bool ALIGNED, int NU>
+__device__ __forceinline__ void set_columns(Place &q) {
+  q.first = q.rank * q.threads * kUnit * NU;
+  q.end = q.dim - q.first;
+#pragma unroll
+  for (int n = 0; n < NU; ++n) {
+    const int c = (q.t + n * q.threads) * kUnit;
+    q.live[n] = c < q.end;
+    q.at[n] = max(0, min(c, q.end - kUnit));
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ float2 pair_of(const T *v) {
+  if constexpr (sizeof(T) == 2) return unpack2<T>(*reinterpret_cast<const uint32_t *>(v));
+  else return make_float2(v[0], v[1]);
+}
+
+// `row`: the row's column `first`.
+template <typename T, bool ALIGNED, int NU>
+__device__ __forceinline__ void load_cols(float2 (&f)[4 * NU], const T *row, const Place &q) {
+  if constexpr (ALIGNED) {
+#pragma unroll
+    for (int n = 0; n < NU; ++n) {
+      alignas(16) T v[kUnit];
+      constexpr int pieces = sizeof(v) / 16;
+      uint4 raw[pieces];
+#pragma unroll
+      for (int i = 0; i < pieces; ++i) raw[i] = reinterpret_cast<const uint4 *>(row + q.at[n])[i];
+      memcpy(v, raw, sizeof(v));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f[4 * n + i] = pair_of<T>(v + 2 * i);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4 * NU; ++i) {
+      const int c = q.t + 2 * i * q.threads;
+      f[i].x = c < q.end ? to_f32<T>(row[c]) : 0.f;
+      f[i].y = c + q.threads < q.end ? to_f32<T>(row[c + q.threads]) : 0.f;
+    }
+  }
+}
+
+template <typename T, bool ALIGNED, int NU>
+__device__ __forceinline__ void store_cols(T *row, const float2 (&f)[4 * NU], const Place &q) {
+  if constexpr (ALIGNED) {
+#pragma unroll
+    for (int n = 0; n < NU; ++n) {
+      if (!q.live[n]) continue;
+      const float2 *v = f + 4 * n;
+      if constexpr (sizeof(T) == 4) {
+        reinterpret_cast<float4 *>(row + q.at[n])[0] = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+        reinterpret_cast<float4 *>(row + q.at[n])[1] = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);
+      } else {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if constexpr (std::is_same<T, __nv_bfloat16>::value) w[i] = sm100::pack_bf16(v[i].x, v[i].y);
+          else w[i] = sm100::pack_f16(v[i].x, v[i].y);
+        }
+        *reinterpret_cast<uint4 *>(row + q.at[n]) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4 * NU; ++i) {
+      const int c = q.t + 2 * i * q.threads;
+      if (c < q.end) row[c] = from_f32<T>(f[i].x);
+      if (c + q.threads < q.end) row[c + q.threads] = from_f32<T>(f[i].y);
+    }
+  }
+}
+
+// What the thread adds to a sum over the row, from its columns' v: nothing for units past the end
+// (unaligned columns there hold zeros already).
+template <bool ALIGNED, int NU>
+__device__ __forceinline__ float total(const Place &q, const float2 (&v)[NU]) {
+  float s = 0.f;
+#pragma unroll
+  for (int n = 0; n < NU; ++n) s += ALIGNED && !q.live[n] ? 0.f : v[n].x + v[n].y;
+  return s;
+}
+
+struct Exchange {
+  float slots[2][16][4];               // [2][warps of the CTA][values]
+  float peers[2][kMaxCluster][4];      // [2][CTA of the cluster][values]
+};
+
+// Sums of N values over the warp, in every lane.  Two or three values share their way down: lanes 16 to 31 take
+// over the second value's half in the first step, and lanes 8 to 15 the third's in the next, so
+// that later steps move one value each; a lane of each kind then hands its total out.
+__device__ __forceinline__ void warp_sums(int lane, float (&v)[1]) { v[0] = warp_sum(v[0]); }
+__device__ __forceinline__ void warp_sums(int lane, float (&v)[2]) {
+  const bool high = lane & 16;
+  const float keep = high ? v[1] : v[0], give = high ? v[0] : v[1];
+  float s = keep + __shfl_xor_sync(0xffffffffu, give, 16);
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  v[0] = __shfl_sync(0xffffffffu, s, 0);
+  v[1] = __shfl_sync(0xffffffffu, s, 16);
+}
+__device__ __forceinline__ void warp_sums(int lane, float (&v)[3]) {
+  float two[2] = {v[0], v[1]};
+  warp_sums(lane, two);
+  v[0] = two[0];
+  v[1] = two[1];
+  v[2] = warp_sum(v[2]);
+}
+
+// N values of every thread summed over the row, the same total in every thread, always added in the
+// same order.  The shared slots alternate between calls (`at`): a thread two calls ahead has passed the
+// barrier of the call between, so nobody still reads the slots it writes.
+struct RowSum {
+  Exchange *x;
+  int members;
+  int at = 0;
+
+  template <int N>
+  __device__ __forceinline__ void operator()(const Place &q, float (&v)[N]) {
+    warp_sums(q.lane, v);
+    if (q.warps > 1) {
+      if (q.lane == 0) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) x->slots[at][q.group * q.warps + q.warp][i] = v[i];
+      }
+      q.barrier();
+      const float4 w = q.lane < q.warps ? *reinterpret_cast<const float4 *>(x->slots[at][q.group * q.warps + q.lane])
+                                        : make_float4(0.f, 0.f, 0.f, 0.f);
+      v[0] = w.x;
+      if constexpr (N > 1) v[1] = w.y;
+      if constexpr (N > 2) v[2] = w.z;
+      warp_sums(q.lane, v);
+      if (members > 1) over_cluster(q, v);
+      at ^= 1;
+    }
+  }
+
+  // Mean and sum of squares about it: each warp takes its own mean and the squares about that, and the
+  // warps' pairs are joined (n (mean_w - mean)^2 each), so one barrier serves both and nothing cancels
+  // where the mean is large.
+  template <bool ALIGNED, int NU>
+  __device__ __forceinline__ float2 moments(const Place &q, const float2 (&z)[4 * NU], float inv_dim) {
+    float2 s[NU], d2[NU];
+    float count = 0.f;   // columns of the warp
+    if constexpr (ALIGNED) {
+#pragma unroll
+      for (int n = 0; n < NU; ++n)
+        count += (float)(kUnit * __popc(__ballot_sync(0xffffffffu, q.live[n])));
+    } else {
+      const int base = q.warp * 32;
+#pragma unroll
+      for (int j = 0; j < kUnit * NU; ++j) count += (float)max(0, min(32, q.end - base - j * q.threads));
+    }
+#pragma unroll
+    for (int n = 0; n < NU; ++n) s[n] = add2(add2(z[4 * n], z[4 * n + 1]), add2(z[4 * n + 2], z[4 * n + 3]));
+    float mean = warp_sum(total<ALIGNED, NU>(q, s));
+    mean = q.warps == 1 ? mean * inv_dim : count > 0.f ? mean / count : 0.f;
+#pragma unroll
+    for (int n = 0; n < NU; ++n) {
+      d2[n] = splat(0.f);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float2 d = sub2(z[4 * n + i], splat(mean));
+        if constexpr (!ALIGNED) {
+          if (!q.has<ALIGNED>(8 * n + 2 * i)) d.x = 0.f;
+          if (!q.has<ALIGNED>(8 * n + 2 * i + 1)) d.y = 0.f;
+        }
+        d2[n] = fma2(d, d, d2[n]);
+      }
+    }
+    float m2 = warp_sum(total<ALIGNED, NU>(q, d2));
+    if (q.warps == 1) return make_float2(mean, m2);
+    if (q.lane == 0)
+      *reinterpret_cast<float4 *>(x->slots[at][q.group * q.warps + q.warp]) =
+          make_float4(count, count * mean, m2, mean);
+    q.barrier();
+    const float4 w = q.lane < q.warps ? *reinterpret_cast<const float4 *>(x->slots[at][q.group * q.warps + q.lane])
+                                      : make_float4(0.f, 0.f, 0.f, 0.f);
+    float two[2] = {w.x, w.y};
+    warp_sums(q.lane, two);
+    mean = two[0] > 0.f ? two[1] / two[0] : 0.f;   // a CTA of the cluster may have no columns
+    const float off = w.w - mean;
+    m2 = warp_sum(fmaf(w.x * off, off, w.z));
+    if (members > 1) {
+      float v[2] = {two[0], two[0] * mean};
+      over_cluster(q, v);
+      const float all = v[1] / v[0], d = mean - all;
+      at ^= 1;
+      float u[1] = {fmaf(two[0] * d, d, m2)};
+      over_cluster(q, u);
+      mean = all;
+      m2 = u[0];
+    }
+    at ^= 1;
+    return make_float2(mean, m2);
+  }
+
+  template <int N>
+  __device__ __forceinline__ void over_cluster(const Place &q, float (&v)[N]) {
+    if (q.warp == 0 && q.lane < members) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const uint32_t mine = sm100::smem_u32(&x->peers[at][q.rank][i]);
+        uint32_t theirs;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(theirs) : "r"(mine), "r"(q.lane));
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(theirs), "f"(v[i]) : "memory");
+      }
+    }
+    __syncwarp();
+    cluster_sync();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      v[i] = 0.f;
+      for (int c = 0; c < members; ++c) v[i] += x->peers[at][c][i];
+    }
+  }
+};
+
+// ------------------------------------------------------------------------ the ring of row batches
+// Batches of a CTA's slice, group by group: batch b of a segment is rows [b R, (b + 1) R) of the slice.
+struct Batches {
+  int seg, b, seg_step, per_slice, row0, row1;
+  __device__ __forceinline__ void settle(const Args &a, int group) {
+    while (seg < a.segments && b >= per_slice) {
+      seg += seg_step;
+      b = group;
+    }
+  }
+  __device__ __forceinline__ void next(const Args &a, int group) {
+    b += a.groups;
+    settle(a, group);
+  }
+  __device__ __forceinline__ int row(const Args &a) const { return seg * a.segment_rows + row0 + b * a.batch_rows; }
+  __device__ __forceinline__ int count(const Args &a) const { return min(a.batch_rows, row1 - row0 - b * a.batch_rows); }
+};
+
+__device__ __forceinline__ Batches batches_of(const Args &a, int group, int cta, int ctas) {
+  Batches k;
+  const int slice = cta % a.slices;
+  k.row0 = (int)((int64_t)a.segment_rows * slice / a.slices);
+  k.row1 = (int)((int64_t)a.segment_rows * (slice + 1) / a.slices);
+  k.per_slice = (k.row1 - k.row0 + a.batch_rows - 1) / a.batch_rows;
+  k.seg = cta / a.slices;
+  k.seg_step = ctas / a.slices;
+  k.b = group;
+  if (k.per_slice <= group) k.seg = a.segments;   // no batch for this group in any segment
+  return k;
+}
+
+// The bytes of one array's batch of `n` rows from `row` on in this CTA's columns.  Unaligned rows are copied with
+// the up to 15 bytes before and after that complete 16-byte pieces; a batch whose pieces would pass the
+// tensor's ends is not copied but read in place.
+template <typename T, bool ALIGNED, int NU>
+struct Span {
+  const char *from;
+  uint32_t bytes, shift;
+  bool copied;
+  __device__ __forceinline__ Span(const Args &a, const Place &q, int array, int row, int n) {
+    const char *base = static_cast<const char *>(a.in[array]);
+    const int cols = max(0, min(q.threads * kUnit * NU, q.end));   // the last CTA of a row may have none
+    from = base + ((int64_t)row * q.dim + q.first) * (int64_t)sizeof(T);
+    bytes = (uint32_t)(((n - 1) * q.dim + cols) * (int)sizeof(T));
+    shift = 0;
+    copied = cols > 0;
+    if constexpr (!ALIGNED) {
+      if (!copied) return;
+      shift = (uint32_t)(reinterpret_cast<uintptr_t>(from) & 15u);
+      const char *lo = from - shift;
+      const uint32_t padded = (shift + bytes + 15u) & ~15u;
+      copied = lo >= base && lo + padded <= base + a.p.rows * (int64_t)q.dim * (int64_t)sizeof(T);
+      from = copied ? lo : from;
+      bytes = padded;
+    }
+  }
+};
+
+// Shared memory: exchange slots, keep bits, the rings' barriers and the state of what fills them; then,
+// dynamic, the parameters and each group's ring.
+struct Shared {
+  Exchange exchange;
+  uint64_t bars[kMaxGroups * kMaxStages];
+  Batches ahead[kMaxGroups];
+  int fill_stage[kMaxGroups];
+  uint8_t keep[kMaxRowThreads];
+};
+
+template <typename T, bool ALIGNED, int NU, bool STATS>
+struct Ring {
+  Shared *s;
+  char *data;               // the group's stages
+  int stage = 0, phase = 0;  // of the next batch to use
+
+  __device__ __forceinline__ uint32_t bar(const Place &q, int st) const {
+    return sm100::smem_u32(s->bars + q.group * kMaxStages + st);
+  }
+  // Called by one thread of the group; its place ahead lives in shared memory, not in every thread's
+  // registers.
+  __device__ __forceinline__ void issue(const Args &a, const Place &q) {
+    Batches k = s->ahead[q.group];
+    if (k.seg >= a.segments) return;
+    const int st = s->fill_stage[q.group], n = k.count(a), row = k.row(a);
+    s->fill_stage[q.group] = st + 1 == a.stages ? 0 : st + 1;
+    const uint32_t to = sm100::smem_u32(data + (uint32_t)st * a.stage_bytes), b = bar(q, st);
+    uint32_t bytes = STATS ? 16u * n : 0u;
+#pragma unroll 1
+    for (int i = 0; i < kArrays; ++i)
+      if (a.in[i]) {
+        const Span<T, ALIGNED, NU> span(a, q, i, row, n);
+        if (span.copied) bytes += span.bytes;
+      }
+    sm100::mbar_expect_tx(b, bytes);
+    if (STATS)
+      sm100::bulk_load(to + (uint32_t)a.slot_count * a.slot_bytes, a.stats + 4 * (int64_t)row, 16u * n, b);
+#pragma unroll 1
+    for (int i = 0; i < kArrays; ++i)
+      if (a.in[i]) {
+        const Span<T, ALIGNED, NU> span(a, q, i, row, n);
+        if (span.copied) sm100::bulk_load(to + (uint32_t)a.slots[i] * a.slot_bytes, span.from, span.bytes, b);
+      }
+    k.next(a, q.group);
+    s->ahead[q.group] = k;
+  }
+  // Waits for the next batch and returns where its stage lies.
+  __device__ __forceinline__ char *wait(const Args &a, const Place &q) {
+    char *at = data + (uint32_t)stage * a.stage_bytes;
+    sm100::mbar_wait(bar(q, stage), phase, &g_row_errors, kWaitNs, sm100::kErrProducer);
+    if (++stage == a.stages) {
+      stage = 0;
+      phase ^= 1;
+    }
+    return at;
+  }
+  // Row i of the batch of `n` rows at `row`, from the CTA's first column on.
+  __device__ __forceinline__ const T *row_ptr(const Args &a, const Place &q, const char *at, int array, int row, int n,
+                                              int i) const {
+    const char *slot = at + (uint32_t)a.slots[array] * a.slot_bytes;
+    if constexpr (!ALIGNED) {
+      const Span<T, ALIGNED, NU> span(a, q, array, row, n);
+      slot = span.copied ? slot + span.shift : span.from;
+    }
+    return reinterpret_cast<const T *>(slot) + i * q.dim;
+  }
+  __device__ __forceinline__ float4 stats(const Args &a, const char *at, int i) const {
+    return reinterpret_cast<const float4 *>(at + (uint32_t)a.slot_count * a.slot_bytes)[i];
+  }
+};
+
+template <typename T, bool ALIGNED, int NU, bool STATS>
+__device__ __forceinline__ Ring<T, ALIGNED, NU, STATS> start_ring(const Args &a, const Place &q, Shared *s, char *data,
+                                                                  int cta, int ctas) {
+  Ring<T, ALIGNED, NU, STATS> r{s, data + (size_t)q.group * a.stages * a.stage_bytes};
+  if (threadIdx.x < kMaxGroups * kMaxStages) sm100::mbar_init(sm100::smem_u32(s->bars + threadIdx.x), 1);
+  sm100::fence_mbar_init();
+  if (q.t == 0) {
+    s->ahead[q.group] = batches_of(a, q.group, cta, ctas);
+    s->fill_stage[q.group] = 0;
+  }
+  __syncthreads();
+  if (a.members > 1) cluster_sync();
+  if (q.t == 0) {
+#pragma unroll 1
+    for (int i = 0; i < a.stages - 1; ++i) r.issue(a, q);
+  }
+  return r;
+}
+
+// The parameters' columns of each thread in fp32, in shared memory: two 16-byte pieces a unit, all threads' first
+// pieces and then their second ones, so that a warp reads consecutive banks.  (In registers they would take
+// eight a vector and thread beside the column sums.)  What is not given is its neutral value;
+// `factor` multiplies the post norm's weight and bias (the backward folds the dropout's scale in).
+template <bool ALIGNED, bool BLOCK, bool CENTER, int NU>
+__device__ __forceinline__ void stage_params(float4 *params, const Args &a, const Place &q, float factor) {
+  if (q.group == 0) {
+#pragma unroll
+    for (int k = 0; k < kParams; ++k) {
+      if (!BLOCK && k != kNextW && k != kNextB) continue;
+      if (!CENTER && (k == kPostB || k == kNextB)) continue;
+      const float fill = k == kScale ? a.p.scale_value : k == kPostB || k == kNextB ? 0.f : 1.f;
+      const float mul = k == kPostW || k == kPostB ? factor : 1.f;
+#pragma unroll
+      for (int n = 0; n < NU; ++n) {
+        float f[kUnit];
+#pragma unroll
+        for (int j = 0; j < kUnit; ++j) {
+          const int c = q.col<ALIGNED>(8 * n + j);
+          f[j] = !a.params[k] ? fill * mul : c < q.end ? mul * load_any(a.params[k], a.p.param_dtype, q.first + c) : 0.f;
+        }
+        float4 *to = params + 2 * (param_slot(BLOCK, k) * NU + n) * q.threads + q.t;
+        to[0] = make_float4(f[0], f[1], f[2], f[3]);
+        to[q.threads] = make_float4(f[4], f[5], f[6], f[7]);
+      }
+    }
+  }
+  if (a.groups > 1) __syncthreads();   // otherwise every thread reads what it wrote
+}
+template <int NU>   // k: the vector's place
+__device__ __forceinline__ void param(float2 (&f)[4 * NU], const float4 *params, int k, const Place &q) {
+#pragma unroll
+  for (int n = 0; n < NU; ++n) {
+    const float4 *from = params + 2 * (k * NU + n) * q.threads + q.t;
+    const float4 x = from[0], y = from[q.threads];
+    f[4 * n] = make_float2(x.x, x.y);
+    f[4 * n + 1] = make_float2(x.z, x.w);
+    f[4 * n + 2] = make_float2(y.x, y.y);
+    f[4 * n + 3] = make_float2(y.z, y.w);
+  }
+}
+
+// ------------------------------------------------------------------------ pieces of the formula
+__device__ __forceinline__ float activate(float g, int act) {
+  if (act == P3D_ACT_SIGMOID) return 1.f / (1.f + expf(-g));
+  if (act == P3D_ACT_TANH) return tanhf(g);
+  return g;
+}
+__device__ __forceinline__ float2 activate2(float2 g, int act) {
+  return act == P3D_ACT_IDENTITY ? g : make_float2(activate(g.x, act), activate(g.y, act));
+}
+// act'(gate) from act(gate)
+__device__ __forceinline__ float2 slope2(float2 a, int act) {
+  if (act == P3D_ACT_IDENTITY) return splat(1.f);
+  if (act == P3D_ACT_SIGMOID) return mul2(a, sub2(splat(1.f), a));
+  return fma2(mul2(a, splat(-1.f)), a, splat(1.f));
+}
+
+// Keep bits of the thread's columns of a row.  Unaligned threads own a column of each of many
+// blocks: the row's threads make one block's bits each and pass them through shared memory.
+template <bool ALIGNED, int NU>
+__device__ __forceinline__ uint32_t row_keep(const Args &a, const Place &q, PhiloxKey key, int64_t row, uint8_t *shared) {
+  const p3d_residual &p = a.p;
+  const uint64_t row_block = (uint64_t)row * (uint32_t)((p.dim + 7) / 8) + (uint32_t)(q.first / 8);
+  uint32_t bits = 0;
+  if constexpr (ALIGNED) {
+#pragma unroll
+    for (int n = 0; n < NU; ++n) bits |= keep_bits(key, row_block + q.at[n] / 8, p.threshold) << (8 * n);
+  } else {
+    q.barrier();   // the row before is done with the bits
+#pragma unroll
+    for (int n = 0; n < NU; ++n) {
+      const int b = q.t + n * q.threads;
+      if (8 * b < q.end) shared[b] = (uint8_t)keep_bits(key, row_block + b, p.threshold);
+    }
+    q.barrier();
+#pragma unroll
+    for (int j = 0; j < kUnit * NU; ++j) {
+      const int c = q.t + j * q.threads;
+      if (c < q.end) bits |= ((uint32_t)(shared[c >> 3] >> (c & 7)) & 1u) << j;
+    }
+  }
+  return bits;
+}
+__device__ __forceinline__ float2 kept(uint32_t keep, int i, float2 v) {
+  return make_float2((keep >> (2 * i) & 1u) ? v.x : 0.f, (keep >> (2 * i + 1) & 1u) ? v.y : 0.f);
+}
+
+// (mean, 1/deviation) of a row
+template <bool ALIGNED, bool CENTER, int NU>
+__device__ __forceinline__ float2 row_stats(RowSum &sum, const Place &q, const float2 (&z)[4 * NU], int kind, float eps,
+                                            float inv_dim) {
+  if (CENTER && kind == P3D_NORM_LAYER) {
+    const float2 m = sum.moments<ALIGNED, NU>(q, z, inv_dim);
+    return make_float2(m.x, rsqrtf(fmaf(m.y, inv_dim, eps)));
+  }
+  float2 s[NU];
+#pragma unroll
+  for (int n = 0; n < NU; ++n) {
+    s[n] = mul2(z[4 * n], z[4 * n]);
+#pragma unroll
+    for (int i = 1; i < 4; ++i) s[n] = fma2(z[4 * n + i], z[4 * n + i], s[n]);
+  }
+  float v[1] = {total<ALIGNED, NU>(q, s)};
+  sum(q, v);
+  return make_float2(0.f, rsqrtf(fmaf(v[0], inv_dim, eps)));
+}
+
+// ------------------------------------------------------------------------ forward
+// WHOLE: both norms are there.  GATE: the gate's mode, or kGateAny.  CENTER: a layer norm or a bias somewhere.
+template <typename T, bool ALIGNED, int NU, bool BLOCK, bool WHOLE, int GATE, bool DROP, bool CENTER>
+__global__ void __launch_bounds__(256, NU == 1 ? 4 : 2) fwd_kernel(const __grid_constant__ Args a) {
+  const p3d_residual &p = a.p;
+  extern __shared__ __align__(128) char s_data[];
+  __shared__ Shared s;
+  Place q = place_of<ALIGNED>(a);
+  set_columns<ALIGNED, NU>(q);
+  RowSum sum{&s.exchange, a.members};
+  const int cta = blockIdx.x / a.members, ctas = gridDim.x / a.members;
+  float4 *const params = reinterpret_cast<float4 *>(s_data);
+  auto ring = start_ring<T, ALIGNED, NU, false>(
+      a, q, &s, s_data + (size_t)2 * param_count(BLOCK, CENTER) * NU * a.row_threads * sizeof(float4), cta, ctas);
+  stage_params<ALIGNED, BLOCK, CENTER, NU>(params, a, q, 1.f);
+  const PhiloxKey key = philox_key(DROP ? p.rng : nullptr, p.seed, p.offset);
+  const float drop_scale = DROP ? keep_scale(p.threshold) : 1.f, inv_dim = 1.f / (float)q.dim;
+  const int gate_mode = GATE == kGateAny ? p.gate_mode : GATE;
+  const bool post_norm = WHOLE || p.post_kind != P3D_NORM_NONE, next_norm = WHOLE || p.next_kind != P3D_NORM_NONE;
+  for (Batches k = batches_of(a, q.group, cta, ctas); k.seg < a.segments; k.next(a, q.group)) {
+    const char *at = ring.wait(a, q);
+    const int n = k.count(a), row0 = k.row(a);
+    bool refilled = false;
+    auto refill = [&] {   // every thread of the group has left the batch before
+      if (!refilled && q.t == 0) ring.issue(a, q);
+      refilled = true;
+    };
+#pragma unroll 1
+    for (int i = 0; i < n; ++i) {
+      const int64_t row = row0 + i, base = row * q.dim + q.first;
+      float2 z[4 * NU], w[4 * NU], b[4 * NU];
+      float2 post = make_float2(0.f, 1.f), next = make_float2(0.f, 1.f);
+      if constexpr (BLOCK) {
+        float2 u[4 * NU], g[4 * NU];
+        load_cols<T, ALIGNED, NU>(u, ring.row_ptr(a, q, at, kH, row0, n, i), q);
+        if (gate_mode == P3D_GATE_ELEMENT) load_cols<T, ALIGNED, NU>(g, ring.row_ptr(a, q, at, kGate, row0, n, i), q);
+        if (gate_mode == P3D_GATE_SAMPLE)
+          load_cols<T, ALIGNED, NU>(
+              g, static_cast<const T *>(p.gate) + (int64_t)((int)row / (int)p.rows_per_sample) * q.dim + q.first, q);
+        float token = 1.f;
+        if (gate_mode == P3D_GATE_TOKEN) token = activate(to_f32<T>(static_cast<const T *>(p.gate)[row]), p.gate_act);
+        if (post_norm) {
+          post = row_stats<ALIGNED, CENTER, NU>(sum, q, u, p.post_kind, p.post_eps, inv_dim);
+          refill();
+          param<NU>(w, params, param_slot(BLOCK, kPostW), q);
+          if constexpr (CENTER) param<NU>(b, params, param_slot(BLOCK, kPostB), q);
+#pragma unroll
+          for (int j = 0; j < 4 * NU; ++j) {
+            if constexpr (CENTER) u[j] = fma2(mul2(sub2(u[j], splat(post.x)), splat(post.y)), w[j], b[j]);
+            else u[j] = mul2(mul2(u[j], splat(post.y)), w[j]);
+          }
+        }
+        if (gate_mode == P3D_GATE_TOKEN) {
+#pragma unroll
+          for (int j = 0; j < 4 * NU; ++j) u[j] = mul2(u[j], splat(token));
+        } else if (gate_mode != P3D_GATE_NONE) {
+#pragma unroll
+          for (int j = 0; j < 4 * NU; ++j) u[j] = mul2(u[j], activate2(g[j], p.gate_act));
+        }
+        if constexpr (DROP) {
+          const uint32_t keep = row_keep<ALIGNED, NU>(a, q, key, row, s.keep + q.group * a.row_threads * NU);
+#pragma unroll
+          for (int j = 0; j < 4 * NU; ++j) u[j] = kept(keep, j, mul2(u[j], splat(drop_scale)));
+        }
+        param<NU>(w, params, param_slot(BLOCK, kScale), q);
+        load_cols<T, ALIGNED, NU>(z, ring.row_ptr(a, q, at, kX, row0, n, i), q);
+#pragma unroll
+        for (int j = 0; j < 4 * NU; ++j) {
+          z[j] = fma2(w[j], u[j], z[j]);
+          if constexpr (!ALIGNED) {
+            if (!q.has<ALIGNED>(2 * j)) z[j].x = 0.f;
+            if (!q.has<ALIGNED>(2 * j + 1)) z[j].y = 0.f;
+          }
+        }
+        store_cols<T, ALIGNED, NU>(static_cast<T *>(a.out) + base, z, q);
+      } else {
+        load_cols<T, ALIGNED, NU>(z, ring.row_ptr(a, q, at, kX, row0, n, i), q);
+      }
+      if (next_norm) {
+        next = row_stats<ALIGNED, CENTER, NU>(sum, q, z, p.next_kind, p.next_eps, inv_dim);
+        refill();
+        param<NU>(w, params, param_slot(BLOCK, kNextW), q);
+        if constexpr (CENTER) param<NU>(b, params, param_slot(BLOCK, kNextB), q);
+#pragma unroll
+        for (int j = 0; j < 4 * NU; ++j) {
+          if constexpr (CENTER) z[j] = fma2(mul2(sub2(z[j], splat(next.x)), splat(next.y)), w[j], b[j]);
+          else z[j] = mul2(mul2(z[j], splat(next.y)), w[j]);
+        }
+        store_cols<T, ALIGNED, NU>(static_cast<T *>(a.y) + base, z, q);
+      }
+      if (a.stats && q.t == 0 && q.rank == 0)
+        reinterpret_cast<float4 *>(a.stats)[row] = make_float4(post.x, post.y, next.x, next.y);
+    }
+    if (!refilled) {
+      q.barrier();
+      refill();
+    }
+  }
+}
+
+// ------------------------------------------------------------------------ backward
+constexpr int kSums = 6;  // dscale, dpost_weight, dpost_bias, dnext_weight, dnext_bias, dgate
+
+// Adds the thread's sums, times `factor`, over the CTA's row groups (in group order) and writes them to dst.
+template <bool ALIGNED>
+__device__ __forceinline__ void join_groups(float2 (&acc)[4], float factor, float *smem, float *dst, const Args &a,
+                                            const Place &q) {
+  float v[kUnit];
+#pragma unroll
+  for (int j = 0; j < kUnit; ++j) v[j] = (j & 1 ? acc[j / 2].y : acc[j / 2].x) * factor;
+  if (a.groups > 1) {
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kUnit; ++j) smem[(q.group * kUnit + j) * a.row_threads + q.t] = v[j];
+    __syncthreads();
+    if (q.group == 0) {
+#pragma unroll
+      for (int j = 0; j < kUnit; ++j)
+        for (int g = 1; g < a.groups; ++g) v[j] += smem[(g * kUnit + j) * a.row_threads + q.t];
+    }
+  }
+  if (q.group == 0) {
+#pragma unroll
+    for (int j = 0; j < kUnit; ++j) {
+      const int c = q.col<ALIGNED>(j);
+      if (c < q.end) dst[q.first + c] = v[j];
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) acc[j] = splat(0.f);
+}
+
+// WHOLE: both norms, both upstream gradients and both gradients of tensors are there.
+template <typename T, bool ALIGNED, bool BLOCK, bool WHOLE, int GATE, bool DROP, bool CENTER>
+__global__ void __launch_bounds__(512, 1) bwd_kernel(const __grid_constant__ Args a) {
+  constexpr bool kGated = BLOCK && GATE != P3D_GATE_NONE;
+  const p3d_residual &p = a.p;
+  extern __shared__ __align__(128) char s_data[];
+  __shared__ Shared s;
+  Place q = place_of<ALIGNED>(a);
+  set_columns<ALIGNED, 1>(q);
+  RowSum sum{&s.exchange, a.members};
+  const int cta = blockIdx.x / a.members, ctas = gridDim.x / a.members;
+  float4 *const params = reinterpret_cast<float4 *>(s_data);
+  auto ring = start_ring<T, ALIGNED, 1, true>(
+      a, q, &s, s_data + (size_t)2 * param_count(BLOCK, CENTER) * a.row_threads * sizeof(float4), cta, ctas);
+  float *joins = reinterpret_cast<float *>(ring.data + (size_t)(a.groups - q.group) * a.stages * a.stage_bytes);
+  const PhiloxKey key = philox_key(DROP ? p.rng : nullptr, p.seed, p.offset);
+  // the dropout's scale is folded into the post norm's weight and bias, and into their gradients' sums at the end
+  const float drop_scale = DROP ? keep_scale(p.threshold) : 1.f;
+  stage_params<ALIGNED, BLOCK, CENTER, 1>(params, a, q, drop_scale);
+  const float inv_dim = 1.f / (float)q.dim;
+  const int gate_mode = GATE == kGateAny ? p.gate_mode : GATE;
+  const bool next_sums = WHOLE || a.in[kDy], has_dout = WHOLE || a.in[kDout];
+  const bool post_norm = WHOLE || p.post_kind != P3D_NORM_NONE, token = kGated && gate_mode == P3D_GATE_TOKEN;
+  const bool want_dx = WHOLE || a.dx, want_dh = WHOLE || a.dh;
+  // means of the normalised rows' gradients: nothing to take off where there is no norm, no mean in an RMS norm
+  const float next_mean = p.next_kind == P3D_NORM_LAYER ? -inv_dim : 0.f;
+  const float post_mean = p.post_kind == P3D_NORM_LAYER ? -inv_dim : 0.f, post_dot = post_norm ? -inv_dim : 0.f;
+  float2 a_scale[4] = {}, a_pw[4] = {}, a_pb[4] = {}, a_nw[4] = {}, a_nb[4] = {}, a_gate[4] = {};
+  const Batches first_batch = batches_of(a, q.group, cta, ctas);
+#pragma unroll 1
+  for (int seg = cta / a.slices; seg < a.segments; seg += first_batch.seg_step) {
+    const T *const sample = static_cast<const T *>(p.gate) + (int64_t)seg * q.dim + q.first;
+    Batches k = first_batch;
+    k.seg = seg;
+#pragma unroll 1
+    for (k.b = q.group; k.b < k.per_slice; k.b += a.groups) {
+      const char *at = ring.wait(a, q);
+      const int n = k.count(a), row0 = k.row(a);
+      bool refilled = false;
+      auto refill = [&] {
+        if (!refilled && q.t == 0) ring.issue(a, q);
+        refilled = true;
+      };
+#pragma unroll 1
+      for (int i = 0; i < n; ++i) {
+        const int64_t row = row0 + i, base = row * q.dim + q.first;
+        const float4 st = ring.stats(a, at, i);   // mean, 1/deviation of h, then of out
+        float2 w[4], u[4], hn[4], act[4], zn[4], G[4];
+        uint32_t keep = 0xffu;
+        if constexpr (BLOCK) {
+          load_cols<T, ALIGNED, 1>(hn, ring.row_ptr(a, q, at, kH, row0, n, i), q);
+          if constexpr (DROP) keep = row_keep<ALIGNED, 1>(a, q, key, row, s.keep + q.group * a.row_threads);
+          if constexpr (kGated) {
+            if (token) {
+              act[0] = splat(activate(to_f32<T>(static_cast<const T *>(p.gate)[row]), p.gate_act));
+#pragma unroll
+              for (int j = 1; j < 4; ++j) act[j] = act[0];
+            } else if (gate_mode == P3D_GATE_NONE) {   // only where the mode is an argument
+#pragma unroll
+              for (int j = 0; j < 4; ++j) act[j] = splat(1.f);
+            } else {
+              load_cols<T, ALIGNED, 1>(
+                  act, gate_mode == P3D_GATE_SAMPLE ? sample : ring.row_ptr(a, q, at, kGate, row0, n, i), q);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) act[j] = activate2(act[j], p.gate_act);
+            }
+          }
+          float2 b[4];
+          param<1>(w, params, param_slot(BLOCK, kPostW), q);
+          if constexpr (CENTER) param<1>(b, params, param_slot(BLOCK, kPostB), q);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if constexpr (CENTER) hn[j] = sub2(hn[j], splat(st.x));
+            hn[j] = mul2(hn[j], splat(st.y));      // h itself without a post norm: mean 0, 1/deviation 1
+            u[j] = CENTER ? fma2(hn[j], w[j], b[j]) : mul2(hn[j], w[j]);
+            if constexpr (DROP) u[j] = kept(keep, j, u[j]);
+          }
+        }
+        // u: the block's output with its dropout, before the gate; d = u act
+        if (has_dout) load_cols<T, ALIGNED, 1>(G, ring.row_ptr(a, q, at, kDout, row0, n, i), q);
+        else
+#pragma unroll
+          for (int j = 0; j < 4; ++j) G[j] = splat(0.f);
+        if (next_sums) {
+          float2 gy[4], s0[1], s1[1];
+          load_cols<T, ALIGNED, 1>(zn, ring.row_ptr(a, q, at, kX, row0, n, i), q);
+          load_cols<T, ALIGNED, 1>(gy, ring.row_ptr(a, q, at, kDy, row0, n, i), q);
+          if constexpr (BLOCK) {
+            param<1>(w, params, param_slot(BLOCK, kScale), q);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) zn[j] = fma2(w[j], kGated ? mul2(u[j], act[j]) : u[j], zn[j]);
+          }
+          param<1>(w, params, param_slot(BLOCK, kNextW), q);
+          s0[0] = s1[0] = splat(0.f);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if constexpr (CENTER) zn[j] = sub2(zn[j], splat(st.z));
+            zn[j] = mul2(zn[j], splat(st.w));
+            a_nw[j] = fma2(gy[j], zn[j], a_nw[j]);
+            if constexpr (CENTER) a_nb[j] = add2(a_nb[j], gy[j]);
+            gy[j] = mul2(gy[j], w[j]);
+            s1[0] = fma2(gy[j], zn[j], s1[0]);
+            if constexpr (CENTER) s0[0] = add2(s0[0], gy[j]);
+          }
+          float m0 = 0.f, m1;
+          if constexpr (CENTER) {
+            float v[2] = {total<ALIGNED, 1>(q, s1), total<ALIGNED, 1>(q, s0)};
+            sum(q, v);
+            m1 = v[0] * -inv_dim;
+            m0 = v[1] * next_mean;
+          } else {
+            float v[1] = {total<ALIGNED, 1>(q, s1)};
+            sum(q, v);
+            m1 = v[0] * -inv_dim;
+          }
+          refill();
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            float2 t = fma2(zn[j], splat(m1), gy[j]);
+            if constexpr (CENTER) t = add2(t, splat(m0));
+            G[j] = fma2(t, splat(st.w), G[j]);
+            if constexpr (!ALIGNED) {   // no column: nothing for the sums below
+              if (!q.has<ALIGNED>(2 * j)) G[j].x = 0.f;
+              if (!q.has<ALIGNED>(2 * j + 1)) G[j].y = 0.f;
+            }
+          }
+        }
+        if (want_dx) store_cols<T, ALIGNED, 1>(static_cast<T *>(a.dx) + base, G, q);
+        if constexpr (BLOCK) {
+          float2 s0[1], s1[1], s2[1], pw[4];
+          param<1>(w, params, param_slot(BLOCK, kScale), q);
+          param<1>(pw, params, param_slot(BLOCK, kPostW), q);
+          s0[0] = s1[0] = s2[0] = splat(0.f);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            a_scale[j] = fma2(G[j], kGated ? mul2(u[j], act[j]) : u[j], a_scale[j]);
+            G[j] = mul2(G[j], w[j]);
+            if constexpr (kGated) {
+              // u holds the dropout's scale already, so this is the gate's gradient
+              const float2 dg = mul2(mul2(G[j], u[j]), slope2(act[j], p.gate_act));
+              if (GATE == kGateAny || GATE == P3D_GATE_TOKEN) s2[0] = add2(s2[0], dg);
+              if (GATE == kGateAny || GATE == P3D_GATE_SAMPLE) a_gate[j] = add2(a_gate[j], dg);
+              G[j] = mul2(G[j], act[j]);
+              if (GATE == kGateAny || GATE == P3D_GATE_ELEMENT) act[j] = dg;
+            }
+            if constexpr (DROP) G[j] = kept(keep, j, G[j]);
+            a_pw[j] = fma2(G[j], hn[j], a_pw[j]);
+            if constexpr (CENTER) a_pb[j] = add2(a_pb[j], G[j]);
+            G[j] = mul2(G[j], pw[j]);
+            s1[0] = fma2(G[j], hn[j], s1[0]);
+            if constexpr (CENTER) s0[0] = add2(s0[0], G[j]);
+          }
+          if constexpr (GATE == kGateAny || GATE == P3D_GATE_ELEMENT) {
+            if (gate_mode == P3D_GATE_ELEMENT && a.dgate)
+              store_cols<T, ALIGNED, 1>(static_cast<T *>(a.dgate) + base, act, q);
+          }
+          float m0 = 0.f, m1 = 0.f;
+          if (post_norm || token) {
+            if constexpr (GATE == kGateAny || GATE == P3D_GATE_TOKEN) {
+              float v[3] = {total<ALIGNED, 1>(q, s1), total<ALIGNED, 1>(q, s0), total<ALIGNED, 1>(q, s2)};
+              sum(q, v);
+              m1 = v[0] * post_dot;
+              m0 = v[1] * post_mean;
+              if (token && a.dgate && q.t == 0 && q.rank == 0) static_cast<T *>(a.dgate)[row] = from_f32<T>(v[2]);
+            } else if constexpr (CENTER) {
+              float v[2] = {total<ALIGNED, 1>(q, s1), total<ALIGNED, 1>(q, s0)};
+              sum(q, v);
+              m1 = v[0] * post_dot;
+              m0 = v[1] * post_mean;
+            } else {
+              float v[1] = {total<ALIGNED, 1>(q, s1)};
+              sum(q, v);
+              m1 = v[0] * post_dot;
+            }
+            refill();
+          }
+          if (want_dh) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              G[j] = fma2(hn[j], splat(m1), G[j]);
+              if constexpr (CENTER) G[j] = add2(G[j], splat(m0));
+              G[j] = mul2(G[j], splat(st.y));
+            }
+            store_cols<T, ALIGNED, 1>(static_cast<T *>(a.dh) + base, G, q);
+          }
+        }
+      }
+      if (!refilled) {
+        q.barrier();
+        refill();
+      }
+    }
+    if constexpr (GATE == kGateAny || GATE == P3D_GATE_SAMPLE) {
+      if (gate_mode == P3D_GATE_SAMPLE && a.dgate)
+        join_groups<ALIGNED>(a_gate, 1.f, joins,
+                             a.partials + ((int64_t)(kSums - 1) * ctas + (int64_t)seg * a.slices + cta % a.slices) * q.dim,
+                             a, q);
+    }
+  }
+  // the slots of sums that this variant does not have are not read either
+  float *const mine = a.partials + (int64_t)cta * q.dim;
+  const int64_t next = (int64_t)ctas * q.dim;
+  if constexpr (BLOCK) {
+    join_groups<ALIGNED>(a_scale, 1.f, joins, mine, a, q);
+    join_groups<ALIGNED>(a_pw, drop_scale, joins, mine + next, a, q);
+    if constexpr (CENTER) join_groups<ALIGNED>(a_pb, drop_scale, joins, mine + 2 * next, a, q);
+  }
+  join_groups<ALIGNED>(a_nw, 1.f, joins, mine + 3 * next, a, q);
+  if constexpr (CENTER) join_groups<ALIGNED>(a_nb, 1.f, joins, mine + 4 * next, a, q);
+}
+
+// ------------------------------------------------------------------------ launches
+template <typename K>
+int launch(K kernel, const Args &a, int64_t ctas, size_t smem, size_t (&seen)[kMaxDevices], cudaStream_t stream) {
+  if (int st = smem_optin(kernel, smem, seen)) return st;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(ctas * a.members));
+  cfg.blockDim = dim3((unsigned)(a.row_threads * a.groups));
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)a.members;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = a.members > 1 ? 1 : 0;
+  P3D_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, a));
+  return P3D_OK;
+}
+
+template <typename T, bool ALIGNED, int NU, bool BLOCK, bool WHOLE, int GATE, bool DROP, bool CENTER>
+int fwd(const Args &a, int64_t ctas, size_t smem, cudaStream_t s) {
+  static size_t seen[kMaxDevices] = {};
+  return launch(fwd_kernel<T, ALIGNED, NU, BLOCK, WHOLE, GATE, DROP, CENTER>, a, ctas, smem, seen, s);
+}
+template <typename T, bool ALIGNED, bool BLOCK, bool WHOLE, int GATE, bool DROP, bool CENTER>
+int bwd(const Args &a, int64_t ctas, size_t smem, cudaStream_t s) {
+  static size_t seen[kMaxDevices] = {};
+  return launch(bwd_kernel<T, ALIGNED, BLOCK, WHOLE, GATE, DROP, CENTER>, a, ctas, smem, seen, s);
+}
+
+// Calls f with `b` as a constant.
+template <typename F>
+int with(bool b, F &&f) {
+  return b ? f(std::true_type{}) : f(std::false_type{});
+}
+// Calls f with the gate's mode as a constant.
+template <typename F>
+int with_gate(int mode, F &&f) {
+  switch (mode) {
+    case P3D_GATE_NONE: return f(std::integral_constant<int, P3D_GATE_NONE>{});
+    case P3D_GATE_ELEMENT: return f(std::integral_constant<int, P3D_GATE_ELEMENT>{});
+    case P3D_GATE_SAMPLE: return f(std::integral_constant<int, P3D_GATE_SAMPLE>{});
+    default: return f(std::integral_constant<int, P3D_GATE_TOKEN>{});
+  }
+}
+
+// Calls that have no block, or a block between two norms (in the backward with all gradients), have
+// variants of their own; the other aligned ones share one that centres.
+inline bool whole_fwd(const Args &a) {
+  return !a.p.h || (a.p.post_kind != P3D_NORM_NONE && a.p.next_kind != P3D_NORM_NONE);
+}
+inline bool whole_bwd(const Args &a) {
+  return !a.p.h || (a.p.post_kind != P3D_NORM_NONE && a.in[kDy] && a.in[kDout] && a.dx && a.dh);
+}
+
+// Aligned rows between two norms, the usual block, get variants of their own for the gate, dropout and centring: each
+// saves registers or instructions of a kernel that is bound by both.  Other calls share variants that read
+// what they have from the arguments.
+template <typename T>
+int run_fwd(const Args &a, bool aligned, bool center, bool two_units, int64_t ctas, size_t smem, cudaStream_t s) {
+  const bool whole = aligned && whole_fwd(a);
+  return with(two_units, [&](auto nu) {
+    constexpr int NU = decltype(nu)::value ? 2 : 1;
+    return with(center, [&](auto ce) {
+      constexpr bool C = decltype(ce)::value;
+      if (!a.p.h)
+        return aligned ? fwd<T, true, NU, false, false, P3D_GATE_NONE, false, C>(a, ctas, smem, s)
+                       : fwd<T, false, NU, false, false, P3D_GATE_NONE, false, C>(a, ctas, smem, s);
+      if (!whole) {
+        if (aligned) return fwd<T, true, NU, true, false, kGateAny, true, true>(a, ctas, smem, s);
+        return with(a.p.threshold != 0, [&](auto dr) {
+          return fwd<T, false, NU, true, false, kGateAny, decltype(dr)::value, C>(a, ctas, smem, s);
+        });
+      }
+      return with_gate(a.p.gate_mode, [&](auto ga) {
+        return with(a.p.threshold != 0, [&](auto dr) {
+          return fwd<T, true, NU, true, true, decltype(ga)::value, decltype(dr)::value, C>(a, ctas, smem, s);
+        });
+      });
+    });
+  });
+}
+
+template <typename T>
+int run_bwd(const Args &a, bool aligned, bool center, int64_t ctas, size_t smem, cudaStream_t s) {
+  const bool whole = aligned && whole_bwd(a);
+  return with(center, [&](auto ce) {
+    constexpr bool C = decltype(ce)::value;
+    if (!a.p.h)
+      return aligned ? bwd<T, true, false, false, P3D_GATE_NONE, false, C>(a, ctas, smem, s)
+                     : bwd<T, false, false, false, P3D_GATE_NONE, false, C>(a, ctas, smem, s);
+    if (!whole) {
+      if (aligned) return bwd<T, true, true, false, kGateAny, true, true>(a, ctas, smem, s);
+      return with(a.p.gate_mode != P3D_GATE_NONE, [&](auto ga) {
+        return with(a.p.threshold != 0, [&](auto dr) {
+          return bwd<T, false, true, false, decltype(ga)::value ? kGateAny : P3D_GATE_NONE, decltype(dr)::value, C>(
+              a, ctas, smem, s);
+        });
+      });
+    }
+    return with_gate(a.p.gate_mode, [&](auto ga) {
+      return with(a.p.threshold != 0, [&](auto dr) {
+        return bwd<T, true, true, true, decltype(ga)::value, decltype(dr)::value, C>(a, ctas, smem, s);
+      });
+    });
+  });
+}
+
+template <typename T>
+int take_errors(unsigned *flags) {
+  unsigned v = 0, zero = 0;
+  P3D_CUDA_TRY(cudaMemcpyFromSymbol(&v, g_row_errors, sizeof(v)));
+  P3D_CUDA_TRY(cudaMemcpyToSymbol(g_row_errors, &zero, sizeof(zero)));
+  *flags |= v;
+  return P3D_OK;
+}
+
+#define P3D_ROW_KERNELS(T)                                                                        \
+  template int run_fwd<T>(const Args &, bool, bool, bool, int64_t, size_t, cudaStream_t);         \
+  template int run_bwd<T>(const Args &, bool, bool, int64_t, size_t, cudaStream_t);               \
+  template int take_errors<T>(unsigned *);
+
+}  // namespace rows
+}  // namespace p3d
