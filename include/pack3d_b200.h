@@ -500,6 +500,32 @@ P3D_API int p3d_fp8_matmul(const void *a, int64_t a_pitch, const void *a_scales,
                    const void *b_scales, int64_t rows, int64_t cols, int64_t k, const void *bias, int bias_dtype,
                    void *out, int out_dtype, void *workspace, size_t workspace_bytes, void *stream);
 
+/*
+ * A linear layer over such matrices, one call a direction.  x [rows, k] and dy [rows, n] of dtype, weight [n, k]
+ *   of weight_dtype, quantised in the call (its gradient, and x's where need_dx / need_dw say so), or
+ *   weight NULL and its values, pitch and scales (square blocks) as kept by the caller.
+ * p3d_fp8_linear_fwd: y [rows, n] = Q(x) Q(weight)^T (+ bias [n] of bias_dtype); saved:
+ *   p3d_fp8_linear_saved() bytes for the backward (may be NULL without gradients): x with blocks of 128
+ *   rows, the weight transposed.
+ * p3d_fp8_linear_bwd: dx [rows, k] of dtype, dw [n, k] of weight_dtype, dbias [n] of bias_dtype or NULL.
+ * saved and workspace (p3d_fp8_linear_*_workspace() bytes) are 256-byte aligned.
+ */
+typedef struct {
+  int64_t rows, k, n;
+  const void *weight;
+  const void *weight_values, *weight_scales;
+  int64_t weight_pitch;
+  int32_t dtype, weight_dtype, bias_dtype;
+  int32_t need_dx, need_dw;
+} p3d_fp8_linear;
+P3D_API size_t p3d_fp8_linear_saved(const p3d_fp8_linear *args);
+P3D_API size_t p3d_fp8_linear_fwd_workspace(const p3d_fp8_linear *args);
+P3D_API size_t p3d_fp8_linear_bwd_workspace(const p3d_fp8_linear *args);
+P3D_API int p3d_fp8_linear_fwd(const p3d_fp8_linear *args, const void *x, const void *bias, void *y, void *saved,
+                       void *workspace, size_t workspace_bytes, void *stream);
+P3D_API int p3d_fp8_linear_bwd(const p3d_fp8_linear *args, const void *dy, const void *saved, void *dx, void *dw,
+                       void *dbias, void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

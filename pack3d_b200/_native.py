@@ -62,9 +62,10 @@ class PeerCopy(ctypes.Structure):
                 ("src_stride", ctypes.c_int64), ("dst_stride", ctypes.c_int64)]
 
 
-#: ``p3d_residual`` of ``include/pack3d_b200.h``, packed by :mod:`pack3d_b200.residual` for each call (packing the
-#: bytes takes a fraction of the time of filling a ctypes structure field by field)
+#: ``p3d_residual`` and ``p3d_fp8_linear`` of ``include/pack3d_b200.h``, packed for each call (packing the bytes
+#: takes a fraction of the time of filling a ctypes structure field by field)
 RESIDUAL = struct.Struct("@2q9P2Q7iI3f4x")
+FP8_LINEAR = struct.Struct("@3q3Pq5i4x")
 
 PEER_HANDLE_BYTES = 64
 PEER_MAX_COPIES = 32
@@ -127,6 +128,11 @@ _SIGNATURES = {
     "p3d_fp8_matmul_workspace": (ctypes.c_size_t, [_c_i64] * 3),
     "p3d_fp8_matmul": (_c_int, [_vp, _c_i64, _vp, _vp, _c_i64, _vp, _c_i64, _c_i64, _c_i64, _vp, _c_int, _vp, _c_int,
                                 _vp, ctypes.c_size_t, _vp]),
+    "p3d_fp8_linear_saved": (ctypes.c_size_t, [_vp]),
+    "p3d_fp8_linear_fwd_workspace": (ctypes.c_size_t, [_vp]),
+    "p3d_fp8_linear_bwd_workspace": (ctypes.c_size_t, [_vp]),
+    "p3d_fp8_linear_fwd": (_c_int, [_vp] * 6 + [ctypes.c_size_t, _vp]),
+    "p3d_fp8_linear_bwd": (_c_int, [_vp] * 7 + [ctypes.c_size_t, _vp]),
     "p3d_peer_alloc": (_c_int, [ctypes.c_size_t, ctypes.POINTER(_vp), _vp]),
     "p3d_peer_free": (_c_int, [_vp]),
     "p3d_peer_open": (_c_int, [_vp, ctypes.POINTER(_vp)]),
@@ -181,6 +187,27 @@ def ptr(t):
 
 def stream_of(device):
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+class on:
+    """``with torch.cuda.device(device)`` where that is not the current device already; gives the current stream's
+    address there."""
+    __slots__ = ("device", "inner")
+
+    def __init__(self, device):
+        self.device = device
+        self.inner = None
+
+    def __enter__(self):
+        if self.device.index != torch.cuda.current_device():
+            self.inner = torch.cuda.device(self.device)
+            self.inner.__enter__()
+        # what torch.cuda.current_stream(device).cuda_stream says, without building a Stream object
+        return torch._C._cuda_getCurrentRawStream(self.device.index)
+
+    def __exit__(self, *exc):
+        if self.inner is not None:
+            self.inner.__exit__(*exc)
 
 
 def device_errors():

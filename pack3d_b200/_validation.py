@@ -12,6 +12,7 @@ callers catching them keep working) with three deliberate differences:
 * the 32-bit indexing limit is replaced by the 64-bit addressing of the
   kernels (a tensor may hold up to 2**40 elements).
 """
+import functools
 import math
 
 import torch
@@ -52,10 +53,14 @@ def validate_inputs(q, kl, vl, kg, vg, weight, bias, gate, sl, sg, geometry, tem
         raise ValueError("temperature must be finite and positive")
 
 
+@functools.lru_cache(maxsize=None)
+def _compute_major(index):
+    return torch.cuda.get_device_capability(index)[0]
+
+
 def check_cuda(q):
     """The backend runs only on CUDA sm_100 devices, in fp32 / fp16 / bf16."""
     if q.device.type != "cuda" or q.dtype not in COMPUTE_DTYPES:
         raise ValueError("b200 backend requires CUDA fp32/fp16/bf16 Q/K/V")
-    major, _ = torch.cuda.get_device_capability(q.device)
-    if major != 10:
+    if _compute_major(q.device.index) != 10:
         raise ValueError("b200 backend targets compute capability 10.x (sm_100a) devices")

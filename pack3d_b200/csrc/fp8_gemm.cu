@@ -4,14 +4,19 @@
 // kind): products of e4m3 and their powers of two are exact in fp32, so nothing but the fp32
 // accumulation and the last rounding is inexact, and no accumulator leaves TMEM before its tile is done.
 //
-// Work unit: a 128 x BN tile of the output, or a slice of its k (split) when there are fewer tiles than
-// SMs; CTAs walk units persistently.  Roles: warp 0 TMA producer (a ring of 128-column slices of both
-// operands, 128-byte rows, SWIZZLE_128B, with the scale bytes of four slices when a new four
-// begin), warp 1 MMA issuer (copies those bytes to TMEM, where one byte of a row's word scales one
-// slice, and issues the products into one of two accumulators), warps 2-5 epilogue (one row a
-// thread).  Few rows of `a` (tokens of a decode step) are taken as the N side (SWAP): the weight's rows
-// then fill the 128 lanes and the token count only sets N.
-// Slices of k go to fp32 partials that a second kernel adds in slice order.
+// Two kernels share the scheme: CTAs walk work units persistently (a tile of the output, or a slice of its k
+// where there are fewer tiles than SMs; slices go to fp32 partials that a second kernel adds in slice
+// order), warp 0 is the TMA producer (a ring of 128-column slices of both operands, 128-byte rows,
+// SWIZZLE_128B, with the scale bytes of four slices when a new four begin), warp 1 the MMA issuer (it
+// copies those bytes to TMEM, where one byte of a row's word scales one slice, and issues the
+// products), the others the epilogue (one row a thread).
+//   pair kernel     256 x 256 (or 128) tiles of a pair of SMs, each holding half of either operand: the L2
+//                   feeds all SMs about 10 TB/s here, and a 128 x 128 tile asks for twice the bytes a
+//                   product that this one does (1.3 against 2.5 PFLOP/s at 16384 x 8192 x 2048).  The
+//                   accumulator of 256 columns has no room for a second beside the scales: the epilogue
+//                   takes it to registers at once and frees it.  Rows go out through shared memory by TMA.
+//   narrow kernel   up to 64 rows of `a` (tokens of a decode step) are the N side: the weight's rows then
+//                   fill the 128 lanes and the token count only sets N.  128 x 128 tiles for up to 128 rows.
 //
 // Every wait is bounded (2 s): on a timeout the kernel records an error bit (p3d_device_errors), drains its
 // copies and MMAs and frees TMEM.
@@ -127,7 +132,7 @@ template <int BN, bool SWAP>
 __global__ void __launch_bounds__(kThreads, 1)
     fp8_gemm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb, const GemmParams p) {
   constexpr int kChunksB = (BN + 127) / 128;            // 512-byte scale chunks of the N operand
-  constexpr uint32_t kBytesA = kTileM * kSlice, kBytesB = BN * kSlice, kBytesS = 512u * (1 + kChunksB);
+  constexpr uint32_t kBytesA = kTileM * kSlice, kBytesB = BN * kSlice;
   constexpr uint32_t kStageBytes = kBytesA + (kBytesB + 1023u) / 1024u * 1024u + 2048u;
   constexpr int kAccCols = BN < 32 ? 32 : BN;
   constexpr int kScaleCols = 4 + 4 * kChunksB;           // per buffer; two buffers
@@ -317,6 +322,305 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
+// ------------------------------------------------------------------------ the pair kernel
+constexpr int kPairThreads = 320;      // producer, MMA issuer, eight epilogue warps
+constexpr int kPairRows = 256;
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t in_cta(uint32_t smem, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void arrive_at(uint32_t cluster_bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+}
+// A wait on arrivals of the other CTA too: ordered over the cluster once the phase is done.
+__device__ __forceinline__ bool wait_cluster(uint32_t bar, uint32_t parity, unsigned role) {
+  const bool ok = mbar_wait(bar, parity, &g_fp8_errors, kWaitNs, role);
+  asm volatile("fence.acq_rel.cluster;" ::: "memory");
+  return ok;
+}
+// Into this CTA's shared memory, signalling a barrier of the pair's first CTA.
+__device__ __forceinline__ void pair_load_2d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int c0, int c1) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, "
+      "%4}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1)
+      : "memory");
+}
+__device__ __forceinline__ void store_3d(const CUtensorMap *map, uint32_t src, int c0, int c1, int c2) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(src), "r"(c0), "r"(c1), "r"(c2)
+               : "memory");
+}
+__device__ __forceinline__ void pair_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb,
+                                         uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void pair_copy_scales(uint32_t tmem, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+}
+// Arrives at the same barrier of both CTAs once all MMAs and copies issued so far are done.
+__device__ __forceinline__ void pair_commit(uint32_t bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+      "h"((uint16_t)3)
+      : "memory");
+}
+
+// 16-byte pieces of a thread's 128-byte row segment, as the 128-byte swizzle lays them out, from fp32 values.
+template <typename T>
+__device__ __forceinline__ void stage_row(char *row_base, int row, const float *v) {
+  constexpr int n = 16 / sizeof(T);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    uint4 w;
+    if constexpr (sizeof(T) == 4) {
+      w = make_uint4(__float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]), __float_as_uint(v[4 * i + 2]),
+                     __float_as_uint(v[4 * i + 3]));
+    } else {
+      uint32_t h[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) h[j] = pack_bf16(v[n * i + 2 * j], v[n * i + 2 * j + 1]);
+        else h[j] = pack_f16(v[n * i + 2 * j], v[n * i + 2 * j + 1]);
+      }
+      w = make_uint4(h[0], h[1], h[2], h[3]);
+    }
+    *reinterpret_cast<uint4 *>(row_base + ((i ^ (row & 7)) * 16)) = w;
+  }
+}
+
+template <typename T, int BN>
+__device__ __forceinline__ void pair_epilogue(const CUtensorMap *tout, const GemmParams &p, const Unit &w, float (&v)[BN / 2],
+                                              int row0, int col0, int lane, char *stage) {
+  constexpr int kCols = 128 / sizeof(T);   // columns of a 128-byte segment
+  if (p.vector) {
+#pragma unroll
+    for (int c = 0; c < BN / 2; c += kCols) {
+      if (col0 + c >= p.cols || row0 >= p.rows) break;   // the same in the whole warp
+      if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+      __syncwarp();
+      stage_row<T>(stage + lane * 128, lane, v + c);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        store_3d(tout, smem_u32(stage), col0 + c, row0, w.split);
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+      }
+    }
+  } else if (row0 + lane < p.rows) {
+    T *dst = static_cast<T *>(p.out) + (int64_t)(row0 + lane) * p.pitch + col0 + (int64_t)w.split * p.split_stride;
+#pragma unroll
+    for (int j = 0; j < BN / 2; ++j)
+      if (col0 + j < p.cols) dst[j] = from_f32<T>(v[j]);
+  }
+}
+
+template <int BN>
+__global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
+    fp8_pair_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb,
+                    const __grid_constant__ CUtensorMap tsa, const __grid_constant__ CUtensorMap tsb,
+                    const __grid_constant__ CUtensorMap tout, const GemmParams p) {
+  constexpr int kChunksB = BN / 128;
+  constexpr uint32_t kBytesA = kTileM * kSlice, kBytesB = BN / 2 * kSlice, kBytesS = 512u * (1 + kChunksB);
+  constexpr uint32_t kStageBytes = kBytesA + kBytesB + 2048u;   // the scale bytes in the last 2048
+  constexpr int kScaleCols = 4 + 4 * kChunksB;
+  constexpr int kAccs = 2 * BN + 2 * kScaleCols <= 512 ? 2 : 1;
+  constexpr int kTmemCols = 512;
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  __shared__ __align__(8) uint64_t s_bars[2 * kMaxStages + 5];
+  __shared__ uint32_t tmem_holder;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+  const uint32_t bars = smem_u32(s_bars);
+  const int S = p.stages;
+  auto full = [&](int s) { return bars + 8u * s; };      // the first CTA's, for both
+  auto empty = [&](int s) { return bars + 8u * (kMaxStages + s); };
+  auto acc_full = [&](int a) { return bars + 8u * (2 * kMaxStages + a); };
+  auto acc_empty = [&](int a) { return bars + 8u * (2 * kMaxStages + 2 + a); };   // the first CTA's, for both
+  const uint32_t drain = bars + 8u * (2 * kMaxStages + 4);
+  const int units = p.tiles_m * p.tiles_n * p.splits, pairs = gridDim.x / 2, pair = blockIdx.x / 2;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(full(s), 1);
+      mbar_init(empty(s), 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(acc_full(a), 1);
+      mbar_init(acc_empty(a), 16);
+    }
+    mbar_init(drain, 1);
+    fence_mbar_init();
+  }
+  if (warp == kMmaWarp) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_holder)),
+                 "r"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  if (warp == kProducerWarp && lane == 0) {
+    prefetch_tmap(&ta);
+    prefetch_tmap(&tb);
+    prefetch_tmap(&tsa);
+    prefetch_tmap(&tsb);
+    if (p.vector) prefetch_tmap(&tout);
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem = tmem_holder;
+
+  if (warp == kProducerWarp) {
+    // ------------------------------------------------------------------ TMA producer, one in each CTA
+    if (lane == 0) {
+      const int groups = (p.slices + 3) / 4;
+      int it = 0, s = 0;
+      uint32_t turn = 1;   // parity of the empty phase to wait for
+      bool ok = true;
+      for (int u = pair; ok && u < units; u += pairs) {
+        const Unit w = unit_of(p, u);
+        const int m0 = 2 * w.tm + (int)rank;   // this CTA's 128 rows; past the end everything reads as zero
+        for (int kb = w.begin; kb < w.end; ++kb, ++it) {
+          if (it >= S && !mbar_wait(empty(s), turn, &g_fp8_errors, kWaitNs, kErrProducer)) {
+            ok = false;
+            break;
+          }
+          const uint32_t st = base + s * kStageBytes, bar = in_cta(full(s), 0);
+          const bool scales = kb == w.begin || kb % 4 == 0;
+          if (rank == 0) mbar_expect_tx(full(s), 2 * (kBytesA + kBytesB + (scales ? kBytesS : 0u)));
+          pair_load_2d(st, &ta, bar, kb * kSlice, m0 * 128);
+          pair_load_2d(st + kBytesA, &tb, bar, kb * kSlice, w.tn * BN + (int)rank * (BN / 2));
+          if (scales) {
+            const uint32_t at = st + kStageBytes - 2048u;
+            pair_load_2d(at, &tsa, bar, 0, m0 * groups + kb / 4);
+            for (int c = 0; c < kChunksB; ++c)
+              pair_load_2d(at + 512u * (1 + c), &tsb, bar, 0, (w.tn * kChunksB + c) * groups + kb / 4);
+          }
+          if (++s == S) {
+            s = 0;
+            turn ^= 1;
+          }
+        }
+      }
+      // every stage used: its products are done, so its copies are too
+      for (int i = it > S ? it - S : 0; i < it; ++i)
+        mbar_wait(empty(i % S), (i / S) & 1, &g_fp8_errors, kWaitNs, kErrTeardown);
+    }
+  } else if (warp == kMmaWarp) {
+    // ------------------------------------------------------------------ MMA issuer, of the first CTA for both
+    if (lane == 0 && rank == 0) {
+      constexpr uint32_t idesc = idesc_scaled(kPairRows, BN);
+      const uint32_t scale_cols = tmem + kAccs * BN;
+      const uint64_t desc_a = desc_sw128(base, 1024), desc_b = desc_sw128(base + kBytesA, 1024);
+      const uint64_t desc_s = desc_scales(base + kStageBytes - 2048u);
+      int n = 0, groups = 0, s = 0;
+      uint32_t turn = 0;
+      bool ok = true;
+      for (int u = pair; ok && u < units; u += pairs, ++n) {
+        const Unit w = unit_of(p, u);
+        const int a = n % kAccs;
+        if (n >= kAccs && !wait_cluster(acc_empty(a), (n / kAccs - 1) & 1, kErrMma)) break;
+        tc_fence_after();
+        for (int kb = w.begin; kb < w.end; ++kb) {
+          if (!mbar_wait(full(s), turn, &g_fp8_errors, kWaitNs, kErrMma)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint64_t off = (uint64_t)(s * kStageBytes >> 4);
+          if (kb == w.begin || kb % 4 == 0) {
+            // the other buffer: products of the four slices before may still read theirs
+            const uint32_t to = scale_cols + (groups & 1) * kScaleCols;
+#pragma unroll
+            for (int c = 0; c < 1 + kChunksB; ++c) pair_copy_scales(to + 4 * c, desc_s + off + 32u * c);
+            ++groups;
+          }
+          const uint32_t sc = scale_cols + ((groups - 1) & 1) * kScaleCols;
+          const uint32_t id = idesc | scale_ids(kb % 4);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)   // 32 columns: 32 bytes along the 128-byte rows
+            pair_mma(tmem + a * BN, desc_a + off + 2 * k, desc_b + off + 2 * k, id, sc, sc + 4,
+                     kb > w.begin || k > 0 ? 1u : 0u);
+          pair_commit(empty(s));
+          if (++s == S) {
+            s = 0;
+            turn ^= 1;
+          }
+        }
+        if (!ok) break;
+        pair_commit(acc_full(a));
+      }
+      pair_commit(drain);
+      mbar_wait(drain, 0, &g_fp8_errors, kWaitNs, kErrTeardown);
+    }
+  } else {
+    // ------------------------------------------------------------------ epilogue
+    const int quarter = warp & 3, half = (warp - 2) >> 2;   // TMEM lanes and columns of this warp
+    const uint32_t from = tmem + ((uint32_t)(quarter * 32) << 16) + half * (BN / 2);
+    char *const stage = reinterpret_cast<char *>(smem_raw) + (base - raw) + S * kStageBytes + (warp - 2) * 4096;
+    int n = 0;
+    for (int u = pair; u < units; u += pairs, ++n) {
+      const Unit w = unit_of(p, u);
+      const int a = n % kAccs;
+      const int row0 = w.tm * kPairRows + (int)rank * 128 + quarter * 32, col0 = w.tn * BN + half * (BN / 2);
+      float add[BN / 64];   // the bias of columns lane, lane + 32, ..
+#pragma unroll
+      for (int i = 0; i < BN / 64; ++i) {
+        const int c = col0 + 32 * i + lane;
+        add[i] = p.bias && c < p.cols ? load_any(p.bias, p.bias_type, c) : 0.f;
+      }
+      const bool ready = mbar_wait(acc_full(a), (n / kAccs) & 1, &g_fp8_errors, kWaitNs, kErrSoftmax);
+      if (!__all_sync(0xffffffffu, ready)) break;
+      tc_fence_after();
+      uint32_t r[BN / 2];
+#pragma unroll
+      for (int c = 0; c < BN / 2; c += 32) tmem_ld32(from + a * BN + c, r + c);
+      tmem_wait_ld();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) arrive_at(in_cta(acc_empty(a), 0));
+      float v[BN / 2];
+#pragma unroll
+      for (int j = 0; j < BN / 2; ++j) v[j] = __uint_as_float(r[j]);
+      if (p.bias) {
+#pragma unroll
+        for (int j = 0; j < BN / 2; ++j) v[j] += __shfl_sync(0xffffffffu, add[j / 32], j % 32);
+      }
+      if (p.out_type == P3D_BF16) pair_epilogue<__nv_bfloat16, BN>(&tout, p, w, v, row0, col0, lane, stage);
+      else if (p.out_type == P3D_F16) pair_epilogue<__half, BN>(&tout, p, w, v, row0, col0, lane, stage);
+      else pair_epilogue<float, BN>(&tout, p, w, v, row0, col0, lane, stage);
+      __syncwarp();
+    }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();   // the other CTA's barriers, shared memory and TMEM are in use until here
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+  }
+}
+
 // out = the partials added in slice order, plus the bias.
 __global__ void __launch_bounds__(256) add_splits_kernel(const float *part, int splits, int64_t rows, int64_t cols,
                                                          const void *bias, int bias_type, void *out, int out_type,
@@ -333,24 +637,52 @@ __global__ void __launch_bounds__(256) add_splits_kernel(const float *part, int 
 
 struct Plan {
   int bn;
-  bool swap;
+  bool swap, pair;
   int tiles_m, tiles_n, splits;
   int64_t rows, cols;   // tile space
 };
 
-// Tokens up to 64 become the N side.  Splits: as many slices of k as fill the SMs, each of at least two
-// 128-column slices.
+// More than 128 rows go to the pair kernel, with the narrower tile where that makes less work of the last wave
+// (a tile costs its columns and about 64 more for filling the pipeline); up to 64 rows (tokens)
+// become the N side.  Splits: as many slices of k as fill the SMs, each of at least two 128-column
+// slices (four for a pair).
 Plan plan_of(int64_t rows, int64_t cols, int64_t k, int sms) {
   Plan p;
+  const int64_t slices = (k + kSlice - 1) / kSlice;
+  p.pair = rows > 128;
   p.swap = rows <= 64;
   p.rows = p.swap ? cols : rows;
   p.cols = p.swap ? rows : cols;
-  p.bn = !p.swap ? 128 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
-  p.tiles_m = (int)((p.rows + kTileM - 1) / kTileM);
+  int64_t slots = sms, least = 2;
+  if (p.pair) {
+    slots = sms / 2;
+    least = 4;
+    p.tiles_m = (int)((rows + kPairRows - 1) / kPairRows);
+    auto cost = [&](int bn) { return (p.tiles_m * ((cols + bn - 1) / bn) + slots - 1) / slots * (bn + 64); };
+    p.bn = cost(128) < cost(256) ? 128 : 256;
+  } else {
+    p.bn = !p.swap ? 128 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+    p.tiles_m = (int)((p.rows + kTileM - 1) / kTileM);
+  }
   p.tiles_n = (int)((p.cols + p.bn - 1) / p.bn);
-  const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n, slices = (k + kSlice - 1) / kSlice;
-  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({sms / std::max<int64_t>(1, tiles), slices / 2, 64}));
+  const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
+  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({slots / std::max<int64_t>(1, tiles), slices / least, 64}));
   return p;
+}
+
+template <int BN>
+int launch_pair(const CUtensorMap &ta, const CUtensorMap &tb, const CUtensorMap &tsa, const CUtensorMap &tsb,
+                const CUtensorMap &tout, GemmParams g, int sms, cudaStream_t s) {
+  constexpr size_t stage = kTileM * kSlice + BN / 2 * kSlice + 2048, staging = 8 * 4096;
+  g.stages = (int)std::min<size_t>(kMaxStages, (224 * 1024 - staging - 1024) / stage);
+  const size_t smem = g.stages * stage + staging + 1024;
+  static size_t seen[kMaxDevices] = {};
+  if (int st = smem_optin(fp8_pair_kernel<BN>, smem, seen)) return st;
+  const int64_t units = (int64_t)g.tiles_m * g.tiles_n * g.splits;
+  const unsigned grid = 2u * (unsigned)std::min<int64_t>(units, sms / 2);
+  fp8_pair_kernel<BN><<<grid, kPairThreads, smem, s>>>(ta, tb, tsa, tsb, tout, g);
+  P3D_LAUNCH_CHECK();
+  return P3D_OK;
 }
 
 template <int BN, bool SWAP>
@@ -424,7 +756,7 @@ extern "C" int p3d_fp8_matmul(const void *a, int64_t a_pitch, const void *a_scal
   }
   {
     const uint64_t dims[2] = {(uint64_t)k, (uint64_t)p.cols}, strides[1] = {(uint64_t)narrow_pitch};
-    const uint32_t box[2] = {kSlice, (uint32_t)p.bn};
+    const uint32_t box[2] = {kSlice, (uint32_t)(p.pair ? p.bn / 2 : p.bn)};
     if (int st = encode_tiled(&tb, CU_TENSOR_MAP_DATA_TYPE_UINT8, narrow, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B))
       return st;
   }
@@ -446,7 +778,30 @@ extern "C" int p3d_fp8_matmul(const void *a, int64_t a_pitch, const void *a_scal
   g.vector = (cols * dtype_size(g.out_type)) % 16 == 0 && ((uintptr_t)g.out & 15) == 0;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   int st;
-  if (!p.swap) st = launch_gemm<128, false>(ta, tb, g, info.sm_count, s);
+  if (p.pair) {
+    CUtensorMap tout = {};
+    if (g.vector) {
+      const int size = dtype_size(g.out_type);
+      const uint64_t dims[3] = {(uint64_t)cols, (uint64_t)rows, (uint64_t)p.splits};
+      const uint64_t strides[2] = {(uint64_t)(cols * size), (uint64_t)(rows * cols * size)};
+      const uint32_t box[3] = {(uint32_t)(128 / size), 32, 1};
+      const CUtensorMapDataType type = g.out_type == P3D_F32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                       : g.out_type == P3D_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                               : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+      if (int e = encode_tiled(&tout, type, g.out, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return e;
+    }
+    CUtensorMap ts[2];   // scale bytes, a row for each 512-byte chunk
+    for (int i = 0; i < 2; ++i) {
+      const uint64_t chunks = (uint64_t)p3d_fp8_scale_bytes(i ? cols : rows, k) / 512;
+      const uint64_t dims[2] = {128, chunks}, strides[1] = {512};
+      const uint32_t box[2] = {128, 1};
+      if (int e = encode_tiled(&ts[i], CU_TENSOR_MAP_DATA_TYPE_UINT32, i ? g.scales_b : g.scales_a, 2, dims, strides, box,
+                               CU_TENSOR_MAP_SWIZZLE_NONE))
+        return e;
+    }
+    st = p.bn == 256 ? launch_pair<256>(ta, tb, ts[0], ts[1], tout, g, info.sm_count, s)
+                     : launch_pair<128>(ta, tb, ts[0], ts[1], tout, g, info.sm_count, s);
+  } else if (!p.swap) st = launch_gemm<128, false>(ta, tb, g, info.sm_count, s);
   else if (p.bn == 16) st = launch_gemm<16, true>(ta, tb, g, info.sm_count, s);
   else if (p.bn == 32) st = launch_gemm<32, true>(ta, tb, g, info.sm_count, s);
   else st = launch_gemm<64, true>(ta, tb, g, info.sm_count, s);

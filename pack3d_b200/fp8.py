@@ -16,7 +16,6 @@ from torch.autograd.function import once_differentiable
 
 from . import _native
 from ._validation import check_cuda
-from .residual import _Guard
 
 BLOCK = 128
 
@@ -73,7 +72,7 @@ def _quantize(x, square=False, rows=True, transposed=False, sums=None):
     q = Fp8Matrix._empty(m, n, x.device) if rows else None
     qt = Fp8Matrix._empty(n, m, x.device) if transposed else None
     lib = _native.lib()
-    with _Guard(x.device):
+    with _native.on(x.device) as stream:
         ws = None
         if sums is not None:
             ws = torch.empty(max(16, lib.p3d_fp8_quantize_workspace(m, n)), dtype=torch.uint8, device=x.device)
@@ -82,8 +81,7 @@ def _quantize(x, square=False, rows=True, transposed=False, sums=None):
             q.values.data_ptr() if q else None, q.values.shape[1] if q else 0, q.scales.data_ptr() if q else None,
             qt.values.data_ptr() if qt else None, qt.values.shape[1] if qt else 0, qt.scales.data_ptr() if qt else None,
             None if sums is None else sums.data_ptr(), 0 if sums is None else _native.DTYPE_CODE[sums.dtype],
-            None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(),
-            _native.stream_of(x.device)), "p3d_fp8_quantize")
+            None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), stream), "p3d_fp8_quantize")
     return q, qt
 
 
@@ -103,14 +101,14 @@ def quantize_weight(weight):
 def _matmul(a, b, bias, dtype):
     out = torch.empty((a.rows, b.rows), dtype=dtype, device=a.device)
     lib = _native.lib()
-    with _Guard(a.device):
+    with _native.on(a.device) as stream:
         need = lib.p3d_fp8_matmul_workspace(a.rows, b.rows, a.cols)
         ws = torch.empty(need, dtype=torch.uint8, device=a.device) if need else None
         _native.check(lib.p3d_fp8_matmul(
             a.values.data_ptr(), a.values.shape[1], a.scales.data_ptr(), b.values.data_ptr(), b.values.shape[1],
             b.scales.data_ptr(), a.rows, b.rows, a.cols, None if bias is None else bias.data_ptr(),
             0 if bias is None else _native.DTYPE_CODE[bias.dtype], out.data_ptr(), _native.DTYPE_CODE[dtype],
-            None if ws is None else ws.data_ptr(), need, _native.stream_of(a.device)), "p3d_fp8_matmul")
+            None if ws is None else ws.data_ptr(), need, stream), "p3d_fp8_matmul")
     return out
 
 
@@ -134,30 +132,64 @@ def fp8_matmul(a, b, *, bias=None, dtype=torch.bfloat16):
     return _matmul(a, b, _check_bias(bias, b.rows, a.device), dtype)
 
 
+def _pack(x, weight, bias, need_dx, need_dw):
+    """``p3d_fp8_linear`` of a call: x [rows, k], the weight a tensor or an :class:`Fp8Matrix`."""
+    code = _native.DTYPE_CODE
+    bias_code = 0 if bias is None else code[bias.dtype]
+    if isinstance(weight, Fp8Matrix):
+        return _native.FP8_LINEAR.pack(*x.shape, weight.rows, 0, weight.values.data_ptr(), weight.scales.data_ptr(),
+                                       weight.values.shape[1], code[x.dtype], 0, bias_code, 0, 0)
+    return _native.FP8_LINEAR.pack(*x.shape, weight.shape[0], weight.data_ptr(), 0, 0, 0, code[x.dtype],
+                                   code[weight.dtype], bias_code, need_dx, need_dw)
+
+
+def _forward(packed, x, bias, n, keep):
+    """``(y, what the backward needs or None)``."""
+    lib = _native.lib()
+    y = x.new_empty((x.shape[0], n))
+    with _native.on(x.device) as stream:
+        saved = x.new_empty(lib.p3d_fp8_linear_saved(packed), dtype=torch.uint8) if keep else None
+        need = lib.p3d_fp8_linear_fwd_workspace(packed)
+        ws = x.new_empty(need, dtype=torch.uint8)
+        status = lib.p3d_fp8_linear_fwd(packed, x.data_ptr(), None if bias is None else bias.data_ptr(), y.data_ptr(),
+                                        None if saved is None else saved.data_ptr(), ws.data_ptr(), need, stream)
+    if status:
+        _native.check(status, "p3d_fp8_linear_fwd")
+    return y, saved
+
+
 class _Fp8Linear(torch.autograd.Function):
     """Forward keeps x and the weight in 8 bits only: x with blocks along its rows for dW, the weight transposed for
     dx (its 128 x 128 blocks serve both directions)."""
 
     @staticmethod
     def forward(ctx, x, weight, bias):
-        need_x, need_w = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
-        xq, xt = _quantize(x, transposed=need_w)
-        wq, wt = _quantize(weight, square=True, transposed=need_x)
-        ctx.meta = (x.shape, weight.shape, x.dtype, weight.dtype, None if bias is None else bias.dtype)
-        ctx.save_for_backward(*(t for q in (xt, wt) for t in ((None, None) if q is None else (q.values, q.scales))))
-        return _matmul(xq, wq, bias, x.dtype)
+        need_x, need_w, _ = ctx.needs_input_grad
+        packed = _pack(x, weight, bias, need_x, need_w)
+        y, saved = _forward(packed, x, bias, weight.shape[0], need_x or need_w)
+        ctx.save_for_backward(saved)
+        ctx.meta = (packed, x.shape, weight.shape, weight.dtype, None if bias is None else bias.dtype)
+        return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        (m, k), (n, _), x_type, w_type, b_type = ctx.meta
+        packed, x_shape, w_shape, w_type, b_type = ctx.meta
         need_x, need_w, need_b = ctx.needs_input_grad
-        xtv, xts, wtv, wts = ctx.saved_tensors
+        saved, = ctx.saved_tensors
         dy = dy.contiguous()
-        db = torch.empty(n, dtype=b_type, device=dy.device) if need_b else None
-        dyq, dyt = _quantize(dy, rows=need_x, transposed=need_w, sums=db)
-        dx = _matmul(dyq, Fp8Matrix(wtv, wts, k, n), None, x_type) if need_x else None
-        dw = _matmul(dyt, Fp8Matrix(xtv, xts, k, m), None, w_type) if need_w else None
+        dx = dy.new_empty(x_shape) if need_x else None
+        dw = dy.new_empty(w_shape, dtype=w_type) if need_w else None
+        db = dy.new_empty(w_shape[0], dtype=b_type) if need_b else None
+        lib = _native.lib()
+        with _native.on(dy.device) as stream:
+            need = lib.p3d_fp8_linear_bwd_workspace(packed)
+            ws = dy.new_empty(need, dtype=torch.uint8)
+            status = lib.p3d_fp8_linear_bwd(packed, dy.data_ptr(), None if saved is None else saved.data_ptr(),
+                                            *(None if t is None else t.data_ptr() for t in (dx, dw, db)), ws.data_ptr(),
+                                            need, stream)
+        if status:
+            _native.check(status, "p3d_fp8_linear_bwd")
         return dx, dw, db
 
 
@@ -180,10 +212,13 @@ def fp8_linear(x, weight, bias=None):
     if weight.device != x.device:
         raise ValueError("x and weight must be on the same device")
     bias = _check_bias(bias, shape[0], x.device)
-    rows = x.reshape(-1, shape[1]).contiguous()
+    rows = x if x.ndim == 2 else x.reshape(-1, shape[1])
+    rows = rows.contiguous()
     grad = torch.is_grad_enabled()
+    wanted = grad and (x.requires_grad or bias is not None and bias.requires_grad or
+                       not kept and weight.requires_grad)
     if kept:
-        if grad and (x.requires_grad or bias is not None and bias.requires_grad):
+        if wanted:
             raise ValueError("an 8-bit weight has no gradients: pass the weight itself, or call under torch.no_grad()")
     elif weight.dtype not in _native.DTYPE_CODE:
         raise ValueError("weight must be fp32, fp16 or bf16")
@@ -191,15 +226,13 @@ def fp8_linear(x, weight, bias=None):
         weight = weight.contiguous()
     if rows.shape[0] == 0:
         y = x.new_empty(0, shape[0])
-        if not kept and grad:   # zero gradients for the weight and bias, as of an empty sum
+        if wanted:   # zero gradients for the weight and bias, as of an empty sum
             y = rows @ weight.t().to(x.dtype) + (0 if bias is None else bias.to(x.dtype))
-    elif kept:
-        y = _matmul(_quantize(rows.detach())[0], weight, bias, x.dtype)
-    elif grad and (x.requires_grad or weight.requires_grad or bias is not None and bias.requires_grad):
+    elif wanted:
         y = _Fp8Linear.apply(rows, weight, bias)
     else:
-        y = _matmul(_quantize(rows)[0], _quantize(weight, square=True)[0], bias, x.dtype)
-    return y.view(*x.shape[:-1], shape[0])
+        y, _ = _forward(_pack(rows, weight, bias, False, False), rows, bias, shape[0], False)
+    return y if x.ndim == 2 else y.view(*x.shape[:-1], shape[0])
 
 
 __all__ = ["BLOCK", "Fp8Matrix", "fp8_linear", "fp8_matmul", "quantize", "quantize_weight"]

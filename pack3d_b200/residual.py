@@ -52,8 +52,8 @@ def _check_spec(spec, x, what):
         raise ValueError(f"{what}: kind must be 'rms' or 'layer'")
     if not (math.isfinite(spec.eps) and spec.eps >= 0):
         raise ValueError(f"{what}: eps must be finite and not negative")
-    for t in (spec.weight, spec.bias):
-        _check_vector(t, x, what)
+    _check_vector(spec.weight, x, what)
+    _check_vector(spec.bias, x, what)
 
 
 def _check_vector(t, x, what):
@@ -88,22 +88,6 @@ def _rng(rng, device):
     return None, seed & 0xFFFFFFFFFFFFFFFF, offset & 0xFFFFFFFFFFFFFFFF
 
 
-class _Guard:
-    """``with torch.cuda.device(d)`` where ``d`` is not the current device already."""
-    __slots__ = ("inner",)
-
-    def __init__(self, device):
-        self.inner = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
-
-    def __enter__(self):
-        if self.inner is not None:
-            self.inner.__enter__()
-
-    def __exit__(self, *exc):
-        if self.inner is not None:
-            self.inner.__exit__(*exc)
-
-
 def _address(t):
     return 0 if t is None else t.data_ptr()
 
@@ -114,10 +98,11 @@ def _run_dropout(x, threshold, rng, seed, offset):
     y = torch.empty_like(x)
     dim = x.shape[-1] if x.ndim else 1
     rows = x.numel() // dim if dim else 0
-    with _Guard(x.device):
-        _native.check(_native.lib().p3d_dropout(x.data_ptr(), y.data_ptr(), _native.DTYPE_CODE[x.dtype], rows, dim,
-                                                threshold, _address(rng) or None, seed, offset,
-                                                _native.stream_of(x.device)), "p3d_dropout")
+    with _native.on(x.device) as stream:
+        status = _native.lib().p3d_dropout(x.data_ptr(), y.data_ptr(), _native.DTYPE_CODE[x.dtype], rows, dim, threshold,
+                                           _address(rng) or None, seed, offset, stream)
+    if status:
+        _native.check(status, "p3d_dropout")
     return y
 
 
@@ -185,13 +170,14 @@ def _run_forward(plan, tensors, save):
     x, h = tensors[0], tensors[1]
     out = None if h is None else torch.empty_like(x)
     y = torch.empty_like(x) if plan.next else None
-    stats = torch.empty((x.numel() // x.shape[-1], 4), dtype=torch.float32, device=x.device) if save else None
+    stats = x.new_empty((x.numel() // x.shape[-1], 4), dtype=torch.float32) if save else None
     if x.numel() == 0:
         return out, y, stats
-    with _Guard(x.device):
-        _native.check(_native.lib().p3d_residual_fwd(_pack(plan, *tensors), _address(out), _address(y),
-                                                     _address(stats), _native.stream_of(x.device)),
-                      "p3d_residual_fwd")
+    with _native.on(x.device) as stream:
+        status = _native.lib().p3d_residual_fwd(_pack(plan, *tensors), _address(out), _address(y), _address(stats),
+                                                stream)
+    if status:
+        _native.check(status, "p3d_residual_fwd")
     return out, y, stats
 
 
@@ -221,34 +207,42 @@ class _Residual(torch.autograd.Function):
         grads = [torch.empty_like(t) if n else None for t, n in zip(tensors, need)]
         packed = _pack(plan, *tensors, rng)
         lib = _native.lib()
-        with _Guard(x.device):
-            ws = torch.empty(max(16, lib.p3d_residual_bwd_workspace(packed)), dtype=torch.uint8, device=x.device)
-            dx, dh, dgate, dpw, dpb, dscale, dnw, dnb = (_address(g) for g in grads)
-            _native.check(lib.p3d_residual_bwd(packed, _address(dout), _address(dy), stats.data_ptr(), dx, dh, dgate,
-                                               dscale, dpw, dpb, dnw, dnb, ws.data_ptr(), ws.numel(),
-                                               _native.stream_of(x.device)), "p3d_residual_bwd")
+        with _native.on(x.device) as stream:
+            need = lib.p3d_residual_bwd_workspace(packed)
+            ws = stats.new_empty(need // 4)
+            dx, dh, dgate, dpw, dpb, dscale, dnw, dnb = map(_address, grads)
+            status = lib.p3d_residual_bwd(packed, _address(dout), _address(dy), stats.data_ptr(), dx, dh, dgate, dscale,
+                                          dpw, dpb, dnw, dnb, ws.data_ptr(), need, stream)
+        if status:
+            _native.check(status, "p3d_residual_bwd")
         return None, None, *grads
 
 
 def _call(plan, rng, tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        return _Residual.apply(plan, rng, *tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return _Residual.apply(plan, rng, *tensors)
     return _run_forward(plan, (*tensors, rng), False)[:2]
 
 
-def _same_params(x, *params):
+def _same_params(*params):
     """The parameters contiguous and of one dtype: where they differ, all in fp32."""
-    dtypes = {t.dtype for t in params if t is not None}
-    if len(dtypes) > 1:
-        params = [None if t is None else t.float() for t in params]
-    return [None if t is None else t.contiguous() for t in params]
+    dtype = None
+    for t in params:
+        if t is not None:
+            if dtype is not None and t.dtype != dtype:
+                params = [None if t is None else t.float() for t in params]
+                break
+            dtype = t.dtype
+    return [t if t is None or t.is_contiguous() else t.contiguous() for t in params]
 
 
 def norm(x, spec):
     """``spec`` (:class:`NormSpec`) of ``x`` over its last dimension, differentiable in ``x``, weight and bias."""
     _check_input(x, "norm")
     _check_spec(spec, x, "norm")
-    w, b = _same_params(x, spec.weight, spec.bias)
+    w, b = _same_params(spec.weight, spec.bias)
     plan = _Plan(0, 0.0, _KINDS[spec.kind], float(spec.eps), 0, 0, 0, 1.0, 0, 0, 0)
     return _call(plan, None, (x.contiguous(), None, None, None, None, None, w, b))[1]
 
@@ -311,7 +305,7 @@ def residual_norm(x, h, *, post_norm=None, gate=None, gate_activation="identity"
         mode, per_sample, gate = _gate_mode(gate, x)
     threshold = _threshold(p)
     tensor, seed, offset = _rng(rng, x.device) if threshold else (None, 0, 0)
-    pw, pb, scale, nw, nb = _same_params(x, post.weight, post.bias, scale, nxt.weight, nxt.bias)
+    pw, pb, scale, nw, nb = _same_params(post.weight, post.bias, scale, nxt.weight, nxt.bias)
     plan = _Plan(_KINDS[post.kind] if post_norm is not None else 0, float(post.eps),
                  _KINDS[nxt.kind] if next_norm is not None else 0, float(nxt.eps), mode,
                  _ACTIVATIONS[gate_activation], per_sample, value, threshold, seed, offset)
