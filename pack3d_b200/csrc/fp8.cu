@@ -14,6 +14,7 @@
 
 #include "common.cuh"
 #include "kernels.cuh"
+#include "sm100.cuh"
 
 namespace p3d {
 namespace {
@@ -23,6 +24,78 @@ constexpr int kBlock = 128;
 __device__ __forceinline__ uint32_t finite_bits(float v) {
   const uint32_t b = __float_as_uint(v) & 0x7fffffffu;
   return b < 0x7f800000u ? b : 0u;
+}
+
+// Magnitudes are compared as their bits.  Two 16-bit ones share a word; a word is `infinite` where either is
+// infinite or NaN, and then the block is gone over again with those left out.
+template <typename T> __device__ __forceinline__ bool infinite(uint32_t m) {
+  constexpr uint32_t top = std::is_same<T, __nv_bfloat16>::value ? 0x7f80u : 0x7c00u;
+  return (m & 0xffffu) >= top || (m >> 16) >= top;
+}
+template <> __device__ __forceinline__ bool infinite<float>(uint32_t m) { return m >= 0x7f800000u; }
+
+// The larger of two such words, half by half for 16-bit types.
+template <typename T> __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
+  if constexpr (sizeof(T) == 2) return __vmaxu2(a, b);
+  else return max(a, b);
+}
+// fp32 bits of the larger half.
+template <typename T> __device__ __forceinline__ uint32_t widest(uint32_t m) {
+  if constexpr (sizeof(T) == 4) return m;
+  const uint32_t h = max(m & 0xffffu, m >> 16);
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) return h << 16;
+  else return __float_as_uint(__half2float(__ushort_as_half((unsigned short)h)));
+}
+
+// Eight values of a row as they lie in memory.
+template <typename T> struct Raw {
+  static constexpr int kWords = 2 * sizeof(T);
+  uint32_t w[kWords];
+};
+
+template <typename T, bool ALIGNED>
+__device__ __forceinline__ Raw<T> load8(const T *row, int64_t col, int64_t cols) {
+  Raw<T> r;
+  if constexpr (ALIGNED) {
+    if (col < cols) {
+#pragma unroll
+      for (int i = 0; i < Raw<T>::kWords / 4; ++i) {
+        const uint4 v = reinterpret_cast<const uint4 *>(row + col)[i];
+        r.w[4 * i] = v.x;
+        r.w[4 * i + 1] = v.y;
+        r.w[4 * i + 2] = v.z;
+        r.w[4 * i + 3] = v.w;
+      }
+      return r;
+    }
+  }
+  alignas(16) T v[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = !ALIGNED && col + j < cols ? row[col + j] : from_f32<T>(0.f);
+  memcpy(r.w, v, sizeof(r.w));
+  return r;
+}
+template <typename T> __device__ __forceinline__ float value(const Raw<T> &r, int j) {
+  if constexpr (sizeof(T) == 4) return __uint_as_float(r.w[j]);
+  else {
+    const float2 f = unpack2<T>(r.w[j / 2]);
+    return j & 1 ? f.y : f.x;
+  }
+}
+template <typename T> __device__ __forceinline__ uint32_t magnitude(uint32_t word) {
+  return word & (sizeof(T) == 2 ? 0x7fff7fffu : 0x7fffffffu);
+}
+template <typename T> __device__ __forceinline__ uint32_t largest8(const Raw<T> &r) {
+  uint32_t m = magnitude<T>(r.w[0]);
+#pragma unroll
+  for (int i = 1; i < Raw<T>::kWords; ++i) m = larger<T>(m, magnitude<T>(r.w[i]));
+  return m;
+}
+template <typename T> __device__ __forceinline__ uint32_t finite_largest8(const Raw<T> &r) {   // in fp32 bits
+  uint32_t m = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) m = max(m, finite_bits(value(r, j)));
+  return m;
 }
 
 // e + 127 of a block whose largest finite magnitude has these bits: 448 = 1.75 * 2^8.
@@ -35,51 +108,34 @@ __device__ __forceinline__ uint32_t scale_byte(uint32_t amax_bits) {
 __device__ __forceinline__ float inverse_scale(uint32_t byte) { return __uint_as_float((254u - byte) << 23); }
 
 // Two values to e4m3 (lo in the low byte).  x * inv + (x - x): the second term is 0 for finite x and
-// NaN otherwise.
-__device__ __forceinline__ uint32_t to_e4m3x2(float lo, float hi, float inv) {
-  lo = fmaf(lo, inv, lo - lo);
-  hi = fmaf(hi, inv, hi - hi);
+// NaN otherwise; a block without infinities needs only the product.
+template <bool CHECK> __device__ __forceinline__ uint32_t to_e4m3x2(float2 v, float inv) {
+  if constexpr (CHECK) {
+    v.x = fmaf(v.x, inv, v.x - v.x);
+    v.y = fmaf(v.y, inv, v.y - v.y);
+  } else {
+    v = sm100::mul2(v, make_float2(inv, inv));
+  }
   uint16_t r;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(v.y), "f"(v.x));
   return r;
 }
-__device__ __forceinline__ uint32_t to_e4m3x4(float a, float b, float c, float d, float inv) {
-  return to_e4m3x2(a, b, inv) | to_e4m3x2(c, d, inv) << 16;
+template <bool CHECK> __device__ __forceinline__ uint32_t to_e4m3x4(float2 lo, float2 hi, float inv) {
+  return __byte_perm(to_e4m3x2<CHECK>(lo, inv), to_e4m3x2<CHECK>(hi, inv), 0x5410);
+}
+template <bool CHECK, typename T> __device__ __forceinline__ uint2 quantize8(const Raw<T> &r, float inv) {
+  float2 v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 2) v[i] = unpack2<T>(r.w[i]);
+    else v[i] = make_float2(__uint_as_float(r.w[2 * i]), __uint_as_float(r.w[2 * i + 1]));
+  }
+  return make_uint2(to_e4m3x4<CHECK>(v[0], v[1], inv), to_e4m3x4<CHECK>(v[2], v[3], inv));
 }
 
 // Where the scale byte of row `r`, block `b` lies; groups = ceil(blocks / 4).
 __device__ __forceinline__ int64_t scale_at(int64_t r, int64_t b, int64_t groups) {
   return ((r / 128) * groups + b / 4) * 512 + (r % 32) * 16 + (r % 128) / 32 * 4 + b % 4;
-}
-
-// Eight elements of a row from column `col` on, zero past its end.
-template <typename T, bool ALIGNED>
-__device__ __forceinline__ void load8(T (&v)[8], const T *row, int64_t col, int64_t cols) {
-  if constexpr (ALIGNED) {
-    if (col < cols) {
-      constexpr int n = sizeof(v) / 16;
-      uint4 raw[n];
-#pragma unroll
-      for (int i = 0; i < n; ++i) raw[i] = reinterpret_cast<const uint4 *>(row + col)[i];
-      memcpy(v, raw, sizeof(v));
-      return;
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = !ALIGNED && col + j < cols ? row[col + j] : from_f32<T>(0.f);
-}
-
-template <typename T>
-__device__ __forceinline__ uint32_t amax8(const T (&v)[8]) {
-  uint32_t m = 0;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) m = max(m, finite_bits(to_f32<T>(v[j])));
-  return m;
-}
-template <typename T>
-__device__ __forceinline__ uint2 quantize8(const T (&v)[8], float inv) {
-  return make_uint2(to_e4m3x4(to_f32<T>(v[0]), to_f32<T>(v[1]), to_f32<T>(v[2]), to_f32<T>(v[3]), inv),
-                    to_e4m3x4(to_f32<T>(v[4]), to_f32<T>(v[5]), to_f32<T>(v[6]), to_f32<T>(v[7]), inv));
 }
 
 struct QuantArgs {
@@ -92,22 +148,42 @@ struct QuantArgs {
   float *sums;             // [row tiles, cols] partial column sums
 };
 
-// 1 x 128 blocks along the rows: sixteen lanes a block, eight elements each.
-template <typename T, bool ALIGNED>
-__global__ void __launch_bounds__(256) quantize_rows_kernel(const QuantArgs a) {
-  const int64_t blocks = (a.cols + kBlock - 1) / kBlock, groups = (blocks + 3) / 4, total = a.rows * blocks;
-  const int sub = threadIdx.x & 15;
-  const int64_t step = (int64_t)gridDim.x * 16;
-  for (int64_t i0 = (int64_t)blockIdx.x * 16; i0 < total; i0 += step) {   // uniform: the shuffles take whole warps
-    const int64_t i = i0 + threadIdx.x / 16, row = i / blocks, b = i - row * blocks, col = b * kBlock + sub * 8;
-    T v[8];
-    load8<T, ALIGNED>(v, static_cast<const T *>(a.x) + row * a.cols, i < total ? col : a.cols, a.cols);
-    uint32_t m = amax8<T>(v);
+// The largest magnitude (fp32 bits, infinities left out) of a 128-element block that sixteen lanes hold; *odd
+// says whether it has infinities or NaN.
+template <typename T>
+__device__ __forceinline__ uint32_t block_amax(const Raw<T> &r, bool *odd) {
+  uint32_t m = largest8<T>(r);
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) m = larger<T>(m, __shfl_xor_sync(0xffffffffu, m, o));
+  *odd = __any_sync(0xffffffffu, infinite<T>(m));   // either half of the warp: both then check every value
+  if (*odd) {
+    m = finite_largest8<T>(r);
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const uint32_t byte = scale_byte(m);
-    if (i < total) {
-      if (col < a.pitch) *reinterpret_cast<uint2 *>(a.q + row * a.pitch + col) = quantize8<T>(v, inverse_scale(byte));
+    return m;
+  }
+  return widest<T>(m);
+}
+
+// 1 x 128 blocks along the rows: sixteen lanes a block, eight elements each; a CTA has sixteen rows and walks
+// their blocks from blockIdx.y on.
+template <typename T, bool ALIGNED>
+__global__ void __launch_bounds__(256) quantize_rows_kernel(const QuantArgs a) {
+  const int blocks = (int)((a.cols + kBlock - 1) / kBlock), groups = (blocks + 3) / 4;
+  const int sub = threadIdx.x & 15;
+  const int64_t row = (int64_t)blockIdx.x * 16 + threadIdx.x / 16;
+  const bool inside = row < a.rows;
+  const T *x = static_cast<const T *>(a.x) + row * a.cols;
+  uint8_t *q = a.q + row * a.pitch;
+#pragma unroll 2
+  for (int b = blockIdx.y; b < blocks; b += gridDim.y) {
+    const int64_t col = (int64_t)b * kBlock + sub * 8;
+    const Raw<T> r = load8<T, ALIGNED>(x, inside ? col : a.cols, a.cols);
+    bool odd;
+    const uint32_t byte = scale_byte(block_amax<T>(r, &odd));
+    if (inside) {
+      const float inv = inverse_scale(byte);
+      if (col < a.pitch) *reinterpret_cast<uint2 *>(q + col) = odd ? quantize8<true, T>(r, inv) : quantize8<false, T>(r, inv);
       if (sub == 0) a.scales[scale_at(row, b, groups)] = (uint8_t)byte;
     }
   }
@@ -117,7 +193,7 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const QuantArgs a) {
 // (SQUARE).  Transposed output: blocks of 128 rows of a column (or the same whole tile), from
 // the tile's copy in shared memory.  Column sums of the tile where asked for.
 template <typename T, bool ALIGNED, bool SQUARE>
-__global__ void __launch_bounds__(256) quantize_tile_kernel(const QuantArgs a) {
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 2) quantize_tile_kernel(const QuantArgs a) {
   constexpr int kPitch = kBlock + 16 / sizeof(T);   // 16 bytes past 128 values: rows start on other banks
   extern __shared__ __align__(16) unsigned char s_raw[];
   T *tile = reinterpret_cast<T *>(s_raw);
@@ -125,17 +201,36 @@ __global__ void __launch_bounds__(256) quantize_tile_kernel(const QuantArgs a) {
   __shared__ float s_sum[4][kBlock];
   const int64_t k0 = (int64_t)blockIdx.x * kBlock, m0 = (int64_t)blockIdx.y * kBlock;
   const int tid = threadIdx.x, sub = tid & 15, r0 = tid / 16;
-  const int64_t groups = ((a.cols + kBlock - 1) / kBlock + 3) / 4;
-  T v[8][8];
+  const int groups = (int)(((a.cols + kBlock - 1) / kBlock + 3) / 4);
+  const bool columns = a.qt || a.sums;
+  Raw<T> v[8];
   uint32_t all = 0;
+  bool odd = false;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int64_t row = m0 + r0 + 16 * i;
-    load8<T, ALIGNED>(v[i], static_cast<const T *>(a.x) + row * a.cols, row < a.rows ? k0 + sub * 8 : a.cols, a.cols);
-    if (a.qt || a.sums) memcpy(tile + (r0 + 16 * i) * kPitch + sub * 8, v[i], sizeof(v[i]));
-    if (SQUARE) all = max(all, amax8<T>(v[i]));
+    v[i] = load8<T, ALIGNED>(static_cast<const T *>(a.x) + row * a.cols, row < a.rows ? k0 + sub * 8 : a.cols, a.cols);
+  }
+  if (columns) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      uint4 *to = reinterpret_cast<uint4 *>(tile + (r0 + 16 * i) * kPitch + sub * 8);
+#pragma unroll
+      for (int j = 0; j < Raw<T>::kWords / 4; ++j)
+        to[j] = make_uint4(v[i].w[4 * j], v[i].w[4 * j + 1], v[i].w[4 * j + 2], v[i].w[4 * j + 3]);
+    }
   }
   if (SQUARE) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = larger<T>(m, largest8<T>(v[i]));
+    odd = __syncthreads_or(infinite<T>(m));
+    if (odd) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) all = max(all, finite_largest8<T>(v[i]));
+    } else {
+      all = widest<T>(m);
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) all = max(all, __shfl_xor_sync(0xffffffffu, all, o));
     if ((tid & 31) == 0) s_max[0][tid / 32] = all;
@@ -147,73 +242,110 @@ __global__ void __launch_bounds__(256) quantize_tile_kernel(const QuantArgs a) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       uint32_t m = all;
-      if (!SQUARE) {
-        m = amax8<T>(v[i]);
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-      }
+      if (!SQUARE) m = block_amax<T>(v[i], &odd);
       const uint32_t byte = scale_byte(m);
       const int64_t row = m0 + r0 + 16 * i, col = k0 + sub * 8;
       if (row < a.rows) {
-        if (col < a.pitch) *reinterpret_cast<uint2 *>(a.q + row * a.pitch + col) = quantize8<T>(v[i], inverse_scale(byte));
+        const float inv = inverse_scale(byte);
+        if (col < a.pitch)
+          *reinterpret_cast<uint2 *>(a.q + row * a.pitch + col) =
+              odd ? quantize8<true, T>(v[i], inv) : quantize8<false, T>(v[i], inv);
         if (sub == 0) a.scales[scale_at(row, blockIdx.x, groups)] = (uint8_t)byte;
       }
     }
   }
-  if (!a.qt && !a.sums) return;
+  if (!columns) return;
   __syncthreads();
-  // a pair of columns and a quarter of the rows a thread
+  // a pair of columns and a quarter of the rows a thread: x[r] is row r's pair
   const int c = (tid & 63) * 2, quarter = tid / 64;
-  float x[2][32];
-  uint32_t m[2] = {0u, 0u};
-  float s[2] = {0.f, 0.f};
+  const T *from = tile + quarter * 32 * kPitch + c;
+  constexpr int kPair = sizeof(T) / 2;   // words of a pair
+  uint32_t x[32 * kPair], m0w = 0, m1w = 0;   // 16 bits: both columns' magnitudes share m0w
+  float2 s = make_float2(0.f, 0.f);
 #pragma unroll
   for (int r = 0; r < 32; ++r) {
-    const T *at = tile + (quarter * 32 + r) * kPitch + c;
-    if constexpr (sizeof(T) == 2) {
-      const float2 f = unpack2<T>(*reinterpret_cast<const uint32_t *>(at));
-      x[0][r] = f.x;
-      x[1][r] = f.y;
+    if constexpr (kPair == 1) {
+      x[r] = *reinterpret_cast<const uint32_t *>(from + r * kPitch);
+      m0w = larger<T>(m0w, magnitude<T>(x[r]));
+      if (a.sums) s = sm100::add2(s, unpack2<T>(x[r]));
     } else {
-      const float2 f = *reinterpret_cast<const float2 *>(at);
-      x[0][r] = f.x;
-      x[1][r] = f.y;
-    }
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      m[h] = max(m[h], finite_bits(x[h][r]));
-      s[h] += x[h][r];
+      const uint2 w = *reinterpret_cast<const uint2 *>(from + r * kPitch);
+      x[2 * r] = w.x;
+      x[2 * r + 1] = w.y;
+      m0w = max(m0w, magnitude<T>(w.x));
+      m1w = max(m1w, magnitude<T>(w.y));
+      if (a.sums) s = sm100::add2(s, make_float2(__uint_as_float(w.x), __uint_as_float(w.y)));
     }
   }
+  auto pair = [&](int r) {
+    if constexpr (kPair == 1) return unpack2<T>(x[r]);
+    else return make_float2(__uint_as_float(x[2 * r]), __uint_as_float(x[2 * r + 1]));
+  };
+  // NaN or infinities anywhere in the tile: both columns' finite magnitudes one by one
+  if (!SQUARE) odd = infinite<T>(m0w) || (kPair == 2 && infinite<T>(m1w));
+  if (!SQUARE) odd = __syncthreads_or(odd);
+  if (!SQUARE) {
+    uint32_t lo, hi;
+    if (odd) {
+      lo = hi = 0;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    if (!SQUARE) s_max[quarter][c + h] = m[h];
-    s_sum[quarter][c + h] = s[h];
+      for (int r = 0; r < 32; ++r) {
+        const float2 f = pair(r);
+        lo = max(lo, finite_bits(f.x));
+        hi = max(hi, finite_bits(f.y));
+      }
+    } else if constexpr (kPair == 1) {
+      lo = widest<T>(m0w & 0xffffu);
+      hi = widest<T>(m0w >> 16);
+    } else {
+      lo = m0w;
+      hi = m1w;
+    }
+    s_max[quarter][c] = lo;
+    s_max[quarter][c + 1] = hi;
+  }
+  if (a.sums) {
+    s_sum[quarter][c] = s.x;
+    s_sum[quarter][c + 1] = s.y;
   }
   __syncthreads();
   if (a.sums && tid < kBlock && k0 + tid < a.cols)
     a.sums[(int64_t)blockIdx.y * a.cols + k0 + tid] = s_sum[0][tid] + s_sum[1][tid] + s_sum[2][tid] + s_sum[3][tid];
   if (!a.qt) return;
-  const int64_t t_groups = ((a.rows + kBlock - 1) / kBlock + 3) / 4;
+  const int t_groups = (int)(((a.rows + kBlock - 1) / kBlock + 3) / 4);
+  uint32_t byte[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    const int64_t col = k0 + c + h;
     if (!SQUARE) all = max(max(s_max[0][c + h], s_max[1][c + h]), max(s_max[2][c + h], s_max[3][c + h]));
-    const uint32_t byte = scale_byte(all);
-    const float inv = inverse_scale(byte);
-    if (col < a.cols) {
+    byte[h] = scale_byte(all);
+    if (quarter == 0 && k0 + c + h < a.cols) a.t_scales[scale_at(k0 + c + h, blockIdx.y, t_groups)] = (uint8_t)byte[h];
+  }
+  const float2 inv = make_float2(inverse_scale(byte[0]), inverse_scale(byte[1]));
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int64_t at = m0 + quarter * 32 + i * 16;
-        uint4 w;
-        w.x = to_e4m3x4(x[h][16 * i], x[h][16 * i + 1], x[h][16 * i + 2], x[h][16 * i + 3], inv);
-        w.y = to_e4m3x4(x[h][16 * i + 4], x[h][16 * i + 5], x[h][16 * i + 6], x[h][16 * i + 7], inv);
-        w.z = to_e4m3x4(x[h][16 * i + 8], x[h][16 * i + 9], x[h][16 * i + 10], x[h][16 * i + 11], inv);
-        w.w = to_e4m3x4(x[h][16 * i + 12], x[h][16 * i + 13], x[h][16 * i + 14], x[h][16 * i + 15], inv);
-        if (at < a.t_pitch) *reinterpret_cast<uint4 *>(a.qt + col * a.t_pitch + at) = w;
+  for (int i = 0; i < 2; ++i) {   // sixteen rows: sixteen bytes of either column
+    uint32_t w[2][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint32_t h[2][2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const float2 p = pair(16 * i + 4 * j + 2 * k), n = pair(16 * i + 4 * j + 2 * k + 1);
+        if (odd) {
+          h[0][k] = to_e4m3x2<true>(make_float2(p.x, n.x), inv.x);
+          h[1][k] = to_e4m3x2<true>(make_float2(p.y, n.y), inv.y);
+        } else {
+          h[0][k] = to_e4m3x2<false>(make_float2(p.x, n.x), inv.x);
+          h[1][k] = to_e4m3x2<false>(make_float2(p.y, n.y), inv.y);
+        }
       }
-      if (quarter == 0) a.t_scales[scale_at(col, blockIdx.y, t_groups)] = (uint8_t)byte;
+      w[0][j] = __byte_perm(h[0][0], h[0][1], 0x5410);
+      w[1][j] = __byte_perm(h[1][0], h[1][1], 0x5410);
     }
+    const int64_t at = m0 + quarter * 32 + i * 16;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      if (k0 + c + h < a.cols && at < a.t_pitch)
+        *reinterpret_cast<uint4 *>(a.qt + (k0 + c + h) * a.t_pitch + at) = make_uint4(w[h][0], w[h][1], w[h][2], w[h][3]);
   }
 }
 
@@ -232,8 +364,9 @@ template <typename T>
 int run_quantize(const QuantArgs &a, bool square, int sms, cudaStream_t s) {
   const bool aligned = a.cols % 8 == 0 && ((uintptr_t)a.x & 15) == 0;
   if (!square && !a.qt && !a.sums) {
-    const int64_t total = a.rows * ((a.cols + kBlock - 1) / kBlock);
-    const unsigned grid = (unsigned)std::min<int64_t>((total + 15) / 16, (int64_t)sms * 16);
+    // few rows: their blocks are dealt out to more CTAs
+    const int64_t across = (a.rows + 15) / 16, blocks = (a.cols + kBlock - 1) / kBlock;
+    const dim3 grid((unsigned)across, (unsigned)std::min<int64_t>(blocks, std::max<int64_t>(1, sms * 8 / across)));
     if (aligned) quantize_rows_kernel<T, true><<<grid, 256, 0, s>>>(a);
     else quantize_rows_kernel<T, false><<<grid, 256, 0, s>>>(a);
     P3D_LAUNCH_CHECK();

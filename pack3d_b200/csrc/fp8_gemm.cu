@@ -40,6 +40,20 @@ constexpr int kProducerWarp = 0, kMmaWarp = 1;
 constexpr uint64_t kWaitNs = 2000000000ull;
 constexpr int kMaxStages = 12;
 
+// mbar_wait that first sleeps on the barrier for up to 2 x 20 us without counting: reading the timer takes
+// longer than the wait for a ring's next stage should.
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, unsigned role) {
+  if (mbar_test_wait(bar, parity) || mbar_try_wait_sleep(bar, parity, 20000u) ||
+      mbar_try_wait_sleep(bar, parity, 20000u))
+    return true;
+  return mbar_wait(bar, parity, &g_fp8_errors, kWaitNs, role);
+}
+// The same by a converged warp, with an answer that the compiler knows to be uniform: what follows then
+// lives in uniform registers, which TMA and MMA instructions take their operands from.
+__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, unsigned role) {
+  return __all_sync(0xffffffffu, wait(bar, parity, role));
+}
+
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int c0, int c1) {
   asm volatile(
       "cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(
@@ -190,7 +204,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint8_t *sb = p.scales_b + (int64_t)(w.tn * BN / 128) * groups * 512;
         for (int kb = w.begin; kb < w.end; ++kb, ++it) {
           const int s = it % S;
-          if (it >= S && !mbar_wait(empty(s), (it / S - 1) & 1, &g_fp8_errors, kWaitNs, kErrProducer)) {
+          if (it >= S && !wait(empty(s), (it / S - 1) & 1, kErrProducer)) {
             ok = false;
             break;
           }
@@ -225,10 +239,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int u = blockIdx.x; ok && u < units; u += gridDim.x, ++n) {
         const Unit w = unit_of(p, u);
         const int a = n & 1;
-        if (n >= 2 && !mbar_wait(acc_empty(a), (n / 2 - 1) & 1, &g_fp8_errors, kWaitNs, kErrMma)) break;
+        if (n >= 2 && !wait(acc_empty(a), (n / 2 - 1) & 1, kErrMma)) break;
         for (int kb = w.begin; kb < w.end; ++kb, ++it) {
           const int s = it % S;
-          if (!mbar_wait(full(s), (it / S) & 1, &g_fp8_errors, kWaitNs, kErrMma)) {
+          if (!wait(full(s), (it / S) & 1, kErrMma)) {
             ok = false;
             break;
           }
@@ -268,7 +282,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int u = blockIdx.x; u < units; u += gridDim.x, ++n) {
       const Unit w = unit_of(p, u);
       const int a = n & 1;
-      const bool ready = mbar_wait(acc_full(a), (n / 2) & 1, &g_fp8_errors, kWaitNs, kErrSoftmax);
+      const bool ready = wait(acc_full(a), (n / 2) & 1, kErrSoftmax);
       if (!__all_sync(0xffffffffu, ready)) break;
       tc_fence_after();
       const int row = w.tm * kTileM + quarter * 32 + lane;
@@ -323,8 +337,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // ------------------------------------------------------------------------ the pair kernel
-constexpr int kPairThreads = 320;      // producer, MMA issuer, eight epilogue warps
 constexpr int kPairRows = 256;
+constexpr int kWarpCols = 64;          // columns of an epilogue warp
+constexpr int epilogue_warps(int bn) { return 4 * bn / kWarpCols; }
 
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
@@ -342,17 +357,26 @@ __device__ __forceinline__ uint32_t in_cta(uint32_t smem, uint32_t rank) {
 __device__ __forceinline__ void arrive_at(uint32_t cluster_bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
 }
-// A wait on arrivals of the other CTA too: ordered over the cluster once the phase is done.
+// A warp's wait on arrivals of the other CTA too (acquired over the cluster).
 __device__ __forceinline__ bool wait_cluster(uint32_t bar, uint32_t parity, unsigned role) {
-  const bool ok = mbar_wait(bar, parity, &g_fp8_errors, kWaitNs, role);
-  asm volatile("fence.acq_rel.cluster;" ::: "memory");
-  return ok;
+  const bool ok = wait(bar, parity, role);
+  uint32_t done;   // the phase is over: this only orders
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return __all_sync(0xffffffffu, ok && done);
 }
+// In what follows a converged warp calls with uniform operands and one elected lane, always the same, issues.
 // Into this CTA's shared memory, signalling a barrier of the pair's first CTA.
 __device__ __forceinline__ void pair_load_2d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int c0, int c1) {
   asm volatile(
-      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, "
-      "%4}], [%2];" ::"r"(dst),
+      "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+      "@e cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, "
+      "%4}], [%2];\n\t}" ::"r"(dst),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1)
       : "memory");
 }
@@ -365,29 +389,44 @@ __device__ __forceinline__ void store_3d(const CUtensorMap *map, uint32_t src, i
 __device__ __forceinline__ void pair_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb,
                                          uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred e, p;\n\telect.sync _|e, 0xffffffff;\n\t"
       "setp.ne.b32 p, %6, 0;\n\t"
-      "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+      "@e tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
       "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
       : "memory");
 }
 __device__ __forceinline__ void pair_copy_scales(uint32_t tmem, uint64_t desc) {
-  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+  asm volatile(
+      "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+      "@e tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;\n\t}" ::"r"(tmem),
+      "l"(desc)
+      : "memory");
 }
 // Arrives at the same barrier of both CTAs once all MMAs and copies issued so far are done.
 __device__ __forceinline__ void pair_commit(uint32_t bar) {
   asm volatile(
-      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+      "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+      "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}" ::"r"(bar),
       "h"((uint16_t)3)
       : "memory");
 }
 
-// 16-byte pieces of a thread's 128-byte row segment, as the 128-byte swizzle lays them out, from fp32 values.
+__device__ __forceinline__ void expect_tx_warp(uint32_t bar, uint32_t bytes) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+      "@e mbarrier.arrive.expect_tx.release.cta.shared::cta.b64 _, [%0], %1;\n\t}" ::"r"(bar),
+      "r"(bytes)
+      : "memory");
+}
+
+constexpr int kStageRow = 64;   // bytes of a row that the epilogue stages at a time (what leaves room for five stages)
+
+// 16-byte pieces of a thread's row segment, as the 64-byte swizzle lays them out, from fp32 values.
 template <typename T>
 __device__ __forceinline__ void stage_row(char *row_base, int row, const float *v) {
   constexpr int n = 16 / sizeof(T);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < kStageRow / 16; ++i) {
     uint4 w;
     if constexpr (sizeof(T) == 4) {
       w = make_uint4(__float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]), __float_as_uint(v[4 * i + 2]),
@@ -401,21 +440,23 @@ __device__ __forceinline__ void stage_row(char *row_base, int row, const float *
       }
       w = make_uint4(h[0], h[1], h[2], h[3]);
     }
-    *reinterpret_cast<uint4 *>(row_base + ((i ^ (row & 7)) * 16)) = w;
+    *reinterpret_cast<uint4 *>(row_base + ((i ^ (row >> 1 & 3)) * 16)) = w;
   }
 }
 
-template <typename T, int BN>
-__device__ __forceinline__ void pair_epilogue(const CUtensorMap *tout, const GemmParams &p, const Unit &w, float (&v)[BN / 2],
-                                              int row0, int col0, int lane, char *stage) {
-  constexpr int kCols = 128 / sizeof(T);   // columns of a 128-byte segment
+// A warp's 32 rows x 64 columns, 64 bytes of every row at a time through shared memory.  Boxes end at out's own
+// rows and columns.
+template <typename T>
+__device__ __forceinline__ void pair_epilogue(const CUtensorMap *tout, const GemmParams &p, const Unit &w,
+                                              const float (&v)[kWarpCols], int row0, int col0, int lane, char *stage) {
+  constexpr int kCols = kStageRow / sizeof(T);
   if (p.vector) {
 #pragma unroll
-    for (int c = 0; c < BN / 2; c += kCols) {
+    for (int c = 0; c < kWarpCols; c += kCols) {
       if (col0 + c >= p.cols || row0 >= p.rows) break;   // the same in the whole warp
       if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
       __syncwarp();
-      stage_row<T>(stage + lane * 128, lane, v + c);
+      stage_row<T>(stage + lane * kStageRow, lane, v + c);
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
@@ -426,13 +467,13 @@ __device__ __forceinline__ void pair_epilogue(const CUtensorMap *tout, const Gem
   } else if (row0 + lane < p.rows) {
     T *dst = static_cast<T *>(p.out) + (int64_t)(row0 + lane) * p.pitch + col0 + (int64_t)w.split * p.split_stride;
 #pragma unroll
-    for (int j = 0; j < BN / 2; ++j)
+    for (int j = 0; j < kWarpCols; ++j)
       if (col0 + j < p.cols) dst[j] = from_f32<T>(v[j]);
   }
 }
 
 template <int BN>
-__global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
+__global__ void __launch_bounds__(64 + 32 * epilogue_warps(BN), 1) __cluster_dims__(2, 1, 1)
     fp8_pair_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb,
                     const __grid_constant__ CUtensorMap tsa, const __grid_constant__ CUtensorMap tsb,
                     const __grid_constant__ CUtensorMap tout, const GemmParams p) {
@@ -445,8 +486,9 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   __shared__ __align__(8) uint64_t s_bars[2 * kMaxStages + 5];
   __shared__ uint32_t tmem_holder;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = cluster_rank();
+  __shared__ __align__(16) float s_bias[epilogue_warps(BN)][kWarpCols];
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const uint32_t rank = __shfl_sync(0xffffffffu, cluster_rank(), 0);
   const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
   const uint32_t bars = smem_u32(s_bars);
   const int S = p.stages;
@@ -464,7 +506,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(acc_full(a), 1);
-      mbar_init(acc_empty(a), 16);
+      mbar_init(acc_empty(a), 2 * epilogue_warps(BN));
     }
     mbar_init(drain, 1);
     fence_mbar_init();
@@ -490,45 +532,46 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
 
   if (warp == kProducerWarp) {
     // ------------------------------------------------------------------ TMA producer, one in each CTA
-    if (lane == 0) {
-      const int groups = (p.slices + 3) / 4;
-      int it = 0, s = 0;
-      uint32_t turn = 1;   // parity of the empty phase to wait for
-      bool ok = true;
-      for (int u = pair; ok && u < units; u += pairs) {
-        const Unit w = unit_of(p, u);
-        const int m0 = 2 * w.tm + (int)rank;   // this CTA's 128 rows; past the end everything reads as zero
-        for (int kb = w.begin; kb < w.end; ++kb, ++it) {
-          if (it >= S && !mbar_wait(empty(s), turn, &g_fp8_errors, kWaitNs, kErrProducer)) {
-            ok = false;
-            break;
-          }
-          const uint32_t st = base + s * kStageBytes, bar = in_cta(full(s), 0);
-          const bool scales = kb == w.begin || kb % 4 == 0;
-          if (rank == 0) mbar_expect_tx(full(s), 2 * (kBytesA + kBytesB + (scales ? kBytesS : 0u)));
-          pair_load_2d(st, &ta, bar, kb * kSlice, m0 * 128);
-          pair_load_2d(st + kBytesA, &tb, bar, kb * kSlice, w.tn * BN + (int)rank * (BN / 2));
-          if (scales) {
-            const uint32_t at = st + kStageBytes - 2048u;
-            pair_load_2d(at, &tsa, bar, 0, m0 * groups + kb / 4);
-            for (int c = 0; c < kChunksB; ++c)
-              pair_load_2d(at + 512u * (1 + c), &tsb, bar, 0, (w.tn * kChunksB + c) * groups + kb / 4);
-          }
-          if (++s == S) {
-            s = 0;
-            turn ^= 1;
-          }
+    const int groups = (p.slices + 3) / 4;
+    const uint32_t full0 = in_cta(bars, 0);   // the first CTA's full barriers
+    int it = 0, s = 0;
+    uint32_t turn = 1;   // parity of the empty phase to wait for
+    bool ok = true;
+    for (int u = pair; ok && u < units; u += pairs) {
+      const Unit w = unit_of(p, u);
+      const int m0 = 2 * w.tm + (int)rank;   // this CTA's 128 rows; past the end everything reads as zero
+      const int rows_b = w.tn * BN + (int)rank * (BN / 2);
+      for (int kb = w.begin; kb < w.end; ++kb, ++it) {
+        if (it >= S && !wait_warp(empty(s), turn, kErrProducer)) {
+          ok = false;
+          break;
+        }
+        const uint32_t st = base + s * kStageBytes, bar = full0 + 8u * s;
+        const bool scales = kb == w.begin || kb % 4 == 0;
+        if (rank == 0) expect_tx_warp(full(s), 2 * (kBytesA + kBytesB + (scales ? kBytesS : 0u)));
+        pair_load_2d(st, &ta, bar, kb * kSlice, m0 * 128);
+        pair_load_2d(st + kBytesA, &tb, bar, kb * kSlice, rows_b);
+        if (scales) {
+          const uint32_t at = st + kStageBytes - 2048u;
+          pair_load_2d(at, &tsa, bar, 0, m0 * groups + kb / 4);
+#pragma unroll
+          for (int c = 0; c < kChunksB; ++c)
+            pair_load_2d(at + 512u * (1 + c), &tsb, bar, 0, (w.tn * kChunksB + c) * groups + kb / 4);
+        }
+        if (++s == S) {
+          s = 0;
+          turn ^= 1;
         }
       }
-      // every stage used: its products are done, so its copies are too
-      for (int i = it > S ? it - S : 0; i < it; ++i)
-        mbar_wait(empty(i % S), (i / S) & 1, &g_fp8_errors, kWaitNs, kErrTeardown);
     }
+    // every stage used: its products are done, so its copies are too
+    for (int i = it > S ? it - S : 0; i < it; ++i)
+      mbar_wait(empty(i % S), (i / S) & 1, &g_fp8_errors, kWaitNs, kErrTeardown);
   } else if (warp == kMmaWarp) {
     // ------------------------------------------------------------------ MMA issuer, of the first CTA for both
-    if (lane == 0 && rank == 0) {
+    if (rank == 0) {
       constexpr uint32_t idesc = idesc_scaled(kPairRows, BN);
-      const uint32_t scale_cols = tmem + kAccs * BN;
+      const uint32_t acc = __shfl_sync(0xffffffffu, tmem, 0), scale_cols = acc + kAccs * BN;
       const uint64_t desc_a = desc_sw128(base, 1024), desc_b = desc_sw128(base + kBytesA, 1024);
       const uint64_t desc_s = desc_scales(base + kStageBytes - 2048u);
       int n = 0, groups = 0, s = 0;
@@ -540,7 +583,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
         if (n >= kAccs && !wait_cluster(acc_empty(a), (n / kAccs - 1) & 1, kErrMma)) break;
         tc_fence_after();
         for (int kb = w.begin; kb < w.end; ++kb) {
-          if (!mbar_wait(full(s), turn, &g_fp8_errors, kWaitNs, kErrMma)) {
+          if (!wait_warp(full(s), turn, kErrMma)) {
             ok = false;
             break;
           }
@@ -557,7 +600,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
           const uint32_t id = idesc | scale_ids(kb % 4);
 #pragma unroll
           for (int k = 0; k < 4; ++k)   // 32 columns: 32 bytes along the 128-byte rows
-            pair_mma(tmem + a * BN, desc_a + off + 2 * k, desc_b + off + 2 * k, id, sc, sc + 4,
+            pair_mma(acc + a * BN, desc_a + off + 2 * k, desc_b + off + 2 * k, id, sc, sc + 4,
                      kb > w.begin || k > 0 ? 1u : 0u);
           pair_commit(empty(s));
           if (++s == S) {
@@ -573,40 +616,46 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
     }
   } else {
     // ------------------------------------------------------------------ epilogue
-    const int quarter = warp & 3, half = (warp - 2) >> 2;   // TMEM lanes and columns of this warp
-    const uint32_t from = tmem + ((uint32_t)(quarter * 32) << 16) + half * (BN / 2);
-    char *const stage = reinterpret_cast<char *>(smem_raw) + (base - raw) + S * kStageBytes + (warp - 2) * 4096;
+    const int quarter = warp & 3, part = (warp - 2) >> 2;   // TMEM lanes and columns of this warp
+    const uint32_t from = tmem + ((uint32_t)(quarter * 32) << 16) + part * kWarpCols;
+    char *const stage = reinterpret_cast<char *>(smem_raw) + (base - raw) + S * kStageBytes + (warp - 2) * 32 * kStageRow;
+    float *const bias = s_bias[warp - 2];
     int n = 0;
     for (int u = pair; u < units; u += pairs, ++n) {
       const Unit w = unit_of(p, u);
       const int a = n % kAccs;
-      const int row0 = w.tm * kPairRows + (int)rank * 128 + quarter * 32, col0 = w.tn * BN + half * (BN / 2);
-      float add[BN / 64];   // the bias of columns lane, lane + 32, ..
+      const int row0 = w.tm * kPairRows + (int)rank * 128 + quarter * 32, col0 = w.tn * BN + part * kWarpCols;
+      if (p.bias) {
 #pragma unroll
-      for (int i = 0; i < BN / 64; ++i) {
-        const int c = col0 + 32 * i + lane;
-        add[i] = p.bias && c < p.cols ? load_any(p.bias, p.bias_type, c) : 0.f;
+        for (int i = lane; i < kWarpCols; i += 32)
+          bias[i] = col0 + i < p.cols ? load_any(p.bias, p.bias_type, col0 + i) : 0.f;
       }
-      const bool ready = mbar_wait(acc_full(a), (n / kAccs) & 1, &g_fp8_errors, kWaitNs, kErrSoftmax);
+      const bool ready = wait(acc_full(a), (n / kAccs) & 1, kErrSoftmax);
       if (!__all_sync(0xffffffffu, ready)) break;
       tc_fence_after();
-      uint32_t r[BN / 2];
+      uint32_t r[kWarpCols];
 #pragma unroll
-      for (int c = 0; c < BN / 2; c += 32) tmem_ld32(from + a * BN + c, r + c);
+      for (int c = 0; c < kWarpCols; c += 32) tmem_ld32(from + a * BN + c, r + c);
       tmem_wait_ld();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) arrive_at(in_cta(acc_empty(a), 0));
-      float v[BN / 2];
+      float v[kWarpCols];
 #pragma unroll
-      for (int j = 0; j < BN / 2; ++j) v[j] = __uint_as_float(r[j]);
+      for (int j = 0; j < kWarpCols; ++j) v[j] = __uint_as_float(r[j]);
       if (p.bias) {
 #pragma unroll
-        for (int j = 0; j < BN / 2; ++j) v[j] += __shfl_sync(0xffffffffu, add[j / 32], j % 32);
+        for (int j = 0; j < kWarpCols; j += 4) {
+          const float4 b = *reinterpret_cast<const float4 *>(bias + j);
+          v[j] += b.x;
+          v[j + 1] += b.y;
+          v[j + 2] += b.z;
+          v[j + 3] += b.w;
+        }
       }
-      if (p.out_type == P3D_BF16) pair_epilogue<__nv_bfloat16, BN>(&tout, p, w, v, row0, col0, lane, stage);
-      else if (p.out_type == P3D_F16) pair_epilogue<__half, BN>(&tout, p, w, v, row0, col0, lane, stage);
-      else pair_epilogue<float, BN>(&tout, p, w, v, row0, col0, lane, stage);
+      if (p.out_type == P3D_BF16) pair_epilogue<__nv_bfloat16>(&tout, p, w, v, row0, col0, lane, stage);
+      else if (p.out_type == P3D_F16) pair_epilogue<__half>(&tout, p, w, v, row0, col0, lane, stage);
+      else pair_epilogue<float>(&tout, p, w, v, row0, col0, lane, stage);
       __syncwarp();
     }
     if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
@@ -673,14 +722,14 @@ Plan plan_of(int64_t rows, int64_t cols, int64_t k, int sms) {
 template <int BN>
 int launch_pair(const CUtensorMap &ta, const CUtensorMap &tb, const CUtensorMap &tsa, const CUtensorMap &tsb,
                 const CUtensorMap &tout, GemmParams g, int sms, cudaStream_t s) {
-  constexpr size_t stage = kTileM * kSlice + BN / 2 * kSlice + 2048, staging = 8 * 4096;
-  g.stages = (int)std::min<size_t>(kMaxStages, (224 * 1024 - staging - 1024) / stage);
+  constexpr size_t stage = kTileM * kSlice + BN / 2 * kSlice + 2048, staging = epilogue_warps(BN) * 32 * kStageRow;
+  g.stages = (int)std::min<size_t>(kMaxStages, (220 * 1024 - staging - 1024) / stage);
   const size_t smem = g.stages * stage + staging + 1024;
   static size_t seen[kMaxDevices] = {};
   if (int st = smem_optin(fp8_pair_kernel<BN>, smem, seen)) return st;
   const int64_t units = (int64_t)g.tiles_m * g.tiles_n * g.splits;
   const unsigned grid = 2u * (unsigned)std::min<int64_t>(units, sms / 2);
-  fp8_pair_kernel<BN><<<grid, kPairThreads, smem, s>>>(ta, tb, tsa, tsb, tout, g);
+  fp8_pair_kernel<BN><<<grid, 64 + 32 * epilogue_warps(BN), smem, s>>>(ta, tb, tsa, tsb, tout, g);
   P3D_LAUNCH_CHECK();
   return P3D_OK;
 }
@@ -784,11 +833,11 @@ extern "C" int p3d_fp8_matmul(const void *a, int64_t a_pitch, const void *a_scal
       const int size = dtype_size(g.out_type);
       const uint64_t dims[3] = {(uint64_t)cols, (uint64_t)rows, (uint64_t)p.splits};
       const uint64_t strides[2] = {(uint64_t)(cols * size), (uint64_t)(rows * cols * size)};
-      const uint32_t box[3] = {(uint32_t)(128 / size), 32, 1};
+      const uint32_t box[3] = {(uint32_t)(kStageRow / size), 32, 1};
       const CUtensorMapDataType type = g.out_type == P3D_F32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                        : g.out_type == P3D_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                                : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-      if (int e = encode_tiled(&tout, type, g.out, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return e;
+      if (int e = encode_tiled(&tout, type, g.out, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_64B)) return e;
     }
     CUtensorMap ts[2];   // scale bytes, a row for each 512-byte chunk
     for (int i = 0; i < 2; ++i) {
