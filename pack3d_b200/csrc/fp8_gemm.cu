@@ -93,7 +93,7 @@ __device__ __forceinline__ uint32_t scale_ids(int byte) { return (uint32_t)byte 
 
 struct GemmParams {
   int rows, cols;          // of the tile space: rows of the 128-lane operand, of the N operand
-  int slices;              // ceil(k / 128)
+  int slices, last_steps;  // ceil(k / 128); ceil(k / 32) of the last one
   int tiles_m, tiles_n, splits;
   const uint8_t *scales_a, *scales_b;   // of the 128-lane operand, of the N operand
   void *out;               // [rows, cols] (SWAP: [cols, rows]) of out_type, or the partials [splits][..] fp32
@@ -444,23 +444,27 @@ __device__ __forceinline__ void stage_row(char *row_base, int row, const float *
   }
 }
 
-// A warp's 32 rows x 64 columns, 64 bytes of every row at a time through shared memory.  Boxes end at out's own
-// rows and columns.
-template <typename T>
+// A warp's 32 rows x 64 columns through shared memory, BOXES times 64 bytes of every row at a time.  Boxes end at
+// out's own rows and columns.
+template <typename T, int BOXES>
 __device__ __forceinline__ void pair_epilogue(const CUtensorMap *tout, const GemmParams &p, const Unit &w,
                                               const float (&v)[kWarpCols], int row0, int col0, int lane, char *stage) {
-  constexpr int kCols = kStageRow / sizeof(T);
+  constexpr int kCols = kStageRow / sizeof(T), kBox = 32 * kStageRow;
   if (p.vector) {
 #pragma unroll
-    for (int c = 0; c < kWarpCols; c += kCols) {
+    for (int c = 0; c < kWarpCols; c += kCols * BOXES) {
       if (col0 + c >= p.cols || row0 >= p.rows) break;   // the same in the whole warp
       if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
       __syncwarp();
-      stage_row<T>(stage + lane * kStageRow, lane, v + c);
+#pragma unroll
+      for (int b = 0; b < BOXES; ++b) stage_row<T>(stage + b * kBox + lane * kStageRow, lane, v + c + b * kCols);
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
-        store_3d(tout, smem_u32(stage), col0 + c, row0, w.split);
+#pragma unroll
+        for (int b = 0; b < BOXES; ++b)
+          if (b == 0 || col0 + c + b * kCols < p.cols)
+            store_3d(tout, smem_u32(stage) + b * kBox, col0 + c + b * kCols, row0, w.split);
         asm volatile("cp.async.bulk.commit_group;" ::: "memory");
       }
     }
@@ -472,7 +476,7 @@ __device__ __forceinline__ void pair_epilogue(const CUtensorMap *tout, const Gem
   }
 }
 
-template <int BN>
+template <int BN, int BOXES>
 __global__ void __launch_bounds__(64 + 32 * epilogue_warps(BN), 1) __cluster_dims__(2, 1, 1)
     fp8_pair_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb,
                     const __grid_constant__ CUtensorMap tsa, const __grid_constant__ CUtensorMap tsb,
@@ -598,9 +602,11 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(BN), 1) __cluster_dim
           }
           const uint32_t sc = scale_cols + ((groups - 1) & 1) * kScaleCols;
           const uint32_t id = idesc | scale_ids(kb % 4);
+          // 32 columns: 32 bytes along the 128-byte rows; the last slice may have fewer than four
+          const int steps = kb + 1 < p.slices ? 4 : p.last_steps;
 #pragma unroll
-          for (int k = 0; k < 4; ++k)   // 32 columns: 32 bytes along the 128-byte rows
-            pair_mma(acc + a * BN, desc_a + off + 2 * k, desc_b + off + 2 * k, id, sc, sc + 4,
+          for (int k = 0; k < 4; ++k)
+            if (k < steps) pair_mma(acc + a * BN, desc_a + off + 2 * k, desc_b + off + 2 * k, id, sc, sc + 4,
                      kb > w.begin || k > 0 ? 1u : 0u);
           pair_commit(empty(s));
           if (++s == S) {
@@ -618,7 +624,7 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(BN), 1) __cluster_dim
     // ------------------------------------------------------------------ epilogue
     const int quarter = warp & 3, part = (warp - 2) >> 2;   // TMEM lanes and columns of this warp
     const uint32_t from = tmem + ((uint32_t)(quarter * 32) << 16) + part * kWarpCols;
-    char *const stage = reinterpret_cast<char *>(smem_raw) + (base - raw) + S * kStageBytes + (warp - 2) * 32 * kStageRow;
+    char *const stage = reinterpret_cast<char *>(smem_raw) + (base - raw) + S * kStageBytes + (warp - 2) * BOXES * 32 * kStageRow;
     float *const bias = s_bias[warp - 2];
     int n = 0;
     for (int u = pair; u < units; u += pairs, ++n) {
@@ -653,9 +659,9 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(BN), 1) __cluster_dim
           v[j + 3] += b.w;
         }
       }
-      if (p.out_type == P3D_BF16) pair_epilogue<__nv_bfloat16>(&tout, p, w, v, row0, col0, lane, stage);
-      else if (p.out_type == P3D_F16) pair_epilogue<__half>(&tout, p, w, v, row0, col0, lane, stage);
-      else pair_epilogue<float>(&tout, p, w, v, row0, col0, lane, stage);
+      if (p.out_type == P3D_BF16) pair_epilogue<__nv_bfloat16, BOXES>(&tout, p, w, v, row0, col0, lane, stage);
+      else if (p.out_type == P3D_F16) pair_epilogue<__half, BOXES>(&tout, p, w, v, row0, col0, lane, stage);
+      else pair_epilogue<float, BOXES>(&tout, p, w, v, row0, col0, lane, stage);
       __syncwarp();
     }
     if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
@@ -719,17 +725,17 @@ Plan plan_of(int64_t rows, int64_t cols, int64_t k, int sms) {
   return p;
 }
 
-template <int BN>
+template <int BN, int BOXES>
 int launch_pair(const CUtensorMap &ta, const CUtensorMap &tb, const CUtensorMap &tsa, const CUtensorMap &tsb,
                 const CUtensorMap &tout, GemmParams g, int sms, cudaStream_t s) {
-  constexpr size_t stage = kTileM * kSlice + BN / 2 * kSlice + 2048, staging = epilogue_warps(BN) * 32 * kStageRow;
+  constexpr size_t stage = kTileM * kSlice + BN / 2 * kSlice + 2048, staging = epilogue_warps(BN) * BOXES * 32 * kStageRow;
   g.stages = (int)std::min<size_t>(kMaxStages, (220 * 1024 - staging - 1024) / stage);
   const size_t smem = g.stages * stage + staging + 1024;
   static size_t seen[kMaxDevices] = {};
-  if (int st = smem_optin(fp8_pair_kernel<BN>, smem, seen)) return st;
+  if (int st = smem_optin(fp8_pair_kernel<BN, BOXES>, smem, seen)) return st;
   const int64_t units = (int64_t)g.tiles_m * g.tiles_n * g.splits;
   const unsigned grid = 2u * (unsigned)std::min<int64_t>(units, sms / 2);
-  fp8_pair_kernel<BN><<<grid, 64 + 32 * epilogue_warps(BN), smem, s>>>(ta, tb, tsa, tsb, tout, g);
+  fp8_pair_kernel<BN, BOXES><<<grid, 64 + 32 * epilogue_warps(BN), smem, s>>>(ta, tb, tsa, tsb, tout, g);
   P3D_LAUNCH_CHECK();
   return P3D_OK;
 }
@@ -813,6 +819,7 @@ extern "C" int p3d_fp8_matmul(const void *a, int64_t a_pitch, const void *a_scal
   g.rows = (int)p.rows;
   g.cols = (int)p.cols;
   g.slices = (int)((k + kSlice - 1) / kSlice);
+  g.last_steps = (int)((k - (int64_t)(g.slices - 1) * kSlice + 31) / 32);
   g.tiles_m = p.tiles_m;
   g.tiles_n = p.tiles_n;
   g.splits = p.splits;
@@ -848,8 +855,10 @@ extern "C" int p3d_fp8_matmul(const void *a, int64_t a_pitch, const void *a_scal
                                CU_TENSOR_MAP_SWIZZLE_NONE))
         return e;
     }
-    st = p.bn == 256 ? launch_pair<256>(ta, tb, ts[0], ts[1], tout, g, info.sm_count, s)
-                     : launch_pair<128>(ta, tb, ts[0], ts[1], tout, g, info.sm_count, s);
+    // a short k makes the epilogue the longer part: it then stages whole 128-byte segments, which costs a stage
+    st = p.bn == 128   ? launch_pair<128, 2>(ta, tb, ts[0], ts[1], tout, g, info.sm_count, s)
+         : g.slices <= 8 ? launch_pair<256, 2>(ta, tb, ts[0], ts[1], tout, g, info.sm_count, s)
+                         : launch_pair<256, 1>(ta, tb, ts[0], ts[1], tout, g, info.sm_count, s);
   } else if (!p.swap) st = launch_gemm<128, false>(ta, tb, g, info.sm_count, s);
   else if (p.bn == 16) st = launch_gemm<16, true>(ta, tb, g, info.sm_count, s);
   else if (p.bn == 32) st = launch_gemm<32, true>(ta, tb, g, info.sm_count, s);
