@@ -314,9 +314,12 @@ extern "C" int p3d_dropout(const void *x, void *y, int dtype, int64_t rows, int6
 
 namespace {
 
-// Threads an SM's registers hold: 64 registers a thread in the forward's narrow form, else 128.
-constexpr int kNarrowThreads = 1024, kWideThreads = 512;
-int per_sm_of(const Shape &s, int threads) { return std::max(1, threads / (s.row_threads * s.groups)); }
+// CTAs that an SM's registers hold: 64 registers a thread in the forward's narrow form and in the backward of a norm
+// by itself, else 128.
+int per_sm_of(const p3d_residual &p, const Shape &s, bool backward) {
+  const int threads = (backward ? p.h == nullptr : s.units == 1) ? 1024 : 512;
+  return std::max(1, threads / (s.row_threads * s.groups));
+}
 
 }  // namespace
 
@@ -339,7 +342,7 @@ extern "C" int p3d_residual_fwd(const p3d_residual *args, void *out, void *y, fl
   a.stats = stats;
   const bool aligned = all_aligned(p, {out, y});
   const bool center = centred(p) || (aligned && !rows::whole_fwd(a));
-  int per_sm = per_sm_of(s, s.units == 1 ? kNarrowThreads : kWideThreads);
+  int per_sm = per_sm_of(p, s, false);
   const size_t smem = lay_out(a, s, aligned, center, false, &per_sm);
   const Split c = split_of(p, s, info.sm_count, per_sm, false);
   a.segments = (int)c.segments;
@@ -354,7 +357,7 @@ extern "C" size_t p3d_residual_bwd_workspace(const p3d_residual *args) {
   DeviceInfo info;
   if (check_args(args, "p3d_residual_bwd_workspace") || args->rows == 0 || device_info(&info)) return 0;
   const Shape s = shape_of(args->dim, args->dtype, true);
-  return partial_floats(*args, split_of(*args, s, info.sm_count, per_sm_of(s, kWideThreads), true)) * sizeof(float);
+  return partial_floats(*args, split_of(*args, s, info.sm_count, per_sm_of(*args, s, true), true)) * sizeof(float);
 }
 
 extern "C" int p3d_residual_bwd(const p3d_residual *args, const void *dout, const void *dy, const float *stats,
@@ -371,7 +374,7 @@ extern "C" int p3d_residual_bwd(const p3d_residual *args, const void *dout, cons
   DeviceInfo info;
   if (int st = device_info(&info)) return st;
   const Shape s = shape_of(p.dim, p.dtype, true);
-  int per_sm = per_sm_of(s, kWideThreads);
+  int per_sm = per_sm_of(p, s, true);
   const Split c = split_of(p, s, info.sm_count, per_sm, true);   // as the workspace was sized
   const size_t need = partial_floats(p, c) * sizeof(float);
   if (workspace_bytes < need || !workspace)

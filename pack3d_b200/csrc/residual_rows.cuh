@@ -104,14 +104,19 @@ struct Place {
 template <bool ALIGNED>
 __device__ __forceinline__ Place place_of(const Args &a) {
   Place q;
+  // group, warp and rank are the same in a whole warp; a shuffle tells the compiler, which then keeps what
+  // follows from them in uniform registers
   q.threads = a.row_threads;
-  q.group = threadIdx.x / a.row_threads;
+  q.group = __shfl_sync(0xffffffffu, (int)threadIdx.x / a.row_threads, 0);
   q.t = threadIdx.x - q.group * a.row_threads;
   q.warps = a.row_threads / 32;
-  q.warp = q.t / 32;
-  q.lane = q.t % 32;
+  q.warp = __shfl_sync(0xffffffffu, q.t / 32, 0);
+  q.lane = threadIdx.x % 32;
   q.rank = 0;
-  if (a.members > 1) asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(q.rank));
+  if (a.members > 1) {
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(q.rank));
+    q.rank = __shfl_sync(0xffffffffu, q.rank, 0);
+  }
   q.dim = a.p.dim;
   return q;
 }
@@ -199,7 +204,7 @@ __device__ __forceinline__ float total(const Place &q, const float2 (&v)[NU]) {
 }
 
 struct Exchange {
-  float slots[2][16][4];               // [2][warps of the CTA][values]
+  alignas(16) float slots[2][4][16];   // [2][values][warps of the CTA]
   float peers[2][kMaxCluster][4];      // [2][CTA of the cluster][values]
 };
 
@@ -232,21 +237,34 @@ struct RowSum {
   int members;
   int at = 0;
 
+  // Sum of a value over the row's warps, read by every thread (slots past the row's are not added).
+  __device__ __forceinline__ float over_warps(const Place &q, int value) const {
+    const float *from = x->slots[at][value] + q.group * q.warps;
+    float s = 0.f;
+    if (q.warps % 4 == 0) {   // groups then start on 16 bytes
+#pragma unroll 1
+      for (int w = 0; w < q.warps; w += 4) {
+        const float4 f = *reinterpret_cast<const float4 *>(from + w);
+        s += (f.x + f.y) + (f.z + f.w);
+      }
+    } else {
+#pragma unroll 1
+      for (int w = 0; w < q.warps; ++w) s += from[w];
+    }
+    return s;
+  }
+
   template <int N>
   __device__ __forceinline__ void operator()(const Place &q, float (&v)[N]) {
     warp_sums(q.lane, v);
     if (q.warps > 1) {
       if (q.lane == 0) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) x->slots[at][q.group * q.warps + q.warp][i] = v[i];
+        for (int i = 0; i < N; ++i) x->slots[at][i][q.group * q.warps + q.warp] = v[i];
       }
       q.barrier();
-      const float4 w = q.lane < q.warps ? *reinterpret_cast<const float4 *>(x->slots[at][q.group * q.warps + q.lane])
-                                        : make_float4(0.f, 0.f, 0.f, 0.f);
-      v[0] = w.x;
-      if constexpr (N > 1) v[1] = w.y;
-      if constexpr (N > 2) v[2] = w.z;
-      warp_sums(q.lane, v);
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = over_warps(q, i);
       if (members > 1) over_cluster(q, v);
       at ^= 1;
     }
@@ -287,17 +305,21 @@ struct RowSum {
     }
     float m2 = warp_sum(total<ALIGNED, NU>(q, d2));
     if (q.warps == 1) return make_float2(mean, m2);
-    if (q.lane == 0)
-      *reinterpret_cast<float4 *>(x->slots[at][q.group * q.warps + q.warp]) =
-          make_float4(count, count * mean, m2, mean);
+    if (q.lane == 0) {
+      const int w = q.group * q.warps + q.warp;
+      x->slots[at][0][w] = count;
+      x->slots[at][1][w] = mean;
+      x->slots[at][2][w] = m2;
+    }
     q.barrier();
-    const float4 w = q.lane < q.warps ? *reinterpret_cast<const float4 *>(x->slots[at][q.group * q.warps + q.lane])
-                                      : make_float4(0.f, 0.f, 0.f, 0.f);
-    float two[2] = {w.x, w.y};
+    const bool mine = q.lane < q.warps;
+    const int w = q.group * q.warps + q.lane;
+    const float n_w = mine ? x->slots[at][0][w] : 0.f, mean_w = mine ? x->slots[at][1][w] : 0.f;
+    float two[2] = {n_w, n_w * mean_w};
     warp_sums(q.lane, two);
     mean = two[0] > 0.f ? two[1] / two[0] : 0.f;   // a CTA of the cluster may have no columns
-    const float off = w.w - mean;
-    m2 = warp_sum(fmaf(w.x * off, off, w.z));
+    const float off = mean_w - mean;
+    m2 = warp_sum(fmaf(n_w * off, off, mine ? x->slots[at][2][w] : 0.f));
     if (members > 1) {
       float v[2] = {two[0], two[0] * mean};
       over_cluster(q, v);
@@ -391,56 +413,78 @@ struct Span {
   }
 };
 
-// Shared memory: exchange slots, keep bits, the rings' barriers and the state of what fills them; then,
-// dynamic, the parameters and each group's ring.
+// Shared memory: exchange slots, keep bits and the rings' barriers; then, dynamic, the parameters and each
+// group's ring.
 struct Shared {
   Exchange exchange;
   uint64_t bars[kMaxGroups * kMaxStages];
-  Batches ahead[kMaxGroups];
-  int fill_stage[kMaxGroups];
   uint8_t keep[kMaxRowThreads];
 };
 
+// Issued by one elected lane of a converged warp.
+__device__ __forceinline__ void elect_expect_tx(uint32_t bar, uint32_t bytes) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+      "@e mbarrier.arrive.expect_tx.release.cta.shared::cta.b64 _, [%0], %1;\n\t}" ::"r"(bar),
+      "r"(bytes)
+      : "memory");
+}
+__device__ __forceinline__ void elect_bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+      "@e cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n\t}" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(bar)
+      : "memory");
+}
+
 template <typename T, bool ALIGNED, int NU, bool STATS>
 struct Ring {
-  Shared *s;
-  char *data;               // the group's stages
+  uint32_t bars;             // the group's
+  char *data;                // the group's stages
   int stage = 0, phase = 0;  // of the next batch to use
+  int fill = 0;              // stage of the next batch to load
+  Batches ahead;             // which is that
 
-  __device__ __forceinline__ uint32_t bar(const Place &q, int st) const {
-    return sm100::smem_u32(s->bars + q.group * kMaxStages + st);
-  }
-  // Called by one thread of the group; its place ahead lives in shared memory, not in every thread's
-  // registers.
+  // Called by the group's first warp, all of it.
   __device__ __forceinline__ void issue(const Args &a, const Place &q) {
-    Batches k = s->ahead[q.group];
-    if (k.seg >= a.segments) return;
-    const int st = s->fill_stage[q.group], n = k.count(a), row = k.row(a);
-    s->fill_stage[q.group] = st + 1 == a.stages ? 0 : st + 1;
-    const uint32_t to = sm100::smem_u32(data + (uint32_t)st * a.stage_bytes), b = bar(q, st);
-    uint32_t bytes = STATS ? 16u * n : 0u;
-#pragma unroll 1
-    for (int i = 0; i < kArrays; ++i)
-      if (a.in[i]) {
-        const Span<T, ALIGNED, NU> span(a, q, i, row, n);
-        if (span.copied) bytes += span.bytes;
+    if (ahead.seg >= a.segments) return;
+    const int n = ahead.count(a), row = ahead.row(a);
+    const uint32_t to = sm100::smem_u32(data) + (uint32_t)fill * a.stage_bytes, b = bars + 8u * fill;
+    fill = fill + 1 == a.stages ? 0 : fill + 1;
+    if constexpr (ALIGNED) {
+      const int cols = max(0, min(q.threads * kUnit * NU, q.end));   // the last CTA of a row may have none
+      const uint32_t bytes = (uint32_t)(((n - 1) * q.dim + cols) * (int)sizeof(T));
+      const int64_t off = ((int64_t)row * q.dim + q.first) * (int64_t)sizeof(T);
+      elect_expect_tx(b, (STATS ? 16u * n : 0u) + (cols > 0 ? bytes * a.slot_count : 0u));
+      if (cols > 0) {
+#pragma unroll
+        for (int i = 0; i < kArrays; ++i)
+          if (a.in[i])
+            elect_bulk_load(to + (uint32_t)a.slots[i] * a.slot_bytes, static_cast<const char *>(a.in[i]) + off, bytes, b);
       }
-    sm100::mbar_expect_tx(b, bytes);
-    if (STATS)
-      sm100::bulk_load(to + (uint32_t)a.slot_count * a.slot_bytes, a.stats + 4 * (int64_t)row, 16u * n, b);
+    } else {
+      uint32_t bytes = STATS ? 16u * n : 0u;
 #pragma unroll 1
-    for (int i = 0; i < kArrays; ++i)
-      if (a.in[i]) {
-        const Span<T, ALIGNED, NU> span(a, q, i, row, n);
-        if (span.copied) sm100::bulk_load(to + (uint32_t)a.slots[i] * a.slot_bytes, span.from, span.bytes, b);
-      }
-    k.next(a, q.group);
-    s->ahead[q.group] = k;
+      for (int i = 0; i < kArrays; ++i)
+        if (a.in[i]) {
+          const Span<T, ALIGNED, NU> span(a, q, i, row, n);
+          if (span.copied) bytes += span.bytes;
+        }
+      elect_expect_tx(b, bytes);
+#pragma unroll 1
+      for (int i = 0; i < kArrays; ++i)
+        if (a.in[i]) {
+          const Span<T, ALIGNED, NU> span(a, q, i, row, n);
+          if (span.copied) elect_bulk_load(to + (uint32_t)a.slots[i] * a.slot_bytes, span.from, span.bytes, b);
+        }
+    }
+    if (STATS) elect_bulk_load(to + (uint32_t)a.slot_count * a.slot_bytes, a.stats + 4 * (int64_t)row, 16u * n, b);
+    ahead.next(a, q.group);
   }
   // Waits for the next batch and returns where its stage lies.
   __device__ __forceinline__ char *wait(const Args &a, const Place &q) {
     char *at = data + (uint32_t)stage * a.stage_bytes;
-    sm100::mbar_wait(bar(q, stage), phase, &g_row_errors, kWaitNs, sm100::kErrProducer);
+    sm100::mbar_wait(bars + 8u * stage, phase, &g_row_errors, kWaitNs, sm100::kErrProducer);
     if (++stage == a.stages) {
       stage = 0;
       phase ^= 1;
@@ -465,16 +509,15 @@ struct Ring {
 template <typename T, bool ALIGNED, int NU, bool STATS>
 __device__ __forceinline__ Ring<T, ALIGNED, NU, STATS> start_ring(const Args &a, const Place &q, Shared *s, char *data,
                                                                   int cta, int ctas) {
-  Ring<T, ALIGNED, NU, STATS> r{s, data + (size_t)q.group * a.stages * a.stage_bytes};
+  Ring<T, ALIGNED, NU, STATS> r;
+  r.bars = sm100::smem_u32(s->bars + q.group * kMaxStages);
+  r.data = data + (size_t)q.group * a.stages * a.stage_bytes;
+  r.ahead = batches_of(a, q.group, cta, ctas);
   if (threadIdx.x < kMaxGroups * kMaxStages) sm100::mbar_init(sm100::smem_u32(s->bars + threadIdx.x), 1);
   sm100::fence_mbar_init();
-  if (q.t == 0) {
-    s->ahead[q.group] = batches_of(a, q.group, cta, ctas);
-    s->fill_stage[q.group] = 0;
-  }
   __syncthreads();
   if (a.members > 1) cluster_sync();
-  if (q.t == 0) {
+  if (q.warp == 0) {
 #pragma unroll 1
     for (int i = 0; i < a.stages - 1; ++i) r.issue(a, q);
   }
@@ -613,7 +656,7 @@ __global__ void __launch_bounds__(256, NU == 1 ? 4 : 2) fwd_kernel(const __grid_
     const int n = k.count(a), row0 = k.row(a);
     bool refilled = false;
     auto refill = [&] {   // every thread of the group has left the batch before
-      if (!refilled && q.t == 0) ring.issue(a, q);
+      if (!refilled && q.warp == 0) ring.issue(a, q);
       refilled = true;
     };
 #pragma unroll 1
@@ -723,7 +766,7 @@ __device__ __forceinline__ void join_groups(float2 (&acc)[4], float factor, floa
 
 // WHOLE: both norms, both upstream gradients and both gradients of tensors are there.
 template <typename T, bool ALIGNED, bool BLOCK, bool WHOLE, int GATE, bool DROP, bool CENTER>
-__global__ void __launch_bounds__(512, 1) bwd_kernel(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(512, BLOCK ? 1 : 2) bwd_kernel(const __grid_constant__ Args a) {
   constexpr bool kGated = BLOCK && GATE != P3D_GATE_NONE;
   const p3d_residual &p = a.p;
   extern __shared__ __align__(128) char s_data[];
@@ -761,7 +804,7 @@ __global__ void __launch_bounds__(512, 1) bwd_kernel(const __grid_constant__ Arg
       const int n = k.count(a), row0 = k.row(a);
       bool refilled = false;
       auto refill = [&] {
-        if (!refilled && q.t == 0) ring.issue(a, q);
+        if (!refilled && q.warp == 0) ring.issue(a, q);
         refilled = true;
       };
 #pragma unroll 1
