@@ -11,9 +11,9 @@
 namespace p3d {
 
 namespace rows {   // instantiated in residual_{f32,f16,bf16}.cu
-extern template int run_fwd<float>(const Args &, bool, bool, bool, int64_t, size_t, cudaStream_t);
-extern template int run_fwd<__half>(const Args &, bool, bool, bool, int64_t, size_t, cudaStream_t);
-extern template int run_fwd<__nv_bfloat16>(const Args &, bool, bool, bool, int64_t, size_t, cudaStream_t);
+extern template int run_fwd<float>(const Args &, bool, bool, int, int, int64_t, size_t, cudaStream_t);
+extern template int run_fwd<__half>(const Args &, bool, bool, int, int, int64_t, size_t, cudaStream_t);
+extern template int run_fwd<__nv_bfloat16>(const Args &, bool, bool, int, int, int64_t, size_t, cudaStream_t);
 extern template int run_bwd<float>(const Args &, bool, bool, int64_t, size_t, cudaStream_t);
 extern template int run_bwd<__half>(const Args &, bool, bool, int64_t, size_t, cudaStream_t);
 extern template int run_bwd<__nv_bfloat16>(const Args &, bool, bool, int64_t, size_t, cudaStream_t);
@@ -133,22 +133,32 @@ __global__ void __launch_bounds__(256) dropout_any_kernel(const T *x, T *y, int6
 // ------------------------------------------------------------------------ host side
 bool aligned16(const void *ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15u) == 0; }
 
-// Threads a row, units of eight columns a thread, rows a CTA works on at once, and CTAs a row.
-//   Forward: two units a thread from 513 columns on, which halves the sums and the bookkeeping an element;
-//   narrower rows keep one, as a warp would not be full.  At most 256 threads a row.
-//   Backward: one unit, whose column sums fill the registers already.  At most 512 threads a row, 256 in 32
-//   bits, where two stages of five arrays of 4096 columns would not fit beside the parameters.
+// Threads that work on a row (or on a warp's rows), lanes a row, units of eight columns a thread, rows or warps of
+// rows a CTA works on at once, and CTAs a row.
+//   Forward: up to 384 columns a warp holds several rows, on 8 or 16 lanes with one or three units each, so that
+//   sums take three or four steps for all of them and the bookkeeping is shared; wider rows take two
+//   units a thread and up to 256 threads.  (One row a warp with one unit a lane: 388 us for
+//   524288 x 192, four rows: 170 us.)
+//   Backward: a row a warp at least and one unit, whose column sums fill the registers already.  At most 512
+//   threads a row, 256 in 32 bits, where two stages of five arrays of 4096 columns would not fit
+//   beside the parameters.
 struct Shape {
-  int row_threads, units, groups, members;
+  int row_threads, lanes, units, groups, members;
+  int columns() const { return (lanes < 32 ? lanes : row_threads) * kUnit * units; }   // of a CTA
+  int rows_at_once() const { return 32 / lanes; }
 };
 Shape shape_of(int dim, int dtype, bool backward) {
   Shape s;
-  s.units = backward || dim <= 512 ? 1 : 2;
-  const int threads = (dim + kUnit * s.units - 1) / (kUnit * s.units), most = backward && dtype != P3D_F32 ? 512 : 256;
   s.members = 1;
-  while (threads > s.members * most) s.members *= 2;
-  const int mine = (threads + s.members - 1) / s.members;
-  s.row_threads = (mine + 31) / 32 * 32;
+  s.lanes = backward || dim > 384 ? 32 : dim > 192 ? 16 : 8;
+  s.units = backward || dim <= 64 ? 1 : s.lanes == 32 ? 2 : 3;
+  s.row_threads = 32;
+  if (s.lanes == 32) {
+    const int threads = (dim + kUnit * s.units - 1) / (kUnit * s.units), most = backward && dtype != P3D_F32 ? 512 : 256;
+    while (threads > s.members * most) s.members *= 2;
+    const int mine = (threads + s.members - 1) / s.members;
+    s.row_threads = (mine + 31) / 32 * 32;
+  }
   s.groups = std::min(rows::kMaxGroups, std::max(1, 256 / s.row_threads));
   return s;
 }
@@ -164,7 +174,8 @@ Split split_of(const p3d_residual &p, const Shape &s, int sms, int per_sm, bool 
   c.segments = by_sample && p.gate_mode == P3D_GATE_SAMPLE ? p.rows / p.rows_per_sample : 1;
   c.segment_rows = p.rows / std::max<int64_t>(c.segments, 1);
   const int64_t room = std::max<int64_t>(1, (int64_t)sms * per_sm / s.members);
-  const int64_t useful = std::max<int64_t>(1, (c.segment_rows + s.groups - 1) / s.groups);
+  const int64_t step = (int64_t)s.groups * s.rows_at_once();
+  const int64_t useful = std::max<int64_t>(1, (c.segment_rows + step - 1) / step);
   c.slices = std::min(useful, std::max<int64_t>(1, room / std::max<int64_t>(c.segments, 1)));
   c.ctas = c.slices * std::min(c.segments, std::max<int64_t>(1, room / c.slices));
   return c;
@@ -175,7 +186,7 @@ Split split_of(const p3d_residual &p, const Shape &s, int sms, int per_sm, bool 
 // share holds, at least two.  Fills in the layout and returns the bytes; *per_sm comes in as the CTAs an SM's
 // registers hold and goes out as what its shared memory holds too.
 size_t lay_out(Args &a, const Shape &s, bool aligned, bool center, bool backward, int *per_sm) {
-  const size_t size = (size_t)dtype_size(a.p.dtype), columns = (size_t)s.row_threads * kUnit * s.units;
+  const size_t size = (size_t)dtype_size(a.p.dtype), columns = (size_t)s.columns(), at_once = (size_t)s.rows_at_once();
   a.row_threads = s.row_threads;
   a.groups = s.groups;
   a.members = s.members;
@@ -186,10 +197,11 @@ size_t lay_out(Args &a, const Shape &s, bool aligned, bool center, bool backward
                        (backward && s.groups > 1 ? s.groups * columns * sizeof(float) : 0);
   const size_t arrays = (size_t)std::max(1, a.slot_count), per_row = s.groups * (arrays * row + 16);
   const size_t all = 216 * 1024, reserve = 4096;   // static shared memory and what the driver keeps
-  while (*per_sm > 1 && all / *per_sm < fixed + 2 * per_row + reserve) --*per_sm;
+  while (*per_sm > 1 && all / *per_sm < fixed + 2 * at_once * per_row + reserve) --*per_sm;
   const size_t share = all / *per_sm - fixed - reserve;
   a.batch_rows = 1;
   if (s.members == 1) a.batch_rows = (int)std::max<size_t>(1, std::min({(size_t)8, 2048 / row, share / (2 * per_row)}));
+  a.batch_rows = (int)std::max(at_once, a.batch_rows / at_once * at_once);   // whole turns of the warp
   const size_t batch = row * a.batch_rows;
   a.slot_bytes = (uint32_t)(aligned ? batch : (batch + 15) / 16 * 16 + 16);
   a.stage_bytes = (uint32_t)(arrays * a.slot_bytes) + 16u * (uint32_t)a.batch_rows;
@@ -349,7 +361,7 @@ extern "C" int p3d_residual_fwd(const p3d_residual *args, void *out, void *y, fl
   a.slices = (int)c.slices;
   a.segment_rows = (int)c.segment_rows;
   return by_type(p.dtype, [&](auto t) {
-    return rows::run_fwd<decltype(t)>(a, aligned, center, s.units == 2, c.ctas, smem, static_cast<cudaStream_t>(stream));
+    return rows::run_fwd<decltype(t)>(a, aligned, center, s.lanes, s.units, c.ctas, smem, static_cast<cudaStream_t>(stream));
   });
 }
 

@@ -85,8 +85,10 @@ struct Place {
   int group, t, warps, warp, lane;
   int rank, first;         // CTA of the cluster, its first column
   int threads, dim, end;   // threads of the row here; columns in all; columns from `first` on
-  bool live[2];            // aligned: whether the unit is inside the row
-  int at[2];               // aligned: the unit's first column from `first` on, inside the row
+  int sub;                 // which of the warp's rows, where it holds several
+  int count;               // unaligned: how many columns the thread has
+  bool live[3];            // aligned: whether the unit is inside the row
+  int at[3];               // aligned: the unit's first column from `first` on, inside the row
 
   __device__ __forceinline__ void barrier() const {   // of the row group
     if (warps > 1) asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(warps * 32) : "memory");
@@ -98,38 +100,46 @@ struct Place {
     return ALIGNED ? (t + j / kUnit * threads) * kUnit + j % kUnit : t + j * threads;
   }
   template <bool ALIGNED>
-  __device__ __forceinline__ bool has(int j) const { return col<ALIGNED>(j) < end; }
+  __device__ __forceinline__ bool has(int j) const { return ALIGNED ? col<true>(j) < end : j < count; }
 };
 
-template <bool ALIGNED>
+// LANES: threads of a row where a warp holds several rows, else 32.
+template <int LANES, bool ALIGNED, int NU>
 __device__ __forceinline__ Place place_of(const Args &a) {
   Place q;
   // group, warp and rank are the same in a whole warp; a shuffle tells the compiler, which then keeps what
   // follows from them in uniform registers
-  q.threads = a.row_threads;
   q.group = __shfl_sync(0xffffffffu, (int)threadIdx.x / a.row_threads, 0);
-  q.t = threadIdx.x - q.group * a.row_threads;
-  q.warps = a.row_threads / 32;
-  q.warp = __shfl_sync(0xffffffffu, q.t / 32, 0);
   q.lane = threadIdx.x % 32;
   q.rank = 0;
-  if (a.members > 1) {
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(q.rank));
-    q.rank = __shfl_sync(0xffffffffu, q.rank, 0);
+  q.sub = 0;
+  if constexpr (LANES < 32) {
+    q.threads = LANES;
+    q.t = q.lane % LANES;
+    q.sub = q.lane / LANES;
+    q.warps = 1;
+    q.warp = 0;
+  } else {
+    q.threads = a.row_threads;
+    q.t = threadIdx.x - q.group * a.row_threads;
+    q.warps = a.row_threads / 32;
+    q.warp = __shfl_sync(0xffffffffu, q.t / 32, 0);
+    if (a.members > 1) {
+      asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(q.rank));
+      q.rank = __shfl_sync(0xffffffffu, q.rank, 0);
+    }
   }
   q.dim = a.p.dim;
-  return q;
-}
-template <bool ALIGNED, int NU>
-__device__ __forceinline__ void set_columns(Place &q) {
   q.first = q.rank * q.threads * kUnit * NU;
   q.end = q.dim - q.first;
+  q.count = ALIGNED ? 0 : max(0, (q.end - q.t + q.threads - 1) / q.threads);
 #pragma unroll
   for (int n = 0; n < NU; ++n) {
     const int c = (q.t + n * q.threads) * kUnit;
     q.live[n] = c < q.end;
     q.at[n] = max(0, min(c, q.end - kUnit));
   }
+  return q;
 }
 
 template <typename T>
@@ -156,19 +166,19 @@ __device__ __forceinline__ void load_cols(float2 (&f)[4 * NU], const T *row, con
   } else {
 #pragma unroll
     for (int i = 0; i < 4 * NU; ++i) {
-      const int c = q.t + 2 * i * q.threads;
-      f[i].x = c < q.end ? to_f32<T>(row[c]) : 0.f;
-      f[i].y = c + q.threads < q.end ? to_f32<T>(row[c + q.threads]) : 0.f;
+      const T *at = row + q.t + 2 * i * q.threads;
+      f[i].x = 2 * i < q.count ? to_f32<T>(at[0]) : 0.f;
+      f[i].y = 2 * i + 1 < q.count ? to_f32<T>(at[q.threads]) : 0.f;
     }
   }
 }
 
 template <typename T, bool ALIGNED, int NU>
-__device__ __forceinline__ void store_cols(T *row, const float2 (&f)[4 * NU], const Place &q) {
+__device__ __forceinline__ void store_cols(T *row, const float2 (&f)[4 * NU], const Place &q, bool valid = true) {
   if constexpr (ALIGNED) {
 #pragma unroll
     for (int n = 0; n < NU; ++n) {
-      if (!q.live[n]) continue;
+      if (!(valid && q.live[n])) continue;
       const float2 *v = f + 4 * n;
       if constexpr (sizeof(T) == 4) {
         reinterpret_cast<float4 *>(row + q.at[n])[0] = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
@@ -186,9 +196,9 @@ __device__ __forceinline__ void store_cols(T *row, const float2 (&f)[4 * NU], co
   } else {
 #pragma unroll
     for (int i = 0; i < 4 * NU; ++i) {
-      const int c = q.t + 2 * i * q.threads;
-      if (c < q.end) row[c] = from_f32<T>(f[i].x);
-      if (c + q.threads < q.end) row[c + q.threads] = from_f32<T>(f[i].y);
+      T *at = row + q.t + 2 * i * q.threads;
+      if (valid && 2 * i < q.count) at[0] = from_f32<T>(f[i].x);
+      if (valid && 2 * i + 1 < q.count) at[q.threads] = from_f32<T>(f[i].y);
     }
   }
 }
@@ -208,30 +218,34 @@ struct Exchange {
   float peers[2][kMaxCluster][4];      // [2][CTA of the cluster][values]
 };
 
-// Sums of N values over the warp, in every lane.  Two or three values share their way down: lanes 16 to 31 take
-// over the second value's half in the first step, and lanes 8 to 15 the third's in the next, so
-// that later steps move one value each; a lane of each kind then hands its total out.
-__device__ __forceinline__ void warp_sums(int lane, float (&v)[1]) { v[0] = warp_sum(v[0]); }
-__device__ __forceinline__ void warp_sums(int lane, float (&v)[2]) {
-  const bool high = lane & 16;
-  const float keep = high ? v[1] : v[0], give = high ? v[0] : v[1];
-  float s = keep + __shfl_xor_sync(0xffffffffu, give, 16);
+// Sums of N values over a row's lanes, in every one of them.  Over a whole warp two values share their way down:
+// lanes 16 to 31 take over the second in the first step, so that later steps move one value; a lane
+// of each kind then hands its total out.
+template <int LANES>
+__device__ __forceinline__ float lane_sum(float v) {
 #pragma unroll
-  for (int o = 8; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  v[0] = __shfl_sync(0xffffffffu, s, 0);
-  v[1] = __shfl_sync(0xffffffffu, s, 16);
+  for (int o = LANES / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
 }
-__device__ __forceinline__ void warp_sums(int lane, float (&v)[3]) {
-  float two[2] = {v[0], v[1]};
-  warp_sums(lane, two);
-  v[0] = two[0];
-  v[1] = two[1];
-  v[2] = warp_sum(v[2]);
+template <int LANES, int N>
+__device__ __forceinline__ void lane_sums(int lane, float (&v)[N]) {
+  if constexpr (LANES == 32 && N >= 2) {
+    const bool high = lane & 16;
+    const float keep = high ? v[1] : v[0], give = high ? v[0] : v[1];
+    const float s = lane_sum<16>(keep + __shfl_xor_sync(0xffffffffu, give, 16));
+    v[0] = __shfl_sync(0xffffffffu, s, 0);
+    v[1] = __shfl_sync(0xffffffffu, s, 16);
+    if constexpr (N > 2) v[2] = lane_sum<32>(v[2]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = lane_sum<LANES>(v[i]);
+  }
 }
 
 // N values of every thread summed over the row, the same total in every thread, always added in the
 // same order.  The shared slots alternate between calls (`at`): a thread two calls ahead has passed the
 // barrier of the call between, so nobody still reads the slots it writes.
+template <int LANES>
 struct RowSum {
   Exchange *x;
   int members;
@@ -256,8 +270,8 @@ struct RowSum {
 
   template <int N>
   __device__ __forceinline__ void operator()(const Place &q, float (&v)[N]) {
-    warp_sums(q.lane, v);
-    if (q.warps > 1) {
+    lane_sums<LANES>(q.lane, v);
+    if (LANES == 32 && q.warps > 1) {
       if (q.lane == 0) {
 #pragma unroll
         for (int i = 0; i < N; ++i) x->slots[at][i][q.group * q.warps + q.warp] = v[i];
@@ -276,8 +290,9 @@ struct RowSum {
   template <bool ALIGNED, int NU>
   __device__ __forceinline__ float2 moments(const Place &q, const float2 (&z)[4 * NU], float inv_dim) {
     float2 s[NU], d2[NU];
-    float count = 0.f;   // columns of the warp
-    if constexpr (ALIGNED) {
+    float count = 0.f;   // columns of the warp, where the row has several
+    if (LANES < 32 || q.warps == 1) {
+    } else if constexpr (ALIGNED) {
 #pragma unroll
       for (int n = 0; n < NU; ++n)
         count += (float)(kUnit * __popc(__ballot_sync(0xffffffffu, q.live[n])));
@@ -288,8 +303,8 @@ struct RowSum {
     }
 #pragma unroll
     for (int n = 0; n < NU; ++n) s[n] = add2(add2(z[4 * n], z[4 * n + 1]), add2(z[4 * n + 2], z[4 * n + 3]));
-    float mean = warp_sum(total<ALIGNED, NU>(q, s));
-    mean = q.warps == 1 ? mean * inv_dim : count > 0.f ? mean / count : 0.f;
+    float mean = lane_sum<LANES>(total<ALIGNED, NU>(q, s));
+    mean = LANES < 32 || q.warps == 1 ? mean * inv_dim : count > 0.f ? mean / count : 0.f;
 #pragma unroll
     for (int n = 0; n < NU; ++n) {
       d2[n] = splat(0.f);
@@ -303,8 +318,8 @@ struct RowSum {
         d2[n] = fma2(d, d, d2[n]);
       }
     }
-    float m2 = warp_sum(total<ALIGNED, NU>(q, d2));
-    if (q.warps == 1) return make_float2(mean, m2);
+    float m2 = lane_sum<LANES>(total<ALIGNED, NU>(q, d2));
+    if (LANES < 32 || q.warps == 1) return make_float2(mean, m2);
     if (q.lane == 0) {
       const int w = q.group * q.warps + q.warp;
       x->slots[at][0][w] = count;
@@ -316,7 +331,7 @@ struct RowSum {
     const int w = q.group * q.warps + q.lane;
     const float n_w = mine ? x->slots[at][0][w] : 0.f, mean_w = mine ? x->slots[at][1][w] : 0.f;
     float two[2] = {n_w, n_w * mean_w};
-    warp_sums(q.lane, two);
+    lane_sums<32>(q.lane, two);
     mean = two[0] > 0.f ? two[1] / two[0] : 0.f;   // a CTA of the cluster may have no columns
     const float off = mean_w - mean;
     m2 = warp_sum(fmaf(n_w * off, off, mine ? x->slots[at][2][w] : 0.f));
@@ -418,7 +433,8 @@ struct Span {
 struct Shared {
   Exchange exchange;
   uint64_t bars[kMaxGroups * kMaxStages];
-  uint8_t keep[kMaxRowThreads];
+  RoundKeys keys;
+  uint8_t keep[3 * 256];
 };
 
 // Issued by one elected lane of a converged warp.
@@ -567,13 +583,19 @@ __device__ __forceinline__ void param(float2 (&f)[4 * NU], const float4 *params,
 }
 
 // ------------------------------------------------------------------------ pieces of the formula
+// 16-bit types take the sigmoid from the fast exponential and reciprocal (a few 2^-22 off, against their 2^-9).
+template <typename T>
 __device__ __forceinline__ float activate(float g, int act) {
-  if (act == P3D_ACT_SIGMOID) return 1.f / (1.f + expf(-g));
+  if (act == P3D_ACT_SIGMOID) {
+    if constexpr (sizeof(T) == 2) return __fdividef(1.f, 1.f + __expf(-g));
+    return 1.f / (1.f + expf(-g));
+  }
   if (act == P3D_ACT_TANH) return tanhf(g);
   return g;
 }
+template <typename T>
 __device__ __forceinline__ float2 activate2(float2 g, int act) {
-  return act == P3D_ACT_IDENTITY ? g : make_float2(activate(g.x, act), activate(g.y, act));
+  return act == P3D_ACT_IDENTITY ? g : make_float2(activate<T>(g.x, act), activate<T>(g.y, act));
 }
 // act'(gate) from act(gate)
 __device__ __forceinline__ float2 slope2(float2 a, int act) {
@@ -585,9 +607,11 @@ __device__ __forceinline__ float2 slope2(float2 a, int act) {
 // Keep bits of the thread's columns of a row.  Unaligned threads own a column of each of many
 // blocks: the row's threads make one block's bits each and pass them through shared memory.
 template <bool ALIGNED, int NU>
-__device__ __forceinline__ uint32_t row_keep(const Args &a, const Place &q, PhiloxKey key, int64_t row, uint8_t *shared) {
+__device__ __forceinline__ uint32_t row_keep(const Args &a, const Place &q, const RoundKeys &key, int64_t row,
+                                             uint8_t *shared) {
   const p3d_residual &p = a.p;
   const uint64_t row_block = (uint64_t)row * (uint32_t)((p.dim + 7) / 8) + (uint32_t)(q.first / 8);
+  shared += q.sub * q.threads * NU;
   uint32_t bits = 0;
   if constexpr (ALIGNED) {
 #pragma unroll
@@ -603,7 +627,7 @@ __device__ __forceinline__ uint32_t row_keep(const Args &a, const Place &q, Phil
 #pragma unroll
     for (int j = 0; j < kUnit * NU; ++j) {
       const int c = q.t + j * q.threads;
-      if (c < q.end) bits |= ((uint32_t)(shared[c >> 3] >> (c & 7)) & 1u) << j;
+      if (j < q.count) bits |= ((uint32_t)(shared[c >> 3] >> (c & 7)) & 1u) << j;
     }
   }
   return bits;
@@ -613,11 +637,11 @@ __device__ __forceinline__ float2 kept(uint32_t keep, int i, float2 v) {
 }
 
 // (mean, 1/deviation) of a row
-template <bool ALIGNED, bool CENTER, int NU>
-__device__ __forceinline__ float2 row_stats(RowSum &sum, const Place &q, const float2 (&z)[4 * NU], int kind, float eps,
+template <bool ALIGNED, bool CENTER, int NU, int LANES>
+__device__ __forceinline__ float2 row_stats(RowSum<LANES> &sum, const Place &q, const float2 (&z)[4 * NU], int kind, float eps,
                                             float inv_dim) {
   if (CENTER && kind == P3D_NORM_LAYER) {
-    const float2 m = sum.moments<ALIGNED, NU>(q, z, inv_dim);
+    const float2 m = sum.template moments<ALIGNED, NU>(q, z, inv_dim);
     return make_float2(m.x, rsqrtf(fmaf(m.y, inv_dim, eps)));
   }
   float2 s[NU];
@@ -633,23 +657,23 @@ __device__ __forceinline__ float2 row_stats(RowSum &sum, const Place &q, const f
 }
 
 // ------------------------------------------------------------------------ forward
-// WHOLE: both norms are there.  GATE: the gate's mode, or kGateAny.  CENTER: a layer norm or a bias somewhere.
-template <typename T, bool ALIGNED, int NU, bool BLOCK, bool WHOLE, int GATE, bool DROP, bool CENTER>
+// WHOLE: both norms are there.  CENTER: a layer norm or a bias somewhere.
+template <typename T, bool ALIGNED, int LANES, int NU, bool BLOCK, bool WHOLE, bool DROP, bool CENTER>
 __global__ void __launch_bounds__(256, NU == 1 ? 4 : 2) fwd_kernel(const __grid_constant__ Args a) {
   const p3d_residual &p = a.p;
   extern __shared__ __align__(128) char s_data[];
   __shared__ Shared s;
-  Place q = place_of<ALIGNED>(a);
-  set_columns<ALIGNED, NU>(q);
-  RowSum sum{&s.exchange, a.members};
+  constexpr int kRows = 32 / LANES;   // of a warp at once
+  const Place q = place_of<LANES, ALIGNED, NU>(a);
+  RowSum<LANES> sum{&s.exchange, a.members};
   const int cta = blockIdx.x / a.members, ctas = gridDim.x / a.members;
   float4 *const params = reinterpret_cast<float4 *>(s_data);
+  if constexpr (DROP) s.keys.set(philox_key(p.rng, p.seed, p.offset));
   auto ring = start_ring<T, ALIGNED, NU, false>(
-      a, q, &s, s_data + (size_t)2 * param_count(BLOCK, CENTER) * NU * a.row_threads * sizeof(float4), cta, ctas);
+      a, q, &s, s_data + (size_t)2 * param_count(BLOCK, CENTER) * NU * q.threads * sizeof(float4), cta, ctas);
   stage_params<ALIGNED, BLOCK, CENTER, NU>(params, a, q, 1.f);
-  const PhiloxKey key = philox_key(DROP ? p.rng : nullptr, p.seed, p.offset);
   const float drop_scale = DROP ? keep_scale(p.threshold) : 1.f, inv_dim = 1.f / (float)q.dim;
-  const int gate_mode = GATE == kGateAny ? p.gate_mode : GATE;
+  const int gate_mode = p.gate_mode;
   const bool post_norm = WHOLE || p.post_kind != P3D_NORM_NONE, next_norm = WHOLE || p.next_kind != P3D_NORM_NONE;
   for (Batches k = batches_of(a, q.group, cta, ctas); k.seg < a.segments; k.next(a, q.group)) {
     const char *at = ring.wait(a, q);
@@ -660,7 +684,10 @@ __global__ void __launch_bounds__(256, NU == 1 ? 4 : 2) fwd_kernel(const __grid_
       refilled = true;
     };
 #pragma unroll 1
-    for (int i = 0; i < n; ++i) {
+    for (int i0 = 0; i0 < n; i0 += kRows) {
+      // past the batch's end a lane group goes over its last row again, without storing
+      const bool valid = LANES == 32 || i0 + q.sub < n;
+      const int i = LANES == 32 ? i0 : min(i0 + q.sub, n - 1);
       const int64_t row = row0 + i, base = row * q.dim + q.first;
       float2 z[4 * NU], w[4 * NU], b[4 * NU];
       float2 post = make_float2(0.f, 1.f), next = make_float2(0.f, 1.f);
@@ -672,7 +699,7 @@ __global__ void __launch_bounds__(256, NU == 1 ? 4 : 2) fwd_kernel(const __grid_
           load_cols<T, ALIGNED, NU>(
               g, static_cast<const T *>(p.gate) + (int64_t)((int)row / (int)p.rows_per_sample) * q.dim + q.first, q);
         float token = 1.f;
-        if (gate_mode == P3D_GATE_TOKEN) token = activate(to_f32<T>(static_cast<const T *>(p.gate)[row]), p.gate_act);
+        if (gate_mode == P3D_GATE_TOKEN) token = activate<T>(to_f32<T>(static_cast<const T *>(p.gate)[row]), p.gate_act);
         if (post_norm) {
           post = row_stats<ALIGNED, CENTER, NU>(sum, q, u, p.post_kind, p.post_eps, inv_dim);
           refill();
@@ -689,10 +716,10 @@ __global__ void __launch_bounds__(256, NU == 1 ? 4 : 2) fwd_kernel(const __grid_
           for (int j = 0; j < 4 * NU; ++j) u[j] = mul2(u[j], splat(token));
         } else if (gate_mode != P3D_GATE_NONE) {
 #pragma unroll
-          for (int j = 0; j < 4 * NU; ++j) u[j] = mul2(u[j], activate2(g[j], p.gate_act));
+          for (int j = 0; j < 4 * NU; ++j) u[j] = mul2(u[j], activate2<T>(g[j], p.gate_act));
         }
         if constexpr (DROP) {
-          const uint32_t keep = row_keep<ALIGNED, NU>(a, q, key, row, s.keep + q.group * a.row_threads * NU);
+          const uint32_t keep = row_keep<ALIGNED, NU>(a, q, s.keys, row, s.keep + q.group * a.row_threads * NU);
 #pragma unroll
           for (int j = 0; j < 4 * NU; ++j) u[j] = kept(keep, j, mul2(u[j], splat(drop_scale)));
         }
@@ -706,7 +733,7 @@ __global__ void __launch_bounds__(256, NU == 1 ? 4 : 2) fwd_kernel(const __grid_
             if (!q.has<ALIGNED>(2 * j + 1)) z[j].y = 0.f;
           }
         }
-        store_cols<T, ALIGNED, NU>(static_cast<T *>(a.out) + base, z, q);
+        store_cols<T, ALIGNED, NU>(static_cast<T *>(a.out) + base, z, q, valid);
       } else {
         load_cols<T, ALIGNED, NU>(z, ring.row_ptr(a, q, at, kX, row0, n, i), q);
       }
@@ -720,9 +747,9 @@ __global__ void __launch_bounds__(256, NU == 1 ? 4 : 2) fwd_kernel(const __grid_
           if constexpr (CENTER) z[j] = fma2(mul2(sub2(z[j], splat(next.x)), splat(next.y)), w[j], b[j]);
           else z[j] = mul2(mul2(z[j], splat(next.y)), w[j]);
         }
-        store_cols<T, ALIGNED, NU>(static_cast<T *>(a.y) + base, z, q);
+        store_cols<T, ALIGNED, NU>(static_cast<T *>(a.y) + base, z, q, valid);
       }
-      if (a.stats && q.t == 0 && q.rank == 0)
+      if (a.stats && q.t == 0 && q.rank == 0 && valid)
         reinterpret_cast<float4 *>(a.stats)[row] = make_float4(post.x, post.y, next.x, next.y);
     }
     if (!refilled) {
@@ -771,15 +798,14 @@ __global__ void __launch_bounds__(512, BLOCK ? 1 : 2) bwd_kernel(const __grid_co
   const p3d_residual &p = a.p;
   extern __shared__ __align__(128) char s_data[];
   __shared__ Shared s;
-  Place q = place_of<ALIGNED>(a);
-  set_columns<ALIGNED, 1>(q);
-  RowSum sum{&s.exchange, a.members};
+  const Place q = place_of<32, ALIGNED, 1>(a);
+  RowSum<32> sum{&s.exchange, a.members};
   const int cta = blockIdx.x / a.members, ctas = gridDim.x / a.members;
   float4 *const params = reinterpret_cast<float4 *>(s_data);
+  if constexpr (DROP) s.keys.set(philox_key(p.rng, p.seed, p.offset));
   auto ring = start_ring<T, ALIGNED, 1, true>(
       a, q, &s, s_data + (size_t)2 * param_count(BLOCK, CENTER) * a.row_threads * sizeof(float4), cta, ctas);
   float *joins = reinterpret_cast<float *>(ring.data + (size_t)(a.groups - q.group) * a.stages * a.stage_bytes);
-  const PhiloxKey key = philox_key(DROP ? p.rng : nullptr, p.seed, p.offset);
   // the dropout's scale is folded into the post norm's weight and bias, and into their gradients' sums at the end
   const float drop_scale = DROP ? keep_scale(p.threshold) : 1.f;
   stage_params<ALIGNED, BLOCK, CENTER, 1>(params, a, q, drop_scale);
@@ -815,10 +841,10 @@ __global__ void __launch_bounds__(512, BLOCK ? 1 : 2) bwd_kernel(const __grid_co
         uint32_t keep = 0xffu;
         if constexpr (BLOCK) {
           load_cols<T, ALIGNED, 1>(hn, ring.row_ptr(a, q, at, kH, row0, n, i), q);
-          if constexpr (DROP) keep = row_keep<ALIGNED, 1>(a, q, key, row, s.keep + q.group * a.row_threads);
+          if constexpr (DROP) keep = row_keep<ALIGNED, 1>(a, q, s.keys, row, s.keep + q.group * a.row_threads);
           if constexpr (kGated) {
             if (token) {
-              act[0] = splat(activate(to_f32<T>(static_cast<const T *>(p.gate)[row]), p.gate_act));
+              act[0] = splat(activate<T>(to_f32<T>(static_cast<const T *>(p.gate)[row]), p.gate_act));
 #pragma unroll
               for (int j = 1; j < 4; ++j) act[j] = act[0];
             } else if (gate_mode == P3D_GATE_NONE) {   // only where the mode is an argument
@@ -828,7 +854,7 @@ __global__ void __launch_bounds__(512, BLOCK ? 1 : 2) bwd_kernel(const __grid_co
               load_cols<T, ALIGNED, 1>(
                   act, gate_mode == P3D_GATE_SAMPLE ? sample : ring.row_ptr(a, q, at, kGate, row0, n, i), q);
 #pragma unroll
-              for (int j = 0; j < 4; ++j) act[j] = activate2(act[j], p.gate_act);
+              for (int j = 0; j < 4; ++j) act[j] = activate2<T>(act[j], p.gate_act);
             }
           }
           float2 b[4];
@@ -994,10 +1020,10 @@ int launch(K kernel, const Args &a, int64_t ctas, size_t smem, size_t (&seen)[kM
   return P3D_OK;
 }
 
-template <typename T, bool ALIGNED, int NU, bool BLOCK, bool WHOLE, int GATE, bool DROP, bool CENTER>
+template <typename T, bool ALIGNED, int LANES, int NU, bool BLOCK, bool WHOLE, bool DROP, bool CENTER>
 int fwd(const Args &a, int64_t ctas, size_t smem, cudaStream_t s) {
   static size_t seen[kMaxDevices] = {};
-  return launch(fwd_kernel<T, ALIGNED, NU, BLOCK, WHOLE, GATE, DROP, CENTER>, a, ctas, smem, seen, s);
+  return launch(fwd_kernel<T, ALIGNED, LANES, NU, BLOCK, WHOLE, DROP, CENTER>, a, ctas, smem, seen, s);
 }
 template <typename T, bool ALIGNED, bool BLOCK, bool WHOLE, int GATE, bool DROP, bool CENTER>
 int bwd(const Args &a, int64_t ctas, size_t smem, cudaStream_t s) {
@@ -1030,32 +1056,32 @@ inline bool whole_bwd(const Args &a) {
   return !a.p.h || (a.p.post_kind != P3D_NORM_NONE && a.in[kDy] && a.in[kDout] && a.dx && a.dh);
 }
 
-// Aligned rows between two norms, the usual block, get variants of their own for the gate, dropout and centring: each
+// Aligned rows between two norms, the usual block, get variants of their own for dropout, centring and (in the
+// backward) the gate: each
 // saves registers or instructions of a kernel that is bound by both.  Other calls share variants that read
 // what they have from the arguments.
-template <typename T>
-int run_fwd(const Args &a, bool aligned, bool center, bool two_units, int64_t ctas, size_t smem, cudaStream_t s) {
-  const bool whole = aligned && whole_fwd(a);
-  return with(two_units, [&](auto nu) {
-    constexpr int NU = decltype(nu)::value ? 2 : 1;
-    return with(center, [&](auto ce) {
-      constexpr bool C = decltype(ce)::value;
-      if (!a.p.h)
-        return aligned ? fwd<T, true, NU, false, false, P3D_GATE_NONE, false, C>(a, ctas, smem, s)
-                       : fwd<T, false, NU, false, false, P3D_GATE_NONE, false, C>(a, ctas, smem, s);
-      if (!whole) {
-        if (aligned) return fwd<T, true, NU, true, false, kGateAny, true, true>(a, ctas, smem, s);
-        return with(a.p.threshold != 0, [&](auto dr) {
-          return fwd<T, false, NU, true, false, kGateAny, decltype(dr)::value, C>(a, ctas, smem, s);
-        });
-      }
-      return with_gate(a.p.gate_mode, [&](auto ga) {
-        return with(a.p.threshold != 0, [&](auto dr) {
-          return fwd<T, true, NU, true, true, decltype(ga)::value, decltype(dr)::value, C>(a, ctas, smem, s);
-        });
-      });
+template <typename T, int LANES, int NU>
+int fwd_of(const Args &a, bool aligned, bool center, int64_t ctas, size_t smem, cudaStream_t s) {
+  return with(center, [&](auto ce) {
+    constexpr bool C = decltype(ce)::value;
+    if (!a.p.h)
+      return aligned ? fwd<T, true, LANES, NU, false, false, false, C>(a, ctas, smem, s)
+                     : fwd<T, false, LANES, NU, false, false, false, C>(a, ctas, smem, s);
+    if (aligned && !whole_fwd(a)) return fwd<T, true, LANES, NU, true, false, true, true>(a, ctas, smem, s);
+    return with(a.p.threshold != 0, [&](auto dr) {
+      constexpr bool D = decltype(dr)::value;
+      return aligned ? fwd<T, true, LANES, NU, true, true, D, C>(a, ctas, smem, s)
+                     : fwd<T, false, LANES, NU, true, false, D, C>(a, ctas, smem, s);
     });
   });
+}
+// lanes, units: of the forward's layout, as shape_of chooses them.
+template <typename T>
+int run_fwd(const Args &a, bool aligned, bool center, int lanes, int units, int64_t ctas, size_t smem, cudaStream_t s) {
+  if (lanes == 8 && units == 1) return fwd_of<T, 8, 1>(a, aligned, center, ctas, smem, s);
+  if (lanes == 8) return fwd_of<T, 8, 3>(a, aligned, center, ctas, smem, s);
+  if (lanes == 16) return fwd_of<T, 16, 3>(a, aligned, center, ctas, smem, s);
+  return fwd_of<T, 32, 2>(a, aligned, center, ctas, smem, s);
 }
 
 template <typename T>
@@ -1093,7 +1119,7 @@ int take_errors(unsigned *flags) {
 }
 
 #define P3D_ROW_KERNELS(T)                                                                        \
-  template int run_fwd<T>(const Args &, bool, bool, bool, int64_t, size_t, cudaStream_t);         \
+  template int run_fwd<T>(const Args &, bool, bool, int, int, int64_t, size_t, cudaStream_t);      \
   template int run_bwd<T>(const Args &, bool, bool, int64_t, size_t, cudaStream_t);               \
   template int take_errors<T>(unsigned *);
 
