@@ -196,9 +196,10 @@ size_t lay_out(Args &a, const Shape &s, bool aligned, bool center, bool backward
   const size_t fixed = (size_t)rows::param_count(a.p.h != nullptr, center) * columns * sizeof(float) +
                        (backward && s.groups > 1 ? s.groups * columns * sizeof(float) : 0);
   const size_t arrays = (size_t)std::max(1, a.slot_count), per_row = s.groups * (arrays * row + 16);
-  const size_t all = 216 * 1024, reserve = 4096;   // static shared memory and what the driver keeps
-  while (*per_sm > 1 && all / *per_sm < fixed + 2 * at_once * per_row + reserve) --*per_sm;
-  const size_t share = all / *per_sm - fixed - reserve;
+  const size_t all = 228 * 1024, reserve = 4096;   // static shared memory and what the driver keeps of a CTA
+  const size_t pad = aligned ? 0 : 2 * s.groups * arrays * 32;   // what unaligned copies take more, in two stages
+  while (*per_sm > 1 && all / *per_sm < fixed + 2 * at_once * per_row + pad + reserve) --*per_sm;
+  const size_t share = all / *per_sm - fixed - pad - reserve;
   a.batch_rows = 1;
   if (s.members == 1) a.batch_rows = (int)std::max<size_t>(1, std::min({(size_t)8, 2048 / row, share / (2 * per_row)}));
   a.batch_rows = (int)std::max(at_once, a.batch_rows / at_once * at_once);   // whole turns of the warp

@@ -78,15 +78,15 @@ __device__ __forceinline__ void cluster_sync() {
 // ------------------------------------------------------------------------ a thread's columns of a row
 // Aligned: units of eight consecutive columns that move in 16-byte pieces, a thread's second unit
 // row_threads units after its first.  Threads past the row's end read its last unit and neither
-// add to a sum nor store.  Otherwise (odd dim, or a pointer off 16 bytes) column j of the thread
-// is j * row_threads columns after its first, so that the lanes of a warp stay on consecutive
-// elements; columns past the end read as zero.
+// add to a sum nor store.  Otherwise (odd dim, or a pointer off 16 bytes) a warp has a run of columns and a lane
+// every 32nd of them, so that the lanes stay on consecutive elements at offsets known to the compiler;
+// columns past the end read as zero.
 struct Place {
   int group, t, warps, warp, lane;
   int rank, first;         // CTA of the cluster, its first column
   int threads, dim, end;   // threads of the row here; columns in all; columns from `first` on
   int sub;                 // which of the warp's rows, where it holds several
-  int count;               // unaligned: how many columns the thread has
+  int base, count;         // unaligned: the thread's first column from `first` on, and how many it has
   bool live[3];            // aligned: whether the unit is inside the row
   int at[3];               // aligned: the unit's first column from `first` on, inside the row
 
@@ -95,12 +95,10 @@ struct Place {
     else __syncwarp();
   }
   // Column j of the thread (from `first` on).
-  template <bool ALIGNED>
+  template <bool ALIGNED, int LANES>
   __device__ __forceinline__ int col(int j) const {
-    return ALIGNED ? (t + j / kUnit * threads) * kUnit + j % kUnit : t + j * threads;
+    return ALIGNED ? (t + j / kUnit * threads) * kUnit + j % kUnit : base + j * LANES;
   }
-  template <bool ALIGNED>
-  __device__ __forceinline__ bool has(int j) const { return ALIGNED ? col<true>(j) < end : j < count; }
 };
 
 // LANES: threads of a row where a warp holds several rows, else 32.
@@ -132,7 +130,8 @@ __device__ __forceinline__ Place place_of(const Args &a) {
   q.dim = a.p.dim;
   q.first = q.rank * q.threads * kUnit * NU;
   q.end = q.dim - q.first;
-  q.count = ALIGNED ? 0 : max(0, (q.end - q.t + q.threads - 1) / q.threads);
+  q.base = LANES < 32 ? q.t : q.warp * 32 * kUnit * NU + q.lane;
+  q.count = ALIGNED ? 0 : min(kUnit * NU, max(0, (q.end - q.base + LANES - 1) / LANES));
 #pragma unroll
   for (int n = 0; n < NU; ++n) {
     const int c = (q.t + n * q.threads) * kUnit;
@@ -149,7 +148,7 @@ __device__ __forceinline__ float2 pair_of(const T *v) {
 }
 
 // `row`: the row's column `first`.
-template <typename T, bool ALIGNED, int NU>
+template <typename T, bool ALIGNED, int NU, int LANES>
 __device__ __forceinline__ void load_cols(float2 (&f)[4 * NU], const T *row, const Place &q) {
   if constexpr (ALIGNED) {
 #pragma unroll
@@ -166,14 +165,14 @@ __device__ __forceinline__ void load_cols(float2 (&f)[4 * NU], const T *row, con
   } else {
 #pragma unroll
     for (int i = 0; i < 4 * NU; ++i) {
-      const T *at = row + q.t + 2 * i * q.threads;
+      const T *at = row + q.base + 2 * i * LANES;
       f[i].x = 2 * i < q.count ? to_f32<T>(at[0]) : 0.f;
-      f[i].y = 2 * i + 1 < q.count ? to_f32<T>(at[q.threads]) : 0.f;
+      f[i].y = 2 * i + 1 < q.count ? to_f32<T>(at[LANES]) : 0.f;
     }
   }
 }
 
-template <typename T, bool ALIGNED, int NU>
+template <typename T, bool ALIGNED, int NU, int LANES>
 __device__ __forceinline__ void store_cols(T *row, const float2 (&f)[4 * NU], const Place &q, bool valid = true) {
   if constexpr (ALIGNED) {
 #pragma unroll
@@ -196,9 +195,9 @@ __device__ __forceinline__ void store_cols(T *row, const float2 (&f)[4 * NU], co
   } else {
 #pragma unroll
     for (int i = 0; i < 4 * NU; ++i) {
-      T *at = row + q.t + 2 * i * q.threads;
+      T *at = row + q.base + 2 * i * LANES;
       if (valid && 2 * i < q.count) at[0] = from_f32<T>(f[i].x);
-      if (valid && 2 * i + 1 < q.count) at[q.threads] = from_f32<T>(f[i].y);
+      if (valid && 2 * i + 1 < q.count) at[LANES] = from_f32<T>(f[i].y);
     }
   }
 }
@@ -297,9 +296,7 @@ struct RowSum {
       for (int n = 0; n < NU; ++n)
         count += (float)(kUnit * __popc(__ballot_sync(0xffffffffu, q.live[n])));
     } else {
-      const int base = q.warp * 32;
-#pragma unroll
-      for (int j = 0; j < kUnit * NU; ++j) count += (float)max(0, min(32, q.end - base - j * q.threads));
+      count = (float)max(0, min(32 * kUnit * NU, q.end - q.warp * 32 * kUnit * NU));
     }
 #pragma unroll
     for (int n = 0; n < NU; ++n) s[n] = add2(add2(z[4 * n], z[4 * n + 1]), add2(z[4 * n + 2], z[4 * n + 3]));
@@ -312,8 +309,8 @@ struct RowSum {
       for (int i = 0; i < 4; ++i) {
         float2 d = sub2(z[4 * n + i], splat(mean));
         if constexpr (!ALIGNED) {
-          if (!q.has<ALIGNED>(8 * n + 2 * i)) d.x = 0.f;
-          if (!q.has<ALIGNED>(8 * n + 2 * i + 1)) d.y = 0.f;
+          if (8 * n + 2 * i >= q.count) d.x = 0.f;
+          if (8 * n + 2 * i + 1 >= q.count) d.y = 0.f;
         }
         d2[n] = fma2(d, d, d2[n]);
       }
@@ -401,32 +398,16 @@ __device__ __forceinline__ Batches batches_of(const Args &a, int group, int cta,
   return k;
 }
 
-// The bytes of one array's batch of `n` rows from `row` on in this CTA's columns.  Unaligned rows are copied with
-// the up to 15 bytes before and after that complete 16-byte pieces; a batch whose pieces would pass the
-// tensor's ends is not copied but read in place.
-template <typename T, bool ALIGNED, int NU>
-struct Span {
-  const char *from;
-  uint32_t bytes, shift;
-  bool copied;
-  __device__ __forceinline__ Span(const Args &a, const Place &q, int array, int row, int n) {
-    const char *base = static_cast<const char *>(a.in[array]);
-    const int cols = max(0, min(q.threads * kUnit * NU, q.end));   // the last CTA of a row may have none
-    from = base + ((int64_t)row * q.dim + q.first) * (int64_t)sizeof(T);
-    bytes = (uint32_t)(((n - 1) * q.dim + cols) * (int)sizeof(T));
-    shift = 0;
-    copied = cols > 0;
-    if constexpr (!ALIGNED) {
-      if (!copied) return;
-      shift = (uint32_t)(reinterpret_cast<uintptr_t>(from) & 15u);
-      const char *lo = from - shift;
-      const uint32_t padded = (shift + bytes + 15u) & ~15u;
-      copied = lo >= base && lo + padded <= base + a.p.rows * (int64_t)q.dim * (int64_t)sizeof(T);
-      from = copied ? lo : from;
-      bytes = padded;
-    }
-  }
-};
+// The bytes of one array's unaligned batch of `n` rows from `row` on in this CTA's columns: they are copied with
+// the up to 15 bytes before and after that complete 16-byte pieces.  The batches with the tensor's first
+// and last row, whose pieces would pass its ends, are not copied but read in place.
+__device__ __forceinline__ bool in_place(const Args &a, int row, int n) { return row == 0 || row + n == (int)a.p.rows; }
+// Bytes from the last 16-byte boundary to column `first` of `row`.
+template <typename T>
+__device__ __forceinline__ uint32_t shift_of(const Args &a, const Place &q, int array, int row) {
+  const uint32_t base = (uint32_t)reinterpret_cast<uintptr_t>(a.in[array]);
+  return (base + ((uint32_t)row * (uint32_t)q.dim + (uint32_t)q.first) * (uint32_t)sizeof(T)) & 15u;
+}
 
 // Shared memory: exchange slots, keep bits and the rings' barriers; then, dynamic, the parameters and each
 // group's ring.
@@ -467,32 +448,35 @@ struct Ring {
     const int n = ahead.count(a), row = ahead.row(a);
     const uint32_t to = sm100::smem_u32(data) + (uint32_t)fill * a.stage_bytes, b = bars + 8u * fill;
     fill = fill + 1 == a.stages ? 0 : fill + 1;
+    const int cols = max(0, min(q.threads * kUnit * NU, q.end));   // the last CTA of a row may have none
+    const uint32_t bytes = (uint32_t)(((n - 1) * q.dim + cols) * (int)sizeof(T));
+    const int64_t off = ((int64_t)row * q.dim + q.first) * (int64_t)sizeof(T);
+    const bool copied = cols > 0 && (ALIGNED || !in_place(a, row, n));
     if constexpr (ALIGNED) {
-      const int cols = max(0, min(q.threads * kUnit * NU, q.end));   // the last CTA of a row may have none
-      const uint32_t bytes = (uint32_t)(((n - 1) * q.dim + cols) * (int)sizeof(T));
-      const int64_t off = ((int64_t)row * q.dim + q.first) * (int64_t)sizeof(T);
-      elect_expect_tx(b, (STATS ? 16u * n : 0u) + (cols > 0 ? bytes * a.slot_count : 0u));
-      if (cols > 0) {
+      elect_expect_tx(b, (STATS ? 16u * n : 0u) + (copied ? bytes * a.slot_count : 0u));
+      if (copied) {
 #pragma unroll
         for (int i = 0; i < kArrays; ++i)
           if (a.in[i])
             elect_bulk_load(to + (uint32_t)a.slots[i] * a.slot_bytes, static_cast<const char *>(a.in[i]) + off, bytes, b);
       }
     } else {
-      uint32_t bytes = STATS ? 16u * n : 0u;
+      uint32_t all = STATS ? 16u * n : 0u;
+      if (copied) {
 #pragma unroll 1
-      for (int i = 0; i < kArrays; ++i)
-        if (a.in[i]) {
-          const Span<T, ALIGNED, NU> span(a, q, i, row, n);
-          if (span.copied) bytes += span.bytes;
-        }
-      elect_expect_tx(b, bytes);
+        for (int i = 0; i < kArrays; ++i)
+          if (a.in[i]) all += (shift_of<T>(a, q, i, row) + bytes + 15u) & ~15u;
+      }
+      elect_expect_tx(b, all);
+      if (copied) {
 #pragma unroll 1
-      for (int i = 0; i < kArrays; ++i)
-        if (a.in[i]) {
-          const Span<T, ALIGNED, NU> span(a, q, i, row, n);
-          if (span.copied) elect_bulk_load(to + (uint32_t)a.slots[i] * a.slot_bytes, span.from, span.bytes, b);
-        }
+        for (int i = 0; i < kArrays; ++i)
+          if (a.in[i]) {
+            const uint32_t shift = shift_of<T>(a, q, i, row);
+            elect_bulk_load(to + (uint32_t)a.slots[i] * a.slot_bytes, static_cast<const char *>(a.in[i]) + off - shift,
+                            (shift + bytes + 15u) & ~15u, b);
+          }
+      }
     }
     if (STATS) elect_bulk_load(to + (uint32_t)a.slot_count * a.slot_bytes, a.stats + 4 * (int64_t)row, 16u * n, b);
     ahead.next(a, q.group);
@@ -512,8 +496,9 @@ struct Ring {
                                               int i) const {
     const char *slot = at + (uint32_t)a.slots[array] * a.slot_bytes;
     if constexpr (!ALIGNED) {
-      const Span<T, ALIGNED, NU> span(a, q, array, row, n);
-      slot = span.copied ? slot + span.shift : span.from;
+      slot += shift_of<T>(a, q, array, row);
+      if (in_place(a, row, n))
+        slot = static_cast<const char *>(a.in[array]) + ((int64_t)row * q.dim + q.first) * (int64_t)sizeof(T);
     }
     return reinterpret_cast<const T *>(slot) + i * q.dim;
   }
@@ -544,7 +529,7 @@ __device__ __forceinline__ Ring<T, ALIGNED, NU, STATS> start_ring(const Args &a,
 // pieces and then their second ones, so that a warp reads consecutive banks.  (In registers they would take
 // eight a vector and thread beside the column sums.)  What is not given is its neutral value;
 // `factor` multiplies the post norm's weight and bias (the backward folds the dropout's scale in).
-template <bool ALIGNED, bool BLOCK, bool CENTER, int NU>
+template <bool ALIGNED, bool BLOCK, bool CENTER, int NU, int LANES>
 __device__ __forceinline__ void stage_params(float4 *params, const Args &a, const Place &q, float factor) {
   if (q.group == 0) {
 #pragma unroll
@@ -558,7 +543,7 @@ __device__ __forceinline__ void stage_params(float4 *params, const Args &a, cons
         float f[kUnit];
 #pragma unroll
         for (int j = 0; j < kUnit; ++j) {
-          const int c = q.col<ALIGNED>(8 * n + j);
+          const int c = q.col<ALIGNED, LANES>(8 * n + j);
           f[j] = !a.params[k] ? fill * mul : c < q.end ? mul * load_any(a.params[k], a.p.param_dtype, q.first + c) : 0.f;
         }
         float4 *to = params + 2 * (param_slot(BLOCK, k) * NU + n) * q.threads + q.t;
@@ -583,13 +568,10 @@ __device__ __forceinline__ void param(float2 (&f)[4 * NU], const float4 *params,
 }
 
 // ------------------------------------------------------------------------ pieces of the formula
-// 16-bit types take the sigmoid from the fast exponential and reciprocal (a few 2^-22 off, against their 2^-9).
+// 16-bit types take the sigmoid's exponential from the fast unit (a few 2^-22 off, against their 2^-9).
 template <typename T>
 __device__ __forceinline__ float activate(float g, int act) {
-  if (act == P3D_ACT_SIGMOID) {
-    if constexpr (sizeof(T) == 2) return __fdividef(1.f, 1.f + __expf(-g));
-    return 1.f / (1.f + expf(-g));
-  }
+  if (act == P3D_ACT_SIGMOID) return __fdividef(1.f, 1.f + (sizeof(T) == 2 ? __expf(-g) : expf(-g)));
   if (act == P3D_ACT_TANH) return tanhf(g);
   return g;
 }
@@ -605,28 +587,30 @@ __device__ __forceinline__ float2 slope2(float2 a, int act) {
 }
 
 // Keep bits of the thread's columns of a row.  Unaligned threads own a column of each of many
-// blocks: the row's threads make one block's bits each and pass them through shared memory.
-template <bool ALIGNED, int NU>
+// blocks: the lanes of a row (of a warp's run of columns) make a block's bits each and pass them
+// through shared memory.
+template <bool ALIGNED, int NU, int LANES>
 __device__ __forceinline__ uint32_t row_keep(const Args &a, const Place &q, const RoundKeys &key, int64_t row,
                                              uint8_t *shared) {
   const p3d_residual &p = a.p;
   const uint64_t row_block = (uint64_t)row * (uint32_t)((p.dim + 7) / 8) + (uint32_t)(q.first / 8);
-  shared += q.sub * q.threads * NU;
   uint32_t bits = 0;
   if constexpr (ALIGNED) {
 #pragma unroll
     for (int n = 0; n < NU; ++n) bits |= keep_bits(key, row_block + q.at[n] / 8, p.threshold) << (8 * n);
   } else {
-    q.barrier();   // the row before is done with the bits
+    const int lane = LANES < 32 ? q.t : q.lane, run = q.base - lane;   // the run's first column
+    shared += (LANES < 32 ? q.sub : q.warp) * LANES * NU;
+    __syncwarp();   // the row before is done with the bits
 #pragma unroll
     for (int n = 0; n < NU; ++n) {
-      const int b = q.t + n * q.threads;
-      if (8 * b < q.end) shared[b] = (uint8_t)keep_bits(key, row_block + b, p.threshold);
+      const int b = lane + n * LANES;
+      if (run + 8 * b < q.end) shared[b] = (uint8_t)keep_bits(key, row_block + run / 8 + b, p.threshold);
     }
-    q.barrier();
+    __syncwarp();
 #pragma unroll
     for (int j = 0; j < kUnit * NU; ++j) {
-      const int c = q.t + j * q.threads;
+      const int c = lane + j * LANES;
       if (j < q.count) bits |= ((uint32_t)(shared[c >> 3] >> (c & 7)) & 1u) << j;
     }
   }
@@ -671,7 +655,7 @@ __global__ void __launch_bounds__(256, NU == 1 ? 4 : 2) fwd_kernel(const __grid_
   if constexpr (DROP) s.keys.set(philox_key(p.rng, p.seed, p.offset));
   auto ring = start_ring<T, ALIGNED, NU, false>(
       a, q, &s, s_data + (size_t)2 * param_count(BLOCK, CENTER) * NU * q.threads * sizeof(float4), cta, ctas);
-  stage_params<ALIGNED, BLOCK, CENTER, NU>(params, a, q, 1.f);
+  stage_params<ALIGNED, BLOCK, CENTER, NU, LANES>(params, a, q, 1.f);
   const float drop_scale = DROP ? keep_scale(p.threshold) : 1.f, inv_dim = 1.f / (float)q.dim;
   const int gate_mode = p.gate_mode;
   const bool post_norm = WHOLE || p.post_kind != P3D_NORM_NONE, next_norm = WHOLE || p.next_kind != P3D_NORM_NONE;
@@ -693,10 +677,10 @@ __global__ void __launch_bounds__(256, NU == 1 ? 4 : 2) fwd_kernel(const __grid_
       float2 post = make_float2(0.f, 1.f), next = make_float2(0.f, 1.f);
       if constexpr (BLOCK) {
         float2 u[4 * NU], g[4 * NU];
-        load_cols<T, ALIGNED, NU>(u, ring.row_ptr(a, q, at, kH, row0, n, i), q);
-        if (gate_mode == P3D_GATE_ELEMENT) load_cols<T, ALIGNED, NU>(g, ring.row_ptr(a, q, at, kGate, row0, n, i), q);
+        load_cols<T, ALIGNED, NU, LANES>(u, ring.row_ptr(a, q, at, kH, row0, n, i), q);
+        if (gate_mode == P3D_GATE_ELEMENT) load_cols<T, ALIGNED, NU, LANES>(g, ring.row_ptr(a, q, at, kGate, row0, n, i), q);
         if (gate_mode == P3D_GATE_SAMPLE)
-          load_cols<T, ALIGNED, NU>(
+          load_cols<T, ALIGNED, NU, LANES>(
               g, static_cast<const T *>(p.gate) + (int64_t)((int)row / (int)p.rows_per_sample) * q.dim + q.first, q);
         float token = 1.f;
         if (gate_mode == P3D_GATE_TOKEN) token = activate<T>(to_f32<T>(static_cast<const T *>(p.gate)[row]), p.gate_act);
@@ -719,23 +703,23 @@ __global__ void __launch_bounds__(256, NU == 1 ? 4 : 2) fwd_kernel(const __grid_
           for (int j = 0; j < 4 * NU; ++j) u[j] = mul2(u[j], activate2<T>(g[j], p.gate_act));
         }
         if constexpr (DROP) {
-          const uint32_t keep = row_keep<ALIGNED, NU>(a, q, s.keys, row, s.keep + q.group * a.row_threads * NU);
+          const uint32_t keep = row_keep<ALIGNED, NU, LANES>(a, q, s.keys, row, s.keep + q.group * a.row_threads * NU);
 #pragma unroll
           for (int j = 0; j < 4 * NU; ++j) u[j] = kept(keep, j, mul2(u[j], splat(drop_scale)));
         }
         param<NU>(w, params, param_slot(BLOCK, kScale), q);
-        load_cols<T, ALIGNED, NU>(z, ring.row_ptr(a, q, at, kX, row0, n, i), q);
+        load_cols<T, ALIGNED, NU, LANES>(z, ring.row_ptr(a, q, at, kX, row0, n, i), q);
 #pragma unroll
         for (int j = 0; j < 4 * NU; ++j) {
           z[j] = fma2(w[j], u[j], z[j]);
           if constexpr (!ALIGNED) {
-            if (!q.has<ALIGNED>(2 * j)) z[j].x = 0.f;
-            if (!q.has<ALIGNED>(2 * j + 1)) z[j].y = 0.f;
+            if (2 * j >= q.count) z[j].x = 0.f;
+            if (2 * j + 1 >= q.count) z[j].y = 0.f;
           }
         }
-        store_cols<T, ALIGNED, NU>(static_cast<T *>(a.out) + base, z, q, valid);
+        store_cols<T, ALIGNED, NU, LANES>(static_cast<T *>(a.out) + base, z, q, valid);
       } else {
-        load_cols<T, ALIGNED, NU>(z, ring.row_ptr(a, q, at, kX, row0, n, i), q);
+        load_cols<T, ALIGNED, NU, LANES>(z, ring.row_ptr(a, q, at, kX, row0, n, i), q);
       }
       if (next_norm) {
         next = row_stats<ALIGNED, CENTER, NU>(sum, q, z, p.next_kind, p.next_eps, inv_dim);
@@ -747,7 +731,7 @@ __global__ void __launch_bounds__(256, NU == 1 ? 4 : 2) fwd_kernel(const __grid_
           if constexpr (CENTER) z[j] = fma2(mul2(sub2(z[j], splat(next.x)), splat(next.y)), w[j], b[j]);
           else z[j] = mul2(mul2(z[j], splat(next.y)), w[j]);
         }
-        store_cols<T, ALIGNED, NU>(static_cast<T *>(a.y) + base, z, q, valid);
+        store_cols<T, ALIGNED, NU, LANES>(static_cast<T *>(a.y) + base, z, q, valid);
       }
       if (a.stats && q.t == 0 && q.rank == 0 && valid)
         reinterpret_cast<float4 *>(a.stats)[row] = make_float4(post.x, post.y, next.x, next.y);
@@ -783,7 +767,7 @@ __device__ __forceinline__ void join_groups(float2 (&acc)[4], float factor, floa
   if (q.group == 0) {
 #pragma unroll
     for (int j = 0; j < kUnit; ++j) {
-      const int c = q.col<ALIGNED>(j);
+      const int c = q.col<ALIGNED, 32>(j);
       if (c < q.end) dst[q.first + c] = v[j];
     }
   }
@@ -808,7 +792,7 @@ __global__ void __launch_bounds__(512, BLOCK ? 1 : 2) bwd_kernel(const __grid_co
   float *joins = reinterpret_cast<float *>(ring.data + (size_t)(a.groups - q.group) * a.stages * a.stage_bytes);
   // the dropout's scale is folded into the post norm's weight and bias, and into their gradients' sums at the end
   const float drop_scale = DROP ? keep_scale(p.threshold) : 1.f;
-  stage_params<ALIGNED, BLOCK, CENTER, 1>(params, a, q, drop_scale);
+  stage_params<ALIGNED, BLOCK, CENTER, 1, 32>(params, a, q, drop_scale);
   const float inv_dim = 1.f / (float)q.dim;
   const int gate_mode = GATE == kGateAny ? p.gate_mode : GATE;
   const bool next_sums = WHOLE || a.in[kDy], has_dout = WHOLE || a.in[kDout];
@@ -840,8 +824,8 @@ __global__ void __launch_bounds__(512, BLOCK ? 1 : 2) bwd_kernel(const __grid_co
         float2 w[4], u[4], hn[4], act[4], zn[4], G[4];
         uint32_t keep = 0xffu;
         if constexpr (BLOCK) {
-          load_cols<T, ALIGNED, 1>(hn, ring.row_ptr(a, q, at, kH, row0, n, i), q);
-          if constexpr (DROP) keep = row_keep<ALIGNED, 1>(a, q, s.keys, row, s.keep + q.group * a.row_threads);
+          load_cols<T, ALIGNED, 1, 32>(hn, ring.row_ptr(a, q, at, kH, row0, n, i), q);
+          if constexpr (DROP) keep = row_keep<ALIGNED, 1, 32>(a, q, s.keys, row, s.keep + q.group * a.row_threads);
           if constexpr (kGated) {
             if (token) {
               act[0] = splat(activate<T>(to_f32<T>(static_cast<const T *>(p.gate)[row]), p.gate_act));
@@ -851,7 +835,7 @@ __global__ void __launch_bounds__(512, BLOCK ? 1 : 2) bwd_kernel(const __grid_co
 #pragma unroll
               for (int j = 0; j < 4; ++j) act[j] = splat(1.f);
             } else {
-              load_cols<T, ALIGNED, 1>(
+              load_cols<T, ALIGNED, 1, 32>(
                   act, gate_mode == P3D_GATE_SAMPLE ? sample : ring.row_ptr(a, q, at, kGate, row0, n, i), q);
 #pragma unroll
               for (int j = 0; j < 4; ++j) act[j] = activate2<T>(act[j], p.gate_act);
@@ -869,14 +853,14 @@ __global__ void __launch_bounds__(512, BLOCK ? 1 : 2) bwd_kernel(const __grid_co
           }
         }
         // u: the block's output with its dropout, before the gate; d = u act
-        if (has_dout) load_cols<T, ALIGNED, 1>(G, ring.row_ptr(a, q, at, kDout, row0, n, i), q);
+        if (has_dout) load_cols<T, ALIGNED, 1, 32>(G, ring.row_ptr(a, q, at, kDout, row0, n, i), q);
         else
 #pragma unroll
           for (int j = 0; j < 4; ++j) G[j] = splat(0.f);
         if (next_sums) {
           float2 gy[4], s0[1], s1[1];
-          load_cols<T, ALIGNED, 1>(zn, ring.row_ptr(a, q, at, kX, row0, n, i), q);
-          load_cols<T, ALIGNED, 1>(gy, ring.row_ptr(a, q, at, kDy, row0, n, i), q);
+          load_cols<T, ALIGNED, 1, 32>(zn, ring.row_ptr(a, q, at, kX, row0, n, i), q);
+          load_cols<T, ALIGNED, 1, 32>(gy, ring.row_ptr(a, q, at, kDy, row0, n, i), q);
           if constexpr (BLOCK) {
             param<1>(w, params, param_slot(BLOCK, kScale), q);
 #pragma unroll
@@ -912,12 +896,12 @@ __global__ void __launch_bounds__(512, BLOCK ? 1 : 2) bwd_kernel(const __grid_co
             if constexpr (CENTER) t = add2(t, splat(m0));
             G[j] = fma2(t, splat(st.w), G[j]);
             if constexpr (!ALIGNED) {   // no column: nothing for the sums below
-              if (!q.has<ALIGNED>(2 * j)) G[j].x = 0.f;
-              if (!q.has<ALIGNED>(2 * j + 1)) G[j].y = 0.f;
+              if (2 * j >= q.count) G[j].x = 0.f;
+              if (2 * j + 1 >= q.count) G[j].y = 0.f;
             }
           }
         }
-        if (want_dx) store_cols<T, ALIGNED, 1>(static_cast<T *>(a.dx) + base, G, q);
+        if (want_dx) store_cols<T, ALIGNED, 1, 32>(static_cast<T *>(a.dx) + base, G, q);
         if constexpr (BLOCK) {
           float2 s0[1], s1[1], s2[1], pw[4];
           param<1>(w, params, param_slot(BLOCK, kScale), q);
@@ -944,7 +928,7 @@ __global__ void __launch_bounds__(512, BLOCK ? 1 : 2) bwd_kernel(const __grid_co
           }
           if constexpr (GATE == kGateAny || GATE == P3D_GATE_ELEMENT) {
             if (gate_mode == P3D_GATE_ELEMENT && a.dgate)
-              store_cols<T, ALIGNED, 1>(static_cast<T *>(a.dgate) + base, act, q);
+              store_cols<T, ALIGNED, 1, 32>(static_cast<T *>(a.dgate) + base, act, q);
           }
           float m0 = 0.f, m1 = 0.f;
           if (post_norm || token) {
@@ -973,7 +957,7 @@ __global__ void __launch_bounds__(512, BLOCK ? 1 : 2) bwd_kernel(const __grid_co
               if constexpr (CENTER) G[j] = add2(G[j], splat(m0));
               G[j] = mul2(G[j], splat(st.y));
             }
-            store_cols<T, ALIGNED, 1>(static_cast<T *>(a.dh) + base, G, q);
+            store_cols<T, ALIGNED, 1, 32>(static_cast<T *>(a.dh) + base, G, q);
           }
         }
       }
