@@ -163,6 +163,51 @@ Shape shape_of(int dim, int dtype, bool backward) {
   return s;
 }
 
+// Whether a call needs a mean or a bias.
+bool centred(const p3d_residual &p) {
+  return p.post_kind == P3D_NORM_LAYER || p.next_kind == P3D_NORM_LAYER || p.post_bias || p.next_bias;
+}
+
+constexpr size_t kSharedPerSm = 228 * 1024, kSharedReserve = 4096;   // reserve: static, and what the driver keeps of a CTA
+
+// Dynamic shared memory without the rings, and what a stage of one row (or turn of the warps) takes.
+struct Room {
+  size_t fixed, stage;
+};
+Room room_of(const Shape &s, int dim, int dtype, size_t arrays, size_t params, bool aligned, bool backward) {
+  const size_t columns = (size_t)s.columns(), row = std::min((size_t)dim, columns) * (size_t)dtype_size(dtype);
+  Room r;
+  r.fixed = params * columns * sizeof(float) + (backward && s.groups > 1 ? s.groups * columns * sizeof(float) : 0);
+  r.stage = s.groups * (s.rows_at_once() * (arrays * row + 16) + (aligned ? 0 : arrays * 32));
+  return r;
+}
+
+// CTAs that an SM's registers hold: 64 registers a thread in the forward's narrowest form and in the backward of a norm
+// by itself, else 128.
+int per_sm_of(const p3d_residual &p, const Shape &s, bool backward) {
+  const int threads = (backward ? p.h == nullptr : s.units == 1) ? 1024 : 512;
+  return std::max(1, threads / (s.row_threads * s.groups));
+}
+
+// The row groups of a CTA: of 256 threads' worth and its halves the number that keeps most threads on an SM, as
+// far as that can be told from the call's description (all streams there, rows unaligned).
+Shape shape_for(const p3d_residual &p, bool backward) {
+  Shape best = shape_of(p.dim, p.dtype, backward);
+  const size_t arrays = (p.h ? 2 : 1) * (backward ? 2 : 1) + (p.gate_mode == P3D_GATE_ELEMENT ? 1 : 0);
+  const size_t params = rows::param_count(p.h != nullptr, centred(p));
+  int most = 0;
+  for (Shape s = best; s.groups >= 1; s.groups /= 2) {
+    const Room r = room_of(s, p.dim, p.dtype, arrays, params, false, backward);
+    const int fit = (int)std::max<size_t>(1, kSharedPerSm / (r.fixed + 2 * r.stage + kSharedReserve));
+    const int threads = std::min(fit, per_sm_of(p, s, backward)) * s.row_threads * s.groups;
+    if (threads > most) {
+      most = threads;
+      best = s;
+    }
+  }
+  return best;
+}
+
 // How the rows are cut over the CTAs: contiguous slices of the whole or, with a gate for each sample in the
 // backward, of every sample, so that the sample's gradient is summed in registers.  per_sm: CTAs an SM
 // is meant to hold.
@@ -186,33 +231,24 @@ Split split_of(const p3d_residual &p, const Shape &s, int sms, int per_sm, bool 
 // share holds, at least two.  Fills in the layout and returns the bytes; *per_sm comes in as the CTAs an SM's
 // registers hold and goes out as what its shared memory holds too.
 size_t lay_out(Args &a, const Shape &s, bool aligned, bool center, bool backward, int *per_sm) {
-  const size_t size = (size_t)dtype_size(a.p.dtype), columns = (size_t)s.columns(), at_once = (size_t)s.rows_at_once();
   a.row_threads = s.row_threads;
   a.groups = s.groups;
   a.members = s.members;
   a.slot_count = 0;
   for (int i = 0; i < rows::kArrays; ++i) a.slots[i] = a.in[i] ? a.slot_count++ : 0;
-  const size_t row = std::min((size_t)a.p.dim, columns) * size;
-  const size_t fixed = (size_t)rows::param_count(a.p.h != nullptr, center) * columns * sizeof(float) +
-                       (backward && s.groups > 1 ? s.groups * columns * sizeof(float) : 0);
-  const size_t arrays = (size_t)std::max(1, a.slot_count), per_row = s.groups * (arrays * row + 16);
-  const size_t all = 228 * 1024, reserve = 4096;   // static shared memory and what the driver keeps of a CTA
-  const size_t pad = aligned ? 0 : 2 * s.groups * arrays * 32;   // what unaligned copies take more, in two stages
-  while (*per_sm > 1 && all / *per_sm < fixed + 2 * at_once * per_row + pad + reserve) --*per_sm;
-  const size_t share = all / *per_sm - fixed - pad - reserve;
-  a.batch_rows = 1;
-  if (s.members == 1) a.batch_rows = (int)std::max<size_t>(1, std::min({(size_t)8, 2048 / row, share / (2 * per_row)}));
-  a.batch_rows = (int)std::max(at_once, a.batch_rows / at_once * at_once);   // whole turns of the warp
+  const size_t arrays = (size_t)std::max(1, a.slot_count), at_once = (size_t)s.rows_at_once();
+  const size_t row = (size_t)std::min(a.p.dim, s.columns()) * (size_t)dtype_size(a.p.dtype);
+  const Room r = room_of(s, a.p.dim, a.p.dtype, arrays, rows::param_count(a.p.h != nullptr, center), aligned, backward);
+  while (*per_sm > 1 && kSharedPerSm / *per_sm < r.fixed + 2 * r.stage + kSharedReserve) --*per_sm;
+  const size_t share = kSharedPerSm / *per_sm - r.fixed - kSharedReserve;
+  size_t turns = 1;   // rows (or turns of a warp's rows) a batch
+  if (s.members == 1) turns = std::max<size_t>(1, std::min({8 / at_once, 2048 / (at_once * row), share / (2 * r.stage)}));
+  a.batch_rows = (int)(turns * at_once);
   const size_t batch = row * a.batch_rows;
   a.slot_bytes = (uint32_t)(aligned ? batch : (batch + 15) / 16 * 16 + 16);
   a.stage_bytes = (uint32_t)(arrays * a.slot_bytes) + 16u * (uint32_t)a.batch_rows;
   a.stages = (int)std::max<size_t>(2, std::min<size_t>(rows::kMaxStages, share / (s.groups * (size_t)a.stage_bytes)));
-  return (size_t)s.groups * a.stages * a.stage_bytes + fixed;
-}
-
-// Whether a call needs a mean or a bias.
-bool centred(const p3d_residual &p) {
-  return p.post_kind == P3D_NORM_LAYER || p.next_kind == P3D_NORM_LAYER || p.post_bias || p.next_bias;
+  return (size_t)s.groups * a.stages * a.stage_bytes + r.fixed;
 }
 
 // What the layout goes by, without the tensors that only the call itself has.
@@ -325,17 +361,6 @@ extern "C" int p3d_dropout(const void *x, void *y, int dtype, int64_t rows, int6
   });
 }
 
-namespace {
-
-// CTAs that an SM's registers hold: 64 registers a thread in the forward's narrow form and in the backward of a norm
-// by itself, else 128.
-int per_sm_of(const p3d_residual &p, const Shape &s, bool backward) {
-  const int threads = (backward ? p.h == nullptr : s.units == 1) ? 1024 : 512;
-  return std::max(1, threads / (s.row_threads * s.groups));
-}
-
-}  // namespace
-
 extern "C" int p3d_residual_fwd(const p3d_residual *args, void *out, void *y, float *stats, void *stream) {
   if (int st = check_args(args, "p3d_residual_fwd")) return st;
   const p3d_residual &p = *args;
@@ -344,7 +369,7 @@ extern "C" int p3d_residual_fwd(const p3d_residual *args, void *out, void *y, fl
   P3D_CHECK_ARG(aligned16(stats), "p3d_residual_fwd: stats must be 16-byte aligned");
   DeviceInfo info;
   if (int st = device_info(&info)) return st;
-  const Shape s = shape_of(p.dim, p.dtype, false);
+  const Shape s = shape_for(p, false);
   Args a = {};
   set_params(a, p);
   a.in[rows::kX] = p.x;
@@ -369,7 +394,7 @@ extern "C" int p3d_residual_fwd(const p3d_residual *args, void *out, void *y, fl
 extern "C" size_t p3d_residual_bwd_workspace(const p3d_residual *args) {
   DeviceInfo info;
   if (check_args(args, "p3d_residual_bwd_workspace") || args->rows == 0 || device_info(&info)) return 0;
-  const Shape s = shape_of(args->dim, args->dtype, true);
+  const Shape s = shape_for(*args, true);
   return partial_floats(*args, split_of(*args, s, info.sm_count, per_sm_of(*args, s, true), true)) * sizeof(float);
 }
 
@@ -386,7 +411,7 @@ extern "C" int p3d_residual_bwd(const p3d_residual *args, const void *dout, cons
                 "p3d_residual_bwd: gradients of a block that is not there");
   DeviceInfo info;
   if (int st = device_info(&info)) return st;
-  const Shape s = shape_of(p.dim, p.dtype, true);
+  const Shape s = shape_for(p, true);
   int per_sm = per_sm_of(p, s, true);
   const Split c = split_of(p, s, info.sm_count, per_sm, true);   // as the workspace was sized
   const size_t need = partial_floats(p, c) * sizeof(float);

@@ -250,21 +250,20 @@ struct RowSum {
   int members;
   int at = 0;
 
-  // Sum of a value over the row's warps, read by every thread (slots past the row's are not added).
-  __device__ __forceinline__ float over_warps(const Place &q, int value) const {
-    const float *from = x->slots[at][value] + q.group * q.warps;
-    float s = 0.f;
-    if (q.warps % 4 == 0) {   // groups then start on 16 bytes
-#pragma unroll 1
-      for (int w = 0; w < q.warps; w += 4) {
-        const float4 f = *reinterpret_cast<const float4 *>(from + w);
-        s += (f.x + f.y) + (f.z + f.w);
-      }
+  // Sums of N values over the row's warps (up to sixteen): each half of a warp adds up one value's slots, both
+  // halves the same one where there is one.
+  template <int N>
+  __device__ __forceinline__ void over_warps(const Place &q, float (&v)[N]) const {
+    const int w = q.lane & 15, from = q.group * q.warps + w;
+    const bool mine = w < q.warps;
+    if constexpr (N == 1) {
+      v[0] = lane_sum<16>(mine ? x->slots[at][0][from] : 0.f);
     } else {
-#pragma unroll 1
-      for (int w = 0; w < q.warps; ++w) s += from[w];
+      const float s = lane_sum<16>(mine ? x->slots[at][q.lane >> 4][from] : 0.f);
+      v[0] = __shfl_sync(0xffffffffu, s, 0);
+      v[1] = __shfl_sync(0xffffffffu, s, 16);
+      if constexpr (N > 2) v[2] = lane_sum<16>(mine ? x->slots[at][2][from] : 0.f);
     }
-    return s;
   }
 
   template <int N>
@@ -276,8 +275,7 @@ struct RowSum {
         for (int i = 0; i < N; ++i) x->slots[at][i][q.group * q.warps + q.warp] = v[i];
       }
       q.barrier();
-#pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = over_warps(q, i);
+      over_warps(q, v);
       if (members > 1) over_cluster(q, v);
       at ^= 1;
     }
@@ -932,7 +930,12 @@ __global__ void __launch_bounds__(512, BLOCK ? 1 : 2) bwd_kernel(const __grid_co
           }
           float m0 = 0.f, m1 = 0.f;
           if (post_norm || token) {
-            if constexpr (GATE == kGateAny || GATE == P3D_GATE_TOKEN) {
+            if constexpr (GATE == P3D_GATE_TOKEN && !CENTER) {
+              float v[2] = {total<ALIGNED, 1>(q, s1), total<ALIGNED, 1>(q, s2)};
+              sum(q, v);
+              m1 = v[0] * post_dot;
+              if (a.dgate && q.t == 0 && q.rank == 0) static_cast<T *>(a.dgate)[row] = from_f32<T>(v[1]);
+            } else if constexpr (GATE == kGateAny || GATE == P3D_GATE_TOKEN) {
               float v[3] = {total<ALIGNED, 1>(q, s1), total<ALIGNED, 1>(q, s0), total<ALIGNED, 1>(q, s2)};
               sum(q, v);
               m1 = v[0] * post_dot;
