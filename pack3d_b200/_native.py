@@ -6,7 +6,9 @@ has not been built (``python -m pack3d_b200.build``); there is no fallback.
 from __future__ import annotations
 
 import ctypes
-import struct
+import importlib.machinery
+import importlib.util
+import sysconfig
 import threading
 from pathlib import Path
 
@@ -61,11 +63,6 @@ class PeerCopy(ctypes.Structure):
     _fields_ = [("src", _vp), ("dst", _vp), ("rows", ctypes.c_int64), ("row_bytes", ctypes.c_int64),
                 ("src_stride", ctypes.c_int64), ("dst_stride", ctypes.c_int64)]
 
-
-#: ``p3d_residual`` and ``p3d_fp8_linear`` of ``include/pack3d_b200.h``, packed for each call (packing the bytes
-#: takes a fraction of the time of filling a ctypes structure field by field)
-RESIDUAL = struct.Struct("@2q9P2Q7iI3f4x")
-FP8_LINEAR = struct.Struct("@3q3Pq5i4x")
 
 PEER_HANDLE_BYTES = 64
 PEER_MAX_COPIES = 32
@@ -151,6 +148,7 @@ _SIGNATURES = {
 }
 
 _lock = threading.Lock()
+_host_lock = threading.Lock()
 _lib = None
 
 
@@ -169,6 +167,30 @@ def lib():
                     fn.restype, fn.argtypes = restype, argtypes
                 _lib = handle
     return _lib
+
+
+def _load_host():
+    path = LIB_PATH.parent / ("pack3d_b200_host" + sysconfig.get_config_var("EXT_SUFFIX"))
+    if not path.exists():
+        raise RuntimeError(f"pack3d_b200 host module missing at {path}; build it with `python -m pack3d_b200.build`")
+    lib()   # the library it calls
+    loader = importlib.machinery.ExtensionFileLoader("pack3d_b200_host", str(path))
+    module = importlib.util.module_from_spec(importlib.util.spec_from_loader("pack3d_b200_host", loader, origin=str(path)))
+    loader.exec_module(module)
+    return module
+
+
+_host = None
+
+
+def host():
+    """The PyTorch host module (``csrc/host.cpp``), loaded once; raises if it is missing."""
+    global _host
+    if _host is None:
+        with _host_lock:
+            if _host is None:
+                _host = _load_host()
+    return _host
 
 
 def check(status, what):

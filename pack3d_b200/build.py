@@ -1,4 +1,5 @@
-"""Build ``libpack3d_b200.so`` in-tree from ``csrc/*.cu`` with nvcc for sm_100a.
+"""Build ``libpack3d_b200.so`` in-tree from ``csrc/*.cu`` with nvcc for sm_100a, and the PyTorch host module
+``pack3d_b200_host`` from ``csrc/host.cpp`` with g++.
 
     python -m pack3d_b200.build            # incremental
     python -m pack3d_b200.build --force    # rebuild everything
@@ -11,6 +12,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -53,8 +55,34 @@ def _compile(source, obj, verbose):
     return run.stderr
 
 
+def host_path():
+    """Where the host module is built: it carries the interpreter's suffix, as it uses its headers."""
+    return LIB.parent / ("pack3d_b200_host" + sysconfig.get_config_var("EXT_SUFFIX"))
+
+
+def _build_host():
+    import torch
+    gxx = shutil.which("g++")
+    if not gxx:
+        raise RuntimeError("g++ not found; it is required to build the host module of pack3d_b200")
+    home = Path(torch.__file__).parent
+    cuda = Path(nvcc()).resolve().parents[1]
+    system = [home / "include", home / "include" / "torch" / "csrc" / "api" / "include", cuda / "include",
+              Path(sysconfig.get_paths()["include"])]
+    cmd = [gxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", str(INCLUDE)]
+    for path in system:
+        cmd += ["-isystem", str(path)]
+    cmd += [str(SRC / "host.cpp"), "-o", str(host_path()), "-L", str(LIB.parent), f"-l:{LIB.name}", "-Wl,-rpath,$ORIGIN",
+            "-L", str(home / "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda"]
+    run = subprocess.run(cmd, capture_output=True, text=True)
+    if run.returncode != 0:
+        raise RuntimeError(f"g++ failed for host.cpp:\n{run.stderr}")
+
+
 def build(force=False, verbose=False, jobs=None):
-    """Compile every CUDA source for sm_100a and link the shared library; returns its path."""
+    """Compile every CUDA source for sm_100a, link the shared library and build the host module beside it; returns the
+    library's path."""
     BUILD.mkdir(exist_ok=True)
     LIB.parent.mkdir(exist_ok=True)
     sources = sorted(SRC.glob("*.cu"))
@@ -76,6 +104,8 @@ def build(force=False, verbose=False, jobs=None):
         run = subprocess.run(cmd, capture_output=True, text=True)
         if run.returncode != 0:
             raise RuntimeError(f"link failed:\n{run.stderr}")
+    if force or _stale(host_path(), [SRC / "host.cpp", *INCLUDE.glob("*.h")]):
+        _build_host()
     return LIB
 
 

@@ -12,7 +12,6 @@ to nearest even is the only one; products are exact in fp32.  NaN and infinities
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _native
 from ._validation import check_cuda
@@ -132,67 +131,6 @@ def fp8_matmul(a, b, *, bias=None, dtype=torch.bfloat16):
     return _matmul(a, b, _check_bias(bias, b.rows, a.device), dtype)
 
 
-def _pack(x, weight, bias, need_dx, need_dw):
-    """``p3d_fp8_linear`` of a call: x [rows, k], the weight a tensor or an :class:`Fp8Matrix`."""
-    code = _native.DTYPE_CODE
-    bias_code = 0 if bias is None else code[bias.dtype]
-    if isinstance(weight, Fp8Matrix):
-        return _native.FP8_LINEAR.pack(*x.shape, weight.rows, 0, weight.values.data_ptr(), weight.scales.data_ptr(),
-                                       weight.values.shape[1], code[x.dtype], 0, bias_code, 0, 0)
-    return _native.FP8_LINEAR.pack(*x.shape, weight.shape[0], weight.data_ptr(), 0, 0, 0, code[x.dtype],
-                                   code[weight.dtype], bias_code, need_dx, need_dw)
-
-
-def _forward(packed, x, bias, n, keep):
-    """``(y, what the backward needs or None)``."""
-    lib = _native.lib()
-    y = x.new_empty((x.shape[0], n))
-    with _native.on(x.device) as stream:
-        saved = x.new_empty(lib.p3d_fp8_linear_saved(packed), dtype=torch.uint8) if keep else None
-        need = lib.p3d_fp8_linear_fwd_workspace(packed)
-        ws = x.new_empty(need, dtype=torch.uint8)
-        status = lib.p3d_fp8_linear_fwd(packed, x.data_ptr(), None if bias is None else bias.data_ptr(), y.data_ptr(),
-                                        None if saved is None else saved.data_ptr(), ws.data_ptr(), need, stream)
-    if status:
-        _native.check(status, "p3d_fp8_linear_fwd")
-    return y, saved
-
-
-class _Fp8Linear(torch.autograd.Function):
-    """Forward keeps x and the weight in 8 bits only: x with blocks along its rows for dW, the weight transposed for
-    dx (its 128 x 128 blocks serve both directions)."""
-
-    @staticmethod
-    def forward(ctx, x, weight, bias):
-        need_x, need_w, _ = ctx.needs_input_grad
-        packed = _pack(x, weight, bias, need_x, need_w)
-        y, saved = _forward(packed, x, bias, weight.shape[0], need_x or need_w)
-        ctx.save_for_backward(saved)
-        ctx.meta = (packed, x.shape, weight.shape, weight.dtype, None if bias is None else bias.dtype)
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        packed, x_shape, w_shape, w_type, b_type = ctx.meta
-        need_x, need_w, need_b = ctx.needs_input_grad
-        saved, = ctx.saved_tensors
-        dy = dy.contiguous()
-        dx = dy.new_empty(x_shape) if need_x else None
-        dw = dy.new_empty(w_shape, dtype=w_type) if need_w else None
-        db = dy.new_empty(w_shape[0], dtype=b_type) if need_b else None
-        lib = _native.lib()
-        with _native.on(dy.device) as stream:
-            need = lib.p3d_fp8_linear_bwd_workspace(packed)
-            ws = dy.new_empty(need, dtype=torch.uint8)
-            status = lib.p3d_fp8_linear_bwd(packed, dy.data_ptr(), None if saved is None else saved.data_ptr(),
-                                            *(None if t is None else t.data_ptr() for t in (dx, dw, db)), ws.data_ptr(),
-                                            need, stream)
-        if status:
-            _native.check(status, "p3d_fp8_linear_bwd")
-        return dx, dw, db
-
-
 def fp8_linear(x, weight, bias=None):
     """``x weight^T + bias`` over the last dimension of ``x`` with both operands in 8-bit blocks.
 
@@ -202,37 +140,9 @@ def fp8_linear(x, weight, bias=None):
     is the tokens), the weight 128 x 128.  The result has x's dtype, gradients their inputs'; the bias's gradient is
     summed in fp32.
     """
-    check_cuda(x)
-    if x.ndim < 1:
-        raise ValueError("fp8_linear needs at least one dimension")
-    kept = isinstance(weight, Fp8Matrix)
-    shape = weight.shape
-    if len(shape) != 2 or x.shape[-1] != shape[1] or shape[0] < 1 or shape[1] < 1:
-        raise ValueError(f"weight must be [out, {x.shape[-1]}], got {list(shape)}")
-    if weight.device != x.device:
-        raise ValueError("x and weight must be on the same device")
-    bias = _check_bias(bias, shape[0], x.device)
-    rows = x if x.ndim == 2 else x.reshape(-1, shape[1])
-    rows = rows.contiguous()
-    grad = torch.is_grad_enabled()
-    wanted = grad and (x.requires_grad or bias is not None and bias.requires_grad or
-                       not kept and weight.requires_grad)
-    if kept:
-        if wanted:
-            raise ValueError("an 8-bit weight has no gradients: pass the weight itself, or call under torch.no_grad()")
-    elif weight.dtype not in _native.DTYPE_CODE:
-        raise ValueError("weight must be fp32, fp16 or bf16")
-    else:
-        weight = weight.contiguous()
-    if rows.shape[0] == 0:
-        y = x.new_empty(0, shape[0])
-        if wanted:   # zero gradients for the weight and bias, as of an empty sum
-            y = rows @ weight.t().to(x.dtype) + (0 if bias is None else bias.to(x.dtype))
-    elif wanted:
-        y = _Fp8Linear.apply(rows, weight, bias)
-    else:
-        y, _ = _forward(_pack(rows, weight, bias, False, False), rows, bias, shape[0], False)
-    return y if x.ndim == 2 else y.view(*x.shape[:-1], shape[0])
+    if isinstance(weight, Fp8Matrix):
+        return _native.host().fp8_linear(x, None, bias, weight.values, weight.scales, weight.rows, weight.cols)
+    return _native.host().fp8_linear(x, weight, bias, None, None, 0, 0)
 
 
 __all__ = ["BLOCK", "Fp8Matrix", "fp8_linear", "fp8_matmul", "quantize", "quantize_weight"]

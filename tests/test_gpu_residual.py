@@ -335,6 +335,27 @@ def test_norm_matches_residual_and_gradient_by_differences(cuda_device):
             assert abs(numeric - analytic) < 1e-3
 
 
+def test_second_derivative_is_refused(cuda_device):
+    from pack3d_b200 import NormSpec, dropout, fp8_linear, norm
+    x = torch.randn(6, 32, device=cuda_device, requires_grad=True)
+    w = torch.randn(16, 32, device=cuda_device, requires_grad=True)
+    for f in (lambda t: dropout(t, 0.5, (1, 2)), lambda t: norm(t, NormSpec()), lambda t: fp8_linear(t, w)):
+        y = f(x)
+        dy = torch.ones_like(y, requires_grad=True)
+        dx, = torch.autograd.grad(y, [x], dy, create_graph=True)
+        with pytest.raises(RuntimeError, match="differentiate twice"):
+            dx.sum().backward()
+
+
+def test_changed_input_is_noticed(cuda_device):
+    from pack3d_b200 import NormSpec, norm
+    x = torch.randn(6, 32, device=cuda_device, requires_grad=True) * 1
+    y = norm(x, NormSpec())
+    x.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
 def test_refusals(cuda_device):
     from pack3d_b200 import NormSpec, dropout, norm, residual_norm
     x = torch.randn(4, 6, 32, device=cuda_device)
