@@ -4,25 +4,30 @@
 // kind): products of e4m3 and their powers of two are exact in fp32, so nothing but the fp32
 // accumulation and the last rounding is inexact, and no accumulator leaves TMEM before its tile is done.
 //
-// Two kernels share the scheme: CTAs walk work units persistently (a tile of the output, or a slice of its k
-// where there are fewer tiles than SMs; slices go to fp32 partials that a second kernel adds in slice
-// order), warp 0 is the TMA producer (a ring of 128-column slices of both operands, 128-byte rows,
+// Two kernels share the scheme: warp 0 is the TMA producer (a ring of 128-column slices of the operands, 128-byte rows,
 // SWIZZLE_128B, with the scale bytes of four slices when a new four begin), warp 1 the MMA issuer (it
 // copies those bytes to TMEM, where one byte of a row's word scales one slice, and issues the
-// products), the others the epilogue (one row a thread).
-//   pair kernel     256 x 256 (or 128) tiles of a pair of SMs, each holding half of either operand: the L2
-//                   feeds all SMs about 10 TB/s here, and a 128 x 128 tile asks for twice the bytes a
-//                   product that this one does (1.3 against 2.5 PFLOP/s at 16384 x 8192 x 2048).  The
-//                   accumulator of 256 columns has no room for a second beside the scales: the epilogue
-//                   takes it to registers at once and frees it.  Rows go out through shared memory by TMA.
-//   narrow kernel   up to 64 rows of `a` (tokens of a decode step) are the N side: the weight's rows then
-//                   fill the 128 lanes and the token count only sets N.  128 x 128 tiles for up to 128 rows.
+// products), the others the epilogue (one row a thread).  Producer and issuer run as whole warps on
+// values that the compiler knows to be uniform, one elected lane issuing: as single threads they took
+// about 600 cycles a slice to bring operands to uniform registers, more than the products.
+//   pair kernel     256 x 256 (or 128) tiles of a pair of SMs, each holding half of either operand, CTAs
+//                   walking tiles (or, where there are fewer tiles than pairs, parts of k, which go to fp32
+//                   partials that a second kernel adds in order).  The accumulator of 256 columns has
+//                   no room for a second beside the scales: the epilogue takes it to registers at
+//                   once and frees it.  Rows go out through shared memory by TMA.  Measured on B200:
+//                   16384 x 2048 x 8192 177 us (3.1 PFLOP/s), 16384 x 8192 x 2048 209 us (2.6),
+//                   262144 x 768 x 192 122 us (bound by the 402 MB it writes: 105 us at the 3.85 TB/s of a fill).
+//   narrow kernel   up to 128 rows of `a` (tokens of a decode step) are the N side: the weight's rows
+//                   fill the 128 lanes and the token count only sets N.  The CTAs of a cluster each take a
+//                   part of k and add them through each other's shared memory.  Up to 32 tokens
+//                   may come unquantised.
 //
 // Every wait is bounded (2 s): on a timeout the kernel records an error bit (p3d_device_errors), drains its
 // copies and MMAs and frees TMEM.
 #include <algorithm>
 
 #include "common.cuh"
+#include "fp8_quant.cuh"
 #include "kernels.cuh"
 #include "sm100.cuh"
 #include "tma_host.cuh"
@@ -35,7 +40,6 @@ using namespace sm100;
 __device__ unsigned g_fp8_errors = 0;
 
 constexpr int kTileM = 128, kSlice = 128;
-constexpr int kThreads = 192;
 constexpr int kProducerWarp = 0, kMmaWarp = 1;
 constexpr uint64_t kWaitNs = 2000000000ull;
 constexpr int kMaxStages = 12;
@@ -54,29 +58,54 @@ __device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, unsigne
   return __all_sync(0xffffffffu, wait(bar, parity, role));
 }
 
-__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int c0, int c1) {
+// In what follows a converged warp calls with uniform operands and one elected lane, always the same, issues.
+__device__ __forceinline__ void expect_tx_warp(uint32_t bar, uint32_t bytes) {
   asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(
-          dst),
+      "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+      "@e mbarrier.arrive.expect_tx.release.cta.shared::cta.b64 _, [%0], %1;\n\t}" ::"r"(bar),
+      "r"(bytes)
+      : "memory");
+}
+__device__ __forceinline__ void load_2d_warp(uint32_t dst, const CUtensorMap *map, uint32_t bar, int c0, int c1) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+      "@e cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];\n\t}" ::
+          "r"(dst),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1)
       : "memory");
 }
-
 // D[tmem] (+)= A[smem desc] * B[smem desc]^T, e4m3, each row of A and of B times the power of two in its
 // byte of the scale words in TMEM; K = 32.
-__device__ __forceinline__ void mma_scaled(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb,
-                                           uint32_t accumulate) {
+__device__ __forceinline__ void mma_scaled_warp(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb,
+                                                uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred e, p;\n\telect.sync _|e, 0xffffffff;\n\t"
       "setp.ne.b32 p, %6, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+      "@e tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
       "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
       : "memory");
 }
-
 // 32 rows of 16 bytes from shared memory to four columns of TMEM, repeated in every quarter of its lanes.
-__device__ __forceinline__ void copy_scales(uint32_t tmem, uint64_t desc) {
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+__device__ __forceinline__ void copy_scales_warp(uint32_t tmem, uint64_t desc) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+      "@e tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;\n\t}" ::"r"(tmem),
+      "l"(desc)
+      : "memory");
+}
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t in_cta(uint32_t smem, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem), "r"(rank));
+  return r;
 }
 
 // Unswizzled descriptor of 512 scale bytes: 8-row groups of 16-byte rows, 128 bytes apart.
@@ -92,15 +121,15 @@ __host__ __device__ constexpr uint32_t idesc_scaled(int m, int n) {
 __device__ __forceinline__ uint32_t scale_ids(int byte) { return (uint32_t)byte << 4 | (uint32_t)byte << 29; }
 
 struct GemmParams {
-  int rows, cols;          // of the tile space: rows of the 128-lane operand, of the N operand
+  int rows, cols;
   int slices, last_steps;  // ceil(k / 128); ceil(k / 32) of the last one
   int tiles_m, tiles_n, splits;
-  const uint8_t *scales_a, *scales_b;   // of the 128-lane operand, of the N operand
-  void *out;               // [rows, cols] (SWAP: [cols, rows]) of out_type, or the partials [splits][..] fp32
+  const uint8_t *scales_a, *scales_b;
+  void *out;               // [rows, cols] of out_type, or the partials [splits][rows, cols] fp32
   int64_t pitch;           // elements between out's rows
   int64_t split_stride;    // elements between partials
   const void *bias;        // over out's columns, of bias_type, or null
-  int out_type, bias_type, vector;   // vector: 16-byte stores are aligned
+  int out_type, bias_type, vector;   // vector: rows are whole, aligned 16-byte pieces
   int stages;
 };
 
@@ -121,62 +150,87 @@ __device__ __forceinline__ Unit unit_of(const GemmParams &p, int u) {
   return r;
 }
 
-template <typename T>
-__device__ __forceinline__ void store_row(T *dst, const float (&v)[32], int valid, bool vector) {
-  if (vector && valid >= 32) {
-    constexpr int n = 16 / sizeof(T);
-#pragma unroll
-    for (int i = 0; i < 32 / n; ++i) {
-      T t[n];
-#pragma unroll
-      for (int j = 0; j < n; ++j) t[j] = from_f32<T>(v[i * n + j]);
-      uint4 w;
-      memcpy(&w, t, 16);
-      reinterpret_cast<uint4 *>(dst)[i] = w;
+// ------------------------------------------------------------------------ the narrow kernel
+constexpr int kNarrowThreads = 192;   // producer, MMA issuer, four epilogue warps
+constexpr int kMaxSplits = 8;         // CTAs of a cluster
+
+// Up to BN rows of a (tokens) against 128 rows of b a CTA; the CTAs of a cluster each take a part of k.
+// FUSED: a comes in its own type and the epilogue warps, which have nothing else to do yet, quantise this CTA's
+// part of it into shared memory while the first slices of b are on their way.
+struct NarrowParams {
+  int rows, cols;          // of b (the weight) and of a (the tokens)
+  int slices, last_steps;  // ceil(k / 128); ceil(k / 32) of the last one
+  int64_t k;
+  const uint8_t *scales_b, *scales_a;
+  const void *x;           // FUSED: a [cols, k] of x_type
+  int x_type, x_slices;    // slices of a that a CTA holds
+  void *out;               // [cols, rows] of out_type
+  const void *bias;
+  int out_type, bias_type, stages;
+};
+
+template <int BN>
+__device__ __forceinline__ uint32_t narrow_stage_bytes(bool fused) {
+  return kTileM * kSlice + (fused ? 0 : BN * kSlice) + 1024u;
+}
+
+// Blocks of x in slices [begin, end) into the layout that TMA would give them: 128-byte rows, 16-byte piece j of row r
+// at j ^ (r % 8); scale bytes in the order of fp8.cu's, from group begin / 4 on.
+template <typename T, int BN>
+__device__ __forceinline__ void quantize_tokens(const NarrowParams &p, char *values, char *scales, int begin, int end, int t) {
+  using namespace quant;
+  const bool aligned = p.k % 8 == 0 && (reinterpret_cast<uintptr_t>(p.x) & 15) == 0;
+  const int sub = t & 15, n = end - begin, total = p.cols * n;
+  for (int i0 = 0; i0 < total; i0 += 8) {   // eight blocks at a time, a half warp each
+    const int i = i0 + t / 16, row = i / n, kb = i - row * n + begin;
+    const bool inside = i < total;
+    const T *x = static_cast<const T *>(p.x) + (int64_t)(inside ? row : 0) * p.k;
+    const int64_t col = inside ? (int64_t)kb * kSlice + sub * 8 : p.k;
+    const Raw<T> r = aligned ? load8<T, true>(x, col, p.k) : load8<T, false>(x, col, p.k);
+    bool odd;
+    const uint32_t byte = scale_byte(block_amax<T>(r, &odd));
+    if (inside) {
+      const float inv = inverse_scale(byte);
+      const uint2 v = odd ? quantize8<true, T>(r, inv) : quantize8<false, T>(r, inv);
+      char *at = values + (kb - begin) * (BN * kSlice) + row * kSlice;
+      *reinterpret_cast<uint2 *>(at + (((sub >> 1) ^ (row & 7)) * 16) + (sub & 1) * 8) = v;
+      if (sub == 0) scales[(kb / 4 - begin / 4) * 512 + (row % 32) * 16 + row / 32 * 4 + kb % 4] = (char)byte;
     }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 32; ++j)
-      if (j < valid) dst[j] = from_f32<T>(v[j]);
   }
 }
 
-// BN: columns of a tile; SWAP: out is written transposed (its rows are this kernel's columns).
-template <int BN, bool SWAP>
-__global__ void __launch_bounds__(kThreads, 1)
-    fp8_gemm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb, const GemmParams p) {
-  constexpr int kChunksB = (BN + 127) / 128;            // 512-byte scale chunks of the N operand
-  constexpr uint32_t kBytesA = kTileM * kSlice, kBytesB = BN * kSlice;
-  constexpr uint32_t kStageBytes = kBytesA + (kBytesB + 1023u) / 1024u * 1024u + 2048u;
-  constexpr int kAccCols = BN < 32 ? 32 : BN;
-  constexpr int kScaleCols = 4 + 4 * kChunksB;           // per buffer; two buffers
-  constexpr int kUsed = 2 * kAccCols + 2 * kScaleCols;
-  constexpr int kTmemCols = kUsed <= 128 ? 128 : kUsed <= 256 ? 256 : 512;
-  static_assert(kUsed <= 512, "TMEM");
+template <int BN, bool FUSED>
+__global__ void __launch_bounds__(kNarrowThreads, 1)
+    fp8_narrow_kernel(const __grid_constant__ CUtensorMap tb, const __grid_constant__ CUtensorMap ta, const NarrowParams p) {
+  constexpr uint32_t kBytesW = kTileM * kSlice, kBytesX = FUSED ? 0 : BN * kSlice;
+  constexpr uint32_t kStageBytes = kBytesW + kBytesX + 1024u;   // and the scale bytes of either
+  constexpr int kAccCols = BN < 32 ? 32 : BN, kUsed = kAccCols + 16;
+  constexpr int kTmemCols = kUsed <= 64 ? 64 : kUsed <= 128 ? 128 : 256;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
-  __shared__ __align__(8) uint64_t s_bars[2 * kMaxStages + 5];
+  __shared__ __align__(8) uint64_t s_bars[2 * kMaxStages + 2];
   __shared__ uint32_t tmem_holder;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  uint32_t splits;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(splits));
+  const uint32_t split = __shfl_sync(0xffffffffu, cluster_rank(), 0);
+  const int tile = blockIdx.x / splits;
+  const int begin = (int)((int64_t)p.slices * split / splits), end = (int)((int64_t)p.slices * (split + 1) / splits);
+  const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
   const uint32_t bars = smem_u32(s_bars);
   const int S = p.stages;
+  const uint32_t x_at = base + S * kStageBytes, xs_at = x_at + p.x_slices * (BN * kSlice);   // FUSED
   auto full = [&](int s) { return bars + 8u * s; };
   auto empty = [&](int s) { return bars + 8u * (kMaxStages + s); };
-  auto acc_full = [&](int a) { return bars + 8u * (2 * kMaxStages + a); };
-  auto acc_empty = [&](int a) { return bars + 8u * (2 * kMaxStages + 2 + a); };
-  const uint32_t drain = bars + 8u * (2 * kMaxStages + 4);
-  const int units = p.tiles_m * p.tiles_n * p.splits;
+  const uint32_t acc_full = bars + 8u * (2 * kMaxStages), x_full = acc_full + 8u;
+  const int groups = (p.slices + 3) / 4;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
       mbar_init(full(s), 1);
       mbar_init(empty(s), 1);
     }
-    for (int a = 0; a < 2; ++a) {
-      mbar_init(acc_full(a), 1);
-      mbar_init(acc_empty(a), 4);
-    }
-    mbar_init(drain, 1);
+    mbar_init(acc_full, 1);
+    mbar_init(x_full, 4);
     fence_mbar_init();
   }
   if (warp == kMmaWarp) {
@@ -184,151 +238,132 @@ __global__ void __launch_bounds__(kThreads, 1)
     tmem_relinquish();
   }
   if (warp == kProducerWarp && lane == 0) {
-    prefetch_tmap(&ta);
     prefetch_tmap(&tb);
+    if (!FUSED) prefetch_tmap(&ta);
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = tmem_holder;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_holder, 0);
 
+  bool done = true;   // of the epilogue warps: the products are there
   if (warp == kProducerWarp) {
     // ------------------------------------------------------------------ TMA producer
-    if (lane == 0) {
-      const int groups = (p.slices + 3) / 4;
-      int it = 0;
-      bool ok = true;
-      for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
-        const Unit w = unit_of(p, u);
-        const uint8_t *sa = p.scales_a + (int64_t)w.tm * groups * 512;
-        const uint8_t *sb = p.scales_b + (int64_t)(w.tn * BN / 128) * groups * 512;
-        for (int kb = w.begin; kb < w.end; ++kb, ++it) {
-          const int s = it % S;
-          if (it >= S && !wait(empty(s), (it / S - 1) & 1, kErrProducer)) {
-            ok = false;
-            break;
-          }
-          const uint32_t st = base + s * kStageBytes;
-          const bool scales = kb == w.begin || kb % 4 == 0;
-          // the last tile of the N operand may have one chunk of 128 rows fewer than BN
-          const int chunks_b = min(kChunksB, (p.cols - w.tn * BN + 127) / 128);
-          mbar_expect_tx(full(s), kBytesA + kBytesB + (scales ? 512u * (1 + chunks_b) : 0u));
-          tma_load_2d(st, &ta, full(s), kb * kSlice, w.tm * kTileM);
-          tma_load_2d(st + kBytesA, &tb, full(s), kb * kSlice, w.tn * BN);
-          if (scales) {
-            const uint32_t at = st + kStageBytes - 2048u;
-            bulk_load(at, sa + (int64_t)(kb / 4) * 512, 512u, full(s));
-            for (int c = 0; c < chunks_b; ++c)
-              bulk_load(at + 512u * (1 + c), sb + ((int64_t)c * groups + kb / 4) * 512, 512u, full(s));
-          }
-        }
+    int s = 0, it = 0;
+    uint32_t turn = 1;
+    for (int kb = begin; kb < end; ++kb, ++it) {
+      if (it >= S && !wait_warp(empty(s), turn, kErrProducer)) break;
+      const uint32_t st = base + s * kStageBytes, at = st + kBytesW + kBytesX;
+      const bool scales = kb == begin || kb % 4 == 0;
+      expect_tx_warp(full(s), kBytesW + kBytesX + (scales ? (FUSED ? 512u : 1024u) : 0u));
+      load_2d_warp(st, &tb, full(s), kb * kSlice, tile * kTileM);
+      if (!FUSED) load_2d_warp(st + kBytesW, &ta, full(s), kb * kSlice, 0);
+      if (scales && lane == 0) {
+        bulk_load(at, p.scales_b + ((int64_t)tile * groups + kb / 4) * 512, 512u, full(s));
+        if (!FUSED) bulk_load(at + 512u, p.scales_a + (int64_t)(kb / 4) * 512, 512u, full(s));
       }
-      // no copies in flight into shared memory this CTA gives up
-      for (int i = it > S ? it - S : 0; i < it; ++i)
-        mbar_wait(full(i % S), (i / S) & 1, &g_fp8_errors, kWaitNs, kErrTeardown);
+      __syncwarp();
+      if (++s == S) {
+        s = 0;
+        turn ^= 1;
+      }
     }
+    // every stage used: its products are done, so its copies are too
+    for (int i = it > S ? it - S : 0; i < it; ++i)
+      mbar_wait(empty(i % S), (i / S) & 1, &g_fp8_errors, kWaitNs, kErrTeardown);
   } else if (warp == kMmaWarp) {
     // ------------------------------------------------------------------ MMA issuer
-    if (lane == 0) {
-      constexpr uint32_t idesc = idesc_scaled(kTileM, BN);
-      const uint32_t scale_cols = tmem + 2 * kAccCols;
-      const uint64_t desc_a = desc_sw128(base, 1024), desc_b = desc_sw128(base + kBytesA, 1024);
-      const uint64_t desc_s = desc_scales(base + kStageBytes - 2048u);
-      int it = 0, n = 0, groups = 0;
-      bool ok = true;
-      for (int u = blockIdx.x; ok && u < units; u += gridDim.x, ++n) {
-        const Unit w = unit_of(p, u);
-        const int a = n & 1;
-        if (n >= 2 && !wait(acc_empty(a), (n / 2 - 1) & 1, kErrMma)) break;
-        for (int kb = w.begin; kb < w.end; ++kb, ++it) {
-          const int s = it % S;
-          if (!wait(full(s), (it / S) & 1, kErrMma)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const uint64_t off = (uint64_t)(s * kStageBytes >> 4);
-          if (kb == w.begin || kb % 4 == 0) {
-            // the other buffer: products of the four slices before may still read theirs
-            const uint32_t to = scale_cols + (groups & 1) * kScaleCols;
-#pragma unroll
-            for (int c = 0; c < 1 + kChunksB; ++c) copy_scales(to + 4 * c, desc_s + off + 32u * c);
-            ++groups;
-          }
-          const uint32_t sc = scale_cols + ((groups - 1) & 1) * kScaleCols;
-          const uint32_t id = idesc | scale_ids(kb % 4);
-#pragma unroll
-          for (int k = 0; k < 4; ++k)   // 32 columns: 32 bytes along the 128-byte rows
-            mma_scaled(tmem + a * kAccCols, desc_a + off + 2 * k, desc_b + off + 2 * k, id, sc, sc + 4,
-                       kb > w.begin || k > 0 ? 1u : 0u);
-          mma_commit(empty(s));
-        }
-        if (!ok) break;
-        mma_commit(acc_full(a));
-      }
-      // drain: every commit of this CTA before its barriers and TMEM go away
-      mma_commit(drain);
-      mbar_wait(drain, 0, &g_fp8_errors, kWaitNs, kErrTeardown);
-      for (int i = it > S ? it - S : 0; i < it; ++i)
-        mbar_wait(empty(i % S), (i / S) & 1, &g_fp8_errors, kWaitNs, kErrTeardown);
-      for (int i = n > 2 ? n - 2 : 0; i < n; ++i)
-        mbar_wait(acc_full(i & 1), (i / 2) & 1, &g_fp8_errors, kWaitNs, kErrTeardown);
-    }
-  } else {
-    // ------------------------------------------------------------------ epilogue
-    const int quarter = warp & 3;   // TMEM lanes this warp may read
-    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
-    int n = 0;
-    for (int u = blockIdx.x; u < units; u += gridDim.x, ++n) {
-      const Unit w = unit_of(p, u);
-      const int a = n & 1;
-      const bool ready = wait(acc_full(a), (n / 2) & 1, kErrSoftmax);
-      if (!__all_sync(0xffffffffu, ready)) break;
+    constexpr uint32_t idesc = idesc_scaled(kTileM, BN);
+    const uint32_t scale_cols = tmem + kAccCols;
+    const uint64_t desc_w = desc_sw128(base, 1024), desc_x = desc_sw128(FUSED ? x_at : base + kBytesW, 1024);
+    const uint64_t desc_s = desc_scales(base + kBytesW + kBytesX), desc_xs = desc_scales(FUSED ? xs_at : 0u);
+    bool ok = !FUSED || wait_warp(x_full, 0, kErrMma);
+    int s = 0, copied = 0;
+    uint32_t turn = 0;
+    for (int kb = begin; ok && kb < end; ++kb) {
+      ok = wait_warp(full(s), turn, kErrMma);
+      if (!ok) break;
       tc_fence_after();
-      const int row = w.tm * kTileM + quarter * 32 + lane;
-      constexpr int kWide = BN < 32 ? BN : 32;
-#pragma unroll 1
-      for (int c0 = 0; c0 < BN; c0 += 32) {
-        const int col = w.tn * BN + c0, valid = min(kWide, p.cols - col);
-        if (valid <= 0) break;
-        uint32_t raw[32];
-        tmem_ld32(lanes + a * kAccCols + c0, raw);
-        tmem_wait_ld();
-        float v[32];
-#pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(raw[j]);
-        if (row < p.rows) {
-          if constexpr (!SWAP) {
-            if (p.bias) {
-#pragma unroll
-              for (int j = 0; j < 32; ++j)
-                if (j < valid) v[j] += load_any(p.bias, p.bias_type, col + j);
-            }
-            const int64_t at = (int64_t)row * p.pitch + col + (int64_t)w.split * p.split_stride;
-            switch (p.out_type) {
-              case P3D_F16: store_row(static_cast<__half *>(p.out) + at, v, valid, p.vector); break;
-              case P3D_BF16: store_row(static_cast<__nv_bfloat16 *>(p.out) + at, v, valid, p.vector); break;
-              default: store_row(static_cast<float *>(p.out) + at, v, valid, p.vector);
-            }
-          } else {
-            // lanes hold consecutive columns of out: each store is one run of its row
-            const float add = p.bias ? load_any(p.bias, p.bias_type, row) : 0.f;
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (j < valid)
-                store_any(p.out, p.out_type, (int64_t)(col + j) * p.pitch + row + (int64_t)w.split * p.split_stride,
-                          v[j] + add);
-          }
-        }
-        __syncwarp();   // the TMEM loads take the whole warp
+      const uint64_t off = (uint64_t)(s * kStageBytes >> 4);
+      if (kb == begin || kb % 4 == 0) {
+        // the other buffer: products of the four slices before may still read theirs
+        const uint32_t to = scale_cols + (copied & 1) * 8;
+        copy_scales_warp(to, desc_s + off);
+        copy_scales_warp(to + 4, FUSED ? desc_xs + (uint64_t)((kb / 4 - begin / 4) * 512 >> 4) : desc_s + off + 32u);
+        ++copied;
       }
-      tc_fence_before();
+      const uint32_t sc = scale_cols + ((copied - 1) & 1) * 8, id = idesc | scale_ids(kb % 4);
+      const uint64_t x_off = FUSED ? (uint64_t)((kb - begin) * (BN * kSlice) >> 4) : off;
+      // 32 columns: 32 bytes along the 128-byte rows; the last slice may have fewer than four
+      const int steps = kb + 1 < p.slices ? 4 : p.last_steps;
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (k < steps)
+          mma_scaled_warp(tmem, desc_w + off + 2 * k, desc_x + x_off + 2 * k, id, sc, sc + 4, kb > begin || k > 0 ? 1u : 0u);
+      mma_commit_warp(empty(s));
+      if (++s == S) {
+        s = 0;
+        turn ^= 1;
+      }
+    }
+    mma_commit_warp(acc_full);
+    mbar_wait(acc_full, 0, &g_fp8_errors, kWaitNs, kErrTeardown);
+  } else {
+    // ------------------------------------------------------------------ quantiser, then epilogue
+    if constexpr (FUSED) {
+      const int t = threadIdx.x - 64;
+      char *const values = reinterpret_cast<char *>(smem_raw) + (x_at - raw);
+      char *const scales = reinterpret_cast<char *>(smem_raw) + (xs_at - raw);
+      if (p.x_type == P3D_BF16) quantize_tokens<__nv_bfloat16, BN>(p, values, scales, begin, end, t);
+      else if (p.x_type == P3D_F16) quantize_tokens<__half, BN>(p, values, scales, begin, end, t);
+      else quantize_tokens<float, BN>(p, values, scales, begin, end, t);
+      fence_proxy_async_smem();   // written here, read by the tensor core
       __syncwarp();
-      if (lane == 0) mbar_arrive(acc_empty(a));
+      if (lane == 0) mbar_arrive(x_full);
+    }
+    done = __all_sync(0xffffffffu, wait(acc_full, 0, kErrSoftmax));
+    tc_fence_after();
+  }
+  // a thread's row of b; columns are tokens
+  const int quarter = warp & 3, r = quarter * 32 + lane, row = tile * kTileM + r;
+  const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
+  float *const part = reinterpret_cast<float *>(smem_raw + (base - raw));   // [BN][128], over the ring, which is done with
+  const float add = warp >= 2 && p.bias && row < p.rows ? load_any(p.bias, p.bias_type, row) : 0.f;
+  if (warp >= 2 && done) {
+#pragma unroll 1
+    for (int c0 = 0; c0 < p.cols; c0 += 32) {
+      uint32_t v[32];
+      tmem_ld32(lanes + c0, v);
+      tmem_wait_ld();
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (c0 + j < p.cols) {
+          if (splits > 1) part[(c0 + j) * kTileM + r] = __uint_as_float(v[j]);
+          else if (row < p.rows) store_any(p.out, p.out_type, (int64_t)(c0 + j) * p.rows + row, __uint_as_float(v[j]) + add);
+        }
+      __syncwarp();
     }
   }
   __syncwarp();
   tc_fence_before();
+  if (splits > 1) {
+    // tokens split, split + splits, ..: the parts of k in order, from each CTA's shared memory
+    cluster_sync();
+    if (warp >= 2 && done && row < p.rows) {
+      for (int c = split; c < p.cols; c += splits) {
+        const uint32_t at = smem_u32(part + c * kTileM + r);
+        float sum = 0.f;
+        for (uint32_t q = 0; q < splits; ++q) {
+          float v;
+          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(in_cta(at, q)) : "memory");
+          sum += v;
+        }
+        store_any(p.out, p.out_type, (int64_t)c * p.rows + row, sum + add);
+      }
+    }
+    __syncwarp();
+    cluster_sync();   // nobody reads this CTA's shared memory any more
+  }
   __syncthreads();
   if (warp == kMmaWarp) {
     tc_fence_after();
@@ -341,19 +376,6 @@ constexpr int kPairRows = 256;
 constexpr int kWarpCols = 64;          // columns of an epilogue warp
 constexpr int epilogue_warps(int bn) { return 4 * bn / kWarpCols; }
 
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ uint32_t in_cta(uint32_t smem, uint32_t rank) {
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem), "r"(rank));
-  return r;
-}
 __device__ __forceinline__ void arrive_at(uint32_t cluster_bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
 }
@@ -370,7 +392,6 @@ __device__ __forceinline__ bool wait_cluster(uint32_t bar, uint32_t parity, unsi
       : "memory");
   return __all_sync(0xffffffffu, ok && done);
 }
-// In what follows a converged warp calls with uniform operands and one elected lane, always the same, issues.
 // Into this CTA's shared memory, signalling a barrier of the pair's first CTA.
 __device__ __forceinline__ void pair_load_2d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int c0, int c1) {
   asm volatile(
@@ -408,14 +429,6 @@ __device__ __forceinline__ void pair_commit(uint32_t bar) {
       "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
       "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}" ::"r"(bar),
       "h"((uint16_t)3)
-      : "memory");
-}
-
-__device__ __forceinline__ void expect_tx_warp(uint32_t bar, uint32_t bytes) {
-  asm volatile(
-      "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
-      "@e mbarrier.arrive.expect_tx.release.cta.shared::cta.b64 _, [%0], %1;\n\t}" ::"r"(bar),
-      "r"(bytes)
       : "memory");
 }
 
@@ -692,37 +705,38 @@ __global__ void __launch_bounds__(256) add_splits_kernel(const float *part, int 
 
 struct Plan {
   int bn;
-  bool swap, pair;
+  bool pair;
   int tiles_m, tiles_n, splits;
-  int64_t rows, cols;   // tile space
 };
 
-// More than 128 rows go to the pair kernel, with the narrower tile where that makes less work of the last wave
-// (a tile costs its columns and about 64 more for filling the pipeline); up to 64 rows (tokens)
-// become the N side.  Splits: as many slices of k as fill the SMs, each of at least two 128-column
-// slices (four for a pair).
+// Up to 128 rows (tokens) are the narrow kernel's; more go to the pair kernel, with the narrower tile where that
+// makes less work of the last wave (a tile costs its columns and about 64 more for filling the
+// pipeline).  Splits: as many parts of k as fill the SMs, each of at least two 128-column slices (four for
+// a pair); the narrow kernel's are a cluster, at most eight.
 Plan plan_of(int64_t rows, int64_t cols, int64_t k, int sms) {
   Plan p;
   const int64_t slices = (k + kSlice - 1) / kSlice;
   p.pair = rows > 128;
-  p.swap = rows <= 64;
-  p.rows = p.swap ? cols : rows;
-  p.cols = p.swap ? rows : cols;
-  int64_t slots = sms, least = 2;
-  if (p.pair) {
-    slots = sms / 2;
-    least = 4;
-    p.tiles_m = (int)((rows + kPairRows - 1) / kPairRows);
-    auto cost = [&](int bn) { return (p.tiles_m * ((cols + bn - 1) / bn) + slots - 1) / slots * (bn + 64); };
-    p.bn = cost(128) < cost(256) ? 128 : 256;
-  } else {
-    p.bn = !p.swap ? 128 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
-    p.tiles_m = (int)((p.rows + kTileM - 1) / kTileM);
+  if (!p.pair) {
+    p.bn = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
+    p.tiles_m = (int)((cols + kTileM - 1) / kTileM);
+    p.tiles_n = 1;
+    p.splits = 1;
+    while (p.splits < kMaxSplits && (int64_t)p.tiles_m * p.splits * 2 <= sms && slices >= 4 * p.splits) p.splits *= 2;
+    return p;
   }
-  p.tiles_n = (int)((p.cols + p.bn - 1) / p.bn);
+  const int64_t slots = sms / 2;
+  p.tiles_m = (int)((rows + kPairRows - 1) / kPairRows);
+  auto cost = [&](int bn) { return (p.tiles_m * ((cols + bn - 1) / bn) + slots - 1) / slots * (bn + 64); };
+  p.bn = cost(128) < cost(256) ? 128 : 256;
+  p.tiles_n = (int)((cols + p.bn - 1) / p.bn);
   const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
-  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({slots / std::max<int64_t>(1, tiles), slices / least, 64}));
+  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({slots / std::max<int64_t>(1, tiles), slices / 4, 64}));
   return p;
+}
+
+size_t partial_bytes(const Plan &p, int64_t rows, int64_t cols) {
+  return p.pair && p.splits > 1 ? (size_t)p.splits * rows * cols * sizeof(float) : 0;
 }
 
 template <int BN, int BOXES>
@@ -740,16 +754,28 @@ int launch_pair(const CUtensorMap &ta, const CUtensorMap &tb, const CUtensorMap 
   return P3D_OK;
 }
 
-template <int BN, bool SWAP>
-int launch_gemm(const CUtensorMap &ta, const CUtensorMap &tb, GemmParams g, int sms, cudaStream_t s) {
-  constexpr size_t stage = kTileM * kSlice + (BN * kSlice + 1023) / 1024 * 1024 + 2048;
-  g.stages = (int)std::min<size_t>(kMaxStages, (220 * 1024) / stage);
-  const size_t smem = g.stages * stage + 1024;
+// What a narrow launch holds: a ring of at least three stages and, fused, its part of the tokens.
+template <int BN, bool FUSED>
+int launch_narrow(const CUtensorMap &tb, const CUtensorMap &ta, NarrowParams g, int tiles, int splits, cudaStream_t s) {
+  constexpr size_t stage = kTileM * kSlice + (FUSED ? 0 : BN * kSlice) + 1024;
+  const size_t x_bytes = FUSED ? (size_t)g.x_slices * BN * kSlice + ((size_t)g.x_slices / 4 + 2) * 512 : 0;
+  const size_t part = (size_t)BN * kTileM * sizeof(float);
+  g.stages = (int)std::min<size_t>(kMaxStages, (216 * 1024 - 1024 - x_bytes) / stage);
+  const size_t smem = std::max(g.stages * stage + x_bytes, splits > 1 ? part : (size_t)0) + 1024;
   static size_t seen[kMaxDevices] = {};
-  if (int st = smem_optin(fp8_gemm_kernel<BN, SWAP>, smem, seen)) return st;
-  const int64_t units = (int64_t)g.tiles_m * g.tiles_n * g.splits;
-  fp8_gemm_kernel<BN, SWAP><<<(unsigned)std::min<int64_t>(units, sms), kThreads, smem, s>>>(ta, tb, g);
-  P3D_LAUNCH_CHECK();
+  if (int st = smem_optin(fp8_narrow_kernel<BN, FUSED>, smem, seen)) return st;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(tiles * splits));
+  cfg.blockDim = dim3(kNarrowThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)splits;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  P3D_CUDA_TRY(cudaLaunchKernelEx(&cfg, fp8_narrow_kernel<BN, FUSED>, tb, ta, g));
   return P3D_OK;
 }
 
@@ -775,11 +801,79 @@ int take_fp8_errors(unsigned *flags) {
 
 using namespace p3d;
 
+namespace {
+
+// The narrow product: tokens a (8-bit, with a_scales) or x (of x_type), against b.
+int run_narrow(const Plan &p, const void *x, int x_type, const void *a, int64_t a_pitch, const void *a_scales, const void *b,
+               int64_t b_pitch, const void *b_scales, int64_t rows, int64_t cols, int64_t k, const void *bias,
+               int bias_type, void *out, int out_type, cudaStream_t s) {
+  CUtensorMap tb, ta = {};
+  {
+    const uint64_t dims[2] = {(uint64_t)k, (uint64_t)cols}, strides[1] = {(uint64_t)b_pitch};
+    const uint32_t box[2] = {kSlice, kTileM};
+    if (int st = encode_tiled(&tb, CU_TENSOR_MAP_DATA_TYPE_UINT8, b, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return st;
+  }
+  if (!x) {
+    const uint64_t dims[2] = {(uint64_t)k, (uint64_t)rows}, strides[1] = {(uint64_t)a_pitch};
+    const uint32_t box[2] = {kSlice, (uint32_t)p.bn};
+    if (int st = encode_tiled(&ta, CU_TENSOR_MAP_DATA_TYPE_UINT8, a, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return st;
+  }
+  NarrowParams g = {};
+  g.rows = (int)cols;
+  g.cols = (int)rows;
+  g.k = k;
+  g.slices = (int)((k + kSlice - 1) / kSlice);
+  g.last_steps = (int)((k - (int64_t)(g.slices - 1) * kSlice + 31) / 32);
+  g.scales_b = static_cast<const uint8_t *>(b_scales);
+  g.scales_a = static_cast<const uint8_t *>(a_scales);
+  g.x = x;
+  g.x_type = x_type;
+  g.x_slices = x ? (g.slices + p.splits - 1) / p.splits : 0;
+  g.out = out;
+  g.out_type = out_type;
+  g.bias = bias;
+  g.bias_type = bias_type;
+  if (x) return p.bn == 16 ? launch_narrow<16, true>(tb, ta, g, p.tiles_m, p.splits, s)
+                           : launch_narrow<32, true>(tb, ta, g, p.tiles_m, p.splits, s);
+  switch (p.bn) {
+    case 16: return launch_narrow<16, false>(tb, ta, g, p.tiles_m, p.splits, s);
+    case 32: return launch_narrow<32, false>(tb, ta, g, p.tiles_m, p.splits, s);
+    case 64: return launch_narrow<64, false>(tb, ta, g, p.tiles_m, p.splits, s);
+    default: return launch_narrow<128, false>(tb, ta, g, p.tiles_m, p.splits, s);
+  }
+}
+
+}  // namespace
+
+namespace p3d {
+
+// Whether launch_fp8_tokens takes these extents: up to 32 tokens of which a CTA's part fits beside the ring, and few
+// enough weight tiles that quantising the tokens in each of them does not outweigh the launch that it saves.
+bool fp8_tokens_fit(int64_t rows, int64_t cols, int64_t k) {
+  DeviceInfo info;
+  if (rows > 32 || check_extents(rows, cols, k, "p3d_fp8_linear_fwd") || device_info(&info)) return false;
+  const Plan p = plan_of(rows, cols, k, info.sm_count);
+  const int64_t slices = ((k + kSlice - 1) / kSlice + p.splits - 1) / p.splits;
+  return slices * p.bn * kSlice <= 64 * 1024 && rows * slices <= 256 && p.tiles_m * p.splits <= 2 * info.sm_count;
+}
+
+int launch_fp8_tokens(const void *x, int x_type, const void *b, int64_t b_pitch, const void *b_scales, int64_t rows,
+                      int64_t cols, int64_t k, const void *bias, int bias_type, void *out, int out_type, cudaStream_t s) {
+  DeviceInfo info;
+  if (int st = device_info(&info)) return st;
+  if (info.major != 10) return fail(P3D_ERR_DEVICE, "p3d_fp8_linear_fwd needs an sm_100 device");
+  P3D_CHECK_ARG(b_pitch >= k && b_pitch % 16 == 0 && (((uintptr_t)b | (uintptr_t)b_scales) & 15) == 0,
+                "p3d_fp8_linear_fwd: the weight's pitch must be a multiple of 16 and hold k columns, aligned to 16 bytes");
+  return run_narrow(plan_of(rows, cols, k, info.sm_count), x, x_type, nullptr, 0, nullptr, b, b_pitch, b_scales, rows, cols, k,
+                    bias, bias_type, out, out_type, s);
+}
+
+}  // namespace p3d
+
 extern "C" size_t p3d_fp8_matmul_workspace(int64_t rows, int64_t cols, int64_t k) {
   DeviceInfo info;
   if (check_extents(rows, cols, k, "p3d_fp8_matmul_workspace") || device_info(&info)) return 0;
-  const Plan p = plan_of(rows, cols, k, info.sm_count);
-  return p.splits > 1 ? (size_t)p.splits * rows * cols * sizeof(float) : 0;
+  return partial_bytes(plan_of(rows, cols, k, info.sm_count), rows, cols);
 }
 
 extern "C" int p3d_fp8_matmul(const void *a, int64_t a_pitch, const void *a_scales, const void *b, int64_t b_pitch,
@@ -797,34 +891,34 @@ extern "C" int p3d_fp8_matmul(const void *a, int64_t a_pitch, const void *a_scal
   if (int st = device_info(&info)) return st;
   if (info.major != 10) return fail(P3D_ERR_DEVICE, "p3d_fp8_matmul needs an sm_100 device");
   const Plan p = plan_of(rows, cols, k, info.sm_count);
-  const size_t need = p.splits > 1 ? (size_t)p.splits * rows * cols * sizeof(float) : 0;
+  const size_t need = partial_bytes(p, rows, cols);
   if (need && (!workspace || workspace_bytes < need))
     return fail(P3D_ERR_WORKSPACE, "p3d_fp8_matmul: workspace of %zu bytes, %zu needed", workspace_bytes, need);
-  const void *wide = p.swap ? b : a, *narrow = p.swap ? a : b;
-  const int64_t wide_pitch = p.swap ? b_pitch : a_pitch, narrow_pitch = p.swap ? a_pitch : b_pitch;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (!p.pair)
+    return run_narrow(p, nullptr, 0, a, a_pitch, a_scales, b, b_pitch, b_scales, rows, cols, k, bias, bias_dtype, out, out_dtype,
+                      s);
   CUtensorMap ta, tb;
   {
-    const uint64_t dims[2] = {(uint64_t)k, (uint64_t)p.rows}, strides[1] = {(uint64_t)wide_pitch};
+    const uint64_t dims[2] = {(uint64_t)k, (uint64_t)rows}, strides[1] = {(uint64_t)a_pitch};
     const uint32_t box[2] = {kSlice, kTileM};
-    if (int st = encode_tiled(&ta, CU_TENSOR_MAP_DATA_TYPE_UINT8, wide, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B))
-      return st;
+    if (int st = encode_tiled(&ta, CU_TENSOR_MAP_DATA_TYPE_UINT8, a, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return st;
   }
   {
-    const uint64_t dims[2] = {(uint64_t)k, (uint64_t)p.cols}, strides[1] = {(uint64_t)narrow_pitch};
-    const uint32_t box[2] = {kSlice, (uint32_t)(p.pair ? p.bn / 2 : p.bn)};
-    if (int st = encode_tiled(&tb, CU_TENSOR_MAP_DATA_TYPE_UINT8, narrow, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B))
-      return st;
+    const uint64_t dims[2] = {(uint64_t)k, (uint64_t)cols}, strides[1] = {(uint64_t)b_pitch};
+    const uint32_t box[2] = {kSlice, (uint32_t)p.bn / 2};
+    if (int st = encode_tiled(&tb, CU_TENSOR_MAP_DATA_TYPE_UINT8, b, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return st;
   }
   GemmParams g = {};
-  g.rows = (int)p.rows;
-  g.cols = (int)p.cols;
+  g.rows = (int)rows;
+  g.cols = (int)cols;
   g.slices = (int)((k + kSlice - 1) / kSlice);
   g.last_steps = (int)((k - (int64_t)(g.slices - 1) * kSlice + 31) / 32);
   g.tiles_m = p.tiles_m;
   g.tiles_n = p.tiles_n;
   g.splits = p.splits;
-  g.scales_a = static_cast<const uint8_t *>(p.swap ? b_scales : a_scales);
-  g.scales_b = static_cast<const uint8_t *>(p.swap ? a_scales : b_scales);
+  g.scales_a = static_cast<const uint8_t *>(a_scales);
+  g.scales_b = static_cast<const uint8_t *>(b_scales);
   g.out = p.splits > 1 ? workspace : out;
   g.out_type = p.splits > 1 ? (int)P3D_F32 : out_dtype;
   g.pitch = cols;
@@ -832,9 +926,8 @@ extern "C" int p3d_fp8_matmul(const void *a, int64_t a_pitch, const void *a_scal
   g.bias = p.splits > 1 ? nullptr : bias;
   g.bias_type = bias_dtype;
   g.vector = (cols * dtype_size(g.out_type)) % 16 == 0 && ((uintptr_t)g.out & 15) == 0;
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
   int st;
-  if (p.pair) {
+  {
     CUtensorMap tout = {};
     if (g.vector) {
       const int size = dtype_size(g.out_type);
@@ -859,10 +952,7 @@ extern "C" int p3d_fp8_matmul(const void *a, int64_t a_pitch, const void *a_scal
     st = p.bn == 128   ? launch_pair<128, 2>(ta, tb, ts[0], ts[1], tout, g, info.sm_count, s)
          : g.slices <= 8 ? launch_pair<256, 2>(ta, tb, ts[0], ts[1], tout, g, info.sm_count, s)
                          : launch_pair<256, 1>(ta, tb, ts[0], ts[1], tout, g, info.sm_count, s);
-  } else if (!p.swap) st = launch_gemm<128, false>(ta, tb, g, info.sm_count, s);
-  else if (p.bn == 16) st = launch_gemm<16, true>(ta, tb, g, info.sm_count, s);
-  else if (p.bn == 32) st = launch_gemm<32, true>(ta, tb, g, info.sm_count, s);
-  else st = launch_gemm<64, true>(ta, tb, g, info.sm_count, s);
+  }
   if (st != P3D_OK || p.splits == 1) return st;
   const unsigned grid = (unsigned)std::min<int64_t>((rows * cols + 255) / 256, (int64_t)info.sm_count * 8);
   add_splits_kernel<<<grid, 256, 0, s>>>(static_cast<const float *>(workspace), p.splits, rows, cols, bias, bias_dtype,

@@ -52,10 +52,12 @@ struct Forward {
   void *sums;
   size_t sum_bytes, bytes;
 };
+// Few tokens without a gradient of the weight are quantised inside their product.
+bool in_product(const p3d_fp8_linear &a) { return !a.need_dw && fp8_tokens_fit(a.rows, a.n, a.k); }
 Forward forward_of(const p3d_fp8_linear &a, void *buffer) {
   Pieces p{static_cast<char *>(buffer)};
   Forward f = {};
-  f.x = take_matrix(p, a.rows, a.k);
+  if (!in_product(a)) f.x = take_matrix(p, a.rows, a.k);
   if (a.weight) f.w = take_matrix(p, a.n, a.k);
   f.sum_bytes = p3d_fp8_matmul_workspace(a.rows, a.n, a.k);
   f.sums = p.take(f.sum_bytes);
@@ -113,13 +115,15 @@ extern "C" int p3d_fp8_linear_fwd(const p3d_fp8_linear *a, const void *x, const 
   P3D_CHECK_ARG(!(a->need_dx || a->need_dw) || (a->weight && saved && ((uintptr_t)saved & 255) == 0),
                 "p3d_fp8_linear_fwd: gradients need the weight itself and 256-byte aligned room for what they keep");
   const Forward f = forward_of(*a, workspace);
-  if (!workspace || ((uintptr_t)workspace & 255) || workspace_bytes < f.bytes)
+  if (f.bytes && (!workspace || ((uintptr_t)workspace & 255) || workspace_bytes < f.bytes))
     return fail(P3D_ERR_WORKSPACE, "p3d_fp8_linear_fwd: 256-byte aligned workspace of %zu bytes, %zu needed",
                 workspace_bytes, f.bytes);
   const Saved s = saved_of(*a, saved);
-  if (int st = p3d_fp8_quantize(x, a->dtype, a->rows, a->k, 0, f.x.values, f.x.pitch, f.x.scales, s.xt.values, s.xt.pitch,
+  const bool tokens = in_product(*a);
+  if (!tokens)
+    if (int st = p3d_fp8_quantize(x, a->dtype, a->rows, a->k, 0, f.x.values, f.x.pitch, f.x.scales, s.xt.values, s.xt.pitch,
                                 s.xt.scales, nullptr, 0, nullptr, 0, stream))
-    return st;
+      return st;
   Matrix w = f.w;
   if (a->weight) {
     if (int st = p3d_fp8_quantize(a->weight, a->weight_dtype, a->n, a->k, 1, w.values, w.pitch, w.scales, s.wt.values,
@@ -128,6 +132,9 @@ extern "C" int p3d_fp8_linear_fwd(const p3d_fp8_linear *a, const void *x, const 
   } else {
     w = Matrix{a->n, a->k, a->weight_pitch, const_cast<void *>(a->weight_values), const_cast<void *>(a->weight_scales)};
   }
+  if (tokens)
+    return launch_fp8_tokens(x, a->dtype, w.values, w.pitch, w.scales, a->rows, a->n, a->k, bias, a->bias_dtype, y, a->dtype,
+                             static_cast<cudaStream_t>(stream));
   return p3d_fp8_matmul(f.x.values, f.x.pitch, f.x.scales, w.values, w.pitch, w.scales, a->rows, a->n, a->k, bias,
                         a->bias_dtype, y, a->dtype, f.sums, f.sum_bytes, stream);
 }

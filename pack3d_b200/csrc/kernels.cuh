@@ -86,6 +86,10 @@ int launch_proj_split(const ProjArgs &a, cudaStream_t stream);
 int take_proj_errors(unsigned *flags);
 int take_peer_errors(unsigned *flags);  // peer.cu
 int take_fp8_errors(unsigned *flags);   // fp8_gemm.cu
+// Up to 32 tokens x [rows, k] of x_type, quantised in the kernel, against an 8-bit weight (fp8_gemm.cu).
+bool fp8_tokens_fit(int64_t rows, int64_t cols, int64_t k);
+int launch_fp8_tokens(const void *x, int x_type, const void *b, int64_t b_pitch, const void *b_scales, int64_t rows,
+                      int64_t cols, int64_t k, const void *bias, int bias_type, void *out, int out_type, cudaStream_t s);
 int take_row_errors(unsigned *flags);   // residual.cu
 // out[c] (of dtype) = sum over i < count of partials[i, c], in a fixed order (residual.cu)
 int launch_column_join(const float *partials, void *out, int dtype, int64_t count, int dim, cudaStream_t s);

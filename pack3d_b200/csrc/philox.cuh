@@ -62,24 +62,35 @@ __device__ __forceinline__ uint4 philox(const RoundKeys &keys, uint64_t block) {
   return c;
 }
 
-// The eight keep decisions of a block as bits: element j is kept when its 16-bit field (field
-// j % 2 of word j / 2, low half first) is at least `threshold`, so the drop probability is
-// threshold / 65536.  Sixteen bits an element instead of 32 halve the rounds; the probability
-// asked for is met within 2^-17.
-template <typename Keys>
-__device__ __forceinline__ uint32_t keep_bits(const Keys &keys, uint64_t block, uint32_t threshold) {
-  const uint4 r = philox(keys, block);
-  uint32_t bits = 0;
-  bits |= (r.x & 0xffffu) >= threshold ? 1u : 0u;
-  bits |= (r.x >> 16) >= threshold ? 2u : 0u;
-  bits |= (r.y & 0xffffu) >= threshold ? 4u : 0u;
-  bits |= (r.y >> 16) >= threshold ? 8u : 0u;
-  bits |= (r.z & 0xffffu) >= threshold ? 16u : 0u;
-  bits |= (r.z >> 16) >= threshold ? 32u : 0u;
-  bits |= (r.w & 0xffffu) >= threshold ? 64u : 0u;
-  bits |= (r.w >> 16) >= threshold ? 128u : 0u;
-  return bits;
-}
+// Element j of a block is kept when its 16-bit field (field j % 2 of word j / 2, low half first) is at least
+// `threshold`, so the drop probability is threshold / 65536.  Sixteen bits an element instead of 32 halve
+// the rounds; the probability asked for is met within 2^-17.  A field is compared in the upper half of a
+// word, where the bits below it change nothing: the high field as it lies, the low one shifted up.
+struct Keep {
+  uint32_t bound;   // threshold << 16; with threshold 65536 no word reaches it
+  bool none;        // everything is dropped
+  __device__ __forceinline__ explicit Keep(uint32_t threshold)
+      : bound(threshold >= 65536u ? 0xffffffffu : threshold << 16), none(threshold >= 65536u) {}
+  template <typename Keys>
+  __device__ __forceinline__ void words(const Keys &keys, uint64_t block, uint32_t *w) const {
+    const uint4 r = philox(keys, block);
+    w[0] = none ? 0u : r.x;
+    w[1] = none ? 0u : r.y;
+    w[2] = none ? 0u : r.z;
+    w[3] = none ? 0u : r.w;
+  }
+  __device__ __forceinline__ bool low(uint32_t word) const { return (word << 16) >= bound; }
+  __device__ __forceinline__ bool high(uint32_t word) const { return word >= bound; }
+  // The eight decisions as bits.
+  template <typename Keys>
+  __device__ __forceinline__ uint32_t bits(const Keys &keys, uint64_t block) const {
+    uint32_t w[4], b = 0;
+    words(keys, block, w);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) b |= (low(w[i]) ? 1u << (2 * i) : 0u) | (high(w[i]) ? 2u << (2 * i) : 0u);
+    return b;
+  }
+};
 
 // 1 / (1 - p) of the probability actually used; 0 when everything is dropped.
 __host__ __device__ inline float keep_scale(uint32_t threshold) {

@@ -75,20 +75,40 @@ struct Eight {
   __device__ __forceinline__ void set(int j, float f) { v[j] = from_f32<T>(f); }
 };
 
-// dim a multiple of 8 and 16-byte pointers: block b is elements [8b, 8b + 8) of the whole tensor.
+// dim a multiple of 8 and 16-byte pointers: block b is elements [8b, 8b + 8) of the whole tensor.  Bound by issue as
+// much as by HBM (about a hundred instructions a block, forty of them the rounds): the round keys come from
+// shared memory, and two blocks at a time hide the rounds' latency.
 template <typename T>
 __global__ void __launch_bounds__(256) dropout_kernel(const T *x, T *y, int64_t blocks, uint32_t threshold,
                                                       const uint64_t *rng, uint64_t seed, uint64_t offset) {
-  const PhiloxKey key = philox_key(rng, seed, offset);
+  __shared__ RoundKeys keys;
+  keys.set(philox_key(rng, seed, offset));
+  __syncthreads();
+  const Keep keep(threshold);
   const float scale = keep_scale(threshold);
   const int64_t step = (int64_t)gridDim.x * blockDim.x;
-  for (int64_t b = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; b < blocks; b += step) {
-    Eight<T> c;
-    c.load(x + b * 8);
-    const uint32_t keep = keep_bits(key, (uint64_t)b, threshold);
+  auto one = [&](int64_t b, Eight<T> &c) {
+    uint32_t w[4];
+    keep.words(keys, (uint64_t)b, w);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) c.set(j, (keep >> j & 1u) ? c[j] * scale : 0.f);
-    c.store(y + b * 8);
+    for (int j = 0; j < 8; ++j)
+      c.set(j, (j & 1 ? keep.high(w[j / 2]) : keep.low(w[j / 2])) ? c[j] * scale : 0.f);
+  };
+  int64_t b = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  for (; b + step < blocks; b += 2 * step) {
+    Eight<T> p, q;
+    p.load(x + b * 8);
+    q.load(x + (b + step) * 8);
+    one(b, p);
+    one(b + step, q);
+    p.store(y + b * 8);
+    q.store(y + (b + step) * 8);
+  }
+  if (b < blocks) {
+    Eight<T> p;
+    p.load(x + b * 8);
+    one(b, p);
+    p.store(y + b * 8);
   }
 }
 
@@ -99,6 +119,7 @@ __global__ void __launch_bounds__(256) dropout_any_kernel(const T *x, T *y, int6
                                                           uint32_t threshold, const uint64_t *rng, uint64_t seed,
                                                           uint64_t offset) {
   const PhiloxKey key = philox_key(rng, seed, offset);
+  const Keep keep(threshold);
   const float scale = keep_scale(threshold);
   const int64_t row_blocks = (dim + 7) / 8, step = (int64_t)gridDim.x * blockDim.x;
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i * 8 < total; i += step) {
@@ -110,7 +131,7 @@ __global__ void __launch_bounds__(256) dropout_any_kernel(const T *x, T *y, int6
 #pragma unroll
       for (int j = 0; j < 8; ++j) c.v[j] = e + j < total ? x[e + j] : from_f32<T>(0.f);
     int64_t row = e / dim, col = e - row * dim;
-    uint32_t keep = keep_bits(key, (uint64_t)(row * row_blocks + col / 8), threshold);
+    uint32_t bits = keep.bits(key, (uint64_t)(row * row_blocks + col / 8));
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       if (j > 0) {
@@ -118,9 +139,9 @@ __global__ void __launch_bounds__(256) dropout_any_kernel(const T *x, T *y, int6
           col = 0;
           ++row;
         }
-        if ((col & 7) == 0) keep = keep_bits(key, (uint64_t)(row * row_blocks + col / 8), threshold);
+        if ((col & 7) == 0) bits = keep.bits(key, (uint64_t)(row * row_blocks + col / 8));
       }
-      c.set(j, (keep >> (col & 7) & 1u) ? c[j] * scale : 0.f);
+      c.set(j, (bits >> (col & 7) & 1u) ? c[j] * scale : 0.f);
     }
     if (whole) c.store(y + e);
     else
@@ -345,7 +366,7 @@ extern "C" int p3d_dropout(const void *x, void *y, int dtype, int64_t rows, int6
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool aligned = aligned16(x) && aligned16(y);
   const int64_t total = rows * dim, blocks = (total + 7) / 8;
-  const unsigned grid = (unsigned)std::min<int64_t>((blocks + 255) / 256, (int64_t)info.sm_count * 8);
+  const unsigned grid = (unsigned)std::min<int64_t>((blocks + 255) / 256, (int64_t)info.sm_count * 4);
   return by_type(dtype, [&](auto t) {
     using T = decltype(t);
     const T *in = static_cast<const T *>(x);

@@ -584,39 +584,44 @@ __device__ __forceinline__ float2 slope2(float2 a, int act) {
   return fma2(mul2(a, splat(-1.f)), a, splat(1.f));
 }
 
-// Keep bits of the thread's columns of a row.  Unaligned threads own a column of each of many
-// blocks: the lanes of a row (of a warp's run of columns) make a block's bits each and pass them
-// through shared memory.
+// Keep decisions of the thread's columns of a row: aligned, its units' random words; unaligned threads own a column
+// of each of many blocks, so the lanes of a row (of a warp's run of columns) make a block's decisions
+// each and pass them through shared memory as bits.
 template <bool ALIGNED, int NU, int LANES>
-__device__ __forceinline__ uint32_t row_keep(const Args &a, const Place &q, const RoundKeys &key, int64_t row,
-                                             uint8_t *shared) {
-  const p3d_residual &p = a.p;
-  const uint64_t row_block = (uint64_t)row * (uint32_t)((p.dim + 7) / 8) + (uint32_t)(q.first / 8);
-  uint32_t bits = 0;
-  if constexpr (ALIGNED) {
+struct RowKeep {
+  uint32_t w[ALIGNED ? 4 * NU : 1];
+
+  __device__ __forceinline__ void draw(const Args &a, const Place &q, const Keep &keep, const RoundKeys &key, int64_t row,
+                                       uint8_t *shared) {
+    const uint64_t row_block = (uint64_t)row * (uint32_t)((a.p.dim + 7) / 8) + (uint32_t)(q.first / 8);
+    if constexpr (ALIGNED) {
 #pragma unroll
-    for (int n = 0; n < NU; ++n) bits |= keep_bits(key, row_block + q.at[n] / 8, p.threshold) << (8 * n);
-  } else {
-    const int lane = LANES < 32 ? q.t : q.lane, run = q.base - lane;   // the run's first column
-    shared += (LANES < 32 ? q.sub : q.warp) * LANES * NU;
-    __syncwarp();   // the row before is done with the bits
+      for (int n = 0; n < NU; ++n) keep.words(key, row_block + q.at[n] / 8, w + 4 * n);
+    } else {
+      const int lane = LANES < 32 ? q.t : q.lane, run = q.base - lane;   // the run's first column
+      shared += (LANES < 32 ? q.sub : q.warp) * LANES * NU;
+      __syncwarp();   // the row before is done with the bits
 #pragma unroll
-    for (int n = 0; n < NU; ++n) {
-      const int b = lane + n * LANES;
-      if (run + 8 * b < q.end) shared[b] = (uint8_t)keep_bits(key, row_block + run / 8 + b, p.threshold);
-    }
-    __syncwarp();
+      for (int n = 0; n < NU; ++n) {
+        const int b = lane + n * LANES;
+        if (run + 8 * b < q.end) shared[b] = (uint8_t)keep.bits(key, row_block + run / 8 + b);
+      }
+      __syncwarp();
+      w[0] = 0;
 #pragma unroll
-    for (int j = 0; j < kUnit * NU; ++j) {
-      const int c = lane + j * LANES;
-      if (j < q.count) bits |= ((uint32_t)(shared[c >> 3] >> (c & 7)) & 1u) << j;
+      for (int j = 0; j < kUnit * NU; ++j) {
+        const int c = lane + j * LANES;
+        if (j < q.count) w[0] |= ((uint32_t)(shared[c >> 3] >> (c & 7)) & 1u) << j;
+      }
     }
   }
-  return bits;
-}
-__device__ __forceinline__ float2 kept(uint32_t keep, int i, float2 v) {
-  return make_float2((keep >> (2 * i) & 1u) ? v.x : 0.f, (keep >> (2 * i + 1) & 1u) ? v.y : 0.f);
-}
+  // v with what is dropped of columns 2 i and 2 i + 1 set to zero
+  __device__ __forceinline__ float2 operator()(const Keep &keep, int i, float2 v) const {
+    const bool lo = ALIGNED ? keep.low(w[ALIGNED ? i : 0]) : (w[0] >> (2 * i) & 1u);
+    const bool hi = ALIGNED ? keep.high(w[ALIGNED ? i : 0]) : (w[0] >> (2 * i + 1) & 1u);
+    return make_float2(lo ? v.x : 0.f, hi ? v.y : 0.f);
+  }
+};
 
 // (mean, 1/deviation) of a row
 template <bool ALIGNED, bool CENTER, int NU, int LANES>
@@ -654,6 +659,7 @@ __global__ void __launch_bounds__(256, NU == 1 ? 4 : 2) fwd_kernel(const __grid_
   auto ring = start_ring<T, ALIGNED, NU, false>(
       a, q, &s, s_data + (size_t)2 * param_count(BLOCK, CENTER) * NU * q.threads * sizeof(float4), cta, ctas);
   stage_params<ALIGNED, BLOCK, CENTER, NU, LANES>(params, a, q, 1.f);
+  const Keep keep(p.threshold);
   const float drop_scale = DROP ? keep_scale(p.threshold) : 1.f, inv_dim = 1.f / (float)q.dim;
   const int gate_mode = p.gate_mode;
   const bool post_norm = WHOLE || p.post_kind != P3D_NORM_NONE, next_norm = WHOLE || p.next_kind != P3D_NORM_NONE;
@@ -701,7 +707,8 @@ __global__ void __launch_bounds__(256, NU == 1 ? 4 : 2) fwd_kernel(const __grid_
           for (int j = 0; j < 4 * NU; ++j) u[j] = mul2(u[j], activate2<T>(g[j], p.gate_act));
         }
         if constexpr (DROP) {
-          const uint32_t keep = row_keep<ALIGNED, NU, LANES>(a, q, s.keys, row, s.keep + q.group * a.row_threads * NU);
+          RowKeep<ALIGNED, NU, LANES> kept;
+          kept.draw(a, q, keep, s.keys, row, s.keep + q.group * a.row_threads * NU);
 #pragma unroll
           for (int j = 0; j < 4 * NU; ++j) u[j] = kept(keep, j, mul2(u[j], splat(drop_scale)));
         }
@@ -789,6 +796,7 @@ __global__ void __launch_bounds__(512, BLOCK ? 1 : 2) bwd_kernel(const __grid_co
       a, q, &s, s_data + (size_t)2 * param_count(BLOCK, CENTER) * a.row_threads * sizeof(float4), cta, ctas);
   float *joins = reinterpret_cast<float *>(ring.data + (size_t)(a.groups - q.group) * a.stages * a.stage_bytes);
   // the dropout's scale is folded into the post norm's weight and bias, and into their gradients' sums at the end
+  const Keep keep(p.threshold);
   const float drop_scale = DROP ? keep_scale(p.threshold) : 1.f;
   stage_params<ALIGNED, BLOCK, CENTER, 1, 32>(params, a, q, drop_scale);
   const float inv_dim = 1.f / (float)q.dim;
@@ -820,10 +828,10 @@ __global__ void __launch_bounds__(512, BLOCK ? 1 : 2) bwd_kernel(const __grid_co
         const int64_t row = row0 + i, base = row * q.dim + q.first;
         const float4 st = ring.stats(a, at, i);   // mean, 1/deviation of h, then of out
         float2 w[4], u[4], hn[4], act[4], zn[4], G[4];
-        uint32_t keep = 0xffu;
+        RowKeep<ALIGNED, 1, 32> kept;
         if constexpr (BLOCK) {
           load_cols<T, ALIGNED, 1, 32>(hn, ring.row_ptr(a, q, at, kH, row0, n, i), q);
-          if constexpr (DROP) keep = row_keep<ALIGNED, 1, 32>(a, q, s.keys, row, s.keep + q.group * a.row_threads);
+          if constexpr (DROP) kept.draw(a, q, keep, s.keys, row, s.keep + q.group * a.row_threads);
           if constexpr (kGated) {
             if (token) {
               act[0] = splat(activate<T>(to_f32<T>(static_cast<const T *>(p.gate)[row]), p.gate_act));
