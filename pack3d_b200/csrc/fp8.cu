@@ -31,28 +31,192 @@ struct QuantArgs {
   float *sums;             // [row tiles, cols] partial column sums
 };
 
-// 1 x 128 blocks along the rows: sixteen lanes a block, eight elements each; a CTA has sixteen rows and walks
-// their blocks from blockIdx.y on.
+// 1 x 128 blocks along the rows: sixteen lanes a block, eight elements each; a CTA takes sixteen rows and sixteen more
+// gridDim.x groups further on, so that two loads are on their way, and walks their blocks from blockIdx.y on.
 template <typename T, bool ALIGNED>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const QuantArgs a) {
   const int blocks = (int)((a.cols + kBlock - 1) / kBlock), groups = (blocks + 3) / 4;
   const int sub = threadIdx.x & 15;
-  const int64_t row = (int64_t)blockIdx.x * 16 + threadIdx.x / 16;
-  const bool inside = row < a.rows;
-  const T *x = static_cast<const T *>(a.x) + row * a.cols;
-  uint8_t *q = a.q + row * a.pitch;
-#pragma unroll 2
-  for (int b = blockIdx.y; b < blocks; b += gridDim.y) {
-    const int64_t col = (int64_t)b * kBlock + sub * 8;
-    const Raw<T> r = load8<T, ALIGNED>(x, inside ? col : a.cols, a.cols);
+  const int64_t step = (int64_t)gridDim.x * 16;
+  auto write = [&](const Raw<T> &r, int64_t row, int b, int64_t col) {
     bool odd;
     const uint32_t byte = scale_byte(block_amax<T>(r, &odd));
-    if (inside) {
+    if (row < a.rows) {
       const float inv = inverse_scale(byte);
-      if (col < a.pitch) *reinterpret_cast<uint2 *>(q + col) = odd ? quantize8<true, T>(r, inv) : quantize8<false, T>(r, inv);
+      if (col < a.pitch)
+        *reinterpret_cast<uint2 *>(a.q + row * a.pitch + col) = odd ? quantize8<true, T>(r, inv) : quantize8<false, T>(r, inv);
       if (sub == 0) a.scales[scale_at(row, b, groups)] = (uint8_t)byte;
     }
+  };
+  // the loop is the same for the whole CTA: the shuffles take whole warps
+  for (int64_t r0 = (int64_t)blockIdx.x * 16; r0 < a.rows; r0 += 2 * step) {
+    const int64_t row = r0 + threadIdx.x / 16, next = row + step;
+    for (int b = blockIdx.y; b < blocks; b += gridDim.y) {
+      const int64_t col = (int64_t)b * kBlock + sub * 8;
+      const Raw<T> u = load8<T, ALIGNED>(static_cast<const T *>(a.x) + row * a.cols, row < a.rows ? col : a.cols, a.cols);
+      const Raw<T> v = load8<T, ALIGNED>(static_cast<const T *>(a.x) + next * a.cols, next < a.rows ? col : a.cols, a.cols);
+      write(u, row, b, col);
+      if (r0 + step < a.rows) write(v, next, b, col);
+    }
   }
+}
+
+// What follows the loads of a tile.  CHECK: the tile has infinities.  FULL: all its rows and columns exist.
+template <typename T, bool SQUARE, bool CHECK, bool FULL>
+__device__ __forceinline__ void quantize_loaded(const QuantArgs &a, const Raw<T> (&v)[8], const uint32_t (&largest)[8],
+                                                T *tile, uint32_t (&s_max)[4][kBlock], float (&s_sum)[4][kBlock]) {
+  constexpr int kPitch = kBlock + 16 / sizeof(T);
+  const int64_t k0 = (int64_t)blockIdx.x * kBlock, m0 = (int64_t)blockIdx.y * kBlock;
+  const int tid = threadIdx.x, sub = tid & 15, r0 = tid / 16;
+  uint32_t all = 0;
+  if constexpr (SQUARE) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) all = max(all, CHECK ? finite_largest8<T>(v[i]) : widest<T>(largest[i]));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) all = max(all, __shfl_xor_sync(0xffffffffu, all, o));
+    if ((tid & 31) == 0) s_max[0][tid / 32] = all;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 8; ++w) all = max(all, s_max[0][w]);
+  }
+  if (a.q) {
+    uint32_t byte[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      uint32_t m = all;
+      if constexpr (!SQUARE) {
+        m = CHECK ? finite_largest8<T>(v[i]) : largest[i];
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) {
+          const uint32_t other = __shfl_xor_sync(0xffffffffu, m, o);
+          m = CHECK ? max(m, other) : larger<T>(m, other);
+        }
+        if constexpr (!CHECK) m = widest<T>(m);
+      }
+      byte[i] = scale_byte(m);
+    }
+    const int64_t col = k0 + sub * 8;
+    uint8_t *q = a.q + (m0 + r0) * a.pitch + col;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (FULL || (m0 + r0 + 16 * i < a.rows && col < a.pitch))
+        *reinterpret_cast<uint2 *>(q + 16 * i * a.pitch) = quantize8<CHECK, T>(v[i], inverse_scale(byte[i]));
+    if (sub == 0) {   // rows r0 + 16 i, r0 < 16: 256 bytes on for odd i, four for every second i (see scale_at)
+      uint8_t *to = a.scales + scale_at(m0 + r0, blockIdx.x, ((a.cols + kBlock - 1) / kBlock + 3) / 4);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (FULL || m0 + r0 + 16 * i < a.rows) to[(i & 1) * 256 + (i >> 1) * 4] = (uint8_t)byte[i];
+    }
+  }
+  if (!a.qt && !a.sums) return;
+  // a pair of columns and a quarter of the rows a thread: x[r] is row r's pair
+  const int c = (tid & 63) * 2, quarter = tid / 64;
+  const T *from = tile + quarter * 32 * kPitch + c;
+  constexpr int kPair = sizeof(T) / 2;   // words of a pair
+  uint32_t x[32 * kPair], m0w = 0, m1w = 0;   // 16 bits: both columns' magnitudes share m0w
+#pragma unroll
+  for (int r = 0; r < 32; ++r) {
+    if constexpr (kPair == 1) {
+      x[r] = *reinterpret_cast<const uint32_t *>(from + r * kPitch);
+      m0w = larger<T>(m0w, x[r]);
+    } else {
+      const uint2 w = *reinterpret_cast<const uint2 *>(from + r * kPitch);
+      x[2 * r] = w.x;
+      x[2 * r + 1] = w.y;
+      m0w = larger<T>(m0w, w.x);
+      m1w = larger<T>(m1w, w.y);
+    }
+  }
+  auto pair = [&](int r) {
+    if constexpr (kPair == 1) return unpack2<T>(x[r]);
+    else return make_float2(__uint_as_float(x[2 * r]), __uint_as_float(x[2 * r + 1]));
+  };
+  if (a.sums) {
+    float2 s = pair(0);
+#pragma unroll
+    for (int r = 1; r < 32; ++r) s = sm100::add2(s, pair(r));
+    *reinterpret_cast<float2 *>(&s_sum[quarter][c]) = s;
+  }
+  if constexpr (!SQUARE) {
+    uint2 m;
+    if constexpr (CHECK) {
+      m = make_uint2(0u, 0u);
+#pragma unroll
+      for (int r = 0; r < 32; ++r) {
+        const float2 f = pair(r);
+        m.x = max(m.x, finite_bits(f.x));
+        m.y = max(m.y, finite_bits(f.y));
+      }
+    } else if constexpr (kPair == 1) {
+      m = make_uint2(widest<T>(m0w & 0x7fffu), widest<T>(m0w >> 16 & 0x7fffu));
+    } else {
+      m = make_uint2(widest<T>(m0w), widest<T>(m1w));
+    }
+    *reinterpret_cast<uint2 *>(&s_max[quarter][c]) = m;
+  }
+  __syncthreads();
+  if (a.sums && tid < kBlock && k0 + tid < a.cols)
+    a.sums[(int64_t)blockIdx.y * a.cols + k0 + tid] = s_sum[0][tid] + s_sum[1][tid] + s_sum[2][tid] + s_sum[3][tid];
+  if (!a.qt) return;
+  uint32_t byte[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    if constexpr (!SQUARE) all = max(max(s_max[0][c + h], s_max[1][c + h]), max(s_max[2][c + h], s_max[3][c + h]));
+    byte[h] = scale_byte(all);
+  }
+  if (quarter == 0) {   // rows c and c + 1 of the transposed matrix: sixteen bytes apart (c is even)
+    uint8_t *to = a.t_scales + scale_at(k0 + c, blockIdx.y, ((a.rows + kBlock - 1) / kBlock + 3) / 4);
+    if (FULL || k0 + c < a.cols) to[0] = (uint8_t)byte[0];
+    if (FULL || k0 + c + 1 < a.cols) to[16] = (uint8_t)byte[1];
+  }
+  const float2 inv = make_float2(inverse_scale(byte[0]), inverse_scale(byte[1]));
+  // over the tile, whose values are in registers now: the transposed bytes, rows of 144 bytes apart, from which
+  // whole 128-byte lines go out (16 bytes at a row's pitch would touch as many half sectors)
+  constexpr int kOut = kBlock + 16;
+  uint8_t *out = reinterpret_cast<uint8_t *>(tile);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {   // sixteen rows: sixteen bytes of either column
+    uint32_t w[2][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint32_t h[2][2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const float2 p = pair(16 * i + 4 * j + 2 * k), n = pair(16 * i + 4 * j + 2 * k + 1);
+        h[0][k] = to_e4m3x2<CHECK>(make_float2(p.x, n.x), inv.x);
+        h[1][k] = to_e4m3x2<CHECK>(make_float2(p.y, n.y), inv.y);
+      }
+      w[0][j] = __byte_perm(h[0][0], h[0][1], 0x5410);
+      w[1][j] = __byte_perm(h[1][0], h[1][1], 0x5410);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      *reinterpret_cast<uint4 *>(out + (c + h) * kOut + quarter * 32 + i * 16) = make_uint4(w[h][0], w[h][1], w[h][2], w[h][3]);
+  }
+  __syncthreads();
+  const int piece = (tid & 7) * 16;
+  uint8_t *qt = a.qt + k0 * a.t_pitch + m0 + piece;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int col = tid / 8 + 32 * i;
+    if (FULL || (k0 + col < a.cols && m0 + piece < a.t_pitch))
+      *reinterpret_cast<uint4 *>(qt + (int64_t)col * a.t_pitch) = *reinterpret_cast<const uint4 *>(out + col * kOut + piece);
+  }
+}
+
+// A tile with infinities: its values are read again, so that the kernel's own path keeps its registers.
+template <typename T, bool SQUARE>
+__device__ __noinline__ void quantize_odd(const QuantArgs &a, T *tile, uint32_t (&s_max)[4][kBlock],
+                                          float (&s_sum)[4][kBlock]) {
+  const int64_t m0 = (int64_t)blockIdx.y * kBlock + threadIdx.x / 16, col = (int64_t)blockIdx.x * kBlock + (threadIdx.x & 15) * 8;
+  Raw<T> v[8];
+  const uint32_t none[8] = {};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int64_t row = m0 + 16 * i;
+    v[i] = load8<T, false>(static_cast<const T *>(a.x) + row * a.cols, row < a.rows ? col : a.cols, a.cols);
+  }
+  quantize_loaded<T, SQUARE, true, false>(a, v, none, tile, s_max, s_sum);
 }
 
 // One 128 x 128 tile a CTA, read once.  Row output: 1 x 128 blocks, or the whole tile as one block
@@ -63,156 +227,33 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 2) quantize_tile_ker
   constexpr int kPitch = kBlock + 16 / sizeof(T);   // 16 bytes past 128 values: rows start on other banks
   extern __shared__ __align__(16) unsigned char s_raw[];
   T *tile = reinterpret_cast<T *>(s_raw);
-  __shared__ uint32_t s_max[4][kBlock];
-  __shared__ float s_sum[4][kBlock];
+  __shared__ __align__(16) uint32_t s_max[4][kBlock];
+  __shared__ __align__(16) float s_sum[4][kBlock];
   const int64_t k0 = (int64_t)blockIdx.x * kBlock, m0 = (int64_t)blockIdx.y * kBlock;
   const int tid = threadIdx.x, sub = tid & 15, r0 = tid / 16;
-  const int groups = (int)(((a.cols + kBlock - 1) / kBlock + 3) / 4);
-  const bool columns = a.qt || a.sums;
+  const bool full = m0 + kBlock <= a.rows && k0 + kBlock <= a.cols;
   Raw<T> v[8];
-  uint32_t all = 0;
+  uint32_t largest[8];
   bool odd = false;
+  const T *x = static_cast<const T *>(a.x) + (m0 + r0) * a.cols;
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    v[i] = load8<T, ALIGNED>(x + 16 * i * a.cols, full || m0 + r0 + 16 * i < a.rows ? k0 + sub * 8 : a.cols, a.cols);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const int64_t row = m0 + r0 + 16 * i;
-    v[i] = load8<T, ALIGNED>(static_cast<const T *>(a.x) + row * a.cols, row < a.rows ? k0 + sub * 8 : a.cols, a.cols);
-  }
-  if (columns) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    if (a.qt || a.sums) {
       uint4 *to = reinterpret_cast<uint4 *>(tile + (r0 + 16 * i) * kPitch + sub * 8);
 #pragma unroll
       for (int j = 0; j < Raw<T>::kWords / 4; ++j)
         to[j] = make_uint4(v[i].w[4 * j], v[i].w[4 * j + 1], v[i].w[4 * j + 2], v[i].w[4 * j + 3]);
     }
+    largest[i] = largest8<T>(v[i]);
+    odd |= infinite<T>(largest[i]);
   }
-  if (SQUARE) {
-    uint32_t m = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) m = larger<T>(m, largest8<T>(v[i]));
-    odd = __syncthreads_or(infinite<T>(m));
-    if (odd) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) all = max(all, finite_largest8<T>(v[i]));
-    } else {
-      all = widest<T>(m);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) all = max(all, __shfl_xor_sync(0xffffffffu, all, o));
-    if ((tid & 31) == 0) s_max[0][tid / 32] = all;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < 8; ++w) all = max(all, s_max[0][w]);
-  }
-  if (a.q) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      uint32_t m = all;
-      if (!SQUARE) m = block_amax<T>(v[i], &odd);
-      const uint32_t byte = scale_byte(m);
-      const int64_t row = m0 + r0 + 16 * i, col = k0 + sub * 8;
-      if (row < a.rows) {
-        const float inv = inverse_scale(byte);
-        if (col < a.pitch)
-          *reinterpret_cast<uint2 *>(a.q + row * a.pitch + col) =
-              odd ? quantize8<true, T>(v[i], inv) : quantize8<false, T>(v[i], inv);
-        if (sub == 0) a.scales[scale_at(row, blockIdx.x, groups)] = (uint8_t)byte;
-      }
-    }
-  }
-  if (!columns) return;
-  __syncthreads();
-  // a pair of columns and a quarter of the rows a thread: x[r] is row r's pair
-  const int c = (tid & 63) * 2, quarter = tid / 64;
-  const T *from = tile + quarter * 32 * kPitch + c;
-  constexpr int kPair = sizeof(T) / 2;   // words of a pair
-  uint32_t x[32 * kPair], m0w = 0, m1w = 0;   // 16 bits: both columns' magnitudes share m0w
-  float2 s = make_float2(0.f, 0.f);
-#pragma unroll
-  for (int r = 0; r < 32; ++r) {
-    if constexpr (kPair == 1) {
-      x[r] = *reinterpret_cast<const uint32_t *>(from + r * kPitch);
-      m0w = larger<T>(m0w, magnitude<T>(x[r]));
-      if (a.sums) s = sm100::add2(s, unpack2<T>(x[r]));
-    } else {
-      const uint2 w = *reinterpret_cast<const uint2 *>(from + r * kPitch);
-      x[2 * r] = w.x;
-      x[2 * r + 1] = w.y;
-      m0w = max(m0w, magnitude<T>(w.x));
-      m1w = max(m1w, magnitude<T>(w.y));
-      if (a.sums) s = sm100::add2(s, make_float2(__uint_as_float(w.x), __uint_as_float(w.y)));
-    }
-  }
-  auto pair = [&](int r) {
-    if constexpr (kPair == 1) return unpack2<T>(x[r]);
-    else return make_float2(__uint_as_float(x[2 * r]), __uint_as_float(x[2 * r + 1]));
-  };
-  // NaN or infinities anywhere in the tile: both columns' finite magnitudes one by one
-  if (!SQUARE) odd = infinite<T>(m0w) || (kPair == 2 && infinite<T>(m1w));
-  if (!SQUARE) odd = __syncthreads_or(odd);
-  if (!SQUARE) {
-    uint32_t lo, hi;
-    if (odd) {
-      lo = hi = 0;
-#pragma unroll
-      for (int r = 0; r < 32; ++r) {
-        const float2 f = pair(r);
-        lo = max(lo, finite_bits(f.x));
-        hi = max(hi, finite_bits(f.y));
-      }
-    } else if constexpr (kPair == 1) {
-      lo = widest<T>(m0w & 0xffffu);
-      hi = widest<T>(m0w >> 16);
-    } else {
-      lo = m0w;
-      hi = m1w;
-    }
-    s_max[quarter][c] = lo;
-    s_max[quarter][c + 1] = hi;
-  }
-  if (a.sums) {
-    s_sum[quarter][c] = s.x;
-    s_sum[quarter][c + 1] = s.y;
-  }
-  __syncthreads();
-  if (a.sums && tid < kBlock && k0 + tid < a.cols)
-    a.sums[(int64_t)blockIdx.y * a.cols + k0 + tid] = s_sum[0][tid] + s_sum[1][tid] + s_sum[2][tid] + s_sum[3][tid];
-  if (!a.qt) return;
-  const int t_groups = (int)(((a.rows + kBlock - 1) / kBlock + 3) / 4);
-  uint32_t byte[2];
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    if (!SQUARE) all = max(max(s_max[0][c + h], s_max[1][c + h]), max(s_max[2][c + h], s_max[3][c + h]));
-    byte[h] = scale_byte(all);
-    if (quarter == 0 && k0 + c + h < a.cols) a.t_scales[scale_at(k0 + c + h, blockIdx.y, t_groups)] = (uint8_t)byte[h];
-  }
-  const float2 inv = make_float2(inverse_scale(byte[0]), inverse_scale(byte[1]));
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {   // sixteen rows: sixteen bytes of either column
-    uint32_t w[2][4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      uint32_t h[2][2];
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const float2 p = pair(16 * i + 4 * j + 2 * k), n = pair(16 * i + 4 * j + 2 * k + 1);
-        if (odd) {
-          h[0][k] = to_e4m3x2<true>(make_float2(p.x, n.x), inv.x);
-          h[1][k] = to_e4m3x2<true>(make_float2(p.y, n.y), inv.y);
-        } else {
-          h[0][k] = to_e4m3x2<false>(make_float2(p.x, n.x), inv.x);
-          h[1][k] = to_e4m3x2<false>(make_float2(p.y, n.y), inv.y);
-        }
-      }
-      w[0][j] = __byte_perm(h[0][0], h[0][1], 0x5410);
-      w[1][j] = __byte_perm(h[1][0], h[1][1], 0x5410);
-    }
-    const int64_t at = m0 + quarter * 32 + i * 16;
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-      if (k0 + c + h < a.cols && at < a.t_pitch)
-        *reinterpret_cast<uint4 *>(a.qt + (k0 + c + h) * a.t_pitch + at) = make_uint4(w[h][0], w[h][1], w[h][2], w[h][3]);
-  }
+  odd = __syncthreads_or(odd);   // and the tile is there
+  if (odd) quantize_odd<T, SQUARE>(a, tile, s_max, s_sum);
+  else if (full) quantize_loaded<T, SQUARE, false, true>(a, v, largest, tile, s_max, s_sum);
+  else quantize_loaded<T, SQUARE, false, false>(a, v, largest, tile, s_max, s_sum);
 }
 
 template <typename T, bool ALIGNED, bool SQUARE>
@@ -230,8 +271,8 @@ template <typename T>
 int run_quantize(const QuantArgs &a, bool square, int sms, cudaStream_t s) {
   const bool aligned = a.cols % 8 == 0 && ((uintptr_t)a.x & 15) == 0;
   if (!square && !a.qt && !a.sums) {
-    // few rows: their blocks are dealt out to more CTAs
-    const int64_t across = (a.rows + 15) / 16, blocks = (a.cols + kBlock - 1) / kBlock;
+    // as many CTAs as the SMs hold; few rows: their blocks are dealt out to more CTAs
+    const int64_t across = std::min<int64_t>((a.rows + 15) / 16, sms * 8), blocks = (a.cols + kBlock - 1) / kBlock;
     const dim3 grid((unsigned)across, (unsigned)std::min<int64_t>(blocks, std::max<int64_t>(1, sms * 8 / across)));
     if (aligned) quantize_rows_kernel<T, true><<<grid, 256, 0, s>>>(a);
     else quantize_rows_kernel<T, false><<<grid, 256, 0, s>>>(a);

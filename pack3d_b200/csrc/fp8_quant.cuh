@@ -16,23 +16,26 @@ __device__ __forceinline__ uint32_t finite_bits(float v) {
   return b < 0x7f800000u ? b : 0u;
 }
 
-// Magnitudes are compared as their bits.  Two 16-bit ones share a word; a word is `infinite` where either is
-// infinite or NaN, and then the block is gone over again with those left out.
+// Magnitudes of a block are compared two 16-bit ones at a time, NaN left out; a word is `infinite` where either half is
+// infinite (or both operands were NaN), and then the block is gone over again with infinities left out.
 template <typename T> __device__ __forceinline__ bool infinite(uint32_t m) {
   constexpr uint32_t top = std::is_same<T, __nv_bfloat16>::value ? 0x7f80u : 0x7c00u;
-  return (m & 0xffffu) >= top || (m >> 16) >= top;
+  return (m & 0x7fffu) >= top || (m >> 16 & 0x7fffu) >= top;
 }
-template <> __device__ __forceinline__ bool infinite<float>(uint32_t m) { return m >= 0x7f800000u; }
+template <> __device__ __forceinline__ bool infinite<float>(uint32_t m) { return (m & 0x7fffffffu) >= 0x7f800000u; }
 
-// The larger of two such words, half by half for 16-bit types.
+// The larger magnitude of two words, half by half for 16-bit types; the sign bits of the result mean nothing.
 template <typename T> __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
-  if constexpr (sizeof(T) == 2) return __vmaxu2(a, b);
-  else return max(a, b);
+  uint32_t r;
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) asm("max.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else if constexpr (std::is_same<T, __half>::value) asm("max.xorsign.abs.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else r = __float_as_uint(fmaxf(fabsf(__uint_as_float(a)), fabsf(__uint_as_float(b))));
+  return r;
 }
 // fp32 bits of the larger half.
 template <typename T> __device__ __forceinline__ uint32_t widest(uint32_t m) {
-  if constexpr (sizeof(T) == 4) return m;
-  const uint32_t h = max(m & 0xffffu, m >> 16);
+  if constexpr (sizeof(T) == 4) return m & 0x7fffffffu;
+  const uint32_t h = max(m & 0x7fffu, m >> 16 & 0x7fffu);
   if constexpr (std::is_same<T, __nv_bfloat16>::value) return h << 16;
   else return __float_as_uint(__half2float(__ushort_as_half((unsigned short)h)));
 }
@@ -72,13 +75,10 @@ template <typename T> __device__ __forceinline__ float value(const Raw<T> &r, in
     return j & 1 ? f.y : f.x;
   }
 }
-template <typename T> __device__ __forceinline__ uint32_t magnitude(uint32_t word) {
-  return word & (sizeof(T) == 2 ? 0x7fff7fffu : 0x7fffffffu);
-}
 template <typename T> __device__ __forceinline__ uint32_t largest8(const Raw<T> &r) {
-  uint32_t m = magnitude<T>(r.w[0]);
+  uint32_t m = larger<T>(r.w[0], r.w[1]);
 #pragma unroll
-  for (int i = 1; i < Raw<T>::kWords; ++i) m = larger<T>(m, magnitude<T>(r.w[i]));
+  for (int i = 2; i < Raw<T>::kWords; ++i) m = larger<T>(m, r.w[i]);
   return m;
 }
 template <typename T> __device__ __forceinline__ uint32_t finite_largest8(const Raw<T> &r) {   // in fp32 bits
@@ -98,7 +98,7 @@ __device__ __forceinline__ uint32_t scale_byte(uint32_t amax_bits) {
 __device__ __forceinline__ float inverse_scale(uint32_t byte) { return __uint_as_float((254u - byte) << 23); }
 
 // Two values to e4m3 (lo in the low byte).  x * inv + (x - x): the second term is 0 for finite x and
-// NaN otherwise; a block without infinities needs only the product.
+// NaN otherwise; a block without infinities needs only the product (NaN stays NaN).
 template <bool CHECK> __device__ __forceinline__ uint32_t to_e4m3x2(float2 v, float inv) {
   if constexpr (CHECK) {
     v.x = fmaf(v.x, inv, v.x - v.x);
