@@ -30,25 +30,27 @@ using rows::kUnit;
 
 constexpr int kMaxDim = 16384;   // 512 threads of four CTAs in 16 bits, 256 of eight in 32
 
-// out[row, c] = sum over k of in[row, k, c], k in order within each of eight interleaved runs, the runs
-// in order.  One CTA sums 32 columns of one row.
+// out[row, c] = sum over k of in[row, k, c], k in order within each of 32 interleaved runs, the runs in order.  One CTA
+// sums 32 columns of one row.
+constexpr int kRuns = 32;
 struct Joins {
   void *out[kSums - 1];
 };
 template <typename P>
-__global__ void __launch_bounds__(256) join_kernel(const float *in, P *single, Joins several, int64_t k_count, int dim) {
-  __shared__ float s[8][33];
+__global__ void __launch_bounds__(32 * kRuns) join_kernel(const float *in, P *single, Joins several, int64_t k_count, int dim) {
+  __shared__ float s[kRuns][33];
   P *out = single ? single + (int64_t)blockIdx.y * dim : static_cast<P *>(several.out[blockIdx.y]);
   if (out == nullptr) return;
   const int c = blockIdx.x * 32 + threadIdx.x;
   const float *src = in + (int64_t)blockIdx.y * k_count * dim;
   float v = 0.f;
   if (c < dim)
-    for (int64_t k = threadIdx.y; k < k_count; k += 8) v += src[k * dim + c];
+    for (int64_t k = threadIdx.y; k < k_count; k += kRuns) v += src[k * dim + c];
   s[threadIdx.y][threadIdx.x] = v;
   __syncthreads();
   if (threadIdx.y == 0 && c < dim) {
-    for (int i = 1; i < 8; ++i) v += s[i][threadIdx.x];
+#pragma unroll
+    for (int i = 1; i < kRuns; ++i) v += s[i][threadIdx.x];
     out[c] = from_f32<P>(v);
   }
 }
@@ -340,7 +342,7 @@ int take_row_errors(unsigned *flags) {
 }
 
 int launch_column_join(const float *partials, void *out, int dtype, int64_t count, int dim, cudaStream_t s) {
-  const dim3 grid((unsigned)((dim + 31) / 32)), block(32, 8);
+  const dim3 grid((unsigned)((dim + 31) / 32)), block(32, kRuns);
   by_type(dtype, [&](auto t) {
     using T = decltype(t);
     join_kernel<T><<<grid, block, 0, s>>>(partials, static_cast<T *>(out), Joins{}, count, dim);
@@ -463,7 +465,7 @@ extern "C" int p3d_residual_bwd(const p3d_residual *args, const void *dout, cons
       }))
     return status;
   // the column sums over the CTAs
-  const dim3 block(32, 8);
+  const dim3 block(32, kRuns);
   const unsigned tiles = (unsigned)((p.dim + 31) / 32);
   const Joins j = {{dscale, dpost_weight, dpost_bias, dnext_weight, dnext_bias}};
   if (dscale || dpost_weight || dpost_bias || dnext_weight || dnext_bias) {

@@ -573,15 +573,35 @@ __device__ __forceinline__ float activate(float g, int act) {
   if (act == P3D_ACT_TANH) return tanhf(g);
   return g;
 }
-template <typename T>
-__device__ __forceinline__ float2 activate2(float2 g, int act) {
-  return act == P3D_ACT_IDENTITY ? g : make_float2(activate<T>(g.x, act), activate<T>(g.y, act));
+// Over a thread's columns, the kind chosen once: a choice for each element would put every kind's code between the
+// others'.
+template <typename T, int N>
+__device__ __forceinline__ void activate_all(float2 (&g)[N], int act) {
+  if (act == P3D_ACT_SIGMOID) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      g[i] = make_float2(activate<T>(g[i].x, P3D_ACT_SIGMOID), activate<T>(g[i].y, P3D_ACT_SIGMOID));
+  } else if (act == P3D_ACT_TANH) {
+#pragma unroll 1
+    for (int i = 0; i < N; ++i) {
+      // one copy of the code; the array stays in registers
+      float2 v = g[0];
+#pragma unroll
+      for (int j = 0; j + 1 < N; ++j) g[j] = g[j + 1];
+      v.x = tanhf(v.x);
+      v.y = tanhf(v.y);
+      g[N - 1] = v;
+    }
+  }
 }
-// act'(gate) from act(gate)
-__device__ __forceinline__ float2 slope2(float2 a, int act) {
-  if (act == P3D_ACT_IDENTITY) return splat(1.f);
-  if (act == P3D_ACT_SIGMOID) return mul2(a, sub2(splat(1.f), a));
-  return fma2(mul2(a, splat(-1.f)), a, splat(1.f));
+// d act'(gate) from act(gate) over a thread's columns
+template <int N>
+__device__ __forceinline__ void times_slope(float2 (&d)[N], const float2 (&a)[N], int act) {
+  if (act == P3D_ACT_IDENTITY) return;
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    d[i] = mul2(d[i], act == P3D_ACT_SIGMOID ? mul2(a[i], sub2(splat(1.f), a[i]))
+                                             : fma2(mul2(a[i], splat(-1.f)), a[i], splat(1.f)));
 }
 
 // Keep decisions of the thread's columns of a row: aligned, its units' random words; unaligned threads own a column
@@ -703,8 +723,9 @@ __global__ void __launch_bounds__(256, NU == 1 ? 4 : 2) fwd_kernel(const __grid_
 #pragma unroll
           for (int j = 0; j < 4 * NU; ++j) u[j] = mul2(u[j], splat(token));
         } else if (gate_mode != P3D_GATE_NONE) {
+          activate_all<T>(g, p.gate_act);
 #pragma unroll
-          for (int j = 0; j < 4 * NU; ++j) u[j] = mul2(u[j], activate2<T>(g[j], p.gate_act));
+          for (int j = 0; j < 4 * NU; ++j) u[j] = mul2(u[j], g[j]);
         }
         if constexpr (DROP) {
           RowKeep<ALIGNED, NU, LANES> kept;
@@ -843,8 +864,7 @@ __global__ void __launch_bounds__(512, BLOCK ? 1 : 2) bwd_kernel(const __grid_co
             } else {
               load_cols<T, ALIGNED, 1, 32>(
                   act, gate_mode == P3D_GATE_SAMPLE ? sample : ring.row_ptr(a, q, at, kGate, row0, n, i), q);
-#pragma unroll
-              for (int j = 0; j < 4; ++j) act[j] = activate2<T>(act[j], p.gate_act);
+              activate_all<T>(act, p.gate_act);
             }
           }
           float2 b[4];
@@ -913,18 +933,30 @@ __global__ void __launch_bounds__(512, BLOCK ? 1 : 2) bwd_kernel(const __grid_co
           param<1>(w, params, param_slot(BLOCK, kScale), q);
           param<1>(pw, params, param_slot(BLOCK, kPostW), q);
           s0[0] = s1[0] = s2[0] = splat(0.f);
+          if constexpr (kGated) {
+            // zn is free: the gate's gradient.  u holds the dropout's scale already.
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              a_scale[j] = fma2(G[j], mul2(u[j], act[j]), a_scale[j]);
+              G[j] = mul2(G[j], w[j]);
+              zn[j] = mul2(G[j], u[j]);
+              G[j] = mul2(G[j], act[j]);
+            }
+            times_slope(zn, act, p.gate_act);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              if (GATE == kGateAny || GATE == P3D_GATE_TOKEN) s2[0] = add2(s2[0], zn[j]);
+              if (GATE == kGateAny || GATE == P3D_GATE_SAMPLE) a_gate[j] = add2(a_gate[j], zn[j]);
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              a_scale[j] = fma2(G[j], u[j], a_scale[j]);
+              G[j] = mul2(G[j], w[j]);
+            }
+          }
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            a_scale[j] = fma2(G[j], kGated ? mul2(u[j], act[j]) : u[j], a_scale[j]);
-            G[j] = mul2(G[j], w[j]);
-            if constexpr (kGated) {
-              // u holds the dropout's scale already, so this is the gate's gradient
-              const float2 dg = mul2(mul2(G[j], u[j]), slope2(act[j], p.gate_act));
-              if (GATE == kGateAny || GATE == P3D_GATE_TOKEN) s2[0] = add2(s2[0], dg);
-              if (GATE == kGateAny || GATE == P3D_GATE_SAMPLE) a_gate[j] = add2(a_gate[j], dg);
-              G[j] = mul2(G[j], act[j]);
-              if (GATE == kGateAny || GATE == P3D_GATE_ELEMENT) act[j] = dg;
-            }
             if constexpr (DROP) G[j] = kept(keep, j, G[j]);
             a_pw[j] = fma2(G[j], hn[j], a_pw[j]);
             if constexpr (CENTER) a_pb[j] = add2(a_pb[j], G[j]);
@@ -934,7 +966,7 @@ __global__ void __launch_bounds__(512, BLOCK ? 1 : 2) bwd_kernel(const __grid_co
           }
           if constexpr (GATE == kGateAny || GATE == P3D_GATE_ELEMENT) {
             if (gate_mode == P3D_GATE_ELEMENT && a.dgate)
-              store_cols<T, ALIGNED, 1, 32>(static_cast<T *>(a.dgate) + base, act, q);
+              store_cols<T, ALIGNED, 1, 32>(static_cast<T *>(a.dgate) + base, zn, q);
           }
           float m0 = 0.f, m1 = 0.f;
           if (post_norm || token) {
