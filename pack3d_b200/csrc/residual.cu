@@ -258,7 +258,7 @@ size_t lay_out(Args &a, const Shape &s, bool aligned, bool center, bool backward
   a.groups = s.groups;
   a.members = s.members;
   a.slot_count = 0;
-  for (int i = 0; i < rows::kArrays; ++i) a.slots[i] = a.in[i] ? a.slot_count++ : 0;
+  for (int i = 0; i < rows::kArrays; ++i) a.slot_count += a.in[i] ? 1 : 0;
   const size_t arrays = (size_t)std::max(1, a.slot_count), at_once = (size_t)s.rows_at_once();
   const size_t row = (size_t)std::min(a.p.dim, s.columns()) * (size_t)dtype_size(a.p.dtype);
   const Room r = room_of(s, a.p.dim, a.p.dtype, arrays, rows::param_count(a.p.h != nullptr, center), aligned, backward);
@@ -268,8 +268,14 @@ size_t lay_out(Args &a, const Shape &s, bool aligned, bool center, bool backward
   if (s.members == 1) turns = std::max<size_t>(1, std::min({8 / at_once, 2048 / (at_once * row), share / (2 * r.stage)}));
   a.batch_rows = (int)(turns * at_once);
   const size_t batch = row * a.batch_rows;
-  a.slot_bytes = (uint32_t)(aligned ? batch : (batch + 15) / 16 * 16 + 16);
-  a.stage_bytes = (uint32_t)(arrays * a.slot_bytes) + 16u * (uint32_t)a.batch_rows;
+  const uint32_t slot = (uint32_t)(aligned ? batch : (batch + 15) / 16 * 16 + 16);
+  a.stats_at = 0;
+  for (int i = 0; i < rows::kArrays; ++i)
+    if (a.in[i]) {
+      a.slots[i] = a.stats_at;
+      a.stats_at += slot;
+    }
+  a.stage_bytes = a.stats_at + 16u * (uint32_t)a.batch_rows;
   a.stages = (int)std::max<size_t>(2, std::min<size_t>(rows::kMaxStages, share / (s.groups * (size_t)a.stage_bytes)));
   return (size_t)s.groups * a.stages * a.stage_bytes + r.fixed;
 }

@@ -61,10 +61,9 @@ struct Args {
   float *partials;  // [kSums - 1][CTA slots][dim], then the sample gate's [samples][slices][dim]
   int row_threads, groups, members;
   int batch_rows, stages;
-  uint32_t slot_bytes;       // of one array's batch in the ring
-  uint32_t stage_bytes;      // of all arrays and the statistics
-  int slots[kArrays];        // ring slot of each array
-  int slot_count;
+  uint32_t stage_bytes;      // of all arrays' batches and the statistics
+  uint32_t slots[kArrays], stats_at;   // where each lies in a stage
+  int slot_count;            // arrays
   int segments, slices, segment_rows;   // the rows are `segments` runs, each cut into slices
 };
 
@@ -366,33 +365,39 @@ struct RowSum {
 };
 
 // ------------------------------------------------------------------------ the ring of row batches
-// Batches of a CTA's slice, group by group: batch b of a segment is rows [b R, (b + 1) R) of the slice.
+// The batches of a row group, in order: R = batch_rows rows from `row` on, groups * R rows apart within the CTA's slice
+// of a segment, which ends at `end`.
 struct Batches {
-  int seg, b, seg_step, per_slice, row0, row1;
-  __device__ __forceinline__ void settle(const Args &a, int group) {
-    while (seg < a.segments && b >= per_slice) {
+  int seg, row, end;
+  int first, size, seg_step, stride;   // of the group in a slice: first row, rows of the slice from there; steps
+
+  __device__ __forceinline__ void enter(const Args &a) {   // segment seg
+    row = seg * a.segment_rows + first;
+    end = row + size;
+  }
+  __device__ __forceinline__ bool valid(const Args &a) const { return seg < a.segments; }
+  __device__ __forceinline__ void next(const Args &a) {
+    row += stride;
+    if (row >= end) {
       seg += seg_step;
-      b = group;
+      if (valid(a)) enter(a);
     }
   }
-  __device__ __forceinline__ void next(const Args &a, int group) {
-    b += a.groups;
-    settle(a, group);
-  }
-  __device__ __forceinline__ int row(const Args &a) const { return seg * a.segment_rows + row0 + b * a.batch_rows; }
-  __device__ __forceinline__ int count(const Args &a) const { return min(a.batch_rows, row1 - row0 - b * a.batch_rows); }
+  __device__ __forceinline__ int count(const Args &a) const { return min(a.batch_rows, end - row); }
 };
 
 __device__ __forceinline__ Batches batches_of(const Args &a, int group, int cta, int ctas) {
   Batches k;
   const int slice = cta % a.slices;
-  k.row0 = (int)((int64_t)a.segment_rows * slice / a.slices);
-  k.row1 = (int)((int64_t)a.segment_rows * (slice + 1) / a.slices);
-  k.per_slice = (k.row1 - k.row0 + a.batch_rows - 1) / a.batch_rows;
-  k.seg = cta / a.slices;
+  const int row0 = (int)((int64_t)a.segment_rows * slice / a.slices);
+  const int row1 = (int)((int64_t)a.segment_rows * (slice + 1) / a.slices);
+  k.first = row0 + group * a.batch_rows;
+  k.size = row1 - k.first;
   k.seg_step = ctas / a.slices;
-  k.b = group;
-  if (k.per_slice <= group) k.seg = a.segments;   // no batch for this group in any segment
+  k.stride = a.groups * a.batch_rows;
+  k.seg = k.size > 0 ? cta / a.slices : a.segments;   // no batch for this group in any segment
+  k.row = k.end = 0;
+  if (k.valid(a)) k.enter(a);
   return k;
 }
 
@@ -442,8 +447,8 @@ struct Ring {
 
   // Called by the group's first warp, all of it.
   __device__ __forceinline__ void issue(const Args &a, const Place &q) {
-    if (ahead.seg >= a.segments) return;
-    const int n = ahead.count(a), row = ahead.row(a);
+    if (!ahead.valid(a)) return;
+    const int n = ahead.count(a), row = ahead.row;
     const uint32_t to = sm100::smem_u32(data) + (uint32_t)fill * a.stage_bytes, b = bars + 8u * fill;
     fill = fill + 1 == a.stages ? 0 : fill + 1;
     const int cols = max(0, min(q.threads * kUnit * NU, q.end));   // the last CTA of a row may have none
@@ -456,7 +461,7 @@ struct Ring {
 #pragma unroll
         for (int i = 0; i < kArrays; ++i)
           if (a.in[i])
-            elect_bulk_load(to + (uint32_t)a.slots[i] * a.slot_bytes, static_cast<const char *>(a.in[i]) + off, bytes, b);
+            elect_bulk_load(to + a.slots[i], static_cast<const char *>(a.in[i]) + off, bytes, b);
       }
     } else {
       uint32_t all = STATS ? 16u * n : 0u;
@@ -471,13 +476,13 @@ struct Ring {
         for (int i = 0; i < kArrays; ++i)
           if (a.in[i]) {
             const uint32_t shift = shift_of<T>(a, q, i, row);
-            elect_bulk_load(to + (uint32_t)a.slots[i] * a.slot_bytes, static_cast<const char *>(a.in[i]) + off - shift,
+            elect_bulk_load(to + a.slots[i], static_cast<const char *>(a.in[i]) + off - shift,
                             (shift + bytes + 15u) & ~15u, b);
           }
       }
     }
-    if (STATS) elect_bulk_load(to + (uint32_t)a.slot_count * a.slot_bytes, a.stats + 4 * (int64_t)row, 16u * n, b);
-    ahead.next(a, q.group);
+    if (STATS) elect_bulk_load(to + a.stats_at, a.stats + 4 * (int64_t)row, 16u * n, b);
+    ahead.next(a);
   }
   // Waits for the next batch and returns where its stage lies.
   __device__ __forceinline__ char *wait(const Args &a, const Place &q) {
@@ -492,7 +497,7 @@ struct Ring {
   // Row i of the batch of `n` rows at `row`, from the CTA's first column on.
   __device__ __forceinline__ const T *row_ptr(const Args &a, const Place &q, const char *at, int array, int row, int n,
                                               int i) const {
-    const char *slot = at + (uint32_t)a.slots[array] * a.slot_bytes;
+    const char *slot = at + a.slots[array];
     if constexpr (!ALIGNED) {
       slot += shift_of<T>(a, q, array, row);
       if (in_place(a, row, n))
@@ -501,7 +506,7 @@ struct Ring {
     return reinterpret_cast<const T *>(slot) + i * q.dim;
   }
   __device__ __forceinline__ float4 stats(const Args &a, const char *at, int i) const {
-    return reinterpret_cast<const float4 *>(at + (uint32_t)a.slot_count * a.slot_bytes)[i];
+    return reinterpret_cast<const float4 *>(at + a.stats_at)[i];
   }
 };
 
@@ -527,28 +532,35 @@ __device__ __forceinline__ Ring<T, ALIGNED, NU, STATS> start_ring(const Args &a,
 // pieces and then their second ones, so that a warp reads consecutive banks.  (In registers they would take
 // eight a vector and thread beside the column sums.)  What is not given is its neutral value;
 // `factor` multiplies the post norm's weight and bias (the backward folds the dropout's scale in).
-template <bool ALIGNED, bool BLOCK, bool CENTER, int NU, int LANES>
-__device__ __forceinline__ void stage_params(float4 *params, const Args &a, const Place &q, float factor) {
-  if (q.group == 0) {
+template <typename P, bool ALIGNED, bool BLOCK, bool CENTER, int NU, int LANES>
+__device__ __forceinline__ void stage_params_of(float4 *params, const Args &a, const Place &q, float factor) {
 #pragma unroll
-    for (int k = 0; k < kParams; ++k) {
-      if (!BLOCK && k != kNextW && k != kNextB) continue;
-      if (!CENTER && (k == kPostB || k == kNextB)) continue;
+  for (int k = 0; k < kParams; ++k) {
+    if (!BLOCK && k != kNextW && k != kNextB) continue;
+    if (!CENTER && (k == kPostB || k == kNextB)) continue;
+    float2 f[4 * NU];
+    if (a.params[k]) {   // all of a vector's loads at once
+      load_cols<P, ALIGNED, NU, LANES>(f, static_cast<const P *>(a.params[k]) + q.first, q);
+    } else {
       const float fill = k == kScale ? a.p.scale_value : k == kPostB || k == kNextB ? 0.f : 1.f;
-      const float mul = k == kPostW || k == kPostB ? factor : 1.f;
 #pragma unroll
-      for (int n = 0; n < NU; ++n) {
-        float f[kUnit];
-#pragma unroll
-        for (int j = 0; j < kUnit; ++j) {
-          const int c = q.col<ALIGNED, LANES>(8 * n + j);
-          f[j] = !a.params[k] ? fill * mul : c < q.end ? mul * load_any(a.params[k], a.p.param_dtype, q.first + c) : 0.f;
-        }
-        float4 *to = params + 2 * (param_slot(BLOCK, k) * NU + n) * q.threads + q.t;
-        to[0] = make_float4(f[0], f[1], f[2], f[3]);
-        to[q.threads] = make_float4(f[4], f[5], f[6], f[7]);
-      }
+      for (int i = 0; i < 4 * NU; ++i) f[i] = splat(fill);
     }
+    const float mul = k == kPostW || k == kPostB ? factor : 1.f;
+#pragma unroll
+    for (int n = 0; n < NU; ++n) {
+      const float2 *v = f + 4 * n;
+      float4 *to = params + 2 * (param_slot(BLOCK, k) * NU + n) * q.threads + q.t;
+      to[0] = make_float4(v[0].x * mul, v[0].y * mul, v[1].x * mul, v[1].y * mul);
+      to[q.threads] = make_float4(v[2].x * mul, v[2].y * mul, v[3].x * mul, v[3].y * mul);
+    }
+  }
+}
+template <typename T, bool ALIGNED, bool BLOCK, bool CENTER, int NU, int LANES>
+__device__ __forceinline__ void stage_params(float4 *params, const Args &a, const Place &q, float factor) {
+  if (q.group == 0 && (!ALIGNED || q.end > 0)) {   // the last CTA of a row may have no columns
+    if (sizeof(T) == 4 || a.p.param_dtype != P3D_F32) stage_params_of<T, ALIGNED, BLOCK, CENTER, NU, LANES>(params, a, q, factor);
+    else stage_params_of<float, ALIGNED, BLOCK, CENTER, NU, LANES>(params, a, q, factor);
   }
   if (a.groups > 1) __syncthreads();   // otherwise every thread reads what it wrote
 }
@@ -678,14 +690,14 @@ __global__ void __launch_bounds__(256, NU == 1 ? 4 : 2) fwd_kernel(const __grid_
   if constexpr (DROP) s.keys.set(philox_key(p.rng, p.seed, p.offset));
   auto ring = start_ring<T, ALIGNED, NU, false>(
       a, q, &s, s_data + (size_t)2 * param_count(BLOCK, CENTER) * NU * q.threads * sizeof(float4), cta, ctas);
-  stage_params<ALIGNED, BLOCK, CENTER, NU, LANES>(params, a, q, 1.f);
+  stage_params<T, ALIGNED, BLOCK, CENTER, NU, LANES>(params, a, q, 1.f);
   const Keep keep(p.threshold);
   const float drop_scale = DROP ? keep_scale(p.threshold) : 1.f, inv_dim = 1.f / (float)q.dim;
   const int gate_mode = p.gate_mode;
   const bool post_norm = WHOLE || p.post_kind != P3D_NORM_NONE, next_norm = WHOLE || p.next_kind != P3D_NORM_NONE;
-  for (Batches k = batches_of(a, q.group, cta, ctas); k.seg < a.segments; k.next(a, q.group)) {
+  for (Batches k = batches_of(a, q.group, cta, ctas); k.valid(a); k.next(a)) {
     const char *at = ring.wait(a, q);
-    const int n = k.count(a), row0 = k.row(a);
+    const int n = k.count(a), row0 = k.row;
     bool refilled = false;
     auto refill = [&] {   // every thread of the group has left the batch before
       if (!refilled && q.warp == 0) ring.issue(a, q);
@@ -819,7 +831,7 @@ __global__ void __launch_bounds__(512, BLOCK ? 1 : 2) bwd_kernel(const __grid_co
   // the dropout's scale is folded into the post norm's weight and bias, and into their gradients' sums at the end
   const Keep keep(p.threshold);
   const float drop_scale = DROP ? keep_scale(p.threshold) : 1.f;
-  stage_params<ALIGNED, BLOCK, CENTER, 1, 32>(params, a, q, drop_scale);
+  stage_params<T, ALIGNED, BLOCK, CENTER, 1, 32>(params, a, q, drop_scale);
   const float inv_dim = 1.f / (float)q.dim;
   const int gate_mode = GATE == kGateAny ? p.gate_mode : GATE;
   const bool next_sums = WHOLE || a.in[kDy], has_dout = WHOLE || a.in[kDout];
@@ -836,9 +848,9 @@ __global__ void __launch_bounds__(512, BLOCK ? 1 : 2) bwd_kernel(const __grid_co
     Batches k = first_batch;
     k.seg = seg;
 #pragma unroll 1
-    for (k.b = q.group; k.b < k.per_slice; k.b += a.groups) {
+    for (k.enter(a); k.row < k.end; k.row += k.stride) {
       const char *at = ring.wait(a, q);
-      const int n = k.count(a), row0 = k.row(a);
+      const int n = k.count(a), row0 = k.row;
       bool refilled = false;
       auto refill = [&] {
         if (!refilled && q.warp == 0) ring.issue(a, q);
