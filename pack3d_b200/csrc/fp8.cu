@@ -31,30 +31,54 @@ struct QuantArgs {
   float *sums;             // [row tiles, cols] partial column sums
 };
 
-// 1 x 128 blocks along the rows: sixteen lanes a block, eight elements each; a CTA takes sixteen rows and sixteen more
-// gridDim.x groups further on, so that two loads are on their way, and walks their blocks from blockIdx.y on.
+// 1 x 128 blocks along the rows: eight lanes a block, sixteen elements each (three steps to the block's maximum and one
+// scale for four blocks a warp); a CTA takes 32 rows and 32 more gridDim.x groups further on, so that more
+// loads are on their way, and walks their blocks from blockIdx.y on.
 template <typename T, bool ALIGNED>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const QuantArgs a) {
+  constexpr int kRowsAtOnce = 32;
   const int blocks = (int)((a.cols + kBlock - 1) / kBlock), groups = (blocks + 3) / 4;
-  const int sub = threadIdx.x & 15;
-  const int64_t step = (int64_t)gridDim.x * 16;
-  auto write = [&](const Raw<T> &r, int64_t row, int b, int64_t col) {
-    bool odd;
-    const uint32_t byte = scale_byte(block_amax<T>(r, &odd));
+  const int sub = threadIdx.x & 7;
+  const int64_t step = (int64_t)gridDim.x * kRowsAtOnce;
+  struct Pair {
+    Raw<T> r[2];
+  };
+  auto load = [&](int64_t row, int64_t col) {
+    const T *x = static_cast<const T *>(a.x) + row * a.cols;
+    Pair p;
+    p.r[0] = load8<T, ALIGNED>(x, row < a.rows ? col : a.cols, a.cols);
+    p.r[1] = load8<T, ALIGNED>(x, row < a.rows ? col + 8 : a.cols, a.cols);
+    return p;
+  };
+  auto write = [&](const Pair &p, int64_t row, int b, int64_t col) {
+    uint32_t m = larger<T>(largest8<T>(p.r[0]), largest8<T>(p.r[1]));
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) m = larger<T>(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const bool odd = __any_sync(0xffffffffu, infinite<T>(m));
+    if (odd) {
+      m = max(finite_largest8<T>(p.r[0]), finite_largest8<T>(p.r[1]));
+#pragma unroll
+      for (int o = 4; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    } else {
+      m = widest<T>(m);
+    }
+    const uint32_t byte = scale_byte(m);
     if (row < a.rows) {
       const float inv = inverse_scale(byte);
-      if (col < a.pitch)
-        *reinterpret_cast<uint2 *>(a.q + row * a.pitch + col) = odd ? quantize8<true, T>(r, inv) : quantize8<false, T>(r, inv);
+      if (col < a.pitch) {   // the pitch is whole 16-byte pieces
+        const uint2 lo = odd ? quantize8<true, T>(p.r[0], inv) : quantize8<false, T>(p.r[0], inv);
+        const uint2 hi = odd ? quantize8<true, T>(p.r[1], inv) : quantize8<false, T>(p.r[1], inv);
+        *reinterpret_cast<uint4 *>(a.q + row * a.pitch + col) = make_uint4(lo.x, lo.y, hi.x, hi.y);
+      }
       if (sub == 0) a.scales[scale_at(row, b, groups)] = (uint8_t)byte;
     }
   };
   // the loop is the same for the whole CTA: the shuffles take whole warps
-  for (int64_t r0 = (int64_t)blockIdx.x * 16; r0 < a.rows; r0 += 2 * step) {
-    const int64_t row = r0 + threadIdx.x / 16, next = row + step;
+  for (int64_t r0 = (int64_t)blockIdx.x * kRowsAtOnce; r0 < a.rows; r0 += 2 * step) {
+    const int64_t row = r0 + threadIdx.x / 8, next = row + step;
     for (int b = blockIdx.y; b < blocks; b += gridDim.y) {
-      const int64_t col = (int64_t)b * kBlock + sub * 8;
-      const Raw<T> u = load8<T, ALIGNED>(static_cast<const T *>(a.x) + row * a.cols, row < a.rows ? col : a.cols, a.cols);
-      const Raw<T> v = load8<T, ALIGNED>(static_cast<const T *>(a.x) + next * a.cols, next < a.rows ? col : a.cols, a.cols);
+      const int64_t col = (int64_t)b * kBlock + sub * 16;
+      const Pair u = load(row, col), v = load(next, col);
       write(u, row, b, col);
       if (r0 + step < a.rows) write(v, next, b, col);
     }
@@ -272,7 +296,7 @@ int run_quantize(const QuantArgs &a, bool square, int sms, cudaStream_t s) {
   const bool aligned = a.cols % 8 == 0 && ((uintptr_t)a.x & 15) == 0;
   if (!square && !a.qt && !a.sums) {
     // as many CTAs as the SMs hold; few rows: their blocks are dealt out to more CTAs
-    const int64_t across = std::min<int64_t>((a.rows + 15) / 16, sms * 8), blocks = (a.cols + kBlock - 1) / kBlock;
+    const int64_t across = std::min<int64_t>((a.rows + 31) / 32, sms * 6), blocks = (a.cols + kBlock - 1) / kBlock;
     const dim3 grid((unsigned)across, (unsigned)std::min<int64_t>(blocks, std::max<int64_t>(1, sms * 8 / across)));
     if (aligned) quantize_rows_kernel<T, true><<<grid, 256, 0, s>>>(a);
     else quantize_rows_kernel<T, false><<<grid, 256, 0, s>>>(a);
