@@ -712,7 +712,9 @@ struct Plan {
 // Up to 128 rows (tokens) are the narrow kernel's; more go to the pair kernel, with the narrower tile where that
 // makes less work of the last wave (a tile costs its columns and about 64 more for filling the
 // pipeline).  Splits: as many parts of k as fill the SMs, each of at least two 128-column slices (four for
-// a pair); the narrow kernel's are a cluster, at most eight.
+// a pair); the narrow kernel's are a cluster, at most eight.  The pair kernel's parts cost a second kernel
+// (5 us with its launch, as long as about 30 slices): they have to save more.
+constexpr int kWorthSplitting = 32;
 Plan plan_of(int64_t rows, int64_t cols, int64_t k, int sms) {
   Plan p;
   const int64_t slices = (k + kSlice - 1) / kSlice;
@@ -732,6 +734,7 @@ Plan plan_of(int64_t rows, int64_t cols, int64_t k, int sms) {
   p.tiles_n = (int)((cols + p.bn - 1) / p.bn);
   const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
   p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({slots / std::max<int64_t>(1, tiles), slices / 4, 64}));
+  if (slices - slices / p.splits < kWorthSplitting) p.splits = 1;
   return p;
 }
 
@@ -763,7 +766,8 @@ int launch_narrow(const CUtensorMap &tb, const CUtensorMap &ta, NarrowParams g, 
   g.stages = (int)std::min<size_t>(kMaxStages, (216 * 1024 - 1024 - x_bytes) / stage);
   const size_t smem = std::max(g.stages * stage + x_bytes, splits > 1 ? part : (size_t)0) + 1024;
   static size_t seen[kMaxDevices] = {};
-  if (int st = smem_optin(fp8_narrow_kernel<BN, FUSED>, smem, seen)) return st;
+  // always the same amount: calls of several threads then cannot lower each other's
+  if (int st = smem_optin(fp8_narrow_kernel<BN, FUSED>, std::max<size_t>(smem, 224 * 1024), seen)) return st;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(tiles * splits));
   cfg.blockDim = dim3(kNarrowThreads);

@@ -1048,7 +1048,8 @@ __global__ void __launch_bounds__(512, BLOCK ? 1 : 2) bwd_kernel(const __grid_co
 // ------------------------------------------------------------------------ launches
 template <typename K>
 int launch(K kernel, const Args &a, int64_t ctas, size_t smem, size_t (&seen)[kMaxDevices], cudaStream_t stream) {
-  if (int st = smem_optin(kernel, smem, seen)) return st;
+  // always the same amount: calls of several threads then cannot lower each other's
+  if (int st = smem_optin(kernel, std::max<size_t>(smem, 224 * 1024), seen)) return st;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(ctas * a.members));
   cfg.blockDim = dim3((unsigned)(a.row_threads * a.groups));
