@@ -29,6 +29,7 @@ using rows::kSums;
 using rows::kUnit;
 
 constexpr int kMaxDim = 16384;   // 512 threads of four CTAs in 16 bits, 256 of eight in 32
+constexpr int64_t kMaxRows = ((int64_t)1 << 31) - 1024;
 
 // out[row, c] = sum over k of in[row, k, c], k in order within each of 32 interleaved runs, the runs in order.  One CTA
 // sums 32 columns of one row.
@@ -298,7 +299,8 @@ int check_args(const p3d_residual *p, const char *what) {
   P3D_CHECK_ARG(p->param_dtype == p->dtype || p->param_dtype == P3D_F32,
                 "%s: parameters must be of the tensors' dtype or fp32", what);
   P3D_CHECK_ARG(p->rows >= 0, "%s: bad row count", what);
-  if (p->rows >= (int64_t)1 << 31) return fail(P3D_ERR_UNSUPPORTED, "%s: 2^31 rows or more", what);
+  // the kernels step through the rows in 32 bits, by up to kMaxGroups batches of eight
+  if (p->rows > kMaxRows) return fail(P3D_ERR_UNSUPPORTED, "%s: more than %lld rows", what, (long long)kMaxRows);
   P3D_CHECK_ARG(p->dim >= 1, "%s: dim must be positive", what);
   if (p->dim > kMaxDim) return fail(P3D_ERR_UNSUPPORTED, "%s: dim %d above %d", what, p->dim, kMaxDim);
   P3D_CHECK_ARG(p->post_kind >= P3D_NORM_NONE && p->post_kind <= P3D_NORM_LAYER && p->next_kind >= P3D_NORM_NONE &&

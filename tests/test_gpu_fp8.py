@@ -287,3 +287,19 @@ def test_refusals(cuda_device):
         fp8_matmul(x, kept)
     with pytest.raises(ValueError, match="dtype"):
         fp8_matmul(quantize(x), kept, dtype=torch.float64)
+
+
+def test_linear_offsets_past_32_bits(cuda_device):
+    """More than 2^31 outputs: the last rows are those of a call with these rows alone, in both directions."""
+    from pack3d_b200 import fp8_linear
+    m, k, n, tail = 2 ** 20 + 1000, 136, 2048, 1000
+    g = torch.Generator(device=cuda_device).manual_seed(4)
+    x = torch.empty(m, k, dtype=torch.bfloat16, device=cuda_device).normal_(generator=g).requires_grad_()
+    w = torch.randn(n, k, dtype=torch.bfloat16, device=cuda_device, generator=g)
+    y = fp8_linear(x, w)
+    dy = torch.empty_like(y).normal_(generator=g)
+    y.backward(dy)
+    last = x.detach()[-tail:].clone().requires_grad_()
+    want = fp8_linear(last, w)
+    want.backward(dy[-tail:].clone())
+    assert torch.equal(y[-tail:], want) and torch.equal(x.grad[-tail:], last.grad)

@@ -393,3 +393,24 @@ def test_refusals(cuda_device):
         residual_norm(x, x, gate=x, gate_activation="relu")
     with pytest.raises(ValueError, match="rng"):
         residual_norm(x, x, p=0.5)
+
+
+def test_offsets_past_32_bits(cuda_device):
+    """More than 2^31 elements: the last rows, forward and backward, are those of a call with these rows alone, and
+    their dropout is not that of the rows 2^31 elements before."""
+    from pack3d_b200 import NormSpec, dropout, norm
+    rows, dim, tail = 2 ** 19 + 200, 4096, 200
+    g = torch.Generator(device=cuda_device).manual_seed(3)
+    x = torch.empty(rows, dim, dtype=torch.bfloat16, device=cuda_device).normal_(generator=g).requires_grad_()
+    w = torch.randn(dim, device=cuda_device, generator=g)
+    y = norm(x, NormSpec(w))
+    dy = torch.empty_like(y).normal_(generator=g)
+    y.backward(dy)
+    last = x.detach()[-tail:].clone().requires_grad_()
+    want = norm(last, NormSpec(w))
+    want.backward(dy[-tail:].clone())
+    assert torch.equal(y[-tail:], want) and torch.equal(x.grad[-tail:], last.grad)
+    ones = x.detach().fill_(1.0)
+    kept = dropout(ones, 0.5, (5, 2)) != 0
+    same = (kept[-tail:] == kept[:tail]).float().mean().item()
+    assert abs(same - 0.5) < 5 * 0.5 / (tail * dim) ** 0.5      # five deviations of that many fair coins

@@ -47,6 +47,12 @@ def test_residual_limits_and_pointers(lib):
     assert b"next norm" in lib.p3d_last_error()
 
 
+def test_row_limit_leaves_room_for_a_step(lib):
+    """Row numbers are 32-bit in the kernels and go up to one step (under 1024 rows) past the last row."""
+    assert lib.p3d_residual_fwd(residual(rows=2 ** 31 - 1), DUMMY, DUMMY, 0, None) == 2
+    assert lib.p3d_residual_bwd_workspace(residual(rows=2 ** 31 - 1)) == 0
+
+
 def test_dropout_arguments(lib):
     assert lib.p3d_dropout(DUMMY, DUMMY, 5, 4, 64, 0, None, 0, 0, None) == 1
     assert lib.p3d_dropout(DUMMY, DUMMY, 2, -1, 64, 0, None, 0, 0, None) == 1
