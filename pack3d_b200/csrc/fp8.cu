@@ -89,10 +89,11 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const QuantArgs a) {
 
 // What follows the loads of a tile.  CHECK: the tile has infinities.  FULL: all its rows and columns exist.
 template <typename T, bool SQUARE, bool CHECK, bool FULL>
-__device__ __forceinline__ void quantize_loaded(const QuantArgs &a, const Raw<T> (&v)[8], const uint32_t (&largest)[8],
-                                                T *tile, uint32_t (&s_max)[4][kBlock], float (&s_sum)[4][kBlock]) {
+__device__ __forceinline__ void quantize_loaded(const QuantArgs &a, int tile_row, const Raw<T> (&v)[8],
+                                                const uint32_t (&largest)[8], T *tile, uint32_t (&s_max)[4][kBlock],
+                                                float (&s_sum)[4][kBlock]) {
   constexpr int kPitch = kBlock + 16 / sizeof(T);
-  const int64_t k0 = (int64_t)blockIdx.x * kBlock, m0 = (int64_t)blockIdx.y * kBlock;
+  const int64_t k0 = (int64_t)blockIdx.x * kBlock, m0 = (int64_t)tile_row * kBlock;
   const int tid = threadIdx.x, sub = tid & 15, r0 = tid / 16;
   uint32_t all = 0;
   if constexpr (SQUARE) {
@@ -182,7 +183,7 @@ __device__ __forceinline__ void quantize_loaded(const QuantArgs &a, const Raw<T>
   }
   __syncthreads();
   if (a.sums && tid < kBlock && k0 + tid < a.cols)
-    a.sums[(int64_t)blockIdx.y * a.cols + k0 + tid] = s_sum[0][tid] + s_sum[1][tid] + s_sum[2][tid] + s_sum[3][tid];
+    a.sums[(int64_t)tile_row * a.cols + k0 + tid] = s_sum[0][tid] + s_sum[1][tid] + s_sum[2][tid] + s_sum[3][tid];
   if (!a.qt) return;
   uint32_t byte[2];
 #pragma unroll
@@ -191,7 +192,7 @@ __device__ __forceinline__ void quantize_loaded(const QuantArgs &a, const Raw<T>
     byte[h] = scale_byte(all);
   }
   if (quarter == 0) {   // rows c and c + 1 of the transposed matrix: sixteen bytes apart (c is even)
-    uint8_t *to = a.t_scales + scale_at(k0 + c, blockIdx.y, ((a.rows + kBlock - 1) / kBlock + 3) / 4);
+    uint8_t *to = a.t_scales + scale_at(k0 + c, tile_row, ((a.rows + kBlock - 1) / kBlock + 3) / 4);
     if (FULL || k0 + c < a.cols) to[0] = (uint8_t)byte[0];
     if (FULL || k0 + c + 1 < a.cols) to[16] = (uint8_t)byte[1];
   }
@@ -232,9 +233,9 @@ __device__ __forceinline__ void quantize_loaded(const QuantArgs &a, const Raw<T>
 
 // A tile with infinities: its values are read again, so that the kernel's own path keeps its registers.
 template <typename T, bool SQUARE>
-__device__ __noinline__ void quantize_odd(const QuantArgs &a, T *tile, uint32_t (&s_max)[4][kBlock],
+__device__ __noinline__ void quantize_odd(const QuantArgs &a, int tile_row, T *tile, uint32_t (&s_max)[4][kBlock],
                                           float (&s_sum)[4][kBlock]) {
-  const int64_t m0 = (int64_t)blockIdx.y * kBlock + threadIdx.x / 16, col = (int64_t)blockIdx.x * kBlock + (threadIdx.x & 15) * 8;
+  const int64_t m0 = (int64_t)tile_row * kBlock + threadIdx.x / 16, col = (int64_t)blockIdx.x * kBlock + (threadIdx.x & 15) * 8;
   Raw<T> v[8];
   const uint32_t none[8] = {};
 #pragma unroll
@@ -242,20 +243,17 @@ __device__ __noinline__ void quantize_odd(const QuantArgs &a, T *tile, uint32_t 
     const int64_t row = m0 + 16 * i;
     v[i] = load8<T, false>(static_cast<const T *>(a.x) + row * a.cols, row < a.rows ? col : a.cols, a.cols);
   }
-  quantize_loaded<T, SQUARE, true, false>(a, v, none, tile, s_max, s_sum);
+  quantize_loaded<T, SQUARE, true, false>(a, tile_row, v, none, tile, s_max, s_sum);
 }
 
 // One 128 x 128 tile a CTA, read once.  Row output: 1 x 128 blocks, or the whole tile as one block
 // (SQUARE).  Transposed output: blocks of 128 rows of a column (or the same whole tile), from
 // the tile's copy in shared memory.  Column sums of the tile where asked for.
 template <typename T, bool ALIGNED, bool SQUARE>
-__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 2) quantize_tile_kernel(const QuantArgs a) {
+__device__ __forceinline__ void quantize_tile(const QuantArgs &a, int tile_row, T *tile, uint32_t (&s_max)[4][kBlock],
+                                              float (&s_sum)[4][kBlock]) {
   constexpr int kPitch = kBlock + 16 / sizeof(T);   // 16 bytes past 128 values: rows start on other banks
-  extern __shared__ __align__(16) unsigned char s_raw[];
-  T *tile = reinterpret_cast<T *>(s_raw);
-  __shared__ __align__(16) uint32_t s_max[4][kBlock];
-  __shared__ __align__(16) float s_sum[4][kBlock];
-  const int64_t k0 = (int64_t)blockIdx.x * kBlock, m0 = (int64_t)blockIdx.y * kBlock;
+  const int64_t k0 = (int64_t)blockIdx.x * kBlock, m0 = (int64_t)tile_row * kBlock;
   const int tid = threadIdx.x, sub = tid & 15, r0 = tid / 16;
   const bool full = m0 + kBlock <= a.rows && k0 + kBlock <= a.cols;
   Raw<T> v[8];
@@ -277,18 +275,37 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 2) quantize_tile_ker
     odd |= infinite<T>(largest[i]);
   }
   odd = __syncthreads_or(odd);   // and the tile is there
-  if (odd) quantize_odd<T, SQUARE>(a, tile, s_max, s_sum);
-  else if (full) quantize_loaded<T, SQUARE, false, true>(a, v, largest, tile, s_max, s_sum);
-  else quantize_loaded<T, SQUARE, false, false>(a, v, largest, tile, s_max, s_sum);
+  if (odd) quantize_odd<T, SQUARE>(a, tile_row, tile, s_max, s_sum);
+  else if (full) quantize_loaded<T, SQUARE, false, true>(a, tile_row, v, largest, tile, s_max, s_sum);
+  else quantize_loaded<T, SQUARE, false, false>(a, tile_row, v, largest, tile, s_max, s_sum);
 }
 
-template <typename T, bool ALIGNED, bool SQUARE>
-int launch_tile(const QuantArgs &a, cudaStream_t s) {
+template <typename T> constexpr size_t tile_bytes() { return (size_t)kBlock * (kBlock + 16 / sizeof(T)) * sizeof(T); }
+
+// kBoth: the first x_tiles rows of tiles are x's, with blocks along its rows, the others w's, as square blocks.
+enum : int { kRowBlocks = 0, kSquare = 1, kBoth = 2 };
+template <typename T, bool ALIGNED, int BLOCKS>
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 2)
+    quantize_tile_kernel(const __grid_constant__ QuantArgs x, const __grid_constant__ QuantArgs w, int x_tiles) {
+  extern __shared__ __align__(16) unsigned char s_raw[];
+  T *tile = reinterpret_cast<T *>(s_raw);
+  __shared__ __align__(16) uint32_t s_max[4][kBlock];
+  __shared__ __align__(16) float s_sum[4][kBlock];
+  const int tile_row = blockIdx.y;
+  if (BLOCKS == kRowBlocks || (BLOCKS == kBoth && tile_row < x_tiles))
+    quantize_tile<T, ALIGNED, false>(x, tile_row, tile, s_max, s_sum);
+  else
+    quantize_tile<T, ALIGNED, true>(w, tile_row - x_tiles, tile, s_max, s_sum);
+}
+
+// x or w may be without rows.
+template <typename T, bool ALIGNED, int BLOCKS>
+int launch_tile(const QuantArgs &x, const QuantArgs &w, cudaStream_t s) {
   static size_t seen[kMaxDevices] = {};
-  const size_t smem = (size_t)kBlock * (kBlock + 16 / sizeof(T)) * sizeof(T);
-  if (int st = smem_optin(quantize_tile_kernel<T, ALIGNED, SQUARE>, smem, seen)) return st;
-  const dim3 grid((unsigned)((a.cols + kBlock - 1) / kBlock), (unsigned)((a.rows + kBlock - 1) / kBlock));
-  quantize_tile_kernel<T, ALIGNED, SQUARE><<<grid, 256, smem, s>>>(a);
+  if (int st = smem_optin(quantize_tile_kernel<T, ALIGNED, BLOCKS>, tile_bytes<T>(), seen)) return st;
+  const int64_t x_tiles = (x.rows + kBlock - 1) / kBlock, w_tiles = (w.rows + kBlock - 1) / kBlock;
+  const dim3 grid((unsigned)((std::max(x.cols, w.cols) + kBlock - 1) / kBlock), (unsigned)(x_tiles + w_tiles));
+  quantize_tile_kernel<T, ALIGNED, BLOCKS><<<grid, 256, tile_bytes<T>(), s>>>(x, w, (int)x_tiles);
   P3D_LAUNCH_CHECK();
   return P3D_OK;
 }
@@ -305,11 +322,38 @@ int run_quantize(const QuantArgs &a, bool square, int sms, cudaStream_t s) {
     P3D_LAUNCH_CHECK();
     return P3D_OK;
   }
-  if (square) return aligned ? launch_tile<T, true, true>(a, s) : launch_tile<T, false, true>(a, s);
-  return aligned ? launch_tile<T, true, false>(a, s) : launch_tile<T, false, false>(a, s);
+  const QuantArgs none = {};
+  if (square) return aligned ? launch_tile<T, true, kSquare>(none, a, s) : launch_tile<T, false, kSquare>(none, a, s);
+  return aligned ? launch_tile<T, true, kRowBlocks>(a, none, s) : launch_tile<T, false, kRowBlocks>(a, none, s);
+}
+
+template <typename T>
+int run_both(const QuantArgs &x, const QuantArgs &w, cudaStream_t s) {
+  const bool aligned = x.cols % 8 == 0 && (((uintptr_t)x.x | (uintptr_t)w.x) & 15) == 0;
+  return aligned ? launch_tile<T, true, kBoth>(x, w, s) : launch_tile<T, false, kBoth>(x, w, s);
 }
 
 }  // namespace
+
+int launch_quantize_both(const QuantOperand &x, const QuantOperand &w, int64_t cols, int dtype, cudaStream_t s) {
+  auto args = [&](const QuantOperand &m) {
+    QuantArgs a = {};
+    a.x = m.x;
+    a.rows = m.rows;
+    a.cols = cols;
+    a.q = static_cast<uint8_t *>(m.q);
+    a.scales = static_cast<uint8_t *>(m.scales);
+    a.pitch = m.pitch;
+    a.qt = static_cast<uint8_t *>(m.qt);
+    a.t_scales = static_cast<uint8_t *>(m.t_scales);
+    a.t_pitch = m.t_pitch;
+    return a;
+  };
+  if (dtype == P3D_F32) return run_both<float>(args(x), args(w), s);
+  if (dtype == P3D_F16) return run_both<__half>(args(x), args(w), s);
+  return run_both<__nv_bfloat16>(args(x), args(w), s);
+}
+
 }  // namespace p3d
 
 using namespace p3d;

@@ -120,15 +120,23 @@ extern "C" int p3d_fp8_linear_fwd(const p3d_fp8_linear *a, const void *x, const 
                 workspace_bytes, f.bytes);
   const Saved s = saved_of(*a, saved);
   const bool tokens = in_product(*a);
-  if (!tokens)
-    if (int st = p3d_fp8_quantize(x, a->dtype, a->rows, a->k, 0, f.x.values, f.x.pitch, f.x.scales, s.xt.values, s.xt.pitch,
-                                s.xt.scales, nullptr, 0, nullptr, 0, stream))
-      return st;
   Matrix w = f.w;
-  if (a->weight) {
-    if (int st = p3d_fp8_quantize(a->weight, a->weight_dtype, a->n, a->k, 1, w.values, w.pitch, w.scales, s.wt.values,
-                                  s.wt.pitch, s.wt.scales, nullptr, 0, nullptr, 0, stream))
+  // x's transposed copy makes it a tiles' kernel like the weight's, and one launch does both
+  const bool both = a->need_dw && a->weight && a->dtype == a->weight_dtype && a->rows + a->n <= 65000LL * 128;
+  if (both) {
+    const QuantOperand qx = {x, a->rows, f.x.values, f.x.scales, f.x.pitch, s.xt.values, s.xt.scales, s.xt.pitch};
+    const QuantOperand qw = {a->weight, a->n, w.values, w.scales, w.pitch, s.wt.values, s.wt.scales, s.wt.pitch};
+    if (int st = launch_quantize_both(qx, qw, a->k, a->dtype, static_cast<cudaStream_t>(stream))) return st;
+  } else if (!tokens) {
+    if (int st = p3d_fp8_quantize(x, a->dtype, a->rows, a->k, 0, f.x.values, f.x.pitch, f.x.scales, s.xt.values, s.xt.pitch,
+                                  s.xt.scales, nullptr, 0, nullptr, 0, stream))
       return st;
+  }
+  if (a->weight) {
+    if (!both)
+      if (int st = p3d_fp8_quantize(a->weight, a->weight_dtype, a->n, a->k, 1, w.values, w.pitch, w.scales, s.wt.values,
+                                    s.wt.pitch, s.wt.scales, nullptr, 0, nullptr, 0, stream))
+        return st;
   } else {
     w = Matrix{a->n, a->k, a->weight_pitch, const_cast<void *>(a->weight_values), const_cast<void *>(a->weight_scales)};
   }

@@ -90,6 +90,17 @@ int take_fp8_errors(unsigned *flags);   // fp8_gemm.cu
 bool fp8_tokens_fit(int64_t rows, int64_t cols, int64_t k);
 int launch_fp8_tokens(const void *x, int x_type, const void *b, int64_t b_pitch, const void *b_scales, int64_t rows,
                       int64_t cols, int64_t k, const void *bias, int bias_type, void *out, int out_type, cudaStream_t s);
+// x [rows, cols] with blocks along its rows and w [rows, cols] with square ones, both of dtype, in one launch: their
+// tiles' rows together are at most 65535 (fp8.cu)
+struct QuantOperand {
+  const void *x;
+  int64_t rows;
+  void *q, *scales;     // pitch bytes a row
+  int64_t pitch;
+  void *qt, *t_scales;  // the transposed copy, or null
+  int64_t t_pitch;
+};
+int launch_quantize_both(const QuantOperand &x, const QuantOperand &w, int64_t cols, int dtype, cudaStream_t s);
 int take_row_errors(unsigned *flags);   // residual.cu
 // out[c] (of dtype) = sum over i < count of partials[i, c], in a fixed order (residual.cu)
 int launch_column_join(const float *partials, void *out, int dtype, int64_t count, int dim, cudaStream_t s);
