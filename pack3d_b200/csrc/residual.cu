@@ -466,7 +466,7 @@ extern "C" int p3d_residual_bwd(const p3d_residual *args, const void *dout, cons
   a.slices = (int)c.slices;
   a.segment_rows = (int)c.segment_rows;
   const bool aligned =
-      all_aligned(p, {dout, dy, dx, dh, p.gate_mode == P3D_GATE_ELEMENT ? (const void *)dgate : nullptr});
+      all_aligned(p, {dout, dy, dx, dh, workspace, p.gate_mode == P3D_GATE_ELEMENT ? (const void *)dgate : nullptr});
   const bool center = centred(p) || dpost_bias || dnext_bias || (aligned && !rows::whole_bwd(a));
   const size_t smem = lay_out(a, s, aligned, center, true, &per_sm);
   cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -12,12 +12,17 @@
 // bytes, and the normalised row keeps its 32 bits (the stored one is rounded to 16).  Every
 // thread keeps the column sums of its eight columns over all rows of its CTA in registers; they
 // are joined over the CTA's row groups in shared memory, written once per CTA and summed over the
-// CTAs by a second small kernel, all in a fixed order.
+// CTAs by a second small kernel, all in a fixed order.  With K the gradient of s (u act) where it was kept (times
+// the gate, where that changes from row to row), the block's gradients all come from the sums of K h~ and K: dw = s sum K
+// h~, db = s sum K, ds = w sum K h~ + b sum K and, for a sample's gate, s act' times that.  So two sums a
+// column are kept instead of four, what does not change from row to row (s, w, b, a sample's gate) is
+// multiplied once, and a sample's gate is activated once (364 -> 284 us at 524288 x 192, 120 -> 97 us at 8192 x
+// 4096).
 //
-// Measured on B200 (bf16): 524288 x 192 layer norm, sample gate and dropout, forward 185 us, backward 364 us; 8192 x
-// 4096 RMS norm, token gate, 53 and 120 us; norm by itself 16384 x 4096 51 and 82 us.  Forward at 4.4 to 5.2,
-// backward at 3.3 to 4.9 TB/s: both are bound by issue (55 % of the slots, 230 to 490 instructions a row
-// and warp) before HBM, the backward because its column sums leave room for 512 threads an SM only.
+// Measured on B200 (bf16): 524288 x 192 layer norm, sample gate and dropout, forward 185 us, backward 284 us; 8192 x
+// 4096 RMS norm, token gate, 54 and 97 us; norm by itself 16384 x 4096 51 and 82 us.  Forward at 4.4 to 5.2,
+// backward at 4.1 to 4.9 TB/s: both are bound by issue before HBM, the backward because its column sums leave
+// room for 512 threads an SM only.
 //
 // What a call does not have (a norm, a bias, a gate) is a neutral value in the same formula.  Only what
 // costs registers or many instructions is a variant of its own: whether there is a block at all,
@@ -611,6 +616,10 @@ __device__ __forceinline__ void activate_all(float2 (&g)[N], int act) {
     }
   }
 }
+// act'(gate) from act(gate)
+__device__ __forceinline__ float slope(float a, int act) {
+  return act == P3D_ACT_IDENTITY ? 1.f : act == P3D_ACT_SIGMOID ? a * (1.f - a) : fmaf(-a, a, 1.f);
+}
 // d act'(gate) from act(gate) over a thread's columns
 template <int N>
 __device__ __forceinline__ void times_slope(float2 (&d)[N], const float2 (&a)[N], int act) {
@@ -787,41 +796,71 @@ __global__ void __launch_bounds__(256, NU == 1 ? 4 : 2) fwd_kernel(const __grid_
 }
 
 // ------------------------------------------------------------------------ backward
-constexpr int kSums = 6;  // dscale, dpost_weight, dpost_bias, dnext_weight, dnext_bias, dgate
+constexpr int kSums = 6;  // written: dscale, dpost_weight, dpost_bias, dnext_weight, dnext_bias, dgate
 
-// Adds the thread's sums, times `factor`, over the CTA's row groups (in group order) and writes them to dst.
-template <bool ALIGNED>
-__device__ __forceinline__ void join_groups(float2 (&acc)[4], float factor, float *smem, float *dst, const Args &a,
-                                            const Place &q) {
-  float v[kUnit];
-#pragma unroll
-  for (int j = 0; j < kUnit; ++j) v[j] = (j & 1 ? acc[j / 2].y : acc[j / 2].x) * factor;
+// The thread's sums added over the CTA's row groups (in group order), complete in the first group; they start again at 0.
+__device__ __forceinline__ void join_groups(float2 (&acc)[4], float *smem, const Args &a, const Place &q) {
   if (a.groups > 1) {
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j < kUnit; ++j) smem[(q.group * kUnit + j) * a.row_threads + q.t] = v[j];
+    for (int j = 0; j < 4; ++j) {
+      smem[(q.group * kUnit + 2 * j) * a.row_threads + q.t] = acc[j].x;
+      smem[(q.group * kUnit + 2 * j + 1) * a.row_threads + q.t] = acc[j].y;
+    }
     __syncthreads();
     if (q.group == 0) {
 #pragma unroll
-      for (int j = 0; j < kUnit; ++j)
-        for (int g = 1; g < a.groups; ++g) v[j] += smem[(g * kUnit + j) * a.row_threads + q.t];
+      for (int j = 0; j < 4; ++j)
+        for (int g = 1; g < a.groups; ++g)
+          acc[j] = add2(acc[j], make_float2(smem[(g * kUnit + 2 * j) * a.row_threads + q.t],
+                                            smem[(g * kUnit + 2 * j + 1) * a.row_threads + q.t]));
     }
   }
-  if (q.group == 0) {
+}
+// The thread's columns of a row of sums in global memory.
+template <bool ALIGNED>
+__device__ __forceinline__ void get_sums(float2 (&v)[4], const float *src, const Place &q) {
+  if constexpr (ALIGNED) {
+    const float4 *from = reinterpret_cast<const float4 *>(src + q.first + q.at[0]);
+    const float4 x = from[0], y = from[1];
+    v[0] = make_float2(x.x, x.y);
+    v[1] = make_float2(x.z, x.w);
+    v[2] = make_float2(y.x, y.y);
+    v[3] = make_float2(y.z, y.w);
+  } else {
+    float f[kUnit];
 #pragma unroll
     for (int j = 0; j < kUnit; ++j) {
       const int c = q.col<ALIGNED, 32>(j);
-      if (c < q.end) dst[q.first + c] = v[j];
+      f[j] = c < q.end ? src[q.first + c] : 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = make_float2(f[2 * j], f[2 * j + 1]);
+  }
+}
+template <bool ALIGNED>
+__device__ __forceinline__ void put_sums(const float2 (&v)[4], float *dst, const Place &q) {
+  if constexpr (ALIGNED) {
+    float4 *to = reinterpret_cast<float4 *>(dst + q.first + q.at[0]);
+    if (q.live[0]) {
+      to[0] = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+      to[1] = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < kUnit; ++j) {
+      const int c = q.col<ALIGNED, 32>(j);
+      if (c < q.end) dst[q.first + c] = j & 1 ? v[j / 2].y : v[j / 2].x;
     }
   }
-#pragma unroll
-  for (int j = 0; j < 4; ++j) acc[j] = splat(0.f);
 }
 
 // WHOLE: both norms, both upstream gradients and both gradients of tensors are there.
 template <typename T, bool ALIGNED, bool BLOCK, bool WHOLE, int GATE, bool DROP, bool CENTER>
 __global__ void __launch_bounds__(512, BLOCK ? 1 : 2) bwd_kernel(const __grid_constant__ Args a) {
-  constexpr bool kGated = BLOCK && GATE != P3D_GATE_NONE;
+  constexpr bool kSampled = BLOCK && (GATE == kGateAny || GATE == P3D_GATE_SAMPLE);
+  constexpr bool kTokens = BLOCK && GATE == P3D_GATE_TOKEN;
+  constexpr bool kElements = BLOCK && (GATE == kGateAny || GATE == P3D_GATE_ELEMENT);   // act and v = d / act a column
   const p3d_residual &p = a.p;
   extern __shared__ __align__(128) char s_data[];
   __shared__ Shared s;
@@ -840,16 +879,39 @@ __global__ void __launch_bounds__(512, BLOCK ? 1 : 2) bwd_kernel(const __grid_co
   const float inv_dim = 1.f / (float)q.dim;
   const int gate_mode = GATE == kGateAny ? p.gate_mode : GATE;
   const bool next_sums = WHOLE || a.in[kDy], has_dout = WHOLE || a.in[kDout];
-  const bool post_norm = WHOLE || p.post_kind != P3D_NORM_NONE, token = kGated && gate_mode == P3D_GATE_TOKEN;
+  const bool post_norm = WHOLE || p.post_kind != P3D_NORM_NONE, token = (kTokens || kElements) && gate_mode == P3D_GATE_TOKEN;
   const bool want_dx = WHOLE || a.dx, want_dh = WHOLE || a.dh;
   // means of the normalised rows' gradients: nothing to take off where there is no norm, no mean in an RMS norm
   const float next_mean = p.next_kind == P3D_NORM_LAYER ? -inv_dim : 0.f;
   const float post_mean = p.post_kind == P3D_NORM_LAYER ? -inv_dim : 0.f, post_dot = post_norm ? -inv_dim : 0.f;
-  float2 a_scale[4] = {}, a_pw[4] = {}, a_pb[4] = {}, a_nw[4] = {}, a_nb[4] = {}, a_gate[4] = {};
+  // K: the gradient of d = s (u act) where it was kept, and a gate's part of it that changes from row to row
+  float2 a_kh[4] = {}, a_k[4] = {}, a_nw[4] = {}, a_nb[4] = {};   // sums of K h~, K, dy z~, dy
+  float *const mine = a.partials + (int64_t)cta * q.dim;
+  const int64_t one_sum = (int64_t)ctas * q.dim;
   const Batches first_batch = batches_of(a, q.group, cta, ctas);
 #pragma unroll 1
   for (int seg = cta / a.slices; seg < a.segments; seg += first_batch.seg_step) {
     const T *const sample = static_cast<const T *>(p.gate) + (int64_t)seg * q.dim + q.first;
+    // d of a row is h~ e_w + e_b, times a gate that changes from row to row
+    float2 e_w[4], e_b[4];
+    if constexpr (BLOCK) {
+      float2 f[4];
+      param<1>(e_w, params, param_slot(BLOCK, kPostW), q);
+      if constexpr (CENTER) param<1>(e_b, params, param_slot(BLOCK, kPostB), q);
+      param<1>(f, params, param_slot(BLOCK, kScale), q);
+      if (kSampled && gate_mode == P3D_GATE_SAMPLE) {
+        float2 g[4];
+        load_cols<T, ALIGNED, 1, 32>(g, sample, q);
+        activate_all<T>(g, p.gate_act);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[j] = mul2(f[j], g[j]);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        e_w[j] = mul2(e_w[j], f[j]);
+        if constexpr (CENTER) e_b[j] = mul2(e_b[j], f[j]);
+      }
+    }
     Batches k = first_batch;
     k.seg = seg;
 #pragma unroll 1
@@ -865,37 +927,30 @@ __global__ void __launch_bounds__(512, BLOCK ? 1 : 2) bwd_kernel(const __grid_co
       for (int i = 0; i < n; ++i) {
         const int64_t row = row0 + i, base = row * q.dim + q.first;
         const float4 st = ring.stats(a, at, i);   // mean, 1/deviation of h, then of out
-        float2 w[4], u[4], hn[4], act[4], zn[4], G[4];
+        float2 w[4], v[4], hn[4], act[4], zn[4], G[4];
+        float gate = 1.f;   // the token's
         RowKeep<ALIGNED, 1, 32> kept;
         if constexpr (BLOCK) {
           load_cols<T, ALIGNED, 1, 32>(hn, ring.row_ptr(a, q, at, kH, row0, n, i), q);
           if constexpr (DROP) kept.draw(a, q, keep, s.keys, row, s.keep + q.group * a.row_threads);
-          if constexpr (kGated) {
-            if (token) {
-              act[0] = splat(activate<T>(to_f32<T>(static_cast<const T *>(p.gate)[row]), p.gate_act));
-#pragma unroll
-              for (int j = 1; j < 4; ++j) act[j] = act[0];
-            } else if (gate_mode == P3D_GATE_NONE) {   // only where the mode is an argument
-#pragma unroll
-              for (int j = 0; j < 4; ++j) act[j] = splat(1.f);
-            } else {
-              load_cols<T, ALIGNED, 1, 32>(
-                  act, gate_mode == P3D_GATE_SAMPLE ? sample : ring.row_ptr(a, q, at, kGate, row0, n, i), q);
+          if (token) gate = activate<T>(to_f32<T>(static_cast<const T *>(p.gate)[row]), p.gate_act);
+          if constexpr (kElements) {
+            if (gate_mode == P3D_GATE_ELEMENT) {
+              load_cols<T, ALIGNED, 1, 32>(act, ring.row_ptr(a, q, at, kGate, row0, n, i), q);
               activate_all<T>(act, p.gate_act);
+            } else {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) act[j] = splat(gate);
             }
           }
-          float2 b[4];
-          param<1>(w, params, param_slot(BLOCK, kPostW), q);
-          if constexpr (CENTER) param<1>(b, params, param_slot(BLOCK, kPostB), q);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             if constexpr (CENTER) hn[j] = sub2(hn[j], splat(st.x));
             hn[j] = mul2(hn[j], splat(st.y));      // h itself without a post norm: mean 0, 1/deviation 1
-            u[j] = CENTER ? fma2(hn[j], w[j], b[j]) : mul2(hn[j], w[j]);
-            if constexpr (DROP) u[j] = kept(keep, j, u[j]);
+            v[j] = CENTER ? fma2(hn[j], e_w[j], e_b[j]) : mul2(hn[j], e_w[j]);
+            if constexpr (DROP) v[j] = kept(keep, j, v[j]);
           }
         }
-        // u: the block's output with its dropout, before the gate; d = u act
         if (has_dout) load_cols<T, ALIGNED, 1, 32>(G, ring.row_ptr(a, q, at, kDout, row0, n, i), q);
         else
 #pragma unroll
@@ -905,9 +960,9 @@ __global__ void __launch_bounds__(512, BLOCK ? 1 : 2) bwd_kernel(const __grid_co
           load_cols<T, ALIGNED, 1, 32>(zn, ring.row_ptr(a, q, at, kX, row0, n, i), q);
           load_cols<T, ALIGNED, 1, 32>(gy, ring.row_ptr(a, q, at, kDy, row0, n, i), q);
           if constexpr (BLOCK) {
-            param<1>(w, params, param_slot(BLOCK, kScale), q);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) zn[j] = fma2(w[j], kGated ? mul2(u[j], act[j]) : u[j], zn[j]);
+            for (int j = 0; j < 4; ++j)
+              zn[j] = kElements ? fma2(v[j], act[j], zn[j]) : kTokens ? fma2(v[j], splat(gate), zn[j]) : add2(v[j], zn[j]);
           }
           param<1>(w, params, param_slot(BLOCK, kNextW), q);
           s0[0] = s1[0] = splat(0.f);
@@ -946,58 +1001,45 @@ __global__ void __launch_bounds__(512, BLOCK ? 1 : 2) bwd_kernel(const __grid_co
         }
         if (want_dx) store_cols<T, ALIGNED, 1, 32>(static_cast<T *>(a.dx) + base, G, q);
         if constexpr (BLOCK) {
-          float2 s0[1], s1[1], s2[1], pw[4];
-          param<1>(w, params, param_slot(BLOCK, kScale), q);
-          param<1>(pw, params, param_slot(BLOCK, kPostW), q);
+          float2 s0[1], s1[1], s2[1];
           s0[0] = s1[0] = s2[0] = splat(0.f);
-          if constexpr (kGated) {
-            // zn is free: the gate's gradient.  u holds the dropout's scale already.
+          if constexpr (kElements) {   // zn is free: the gate's gradient
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              a_scale[j] = fma2(G[j], mul2(u[j], act[j]), a_scale[j]);
-              G[j] = mul2(G[j], w[j]);
-              zn[j] = mul2(G[j], u[j]);
+              zn[j] = mul2(G[j], v[j]);
               G[j] = mul2(G[j], act[j]);
             }
             times_slope(zn, act, p.gate_act);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              if (GATE == kGateAny || GATE == P3D_GATE_TOKEN) s2[0] = add2(s2[0], zn[j]);
-              if (GATE == kGateAny || GATE == P3D_GATE_SAMPLE) a_gate[j] = add2(a_gate[j], zn[j]);
-            }
-          } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              a_scale[j] = fma2(G[j], u[j], a_scale[j]);
-              G[j] = mul2(G[j], w[j]);
-            }
-          }
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if constexpr (DROP) G[j] = kept(keep, j, G[j]);
-            a_pw[j] = fma2(G[j], hn[j], a_pw[j]);
-            if constexpr (CENTER) a_pb[j] = add2(a_pb[j], G[j]);
-            G[j] = mul2(G[j], pw[j]);
-            s1[0] = fma2(G[j], hn[j], s1[0]);
-            if constexpr (CENTER) s0[0] = add2(s0[0], G[j]);
-          }
-          if constexpr (GATE == kGateAny || GATE == P3D_GATE_ELEMENT) {
             if (gate_mode == P3D_GATE_ELEMENT && a.dgate)
               store_cols<T, ALIGNED, 1, 32>(static_cast<T *>(a.dgate) + base, zn, q);
           }
+          // G becomes K e_w (a token's gate left out until the end)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if constexpr (DROP) G[j] = kept(keep, j, G[j]);
+            const float2 K = kTokens ? mul2(G[j], splat(gate)) : G[j];
+            a_kh[j] = fma2(K, hn[j], a_kh[j]);
+            if constexpr (CENTER) a_k[j] = add2(a_k[j], K);
+            if constexpr (GATE == kGateAny) s2[0] = add2(s2[0], zn[j]);
+            if constexpr (kTokens && CENTER) s2[0] = fma2(G[j], e_b[j], s2[0]);
+            G[j] = mul2(G[j], e_w[j]);
+            s1[0] = fma2(G[j], hn[j], s1[0]);
+            if constexpr (CENTER) s0[0] = add2(s0[0], G[j]);
+          }
           float m0 = 0.f, m1 = 0.f;
           if (post_norm || token) {
-            if constexpr (GATE == P3D_GATE_TOKEN && !CENTER) {
-              float v[2] = {total<ALIGNED, 1>(q, s1), total<ALIGNED, 1>(q, s2)};
-              sum(q, v);
-              m1 = v[0] * post_dot;
-              if (a.dgate && q.t == 0 && q.rank == 0) static_cast<T *>(a.dgate)[row] = from_f32<T>(v[1]);
-            } else if constexpr (GATE == kGateAny || GATE == P3D_GATE_TOKEN) {
+            float dgate = 0.f;   // the token's: the sum of G v is that of G e_w h~ and of G e_b
+            if constexpr (CENTER && (GATE == kGateAny || kTokens)) {
               float v[3] = {total<ALIGNED, 1>(q, s1), total<ALIGNED, 1>(q, s0), total<ALIGNED, 1>(q, s2)};
               sum(q, v);
               m1 = v[0] * post_dot;
               m0 = v[1] * post_mean;
-              if (token && a.dgate && q.t == 0 && q.rank == 0) static_cast<T *>(a.dgate)[row] = from_f32<T>(v[2]);
+              dgate = kTokens ? (v[0] + v[2]) * slope(gate, p.gate_act) : v[2];
+            } else if constexpr (GATE == kGateAny) {
+              float v[2] = {total<ALIGNED, 1>(q, s1), total<ALIGNED, 1>(q, s2)};
+              sum(q, v);
+              m1 = v[0] * post_dot;
+              dgate = v[1];
             } else if constexpr (CENTER) {
               float v[2] = {total<ALIGNED, 1>(q, s1), total<ALIGNED, 1>(q, s0)};
               sum(q, v);
@@ -1007,7 +1049,9 @@ __global__ void __launch_bounds__(512, BLOCK ? 1 : 2) bwd_kernel(const __grid_co
               float v[1] = {total<ALIGNED, 1>(q, s1)};
               sum(q, v);
               m1 = v[0] * post_dot;
+              if constexpr (kTokens) dgate = v[0] * slope(gate, p.gate_act);
             }
+            if (token && a.dgate && q.t == 0 && q.rank == 0) static_cast<T *>(a.dgate)[row] = from_f32<T>(dgate);
             refill();
           }
           if (want_dh) {
@@ -1015,7 +1059,7 @@ __global__ void __launch_bounds__(512, BLOCK ? 1 : 2) bwd_kernel(const __grid_co
             for (int j = 0; j < 4; ++j) {
               G[j] = fma2(hn[j], splat(m1), G[j]);
               if constexpr (CENTER) G[j] = add2(G[j], splat(m0));
-              G[j] = mul2(G[j], splat(st.y));
+              G[j] = mul2(G[j], splat(kTokens ? st.y * gate : st.y));
             }
             store_cols<T, ALIGNED, 1, 32>(static_cast<T *>(a.dh) + base, G, q);
           }
@@ -1026,23 +1070,66 @@ __global__ void __launch_bounds__(512, BLOCK ? 1 : 2) bwd_kernel(const __grid_co
         refill();
       }
     }
-    if constexpr (GATE == kGateAny || GATE == P3D_GATE_SAMPLE) {
-      if (gate_mode == P3D_GATE_SAMPLE && a.dgate)
-        join_groups<ALIGNED>(a_gate, 1.f, joins,
-                             a.partials + ((int64_t)(kSums - 1) * ctas + (int64_t)seg * a.slices + cta % a.slices) * q.dim,
-                             a, q);
+    // The block's gradients from the two sums: with A = w sum K h~ + b sum K (the sum of K u), dscale = A, dw = s sum
+    // K h~, db = s sum K.  A sample's gate is not in K: dgate = s A act', and the others times act.
+    if constexpr (BLOCK) {
+      // what the CTA's samples before have summed up to, on its way while the groups are joined
+      float2 was[3][4] = {};
+      if (kSampled && seg != cta / a.slices && q.group == 0 && q.end > 0) {
+#pragma unroll
+        for (int i = 0; i < (CENTER ? 3 : 2); ++i) get_sums<ALIGNED>(was[i], mine + i * one_sum, q);
+      }
+      join_groups(a_kh, joins, a, q);
+      if constexpr (CENTER) join_groups(a_k, joins, a, q);
+      if (q.group == 0) {
+        const bool sampled = kSampled && gate_mode == P3D_GATE_SAMPLE;
+        float2 w[4], f[4], A[4];
+        param<1>(w, params, param_slot(BLOCK, kPostW), q);
+        param<1>(f, params, param_slot(BLOCK, kScale), q);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) A[j] = mul2(w[j], a_kh[j]);
+        if constexpr (CENTER) {
+          param<1>(w, params, param_slot(BLOCK, kPostB), q);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) A[j] = fma2(w[j], a_k[j], A[j]);
+        }
+        if (sampled) {
+          float2 g[4], dgate[4];
+          load_cols<T, ALIGNED, 1, 32>(g, sample, q);
+          activate_all<T>(g, p.gate_act);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            dgate[j] = mul2(f[j], A[j]);
+            A[j] = mul2(A[j], g[j]);
+            f[j] = mul2(f[j], g[j]);
+          }
+          times_slope(dgate, g, p.gate_act);
+          if (a.dgate)
+            put_sums<ALIGNED>(dgate, a.partials + (kSums - 1) * one_sum + ((int64_t)seg * a.slices + cta % a.slices) * q.dim,
+                              q);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          f[j] = mul2(f[j], splat(drop_scale));
+          A[j] = add2(was[0][j], A[j]);
+          a_kh[j] = fma2(a_kh[j], f[j], was[1][j]);
+          if constexpr (CENTER) a_k[j] = fma2(a_k[j], f[j], was[2][j]);
+        }
+        // the slots of sums that a variant does not have are not read either
+        put_sums<ALIGNED>(A, mine, q);
+        put_sums<ALIGNED>(a_kh, mine + one_sum, q);
+        if constexpr (CENTER) put_sums<ALIGNED>(a_k, mine + 2 * one_sum, q);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) a_kh[j] = a_k[j] = splat(0.f);
     }
   }
-  // the slots of sums that this variant does not have are not read either
-  float *const mine = a.partials + (int64_t)cta * q.dim;
-  const int64_t next = (int64_t)ctas * q.dim;
-  if constexpr (BLOCK) {
-    join_groups<ALIGNED>(a_scale, 1.f, joins, mine, a, q);
-    join_groups<ALIGNED>(a_pw, drop_scale, joins, mine + next, a, q);
-    if constexpr (CENTER) join_groups<ALIGNED>(a_pb, drop_scale, joins, mine + 2 * next, a, q);
+  join_groups(a_nw, joins, a, q);
+  if (q.group == 0) put_sums<ALIGNED>(a_nw, mine + 3 * one_sum, q);
+  if constexpr (CENTER) {
+    join_groups(a_nb, joins, a, q);
+    if (q.group == 0) put_sums<ALIGNED>(a_nb, mine + 4 * one_sum, q);
   }
-  join_groups<ALIGNED>(a_nw, 1.f, joins, mine + 3 * next, a, q);
-  if constexpr (CENTER) join_groups<ALIGNED>(a_nb, 1.f, joins, mine + 4 * next, a, q);
 }
 
 // ------------------------------------------------------------------------ launches
