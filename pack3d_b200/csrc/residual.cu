@@ -29,6 +29,7 @@ using rows::kSums;
 using rows::kUnit;
 
 constexpr int kMaxDim = 16384;   // 512 threads of four CTAs in 16 bits, 256 of eight in 32
+constexpr int kFoldRows = 8;
 constexpr int64_t kMaxRows = ((int64_t)1 << 31) - 1024;
 
 // out[row, c] = sum over k of in[row, k, c], k in order within each of 32 interleaved runs, the runs in order.  One CTA
@@ -164,7 +165,7 @@ bool aligned16(const void *ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15u
 //   Forward: up to 384 columns a warp holds several rows, on 8 or 16 lanes with one or three units each, so that
 //   sums take three or four steps for all of them and the bookkeeping is shared; wider rows take two
 //   units a thread and up to 256 threads.  (524288 x 192 bf16 with dropout: one row a warp 388 us,
-//   four rows 223 us; 185 us since with leaner bookkeeping.)
+//   four rows 223 us; 163 us since with leaner bookkeeping and the gate folded into the parameters.)
 //   Backward: a row a warp at least and one unit, whose column sums fill the registers already.  At most 512
 //   threads a row, 256 in 32 bits, where two stages of five arrays of 4096 columns would not fit
 //   beside the parameters.
@@ -415,7 +416,14 @@ extern "C" int p3d_residual_fwd(const p3d_residual *args, void *out, void *y, fl
   const bool center = centred(p) || (aligned && !rows::whole_fwd(a));
   int per_sm = per_sm_of(p, s, false);
   const size_t smem = lay_out(a, s, aligned, center, false, &per_sm);
-  const Split c = split_of(p, s, info.sm_count, per_sm, false);
+  Split c = split_of(p, s, info.sm_count, per_sm, false);
+  if (p.gate_mode == P3D_GATE_SAMPLE) {
+    // a CTA that has many rows of a sample (kFoldRows a group) sets that sample's parameters up, else the gate is
+    // read and activated for each row
+    const Split by_sample = split_of(p, s, info.sm_count, per_sm, true);
+    a.gate_folded = by_sample.segment_rows / by_sample.slices >= (int64_t)kFoldRows * s.groups * s.rows_at_once();
+    if (a.gate_folded) c = by_sample;
+  }
   a.segments = (int)c.segments;
   a.slices = (int)c.slices;
   a.segment_rows = (int)c.segment_rows;

@@ -19,8 +19,8 @@
 // multiplied once, and a sample's gate is activated once (364 -> 284 us at 524288 x 192, 120 -> 97 us at 8192 x
 // 4096).
 //
-// Measured on B200 (bf16): 524288 x 192 layer norm, sample gate and dropout, forward 185 us, backward 284 us; 8192 x
-// 4096 RMS norm, token gate, 54 and 97 us; norm by itself 16384 x 4096 51 and 82 us.  Forward at 4.4 to 5.2,
+// Measured on B200 (bf16): 524288 x 192 layer norm, sample gate and dropout, forward 163 us, backward 287 us; 8192 x
+// 4096 RMS norm, token gate, 53 and 99 us; norm by itself 16384 x 4096 50 and 80 us.  Forward at 4.9 to 5.4,
 // backward at 4.1 to 4.9 TB/s: both are bound by issue before HBM, the backward because its column sums leave
 // room for 512 threads an SM only.
 //
@@ -75,6 +75,7 @@ struct Args {
   uint32_t slots[kArrays], stats_at;   // where each lies in a stage
   int slot_count;            // arrays
   int segments, slices, segment_rows;   // the rows are `segments` runs, each cut into slices
+  bool gate_folded;          // forward: the segments are samples, whose gate is multiplied into the parameters
 };
 
 __device__ __forceinline__ float2 splat(float v) { return make_float2(v, v); }
@@ -538,55 +539,6 @@ __device__ __forceinline__ Ring<T, ALIGNED, NU, STATS> start_ring(const Args &a,
   return r;
 }
 
-// The parameters' columns of each thread in fp32, in shared memory: two 16-byte pieces a unit, all threads' first
-// pieces and then their second ones, so that a warp reads consecutive banks.  (In registers they would take
-// eight a vector and thread beside the column sums.)  What is not given is its neutral value;
-// `factor` multiplies the post norm's weight and bias (the backward folds the dropout's scale in).
-template <typename P, bool ALIGNED, bool BLOCK, bool CENTER, int NU, int LANES>
-__device__ __forceinline__ void stage_params_of(float4 *params, const Args &a, const Place &q, float factor) {
-#pragma unroll
-  for (int k = 0; k < kParams; ++k) {
-    if (!BLOCK && k != kNextW && k != kNextB) continue;
-    if (!CENTER && (k == kPostB || k == kNextB)) continue;
-    float2 f[4 * NU];
-    if (a.params[k]) {   // all of a vector's loads at once
-      load_cols<P, ALIGNED, NU, LANES>(f, static_cast<const P *>(a.params[k]) + q.first, q);
-    } else {
-      const float fill = k == kScale ? a.p.scale_value : k == kPostB || k == kNextB ? 0.f : 1.f;
-#pragma unroll
-      for (int i = 0; i < 4 * NU; ++i) f[i] = splat(fill);
-    }
-    const float mul = k == kPostW || k == kPostB ? factor : 1.f;
-#pragma unroll
-    for (int n = 0; n < NU; ++n) {
-      const float2 *v = f + 4 * n;
-      float4 *to = params + 2 * (param_slot(BLOCK, k) * NU + n) * q.threads + q.t;
-      to[0] = make_float4(v[0].x * mul, v[0].y * mul, v[1].x * mul, v[1].y * mul);
-      to[q.threads] = make_float4(v[2].x * mul, v[2].y * mul, v[3].x * mul, v[3].y * mul);
-    }
-  }
-}
-template <typename T, bool ALIGNED, bool BLOCK, bool CENTER, int NU, int LANES>
-__device__ __forceinline__ void stage_params(float4 *params, const Args &a, const Place &q, float factor) {
-  if (q.group == 0 && (!ALIGNED || q.end > 0)) {   // the last CTA of a row may have no columns
-    if (sizeof(T) == 4 || a.p.param_dtype != P3D_F32) stage_params_of<T, ALIGNED, BLOCK, CENTER, NU, LANES>(params, a, q, factor);
-    else stage_params_of<float, ALIGNED, BLOCK, CENTER, NU, LANES>(params, a, q, factor);
-  }
-  if (a.groups > 1) __syncthreads();   // otherwise every thread reads what it wrote
-}
-template <int NU>   // k: the vector's place
-__device__ __forceinline__ void param(float2 (&f)[4 * NU], const float4 *params, int k, const Place &q) {
-#pragma unroll
-  for (int n = 0; n < NU; ++n) {
-    const float4 *from = params + 2 * (k * NU + n) * q.threads + q.t;
-    const float4 x = from[0], y = from[q.threads];
-    f[4 * n] = make_float2(x.x, x.y);
-    f[4 * n + 1] = make_float2(x.z, x.w);
-    f[4 * n + 2] = make_float2(y.x, y.y);
-    f[4 * n + 3] = make_float2(y.z, y.w);
-  }
-}
-
 // ------------------------------------------------------------------------ pieces of the formula
 // 16-bit types take the sigmoid's exponential from the fast unit (a few 2^-22 off, against their 2^-9).
 template <typename T>
@@ -616,6 +568,79 @@ __device__ __forceinline__ void activate_all(float2 (&g)[N], int act) {
     }
   }
 }
+// The parameters' columns of each thread in fp32, in shared memory: two 16-byte pieces a unit, all threads' first
+// pieces and then their second ones, so that a warp reads consecutive banks.  (In registers they would take
+// eight a vector and thread beside the column sums.)  What is not given is its neutral value;
+// `factor`, the dropout's scale, multiplies the post norm's weight and bias; FOLD (the forward): so do the residual's
+// scale, which then has no place of its own, and a sample's gate.
+template <typename P, typename T, bool ALIGNED, bool BLOCK, bool CENTER, bool FOLD, int NU, int LANES>
+__device__ __forceinline__ void stage_params_of(float4 *params, const Args &a, const Place &q, float factor, const T *gate) {
+  float2 fold[4 * NU];
+#pragma unroll
+  for (int i = 0; i < 4 * NU; ++i) fold[i] = splat(factor);
+  if constexpr (FOLD) {
+    if (a.params[kScale]) load_cols<P, ALIGNED, NU, LANES>(fold, static_cast<const P *>(a.params[kScale]) + q.first, q);
+    const float mul = a.params[kScale] ? factor : factor * a.p.scale_value;
+#pragma unroll
+    for (int i = 0; i < 4 * NU; ++i) fold[i] = a.params[kScale] ? mul2(fold[i], splat(mul)) : splat(mul);
+    if (gate) {
+      float2 g[4 * NU];
+      load_cols<T, ALIGNED, NU, LANES>(g, gate + q.first, q);
+      activate_all<T>(g, a.p.gate_act);
+#pragma unroll
+      for (int i = 0; i < 4 * NU; ++i) fold[i] = mul2(fold[i], g[i]);
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < kParams; ++k) {
+    if (!BLOCK && k != kNextW && k != kNextB) continue;
+    if (!CENTER && (k == kPostB || k == kNextB)) continue;
+    if (FOLD && k == kScale) continue;
+    float2 f[4 * NU];
+    if (a.params[k]) {   // all of a vector's loads at once
+      load_cols<P, ALIGNED, NU, LANES>(f, static_cast<const P *>(a.params[k]) + q.first, q);
+    } else {
+      const float fill = k == kScale ? a.p.scale_value : k == kPostB || k == kNextB ? 0.f : 1.f;
+#pragma unroll
+      for (int i = 0; i < 4 * NU; ++i) f[i] = splat(fill);
+    }
+    if (k == kPostW || k == kPostB) {
+#pragma unroll
+      for (int i = 0; i < 4 * NU; ++i) f[i] = mul2(f[i], fold[i]);
+    }
+#pragma unroll
+    for (int n = 0; n < NU; ++n) {
+      const float2 *v = f + 4 * n;
+      float4 *to = params + 2 * (param_slot(BLOCK, k) * NU + n) * q.threads + q.t;
+      to[0] = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+      to[q.threads] = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);
+    }
+  }
+}
+template <typename T, bool ALIGNED, bool BLOCK, bool CENTER, bool FOLD, int NU, int LANES>
+__device__ __forceinline__ void stage_params(float4 *params, const Args &a, const Place &q, float factor,
+                                             const T *gate = nullptr) {
+  if (q.group == 0 && (!ALIGNED || q.end > 0)) {   // the last CTA of a row may have no columns
+    if (sizeof(T) == 4 || a.p.param_dtype != P3D_F32)
+      stage_params_of<T, T, ALIGNED, BLOCK, CENTER, FOLD, NU, LANES>(params, a, q, factor, gate);
+    else
+      stage_params_of<float, T, ALIGNED, BLOCK, CENTER, FOLD, NU, LANES>(params, a, q, factor, gate);
+  }
+  if (a.groups > 1) __syncthreads();   // otherwise every thread reads what it wrote
+}
+template <int NU>   // k: the vector's place
+__device__ __forceinline__ void param(float2 (&f)[4 * NU], const float4 *params, int k, const Place &q) {
+#pragma unroll
+  for (int n = 0; n < NU; ++n) {
+    const float4 *from = params + 2 * (k * NU + n) * q.threads + q.t;
+    const float4 x = from[0], y = from[q.threads];
+    f[4 * n] = make_float2(x.x, x.y);
+    f[4 * n + 1] = make_float2(x.z, x.w);
+    f[4 * n + 2] = make_float2(y.x, y.y);
+    f[4 * n + 3] = make_float2(y.z, y.w);
+  }
+}
+
 // act'(gate) from act(gate)
 __device__ __forceinline__ float slope(float a, int act) {
   return act == P3D_ACT_IDENTITY ? 1.f : act == P3D_ACT_SIGMOID ? a * (1.f - a) : fmaf(-a, a, 1.f);
@@ -704,39 +729,50 @@ __global__ void __launch_bounds__(256, NU == 1 ? 4 : 2) fwd_kernel(const __grid_
   if constexpr (DROP) s.keys.set(philox_key(p.rng, p.seed, p.offset));
   auto ring = start_ring<T, ALIGNED, NU, false>(
       a, q, &s, s_data + (size_t)2 * param_count(BLOCK, CENTER) * NU * q.threads * sizeof(float4), cta, ctas);
-  stage_params<T, ALIGNED, BLOCK, CENTER, NU, LANES>(params, a, q, 1.f);
   const Keep keep(p.threshold);
   const float drop_scale = DROP ? keep_scale(p.threshold) : 1.f, inv_dim = 1.f / (float)q.dim;
-  const int gate_mode = p.gate_mode;
+  const bool folded = BLOCK && a.gate_folded;   // the segments are samples, whose gate the parameters hold
+  const int gate_mode = folded ? P3D_GATE_NONE : p.gate_mode;
   const bool post_norm = WHOLE || p.post_kind != P3D_NORM_NONE, next_norm = WHOLE || p.next_kind != P3D_NORM_NONE;
-  for (Batches k = batches_of(a, q.group, cta, ctas); k.valid(a); k.next(a)) {
-    const char *at = ring.wait(a, q);
-    const int n = k.count(a), row0 = k.row;
-    bool refilled = false;
-    auto refill = [&] {   // every thread of the group has left the batch before
-      if (!refilled && q.warp == 0) ring.issue(a, q);
-      refilled = true;
-    };
+  const Batches first_batch = batches_of(a, q.group, cta, ctas);
 #pragma unroll 1
-    for (int i0 = 0; i0 < n; i0 += kRows) {
-      // past the batch's end a lane group goes over its last row again, without storing
-      const bool valid = LANES == 32 || i0 + q.sub < n;
-      const int i = LANES == 32 ? i0 : min(i0 + q.sub, n - 1);
-      const int64_t row = row0 + i, base = row * q.dim + q.first;
-      float2 z[4 * NU], w[4 * NU], b[4 * NU];
-      float2 post = make_float2(0.f, 1.f), next = make_float2(0.f, 1.f);
-      if constexpr (BLOCK) {
-        float2 u[4 * NU], g[4 * NU];
-        load_cols<T, ALIGNED, NU, LANES>(u, ring.row_ptr(a, q, at, kH, row0, n, i), q);
-        if (gate_mode == P3D_GATE_ELEMENT) load_cols<T, ALIGNED, NU, LANES>(g, ring.row_ptr(a, q, at, kGate, row0, n, i), q);
-        if (gate_mode == P3D_GATE_SAMPLE)
-          load_cols<T, ALIGNED, NU, LANES>(
-              g, static_cast<const T *>(p.gate) + (int64_t)((int)row / (int)p.rows_per_sample) * q.dim + q.first, q);
-        float token = 1.f;
-        if (gate_mode == P3D_GATE_TOKEN) token = activate<T>(to_f32<T>(static_cast<const T *>(p.gate)[row]), p.gate_act);
-        if (post_norm) {
-          post = row_stats<ALIGNED, CENTER, NU>(sum, q, u, p.post_kind, p.post_eps, inv_dim);
-          refill();
+  for (int seg = cta / a.slices; seg < a.segments; seg += first_batch.seg_step) {
+    if (a.groups > 1 && seg != cta / a.slices) __syncthreads();   // the groups are done with the sample before
+    stage_params<T, ALIGNED, BLOCK, CENTER, BLOCK, NU, LANES>(
+        params, a, q, drop_scale, folded ? static_cast<const T *>(p.gate) + (int64_t)seg * q.dim : nullptr);
+    Batches k = first_batch;
+    k.seg = seg;
+#pragma unroll 1
+    for (k.enter(a); k.row < k.end; k.row += k.stride) {
+      const char *at = ring.wait(a, q);
+      const int n = k.count(a), row0 = k.row;
+      bool refilled = false;
+      auto refill = [&] {   // every thread of the group has left the batch before
+        if (!refilled && q.warp == 0) ring.issue(a, q);
+        refilled = true;
+      };
+#pragma unroll 1
+      for (int i0 = 0; i0 < n; i0 += kRows) {
+        // past the batch's end a lane group goes over its last row again, without storing
+        const bool valid = LANES == 32 || i0 + q.sub < n;
+        const int i = LANES == 32 ? i0 : min(i0 + q.sub, n - 1);
+        const int64_t row = row0 + i, base = row * q.dim + q.first;
+        float2 z[4 * NU], w[4 * NU], b[4 * NU];
+        float2 post = make_float2(0.f, 1.f), next = make_float2(0.f, 1.f);
+        if constexpr (BLOCK) {
+          float2 u[4 * NU], g[4 * NU];
+          load_cols<T, ALIGNED, NU, LANES>(u, ring.row_ptr(a, q, at, kH, row0, n, i), q);
+          if (gate_mode == P3D_GATE_ELEMENT) load_cols<T, ALIGNED, NU, LANES>(g, ring.row_ptr(a, q, at, kGate, row0, n, i), q);
+          if (gate_mode == P3D_GATE_SAMPLE)
+            load_cols<T, ALIGNED, NU, LANES>(
+                g, static_cast<const T *>(p.gate) + (int64_t)((int)row / (int)p.rows_per_sample) * q.dim + q.first, q);
+          float token = 1.f;
+          if (gate_mode == P3D_GATE_TOKEN) token = activate<T>(to_f32<T>(static_cast<const T *>(p.gate)[row]), p.gate_act);
+          if (post_norm) {
+            post = row_stats<ALIGNED, CENTER, NU>(sum, q, u, p.post_kind, p.post_eps, inv_dim);
+            refill();
+          }
+          // without a post norm u itself: mean 0, 1/deviation 1
           param<NU>(w, params, param_slot(BLOCK, kPostW), q);
           if constexpr (CENTER) param<NU>(b, params, param_slot(BLOCK, kPostB), q);
 #pragma unroll
@@ -744,53 +780,52 @@ __global__ void __launch_bounds__(256, NU == 1 ? 4 : 2) fwd_kernel(const __grid_
             if constexpr (CENTER) u[j] = fma2(mul2(sub2(u[j], splat(post.x)), splat(post.y)), w[j], b[j]);
             else u[j] = mul2(mul2(u[j], splat(post.y)), w[j]);
           }
-        }
-        if (gate_mode == P3D_GATE_TOKEN) {
+          if (gate_mode == P3D_GATE_TOKEN) {
 #pragma unroll
-          for (int j = 0; j < 4 * NU; ++j) u[j] = mul2(u[j], splat(token));
-        } else if (gate_mode != P3D_GATE_NONE) {
-          activate_all<T>(g, p.gate_act);
+            for (int j = 0; j < 4 * NU; ++j) u[j] = mul2(u[j], splat(token));
+          } else if (gate_mode != P3D_GATE_NONE) {
+            activate_all<T>(g, p.gate_act);
 #pragma unroll
-          for (int j = 0; j < 4 * NU; ++j) u[j] = mul2(u[j], g[j]);
-        }
-        if constexpr (DROP) {
-          RowKeep<ALIGNED, NU, LANES> kept;
-          kept.draw(a, q, keep, s.keys, row, s.keep + q.group * a.row_threads * NU);
-#pragma unroll
-          for (int j = 0; j < 4 * NU; ++j) u[j] = kept(keep, j, mul2(u[j], splat(drop_scale)));
-        }
-        param<NU>(w, params, param_slot(BLOCK, kScale), q);
-        load_cols<T, ALIGNED, NU, LANES>(z, ring.row_ptr(a, q, at, kX, row0, n, i), q);
-#pragma unroll
-        for (int j = 0; j < 4 * NU; ++j) {
-          z[j] = fma2(w[j], u[j], z[j]);
-          if constexpr (!ALIGNED) {
-            if (2 * j >= q.count) z[j].x = 0.f;
-            if (2 * j + 1 >= q.count) z[j].y = 0.f;
+            for (int j = 0; j < 4 * NU; ++j) u[j] = mul2(u[j], g[j]);
           }
-        }
-        store_cols<T, ALIGNED, NU, LANES>(static_cast<T *>(a.out) + base, z, q, valid);
-      } else {
-        load_cols<T, ALIGNED, NU, LANES>(z, ring.row_ptr(a, q, at, kX, row0, n, i), q);
-      }
-      if (next_norm) {
-        next = row_stats<ALIGNED, CENTER, NU>(sum, q, z, p.next_kind, p.next_eps, inv_dim);
-        refill();
-        param<NU>(w, params, param_slot(BLOCK, kNextW), q);
-        if constexpr (CENTER) param<NU>(b, params, param_slot(BLOCK, kNextB), q);
+          if constexpr (DROP) {
+            RowKeep<ALIGNED, NU, LANES> kept;
+            kept.draw(a, q, keep, s.keys, row, s.keep + q.group * a.row_threads * NU);
 #pragma unroll
-        for (int j = 0; j < 4 * NU; ++j) {
-          if constexpr (CENTER) z[j] = fma2(mul2(sub2(z[j], splat(next.x)), splat(next.y)), w[j], b[j]);
-          else z[j] = mul2(mul2(z[j], splat(next.y)), w[j]);
+            for (int j = 0; j < 4 * NU; ++j) u[j] = kept(keep, j, u[j]);
+          }
+          load_cols<T, ALIGNED, NU, LANES>(z, ring.row_ptr(a, q, at, kX, row0, n, i), q);
+#pragma unroll
+          for (int j = 0; j < 4 * NU; ++j) {
+            z[j] = add2(u[j], z[j]);
+            if constexpr (!ALIGNED) {
+              if (2 * j >= q.count) z[j].x = 0.f;
+              if (2 * j + 1 >= q.count) z[j].y = 0.f;
+            }
+          }
+          store_cols<T, ALIGNED, NU, LANES>(static_cast<T *>(a.out) + base, z, q, valid);
+        } else {
+          load_cols<T, ALIGNED, NU, LANES>(z, ring.row_ptr(a, q, at, kX, row0, n, i), q);
         }
-        store_cols<T, ALIGNED, NU, LANES>(static_cast<T *>(a.y) + base, z, q, valid);
+        if (next_norm) {
+          next = row_stats<ALIGNED, CENTER, NU>(sum, q, z, p.next_kind, p.next_eps, inv_dim);
+          refill();
+          param<NU>(w, params, param_slot(BLOCK, kNextW), q);
+          if constexpr (CENTER) param<NU>(b, params, param_slot(BLOCK, kNextB), q);
+#pragma unroll
+          for (int j = 0; j < 4 * NU; ++j) {
+            if constexpr (CENTER) z[j] = fma2(mul2(sub2(z[j], splat(next.x)), splat(next.y)), w[j], b[j]);
+            else z[j] = mul2(mul2(z[j], splat(next.y)), w[j]);
+          }
+          store_cols<T, ALIGNED, NU, LANES>(static_cast<T *>(a.y) + base, z, q, valid);
+        }
+        if (a.stats && q.t == 0 && q.rank == 0 && valid)
+          reinterpret_cast<float4 *>(a.stats)[row] = make_float4(post.x, post.y, next.x, next.y);
       }
-      if (a.stats && q.t == 0 && q.rank == 0 && valid)
-        reinterpret_cast<float4 *>(a.stats)[row] = make_float4(post.x, post.y, next.x, next.y);
-    }
-    if (!refilled) {
-      q.barrier();
-      refill();
+      if (!refilled) {
+        q.barrier();
+        refill();
+      }
     }
   }
 }
@@ -875,7 +910,7 @@ __global__ void __launch_bounds__(512, BLOCK ? 1 : 2) bwd_kernel(const __grid_co
   // the dropout's scale is folded into the post norm's weight and bias, and into their gradients' sums at the end
   const Keep keep(p.threshold);
   const float drop_scale = DROP ? keep_scale(p.threshold) : 1.f;
-  stage_params<T, ALIGNED, BLOCK, CENTER, 1, 32>(params, a, q, drop_scale);
+  stage_params<T, ALIGNED, BLOCK, CENTER, false, 1, 32>(params, a, q, drop_scale);
   const float inv_dim = 1.f / (float)q.dim;
   const int gate_mode = GATE == kGateAny ? p.gate_mode : GATE;
   const bool next_sums = WHOLE || a.in[kDy], has_dout = WHOLE || a.in[kDout];
