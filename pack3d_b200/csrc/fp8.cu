@@ -10,7 +10,7 @@
 //
 // Meant to be bound by HBM: 2 or 4 bytes read and one written an element; with the transposed copy (blocks of
 // 128 rows, for a product that sums over the rows) one more, from the same read.  Measured on B200 (bf16): rows
-// 262144 x 192 33 us (4.5 TB/s), both copies of 16384 x 8192 about 120 us (4.5 TB/s): unpacking,
+// 262144 x 192 33 us (4.5 TB/s), both copies of 16384 x 8192 about 110 us (4.9 TB/s): unpacking,
 // scaling and rounding take about as many issue slots (65 %) as the bytes take time.
 #include <algorithm>
 
