@@ -420,12 +420,12 @@ extern "C" int p3d_residual_fwd(const p3d_residual *args, void *out, void *y, fl
   if (p.gate_mode == P3D_GATE_SAMPLE) {
     // A CTA that has at least kFoldRows turns of a sample's rows sets that sample's parameters up (524288 x 192, two
     // samples: 163 us, read and activated for each row 185 us), where cutting the rows by sample leaves the longest
-    // CTA at most a tenth more of them, which is what it saves (200 samples of 64 x 4096, on 200 CTAs instead of
-    // 296: 320 us against 262).
+    // CTA at most a sixth more of them (16 % more, 512 samples of 1024 x 192: 190 us against 208; 48 % more, 200 of
+    // 64 x 4096: 320 against 262).
     const Split by_sample = split_of(p, s, info.sm_count, per_sm, true);
     const int64_t at_once = by_sample.ctas / by_sample.slices, turns = (by_sample.segments + at_once - 1) / at_once;
     const int64_t rows = (by_sample.segment_rows + by_sample.slices - 1) / by_sample.slices;
-    a.gate_folded = rows >= (int64_t)kFoldRows * s.groups * s.rows_at_once() && turns * rows * c.ctas <= p.rows + p.rows / 10;
+    a.gate_folded = rows >= (int64_t)kFoldRows * s.groups * s.rows_at_once() && turns * rows * c.ctas <= p.rows + p.rows / 6;
     if (a.gate_folded) c = by_sample;
   }
   a.segments = (int)c.segments;
