@@ -27,6 +27,8 @@ namespace {
 using rows::Args;
 using rows::kSums;
 using rows::kUnit;
+using rows::Shape;
+using rows::shape_of;
 
 constexpr int kMaxDim = 16384;   // 512 threads of four CTAs in 16 bits, 256 of eight in 32
 constexpr int kFoldRows = 8;
@@ -159,36 +161,6 @@ __global__ void __launch_bounds__(256) dropout_any_kernel(const T *x, T *y, int6
 
 // ------------------------------------------------------------------------ host side
 bool aligned16(const void *ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15u) == 0; }
-
-// Threads that work on a row (or on a warp's rows), lanes a row, units of eight columns a thread, rows or warps of
-// rows a CTA works on at once, and CTAs a row.
-//   Forward: up to 384 columns a warp holds several rows, on 8 or 16 lanes with one or three units each, so that
-//   sums take three or four steps for all of them and the bookkeeping is shared; wider rows take two
-//   units a thread and up to 256 threads.  (524288 x 192 bf16 with dropout: one row a warp 388 us,
-//   four rows 223 us; 163 us since with leaner bookkeeping and the gate folded into the parameters.)
-//   Backward: a row a warp at least and one unit, whose column sums fill the registers already.  At most 512
-//   threads a row, 256 in 32 bits, where two stages of five arrays of 4096 columns would not fit
-//   beside the parameters.
-struct Shape {
-  int row_threads, lanes, units, groups, members;
-  int columns() const { return (lanes < 32 ? lanes : row_threads) * kUnit * units; }   // of a CTA
-  int rows_at_once() const { return 32 / lanes; }
-};
-Shape shape_of(int dim, int dtype, bool backward) {
-  Shape s;
-  s.members = 1;
-  s.lanes = backward || dim > 384 ? 32 : dim > 192 ? 16 : 8;
-  s.units = backward || dim <= 64 ? 1 : s.lanes == 32 ? 2 : 3;
-  s.row_threads = 32;
-  if (s.lanes == 32) {
-    const int threads = (dim + kUnit * s.units - 1) / (kUnit * s.units), most = backward && dtype != P3D_F32 ? 512 : 256;
-    while (threads > s.members * most) s.members *= 2;
-    const int mine = (threads + s.members - 1) / s.members;
-    s.row_threads = (mine + 31) / 32 * 32;
-  }
-  s.groups = std::min(rows::kMaxGroups, std::max(1, 256 / s.row_threads));
-  return s;
-}
 
 // Whether a call needs a mean or a bias.
 bool centred(const p3d_residual &p) {

@@ -34,6 +34,7 @@
 #include "common.cuh"
 #include "kernels.cuh"
 #include "philox.cuh"
+#include "rows_layout.cuh"
 #include "sm100.cuh"
 
 namespace p3d {
@@ -43,11 +44,8 @@ using sm100::add2;
 using sm100::fma2;
 using sm100::mul2;
 
-constexpr int kUnit = 8;             // columns of a unit; a thread owns one or two (NU)
-constexpr int kMaxRowThreads = 512;  // threads a row of one CTA
 constexpr int kMaxCluster = 8;
 constexpr int kMaxStages = 4;
-constexpr int kMaxGroups = 8;
 constexpr uint64_t kWaitNs = 2000000000ull;
 
 static __device__ unsigned g_row_errors = 0;
@@ -146,7 +144,7 @@ __device__ __forceinline__ Place place_of(const Args &a) {
   for (int n = 0; n < NU; ++n) {
     const int c = (q.t + n * q.threads) * kUnit;
     q.live[n] = c < q.end;
-    q.at[n] = max(0, min(c, q.end - kUnit));
+    q.at[n] = min(c, q.end - kUnit);
   }
   return q;
 }
@@ -337,7 +335,7 @@ struct RowSum {
     const float n_w = mine ? x->slots[at][0][w] : 0.f, mean_w = mine ? x->slots[at][1][w] : 0.f;
     float two[2] = {n_w, n_w * mean_w};
     lane_sums<32>(q.lane, two);
-    mean = two[0] > 0.f ? two[1] / two[0] : 0.f;   // a CTA of the cluster may have no columns
+    mean = two[1] / two[0];
     const float off = mean_w - mean;
     m2 = warp_sum(fmaf(n_w * off, off, mine ? x->slots[at][2][w] : 0.f));
     if (members > 1) {
@@ -462,19 +460,16 @@ struct Ring {
     const int n = ahead.count(a), row = ahead.row;
     const uint32_t to = sm100::smem_u32(data) + (uint32_t)fill * a.stage_bytes, b = bars + 8u * fill;
     fill = fill + 1 == a.stages ? 0 : fill + 1;
-    const int cols = max(0, min(q.threads * kUnit * NU, q.end));   // the last CTA of a row may have none
+    const int cols = min(q.threads * kUnit * NU, q.end);
     const uint32_t bytes = (uint32_t)(((n - 1) * q.dim + cols) * (int)sizeof(T));
     const int64_t off = ((int64_t)row * q.dim + q.first) * (int64_t)sizeof(T);
-    const bool copied = cols > 0 && (ALIGNED || !in_place(a, row, n));
     if constexpr (ALIGNED) {
-      elect_expect_tx(b, (STATS ? 16u * n : 0u) + (copied ? bytes * a.slot_count : 0u));
-      if (copied) {
+      elect_expect_tx(b, (STATS ? 16u * n : 0u) + bytes * a.slot_count);
 #pragma unroll
-        for (int i = 0; i < kArrays; ++i)
-          if (a.in[i])
-            elect_bulk_load(to + a.slots[i], static_cast<const char *>(a.in[i]) + off, bytes, b);
-      }
+      for (int i = 0; i < kArrays; ++i)
+        if (a.in[i]) elect_bulk_load(to + a.slots[i], static_cast<const char *>(a.in[i]) + off, bytes, b);
     } else {
+      const bool copied = !in_place(a, row, n);
       uint32_t all = STATS ? 16u * n : 0u;
       if (copied) {
 #pragma unroll 1
@@ -620,7 +615,7 @@ __device__ __forceinline__ void stage_params_of(float4 *params, const Args &a, c
 template <typename T, bool ALIGNED, bool BLOCK, bool CENTER, bool FOLD, int NU, int LANES>
 __device__ __forceinline__ void stage_params(float4 *params, const Args &a, const Place &q, float factor,
                                              const T *gate = nullptr) {
-  if (q.group == 0 && (!ALIGNED || q.end > 0)) {   // the last CTA of a row may have no columns
+  if (q.group == 0) {
     if (sizeof(T) == 4 || a.p.param_dtype != P3D_F32)
       stage_params_of<T, T, ALIGNED, BLOCK, CENTER, FOLD, NU, LANES>(params, a, q, factor, gate);
     else
@@ -1110,7 +1105,7 @@ __global__ void __launch_bounds__(512, BLOCK ? 1 : 2) bwd_kernel(const __grid_co
     if constexpr (BLOCK) {
       // what the CTA's samples before have summed up to, on its way while the groups are joined
       float2 was[3][4] = {};
-      if (kSampled && seg != cta / a.slices && q.group == 0 && q.end > 0) {
+      if (kSampled && seg != cta / a.slices && q.group == 0) {
 #pragma unroll
         for (int i = 0; i < (CENTER ? 3 : 2); ++i) get_sums<ALIGNED>(was[i], mine + i * one_sum, q);
       }

@@ -1,0 +1,49 @@
+// How the row kernels of the norms lay a row over threads.  Plain C++ where no CUDA compiler reads it, so that the
+// rules can be checked over all widths without a GPU.
+#pragma once
+
+#include <algorithm>
+
+#include "pack3d_b200.h"
+
+namespace p3d {
+namespace rows {
+
+constexpr int kUnit = 8;   // columns of a unit; a thread owns up to three (NU)
+constexpr int kMaxGroups = 8;
+
+// Threads that work on a row (or on a warp's rows), lanes a row, units of eight columns a thread, rows or warps of
+// rows a CTA works on at once, and CTAs a row.
+//   Forward: up to 384 columns a warp holds several rows, on 8 or 16 lanes with one or three units each, so that
+//   sums take three or four steps for all of them and the bookkeeping is shared; wider rows take two
+//   units a thread and up to 256 threads.  (524288 x 192 bf16 with dropout: one row a warp 388 us,
+//   four rows 223 us; 163 us since with leaner bookkeeping and the gate folded into the parameters.)
+//   Backward: a row a warp at least and one unit, whose column sums fill the registers already.  At most 512
+//   threads a row, 256 in 32 bits, where two stages of five arrays of 4096 columns would not fit
+//   beside the parameters.
+struct Shape {
+  int row_threads, lanes, units, groups, members;
+  int columns() const { return (lanes < 32 ? lanes : row_threads) * kUnit * units; }   // of a CTA
+  int rows_at_once() const { return 32 / lanes; }
+};
+inline Shape shape_of(int dim, int dtype, bool backward) {
+  Shape s;
+  s.members = 1;
+  s.lanes = backward || dim > 384 ? 32 : dim > 192 ? 16 : 8;
+  s.units = backward || dim <= 64 ? 1 : s.lanes == 32 ? 2 : 3;
+  s.row_threads = 32;
+  if (s.lanes == 32) {
+    const int threads = (dim + kUnit * s.units - 1) / (kUnit * s.units), most = backward && dtype != P3D_F32 ? 512 : 256;
+    while (threads > s.members * most) s.members *= 2;
+    const int mine = (threads + s.members - 1) / s.members;
+    s.row_threads = (mine + 31) / 32 * 32;
+    // rounded up to whole warps, fewer CTAs may hold the row: every CTA that there is has columns of it (at 8200 columns in
+    // 32 bits seven of 160 threads, not eight)
+    s.members = (threads + s.row_threads - 1) / s.row_threads;
+  }
+  s.groups = std::min(kMaxGroups, std::max(1, 256 / s.row_threads));
+  return s;
+}
+
+}  // namespace rows
+}  // namespace p3d

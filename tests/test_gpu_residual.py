@@ -414,3 +414,10 @@ def test_offsets_past_32_bits(cuda_device):
     kept = dropout(ones, 0.5, (5, 2)) != 0
     same = (kept[-tail:] == kept[:tail]).float().mean().item()
     assert abs(same - 0.5) < 5 * 0.5 / (tail * dim) ** 0.5      # five deviations of that many fair coins
+
+
+@pytest.mark.parametrize("dim", [8200, 8960, 10248, 12296])
+@pytest.mark.parametrize("nxt", [True, False])
+def test_sample_gate_of_rows_over_uneven_clusters(cuda_device, dim, nxt):
+    """fp32 widths whose rows fill fewer than eight CTAs of whole warps, with a gate whose last vector ends the tensor."""
+    check_residual(cuda_device, (3, 5, dim), torch.float32, "layer", "sample", "tanh", nxt=nxt, seed=dim)

@@ -1,0 +1,39 @@
+"""How the row kernels of the norms lay rows out, over all widths, without a GPU: the layout's own source compiled for
+the host."""
+import subprocess
+from pathlib import Path
+
+import pytest
+
+ROOT = Path(__file__).resolve().parents[1]
+
+
+def run(tmp_path, body):
+    """The lines that a C++ program with the row layout in scope prints."""
+    source = tmp_path / "probe.cpp"
+    source.write_text('#include <cstdio>\n#include "rows_layout.cuh"\nusing namespace p3d::rows;\nint main() {\n%s\n}\n' % body)
+    exe = tmp_path / "probe"
+    subprocess.run(["g++", "-std=c++17", "-O1", "-I", str(ROOT / "include"), "-I", str(ROOT / "pack3d_b200" / "csrc"),
+                    str(source), "-o", str(exe)], check=True)
+    return subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.splitlines()
+
+
+def test_every_cta_has_columns_of_its_row(tmp_path):
+    """A CTA of a row's cluster without columns would read the gate of a sample past its end."""
+    lines = run(tmp_path, """
+  for (int dim = 1; dim <= 16384; ++dim)
+    for (int dtype : {P3D_F32, P3D_F16, P3D_BF16})
+      for (bool backward : {false, true}) {
+        const Shape s = shape_of(dim, dtype, backward);
+        const bool held = s.members * s.columns() >= dim, empty = (s.members - 1) * s.columns() >= dim;
+        const bool fits = s.members >= 1 && s.members <= 8 && s.row_threads * s.groups <= 512 && s.groups >= 1 &&
+                          s.groups <= kMaxGroups && (s.members == 1 || s.groups == 1);
+        if (!held || empty || !fits) std::printf("%d %d %d\\n", dim, dtype, (int)backward);
+      }
+""")
+    assert lines == []
+
+
+@pytest.mark.parametrize("dim,members", [(8192, 4), (8200, 7), (8960, 7), (8968, 8), (12296, 7), (16384, 8)])
+def test_ctas_of_wide_fp32_rows(tmp_path, dim, members):
+    assert run(tmp_path, f'std::printf("%d", shape_of({dim}, P3D_F32, true).members);') == [str(members)]
