@@ -243,6 +243,7 @@ size_t lay_out(Args &a, const Shape &s, bool aligned, bool center, bool backward
   size_t turns = 1;   // rows (or turns of a warp's rows) a batch
   if (s.members == 1) turns = std::max<size_t>(1, std::min({8 / at_once, 2048 / (at_once * row), share / (2 * r.stage)}));
   a.batch_rows = (int)(turns * at_once);
+  a.edge_rows = rows::edge_rows((int64_t)a.p.dim * dtype_size(a.p.dtype));
   const size_t batch = row * a.batch_rows;
   const uint32_t slot = (uint32_t)(aligned ? batch : (batch + 15) / 16 * 16 + 16);
   a.stats_at = 0;

@@ -69,6 +69,7 @@ struct Args {
   float *partials;  // [kSums - 1][CTA slots][dim], then the sample gate's [samples][slices][dim]
   int row_threads, groups, members;
   int batch_rows, stages;
+  int edge_rows;             // unaligned: rows at either end whose batches are read in place
   uint32_t stage_bytes;      // of all arrays' batches and the statistics
   uint32_t slots[kArrays], stats_at;   // where each lies in a stage
   int slot_count;            // arrays
@@ -410,10 +411,6 @@ __device__ __forceinline__ Batches batches_of(const Args &a, int group, int cta,
   return k;
 }
 
-// The bytes of one array's unaligned batch of `n` rows from `row` on in this CTA's columns: they are copied with
-// the up to 15 bytes before and after that complete 16-byte pieces.  The batches with the tensor's first
-// and last row, whose pieces would pass its ends, are not copied but read in place.
-__device__ __forceinline__ bool in_place(const Args &a, int row, int n) { return row == 0 || row + n == (int)a.p.rows; }
 // Bytes from the last 16-byte boundary to column `first` of `row`.
 template <typename T>
 __device__ __forceinline__ uint32_t shift_of(const Args &a, const Place &q, int array, int row) {
@@ -469,12 +466,12 @@ struct Ring {
       for (int i = 0; i < kArrays; ++i)
         if (a.in[i]) elect_bulk_load(to + a.slots[i], static_cast<const char *>(a.in[i]) + off, bytes, b);
     } else {
-      const bool copied = !in_place(a, row, n);
+      const bool copied = !in_place(row, n, (int)a.p.rows, a.edge_rows);
       uint32_t all = STATS ? 16u * n : 0u;
       if (copied) {
 #pragma unroll 1
         for (int i = 0; i < kArrays; ++i)
-          if (a.in[i]) all += (shift_of<T>(a, q, i, row) + bytes + 15u) & ~15u;
+          if (a.in[i]) all += piece_bytes(shift_of<T>(a, q, i, row), bytes);
       }
       elect_expect_tx(b, all);
       if (copied) {
@@ -483,7 +480,7 @@ struct Ring {
           if (a.in[i]) {
             const uint32_t shift = shift_of<T>(a, q, i, row);
             elect_bulk_load(to + a.slots[i], static_cast<const char *>(a.in[i]) + off - shift,
-                            (shift + bytes + 15u) & ~15u, b);
+                            piece_bytes(shift, bytes), b);
           }
       }
     }
@@ -506,7 +503,7 @@ struct Ring {
     const char *slot = at + a.slots[array];
     if constexpr (!ALIGNED) {
       slot += shift_of<T>(a, q, array, row);
-      if (in_place(a, row, n))
+      if (in_place(row, n, (int)a.p.rows, a.edge_rows))
         slot = static_cast<const char *>(a.in[array]) + ((int64_t)row * q.dim + q.first) * (int64_t)sizeof(T);
     }
     return reinterpret_cast<const T *>(slot) + i * q.dim;

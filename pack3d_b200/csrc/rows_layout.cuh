@@ -4,7 +4,15 @@
 
 #include <algorithm>
 
+#include <stdint.h>
+
 #include "pack3d_b200.h"
+
+#ifdef __CUDACC__
+#define P3D_ROWS_FN __host__ __device__ __forceinline__
+#else
+#define P3D_ROWS_FN inline
+#endif
 
 namespace p3d {
 namespace rows {
@@ -44,6 +52,14 @@ inline Shape shape_of(int dim, int dtype, bool backward) {
   s.groups = std::min(kMaxGroups, std::max(1, 256 / s.row_threads));
   return s;
 }
+
+// An unaligned batch of `n` rows from `row` on is copied with the up to 15 bytes before and after it that complete 16-byte
+// pieces.  Batches whose pieces may pass the tensor's ends are not copied but read in place: those with one of the
+// edge_rows first or last rows, which is one row at each end, and more where a row is shorter than 15 bytes.
+inline int edge_rows(int64_t row_bytes) { return (int)((15 + row_bytes - 1) / row_bytes); }
+P3D_ROWS_FN bool in_place(int row, int n, int rows, int edge) { return row < edge || row + n > rows - edge; }
+// Bytes of the pieces that hold `bytes` bytes from `shift` after a 16-byte boundary on.
+P3D_ROWS_FN uint32_t piece_bytes(uint32_t shift, uint32_t bytes) { return (shift + bytes + 15u) & ~15u; }
 
 }  // namespace rows
 }  // namespace p3d

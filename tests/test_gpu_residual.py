@@ -421,3 +421,9 @@ def test_offsets_past_32_bits(cuda_device):
 def test_sample_gate_of_rows_over_uneven_clusters(cuda_device, dim, nxt):
     """fp32 widths whose rows fill fewer than eight CTAs of whole warps, with a gate whose last vector ends the tensor."""
     check_residual(cuda_device, (3, 5, dim), torch.float32, "layer", "sample", "tanh", nxt=nxt, seed=dim)
+
+
+@pytest.mark.parametrize("dim", [1, 2, 3, 7])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_rows_shorter_than_a_copied_piece(cuda_device, dim, dtype):
+    check_residual(cuda_device, (2, 301, dim), dtype, "rms", "element", "sigmoid", 0.25, seed=dim)

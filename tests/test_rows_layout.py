@@ -37,3 +37,29 @@ def test_every_cta_has_columns_of_its_row(tmp_path):
 @pytest.mark.parametrize("dim,members", [(8192, 4), (8200, 7), (8960, 7), (8968, 8), (12296, 7), (16384, 8)])
 def test_ctas_of_wide_fp32_rows(tmp_path, dim, members):
     assert run(tmp_path, f'std::printf("%d", shape_of({dim}, P3D_F32, true).members);') == [str(members)]
+
+
+def test_copied_pieces_stay_in_the_tensor(tmp_path):
+    """Unaligned batches are copied in whole 16-byte pieces: for every row length, start of the tensor and batch, the
+    pieces of a batch that is copied lie inside the tensor, and batches away from the ends are copied."""
+    lines = run(tmp_path, """
+  const int rows = 40;
+  for (int bytes = 2; bytes <= 66; bytes += 2)
+    for (int base = 0; base < 16; base += 2)
+      for (int row = 0; row < rows; ++row)
+        for (int n = 1; n <= 8 && row + n <= rows; ++n) {
+          const int start = base + row * bytes, size = n * bytes, total = base + rows * bytes;
+          const uint32_t shift = start & 15;
+          const int from = start - (int)shift, to = from + (int)piece_bytes(shift, size);
+          const bool kept = !in_place(row, n, rows, edge_rows(bytes));
+          const bool inside = from >= base && to <= total, wide = from % 16 == 0 && to >= start + size;
+          const bool middle = row >= 8 && row + n <= rows - 8;
+          if ((kept && !(inside && wide)) || (middle && !kept)) std::printf("%d %d %d %d\\n", bytes, base, row, n);
+        }
+""")
+    assert lines == []
+
+
+@pytest.mark.parametrize("bytes_,edge", [(2, 8), (4, 4), (6, 3), (14, 2), (16, 1), (4004, 1)])
+def test_rows_read_in_place(tmp_path, bytes_, edge):
+    assert run(tmp_path, f'std::printf("%d", edge_rows({bytes_}));') == [str(edge)]
