@@ -6,7 +6,9 @@
 // columns each (up to eight CTAs of a cluster for the widest rows), so the row statistics cost shuffles
 // and no second read.  Row groups of a CTA work independently: each has a ring of row batches in shared
 // memory that bulk copies fill ahead of it, so the bytes in flight do not depend on how many
-// warps fit beside the column sums' registers.
+// warps fit beside the column sums' registers.  A warp waits for a batch for 2 s at most: if that runs out it
+// records an error bit (p3d_device_errors), stores and loads nothing more, makes the sums that it has part in NaN, and waits
+// once more for the copies on their way before it ends.
 //
 // The backward makes out = x + s d again from x and h instead of reading the stored out: the same
 // bytes, and the normalised row keeps its 32 bits (the stored one is rounded to 16).  Every
@@ -77,6 +79,7 @@ struct Args {
   bool gate_folded;          // forward: the segments are samples, whose gate is multiplied into the parameters
 };
 
+__device__ __forceinline__ float nan() { return __uint_as_float(0x7fffffffu); }
 __device__ __forceinline__ float2 splat(float v) { return make_float2(v, v); }
 __device__ __forceinline__ float2 sub2(float2 a, float2 b) { return fma2(b, splat(-1.f), a); }
 
@@ -258,6 +261,7 @@ struct RowSum {
   Exchange *x;
   int members;
   int at = 0;
+  bool ok = true;   // otherwise the warp's rows did not arrive, and it makes the row's sums NaN for all who share them
 
   // Sums of N values over the row's warps (up to sixteen): each half of a warp adds up one value's slots, both
   // halves the same one where there is one.
@@ -281,7 +285,7 @@ struct RowSum {
     if (LANES == 32 && q.warps > 1) {
       if (q.lane == 0) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) x->slots[at][i][q.group * q.warps + q.warp] = v[i];
+        for (int i = 0; i < N; ++i) x->slots[at][i][q.group * q.warps + q.warp] = ok ? v[i] : nan();
       }
       q.barrier();
       over_warps(q, v);
@@ -327,7 +331,7 @@ struct RowSum {
     if (q.lane == 0) {
       const int w = q.group * q.warps + q.warp;
       x->slots[at][0][w] = count;
-      x->slots[at][1][w] = mean;
+      x->slots[at][1][w] = ok ? mean : nan();
       x->slots[at][2][w] = m2;
     }
     q.barrier();
@@ -447,16 +451,14 @@ template <typename T, bool ALIGNED, int NU, bool STATS>
 struct Ring {
   uint32_t bars;             // the group's
   char *data;                // the group's stages
-  int stage = 0, phase = 0;  // of the next batch to use
-  int fill = 0;              // stage of the next batch to load
-  Batches ahead;             // which is that
+  RingState state;
+  Batches ahead;             // the next batch to load
 
   // Called by the group's first warp, all of it.
   __device__ __forceinline__ void issue(const Args &a, const Place &q) {
-    if (!ahead.valid(a)) return;
-    const int n = ahead.count(a), row = ahead.row;
-    const uint32_t to = sm100::smem_u32(data) + (uint32_t)fill * a.stage_bytes, b = bars + 8u * fill;
-    fill = fill + 1 == a.stages ? 0 : fill + 1;
+    if (!state.ok || !ahead.valid(a)) return;
+    const int n = ahead.count(a), row = ahead.row, stage = state.load(a.stages);
+    const uint32_t to = sm100::smem_u32(data) + (uint32_t)stage * a.stage_bytes, b = bars + 8u * stage;
     const int cols = min(q.threads * kUnit * NU, q.end);
     const uint32_t bytes = (uint32_t)(((n - 1) * q.dim + cols) * (int)sizeof(T));
     const int64_t off = ((int64_t)row * q.dim + q.first) * (int64_t)sizeof(T);
@@ -487,15 +489,20 @@ struct Ring {
     if (STATS) elect_bulk_load(to + a.stats_at, a.stats + 4 * (int64_t)row, 16u * n, b);
     ahead.next(a);
   }
-  // Waits for the next batch and returns where its stage lies.
-  __device__ __forceinline__ char *wait(const Args &a, const Place &q) {
-    char *at = data + (uint32_t)stage * a.stage_bytes;
-    sm100::mbar_wait(bars + 8u * stage, phase, &g_row_errors, kWaitNs, sm100::kErrProducer);
-    if (++stage == a.stages) {
-      stage = 0;
-      phase ^= 1;
-    }
-    return at;
+  // Waits for the next batch and returns where its stage lies; state.ok says whether it is there, the same in the whole
+  // warp.
+  __device__ __forceinline__ char *wait(const Args &a) {
+    const int stage = state.use(a.stages, [&](int s, int phase) {
+      return __all_sync(0xffffffffu, sm100::mbar_wait(bars + 8u * s, phase, &g_row_errors, kWaitNs, sm100::kErrProducer));
+    });
+    return data + (uint32_t)stage * a.stage_bytes;
+  }
+  // At the kernel's end: after a batch that did not arrive, the warp that issued waits for its copies.
+  __device__ __forceinline__ void finish(const Args &a, const Place &q) {
+    if (state.ok || q.warp != 0) return;
+    state.drain(a.stages, [&](int s, int phase) {
+      sm100::mbar_wait(bars + 8u * s, phase, &g_row_errors, kWaitNs, sm100::kErrTeardown);
+    });
   }
   // Row i of the batch of `n` rows at `row`, from the CTA's first column on.
   __device__ __forceinline__ const T *row_ptr(const Args &a, const Place &q, const char *at, int array, int row, int n,
@@ -736,7 +743,8 @@ __global__ void __launch_bounds__(256, NU == 1 ? 4 : 2) fwd_kernel(const __grid_
     k.seg = seg;
 #pragma unroll 1
     for (k.enter(a); k.row < k.end; k.row += k.stride) {
-      const char *at = ring.wait(a, q);
+      const char *at = ring.wait(a);
+      const bool ok = sum.ok = ring.state.ok;
       const int n = k.count(a), row0 = k.row;
       bool refilled = false;
       auto refill = [&] {   // every thread of the group has left the batch before
@@ -746,7 +754,7 @@ __global__ void __launch_bounds__(256, NU == 1 ? 4 : 2) fwd_kernel(const __grid_
 #pragma unroll 1
       for (int i0 = 0; i0 < n; i0 += kRows) {
         // past the batch's end a lane group goes over its last row again, without storing
-        const bool valid = LANES == 32 || i0 + q.sub < n;
+        const bool valid = ok && (LANES == 32 || i0 + q.sub < n);
         const int i = LANES == 32 ? i0 : min(i0 + q.sub, n - 1);
         const int64_t row = row0 + i, base = row * q.dim + q.first;
         float2 z[4 * NU], w[4 * NU], b[4 * NU];
@@ -820,6 +828,7 @@ __global__ void __launch_bounds__(256, NU == 1 ? 4 : 2) fwd_kernel(const __grid_
       }
     }
   }
+  ring.finish(a, q);
 }
 
 // ------------------------------------------------------------------------ backward
@@ -916,6 +925,11 @@ __global__ void __launch_bounds__(512, BLOCK ? 1 : 2) bwd_kernel(const __grid_co
   float *const mine = a.partials + (int64_t)cta * q.dim;
   const int64_t one_sum = (int64_t)ctas * q.dim;
   const Batches first_batch = batches_of(a, q.group, cta, ctas);
+  // sums over rows that did not all arrive are NaN
+  auto mark = [&](float2 (&v)[4]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = ring.state.ok ? v[j] : splat(nan());
+  };
 #pragma unroll 1
   for (int seg = cta / a.slices; seg < a.segments; seg += first_batch.seg_step) {
     const T *const sample = static_cast<const T *>(p.gate) + (int64_t)seg * q.dim + q.first;
@@ -943,7 +957,8 @@ __global__ void __launch_bounds__(512, BLOCK ? 1 : 2) bwd_kernel(const __grid_co
     k.seg = seg;
 #pragma unroll 1
     for (k.enter(a); k.row < k.end; k.row += k.stride) {
-      const char *at = ring.wait(a, q);
+      const char *at = ring.wait(a);
+      const bool ok = sum.ok = ring.state.ok;
       const int n = k.count(a), row0 = k.row;
       bool refilled = false;
       auto refill = [&] {
@@ -1026,7 +1041,7 @@ __global__ void __launch_bounds__(512, BLOCK ? 1 : 2) bwd_kernel(const __grid_co
             }
           }
         }
-        if (want_dx) store_cols<T, ALIGNED, 1, 32>(static_cast<T *>(a.dx) + base, G, q);
+        if (want_dx) store_cols<T, ALIGNED, 1, 32>(static_cast<T *>(a.dx) + base, G, q, ok);
         if constexpr (BLOCK) {
           float2 s0[1], s1[1], s2[1];
           s0[0] = s1[0] = s2[0] = splat(0.f);
@@ -1038,7 +1053,7 @@ __global__ void __launch_bounds__(512, BLOCK ? 1 : 2) bwd_kernel(const __grid_co
             }
             times_slope(zn, act, p.gate_act);
             if (gate_mode == P3D_GATE_ELEMENT && a.dgate)
-              store_cols<T, ALIGNED, 1, 32>(static_cast<T *>(a.dgate) + base, zn, q);
+              store_cols<T, ALIGNED, 1, 32>(static_cast<T *>(a.dgate) + base, zn, q, ok);
           }
           // G becomes K e_w (a token's gate left out until the end)
 #pragma unroll
@@ -1078,7 +1093,7 @@ __global__ void __launch_bounds__(512, BLOCK ? 1 : 2) bwd_kernel(const __grid_co
               m1 = v[0] * post_dot;
               if constexpr (kTokens) dgate = v[0] * slope(gate, p.gate_act);
             }
-            if (token && a.dgate && q.t == 0 && q.rank == 0) static_cast<T *>(a.dgate)[row] = from_f32<T>(dgate);
+            if (token && a.dgate && q.t == 0 && q.rank == 0 && ok) static_cast<T *>(a.dgate)[row] = from_f32<T>(dgate);
             refill();
           }
           if (want_dh) {
@@ -1088,7 +1103,7 @@ __global__ void __launch_bounds__(512, BLOCK ? 1 : 2) bwd_kernel(const __grid_co
               if constexpr (CENTER) G[j] = add2(G[j], splat(m0));
               G[j] = mul2(G[j], splat(kTokens ? st.y * gate : st.y));
             }
-            store_cols<T, ALIGNED, 1, 32>(static_cast<T *>(a.dh) + base, G, q);
+            store_cols<T, ALIGNED, 1, 32>(static_cast<T *>(a.dh) + base, G, q, ok);
           }
         }
       }
@@ -1106,8 +1121,12 @@ __global__ void __launch_bounds__(512, BLOCK ? 1 : 2) bwd_kernel(const __grid_co
 #pragma unroll
         for (int i = 0; i < (CENTER ? 3 : 2); ++i) get_sums<ALIGNED>(was[i], mine + i * one_sum, q);
       }
+      mark(a_kh);
       join_groups(a_kh, joins, a, q);
-      if constexpr (CENTER) join_groups(a_k, joins, a, q);
+      if constexpr (CENTER) {
+        mark(a_k);
+        join_groups(a_k, joins, a, q);
+      }
       if (q.group == 0) {
         const bool sampled = kSampled && gate_mode == P3D_GATE_SAMPLE;
         float2 w[4], f[4], A[4];
@@ -1151,12 +1170,15 @@ __global__ void __launch_bounds__(512, BLOCK ? 1 : 2) bwd_kernel(const __grid_co
       for (int j = 0; j < 4; ++j) a_kh[j] = a_k[j] = splat(0.f);
     }
   }
+  mark(a_nw);
   join_groups(a_nw, joins, a, q);
   if (q.group == 0) put_sums<ALIGNED>(a_nw, mine + 3 * one_sum, q);
   if constexpr (CENTER) {
+    mark(a_nb);
     join_groups(a_nb, joins, a, q);
     if (q.group == 0) put_sums<ALIGNED>(a_nb, mine + 4 * one_sum, q);
   }
+  ring.finish(a, q);
 }
 
 // ------------------------------------------------------------------------ launches

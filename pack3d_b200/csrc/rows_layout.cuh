@@ -9,7 +9,7 @@
 #include "pack3d_b200.h"
 
 #ifdef __CUDACC__
-#define P3D_ROWS_FN __host__ __device__ __forceinline__
+#define P3D_ROWS_FN __device__ __forceinline__
 #else
 #define P3D_ROWS_FN inline
 #endif
@@ -60,6 +60,43 @@ inline int edge_rows(int64_t row_bytes) { return (int)((15 + row_bytes - 1) / ro
 P3D_ROWS_FN bool in_place(int row, int n, int rows, int edge) { return row < edge || row + n > rows - edge; }
 // Bytes of the pieces that hold `bytes` bytes from `shift` after a 16-byte boundary on.
 P3D_ROWS_FN uint32_t piece_bytes(uint32_t shift, uint32_t bytes) { return (shift + bytes + 15u) & ~15u; }
+
+// Where a warp is in its group's ring: the stages are filled in turn, at most all but one ahead of the batch in use.
+// A batch that does not arrive in time is the last one waited for: the warp goes through its remaining batches on the
+// stage where it stopped, so that barriers stay matched, and neither loads nor stores.
+struct RingState {
+  int stage = 0, phase = 0;   // of the next batch to use
+  int fill = 0;               // stage of the next batch to load
+  bool ok = true;             // all batches so far have arrived
+
+  P3D_ROWS_FN void step(int stages) {
+    if (++stage == stages) {
+      stage = 0;
+      phase ^= 1;
+    }
+  }
+  P3D_ROWS_FN int load(int stages) {   // the stage to load the next batch into
+    const int s = fill;
+    fill = fill + 1 == stages ? 0 : fill + 1;
+    return s;
+  }
+  // The next batch's stage; arrived(stage, phase) waits for it.
+  template <typename F>
+  P3D_ROWS_FN int use(int stages, F &&arrived) {
+    const int s = stage;
+    if (ok) ok = arrived(s, phase);
+    if (ok) step(stages);
+    return s;
+  }
+  // Waits once more for what is on its way, before the shared memory is given up.
+  template <typename F>
+  P3D_ROWS_FN void drain(int stages, F &&arrived) {
+    while (stage != fill) {
+      arrived(stage, phase);
+      step(stages);
+    }
+  }
+};
 
 }  // namespace rows
 }  // namespace p3d

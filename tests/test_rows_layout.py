@@ -63,3 +63,49 @@ def test_copied_pieces_stay_in_the_tensor(tmp_path):
 @pytest.mark.parametrize("bytes_,edge", [(2, 8), (4, 4), (6, 3), (14, 2), (16, 1), (4004, 1)])
 def test_rows_read_in_place(tmp_path, bytes_, edge):
     assert run(tmp_path, f'std::printf("%d", edge_rows({bytes_}));') == [str(edge)]
+
+
+RING = """
+  // One warp of a group that issues and uses: the kernels' own order of calls on a model of the barriers.  Batch `lost`
+  // never arrives.
+  for (int stages = 2; stages <= 4; ++stages)
+    for (int batches = 1; batches <= 13; ++batches)
+      for (int lost = -1; lost < batches; ++lost) {
+        RingState r;
+        int loaded = 0, used = 0, out = 0, held[4] = {-1, -1, -1, -1}, phases[4] = {1, 1, 1, 1};
+        bool bad = false, seen[16] = {};
+        auto arrived = [&](int s, int phase) {   // the batch that this stage holds in this phase
+          const bool right = held[s] >= 0 && phases[s] == phase;
+          if (!right || seen[held[s]]) bad = true;
+          if (right && held[s] == lost) { ++out; return false; }
+          if (right) seen[held[s]] = true;
+          return right;
+        };
+        auto issue = [&] {
+          if (!r.ok || loaded == batches) return;
+          const int s = r.load(stages);
+          if (held[s] >= 0 && !seen[held[s]]) bad = true;   // over a batch that may still be on its way
+          held[s] = loaded++;
+          phases[s] ^= 1;
+        };
+        for (int i = 0; i < stages - 1; ++i) issue();
+        for (int b = 0; b < batches; ++b) {
+          const int s = r.use(stages, arrived);
+          if (s < 0 || s >= stages || (r.ok && held[s] != b)) bad = true;
+          if (r.ok) ++used;
+          issue();
+        }
+        const int before = out;
+        if (!r.ok) r.drain(stages, arrived);
+        for (int b = 0; b < loaded; ++b)
+          if (!seen[b] && b != lost) bad = true;     // every copy on its way was waited for
+        if (bad || r.ok != (lost < 0) || used != (lost < 0 ? batches : lost) || before != (lost >= 0) || out > 2)
+          std::printf("%d %d %d\\n", stages, batches, lost);
+      }
+"""
+
+
+def test_ring_stops_at_a_batch_that_does_not_arrive(tmp_path):
+    """After a wait that ran out nothing is used, no further batch is loaded or waited for, and the end waits for what is
+    on its way, each batch once; without one, every batch is used in order."""
+    assert run(tmp_path, RING) == []
