@@ -1060,7 +1060,9 @@ __global__ void __launch_bounds__(512, BLOCK ? 1 : 2) bwd_kernel(const __grid_co
           for (int j = 0; j < 4; ++j) {
             if constexpr (DROP) G[j] = kept(keep, j, G[j]);
             const float2 K = kTokens ? mul2(G[j], splat(gate)) : G[j];
-            a_kh[j] = fma2(K, hn[j], a_kh[j]);
+            // what is dropped adds nothing, an infinite h~ included
+            if constexpr (DROP) a_kh[j] = fma2(K, kept(keep, j, hn[j]), a_kh[j]);
+            else a_kh[j] = fma2(K, hn[j], a_kh[j]);
             if constexpr (CENTER) a_k[j] = add2(a_k[j], K);
             if constexpr (GATE == kGateAny) s2[0] = add2(s2[0], zn[j]);
             if constexpr (kTokens && CENTER) s2[0] = fma2(G[j], e_b[j], s2[0]);
@@ -1099,8 +1101,10 @@ __global__ void __launch_bounds__(512, BLOCK ? 1 : 2) bwd_kernel(const __grid_co
           if (want_dh) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              G[j] = fma2(hn[j], splat(m1), G[j]);
-              if constexpr (CENTER) G[j] = add2(G[j], splat(m0));
+              if (post_norm) {   // otherwise h, which may be infinite, has no part in its gradient
+                G[j] = fma2(hn[j], splat(m1), G[j]);
+                if constexpr (CENTER) G[j] = add2(G[j], splat(m0));
+              }
               G[j] = mul2(G[j], splat(kTokens ? st.y * gate : st.y));
             }
             store_cols<T, ALIGNED, 1, 32>(static_cast<T *>(a.dh) + base, G, q, ok);

@@ -427,3 +427,78 @@ def test_sample_gate_of_rows_over_uneven_clusters(cuda_device, dim, nxt):
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_rows_shorter_than_a_copied_piece(cuda_device, dim, dtype):
     check_residual(cuda_device, (2, 301, dim), dtype, "rms", "element", "sigmoid", 0.25, seed=dim)
+
+
+@pytest.mark.parametrize("gate", [None, "element", "token", "sample"])
+@pytest.mark.parametrize("dim", [64, 1024, 77])
+@pytest.mark.parametrize("p,nxt", [(0.0, False), (0.5, False), (0.5, True)])
+@pytest.mark.parametrize("scale", [True, False])
+def test_gradients_beside_infinity_and_nan_in_the_block(cuda_device, gate, dim, p, nxt, scale):
+    """Without a post norm the block's output enters no gradient but the gate's and the scale's: where it is infinite or
+    NaN, its own gradient is as finite as elsewhere, and what is dropped adds nothing to any.  Compared wherever the
+    plain form's gradient is finite; with a next norm only dropped places hold infinities and NaN."""
+    from pack3d_b200 import NormSpec, residual_norm
+    shape, rng, dtype = (2, 6, dim), (7, 8), torch.float32
+    keep = keep_mask(12, dim, p, rng).view(shape).to(cuda_device) if p else None
+    h = make(shape, dtype, cuda_device, 1)
+    bad = torch.zeros(shape, dtype=torch.bool, device=cuda_device)
+    bad[0, 1, 3::9], bad[1, 4, 5::7], bad[1, 2, ::11] = True, True, True
+    if nxt:
+        bad &= ~keep
+    h[bad] = float("inf")
+    h[1, 2][bad[1, 2]] = float("nan")
+    leaves = {"x": make(shape, dtype, cuda_device, 2), "h": h}
+    gate_shape = {None: None, "element": shape, "token": (2, 6, 1), "sample": (2, 1, dim)}[gate]
+    if gate_shape:
+        leaves["gate"] = make(gate_shape, dtype, cuda_device, 3)
+    if scale:
+        leaves["scale"] = make((dim,), dtype, cuda_device, 4, 0.5, 0.2)
+    if nxt:
+        leaves["nw"] = make((dim,), dtype, cuda_device, 5, 1.0, 0.2)
+    for t in leaves.values():
+        t.requires_grad_()
+    exact = {k: t.detach().double().requires_grad_() for k, t in leaves.items()}
+    out, y = residual_norm(leaves["x"], leaves["h"], gate=leaves.get("gate"), gate_activation="tanh",
+                           scale=leaves.get("scale"), next_norm=NormSpec(leaves["nw"]) if nxt else None, p=p, rng=rng)
+    want_out, want_y = plain_residual(exact["x"], exact["h"], None, exact.get("gate"), "tanh", exact.get("scale"),
+                                      (exact["nw"], None, "rms", 1e-6) if nxt else None, keep, 1 / (1 - p))
+    up = [make(shape, dtype, cuda_device, 6 + i) for i in range(1 + nxt)]
+    got = torch.autograd.grad([out, y][:1 + nxt], list(leaves.values()), up)
+    want = torch.autograd.grad([want_out, want_y][:1 + nxt], list(exact.values()), [u.double() for u in up])
+    for name, a, b in zip(leaves, got, want):
+        at = torch.isfinite(b)
+        assert name not in ("x", "h") or at.all()
+        close(a[at], b[at], dtype, {"x": 1, "h": 1, "gate": dim if gate == "token" else 6}.get(name, 12))
+
+
+@pytest.mark.parametrize("gate", [None, "element", "token", "sample"])
+@pytest.mark.parametrize("dim", [64, 1024, 77])
+def test_dropped_infinity_under_an_rms_norm(cuda_device, gate, dim):
+    """An RMS norm takes a row with an infinity to zeros beside it: dropped, the infinity leaves out and the scale's
+    gradient finite."""
+    from pack3d_b200 import NormSpec, residual_norm
+    shape, rng = (2, 6, dim), (7, 8)
+    keep = keep_mask(12, dim, 0.5, rng).view(shape).to(cuda_device)
+    h = make(shape, torch.float32, cuda_device, 1)
+    bad = torch.zeros(shape, dtype=torch.bool, device=cuda_device)
+    bad[0, 1, 3::9], bad[1, 4, 5::7] = True, True
+    h[bad & ~keep] = float("inf")
+    x, w = make(shape, torch.float32, cuda_device, 2), make((dim,), torch.float32, cuda_device, 3, 1.0, 0.2)
+    s, nw = make((dim,), torch.float32, cuda_device, 4, 0.5, 0.2), make((dim,), torch.float32, cuda_device, 5, 1.0, 0.2)
+    gate_shape = {None: None, "element": shape, "token": (2, 6, 1), "sample": (2, 1, dim)}[gate]
+    g = make(gate_shape, torch.float32, cuda_device, 9) if gate_shape else None
+    up = [make(shape, torch.float32, cuda_device, 6 + i) for i in range(2)]
+
+    def grads(run, *leaves):
+        leaves = [t.requires_grad_() for t in leaves]
+        out, y = run(*leaves)
+        return (out, *torch.autograd.grad([out, y], leaves, [u.to(out.dtype) for u in up]))
+
+    got = grads(lambda x, s, nw: residual_norm(x, h.requires_grad_(), post_norm=NormSpec(w), gate=g, gate_activation="tanh", scale=s,
+                                               next_norm=NormSpec(nw), p=0.5, rng=rng), x.clone(), s.clone(), nw.clone())
+    want = grads(lambda x, s, nw: plain_residual(x, h.double(), (w.double(), None, "rms", 1e-6), None if g is None else g.double(),
+                                                 "tanh", s, (nw, None, "rms", 1e-6), keep, 2.0),
+                 x.double(), s.double(), nw.double())
+    for a, b, rows in zip(got, want, (1, 1, 12, 12)):
+        assert torch.isfinite(b).all()
+        close(a, b, torch.float32, rows)
