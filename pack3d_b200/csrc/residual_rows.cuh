@@ -984,6 +984,10 @@ __global__ void __launch_bounds__(512, BLOCK ? 1 : 2) bwd_kernel(const __grid_co
 #pragma unroll
               for (int j = 0; j < 4; ++j) act[j] = splat(gate);
             }
+            if constexpr (DROP) {   // an infinite gate too: 0 * inf would reach out, made again, and the sums
+#pragma unroll
+              for (int j = 0; j < 4; ++j) act[j] = kept(keep, j, act[j]);
+            }
           }
 #pragma unroll
           for (int j = 0; j < 4; ++j) {

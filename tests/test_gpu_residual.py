@@ -502,3 +502,39 @@ def test_dropped_infinity_under_an_rms_norm(cuda_device, gate, dim):
     for a, b, rows in zip(got, want, (1, 1, 12, 12)):
         assert torch.isfinite(b).all()
         close(a, b, torch.float32, rows)
+
+
+@pytest.mark.parametrize("dim", [64, 1024, 77])
+@pytest.mark.parametrize("act", ["identity", "sigmoid", "tanh"])
+@pytest.mark.parametrize("post", [None, "rms", "layer"])
+def test_dropped_infinity_and_nan_in_the_gate(cuda_device, dim, act, post):
+    """A gate value that is infinite or NaN where the element is dropped reaches neither out, y nor any gradient."""
+    from pack3d_b200 import NormSpec, residual_norm
+    shape, rng, dtype = (2, 6, dim), (7, 8), torch.float32
+    keep = keep_mask(12, dim, 0.5, rng).view(shape).to(cuda_device)
+    gate = make(shape, dtype, cuda_device, 1)
+    bad = torch.zeros(shape, dtype=torch.bool, device=cuda_device)
+    bad[0, 1, 3::9], bad[1, 4, 5::7], bad[1, 2, ::11] = True, True, True
+    gate[bad & ~keep] = float("inf")
+    gate[1, 2][(bad & ~keep)[1, 2]] = float("nan")
+    leaves = {"x": make(shape, dtype, cuda_device, 2), "h": make(shape, dtype, cuda_device, 3), "gate": gate,
+              "scale": make((dim,), dtype, cuda_device, 4, 0.5, 0.2), "nw": make((dim,), dtype, cuda_device, 5, 1.0, 0.2)}
+    if post:
+        leaves["pw"] = make((dim,), dtype, cuda_device, 6, 1.0, 0.2)
+    for t in leaves.values():
+        t.requires_grad_()
+    exact = {k: t.detach().double() for k, t in leaves.items()}
+    exact["gate"] = torch.where(keep, exact["gate"], 0.5)     # any finite value: it is dropped
+    exact = {k: t.requires_grad_() for k, t in exact.items()}
+    spec = (lambda of, cls: cls(of["pw"], None, post, 1e-6)) if post else lambda of, cls: None  # noqa: E731
+    out, y = residual_norm(leaves["x"], leaves["h"], post_norm=spec(leaves, NormSpec), gate=leaves["gate"], gate_activation=act,
+                           scale=leaves["scale"], next_norm=NormSpec(leaves["nw"]), p=0.5, rng=rng)
+    want_out, want_y = plain_residual(exact["x"], exact["h"], spec(exact, lambda *a: a), exact["gate"], act, exact["scale"],
+                                      (exact["nw"], None, "rms", 1e-6), keep, 2.0)
+    close(out, want_out, dtype)
+    close(y, want_y, dtype)
+    up = [make(shape, dtype, cuda_device, 7 + i) for i in range(2)]
+    got = torch.autograd.grad([out, y], list(leaves.values()), up)
+    want = torch.autograd.grad([want_out, want_y], list(exact.values()), [u.double() for u in up])
+    for name, a, b in zip(leaves, got, want):
+        close(a, b, dtype, 1 if name in ("x", "h", "gate") else 12)
