@@ -165,6 +165,14 @@ bool wants_grad(std::initializer_list<const Tensor *> tensors) {
   return false;
 }
 
+// Forward-mode derivatives are not there: a tangent is refused, whether or not the tensor takes part in reverse mode too, as
+// a result without one would read as a zero derivative.
+void refuse_tangents(std::initializer_list<const Tensor *> tensors) {
+  for (const Tensor *t : tensors)
+    TORCH_CHECK_NOT_IMPLEMENTED(!(t->defined() && t->_fw_grad(0).defined()),
+                                "forward-mode derivatives of this operator are not implemented");
+}
+
 // ------------------------------------------------------------------------------- dropout
 Tensor run_dropout(const Tensor &x, uint32_t threshold, const Tensor &rng, uint64_t seed, uint64_t offset) {
   const c10::cuda::CUDAGuard guard(x.device());
@@ -188,6 +196,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
   }
   static variable_list backward(AutogradContext *ctx, variable_list dy) {
     const Tensor rng = ctx->get_saved_variables()[0];
+    refuse_tangents({&dy[0]});
     return once({run_dropout(dy[0].detach(), (uint32_t)ctx->saved_data["threshold"].toInt(), rng,
                              (uint64_t)ctx->saved_data["seed"].toInt(), (uint64_t)ctx->saved_data["offset"].toInt()),
                  Tensor(), Tensor(), Tensor(), Tensor()},
@@ -199,6 +208,7 @@ PyObject *py_dropout(PyObject *, PyObject *const *args, Py_ssize_t count) {
   HANDLE_TH_ERRORS
   TORCH_CHECK_VALUE(count == 3, "dropout takes x, p, rng");
   const Tensor x = tensor(args[0], "x");
+  refuse_tangents({&x});
   check_cuda(x);
   const uint32_t threshold = threshold_of(args[1]);
   const Rng r = rng_of(args[2], x);
@@ -279,6 +289,7 @@ struct Residual : torch::autograd::Function<Residual> {
     Tensor dout = block ? up[0] : Tensor(), dy = next ? up[block ? 1 : 0] : Tensor();
     variable_list grads(2 + kTensors);
     if (!dout.defined() && !dy.defined()) return grads;
+    refuse_tangents({&dout, &dy});
     const c10::cuda::CUDAGuard guard(x.device());
     Tensor *d = grads.data() + 2;
     size_t edge = c.rng.defined() ? 1 : 0;   // of the next tensor that is there
@@ -317,6 +328,7 @@ PyObject *run_call(Call &c) {
   c.args.dim = (int32_t)c.t[kX].size(-1);
   c.args.rows = c.t[kX].numel() / c.args.dim;
   c.args.dtype = dtype_code(c.t[kX].scalar_type());
+  for (const Tensor &t : c.t) refuse_tangents({&t});
   same_params(c);
   const bool block = c.t[kH].defined();
   bool grad = false;
@@ -352,6 +364,7 @@ PyObject *py_norm(PyObject *, PyObject *const *args, Py_ssize_t count) {
   HANDLE_TH_ERRORS
   TORCH_CHECK_VALUE(count == 2, "norm takes x, spec");
   const Tensor x = tensor(args[0], "x");
+  refuse_tangents({&x});
   check_input(x, "norm");
   TORCH_CHECK_VALUE(args[1] != Py_None, "norm must be given a NormSpec");
   const Spec s = spec_of(args[1], x, "norm");
@@ -398,6 +411,7 @@ PyObject *py_residual_norm(PyObject *, PyObject *const *args, Py_ssize_t count) 
   HANDLE_TH_ERRORS
   TORCH_CHECK_VALUE(count == 9, "residual_norm takes x, h, post_norm, gate, gate_activation, scale, next_norm, p, rng");
   const Tensor x = tensor(args[0], "x"), h = tensor(args[1], "h");
+  refuse_tangents({&x, &h});
   check_input(x, "residual_norm");
   TORCH_CHECK_VALUE(h.sizes() == x.sizes() && h.scalar_type() == x.scalar_type() && h.device() == x.device(),
                     "h must have the shape, dtype and device of x");
@@ -485,6 +499,7 @@ struct Linear : torch::autograd::Function<Linear> {
   static variable_list backward(AutogradContext *ctx, variable_list up) {
     p3d_fp8_linear a;
     memcpy(&a, ctx->saved_data["args"].toStringRef().data(), sizeof(a));
+    refuse_tangents({&up[0]});
     const Tensor saved = ctx->get_saved_variables()[0], dy = up[0].detach().contiguous();
     const c10::cuda::CUDAGuard guard(dy.device());
     Tensor dx, dw, db;
@@ -510,6 +525,7 @@ PyObject *py_fp8_linear(PyObject *, PyObject *const *args, Py_ssize_t count) {
   const Tensor x = tensor(args[0], "x");
   Tensor weight = tensor_or_none(args[1], "weight"), bias = tensor_or_none(args[2], "bias");
   const Tensor values = tensor_or_none(args[3], "values"), scales = tensor_or_none(args[4], "scales");
+  refuse_tangents({&x, &weight, &bias});
   check_cuda(x);
   TORCH_CHECK_VALUE(x.dim() >= 1, "fp8_linear needs at least one dimension");
   const bool kept = !weight.defined();

@@ -138,7 +138,7 @@ def fp8_linear(x, weight, bias=None):
     and x's are products of 8-bit blocks too), or an :class:`Fp8Matrix` from :func:`quantize_weight` (serving; no
     gradients).  Blocks: x and dy 1 x 128 along the dimension that is summed over (for the weight's gradient that
     is the tokens), the weight 128 x 128.  The result has x's dtype, gradients their inputs'; the bias's gradient is
-    summed in fp32.
+    summed in fp32.  Differentiable once, in reverse mode; second and forward-mode derivatives are refused.
     """
     if isinstance(weight, Fp8Matrix):
         return _native.host().fp8_linear(x, None, bias, weight.values, weight.scales, weight.rows, weight.cols)

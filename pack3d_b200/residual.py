@@ -8,7 +8,7 @@ dropout, residual scale and residual, and dropout by itself, each one kernel in 
 
 No counterpart in the reference, whose layer ends at its own residual (``attention.py:89``).  fp32, fp16 and bf16 CUDA
 tensors, any leading shape, up to 16,384 columns; statistics, sums and gradients of parameters in fp32, each value
-rounded once where it is stored.
+rounded once where it is stored.  Differentiable once, in reverse mode; second and forward-mode derivatives are refused.
 """
 from __future__ import annotations
 

@@ -538,3 +538,36 @@ def test_dropped_infinity_and_nan_in_the_gate(cuda_device, dim, act, post):
     want = torch.autograd.grad([want_out, want_y], list(exact.values()), [u.double() for u in up])
     for name, a, b in zip(leaves, got, want):
         close(a, b, dtype, 1 if name in ("x", "h", "gate") else 12)
+
+
+def test_tangents_are_refused(cuda_device):
+    """Forward-mode derivatives, in any argument and in the upstream gradients: refused with and without reverse mode."""
+    import torch.autograd.forward_ad as forward_ad
+    from pack3d_b200 import NormSpec, dropout, fp8_linear, norm, quantize_weight, residual_norm
+    x, w = torch.randn(6, 32, device=cuda_device), torch.randn(32, device=cuda_device)
+    m = torch.randn(16, 32, device=cuda_device)
+    kept = quantize_weight(m)
+    with forward_ad.dual_level():
+        for grad in (False, True):
+            def dual(t):
+                return forward_ad.make_dual(t.clone().requires_grad_(grad), torch.ones_like(t))  # noqa: B023
+            for call in (lambda: dropout(dual(x), 0.5, (1, 2)), lambda: norm(dual(x), NormSpec()),
+                         lambda: norm(x, NormSpec(dual(w))), lambda: norm(x, NormSpec(w, dual(w))),
+                         lambda: residual_norm(dual(x), x), lambda: residual_norm(x, dual(x)),
+                         lambda: residual_norm(x, x, gate=dual(x)), lambda: residual_norm(x, x, scale=dual(w)),
+                         lambda: residual_norm(x, x, post_norm=NormSpec(dual(w))),
+                         lambda: residual_norm(x, x, next_norm=NormSpec(None, dual(w))),
+                         lambda: fp8_linear(dual(x), m), lambda: fp8_linear(x, dual(m)),
+                         lambda: fp8_linear(x, m, dual(m[:, 0])), lambda: fp8_linear(dual(x).detach(), kept, dual(m[:, 0]))):
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    call()
+        leaf = x.clone().requires_grad_()
+        for f in (lambda t: dropout(t, 0.5, (1, 2)), lambda t: norm(t, NormSpec()), lambda t: residual_norm(t, t)[0],
+                  lambda t: fp8_linear(t, m)):
+            y = f(leaf)
+            up = forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y))
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                torch.autograd.grad(y, [leaf], up)
+    for transform in (lambda f: torch.func.jvp(f, (x,), (x,)),):
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            transform(lambda t: norm(t, NormSpec()))

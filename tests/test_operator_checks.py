@@ -122,3 +122,17 @@ def test_host_module_is_built_beside_the_library():
     with pytest.raises(ValueError, match="takes"):
         module.norm(torch.zeros(2))
     assert ctypes.sizeof(ctypes.c_void_p) == 8
+
+
+def test_tangents_are_refused():
+    """A forward-mode derivative is refused before anything else, not dropped."""
+    import torch.autograd.forward_ad as forward_ad
+    from pack3d_b200 import NormSpec, dropout, fp8_linear, norm, residual_norm
+    x = torch.randn(4, 64)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for call in (lambda: dropout(dual, 0.5, (1, 2)), lambda: norm(dual, NormSpec()), lambda: residual_norm(dual, x),
+                     lambda: residual_norm(x, dual), lambda: fp8_linear(dual, x), lambda: fp8_linear(x, dual),
+                     lambda: fp8_linear(x, x, dual[0])):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
