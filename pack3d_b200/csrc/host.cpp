@@ -532,6 +532,16 @@ PyObject *py_fp8_linear(PyObject *, PyObject *const *args, Py_ssize_t count) {
   const int64_t n = kept ? PyLong_AsLongLong(args[5]) : weight.dim() == 2 ? weight.size(0) : 0;
   const int64_t k = kept ? PyLong_AsLongLong(args[6]) : weight.dim() == 2 ? weight.size(1) : 0;
   TORCH_CHECK_VALUE(n >= 1 && k >= 1 && x.size(-1) == k, "weight must be [out, ", x.size(-1), "], got [", n, ", ", k, "]");
+  if (kept) {   // an Fp8Matrix, whose attributes may have been set since it was made
+    TORCH_CHECK_VALUE(values.defined() && values.scalar_type() == at::kFloat8_e4m3fn && values.dim() == 2 &&
+                          values.is_contiguous() && values.size(0) == n && values.size(1) >= k && values.size(1) % 16 == 0,
+                      "values of a ", n, " x ", k, " Fp8Matrix must be contiguous float8_e4m3fn [rows, pitch], the pitch a "
+                      "multiple of 16 and at least the columns");
+    TORCH_CHECK_VALUE(scales.defined() && scales.scalar_type() == at::kByte && scales.is_contiguous() &&
+                          scales.device() == values.device() && scales.numel() == p3d_fp8_scale_bytes(n, k),
+                      "scales of a ", n, " x ", k, " Fp8Matrix must be ", p3d_fp8_scale_bytes(n, k),
+                      " contiguous uint8 on the device of its values");
+  }
   TORCH_CHECK_VALUE((kept ? values : weight).device() == x.device(), "x and weight must be on the same device");
   TORCH_CHECK_VALUE(kept || dtype_code(weight.scalar_type()) >= 0, "weight must be fp32, fp16 or bf16");
   if (bias.defined()) {

@@ -19,15 +19,33 @@ from ._validation import check_cuda
 BLOCK = 128
 
 
+def _scale_bytes(rows, cols):
+    """512 for every 128 rows and every four blocks of columns."""
+    return -(-rows // BLOCK) * -(-cols // (4 * BLOCK)) * 512
+
+
 class Fp8Matrix:
-    """``values`` [rows, pitch] (``torch.float8_e4m3fn``, pitch a multiple of 16, columns from ``cols`` on unused) and
-    ``scales`` (bytes e + 127 of 2^e, one for each row and block of 128 columns, in the order of
-    ``p3d_fp8_quantize``)."""
+    """``values`` [rows, pitch] (``torch.float8_e4m3fn``, contiguous, pitch a multiple of 16, columns from ``cols`` on
+    unused) and ``scales`` (contiguous bytes e + 127 of 2^e, one for each row and block of 128 columns, in the order of
+    ``p3d_fp8_quantize``), on one device."""
 
     __slots__ = ("values", "scales", "rows", "cols")
 
     def __init__(self, values, scales, rows, cols):
         self.values, self.scales, self.rows, self.cols = values, scales, int(rows), int(cols)
+        self._check()
+
+    def _check(self):
+        """The kernels take addresses, rows and columns from here: refuse what does not fit together."""
+        v, s = self.values, self.scales
+        if not (isinstance(v, torch.Tensor) and v.dtype == torch.float8_e4m3fn and v.ndim == 2 and v.is_contiguous()
+                and v.shape[0] == self.rows >= 1 and v.shape[1] >= self.cols >= 1 and v.shape[1] % 16 == 0):
+            raise ValueError(f"values of a {self.rows} x {self.cols} Fp8Matrix must be contiguous float8_e4m3fn [rows, pitch], "
+                             "the pitch a multiple of 16 and at least the columns")
+        if not (isinstance(s, torch.Tensor) and s.dtype == torch.uint8 and s.is_contiguous() and s.device == v.device
+                and s.numel() == _scale_bytes(self.rows, self.cols)):
+            raise ValueError(f"scales of a {self.rows} x {self.cols} Fp8Matrix must be {_scale_bytes(self.rows, self.cols)} "
+                             "contiguous uint8 on the device of its values")
 
     @property
     def shape(self):
@@ -55,7 +73,7 @@ class Fp8Matrix:
     def _empty(rows, cols, device):
         pitch = -(-cols // 16) * 16
         return Fp8Matrix(torch.empty((rows, pitch), dtype=torch.float8_e4m3fn, device=device),
-                         torch.empty(_native.lib().p3d_fp8_scale_bytes(rows, cols), dtype=torch.uint8, device=device),
+                         torch.empty(_scale_bytes(rows, cols), dtype=torch.uint8, device=device),
                          rows, cols)
 
 
@@ -124,6 +142,8 @@ def fp8_matmul(a, b, *, bias=None, dtype=torch.bfloat16):
     number of columns.  Products and sums in fp32; the order of the sum depends on the extents alone."""
     if not (isinstance(a, Fp8Matrix) and isinstance(b, Fp8Matrix)):
         raise ValueError("fp8_matmul takes two Fp8Matrix")
+    a._check()   # the attributes may have been set since
+    b._check()
     if a.cols != b.cols or a.device != b.device:
         raise ValueError(f"operands must have the same columns and device, got {list(a.shape)} and {list(b.shape)}")
     if dtype not in _native.DTYPE_CODE:

@@ -303,3 +303,24 @@ def test_linear_offsets_past_32_bits(cuda_device):
     want = fp8_linear(last, w)
     want.backward(dy[-tail:].clone())
     assert torch.equal(y[-tail:], want) and torch.equal(x.grad[-tail:], last.grad)
+
+
+def test_changed_parts_of_a_matrix_are_refused(cuda_device):
+    """An Fp8Matrix whose attributes no longer fit together, and tensors off a 16-byte boundary, reach no kernel."""
+    from pack3d_b200 import Fp8Matrix, fp8_linear, fp8_matmul, quantize, quantize_weight
+    x = torch.randn(4, 64, device=cuda_device)
+    qx, w = quantize(x), quantize_weight(torch.randn(130, 64, device=cuda_device))
+    changes = {"values": [w.values.cpu(), w.values[:129], w.values.view(torch.uint8), w.values.t(), w.values[:, :32]],
+               "scales": [w.scales.cpu(), w.scales[:512], w.scales.view(torch.int8), w.scales.repeat(2)[::2]],
+               "rows": [129, 131, 258], "cols": [80]}
+    for name, bads in changes.items():
+        for bad in bads:
+            other = Fp8Matrix(w.values, w.scales, w.rows, w.cols)
+            setattr(other, name, bad)
+            for call in (lambda: fp8_linear(x, other), lambda: fp8_matmul(qx, other), lambda: fp8_matmul(other, qx)):  # noqa: B023
+                with pytest.raises(ValueError):
+                    call()
+    odd = torch.empty(130 * 64 + 1, dtype=torch.uint8, device=cuda_device)[1:].view(torch.float8_e4m3fn).view(130, 64)
+    for call in (lambda m: fp8_linear(x, m), lambda m: fp8_matmul(qx, m)):
+        with pytest.raises(ValueError, match="16"):
+            call(Fp8Matrix(odd, w.scales, 130, 64))

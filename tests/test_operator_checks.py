@@ -136,3 +136,26 @@ def test_tangents_are_refused():
                      lambda: fp8_linear(x, x, dual[0])):
             with pytest.raises(NotImplementedError, match="forward-mode"):
                 call()
+
+
+def test_fp8_matrix_refuses_parts_that_do_not_fit():
+    """Kernels take addresses and extents from it: values, scales, rows and columns have to belong together."""
+    from pack3d_b200 import Fp8Matrix
+    values, scales = torch.zeros(130, 80, dtype=torch.float8_e4m3fn), torch.zeros(1024, dtype=torch.uint8)
+    assert Fp8Matrix(values, scales, 130, 70).shape == (130, 70)
+    for bad in (values.view(torch.uint8), values[:, :64], values[:129], values[0], values.t().contiguous(), None,
+                torch.zeros(130, 72, dtype=torch.float8_e4m3fn), torch.zeros(130, 64, dtype=torch.float8_e4m3fn)):
+        with pytest.raises(ValueError, match="values of a 130 x 70"):
+            Fp8Matrix(bad, scales, 130, 70)
+    for bad in (scales[:512], torch.zeros(2048, dtype=torch.uint8)[::2], scales.view(torch.int8), None, scales.to("meta")):
+        with pytest.raises(ValueError, match="scales of a 130 x 70"):
+            Fp8Matrix(values, bad, 130, 70)
+    for rows, cols in ((128, 70), (131, 70), (130, 0), (130, 81), (0, 70)):
+        with pytest.raises(ValueError):
+            Fp8Matrix(values, scales, rows, cols)
+
+
+def test_scale_bytes_agree_with_the_library(lib):
+    from pack3d_b200.fp8 import _scale_bytes
+    for rows, cols in ((1, 1), (128, 512), (129, 513), (300, 1100), (4096, 16384)):
+        assert _scale_bytes(rows, cols) == lib.p3d_fp8_scale_bytes(rows, cols)
