@@ -12,6 +12,7 @@ to nearest even is the only one; products are exact in fp32.  NaN and infinities
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native
 from ._validation import check_cuda
@@ -134,12 +135,15 @@ def _check_bias(bias, n, device):
         return None
     if bias.shape != (n,) or bias.device != device or bias.dtype not in _native.DTYPE_CODE:
         raise ValueError(f"bias must be {n} fp32, fp16 or bf16 values on the input's device")
+    if bias.requires_grad and torch.is_grad_enabled() or forward_ad.unpack_dual(bias).tangent is not None:
+        raise ValueError("fp8_matmul has no gradients: pass bias.detach(), or call under torch.no_grad()")
     return bias.contiguous()
 
 
 def fp8_matmul(a, b, *, bias=None, dtype=torch.bfloat16):
     """``a b^T`` (``+ bias``) as [a.rows, b.rows] of ``dtype`` (fp32, fp16, bf16) for two :class:`Fp8Matrix` of the same
-    number of columns.  Products and sums in fp32; the order of the sum depends on the extents alone."""
+    number of columns.  Products and sums in fp32; the order of the sum depends on the extents alone.  No gradients: a
+    bias that wants one is refused."""
     if not (isinstance(a, Fp8Matrix) and isinstance(b, Fp8Matrix)):
         raise ValueError("fp8_matmul takes two Fp8Matrix")
     a._check()   # the attributes may have been set since

@@ -324,3 +324,14 @@ def test_changed_parts_of_a_matrix_are_refused(cuda_device):
     for call in (lambda m: fp8_linear(x, m), lambda m: fp8_matmul(qx, m)):
         with pytest.raises(ValueError, match="16"):
             call(Fp8Matrix(odd, w.scales, 130, 64))
+
+
+def test_matmul_has_no_gradients(cuda_device):
+    from pack3d_b200 import fp8_matmul, quantize
+    a = quantize(torch.randn(5, 64, device=cuda_device))
+    bias = torch.randn(5, device=cuda_device, requires_grad=True)
+    with pytest.raises(ValueError, match="no gradients"):
+        fp8_matmul(a, a, bias=bias)
+    with torch.no_grad():
+        got = fp8_matmul(a, a, bias=bias)
+    assert torch.equal(got, fp8_matmul(a, a, bias=bias.detach()))

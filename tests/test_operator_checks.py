@@ -159,3 +159,15 @@ def test_scale_bytes_agree_with_the_library(lib):
     from pack3d_b200.fp8 import _scale_bytes
     for rows, cols in ((1, 1), (128, 512), (129, 513), (300, 1100), (4096, 16384)):
         assert _scale_bytes(rows, cols) == lib.p3d_fp8_scale_bytes(rows, cols)
+
+
+def test_matmul_bias_that_wants_a_gradient_is_refused():
+    import torch.autograd.forward_ad as forward_ad
+    from pack3d_b200.fp8 import _check_bias
+    bias = torch.zeros(3, requires_grad=True)
+    with pytest.raises(ValueError, match="no gradients"):
+        _check_bias(bias, 3, bias.device)
+    with forward_ad.dual_level(), pytest.raises(ValueError, match="no gradients"):
+        _check_bias(forward_ad.make_dual(bias.detach(), torch.ones(3)), 3, bias.device)
+    with torch.no_grad():
+        assert _check_bias(bias, 3, bias.device).shape == (3,)
