@@ -89,6 +89,9 @@ Backward backward_of(const p3d_fp8_linear &a, bool bias, void *buffer) {
 int check(const p3d_fp8_linear *a, const char *what) {
   P3D_CHECK_ARG(a != nullptr, "%s: null arguments", what);
   P3D_CHECK_ARG(a->rows >= 1 && a->k >= 1 && a->n >= 1, "%s: extents must be positive", what);
+  // sizes of buffers stay far below 2^63
+  const int64_t most = (int64_t)1 << 30;
+  if (a->rows > most || a->k > most || a->n > most) return fail(P3D_ERR_UNSUPPORTED, "%s: extents too large", what);
   P3D_CHECK_ARG(dtype_ok(a->dtype) && dtype_ok(a->weight_dtype) && dtype_ok(a->bias_dtype), "%s: unknown dtype", what);
   return P3D_OK;
 }

@@ -171,3 +171,14 @@ def test_matmul_bias_that_wants_a_gradient_is_refused():
         _check_bias(forward_ad.make_dual(bias.detach(), torch.ones(3)), 3, bias.device)
     with torch.no_grad():
         assert _check_bias(bias, 3, bias.device).shape == (3,)
+
+
+@pytest.mark.parametrize("extents", [(2 ** 62, 64, 32), (64, 2 ** 62, 32), (64, 32, 2 ** 62), (2 ** 40, 2 ** 40, 2 ** 40),
+                                     (2 ** 30 + 1, 64, 32)])
+def test_linear_extents_whose_sizes_would_overflow(lib, extents):
+    args = LINEAR.pack(*extents, DUMMY, 0, 0, 0, 2, 2, 2, 1, 1)
+    for size in (lib.p3d_fp8_linear_saved, lib.p3d_fp8_linear_fwd_workspace, lib.p3d_fp8_linear_bwd_workspace):
+        assert size(args) == 0
+    assert lib.p3d_fp8_linear_fwd(args, DUMMY, None, DUMMY, DUMMY, DUMMY, 1 << 40, None) == 2
+    assert lib.p3d_fp8_linear_bwd(args, DUMMY, DUMMY, DUMMY, DUMMY, None, DUMMY, 1 << 40, None) == 2
+    assert b"too large" in lib.p3d_last_error()
