@@ -27,8 +27,9 @@ class FeedForward(nn.Module):
             following = layers[i + 1].pre_norm if i + 1 < len(layers) else None
             x, y = layer(x, normed=y, next_norm=following, rng=(seed, step * len(layers) + i))
 
-    For serving, :meth:`keep_8bit` quantises the weights once; :meth:`forward` then runs without gradients from those
-    (a single token included) until :meth:`keep_8bit` is called again with ``keep=False``.
+    For serving, :meth:`keep_8bit` quantises the weights once; :meth:`forward` then runs without gradients and without
+    dropout from those (a single token included), in ``train()`` too, until :meth:`keep_8bit` is called again with
+    ``keep=False``.
     """
 
     def __init__(self, dim, hidden, *, norm="layer", eps=1e-6, dropout=0.0, residual_scale=0.1,
@@ -56,6 +57,7 @@ class FeedForward(nn.Module):
         for w in (self.w1, self.w2):
             nn.init.normal_(w, std=1 / math.sqrt(w.shape[1]))
         self._kept = None
+        self._kept_from = None
 
     @property
     def pre_norm(self):
@@ -67,9 +69,41 @@ class FeedForward(nn.Module):
         return NormSpec(self.post_weight, self.post_bias, self.kind, self.eps)
 
     def keep_8bit(self, keep=True):
-        """Quantise both weights now and serve from them (``keep=False``: go back to the parameters); returns self."""
-        self._kept = (quantize_weight(self.w1), quantize_weight(self.w2)) if keep else None
+        """Quantise both weights now and serve from them (``keep=False``: go back to the parameters); returns self.
+
+        Weights that change afterwards (``load_state_dict``, in-place updates, ``.to()``, another parameter in their place)
+        are quantised again by the next :meth:`forward`, into the same memory, which captured graphs read.  PyTorch counts
+        neither writes through ``.data`` nor the steps of fused optimizers: after those, call this again.  A weight that is
+        taken out (None, or of another shape) leaves what was kept of it.
+        """
+        weights = (self.w1, self.w2)
+        self._kept = tuple(quantize_weight(w) for w in weights) if keep else None
+        self._kept_from = [(w, w._version) for w in weights] if keep else None
         return self
+
+    def _apply(self, fn, recurse=True):   # .to(), .half(), ..: other values under the same parameters
+        result = super()._apply(fn, recurse)
+        if self._kept is not None:
+            self._kept_from = [(None, 0)] * 2
+        return result
+
+    def _serving(self):
+        """The kept weights, brought up to date with the parameters."""
+        weights = (self.w1, self.w2)
+        for i, (w, (seen, version)) in enumerate(zip(weights, self._kept_from)):
+            if w is seen and (w is None or w._version == version):
+                continue
+            if w is not None and w.is_cuda and w.shape == self._kept[i].shape:
+                if torch.cuda.is_current_stream_capturing():
+                    raise ValueError("weights kept in 8 bits have changed: call keep_8bit() before the capture")
+                new, old = quantize_weight(w), self._kept[i]
+                if old.device == new.device:
+                    old.values.view(torch.uint8).copy_(new.values.view(torch.uint8))
+                    old.scales.copy_(new.scales)
+                else:
+                    self._kept = (*self._kept[:i], new, *self._kept[i + 1:])
+            self._kept_from[i] = (w, 0 if w is None else w._version)
+        return self._kept
 
     def forward(self, x, *, normed=None, gate=None, next_norm=None, rng=None):
         """``(out, next_norm(out))``, the second None without ``next_norm``.  ``gate`` as for :func:`residual_norm`;
@@ -79,7 +113,7 @@ class FeedForward(nn.Module):
             raise ValueError("dropout in training needs rng=(seed, offset)")
         if self._kept is not None and torch.is_grad_enabled():
             raise ValueError("weights kept in 8 bits have no gradients: call under torch.no_grad()")
-        w1, w2 = self._kept if self._kept is not None else (self.w1, self.w2)
+        w1, w2 = self._serving() if self._kept is not None else (self.w1, self.w2)
         y = norm(x, self.pre_norm) if normed is None else normed
         h = torch.nn.functional.gelu(fp8_linear(y, w1, self.b1))
         h = fp8_linear(h, w2, self.b2)

@@ -116,3 +116,76 @@ def test_refusals(cuda_device):
     m.keep_8bit()
     with pytest.raises(ValueError, match="no_grad"):
         m(x)
+
+
+def test_kept_weights_follow_the_parameters(cuda_device):
+    """Served after the weights have changed, by whatever way PyTorch counts, the block answers as with 8-bit weights
+    kept anew; untouched, it quantises nothing."""
+    import copy
+    from pack3d_b200 import FeedForward
+
+    def block(seed):
+        torch.manual_seed(seed)
+        return FeedForward(64, 160).to(cuda_device, torch.bfloat16).eval()
+
+    x = torch.randn(9, 64, device=cuda_device, dtype=torch.bfloat16)
+    m, other = block(1).keep_8bit(), block(2)
+    with torch.no_grad():
+        first = m(x)[0]
+        assert torch.equal(first, block(1)(x)[0])
+        values = m._kept[0].values
+        assert torch.equal(m(x)[0], first) and m._kept[0].values is values
+
+        def same():
+            want = copy.deepcopy(m).keep_8bit(False)(x)[0]
+            got = m(x)[0]
+            return torch.equal(got, want) and not torch.equal(got, first)
+
+        m.load_state_dict(other.state_dict())
+        assert same() and m._kept[0].values.data_ptr() == values.data_ptr()
+        m.w1.mul_(-0.5)
+        assert same()
+        m.w2.copy_(block(3).w2)
+        assert same()
+        torch._foreach_add_([m.w1, m.w2], 0.01)
+        assert same()
+        m.load_state_dict(block(4).state_dict(), assign=True)
+        assert same()
+        m.w1 = torch.nn.Parameter(block(5).w1.detach().clone())
+        assert same()
+        m.half().to(torch.bfloat16)
+        assert same()
+        m.float()
+        x = x.float()
+        assert same()
+        assert torch.equal(copy.deepcopy(m)(x)[0], m(x)[0])
+        served = m(x)[0]
+        m.w1 = None                                   # the full weight is given up: served as before
+        m.w2.data = torch.empty(0, device=cuda_device)
+        assert torch.equal(m(x)[0], served)
+
+
+def test_graph_over_kept_weights(cuda_device):
+    """A captured forward reads the kept weights' memory: after a change and one forward its replay is the new answer;
+    capturing over weights that have changed is refused."""
+    from pack3d_b200 import FeedForward
+    torch.manual_seed(6)
+    m = FeedForward(64, 160).to(cuda_device, torch.bfloat16).eval().keep_8bit()
+    x = torch.randn(3, 64, device=cuda_device, dtype=torch.bfloat16)
+    stream = torch.cuda.Stream()
+    with torch.no_grad():
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            m(x)
+        torch.cuda.current_stream().wait_stream(stream)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = m(x)[0]
+        m.w1.mul_(-0.5)
+        want = m(x)[0]
+        graph.replay()
+        assert torch.equal(out, want)
+        m.w1.mul_(-0.5)
+        with pytest.raises(ValueError, match="before the capture"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                m(x)
