@@ -571,3 +571,57 @@ def test_tangents_are_refused(cuda_device):
     for transform in (lambda f: torch.func.jvp(f, (x,), (x,)),):
         with pytest.raises(NotImplementedError, match="forward-mode"):
             transform(lambda t: norm(t, NormSpec()))
+
+
+def keep_mask_at_once(rows, dim, p, rng):
+    """keep_mask over arrays."""
+    import numpy as np
+    seed, offset = rng
+    n = rows * -(-dim // 8)
+    block = np.arange(n, dtype=np.uint64)
+    low, half = np.uint64(LOW), np.uint64(32)
+    c = [block & low, block >> half, np.full(n, offset & LOW, np.uint64), np.full(n, offset >> 32 & LOW, np.uint64)]
+    k = [seed & LOW, seed >> 32 & LOW]
+    for _ in range(10):
+        p0, p1 = np.uint64(0xD2511F53) * c[0], np.uint64(0xCD9E8D57) * c[2]
+        c = [(p1 >> half) ^ c[1] ^ np.uint64(k[0]), p1 & low, (p0 >> half) ^ c[3] ^ np.uint64(k[1]), p0 & low]
+        k = [(k[0] + 0x9E3779B9) & LOW, (k[1] + 0xBB67AE85) & LOW]
+    fields = np.stack([f for w in c for f in (w & np.uint64(0xFFFF), w >> np.uint64(16))], 1)
+    return torch.from_numpy(fields.reshape(rows, -1)[:, :dim] >= round(65536 * p))
+
+
+def test_keep_masks_agree():
+    assert torch.equal(keep_mask_at_once(7, 43, 0.3, (1 << 40, 5)), keep_mask(7, 43, 0.3, (1 << 40, 5)))
+
+
+# Samples of so many rows that the forward multiplies a sample's gate into the norm's parameters: few samples, each over
+# many CTAs, and many, several to a CTA; one group of rows a CTA and eight.
+FOLDED = [(2, 160001, 40), (1184, 257, 40), (2, 100001, 37), (1184, 260, 37), (1184, 131, 200), (2, 40003, 195), (1184, 9, 2056),
+          (3, 2401, 4096), (5, 3001, 1001)]
+
+
+@pytest.mark.parametrize("shape", FOLDED)
+@pytest.mark.parametrize("act,kind,post,p,scale", [("sigmoid", "layer", True, 0.25, True), ("tanh", "rms", True, 0.0, 0.5),
+                                                   ("sigmoid", "rms", False, 0.25, False), ("identity", "layer", False, 0.0, True)])
+def test_folded_sample_gate(cuda_device, monkeypatch, shape, act, kind, post, p, scale):
+    import sys
+    monkeypatch.setattr(sys.modules[__name__], "keep_mask", keep_mask_at_once)
+    dtype = torch.bfloat16 if shape[1] % 2 else torch.float32
+    check_residual(cuda_device, shape, dtype, kind, "sample", act, p, post, scale=scale, seed=shape[1])
+
+
+@pytest.mark.parametrize("act", ["sigmoid", "tanh"])
+@pytest.mark.parametrize("dim", [40, 37, 200, 4096])
+def test_folded_sample_gate_is_the_gate_of_each_row(cuda_device, act, dim):
+    """The same rows with the gate given for each element: only the order of two multiplications differs."""
+    from pack3d_b200 import NormSpec, residual_norm
+    batch, tokens = (2, 80000) if dim < 300 else (2, 6000)
+    g = torch.Generator(device=cuda_device).manual_seed(dim)
+    x, h = (torch.randn(batch, tokens, dim, device=cuda_device, generator=g) for _ in range(2))
+    gate = torch.randn(batch, 1, dim, device=cuda_device, generator=g)
+    w, s = (torch.randn(dim, device=cuda_device, generator=g) for _ in range(2))
+    run = lambda gate: residual_norm(x, h, post_norm=NormSpec(w), gate=gate, gate_activation=act, scale=s,  # noqa: E731
+                                     next_norm=NormSpec(), p=0.25, rng=(3, 4))
+    for a, b in zip(run(gate), run(gate.expand(x.shape).contiguous())):
+        # eight fp32 roundings of values up to the size of either, and as much again in the deviation that divides y
+        assert ((a - b).abs() <= 2.0 ** -20 * (b.abs() + x.abs() + 1)).all()
