@@ -625,3 +625,26 @@ def test_folded_sample_gate_is_the_gate_of_each_row(cuda_device, act, dim):
     for a, b in zip(run(gate), run(gate.expand(x.shape).contiguous())):
         # eight fp32 roundings of values up to the size of either, and as much again in the deviation that divides y
         assert ((a - b).abs() <= 2.0 ** -20 * (b.abs() + x.abs() + 1)).all()
+
+
+@pytest.mark.parametrize("post,nxt", [("rms", "layer"), ("layer", "rms")])
+@pytest.mark.parametrize("dim", [96, 101, 1032])
+@pytest.mark.parametrize("p", [0.0, 0.25])
+def test_norms_of_two_kinds(cuda_device, post, nxt, dim, p):
+    from pack3d_b200 import NormSpec, residual_norm
+    shape, rng = (3, 7, dim), (5, 6)
+    keep = keep_mask(21, dim, p, rng).view(shape).to(cuda_device) if p else None
+    leaves = [make(shape, torch.float32, cuda_device, 1, 0.3, 1.5), make(shape, torch.float32, cuda_device, 2, -0.2, 0.7)]
+    leaves += [make((dim,), torch.float32, cuda_device, 3 + i, 1.0, 0.2) for i in range(3)]
+    leaves = [t.requires_grad_() for t in leaves]
+    exact = [t.detach().double().requires_grad_() for t in leaves]
+    x, h, pw, nw, s = leaves
+    got = residual_norm(x, h, post_norm=NormSpec(pw, None, post), scale=s, next_norm=NormSpec(nw, None, nxt), p=p, rng=rng)
+    x, h, pw, nw, s = exact
+    want = plain_residual(x, h, (pw, None, post, 1e-6), None, None, s, (nw, None, nxt, 1e-6), keep, 1 / (1 - p))
+    up = [make(shape, torch.float32, cuda_device, 7 + i) for i in range(2)]
+    for a, b in zip(got, want):
+        close(a, b, torch.float32)
+    for i, (a, b) in enumerate(zip(torch.autograd.grad(got, leaves, up),
+                                   torch.autograd.grad(want, exact, [u.double() for u in up]))):
+        close(a, b, torch.float32, 1 if i < 2 else 21)
