@@ -508,7 +508,7 @@ P3D_API int p3d_fp8_matmul(const void *a, int64_t a_pitch, const void *a_scales,
  *   p3d_fp8_linear_saved() bytes for the backward (may be NULL without gradients): x with blocks of 128
  *   rows, the weight transposed.
  * p3d_fp8_linear_bwd: dx [rows, k] of dtype, dw [n, k] of weight_dtype, dbias [n] of bias_dtype or NULL.
- * saved and workspace (p3d_fp8_linear_*_workspace() bytes) are 256-byte aligned.
+ * saved and workspace (p3d_fp8_linear_*_workspace() bytes) are 256-byte aligned; extents are up to 2^30.
  */
 typedef struct {
   int64_t rows, k, n;

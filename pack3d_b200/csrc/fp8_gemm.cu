@@ -16,7 +16,7 @@
 //                   no room for a second beside the scales: the epilogue takes it to registers at
 //                   once and frees it.  Rows go out through shared memory by TMA.  Measured on B200:
 //                   16384 x 2048 x 8192 177 us (3.1 PFLOP/s), 16384 x 8192 x 2048 209 us (2.6),
-//                   262144 x 768 x 192 122 us (bound by the 402 MB it writes: 105 us at the 3.85 TB/s of a fill).
+//                   262144 x 768 x 192 122 us (bound by the 402 MB it writes: 105 us at the 3.8 TB/s of a fill).
 //   narrow kernel   up to 128 rows of `a` (tokens of a decode step) are the N side: the weight's rows
 //                   fill the 128 lanes and the token count only sets N.  The CTAs of a cluster each take a
 //                   part of k and add them through each other's shared memory.  Up to 32 tokens
@@ -168,11 +168,6 @@ struct NarrowParams {
   const void *bias;
   int out_type, bias_type, stages;
 };
-
-template <int BN>
-__device__ __forceinline__ uint32_t narrow_stage_bytes(bool fused) {
-  return kTileM * kSlice + (fused ? 0 : BN * kSlice) + 1024u;
-}
 
 // Blocks of x in slices [begin, end) into the layout that TMA would give them: 128-byte rows, 16-byte piece j of row r
 // at j ^ (r % 8); scale bytes in the order of fp8.cu's, from group begin / 4 on.

@@ -207,9 +207,9 @@ Shape shape_for(const p3d_residual &p, bool backward) {
   return best;
 }
 
-// How the rows are cut over the CTAs: contiguous slices of the whole or, with a gate for each sample in the
-// backward, of every sample, so that the sample's gradient is summed in registers.  per_sm: CTAs an SM
-// is meant to hold.
+// How the rows are cut over the CTAs: contiguous slices of the whole or, by_sample, of every sample that has a gate of its
+// own: always in the backward, so that the sample's gradient is summed in registers, and in the forward
+// where the gate is folded into the parameters.  per_sm: CTAs an SM is meant to hold.
 struct Split {
   int64_t segments, slices, segment_rows, ctas;
 };
@@ -392,9 +392,9 @@ extern "C" int p3d_residual_fwd(const p3d_residual *args, void *out, void *y, fl
   Split c = split_of(p, s, info.sm_count, per_sm, false);
   if (p.gate_mode == P3D_GATE_SAMPLE) {
     // A CTA that has at least kFoldRows turns of a sample's rows sets that sample's parameters up (524288 x 192, two
-    // samples: 163 us, read and activated for each row 185 us), where cutting the rows by sample leaves the longest
+    // samples: 166 us, read and activated for each row 185 us), where cutting the rows by sample leaves the longest
     // CTA at most a sixth more of them (16 % more, 512 samples of 1024 x 192: 190 us against 208; 48 % more, 200 of
-    // 64 x 4096: 320 against 262).
+    // 64 x 4096: 320 against about 260).
     const Split by_sample = split_of(p, s, info.sm_count, per_sm, true);
     const int64_t at_once = by_sample.ctas / by_sample.slices, turns = (by_sample.segments + at_once - 1) / at_once;
     const int64_t rows = (by_sample.segment_rows + by_sample.slices - 1) / by_sample.slices;

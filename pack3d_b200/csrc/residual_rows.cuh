@@ -2,8 +2,9 @@
 // of their backward; instantiated for each type in residual_{f32,f16,bf16}.cu.
 //
 // One pass over the data in each direction, bound by HBM: forward 4 (x, h, out, y) and backward 6 (x, h,
-// dout, dy, dx, dh) values an element, plus the gate's.  A row is held by 32 to 512 threads, eight
-// columns each (up to eight CTAs of a cluster for the widest rows), so the row statistics cost shuffles
+// dout, dy, dx, dh) values an element, plus the gate's.  A row is held by 8 or 16 lanes of a warp with up to 24
+// columns each (forward, up to 384 columns) to 512 threads of each of up to eight CTAs of a cluster, with 16 columns
+// a thread in the forward and eight in the backward (rows_layout.cuh), so the row statistics cost shuffles
 // and no second read.  Row groups of a CTA work independently: each has a ring of row batches in shared
 // memory that bulk copies fill ahead of it, so the bytes in flight do not depend on how many
 // warps fit beside the column sums' registers.  A warp waits for a batch for 2 s at most: if that runs out it
@@ -21,9 +22,10 @@
 // multiplied once, and a sample's gate is activated once (364 -> 284 us at 524288 x 192, 120 -> 97 us at 8192 x
 // 4096).
 //
-// Measured on B200 (bf16): 524288 x 192 layer norm, sample gate and dropout, forward 163 us, backward 287 us; 8192 x
-// 4096 RMS norm, token gate, 53 and 99 us; norm by itself 16384 x 4096 50 and 80 us.  Forward at 4.9 to 5.4,
-// backward at 4.1 to 4.9 TB/s: both are bound by issue before HBM, the backward because its column sums leave
+// Measured on B200 (bf16): 524288 x 192 layer norm, sample gate and dropout, forward 166 us, backward 305 us (287 before
+// dropped values were kept out of its sums when they are infinite and waits that run out ended a warp's
+// stores); 8192 x 4096 RMS norm, token gate, 55 and 99 us; norm by itself 16384 x 4096 51 and 79 us.  Forward at 4.9 to
+// 5.2, backward at 4.0 to 5.1 TB/s: both are bound by issue before HBM, the backward because its column sums leave
 // room for 512 threads an SM only.
 //
 // What a call does not have (a norm, a bias, a gate) is a neutral value in the same formula.  Only what
@@ -539,7 +541,8 @@ __device__ __forceinline__ Ring<T, ALIGNED, NU, STATS> start_ring(const Args &a,
 }
 
 // ------------------------------------------------------------------------ pieces of the formula
-// 16-bit types take the sigmoid's exponential from the fast unit (a few 2^-22 off, against their 2^-9).
+// 16-bit types take the sigmoid's exponential from the fast unit, whose error grows with |g|: two ulp near zero, 2 + 1.2
+// |g| of them elsewhere (2^-19 of the value at 20), against the 2^-9 and 2^-12 of their results.
 template <typename T>
 __device__ __forceinline__ float activate(float g, int act) {
   if (act == P3D_ACT_SIGMOID) return __fdividef(1.f, 1.f + (sizeof(T) == 2 ? __expf(-g) : expf(-g)));

@@ -25,7 +25,7 @@ constexpr int kMaxGroups = 8;
 //   Forward: up to 384 columns a warp holds several rows, on 8 or 16 lanes with one or three units each, so that
 //   sums take three or four steps for all of them and the bookkeeping is shared; wider rows take two
 //   units a thread and up to 256 threads.  (524288 x 192 bf16 with dropout: one row a warp 388 us,
-//   four rows 223 us; 163 us since with leaner bookkeeping and the gate folded into the parameters.)
+//   four rows 223 us; 166 us since with leaner bookkeeping and the gate folded into the parameters.)
 //   Backward: a row a warp at least and one unit, whose column sums fill the registers already.  At most 512
 //   threads a row, 256 in 32 bits, where two stages of five arrays of 4096 columns would not fit
 //   beside the parameters.
