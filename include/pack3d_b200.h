@@ -72,8 +72,9 @@ P3D_API int p3d_device_count(void);
  * bounded wait inside a tensor-core kernel timed out and the kernel unwound; bits
  * 1-4 name the waiting role (2 TMA producer, 4 MMA issuer, 8 softmax / epilogue,
  * 16 a drain before tensor memory is freed); bit 5 (32): a peer-exchange wait
- * (p3d_peer_wait) ran out.  Synchronises with the device.  No
- * reference counterpart (the Triton kernels have no device-side waits). */
+ * (p3d_peer_wait) ran out; bit 6 (64): a page of a p3d_cache table lies outside its
+ * pages.  Synchronises with the device.  No reference counterpart (the Triton kernels
+ * have no device-side waits). */
 P3D_API int p3d_device_errors(unsigned *flags);
 
 /*
@@ -525,6 +526,96 @@ P3D_API int p3d_fp8_linear_fwd(const p3d_fp8_linear *args, const void *x, const 
                        void *workspace, size_t workspace_bytes, void *stream);
 P3D_API int p3d_fp8_linear_bwd(const p3d_fp8_linear *args, const void *dy, const void *saved, void *dx, void *dw,
                        void *dbias, void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * Attention over ordered sequences (pack3d_b200.sequence, pack3d_b200.cache).  No counterpart in the
+ * reference, whose attention is over a geometry of fine blocks and summaries.
+ *
+ * p3d_norm_rotate: for each token and head, y = R(N(x) * weight + bias), N as in p3d_residual over the
+ *   head's dim columns (P3D_NORM_NONE: y = R(x)), R turning columns (2 i, 2 i + 1) of an axis by position * base^(-i /
+ *   pairs[axis]) radians; the axes' pairs follow one another, and columns past the last pair are not
+ *   turned.  Two inputs (queries and keys) share tokens and positions; heads[1] may be 0.  x[i] is read at x + t *
+ *   token_stride + h * head_stride (elements; the dim columns are consecutive), outputs are contiguous [tokens, heads[i],
+ *   dim].  Token t is at row t % position_rows of positions (int64, or int32 with position_bytes 4).  Angles are
+ *   products of whole numbers in 2^-64 turns: exact at any position.  dim even, 2 .. 256; base at least 1.
+ * p3d_norm_rotate_bwd: dx[i] contiguous like the outputs (NULL: not written), dweight[i] and dbias[i] [dim] in
+ *   param_dtype[i] (or NULL), summed over tokens and heads in fp32 in a fixed order.  dy[i] is contiguous.
+ */
+typedef struct {
+  const void *x[2], *weight[2], *bias[2];
+  int64_t token_stride[2], head_stride[2];
+  const void *positions;
+  int64_t position_stride, axis_stride, tokens, position_rows;
+  double base;
+  int32_t heads[2], kind[2], param_dtype[2];
+  float eps[2];
+  int32_t dim, dtype, axes, position_bytes;
+  int32_t pairs[3];
+} p3d_norm_rotate;
+P3D_API int p3d_norm_rotate_fwd(const p3d_norm_rotate *args, void *y0, void *y1, void *stream);
+P3D_API size_t p3d_norm_rotate_bwd_workspace(const p3d_norm_rotate *args);
+P3D_API int p3d_norm_rotate_bwd(const p3d_norm_rotate *args, const void *const dy[2], void *const dx[2],
+                        void *const dweight[2], void *const dbias[2], void *workspace, size_t workspace_bytes,
+                        void *stream);
+
+/*
+ * p3d_sequence: attention over sequences packed one behind the other.  q [q_rows, heads, dim], k and v [k_rows,
+ *   kv_heads, dim] with strides in elements (multiples of 8; the dim columns consecutive; addresses 16-byte aligned), f16
+ *   or bf16, dim a multiple of 8 up to 128.  Sequence b has the rows offsets[b] .. offsets[b + 1] (int32 on the
+ *   device, not decreasing, the first taken as 0).  out[i] = sum_j p_ij v_j, p_i = softmax over the keys j that row i sees of
+ *   scale q_i k_j: all of its sequence, or with `causal` those up to j = i + (keys - queries), so that the last query sees
+ *   the last key.  A row that sees no key, and rows behind the last sequence, are 0.  lse [heads, q_rows] fp32: the natural
+ *   logarithm of each row's sum of exp (-inf where it sees no key), or NULL.
+ *   Offsets that decrease or lie past the rows are cut to the rows: no access leaves the tensors.
+ * p3d_sequence_bwd: dq, dk, dv contiguous (NULL: not written) from out, lse and dout (contiguous); rows behind the last
+ *   sequence get 0.  Every sum has a fixed order: bitwise repeatable.
+ */
+typedef struct {
+  const void *q, *k, *v;
+  int64_t q_stride[2], k_stride[2], v_stride[2]; /* token, head */
+  const int32_t *q_offsets, *k_offsets;          /* [sequences + 1] */
+  int64_t q_rows, k_rows;
+  int32_t sequences, heads, kv_heads, dim, dtype, causal;
+  float scale;
+} p3d_sequence;
+P3D_API int p3d_sequence_fwd(const p3d_sequence *args, void *out, float *lse, void *stream);
+P3D_API size_t p3d_sequence_bwd_workspace(const p3d_sequence *args);
+P3D_API int p3d_sequence_bwd(const p3d_sequence *args, const void *out, const float *lse, const void *dout, void *dq,
+                     void *dk, void *dv, void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * p3d_cache: keys and values in pages.  k, v [pages, kv_heads, page_size, dim] contiguous, of f16, bf16 or fp32, or e4m3
+ *   (P3D_E4M3) with a byte e + 127 in k_scales, v_scales [pages, kv_heads, page_size] for each token and head: the value
+ *   is v * 2^e, e the smallest integer with amax / 2^e <= 448 (at least -126, 0 for zeros), as in p3d_fp8_quantize.
+ *   Token i of sequence b is in place i % page_size of page table[b * table_stride + i / page_size].  dim is a multiple of
+ *   8 up to 256.  Tables, offsets and lengths are int32 on the device.  A page outside [0, pages) is neither read nor
+ *   written; it sets bit 6 (64) of p3d_device_errors.  The same holds for places past table_width pages.
+ * p3d_cache_append: row offsets[b] + i of new_k, new_v (of `dtype`; [rows, kv_heads, dim], strides in elements) becomes
+ *   token starts[b] + i of sequence b.  Rows outside the sequences are not read; two rows for one place leave
+ *   either of them.
+ * p3d_cache_read: token starts[b] + i (starts NULL: i) of sequence b into row offsets[b] + i of out_k, out_v [rows, kv_heads, dim]
+ *   (contiguous, `dtype`); rows outside the sequences are set to 0, rows of bad pages to NaN.
+ * p3d_paged_attention: q [sequences, heads, dim] (f16 or bf16, the cache's dtype where that is 16-bit; strides as above),
+ *   out contiguous: attention of each sequence's one query over the tokens 0 .. lengths[b] of the cache; 0 where that is none,
+ *   NaN where it meets a bad page.  dim up to 128.  workspace: p3d_paged_attention_workspace() bytes.
+ */
+#define P3D_E4M3 3
+typedef struct {
+  void *k, *v;
+  uint8_t *k_scales, *v_scales;
+  const int32_t *table;
+  int64_t pages, table_stride;
+  int32_t table_width, sequences, kv_heads, page_size, dim, dtype;
+} p3d_cache;
+P3D_API int p3d_cache_append(const p3d_cache *cache, const void *new_k, const int64_t k_stride[2], const void *new_v,
+                     const int64_t v_stride[2], int dtype, int64_t rows, const int32_t *starts, const int32_t *offsets,
+                     void *stream);
+P3D_API int p3d_cache_read(const p3d_cache *cache, const int32_t *starts, const int32_t *offsets, int64_t rows, void *out_k,
+                   void *out_v, int dtype, void *stream);
+P3D_API size_t p3d_paged_attention_workspace(const p3d_cache *cache, int heads);
+P3D_API int p3d_paged_attention(const p3d_cache *cache, const void *q, const int64_t q_stride[2], int dtype, int heads,
+                        const int32_t *lengths, float scale, void *out, void *workspace, size_t workspace_bytes,
+                        void *stream);
 
 #ifdef __cplusplus
 }

@@ -130,6 +130,16 @@ _SIGNATURES = {
     "p3d_fp8_linear_bwd_workspace": (ctypes.c_size_t, [_vp]),
     "p3d_fp8_linear_fwd": (_c_int, [_vp] * 6 + [ctypes.c_size_t, _vp]),
     "p3d_fp8_linear_bwd": (_c_int, [_vp] * 7 + [ctypes.c_size_t, _vp]),
+    "p3d_norm_rotate_fwd": (_c_int, [_vp] * 4),
+    "p3d_norm_rotate_bwd_workspace": (ctypes.c_size_t, [_vp]),
+    "p3d_norm_rotate_bwd": (_c_int, [_vp] * 6 + [ctypes.c_size_t, _vp]),
+    "p3d_sequence_fwd": (_c_int, [_vp] * 4),
+    "p3d_sequence_bwd_workspace": (ctypes.c_size_t, [_vp]),
+    "p3d_sequence_bwd": (_c_int, [_vp] * 8 + [ctypes.c_size_t, _vp]),
+    "p3d_cache_append": (_c_int, [_vp] * 5 + [_c_int, _c_i64] + [_vp] * 3),
+    "p3d_cache_read": (_c_int, [_vp] * 3 + [_c_i64, _vp, _vp, _c_int, _vp]),
+    "p3d_paged_attention_workspace": (ctypes.c_size_t, [_vp, _c_int]),
+    "p3d_paged_attention": (_c_int, [_vp] * 3 + [_c_int, _c_int, _vp, _c_f32, _vp, _vp, ctypes.c_size_t, _vp]),
     "p3d_peer_alloc": (_c_int, [ctypes.c_size_t, ctypes.POINTER(_vp), _vp]),
     "p3d_peer_free": (_c_int, [_vp]),
     "p3d_peer_open": (_c_int, [_vp, ctypes.POINTER(_vp)]),

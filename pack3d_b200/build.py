@@ -1,5 +1,5 @@
 """Build ``libpack3d_b200.so`` in-tree from ``csrc/*.cu`` with nvcc for sm_100a, and the PyTorch host module
-``pack3d_b200_host`` from ``csrc/host.cpp`` with g++.
+``pack3d_b200_host`` from ``csrc/host*.cpp`` with g++.
 
     python -m pack3d_b200.build            # incremental
     python -m pack3d_b200.build --force    # rebuild everything
@@ -60,24 +60,37 @@ def host_path():
     return LIB.parent / ("pack3d_b200_host" + sysconfig.get_config_var("EXT_SUFFIX"))
 
 
-def _build_host():
-    import torch
+def _gxx():
     gxx = shutil.which("g++")
     if not gxx:
         raise RuntimeError("g++ not found; it is required to build the host module of pack3d_b200")
+    return gxx
+
+
+def _compile_host(source, obj):
+    import torch
     home = Path(torch.__file__).parent
     cuda = Path(nvcc()).resolve().parents[1]
     system = [home / "include", home / "include" / "torch" / "csrc" / "api" / "include", cuda / "include",
               Path(sysconfig.get_paths()["include"])]
-    cmd = [gxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+    cmd = [_gxx(), "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", str(INCLUDE)]
     for path in system:
         cmd += ["-isystem", str(path)]
-    cmd += [str(SRC / "host.cpp"), "-o", str(host_path()), "-L", str(LIB.parent), f"-l:{LIB.name}", "-Wl,-rpath,$ORIGIN",
-            "-L", str(home / "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda"]
+    run = subprocess.run([*cmd, "-c", str(source), "-o", str(obj)], capture_output=True, text=True)
+    if run.returncode != 0:
+        raise RuntimeError(f"g++ failed for {source.name}:\n{run.stderr}")
+
+
+def _link_host(objects):
+    import torch
+    home = Path(torch.__file__).parent
+    cmd = [_gxx(), "-shared", *map(str, objects), "-o", str(host_path()), "-L", str(LIB.parent), f"-l:{LIB.name}",
+           "-Wl,-rpath,$ORIGIN", "-L", str(home / "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10",
+           "-lc10_cuda"]
     run = subprocess.run(cmd, capture_output=True, text=True)
     if run.returncode != 0:
-        raise RuntimeError(f"g++ failed for host.cpp:\n{run.stderr}")
+        raise RuntimeError(f"linking the host module failed:\n{run.stderr}")
 
 
 def build(force=False, verbose=False, jobs=None):
@@ -104,8 +117,14 @@ def build(force=False, verbose=False, jobs=None):
         run = subprocess.run(cmd, capture_output=True, text=True)
         if run.returncode != 0:
             raise RuntimeError(f"link failed:\n{run.stderr}")
-    if force or _stale(host_path(), [SRC / "host.cpp", *INCLUDE.glob("*.h")]):
-        _build_host()
+    host_sources = sorted(SRC.glob("host*.cpp"))
+    host_objects = [BUILD / (src.stem + ".host.o") for src in host_sources]
+    host_headers = [*SRC.glob("*.h"), *INCLUDE.glob("*.h")]
+    host_todo = [(src, obj) for src, obj in zip(host_sources, host_objects) if force or _stale(obj, [src, *host_headers])]
+    with ThreadPoolExecutor(max_workers=jobs or min(8, os.cpu_count() or 1)) as pool:
+        list(pool.map(lambda so: _compile_host(*so), host_todo))
+    if force or host_todo or _stale(host_path(), host_objects):
+        _link_host(host_objects)
     return LIB
 
 
