@@ -586,7 +586,7 @@ P3D_API int p3d_sequence_bwd(const p3d_sequence *args, const void *out, const fl
 /*
  * p3d_cache: keys and values in pages.  k, v [pages, kv_heads, page_size, dim] contiguous, of f16, bf16 or fp32, or e4m3
  *   (P3D_E4M3) with a byte e + 127 in k_scales, v_scales [pages, kv_heads, page_size] for each token and head: the value
- *   is v * 2^e, e the smallest integer with amax / 2^e <= 448 (at least -126, 0 for zeros), as in p3d_fp8_quantize.
+ *   is v * 2^e, e the smallest integer from -126 on with amax / 2^e <= 448, amax the largest finite magnitude of the dim values.
  *   Token i of sequence b is in place i % page_size of page table[b * table_stride + i / page_size].  dim is a multiple of
  *   8 up to 256.  Tables, offsets and lengths are int32 on the device.  A page outside [0, pages) is neither read nor
  *   written; it sets bit 6 (64) of p3d_device_errors.  The same holds for places past table_width pages.
@@ -597,7 +597,8 @@ P3D_API int p3d_sequence_bwd(const p3d_sequence *args, const void *out, const fl
  *   (contiguous, `dtype`); rows outside the sequences are set to 0, rows of bad pages to NaN.
  * p3d_paged_attention: q [sequences, heads, dim] (f16 or bf16, the cache's dtype where that is 16-bit; strides as above),
  *   out contiguous: attention of each sequence's one query over the tokens 0 .. lengths[b] of the cache; 0 where that is none,
- *   NaN where it meets a bad page.  dim up to 128.  workspace: p3d_paged_attention_workspace() bytes.
+ *   NaN where it meets a bad page.  dim up to 128.  A value's weight over 8 bits is held in f16 relative to the largest
+ *   weight times 2^e.  workspace: p3d_paged_attention_workspace() bytes, 16-byte aligned.
  */
 #define P3D_E4M3 3
 typedef struct {

@@ -1,6 +1,7 @@
 // Keys and values written into pages as they are or in 8 bits, and read back.
 //
-//     8 bits: e the smallest integer with amax / 2^e <= 448 over a token's dim values of one head, e4m3(x / 2^e) and a byte e + 127
+//     8 bits: e the smallest integer from -126 on with amax / 2^e <= 448 over a token's dim values of one head, e4m3(x / 2^e) and a
+//     byte e + 127
 //
 // The scale is a power of two, so scaling is exact and e4m3's rounding the only one; it belongs to one token and head, so that a
 // token is written once and its neighbours in the page never change.
@@ -96,7 +97,7 @@ __global__ void __launch_bounds__(kWarps * 32) append_kernel(const __grid_consta
           } else {
             m = quant::widest<T>(m);
           }
-          const uint32_t byte = quant::scale_byte(m);
+          const uint32_t byte = m ? quant::scale_byte(m) : 1u;
           if (write) {
             *reinterpret_cast<uint2 *>(static_cast<uint8_t *>(which ? p.c.v : p.c.k) + to * p.c.dim + col) =
                 quant::quantize8<true, T>(raw[u], quant::inverse_scale(byte));
