@@ -560,8 +560,8 @@ P3D_API int p3d_norm_rotate_bwd(const p3d_norm_rotate *args, const void *const d
 
 /*
  * p3d_sequence: attention over sequences packed one behind the other.  q [q_rows, heads, dim], k and v [k_rows,
- *   kv_heads, dim] with strides in elements (multiples of 8; the dim columns consecutive; addresses 16-byte aligned), f16
- *   or bf16, dim a multiple of 8 up to 128.  Sequence b has the rows offsets[b] .. offsets[b + 1] (int32 on the
+ *   kv_heads, dim] with strides in elements (positive multiples of 8; the dim columns consecutive; addresses 16-byte aligned),
+ *   f16 or bf16, dim a multiple of 8 up to 128.  Sequence b has the rows offsets[b] .. offsets[b + 1] (int32 on the
  *   device, not decreasing, the first taken as 0).  out[i] = sum_j p_ij v_j, p_i = softmax over the keys j that row i sees of
  *   scale q_i k_j: all of its sequence, or with `causal` those up to j = i + (keys - queries), so that the last query sees
  *   the last key.  A row that sees no key, and rows behind the last sequence, are 0.  lse [heads, q_rows] fp32: the natural

@@ -341,6 +341,7 @@ int p3d_device_errors(unsigned *flags) {
   if (int st = take_row_errors(flags)) return st;
   if (int st = take_cache_errors(flags)) return st;
   if (int st = take_paged_errors(flags)) return st;
+  if (int st = take_sequence_errors(flags)) return st;
   return take_bwd_errors(flags);
 }
 

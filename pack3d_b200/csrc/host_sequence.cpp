@@ -27,11 +27,13 @@ bool flag(PyObject *o, const char *what) {
   return o == Py_True;
 }
 
-// Rows of dim consecutive elements, 16-byte aligned with strides to match: as it is, or a copy.
+// Rows of dim consecutive elements, 16-byte aligned with strides to match: as it is, or a copy. Rows that share memory are
+// copied too: a tensor map has no stride of 0.
 Tensor rows16(const Tensor &t) {
   const int64_t unit = 16 / t.element_size();
   bool fits = t.size(-1) == 1 || t.stride(-1) == 1;
-  for (int64_t i = 0; i + 1 < t.dim(); ++i) fits = fits && (t.size(i) <= 1 || t.stride(i) % unit == 0);
+  for (int64_t i = 0; i + 1 < t.dim(); ++i)
+    fits = fits && (t.size(i) <= 1 || (t.stride(i) % unit == 0 && t.stride(i) > 0 && t.stride(i) < 1ll << 38));
   if (fits && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0) return t;
   return t.is_contiguous() ? t.clone(at::MemoryFormat::Contiguous) : t.contiguous();
 }

@@ -104,6 +104,7 @@ int launch_quantize_both(const QuantOperand &x, const QuantOperand &w, int64_t c
 int take_row_errors(unsigned *flags);   // residual.cu
 int take_cache_errors(unsigned *flags); // cache.cu
 int take_paged_errors(unsigned *flags); // paged.cu
+int take_sequence_errors(unsigned *flags); // sequence.cu
 // out[c] (of dtype) = sum over i < count of partials[i, c], in a fixed order (residual.cu)
 int launch_column_join(const float *partials, void *out, int dtype, int64_t count, int dim, cudaStream_t s);
 

@@ -3,7 +3,8 @@
 
 #include <algorithm>
 
-#include "sequence.cuh"
+#include "kernels.cuh"
+#include "seq_tc.cuh"
 
 namespace p3d {
 namespace {
@@ -21,31 +22,6 @@ template <typename T> __device__ __forceinline__ void store4(T *row, int lane, i
 }
 __device__ __forceinline__ float dot4(const float (&a)[4], const float (&b)[4]) {
   return warp_sum(a[0] * b[0] + a[1] * b[1] + a[2] * b[2] + a[3] * b[3]);
-}
-
-template <typename T>
-__global__ void fwd_kernel(const __grid_constant__ p3d_sequence a, T *out, float *lse) {
-  const int64_t item = (int64_t)blockIdx.x * kWarps + threadIdx.x / 32;
-  const int lane = threadIdx.x & 31, h = (int)(item % a.heads), t = (int)(item / a.heads);
-  if (t >= a.q_rows) return;
-  const int b = cache::sequence_of(a.q_offsets, a.sequences, (int)a.q_rows, t), g = h / (a.heads / a.kv_heads);
-  const seq::Range r = seq::range_of(a, b);
-  const int n = t - r.q0 < r.nq ? seq::seen_by(r, t - r.q0, a.causal) : 0;
-  float q[4], o[4] = {0.f, 0.f, 0.f, 0.f}, k[4], v[4], m = -INFINITY, l = 0.f;
-  load4(static_cast<const T *>(a.q) + t * a.q_stride[0] + h * a.q_stride[1], lane, a.dim, q);
-  for (int j = 0; j < n; ++j) {
-    load4(static_cast<const T *>(a.k) + (int64_t)(r.k0 + j) * a.k_stride[0] + g * a.k_stride[1], lane, a.dim, k);
-    load4(static_cast<const T *>(a.v) + (int64_t)(r.k0 + j) * a.v_stride[0] + g * a.v_stride[1], lane, a.dim, v);
-    const float s = dot4(q, k) * a.scale, top = fmaxf(m, s), old = m == -INFINITY ? 0.f : expf(m - top), p = expf(s - top);
-    l = l * old + p;
-    m = top;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = o[i] * old + p * v[i];
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) o[i] = n ? o[i] / l : 0.f;
-  store4(out + ((int64_t)t * a.heads + h) * a.dim, lane, a.dim, o);
-  if (lse && lane == 0) lse[h * a.q_rows + t] = n ? m + logf(l) : -INFINITY;
 }
 
 template <typename T>
@@ -127,10 +103,20 @@ int check(const p3d_sequence *a, const char *what) {
   bool fits = aligned(a->q) && aligned(a->k) && aligned(a->v);
   for (int i = 0; i < 2; ++i) fits = fits && a->q_stride[i] % 8 == 0 && a->k_stride[i] % 8 == 0 && a->v_stride[i] % 8 == 0;
   P3D_CHECK_ARG(fits, "%s: rows must be 16-byte aligned", what);
+  // as a tensor map takes them
+  auto steps = [&](const int64_t (&stride)[2], int64_t rows, int heads) {
+    return (rows <= 1 || (stride[0] > 0 && stride[0] < 1ll << 38)) && (heads <= 1 || (stride[1] > 0 && stride[1] < 1ll << 38));
+  };
+  P3D_CHECK_ARG(steps(a->q_stride, a->q_rows, a->heads) && steps(a->k_stride, a->k_rows, a->kv_heads) &&
+                    steps(a->v_stride, a->k_rows, a->kv_heads),
+                "%s: strides must be positive and below 2^38", what);
   return P3D_OK;
 }
 
 }  // namespace seq
+
+int take_sequence_errors(unsigned *flags) { return seq::take_errors_fwd(flags); }
+
 }  // namespace p3d
 
 using namespace p3d;
@@ -141,11 +127,7 @@ int p3d_sequence_fwd(const p3d_sequence *a, void *out, float *lse, void *stream)
   if (int st = seq::check(a, "p3d_sequence_fwd")) return st;
   if (a->q_rows == 0) return P3D_OK;
   P3D_CHECK_ARG(out && aligned(out), "p3d_sequence_fwd: the output must be given and 16-byte aligned");
-  const int blocks = blocks_of(a->q_rows * a->heads);
-  if (a->dtype == P3D_F16) fwd_kernel<__half><<<blocks, kWarps * 32, 0, (cudaStream_t)stream>>>(*a, (__half *)out, lse);
-  else fwd_kernel<__nv_bfloat16><<<blocks, kWarps * 32, 0, (cudaStream_t)stream>>>(*a, (__nv_bfloat16 *)out, lse);
-  P3D_LAUNCH_CHECK();
-  return P3D_OK;
+  return seq::launch_fwd(*a, out, lse, (cudaStream_t)stream);
 }
 
 size_t p3d_sequence_bwd_workspace(const p3d_sequence *a) {
