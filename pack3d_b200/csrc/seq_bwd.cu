@@ -1,0 +1,813 @@
+// Attention over packed sequences, backward, on the tensor cores, from lse and delta_i = dout_i . out_i:
+//
+//     P = 2^(S c - lse),  dS = scale P (dO V^T - delta),  dQ = dS K,  dK = dS^T Q,  dV = P^T dO
+//
+// (dS with its scale, so that in f16 it stays in range where the gradients do.)
+//
+// Two kernels, so that each gradient is a sum in one fixed order without atomics: dQ by tiles of queries, dK and dV by tiles of keys. They make
+// S and dP both, seven products of which five are the mathematics' own; the tensor pipe bounds both at dim 128 (a tile of 128 x 128 is
+// 512 cycles a product), the exponentials at dim 64 and below.
+//
+// dQ: a CTA has 128 queries of a head; S in two buffers, dP and dQ fill the tensor memory (512 columns). dS (16-bit) goes over S. The pipe makes S
+//   and dP of the next keys while the softmax warps, in two groups of 64 columns, work on these.
+// dK, dV: a CTA has 128 keys of a KV head and goes over the queries that see them of all heads of its group: S^T = K Q^T and dP^T = V dO^T (keys
+//   on the lanes), P^T over S^T, dS^T over dP^T, both read from tensor memory by dV += P^T dO and dK += dS^T Q. Order: dV(i), S(i + 1), dK(i), dP(i + 1),
+//   so that the exponentials of the next step run beside two products. Where there are few key tiles, a group's heads are shared among
+//   several CTAs, whose sums in fp32 are added by a last kernel.
+//
+// Masks and values that are not finite: as in the forward kernel, operands of border tiles are cleared of infinities and NaN before the
+// product whose weights are 0 for rows that do not see them (K for dQ; dO and Q for dV and dK), once the products that need them
+// as they are have completed. A row that sees such a value is NaN through lse or delta; only dO's in dV are added back.
+#include <math.h>
+
+#include <algorithm>
+
+#include "seq_tc.cuh"
+
+namespace p3d {
+namespace seq {
+namespace {
+
+__device__ unsigned g_seq_bwd_errors = 0;
+
+constexpr int kMmaWarp = 8, kCopyWarp = 9, kThreads = 320, kSoftmaxWarps = 8, kBorders = 3;
+
+struct Params {
+  p3d_sequence a;
+  const float2 *stats;     // [heads][q_rows]: lse * log2(e), scale * delta
+  const void *dout;        // contiguous
+  void *dq, *dk, *dv;
+  float *part;             // [2][parts][k_rows * kv_heads * dim] where parts > 1
+  int parts;
+  int steps;               // of 16 columns
+  uint32_t idesc_out;
+  float sc;                // scale * log2(e)
+};
+
+// 64 columns of scores to weights: 2^(s sc - shift), a quarter of them by polynomial where none is masked.
+__device__ __forceinline__ float2 weight(float2 s, float2 sc, float2 minus, bool poly) {
+  const float2 x = fma2(s, sc, minus);
+  if (poly) {
+    // NaN would not come through
+    const float2 e = exp2_poly2(x);
+    return make_float2(x.x == x.x ? e.x : x.x, x.y == x.y ? e.y : x.y);
+  }
+  return make_float2(ex2_approx(x.x), ex2_approx(x.y));
+}
+
+template <int N>
+__device__ __forceinline__ void load_columns(uint32_t t, float *v) {
+#pragma unroll
+  for (int i = 0; i < N; i += 32) tmem_ld32(t + i, reinterpret_cast<uint32_t *>(v) + i);
+}
+
+// 32 columns of an accumulator into a row of T, or of fp32.
+template <typename T>
+__device__ __forceinline__ void store_columns(uint32_t t, int col, int dim, T *row, float *wide) {
+  uint32_t o[32];
+  tmem_ld32(t + col, o);
+  tmem_wait_ld();
+#pragma unroll
+  for (int k = 0; k < 32; k += 8) {
+    if (col + k >= dim) continue;
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(o[k + i]);
+    if (wide) {
+      reinterpret_cast<float4 *>(wide + col + k)[0] = make_float4(v[0], v[1], v[2], v[3]);
+      reinterpret_cast<float4 *>(wide + col + k)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else if (row) {
+      *reinterpret_cast<uint4 *>(row + col + k) =
+          make_uint4(pack<T>(v[0], v[1]), pack<T>(v[2], v[3]), pack<T>(v[4], v[5]), pack<T>(v[6], v[7]));
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------- dQ
+template <int DP>
+struct LayoutQ {
+  static constexpr uint32_t kTileBytes = DP / 64 * kBox;
+  static constexpr int kK = 3, kV = 2;   // stages
+  static constexpr size_t kBytes = 1024 + (2 + kK + kV) * (size_t)kTileBytes;
+};
+// Parity waits: each waiter of a barrier that completes many times has seen every completion before. Border tiles have barriers of
+// their own: kSeen (their S is complete), kClean (K cleared).
+enum { kQFull, kSFull, kDPFull = kSFull + 2, kDPFree, kDSFull, kDQDone, kDone, kDrainQ, kSeen, kClean = kSeen + kBorders,
+       kKFull = kClean + kBorders, kKEmpty = kKFull + 3, kVFull = kKEmpty + 3, kVEmpty = kVFull + 2, kBarsQ = kVEmpty + 2 };
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads, 1)
+    sequence_dq_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tdo,
+                       const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
+                       const __grid_constant__ Params p) {
+  using L = LayoutQ<DP>;
+  constexpr uint32_t TB = L::kTileBytes;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t bar_mem[kBarsQ];
+  __shared__ uint32_t tmem_holder;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int slot = (int)(gridDim.x / p.a.heads - 1 - blockIdx.x / p.a.heads), head = blockIdx.x % p.a.heads;   // the longest first
+  const int kv = head / (p.a.heads / p.a.kv_heads);
+  const Slot at = find_slot(p.a.q_offsets, p.a.sequences, (int)p.a.q_rows, kTile, slot);
+  const Range r = slot_range(p.a, at.sequence);
+  const int row0 = at.group * kTile;
+  if (at.group < 0 || row0 >= r.nq) return;
+  const int chunks = (seen_by(r, min(row0 + kTile, r.nq) - 1, p.a.causal) + kTile - 1) / kTile;
+  const int border = seen_by(r, row0, p.a.causal) / kTile;
+  if (chunks == 0) {
+    const int row = row0 + threadIdx.x;
+    if (threadIdx.x < kTile && row < r.nq) {
+      uint4 *to = reinterpret_cast<uint4 *>(static_cast<T *>(p.dq) + ((int64_t)(r.q0 + row) * p.a.heads + head) * p.a.dim);
+      for (int i = 0; i < p.a.dim / 8; ++i) to[i] = make_uint4(0, 0, 0, 0);
+    }
+    return;
+  }
+  const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+  const uint32_t k_ring = base + 2 * TB, v_ring = k_ring + L::kK * TB;
+  auto bar = [&](int i) { return smem_u32(&bar_mem[i]); };
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kBarsQ; ++i) mbar_init(bar(i), i == kDPFree || i == kDSFull ? kSoftmaxWarps : 1);
+    fence_mbar_init();
+  }
+  if (warp == kMmaWarp) {
+    tmem_alloc(smem_u32(&tmem_holder), 512);
+    tmem_relinquish();
+  }
+  if (warp == kCopyWarp && lane == 0) {
+    prefetch_tmap(&tq);
+    prefetch_tmap(&tdo);
+    prefetch_tmap(&tk);
+    prefetch_tmap(&tv);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_holder, t_dp = tmem + 256, t_dq = tmem + 384;   // S at 0 and 128
+
+  if (warp == kCopyWarp) {
+    bool ok = true;
+    int n_k = 0, n_v = 0;
+    if (lane == 0) {
+      auto tile = [&](uint32_t dst, const CUtensorMap *map, uint32_t full, int h, int row) {
+        mbar_expect_tx(full, TB);
+        for (int c = 0; c < DP / 64; ++c) tma_load_3d(dst + c * kBox, map, full, 64 * c, h, row);
+      };
+      mbar_expect_tx(bar(kQFull), 2 * TB);
+      for (int c = 0; c < DP / 64; ++c) {
+        tma_load_3d(base + c * kBox, &tq, bar(kQFull), 64 * c, head, r.q0 + row0);
+        tma_load_3d(base + TB + c * kBox, &tdo, bar(kQFull), 64 * c, head, r.q0 + row0);
+      }
+      for (int c = 0; c < chunks; ++c) {
+        int s = c % L::kK;
+        if (c >= L::kK && !mbar_wait(bar(kKEmpty + s), (c / L::kK - 1) & 1, &g_seq_bwd_errors, kWaitNs, kErrProducer)) {
+          ok = false;
+          break;
+        }
+        tile(k_ring + s * TB, &tk, bar(kKFull + s), kv, r.k0 + c * kTile);
+        n_k = c + 1;
+        s = c % L::kV;
+        if (c >= L::kV && !mbar_wait(bar(kVEmpty + s), (c / L::kV - 1) & 1, &g_seq_bwd_errors, kWaitNs, kErrProducer)) {
+          ok = false;
+          break;
+        }
+        tile(v_ring + s * TB, &tv, bar(kVFull + s), kv, r.k0 + c * kTile);
+        n_v = c + 1;
+      }
+    }
+    ok = __all_sync(0xffffffffu, ok);
+    for (int c = min(border, chunks); ok && c < chunks; ++c) {
+      ok = __all_sync(0xffffffffu, mbar_wait(bar(kSeen + c - border), 0, &g_seq_bwd_errors, kWaitNs, kErrProducer));
+      ok = ok && __all_sync(0xffffffffu, mbar_wait(bar(kKFull + c % L::kK), (c / L::kK) & 1, &g_seq_bwd_errors, kWaitNs, kErrProducer));
+      if (!ok) break;
+      tc_fence_after();
+      if (clear_not_finite<T>(smem_raw + (k_ring - raw) + (c % L::kK) * TB, TB)) fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(kClean + c - border));
+    }
+    if (lane == 0) {
+      mbar_wait(bar(kQFull), 0, &g_seq_bwd_errors, kWaitNs, kErrTeardown);
+      for (int i = max(0, n_k - L::kK); i < n_k; ++i)
+        mbar_wait(bar(kKFull + i % L::kK), (i / L::kK) & 1, &g_seq_bwd_errors, kWaitNs, kErrTeardown);
+      for (int i = max(0, n_v - L::kV); i < n_v; ++i)
+        mbar_wait(bar(kVFull + i % L::kV), (i / L::kV) & 1, &g_seq_bwd_errors, kWaitNs, kErrTeardown);
+    }
+  } else if (warp == kMmaWarp) {
+    if (lane == 0) {
+      const uint32_t idesc_s = idesc_f16(128, 128, std::is_same<T, __nv_bfloat16>::value, false);
+      const uint64_t d_q = desc_rows(base), d_do = desc_rows(base + TB), d_k = desc_rows(k_ring), d_v = desc_rows(v_ring),
+                     d_kc = desc_cols(k_ring);
+      int n_s = 0, n_dp = 0, n_dq = 0, n_seen = 0;
+      bool done = false;
+      auto wait = [&](int b, uint32_t parity) {
+        if (!mbar_wait(bar(b), parity, &g_seq_bwd_errors, kWaitNs, kErrMma)) return false;
+        tc_fence_after();
+        return true;
+      };
+      auto issue_s = [&](int c) {
+        const uint64_t k = d_k + ((uint32_t)(c % L::kK) * TB >> 4);
+        for (int j = 0; j < p.steps; ++j) mma_ss(tmem + 128 * (c & 1), d_q + step_rows(j), k + step_rows(j), idesc_s, j > 0);
+        mma_commit(bar(kSFull + (c & 1)));
+        ++n_s;
+        if (c >= border) {
+          mma_commit(bar(kSeen + c - border));
+          ++n_seen;
+        }
+      };
+      auto issue_dp = [&](int c) {
+        const uint64_t v = d_v + ((uint32_t)(c % L::kV) * TB >> 4);
+        for (int j = 0; j < p.steps; ++j) mma_ss(t_dp, d_do + step_rows(j), v + step_rows(j), idesc_s, j > 0);
+        mma_commit(bar(kDPFull));
+        mma_commit(bar(kVEmpty + c % L::kV));
+        ++n_dp;
+      };
+      bool ok = wait(kQFull, 0) && wait(kKFull, 0);
+      if (ok) {
+        issue_s(0);
+        ok = wait(kVFull, 0);
+        if (ok) issue_dp(0);
+      }
+      for (int c = 0; ok && c < chunks; ++c) {
+        if (c + 1 < chunks) {
+          // the buffer of S(c + 1) held dS(c - 1)
+          ok = wait(kKFull + (c + 1) % L::kK, ((c + 1) / L::kK) & 1) && (c == 0 || wait(kDQDone, (c - 1) & 1));
+          if (!ok) break;
+          issue_s(c + 1);
+          ok = wait(kVFull + (c + 1) % L::kV, ((c + 1) / L::kV) & 1) && wait(kDPFree, c & 1);
+          if (!ok) break;
+          issue_dp(c + 1);
+        }
+        ok = (c < border || wait(kClean + c - border, 0)) && wait(kDSFull, c & 1);
+        if (!ok) break;
+        const uint64_t k = d_kc + ((uint32_t)(c % L::kK) * TB >> 4);
+#pragma unroll
+        for (int j = 0; j < kTile / 16; ++j)   // each softmax group's dS lies over its own half of S
+          mma_ts(t_dq, tmem + 128 * (c & 1) + j / 4 * 64 + j % 4 * 8, k + step_cols(j), p.idesc_out, c > 0 || j > 0);
+        mma_commit(bar(kDQDone));
+        mma_commit(bar(kKEmpty + c % L::kK));
+        ++n_dq;
+      }
+      if (ok) {
+        mma_commit(bar(kDone));
+        done = true;
+      }
+      mma_commit(bar(kDrainQ));
+      auto drained = [&](int b, int times) {
+        if (times > 0) mbar_wait(bar(b), (times - 1) & 1, &g_seq_bwd_errors, kWaitNs, kErrTeardown);
+      };
+      drained(kDrainQ, 1);
+      drained(kSFull, (n_s + 1) / 2);
+      drained(kSFull + 1, n_s / 2);
+      drained(kDPFull, n_dp);
+      drained(kDQDone, n_dq);
+      drained(kDone, done);
+      for (int i = 0; i < n_seen; ++i) drained(kSeen + i, 1);
+      for (int s = 0; s < L::kK; ++s) drained(kKEmpty + s, n_dq / L::kK + (s < n_dq % L::kK));
+      for (int s = 0; s < L::kV; ++s) drained(kVEmpty + s, n_dp / L::kV + (s < n_dp % L::kV));
+    }
+  } else {
+    const int half = warp / 4, row = row0 + (warp % 4) * 32 + lane;
+    const bool there = row < r.nq;
+    const int seen = there ? seen_by(r, row, p.a.causal) : 0;
+    const float2 stat = there ? p.stats[(int64_t)head * p.a.q_rows + r.q0 + row] : make_float2(0.f, 0.f);
+    const float2 sc = make_float2(p.sc, p.sc), shift = make_float2(-stat.x, -stat.x), minus = make_float2(-stat.y, -stat.y), scale = make_float2(p.a.scale, p.a.scale);
+    const uint32_t lanes = (uint32_t)((warp % 4) * 32) << 16;
+    bool ok = true;
+    for (int c = 0; c < chunks; ++c) {
+      const uint32_t t_s = tmem + 128 * (c & 1) + 64 * half + lanes;
+      ok = wait_warp(bar(kSFull + (c & 1)), (c >> 1) & 1, &g_seq_bwd_errors, kErrSoftmax);
+      if (!ok) break;
+      float s[64];
+      load_columns<64>(t_s, s);
+      tmem_wait_ld();
+      const int limit = seen - c * kTile - half * 64;
+      const bool masked = __any_sync(0xffffffffu, limit < 64);
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        const float2 w = weight(make_float2(s[2 * i], s[2 * i + 1]), sc, shift, i % 4 == 3 && !masked);
+        s[2 * i] = w.x, s[2 * i + 1] = w.y;
+      }
+      ok = wait_warp(bar(kDPFull), c & 1, &g_seq_bwd_errors, kErrSoftmax);
+      if (!ok) break;
+      float d[64];
+      load_columns<64>(t_dp + 64 * half + lanes, d);
+      tmem_wait_ld();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(kDPFree));
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        const float2 v = mul2(make_float2(s[2 * i], s[2 * i + 1]), fma2(make_float2(d[2 * i], d[2 * i + 1]), scale, minus));
+        s[2 * i] = v.x, s[2 * i + 1] = v.y;
+      }
+      if (masked) {
+#pragma unroll
+        for (int i = 0; i < 64; ++i) s[i] = i < limit ? s[i] : 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < 32; i += 16) {
+        uint32_t pk[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) pk[k] = pack<T>(s[2 * (i + k)], s[2 * (i + k) + 1]);
+        tmem_st16(t_s + i, pk);
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(kDSFull));
+    }
+    if (ok) ok = wait_warp(bar(kDone), 0, &g_seq_bwd_errors, kErrSoftmax);
+    if (ok) {
+      T *to = there ? static_cast<T *>(p.dq) + ((int64_t)(r.q0 + row) * p.a.heads + head) * p.a.dim : nullptr;
+#pragma unroll
+      for (int i = 0; i < DP / 2; i += 32) store_columns<T>(t_dq + lanes, half * (DP / 2) + i, seen > 0 ? p.a.dim : 0, to, nullptr);
+      if (there && seen <= 0)   // a row that sees no key beside rows that do
+        for (int i = half; i < p.a.dim / 8; i += 2) reinterpret_cast<uint4 *>(to)[i] = make_uint4(0, 0, 0, 0);
+    }
+    tmem_wait_st();
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// ------------------------------------------------------------------------------- dK, dV
+template <int DP>
+struct LayoutKV {
+  static constexpr uint32_t kTileBytes = DP / 64 * kBox;
+  static constexpr int kStages = DP == 128 ? 2 : 4;
+  static constexpr uint32_t kStageBytes = 2 * kTileBytes;   // Q, dO
+  static constexpr size_t kBytes = 1024 + 2 * kTileBytes + kStages * (size_t)(kStageBytes + kTile * sizeof(float2));
+};
+enum { kKVFull, kSTFull, kDPTFull, kPFull, kDSTFull, kDVDone, kDKDone, kAllDone, kDrainKV, kSeenKV, kCleanKV, kFullKV };
+template <int DP> constexpr int bars_kv() { return kFullKV + 2 * LayoutKV<DP>::kStages; }
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads, 1)
+    sequence_dkv_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tdo,
+                        const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
+                        const __grid_constant__ Params p) {
+  using L = LayoutKV<DP>;
+  constexpr uint32_t TB = L::kTileBytes;
+  constexpr int NS = L::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t bar_mem[bars_kv<DP>()];
+  __shared__ uint32_t tmem_holder;
+  __shared__ int not_finite;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // keys at a sequence's start are seen by the most queries: in order
+  const int per_slot = p.a.kv_heads * p.parts, slot = blockIdx.x / per_slot, kv = blockIdx.x % per_slot / p.parts,
+            part = blockIdx.x % p.parts;
+  const Slot at = find_slot(p.a.k_offsets, p.a.sequences, (int)p.a.k_rows, kTile, slot);
+  Range r;
+  if (at.sequence < p.a.sequences) {
+    r = range_of(p.a, at.sequence);
+  } else {
+    r = {};
+    r.k0 = cache::offset_at(p.a.k_offsets, at.sequence, (int)p.a.k_rows);
+    r.nk = (int)p.a.k_rows - r.k0;
+  }
+  const int key0 = at.group * kTile;
+  if (at.group < 0 || key0 >= r.nk) return;
+  const int group = p.a.heads / p.a.kv_heads, head0 = kv * group + group * part / p.parts,
+            heads = kv * group + group * (part + 1) / p.parts - head0;
+  // query i sees key j where i >= j - (nk - nq)
+  const int shift = r.nk - r.nq, first = p.a.causal ? max(0, key0 - shift) : 0;
+  const int tiles = first < r.nq ? (r.nq - first + kTile - 1) / kTile : 0, steps = tiles * heads;
+  // a tile of queries from row i on with a pair of query and key that is masked
+  const int whole = p.a.causal ? min(key0 + kTile, r.nk) - 1 - shift : 0;
+  auto is_border = [&](int step) {
+    const int i = first + step % tiles * kTile;
+    return i < whole || i + kTile > r.nq;
+  };
+  const int key = key0 + (warp % 4) * 32 + lane;   // of a softmax thread
+  const bool there = key < r.nk;
+  const int64_t out_row = ((int64_t)(r.k0 + key) * p.a.kv_heads + kv) * p.a.dim;
+  const int64_t part_size = p.a.k_rows * p.a.kv_heads * p.a.dim;
+  float *const wide_k = p.parts > 1 ? p.part + part * part_size : nullptr;
+  float *const wide_v = p.parts > 1 ? p.part + (p.parts + part) * part_size : nullptr;
+  if (steps == 0) {
+    if (warp < 4 && there)
+      for (int i = 0; i < p.a.dim; i += 8) {
+        if (wide_k) {
+          for (int k = 0; k < 8; k += 4) {
+            *reinterpret_cast<float4 *>(wide_k + out_row + i + k) = make_float4(0.f, 0.f, 0.f, 0.f);
+            *reinterpret_cast<float4 *>(wide_v + out_row + i + k) = make_float4(0.f, 0.f, 0.f, 0.f);
+          }
+        } else {
+          if (p.dk) *reinterpret_cast<uint4 *>(static_cast<T *>(p.dk) + out_row + i) = make_uint4(0, 0, 0, 0);
+          if (p.dv) *reinterpret_cast<uint4 *>(static_cast<T *>(p.dv) + out_row + i) = make_uint4(0, 0, 0, 0);
+        }
+      }
+    return;
+  }
+  const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+  uint8_t *const smem = smem_raw + (base - raw);
+  const uint32_t ring = base + 2 * TB;
+  float2 *const stats = reinterpret_cast<float2 *>(smem + 2 * TB + NS * L::kStageBytes);   // [stage][128]
+  auto bar = [&](int i) { return smem_u32(&bar_mem[i]); };
+  auto full = [&](int s) { return bar(kFullKV + s); };
+  auto empty = [&](int s) { return bar(kFullKV + NS + s); };
+  if (threadIdx.x == 0) {
+    not_finite = 0;
+    for (int i = 0; i < bars_kv<DP>(); ++i) mbar_init(bar(i), i == kPFull || i == kDSTFull ? kSoftmaxWarps : 1);
+    fence_mbar_init();
+  }
+  if (warp == kMmaWarp) {
+    tmem_alloc(smem_u32(&tmem_holder), 512);
+    tmem_relinquish();
+  }
+  if (warp == kCopyWarp && lane == 0) {
+    prefetch_tmap(&tq);
+    prefetch_tmap(&tdo);
+    prefetch_tmap(&tk);
+    prefetch_tmap(&tv);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_holder, t_dp = tmem + 128, t_dk = tmem + 256, t_dv = tmem + 384;
+
+  if (warp == kCopyWarp) {
+    bool ok = true;
+    int issued = 0, borders = 0;
+    if (lane == 0) {
+      mbar_expect_tx(bar(kKVFull), 2 * TB);
+      for (int c = 0; c < DP / 64; ++c) {
+        tma_load_3d(base + c * kBox, &tk, bar(kKVFull), 64 * c, kv, r.k0 + key0);
+        tma_load_3d(base + TB + c * kBox, &tv, bar(kKVFull), 64 * c, kv, r.k0 + key0);
+      }
+    }
+    // step n's copies, then what step n - 1 has to have cleared
+    for (int n = 0; n <= steps; ++n) {
+      if (n < steps) {
+        const int s = n % NS, head = head0 + n / tiles, i0 = first + n % tiles * kTile;
+        float2 v[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int i = i0 + lane + 32 * u;
+          v[u] = i < r.nq ? p.stats[(int64_t)head * p.a.q_rows + r.q0 + i] : make_float2(0.f, 0.f);
+        }
+        if (n >= NS) ok = __all_sync(0xffffffffu, mbar_wait(empty(s), (n / NS - 1) & 1, &g_seq_bwd_errors, kWaitNs, kErrProducer));
+        if (!ok) break;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) stats[s * kTile + lane + 32 * u] = v[u];
+        __syncwarp();
+        if (lane == 0) {
+          mbar_expect_tx(full(s), 2 * TB);
+          for (int c = 0; c < DP / 64; ++c) {
+            tma_load_3d(ring + s * L::kStageBytes + c * kBox, &tq, full(s), 64 * c, head, r.q0 + i0);
+            tma_load_3d(ring + s * L::kStageBytes + TB + c * kBox, &tdo, full(s), 64 * c, head, r.q0 + i0);
+          }
+        }
+        issued = n + 1;
+      }
+      if (n >= 1 && is_border(n - 1)) {
+        ok = __all_sync(0xffffffffu, mbar_wait(bar(kSeenKV), borders & 1, &g_seq_bwd_errors, kWaitNs, kErrProducer));
+        ok = ok && __all_sync(0xffffffffu, mbar_wait(full((n - 1) % NS), ((n - 1) / NS) & 1, &g_seq_bwd_errors, kWaitNs, kErrProducer));
+        if (!ok) break;
+        tc_fence_after();
+        uint8_t *const stage = smem + 2 * TB + (n - 1) % NS * L::kStageBytes;
+        const bool q_odd = clear_not_finite<T>(stage, TB), do_odd = clear_not_finite<T>(stage + TB, TB);
+        if (q_odd || do_odd) fence_proxy_async_smem();
+        if (do_odd && lane == 0) not_finite = 1;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(kCleanKV));
+        ++borders;
+      }
+    }
+    if (lane == 0) {
+      mbar_wait(bar(kKVFull), 0, &g_seq_bwd_errors, kWaitNs, kErrTeardown);
+      for (int i = max(0, issued - NS); i < issued; ++i)
+        mbar_wait(full(i % NS), (i / NS) & 1, &g_seq_bwd_errors, kWaitNs, kErrTeardown);
+    }
+  } else if (warp == kMmaWarp) {
+    if (lane == 0) {
+      const uint32_t idesc_s = idesc_f16(128, 128, std::is_same<T, __nv_bfloat16>::value, false);
+      const uint64_t d_k = desc_rows(base), d_v = desc_rows(base + TB), d_ring = desc_rows(ring), d_ringc = desc_cols(ring);
+      int n_s = 0, n_dp = 0, n_dv = 0, n_dk = 0, n_seen = 0, borders = 0;
+      bool done = false;
+      auto wait = [&](uint32_t b, uint32_t parity) {
+        if (!mbar_wait(b, parity, &g_seq_bwd_errors, kWaitNs, kErrMma)) return false;
+        tc_fence_after();
+        return true;
+      };
+      auto stage = [&](int i) { return (uint32_t)(i % NS) * L::kStageBytes >> 4; };
+      auto issue_s = [&](int i) {
+        for (int j = 0; j < p.steps; ++j) mma_ss(tmem, d_k + step_rows(j), d_ring + stage(i) + step_rows(j), idesc_s, j > 0);
+        mma_commit(bar(kSTFull));
+        ++n_s;
+      };
+      auto issue_dp = [&](int i) {
+        const uint64_t o = d_ring + stage(i) + (TB >> 4);
+        for (int j = 0; j < p.steps; ++j) mma_ss(t_dp, d_v + step_rows(j), o + step_rows(j), idesc_s, j > 0);
+        mma_commit(bar(kDPTFull));
+        ++n_dp;
+        if (is_border(i)) {   // covers S too
+          mma_commit(bar(kSeenKV));
+          ++n_seen;
+        }
+      };
+      auto sum = [&](uint32_t to, uint32_t from, uint64_t b, bool more) {
+#pragma unroll
+        for (int j = 0; j < kTile / 16; ++j)
+          mma_ts(to, from + j / 4 * 64 + j % 4 * 8, b + step_cols(j), p.idesc_out, more || j > 0);
+      };
+      bool ok = wait(bar(kKVFull), 0) && wait(full(0), 0);
+      if (ok) {
+        issue_s(0);
+        issue_dp(0);
+      }
+      for (int i = 0; ok && i < steps; ++i) {
+        if (is_border(i)) ok = wait(bar(kCleanKV), borders++ & 1);
+        ok = ok && wait(bar(kPFull), i & 1);
+        if (!ok) break;
+        sum(t_dv, tmem, d_ringc + stage(i) + (TB >> 4), i > 0);
+        mma_commit(bar(kDVDone));
+        ++n_dv;
+        if (i + 1 < steps) {
+          ok = wait(full((i + 1) % NS), ((i + 1) / NS) & 1) && wait(bar(kDVDone), i & 1);
+          if (!ok) break;
+          issue_s(i + 1);
+        }
+        ok = wait(bar(kDSTFull), i & 1);
+        if (!ok) break;
+        sum(t_dk, t_dp, d_ringc + stage(i), i > 0);
+        mma_commit(bar(kDKDone));
+        mma_commit(empty(i % NS));
+        ++n_dk;
+        if (i + 1 < steps) {
+          ok = wait(bar(kDKDone), i & 1);
+          if (!ok) break;
+          issue_dp(i + 1);
+        }
+      }
+      if (ok) {
+        mma_commit(bar(kAllDone));
+        done = true;
+      }
+      mma_commit(bar(kDrainKV));
+      auto drained = [&](uint32_t b, int times) {
+        if (times > 0) mbar_wait(b, (times - 1) & 1, &g_seq_bwd_errors, kWaitNs, kErrTeardown);
+      };
+      drained(bar(kDrainKV), 1);
+      drained(bar(kSTFull), n_s);
+      drained(bar(kDPTFull), n_dp);
+      drained(bar(kDVDone), n_dv);
+      drained(bar(kDKDone), n_dk);
+      drained(bar(kSeenKV), n_seen);
+      drained(bar(kAllDone), done);
+      for (int s = 0; s < NS; ++s) drained(empty(s), n_dk / NS + (s < n_dk % NS));
+    }
+  } else {
+    const int half = warp / 4;
+    const uint32_t lanes = (uint32_t)((warp % 4) * 32) << 16, t_s = tmem + 64 * half + lanes, t_d = t_dp + 64 * half + lanes;
+    const float2 sc = make_float2(p.sc, p.sc), scale = make_float2(p.a.scale, p.a.scale);
+    const int from = p.a.causal ? key - shift : 0;   // the first query that sees this key
+    bool ok = true;
+    for (int i = 0; i < steps; ++i) {
+      const int i0 = first + i % tiles * kTile + half * 64, lo = from - i0, hi = r.nq - i0;
+      const bool masked = __any_sync(0xffffffffu, lo > 0 || hi < 64);
+      const float4 *st = reinterpret_cast<const float4 *>(stats + i % NS * kTile + half * 64);   // two queries each
+      ok = wait_warp(full(i % NS), (i / NS) & 1, &g_seq_bwd_errors, kErrSoftmax) &&
+           wait_warp(bar(kSTFull), i & 1, &g_seq_bwd_errors, kErrSoftmax);
+      if (!ok) break;
+      float s[64];
+      load_columns<64>(t_s, s);
+      tmem_wait_ld();
+#pragma unroll
+      for (int k = 0; k < 32; ++k) {
+        const float4 q = st[k];
+        const float2 w = weight(make_float2(s[2 * k], s[2 * k + 1]), sc, make_float2(-q.x, -q.z), k % 4 == 3 && !masked);
+        s[2 * k] = w.x, s[2 * k + 1] = w.y;
+      }
+      if (masked) {
+#pragma unroll
+        for (int k = 0; k < 64; ++k) s[k] = k >= lo && k < hi ? s[k] : 0.f;
+      }
+#pragma unroll
+      for (int k = 0; k < 32; k += 16) {
+        uint32_t pk[16];
+#pragma unroll
+        for (int u = 0; u < 16; ++u) pk[u] = pack<T>(s[2 * (k + u)], s[2 * (k + u) + 1]);
+        tmem_st16(t_s + k, pk);
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(kPFull));
+      ok = wait_warp(bar(kDPTFull), i & 1, &g_seq_bwd_errors, kErrSoftmax);
+      if (!ok) break;
+      float d[64];
+      load_columns<64>(t_d, d);
+      tmem_wait_ld();
+#pragma unroll
+      for (int k = 0; k < 32; ++k) {
+        const float4 q = st[k];
+        const float2 v = mul2(make_float2(s[2 * k], s[2 * k + 1]), fma2(make_float2(d[2 * k], d[2 * k + 1]), scale, make_float2(-q.y, -q.w)));
+        s[2 * k] = v.x, s[2 * k + 1] = v.y;
+      }
+      if (masked) {
+#pragma unroll
+        for (int k = 0; k < 64; ++k) s[k] = k >= lo && k < hi ? s[k] : 0.f;
+      }
+#pragma unroll
+      for (int k = 0; k < 32; k += 16) {
+        uint32_t pk[16];
+#pragma unroll
+        for (int u = 0; u < 16; ++u) pk[u] = pack<T>(s[2 * (k + u)], s[2 * (k + u) + 1]);
+        tmem_st16(t_d + k, pk);
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(kDSTFull));
+    }
+    if (ok) ok = wait_warp(bar(kAllDone), 0, &g_seq_bwd_errors, kErrSoftmax);
+    if (ok) {
+      // a half of the warps writes dK, the other dV
+      const int dim = there ? p.a.dim : 0;
+      T *const narrow = half ? static_cast<T *>(p.dv) : static_cast<T *>(p.dk);
+      float *const wide = half ? wide_v : wide_k;
+#pragma unroll
+      for (int i = 0; i < DP; i += 32)
+        store_columns<T>((half ? t_dv : t_dk) + lanes, i, dim, narrow ? narrow + out_row : nullptr, wide ? wide + out_row : nullptr);
+      if (half && there && *reinterpret_cast<volatile int *>(&not_finite) && (wide || narrow)) {
+        // dO's infinities and NaN that this key's queries have in border tiles
+        for (int n = 0; n < steps; ++n) {
+          if (!is_border(n)) continue;
+          const int i0 = first + n % tiles * kTile;
+          for (int i = max(i0, from); i < min(i0 + kTile, r.nq); ++i) {
+            const T *o = static_cast<const T *>(p.dout) + ((int64_t)(r.q0 + i) * p.a.heads + head0 + n / tiles) * p.a.dim;
+            for (int c = 0; c < p.a.dim; ++c) {
+              const float v = to_f32<T>(o[c]);
+              if (isfinite(v)) continue;
+              if (wide) wide[out_row + c] += v;
+              else narrow[out_row + c] = from_f32<T>(to_f32<T>(narrow[out_row + c]) + v);
+            }
+          }
+        }
+      }
+    }
+    tmem_wait_st();
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// lse * log2(e) and scale * delta of every row: a row is `lanes` lanes of 16 bytes.
+template <typename T>
+__global__ void __launch_bounds__(256) stats_kernel(const T *out, const T *dout, const float *lse, float2 *stats, int64_t rows,
+                                                    int heads, int64_t tokens, int dim, int lanes, float scale) {
+  const int lane = threadIdx.x & 31, per_warp = 32 / lanes, col = lane % lanes * 8;
+  const int64_t stride = (int64_t)gridDim.x * 8 * per_warp;
+  // whole warps take part in the sums: rows past the last are zeros
+  for (int64_t row0 = ((int64_t)blockIdx.x * 8 + threadIdx.x / 32) * per_warp; row0 < rows; row0 += stride) {
+    const int64_t row = row0 + lane / lanes;
+    float sum = 0.f;
+    if (row < rows && col < dim) {
+      const uint4 a = __ldcs(reinterpret_cast<const uint4 *>(out + row * dim + col)), b = __ldcs(reinterpret_cast<const uint4 *>(dout + row * dim + col));
+      const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 u = unpack2<T>(x[i]), v = unpack2<T>(y[i]);
+        sum = fmaf(u.x, v.x, fmaf(u.y, v.y, sum));
+      }
+    }
+    for (int o = lanes / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (row < rows && lane % lanes == 0) {
+      const int64_t t = row / heads;
+      const int64_t to = (row - t * heads) * tokens + t;
+      stats[to] = make_float2(lse[to] * 1.4426950408889634f, sum * scale);
+    }
+  }
+}
+
+// dk and dv from the sums of the parts, added in order.
+template <typename T>
+__global__ void __launch_bounds__(256) join_parts_kernel(const float *part, int parts, int64_t size, T *dk, T *dv) {
+  T *const out = blockIdx.y ? dv : dk;
+  if (!out) return;
+  for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < size; i += (int64_t)gridDim.x * 1024) {
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int q = 0; q < parts; ++q) {
+      const float4 v = *reinterpret_cast<const float4 *>(part + ((int64_t)blockIdx.y * parts + q) * size + i);
+      sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+    }
+    *reinterpret_cast<uint2 *>(out + i) = make_uint2(pack<T>(sum.x, sum.y), pack<T>(sum.z, sum.w));
+  }
+}
+
+// CTAs that share a group's heads: enough that the key tiles fill the device's SMs twice over, as far as heads go.
+int parts_of(const p3d_sequence &a, int sms) {
+  const int64_t tiles = ((a.k_rows + kTile - 1) / kTile) * a.kv_heads;
+  return (int)std::max<int64_t>(1, std::min<int64_t>(a.heads / a.kv_heads, 2 * sms / std::max<int64_t>(tiles, 1)));
+}
+
+template <typename T, int DP>
+int launch_t(const Params &p, const void *out, const float *lse, float2 *stats, cudaStream_t s) {
+  const p3d_sequence &a = p.a;
+  CUtensorMap tq, tdo, tk, tv;
+  if (a.q_rows && a.k_rows) {
+    const int64_t rows = a.q_rows * a.heads;
+    int lanes = 1;
+    while (lanes * 8 < a.dim) lanes *= 2;
+    const int64_t blocks = std::min<int64_t>((rows * lanes + 255) / 256, 148 * 16);
+    stats_kernel<T><<<(unsigned)blocks, 256, 0, s>>>((const T *)out, (const T *)p.dout, lse, stats, rows, a.heads, a.q_rows, a.dim, lanes,
+                                                        a.scale);
+    P3D_LAUNCH_CHECK();
+    const int64_t dense[2] = {(int64_t)a.heads * a.dim, a.dim};
+    if (int st = encode_heads(&tq, a.dtype, a.q, a.dim, a.heads, a.q_rows, a.q_stride)) return st;
+    if (int st = encode_heads(&tdo, a.dtype, p.dout, a.dim, a.heads, a.q_rows, dense)) return st;
+    if (int st = encode_heads(&tk, a.dtype, a.k, a.dim, a.kv_heads, a.k_rows, a.k_stride)) return st;
+    if (int st = encode_heads(&tv, a.dtype, a.v, a.dim, a.kv_heads, a.k_rows, a.v_stride)) return st;
+  }
+  if (p.dq && a.q_rows) {
+    if (a.k_rows == 0) {
+      P3D_CUDA_TRY(cudaMemsetAsync(p.dq, 0, (size_t)a.q_rows * a.heads * a.dim * 2, s));
+    } else {
+      const int64_t grid = slots_of(a.q_rows, a.sequences, kTile) * a.heads;
+      if (grid > 0x7fffffff) return fail(P3D_ERR_UNSUPPORTED, "p3d_sequence_bwd: too many tiles");
+      static size_t seen[kMaxDevices] = {};
+      if (int st = smem_optin(sequence_dq_kernel<T, DP>, LayoutQ<DP>::kBytes, seen)) return st;
+      sequence_dq_kernel<T, DP><<<(unsigned)grid, kThreads, LayoutQ<DP>::kBytes, s>>>(tq, tdo, tk, tv, p);
+      P3D_LAUNCH_CHECK();
+    }
+  }
+  if ((p.dk || p.dv) && a.k_rows) {
+    if (a.q_rows == 0) {
+      const size_t bytes = (size_t)a.k_rows * a.kv_heads * a.dim * 2;
+      if (p.dk) P3D_CUDA_TRY(cudaMemsetAsync(p.dk, 0, bytes, s));
+      if (p.dv) P3D_CUDA_TRY(cudaMemsetAsync(p.dv, 0, bytes, s));
+      return P3D_OK;
+    }
+    const int64_t grid = slots_of(a.k_rows, a.sequences, kTile) * a.kv_heads * p.parts;
+    if (grid > 0x7fffffff) return fail(P3D_ERR_UNSUPPORTED, "p3d_sequence_bwd: too many tiles");
+    static size_t seen[kMaxDevices] = {};
+    if (int st = smem_optin(sequence_dkv_kernel<T, DP>, LayoutKV<DP>::kBytes, seen)) return st;
+    sequence_dkv_kernel<T, DP><<<(unsigned)grid, kThreads, LayoutKV<DP>::kBytes, s>>>(tq, tdo, tk, tv, p);
+    P3D_LAUNCH_CHECK();
+    if (p.parts > 1) {
+      const int64_t size = a.k_rows * a.kv_heads * a.dim;
+      join_parts_kernel<T><<<dim3((unsigned)std::min<int64_t>((size + 1023) / 1024, 148 * 8), 2), 256, 0, s>>>(
+          p.part, p.parts, size, (T *)p.dk, (T *)p.dv);
+      P3D_LAUNCH_CHECK();
+    }
+  }
+  return P3D_OK;
+}
+
+size_t stats_bytes(const p3d_sequence &a) { return ((size_t)a.q_rows * a.heads * sizeof(float2) + 255) / 256 * 256; }
+
+}  // namespace
+
+int bwd_workspace(const p3d_sequence &a, size_t *bytes) {
+  DeviceInfo info;
+  if (int st = device_info(&info)) return st;
+  const int parts = parts_of(a, info.sm_count);
+  *bytes = stats_bytes(a) + (parts > 1 ? 2 * sizeof(float) * (size_t)parts * a.k_rows * a.kv_heads * a.dim : 0);
+  return P3D_OK;
+}
+
+int launch_bwd(const p3d_sequence &a, const void *out, const float *lse, const void *dout, void *dq, void *dk, void *dv,
+               void *workspace, size_t workspace_bytes, cudaStream_t s) {
+  size_t need = 0;
+  if (int st = bwd_workspace(a, &need)) return st;
+  if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16))
+    return fail(P3D_ERR_WORKSPACE, "p3d_sequence_bwd: aligned workspace of %zu bytes needed", need);
+  DeviceInfo info;
+  if (int st = device_info(&info)) return st;
+  Params p = {};
+  p.a = a;
+  p.dout = dout;
+  p.dq = dq, p.dk = dk, p.dv = dv;
+  float2 *const stats = static_cast<float2 *>(workspace);
+  p.stats = stats;
+  p.parts = parts_of(a, info.sm_count);
+  p.part = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + stats_bytes(a));
+  p.steps = (a.dim + 15) / 16;
+  p.idesc_out = idesc_f16(128, p.steps * 16, a.dtype == P3D_BF16, true);
+  p.sc = a.scale * 1.4426950408889634f;
+  if (a.dtype == P3D_BF16)
+    return padded(a.dim) == 64 ? launch_t<__nv_bfloat16, 64>(p, out, lse, stats, s) : launch_t<__nv_bfloat16, 128>(p, out, lse, stats, s);
+  return padded(a.dim) == 64 ? launch_t<__half, 64>(p, out, lse, stats, s) : launch_t<__half, 128>(p, out, lse, stats, s);
+}
+
+int take_errors_bwd(unsigned *flags) {
+  unsigned v = 0, zero = 0;
+  P3D_CUDA_TRY(cudaMemcpyFromSymbol(&v, g_seq_bwd_errors, sizeof(v)));
+  P3D_CUDA_TRY(cudaMemcpyToSymbol(g_seq_bwd_errors, &zero, sizeof(zero)));
+  *flags |= v;
+  return P3D_OK;
+}
+
+}  // namespace seq
+}  // namespace p3d

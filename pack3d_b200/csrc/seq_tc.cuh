@@ -121,6 +121,10 @@ inline int encode_heads(CUtensorMap *map, int dtype, const void *p, int dim, int
 
 int take_errors_fwd(unsigned *flags);   // seq_fwd.cu
 int launch_fwd(const p3d_sequence &a, void *out, float *lse, cudaStream_t s);
+int take_errors_bwd(unsigned *flags);   // seq_bwd.cu
+int bwd_workspace(const p3d_sequence &a, size_t *bytes);
+int launch_bwd(const p3d_sequence &a, const void *out, const float *lse, const void *dout, void *dq, void *dk, void *dv,
+               void *workspace, size_t workspace_bytes, cudaStream_t s);
 
 }  // namespace seq
 }  // namespace p3d

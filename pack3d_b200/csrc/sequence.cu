@@ -1,7 +1,5 @@
-// Attention over packed sequences, a warp to a row: each lane holds four columns and the dot products are warp sums.
+// p3d_sequence: the checks of arguments and the entry points; the kernels are in seq_fwd.cu and seq_bwd.cu.
 #include <math.h>
-
-#include <algorithm>
 
 #include "kernels.cuh"
 #include "seq_tc.cuh"
@@ -9,77 +7,6 @@
 namespace p3d {
 namespace {
 
-constexpr int kWarps = 8;
-
-template <typename T> __device__ __forceinline__ void load4(const T *row, int lane, int dim, float (&v)[4]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = lane * 4 + i < dim ? to_f32<T>(row[lane * 4 + i]) : 0.f;
-}
-template <typename T> __device__ __forceinline__ void store4(T *row, int lane, int dim, const float (&v)[4]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (lane * 4 + i < dim) row[lane * 4 + i] = from_f32<T>(v[i]);
-}
-__device__ __forceinline__ float dot4(const float (&a)[4], const float (&b)[4]) {
-  return warp_sum(a[0] * b[0] + a[1] * b[1] + a[2] * b[2] + a[3] * b[3]);
-}
-
-template <typename T>
-__global__ void dq_kernel(const __grid_constant__ p3d_sequence a, const T *out, const float *lse, const T *dout, T *dq) {
-  const int64_t item = (int64_t)blockIdx.x * kWarps + threadIdx.x / 32;
-  const int lane = threadIdx.x & 31, h = (int)(item % a.heads), t = (int)(item / a.heads);
-  if (t >= a.q_rows) return;
-  const int b = cache::sequence_of(a.q_offsets, a.sequences, (int)a.q_rows, t), g = h / (a.heads / a.kv_heads);
-  const seq::Range r = seq::range_of(a, b);
-  const int n = t - r.q0 < r.nq ? seq::seen_by(r, t - r.q0, a.causal) : 0;
-  const int64_t row = ((int64_t)t * a.heads + h) * a.dim;
-  float q[4], o[4], d[4], k[4], v[4], sum[4] = {0.f, 0.f, 0.f, 0.f};
-  load4(static_cast<const T *>(a.q) + t * a.q_stride[0] + h * a.q_stride[1], lane, a.dim, q);
-  load4(out + row, lane, a.dim, o);
-  load4(dout + row, lane, a.dim, d);
-  const float delta = dot4(o, d), l = lse[h * a.q_rows + t];
-  for (int j = 0; j < n; ++j) {
-    load4(static_cast<const T *>(a.k) + (int64_t)(r.k0 + j) * a.k_stride[0] + g * a.k_stride[1], lane, a.dim, k);
-    load4(static_cast<const T *>(a.v) + (int64_t)(r.k0 + j) * a.v_stride[0] + g * a.v_stride[1], lane, a.dim, v);
-    const float ds = expf(dot4(q, k) * a.scale - l) * (dot4(d, v) - delta) * a.scale;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) sum[i] += ds * k[i];
-  }
-  store4(dq + row, lane, a.dim, sum);
-}
-
-template <typename T>
-__global__ void dkv_kernel(const __grid_constant__ p3d_sequence a, const T *out, const float *lse, const T *dout, T *dk, T *dv) {
-  const int64_t item = (int64_t)blockIdx.x * kWarps + threadIdx.x / 32;
-  const int lane = threadIdx.x & 31, g = (int)(item % a.kv_heads), t = (int)(item / a.kv_heads), group = a.heads / a.kv_heads;
-  if (t >= a.k_rows) return;
-  const int b = cache::sequence_of(a.k_offsets, a.sequences, (int)a.k_rows, t);
-  const seq::Range r = seq::range_of(a, b);
-  const int j = t - r.k0;
-  const int i0 = j >= r.nk ? r.nq : a.causal ? max(0, j + r.nq - r.nk) : 0;   // the first row that sees key j
-  float q[4], o[4], d[4], k[4], v[4], sk[4] = {0.f, 0.f, 0.f, 0.f}, sv[4] = {0.f, 0.f, 0.f, 0.f};
-  load4(static_cast<const T *>(a.k) + t * a.k_stride[0] + g * a.k_stride[1], lane, a.dim, k);
-  load4(static_cast<const T *>(a.v) + t * a.v_stride[0] + g * a.v_stride[1], lane, a.dim, v);
-  for (int h = g * group; h < (g + 1) * group; ++h)
-    for (int i = i0; i < r.nq; ++i) {
-      const int64_t row = ((int64_t)(r.q0 + i) * a.heads + h) * a.dim;
-      load4(static_cast<const T *>(a.q) + (int64_t)(r.q0 + i) * a.q_stride[0] + h * a.q_stride[1], lane, a.dim, q);
-      load4(out + row, lane, a.dim, o);
-      load4(dout + row, lane, a.dim, d);
-      const float p = expf(dot4(q, k) * a.scale - lse[h * a.q_rows + r.q0 + i]);
-      const float ds = p * (dot4(d, v) - dot4(o, d)) * a.scale;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        sk[c] += ds * q[c];
-        sv[c] += p * d[c];
-      }
-    }
-  const int64_t row = ((int64_t)t * a.kv_heads + g) * a.dim;
-  if (dk) store4(dk + row, lane, a.dim, sk);
-  if (dv) store4(dv + row, lane, a.dim, sv);
-}
-
-int blocks_of(int64_t warps) { return (int)((warps + kWarps - 1) / kWarps); }
 bool aligned(const void *q) { return (uintptr_t)q % 16 == 0; }
 
 }  // namespace
@@ -115,7 +42,10 @@ int check(const p3d_sequence *a, const char *what) {
 
 }  // namespace seq
 
-int take_sequence_errors(unsigned *flags) { return seq::take_errors_fwd(flags); }
+int take_sequence_errors(unsigned *flags) {
+  if (int st = seq::take_errors_fwd(flags)) return st;
+  return seq::take_errors_bwd(flags);
+}
 
 }  // namespace p3d
 
@@ -131,26 +61,19 @@ int p3d_sequence_fwd(const p3d_sequence *a, void *out, float *lse, void *stream)
 }
 
 size_t p3d_sequence_bwd_workspace(const p3d_sequence *a) {
-  return 0;
+  size_t bytes = 0;
+  if (seq::check(a, "p3d_sequence_bwd") != P3D_OK || seq::bwd_workspace(*a, &bytes) != P3D_OK) return 0;
+  return bytes;
 }
 
 int p3d_sequence_bwd(const p3d_sequence *a, const void *out, const float *lse, const void *dout, void *dq, void *dk, void *dv,
                      void *workspace, size_t workspace_bytes, void *stream) {
   if (int st = seq::check(a, "p3d_sequence_bwd")) return st;
-  const cudaStream_t s = (cudaStream_t)stream;
   P3D_CHECK_ARG(!a->q_rows || (out && lse && dout && aligned(out) && aligned(dout)),
                 "p3d_sequence_bwd: out, lse and dout must be given and 16-byte aligned");
-  auto go = [&](auto type) {
-    using T = decltype(type);
-    if (dq && a->q_rows)
-      dq_kernel<T><<<blocks_of(a->q_rows * a->heads), kWarps * 32, 0, s>>>(*a, (const T *)out, lse, (const T *)dout, (T *)dq);
-    if ((dk || dv) && a->k_rows)
-      dkv_kernel<T><<<blocks_of(a->k_rows * a->kv_heads), kWarps * 32, 0, s>>>(*a, (const T *)out, lse, (const T *)dout,
-                                                                               (T *)dk, (T *)dv);
-  };
-  a->dtype == P3D_F16 ? go(__half()) : go(__nv_bfloat16());
-  P3D_LAUNCH_CHECK();
-  return P3D_OK;
+  P3D_CHECK_ARG(aligned(dq) && aligned(dk) && aligned(dv), "p3d_sequence_bwd: gradients must be 16-byte aligned");
+  if (a->sequences == 0) return P3D_OK;
+  return seq::launch_bwd(*a, out, lse, dout, dq, dk, dv, workspace, workspace_bytes, (cudaStream_t)stream);
 }
 
 }  // extern "C"
