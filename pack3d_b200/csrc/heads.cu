@@ -10,12 +10,14 @@
 //
 // Bound by HBM: forward reads x and writes y, backward reads x and dy and writes dx; nothing is saved between them but x, as
 // N(x) costs less to make again than to read. Layout: a row (token, head) of D columns is S = D / 8 lanes (up to a power of two), 16
-// bytes each; 32 / S rows a pass, U passes of loads in flight. A lane keeps the same four pairs for all rows, so a token's
-// angles are computed once for its rows, and each of the 32 / S lane groups computes a share of the four and hands it round by
+// bytes each; 32 / S rows a pass, U passes an item, an item a warp. A warp has the same heads of one token after another, so that a
+// lane's parameters and places are fixed, and the rows of two items ahead are in flight while one is worked on. A lane holds the
+// same four pairs of every row, and each of the 32 / S lane groups computes a share of their angles and hands it round by
 // shuffles.
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 #include "sm100.cuh"
@@ -23,7 +25,7 @@
 namespace p3d {
 namespace {
 
-constexpr int kWarps = 8;
+constexpr int kWarps = 4, kAhead = 2;
 constexpr int kMaxPairs = 128;
 
 struct RotateParams {
@@ -33,39 +35,46 @@ struct RotateParams {
   float *partial;  // [4][blocks][dim]: dweight 0, 1, dbias 0, 1
   const void *pos;
   int64_t ts0, ts1, hs0, hs1, ps, as;
-  uint32_t items, chunks, tokens, position_rows;
+  uint32_t tokens, position_rows, chunks;   // chunks: items of a token; the grid's warps are a multiple of it
   int h0, h1, kind0, kind1, pd0, pd1, dim, pos4;
   float eps0, eps1;
   int end0, end1, end2;   // pairs up to the end of each axis
   uint64_t turns[kMaxPairs];
 };
 
-// Eight columns of a row in fp32; those past `n` are zero.
+// Eight columns of a row as they lie in memory; those past `n` are zero.
+template <typename T> struct Raw {
+  uint32_t w[2 * sizeof(T)];
+};
 template <typename T, bool kVec>
-__device__ __forceinline__ void load8(const T *p, int n, float2 (&v)[4]) {
+__device__ __forceinline__ void load8(Raw<T> &r, const T *p, int n) {
+  constexpr int kWords = 2 * sizeof(T);
   if constexpr (kVec) {
-    if (n <= 0) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = make_float2(0.f, 0.f);
-    } else if constexpr (sizeof(T) == 2) {
-      const uint4 raw = __ldcs(reinterpret_cast<const uint4 *>(p));
-      v[0] = unpack2<T>(raw.x), v[1] = unpack2<T>(raw.y), v[2] = unpack2<T>(raw.z), v[3] = unpack2<T>(raw.w);
-    } else {
-      const float4 a = __ldcs(reinterpret_cast<const float4 *>(p)), b = __ldcs(reinterpret_cast<const float4 *>(p) + 1);
-      v[0] = make_float2(a.x, a.y), v[1] = make_float2(a.z, a.w);
-      v[2] = make_float2(b.x, b.y), v[3] = make_float2(b.z, b.w);
+    for (int i = 0; i < kWords; i += 4) {
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (n > 0) v = __ldcs(reinterpret_cast<const uint4 *>(p) + i / 4);
+      r.w[i] = v.x, r.w[i + 1] = v.y, r.w[i + 2] = v.z, r.w[i + 3] = v.w;
     }
   } else {
+    alignas(16) T v[8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      v[i] = make_float2(2 * i < n ? to_f32<T>(p[2 * i]) : 0.f, 2 * i + 1 < n ? to_f32<T>(p[2 * i + 1]) : 0.f);
+    for (int i = 0; i < 8; ++i) v[i] = i < n ? p[i] : from_f32<T>(0.f);
+    memcpy(r.w, v, sizeof(r.w));
+  }
+}
+template <typename T>
+__device__ __forceinline__ void unpack8(const Raw<T> &r, float2 (&v)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 2) v[i] = unpack2<T>(r.w[i]);
+    else v[i] = make_float2(__uint_as_float(r.w[2 * i]), __uint_as_float(r.w[2 * i + 1]));
   }
 }
 
 template <typename T> __device__ __forceinline__ uint32_t pack2(float2 v);
 template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float2 v) { return sm100::pack_bf16(v.x, v.y); }
 template <> __device__ __forceinline__ uint32_t pack2<__half>(float2 v) { return sm100::pack_f16(v.x, v.y); }
-template <> __device__ __forceinline__ uint32_t pack2<float>(float2) { return 0; }
 
 template <typename T, bool kVec>
 __device__ __forceinline__ void store8(T *p, int n, const float2 (&v)[4]) {
@@ -107,214 +116,278 @@ template <int S>
 struct Phases {
   static constexpr int R = 32 / S, kGroups = R < 4 ? R : 4, kMine = 4 / kGroups;
   uint64_t turn[kMine];
-  int axis[kMine];
-  float2 cs[4], sn[4];   // (cos, cos) and (-sin, sin) of each pair
+  int64_t axis[kMine];   // where the axis lies in a token's positions
   __device__ __forceinline__ void init(const RotateParams &p, int lane) {
     const int chunk = lane % S, group = lane / S % kGroups;
 #pragma unroll
     for (int m = 0; m < kMine; ++m) {
       const int pair = chunk * 4 + m * kGroups + group;
       turn[m] = pair < p.end2 ? p.turns[pair] : 0;
-      axis[m] = pair < p.end0 || pair >= p.end2 ? 0 : pair < p.end1 ? 1 : 2;
+      axis[m] = p.as * (pair < p.end0 || pair >= p.end2 ? 0 : pair < p.end1 ? 1 : 2);
     }
   }
-  template <typename T>
-  __device__ __forceinline__ void at(const RotateParams &p, uint32_t token, int lane) {
+  struct Position {
+    int64_t at[kMine];
+  };
+  __device__ __forceinline__ Position load(const RotateParams &p, uint32_t token) const {
+    Position r;
     const uint32_t row = p.position_rows == p.tokens ? token : token % p.position_rows;
-    float c[kMine], s[kMine];
 #pragma unroll
     for (int m = 0; m < kMine; ++m) {
-      const int64_t where = (int64_t)row * p.ps + axis[m] * p.as;
-      const int64_t pos = p.pos4 ? static_cast<const int32_t *>(p.pos)[where] : static_cast<const int64_t *>(p.pos)[where];
-      const int32_t part = (int32_t)(((uint64_t)pos * turn[m]) >> 32);   // 2^-32 turns, -0.5 .. 0.5
-      const float half_turns = (float)part * 4.656612873077393e-10f;     // 2^-31
-      if constexpr (sizeof(T) == 2)
-        __sincosf(half_turns * 3.14159265f, &s[m], &c[m]);
-      else
-        sincospif(half_turns, &s[m], &c[m]);
+      const int64_t where = (int64_t)row * p.ps + axis[m];
+      r.at[m] = token >= p.tokens ? 0 : p.pos4 ? static_cast<const int32_t *>(p.pos)[where] : static_cast<const int64_t *>(p.pos)[where];
     }
+    return r;
+  }
+  struct Angles {
+    float c[4], s[4];
+    // R(pos), or R(-pos) for kBack, of the four pairs
+    template <bool kBack>
+    __device__ __forceinline__ void turn4(float2 (&v)[4]) const {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float a = v[i].x, b = v[i].y, t = kBack ? -s[i] : s[i];
+        v[i] = make_float2(fmaf(-b, t, a * c[i]), fmaf(a, t, b * c[i]));
+      }
+    }
+  };
+  template <typename T>
+  __device__ __forceinline__ Angles angles(const Position &at, int lane) const {
+    float mc[kMine], ms[kMine];
+#pragma unroll
+    for (int m = 0; m < kMine; ++m) {
+      const int32_t part = (int32_t)(((uint64_t)at.at[m] * turn[m]) >> 32);   // 2^-32 turns, -0.5 .. 0.5
+      if constexpr (sizeof(T) == 2) __sincosf((float)part * 1.4629180792671596e-9f, &ms[m], &mc[m]);   // 2 pi 2^-32
+      else sincospif((float)part * 4.656612873077393e-10f, &ms[m], &mc[m]);                            // 2^-31
+    }
+    Angles r;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int from = (i % kGroups) * S + lane % S;
-      const float ci = __shfl_sync(0xffffffffu, c[i / kGroups], from);
-      const float si = __shfl_sync(0xffffffffu, s[i / kGroups], from);
-      cs[i] = make_float2(ci, ci);
-      sn[i] = make_float2(-si, si);
+      r.c[i] = __shfl_sync(0xffffffffu, mc[i / kGroups], from);
+      r.s[i] = __shfl_sync(0xffffffffu, ms[i / kGroups], from);
     }
-  }
-  // R(pos), or R(-pos) for kBack, of the four pairs
-  template <bool kBack>
-  __device__ __forceinline__ void turn4(float2 (&v)[4]) const {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 swapped = kBack ? make_float2(-v[i].y, -v[i].x) : make_float2(v[i].y, v[i].x);
-      v[i] = sm100::fma2(swapped, sn[i], sm100::mul2(v[i], cs[i]));
-    }
+    return r;
   }
 };
 
-// N(x) in place; returns 1 / deviation (1 without a norm).
+// N(x) in place; returns 1 / deviation (1 without a norm).  Kinds may differ within a warp: all lanes take part in the sums.
 template <int S>
-__device__ __forceinline__ float normalise(float2 (&v)[4], int n, int kind, float eps, float inv_dim) {
-  if (kind == P3D_NORM_NONE) return 1.f;
-  if (kind == P3D_NORM_LAYER) {
+__device__ __forceinline__ float normalise(float2 (&v)[4], int n, int kind, float eps, float inv_dim, bool any_layer) {
+  if (any_layer) {
     const float2 t = sm100::add2(sm100::add2(v[0], v[1]), sm100::add2(v[2], v[3]));
     const float mean = row_sum<S>(t.x + t.y) * inv_dim;
+    if (kind == P3D_NORM_LAYER) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[i].x = 2 * i < n ? v[i].x - mean : 0.f;
-      v[i].y = 2 * i + 1 < n ? v[i].y - mean : 0.f;
+      for (int i = 0; i < 4; ++i) {
+        v[i].x = 2 * i < n ? v[i].x - mean : 0.f;
+        v[i].y = 2 * i + 1 < n ? v[i].y - mean : 0.f;
+      }
     }
   }
   float2 q = sm100::mul2(v[0], v[0]);
 #pragma unroll
   for (int i = 1; i < 4; ++i) q = sm100::fma2(v[i], v[i], q);
-  const float r = rsqrtf(row_sum<S>(q.x + q.y) * inv_dim + eps);
+  const float sum = row_sum<S>(q.x + q.y);
+  const float r = kind == P3D_NORM_NONE ? 1.f : rsqrtf(fmaf(sum, inv_dim, eps));
 #pragma unroll
   for (int i = 0; i < 4; ++i) v[i] = sm100::mul2(v[i], make_float2(r, r));
   return r;
 }
 
-// A row: its input, its place in the contiguous output, its norm.
+// A lane's row of every token that its warp visits: addresses at the warp's first token and steps to the next one.
 struct Row {
-  int64_t in, out;
-  bool second;
+  bool on, second;
+  int64_t in, in_step, out, out_step;   // elements
 };
-__device__ __forceinline__ Row row_at(const RotateParams &p, uint32_t token, int h) {
+__device__ __forceinline__ Row row_of(const RotateParams &p, int h, uint32_t token, uint32_t tokens_step, int c) {
   Row r;
   r.second = h >= p.h0;
-  const int head = r.second ? h - p.h0 : h;
-  r.in = (int64_t)token * (r.second ? p.ts1 : p.ts0) + head * (r.second ? p.hs1 : p.hs0);
-  r.out = ((int64_t)token * (r.second ? p.h1 : p.h0) + head) * p.dim;
+  r.on = h < p.h0 + p.h1 && c < p.dim;
+  const int head = r.second ? h - p.h0 : h, heads = r.second ? p.h1 : p.h0;
+  const int64_t ts = r.second ? p.ts1 : p.ts0;
+  r.in = (int64_t)token * ts + head * (r.second ? p.hs1 : p.hs0) + c;
+  r.in_step = (int64_t)tokens_step * ts;
+  r.out = ((int64_t)token * heads + head) * p.dim + c;
+  r.out_step = (int64_t)tokens_step * heads * p.dim;
   return r;
 }
 
-template <typename T, int S, int U, bool kVec>
-__global__ void __launch_bounds__(kWarps * 32) norm_rotate_kernel(const __grid_constant__ RotateParams p) {
+template <typename T, int S, int U, bool kVec, bool kBias>
+__global__ void __launch_bounds__(kWarps * 32, sizeof(T) == 2 && kVec && !kBias ? 5 : 3)
+    norm_rotate_kernel(const __grid_constant__ RotateParams p) {
   constexpr int R = 32 / S;
-  const int lane = threadIdx.x & 31, c = lane % S * 8, n = p.dim - c, rows = p.h0 + p.h1;
+  const int lane = threadIdx.x & 31, c = lane % S * 8, n = p.dim - c;
+  const uint32_t warp = blockIdx.x * kWarps + threadIdx.x / 32, step = gridDim.x * kWarps / p.chunks;
+  const uint32_t token0 = warp / p.chunks;
   const float inv_dim = 1.f / p.dim;
+  const bool any_layer = p.kind0 == P3D_NORM_LAYER || p.kind1 == P3D_NORM_LAYER;
   Phases<S> ph;
   ph.init(p, lane);
-  float2 w[2][4], b[2][4];
-  load_param(p.w0, p.pd0, c, n, 1.f, w[0]);
-  load_param(p.w1, p.pd1, c, n, 1.f, w[1]);
-  load_param(p.b0, p.pd0, c, n, 0.f, b[0]);
-  load_param(p.b1, p.pd1, c, n, 0.f, b[1]);
-  const uint32_t stride = gridDim.x * kWarps;
-  for (uint32_t item = blockIdx.x * kWarps + threadIdx.x / 32; item < p.items; item += stride) {
-    const uint32_t token = p.chunks == 1 ? item : item / p.chunks;
-    const int first = (int)(item - token * p.chunks) * U * R + lane / S;
-    float2 v[U][4];
+  Row row[U];
+  const T *in[U];
+  T *out[U];
+  float2 w[U][4], b[U][4];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    row[u] = row_of(p, ((int)(warp - token0 * p.chunks) * U + u) * R + lane / S, token0, step, c);
+    in[u] = static_cast<const T *>(row[u].second ? p.x1 : p.x0) + row[u].in;
+    out[u] = static_cast<T *>(row[u].second ? p.y1 : p.y0) + row[u].out;
+    load_param(row[u].second ? p.w1 : p.w0, row[u].second ? p.pd1 : p.pd0, c, n, 1.f, w[u]);
+    if constexpr (kBias) load_param(row[u].second ? p.b1 : p.b0, row[u].second ? p.pd1 : p.pd0, c, n, 0.f, b[u]);
+  }
+  Raw<T> ahead[kAhead][U];
+  typename Phases<S>::Position position[kAhead];
+  auto fetch = [&](Raw<T> (&r)[U], typename Phases<S>::Position &at, uint32_t token) {
+    at = ph.load(p, token);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int h = first + u * R;
-      const Row r = row_at(p, token, h);
-      load8<T, kVec>(static_cast<const T *>(r.second ? p.x1 : p.x0) + r.in + c, h < rows ? n : 0, v[u]);
+      load8<T, kVec>(r[u], in[u], row[u].on && token < p.tokens ? n : 0);
+      in[u] += row[u].in_step;
     }
-    ph.template at<T>(p, token, lane);
+  };
+  // tokens are below 2^31 and steps far smaller: no token number wraps
+#pragma unroll
+  for (int k = 0; k < kAhead; ++k) fetch(ahead[k], position[k], token0 + k * step);
+  for (uint32_t token = token0; token < p.tokens; token += step) {
+    Raw<T> now[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) now[u] = ahead[0][u];
+    const typename Phases<S>::Angles turn = ph.template angles<T>(position[0], lane);
+#pragma unroll
+    for (int k = 0; k + 1 < kAhead; ++k) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) ahead[k][u] = ahead[k + 1][u];
+      position[k] = position[k + 1];
+    }
+    fetch(ahead[kAhead - 1], position[kAhead - 1], token + kAhead * step);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int h = first + u * R;
-      const Row r = row_at(p, token, h);
-      normalise<S>(v[u], n, r.second ? p.kind1 : p.kind0, r.second ? p.eps1 : p.eps0, inv_dim);
+      float2 v[4];
+      unpack8(now[u], v);
+      normalise<S>(v, n, row[u].second ? p.kind1 : p.kind0, row[u].second ? p.eps1 : p.eps0, inv_dim, any_layer);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        v[u][i] = r.second ? sm100::fma2(v[u][i], w[1][i], b[1][i]) : sm100::fma2(v[u][i], w[0][i], b[0][i]);
-      ph.template turn4<false>(v[u]);
-      store8<T, kVec>(static_cast<T *>(r.second ? p.y1 : p.y0) + r.out + c, h < rows ? n : 0, v[u]);
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (kBias) v[i] = sm100::fma2(v[i], w[u][i], b[u][i]);
+        else v[i] = sm100::mul2(v[i], w[u][i]);
+      }
+      turn.template turn4<false>(v);
+      store8<T, kVec>(out[u], row[u].on ? n : 0, v);
+      out[u] += row[u].out_step;
     }
   }
 }
 
-template <typename T, int S, int U, bool kVec, bool kParams>
-__global__ void __launch_bounds__(kWarps * 32) norm_rotate_bwd_kernel(const __grid_constant__ RotateParams p) {
+template <typename T, int S, bool kVec, bool kParams>
+__global__ void __launch_bounds__(kWarps * 32, sizeof(T) == 2 && kVec ? 4 : 3)
+    norm_rotate_bwd_kernel(const __grid_constant__ RotateParams p) {
   constexpr int R = 32 / S;
-  const int lane = threadIdx.x & 31, c = lane % S * 8, n = p.dim - c, rows = p.h0 + p.h1;
+  const int lane = threadIdx.x & 31, c = lane % S * 8, n = p.dim - c;
+  const uint32_t warp = blockIdx.x * kWarps + threadIdx.x / 32, step = gridDim.x * kWarps / p.chunks;
+  const uint32_t token0 = warp / p.chunks;
   const float inv_dim = 1.f / p.dim;
+  const bool any_layer = p.kind0 == P3D_NORM_LAYER || p.kind1 == P3D_NORM_LAYER;
   Phases<S> ph;
   ph.init(p, lane);
-  float2 w[2][4], sum[4][4];   // sums: dweight 0, 1, dbias 0, 1
-  load_param(p.w0, p.pd0, c, n, 1.f, w[0]);
-  load_param(p.w1, p.pd1, c, n, 1.f, w[1]);
+  const Row row = row_of(p, (int)(warp - token0 * p.chunks) * R + lane / S, token0, step, c);
+  const T *in = static_cast<const T *>(row.second ? p.x1 : p.x0) + row.in;
+  const T *up = static_cast<const T *>(row.second ? p.dy1 : p.dy0) + row.out;
+  T *out = static_cast<T *>(row.second ? p.y1 : p.y0);
+  const bool write = out && row.on;
+  out += row.out;
+  const int kind = row.second ? p.kind1 : p.kind0;
+  const float eps = row.second ? p.eps1 : p.eps0;
+  float2 w[4], sum_w[4], sum_b[4];
+  load_param(row.second ? p.w1 : p.w0, row.second ? p.pd1 : p.pd0, c, n, 1.f, w);
 #pragma unroll
-  for (int i = 0; i < 16; ++i) sum[i / 4][i % 4] = make_float2(0.f, 0.f);
-  const uint32_t stride = gridDim.x * kWarps;
-  for (uint32_t item = blockIdx.x * kWarps + threadIdx.x / 32; item < p.items; item += stride) {
-    const uint32_t token = p.chunks == 1 ? item : item / p.chunks;
-    const int first = (int)(item - token * p.chunks) * U * R + lane / S;
-    float2 v[U][4], g[U][4];
+  for (int i = 0; i < 4; ++i) sum_w[i] = sum_b[i] = make_float2(0.f, 0.f);
+  // two tokens at a time: one row's sums over its lanes wait on one another, two rows' do not
+  Raw<T> ahead_x[2], ahead_g[2];
+  typename Phases<S>::Position position[2];
+  auto fetch = [&](int k, uint32_t token) {
+    position[k] = ph.load(p, token);
+    const int m = row.on && token < p.tokens ? n : 0;
+    load8<T, kVec>(ahead_x[k], in, m);
+    load8<T, kVec>(ahead_g[k], up, m);
+    in += row.in_step;
+    up += row.out_step;
+  };
+  fetch(0, token0);
+  fetch(1, token0 + step);
+  for (uint32_t token = token0; token < p.tokens; token += 2 * step) {
+    float2 v[2][4], g[2][4];
+    float dev[2], gn[2], mean[2];
+    typename Phases<S>::Angles turn[2];
+    const bool there[2] = {true, token + step < p.tokens};
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int h = first + u * R;
-      const Row r = row_at(p, token, h);
-      load8<T, kVec>(static_cast<const T *>(r.second ? p.x1 : p.x0) + r.in + c, h < rows ? n : 0, v[u]);
-      load8<T, kVec>(static_cast<const T *>(r.second ? p.dy1 : p.dy0) + r.out + c, h < rows ? n : 0, g[u]);
+    for (int k = 0; k < 2; ++k) {
+      unpack8(ahead_x[k], v[k]);
+      unpack8(ahead_g[k], g[k]);
+      turn[k] = ph.template angles<T>(position[k], lane);
     }
-    ph.template at<T>(p, token, lane);
+    fetch(0, token + 2 * step);
+    fetch(1, token + 3 * step);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int h = first + u * R;
-      const Row r = row_at(p, token, h);
-      const int kind = r.second ? p.kind1 : p.kind0;
-      const float dev = normalise<S>(v[u], n, kind, r.second ? p.eps1 : p.eps0, inv_dim);
-      ph.template turn4<true>(g[u]);
-      if constexpr (kParams) {
-        // rows past the last are zeros in g: an eps of 0 would make their norm NaN
-        if (h < rows) {
-          if (r.second) {
+    for (int k = 0; k < 2; ++k) {
+      // zeros stand for a token that is not there: its norm has to be finite
+      dev[k] = normalise<S>(v[k], n, kind, there[k] ? eps : 1.f, inv_dim, any_layer);
+      turn[k].template turn4<true>(g[k]);
+    }
+    if constexpr (kParams) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              sum[1][i] = sm100::fma2(g[u][i], v[u][i], sum[1][i]);
-              sum[3][i] = sm100::add2(g[u][i], sum[3][i]);
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              sum[0][i] = sm100::fma2(g[u][i], v[u][i], sum[0][i]);
-              sum[2][i] = sm100::add2(g[u][i], sum[2][i]);
-            }
-          }
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) g[u][i] = sm100::mul2(g[u][i], r.second ? w[1][i] : w[0][i]);
-      if (kind != P3D_NORM_NONE) {
-        float2 t = sm100::mul2(g[u][0], v[u][0]);
-#pragma unroll
-        for (int i = 1; i < 4; ++i) t = sm100::fma2(g[u][i], v[u][i], t);
-        const float gn = -row_sum<S>(t.x + t.y) * inv_dim;
-        float mean = 0.f;
-        if (kind == P3D_NORM_LAYER) {
-          t = sm100::add2(sm100::add2(g[u][0], g[u][1]), sm100::add2(g[u][2], g[u][3]));
-          mean = -row_sum<S>(t.x + t.y) * inv_dim;
-        }
+      for (int k = 0; k < 2; ++k)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          g[u][i] = sm100::fma2(v[u][i], make_float2(gn, gn), sm100::add2(g[u][i], make_float2(mean, mean)));
-          g[u][i] = sm100::mul2(g[u][i], make_float2(dev, dev));
+          sum_w[i] = sm100::fma2(g[k][i], v[k][i], sum_w[i]);
+          sum_b[i] = sm100::add2(g[k][i], sum_b[i]);
+        }
+    }
+    // the norm of a lane group without a row (zeros, an eps of 0) is NaN and goes nowhere; kinds may differ within a warp, the
+    // sums are over a row's lanes, so all lanes take part in them
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) g[k][i] = sm100::mul2(g[k][i], w[i]);
+      float2 t = sm100::mul2(g[k][0], v[k][0]);
+#pragma unroll
+      for (int i = 1; i < 4; ++i) t = sm100::fma2(g[k][i], v[k][i], t);
+      gn[k] = -row_sum<S>(t.x + t.y) * inv_dim;
+      mean[k] = 0.f;
+      if (any_layer) {
+        t = sm100::add2(sm100::add2(g[k][0], g[k][1]), sm100::add2(g[k][2], g[k][3]));
+        mean[k] = -row_sum<S>(t.x + t.y) * inv_dim;
+      }
+      if (kind != P3D_NORM_LAYER) mean[k] = 0.f;
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      if (kind != P3D_NORM_NONE) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          g[k][i] = sm100::fma2(v[k][i], make_float2(gn[k], gn[k]), sm100::add2(g[k][i], make_float2(mean[k], mean[k])));
+          g[k][i] = sm100::mul2(g[k][i], make_float2(dev[k], dev[k]));
         }
       }
-      T *const dx = static_cast<T *>(r.second ? p.y1 : p.y0);
-      if (dx) store8<T, kVec>(dx + r.out + c, h < rows ? n : 0, g[u]);
+      store8<T, kVec>(out, write && there[k] ? n : 0, g[k]);
+      out += row.out_step;
     }
   }
   if constexpr (kParams) {
-    // the rows of a warp, then the warps of the block, each in a fixed order
+    // the rows of a warp (each of the first or the second input), then the warps of the block, each in a fixed order
     __shared__ float2 joined[kWarps][S][4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
+      __syncthreads();
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < 4; ++i) {
+        float2 v = k < 2 ? sum_w[i] : sum_b[i];
+        if (!row.on || row.second != (k % 2 == 1)) v = make_float2(0.f, 0.f);
 #pragma unroll
         for (int o = S; o < 32; o <<= 1) {
-          sum[k][i].x += __shfl_xor_sync(0xffffffffu, sum[k][i].x, o);
-          sum[k][i].y += __shfl_xor_sync(0xffffffffu, sum[k][i].y, o);
+          v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+          v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
         }
-      __syncthreads();
-      if (lane < S) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) joined[threadIdx.x / 32][lane][i] = sum[k][i];
+        if (lane < S) joined[threadIdx.x / 32][lane][i] = v;
       }
       __syncthreads();
       for (int col = threadIdx.x; col < p.dim; col += kWarps * 32) {
@@ -338,8 +411,11 @@ __global__ void __launch_bounds__(1024) rotate_join_kernel(const float *partial,
   const int dtype = k == 0 ? j.dtype[0] : k == 1 ? j.dtype[1] : k == 2 ? j.dtype[2] : j.dtype[3];
   if (!out) return;
   float v = 0.f;
-  if (col < dim)
-    for (int i = threadIdx.x / 32; i < blocks; i += 32) v += partial[((int64_t)k * blocks + i) * dim + col];
+  if (col < dim) {
+    const float *from = partial + (int64_t)k * blocks * dim + col;
+#pragma unroll 8
+    for (int i = threadIdx.x / 32; i < blocks; i += 32) v += from[(int64_t)i * dim];
+  }
   s[threadIdx.x / 32][threadIdx.x % 32] = v;
   __syncthreads();
   if (threadIdx.x >= 32 || col >= dim) return;
@@ -351,8 +427,7 @@ __global__ void __launch_bounds__(1024) rotate_join_kernel(const float *partial,
 // ------------------------------------------------------------------------------- host
 struct Plan {
   RotateParams p;
-  int lanes, passes, vec;
-  int warps;   // that one wave of the device holds
+  int lanes, passes, vec, sms;
 };
 
 int plan(const p3d_norm_rotate *a, Plan *out) {
@@ -423,65 +498,74 @@ int plan(const p3d_norm_rotate *a, Plan *out) {
   out->vec = a->dim % 8 == 0 && fits(p.x0, p.ts0, p.hs0) && (!p.h1 || fits(p.x1, p.ts1, p.hs1));
   DeviceInfo info;
   if (int st = device_info(&info)) return st;
-  out->warps = info.sm_count * 32;
+  out->sms = info.sm_count;
   return P3D_OK;
 }
 
-// Passes of a warp's item: as many loads in flight as the row's heads give, but not so many that the device's warps lack items.
-int set_items(Plan *pl, int most) {
-  int u = 1;
-  while (u < most && u < pl->passes && (int64_t)pl->p.tokens * ((pl->passes + 2 * u - 1) / (2 * u)) >= pl->warps) u *= 2;
-  pl->p.chunks = (pl->passes + u - 1) / u;
-  pl->p.items = pl->p.tokens * pl->p.chunks;
-  return u;
+// Blocks so that `per_sm` fill the device or each warp has one item, with the warps a multiple of a token's items.
+int set_items(Plan *pl, int u, int per_sm) {
+  RotateParams &p = pl->p;
+  p.chunks = (uint32_t)(pl->passes + u - 1) / u;
+  uint32_t unit = p.chunks, warps = kWarps;   // blocks that make whole tokens
+  while (unit % 2 == 0 && warps > 1) unit /= 2, warps /= 2;
+  const int64_t most = std::max<int64_t>((int64_t)pl->sms * per_sm / unit, 1);
+  const int64_t need = ((int64_t)p.tokens * p.chunks + (int64_t)unit * kWarps - 1) / ((int64_t)unit * kWarps);
+  return (int)(std::min(most, need) * unit);
 }
 
-template <typename T, int S, int U, bool kVec>
-int launch_u(const Plan &pl, bool backward, bool params, int blocks, cudaStream_t s) {
-  if (!backward)
-    norm_rotate_kernel<T, S, U, kVec><<<blocks, kWarps * 32, 0, s>>>(pl.p);
-  else if (params)
-    norm_rotate_bwd_kernel<T, S, U, kVec, true><<<blocks, kWarps * 32, 0, s>>>(pl.p);
-  else
-    norm_rotate_bwd_kernel<T, S, U, kVec, false><<<blocks, kWarps * 32, 0, s>>>(pl.p);
+// Two passes an item, where a warp's first item leaves work for the others.
+int passes_of(const Plan &pl) { return pl.vec && pl.passes >= 2 && (int64_t)pl.p.tokens * pl.passes >= 8ll * pl.sms ? 2 : 1; }
+
+template <typename T, int S>
+int launch_s(Plan pl, bool backward, bool params, int blocks, int u, cudaStream_t s) {
+  const RotateParams &p = pl.p;
+  const bool bias = p.b0 || p.b1;
+  auto fwd = [&](auto vec, auto passes, auto with_bias) {
+    norm_rotate_kernel<T, S, decltype(passes)::value, decltype(vec)::value, decltype(with_bias)::value><<<blocks, kWarps * 32, 0, s>>>(p);
+  };
+  auto bwd = [&](auto vec, auto with_params) {
+    norm_rotate_bwd_kernel<T, S, decltype(vec)::value, decltype(with_params)::value><<<blocks, kWarps * 32, 0, s>>>(p);
+  };
+  using One = std::integral_constant<int, 1>;
+  using Two = std::integral_constant<int, 2>;
+  using Yes = std::true_type;
+  using No = std::false_type;
+  if (backward) {
+    if (pl.vec) params ? bwd(Yes(), Yes()) : bwd(Yes(), No());
+    else params ? bwd(No(), Yes()) : bwd(No(), No());
+  } else if (!pl.vec) {
+    fwd(No(), One(), Yes());
+  } else if (u == 2) {
+    bias ? fwd(Yes(), Two(), Yes()) : fwd(Yes(), Two(), No());
+  } else {
+    bias ? fwd(Yes(), One(), Yes()) : fwd(Yes(), One(), No());
+  }
   P3D_LAUNCH_CHECK();
   return P3D_OK;
 }
 
-template <typename T, int S>
-int launch_s(const Plan &pl, int u, bool backward, bool params, int blocks, cudaStream_t s) {
-  if (!pl.vec) return launch_u<T, S, 1, false>(pl, backward, params, blocks, s);
-  switch (u) {
-    case 1: return launch_u<T, S, 1, true>(pl, backward, params, blocks, s);
-    case 2: return launch_u<T, S, 2, true>(pl, backward, params, blocks, s);
-    default: return launch_u<T, S, 4, true>(pl, backward, params, blocks, s);
-  }
-}
-
 template <typename T>
-int launch_t(const Plan &pl, int u, bool backward, bool params, int blocks, cudaStream_t s) {
+int launch_t(const Plan &pl, bool backward, bool params, int blocks, int u, cudaStream_t s) {
   switch (pl.lanes) {
-    case 1: return launch_s<T, 1>(pl, u, backward, params, blocks, s);
-    case 2: return launch_s<T, 2>(pl, u, backward, params, blocks, s);
-    case 4: return launch_s<T, 4>(pl, u, backward, params, blocks, s);
-    case 8: return launch_s<T, 8>(pl, u, backward, params, blocks, s);
-    case 16: return launch_s<T, 16>(pl, u, backward, params, blocks, s);
-    default: return launch_s<T, 32>(pl, u, backward, params, blocks, s);
+    case 1: return launch_s<T, 1>(pl, backward, params, blocks, u, s);
+    case 2: return launch_s<T, 2>(pl, backward, params, blocks, u, s);
+    case 4: return launch_s<T, 4>(pl, backward, params, blocks, u, s);
+    case 8: return launch_s<T, 8>(pl, backward, params, blocks, u, s);
+    case 16: return launch_s<T, 16>(pl, backward, params, blocks, u, s);
+    default: return launch_s<T, 32>(pl, backward, params, blocks, u, s);
   }
 }
 
-int launch(const Plan &pl, int dtype, int u, bool backward, bool params, int blocks, cudaStream_t s) {
+int launch(const Plan &pl, int dtype, bool backward, bool params, int blocks, int u, cudaStream_t s) {
   switch (dtype) {
-    case P3D_F16: return launch_t<__half>(pl, u, backward, params, blocks, s);
-    case P3D_BF16: return launch_t<__nv_bfloat16>(pl, u, backward, params, blocks, s);
-    default: return launch_t<float>(pl, u, backward, params, blocks, s);
+    case P3D_F16: return launch_t<__half>(pl, backward, params, blocks, u, s);
+    case P3D_BF16: return launch_t<__nv_bfloat16>(pl, backward, params, blocks, u, s);
+    default: return launch_t<float>(pl, backward, params, blocks, u, s);
   }
 }
 
-// Blocks of the backward: what one wave holds, as each leaves a row of partial sums.
-int backward_blocks(const Plan &pl) {
-  return (int)std::min<int64_t>((pl.p.items + kWarps - 1) / kWarps, std::max(1, pl.warps / 32 * 2));
-}
+// Blocks an SM, by the kernels' registers.
+constexpr int kPerSmForward = 5, kPerSmBackward = 4;
 
 }  // namespace
 }  // namespace p3d
@@ -497,16 +581,14 @@ int p3d_norm_rotate_fwd(const p3d_norm_rotate *args, void *y0, void *y1, void *s
   P3D_CHECK_ARG(y0 && (y1 || !args->heads[1]), "p3d_norm_rotate_fwd: null output");
   pl.vec = pl.vec && (uintptr_t)y0 % 16 == 0 && (uintptr_t)y1 % 16 == 0;
   pl.p.y0 = y0, pl.p.y1 = y1;
-  const int u = set_items(&pl, pl.vec ? 4 : 1);
-  const int64_t blocks = std::min<int64_t>((pl.p.items + kWarps - 1) / kWarps, pl.warps / 32 * 6);
-  return launch(pl, args->dtype, u, false, false, (int)blocks, (cudaStream_t)stream);
+  const int u = passes_of(pl), blocks = set_items(&pl, u, kPerSmForward);
+  return launch(pl, args->dtype, false, false, blocks, u, (cudaStream_t)stream);
 }
 
 size_t p3d_norm_rotate_bwd_workspace(const p3d_norm_rotate *args) {
   Plan pl;
   if (plan(args, &pl) != P3D_OK || args->tokens == 0) return 0;
-  set_items(&pl, 1);
-  return sizeof(float) * 4 * (size_t)backward_blocks(pl) * pl.p.dim;
+  return sizeof(float) * 4 * (size_t)set_items(&pl, 1, kPerSmBackward) * pl.p.dim;
 }
 
 int p3d_norm_rotate_bwd(const p3d_norm_rotate *args, const void *const dy[2], void *const dx[2], void *const dweight[2],
@@ -522,14 +604,12 @@ int p3d_norm_rotate_bwd(const p3d_norm_rotate *args, const void *const dy[2], vo
   auto aligned = [](const void *q) { return (uintptr_t)q % 16 == 0; };
   pl.vec = pl.vec && aligned(dy[0]) && aligned(dy[1]) && aligned(dx[0]) && aligned(dx[1]);
   pl.p.dy0 = dy[0], pl.p.dy1 = dy[1], pl.p.y0 = dx[0], pl.p.y1 = dx[1];
-  // two passes in flight: four take the registers of the parameters' sums
-  const int u = set_items(&pl, pl.vec ? 2 : 1);
-  const int blocks = backward_blocks(pl);
+  const int blocks = set_items(&pl, 1, kPerSmBackward);
   pl.p.partial = static_cast<float *>(workspace);
   if (params && (!workspace || workspace_bytes < sizeof(float) * 4 * (size_t)blocks * pl.p.dim))
     return fail(P3D_ERR_WORKSPACE, "p3d_norm_rotate_bwd: workspace of %zu bytes needed",
                 sizeof(float) * 4 * (size_t)blocks * pl.p.dim);
-  if (int st = launch(pl, args->dtype, u, true, params, blocks, (cudaStream_t)stream)) return st;
+  if (int st = launch(pl, args->dtype, true, params, blocks, 1, (cudaStream_t)stream)) return st;
   if (!params) return P3D_OK;
   JoinParams j = {{dweight[0], dweight[1], dbias[0], dbias[1]},
                   {args->param_dtype[0], args->param_dtype[1], args->param_dtype[0], args->param_dtype[1]}};
