@@ -9,7 +9,8 @@
 //   key are the columns that it contributes to two (8-bit: four) products, and 16 consecutive bytes of a value row are its
 //   column in eight (sixteen) of them. The heads of a group are the products' 16 rows (padded: the tensor pipe has time to
 //   spare at this intensity).
-// * A tile's values and the next tile's keys are in flight while a tile is worked on; the page table is read a tile further ahead.
+// * The next tile's keys are asked for as soon as this one's are used, and its values likewise: one memory latency a tile, with both
+//   under way (values asked for at a tile's start instead: two, 0.23 ms for 0.16). The page table is read a tile further ahead.
 // * 8 bits: e4m3 goes to f16 exactly. A query is brought below 2 by a power of two, the keys' scales multiply the scores. The
 //   values' scales 2^e go into the weights, which are held relative to the largest weighted scale, m = max(s_t + e_t), so that they
 //   fit f16 whatever the scales; the sum of weights without them stays in fp32.
@@ -347,9 +348,9 @@ __device__ __forceinline__ void attend(const Params &p, Shared<DP> &sh, int b, i
   uint32_t now = W::resolve(p, b, g, n, first, lane), next = W::resolve(p, b, g, last > first + kStep ? n : 0, first + kStep, lane);
   uint32_t kb, vb;
   w.load_k(p, now, lane);
+  w.load_v(p, now, lane);
   scale_bytes(now, kb, vb);
   for (int64_t at = first; at < last; at += kStep) {
-    w.load_v(p, now, lane);
     float s[W::NT][4];
     w.scores(s);
     uint32_t kb2, vb2;
@@ -357,6 +358,7 @@ __device__ __forceinline__ void attend(const Params &p, Shared<DP> &sh, int b, i
     scale_bytes(next, kb2, vb2);
     const uint32_t after = W::resolve(p, b, g, at + 2 * kStep < last ? n : 0, at + 2 * kStep, lane);
     w.add(s, now, kb, vb, lane);
+    w.load_v(p, next, lane);
     now = next, next = after, kb = kb2, vb = vb2;
   }
   const int r = lane / 4, c = lane % 4;
@@ -493,11 +495,15 @@ __global__ void __launch_bounds__(kWarps * 32, per_sm(k8, DP)) paged_kernel(cons
   }
 }
 
-// The pieces of one head (a block), added in the order of the line; empty sequences get 0.
-template <typename T, int DP>
+// The pieces of one query head (a block), added in the order of the line; empty sequences get 0.
+constexpr int kMaxPieces = 1024;
+template <typename T>
 __global__ void __launch_bounds__(kWarps * 32) join_kernel(const __grid_constant__ Params p, int unit) {
-  const int heads = p.c.kv_heads * p.row_tiles, b = blockIdx.x / heads, h = blockIdx.x % heads, g = h / p.row_tiles;
-  const int head0 = g * p.group + h % p.row_tiles * kRows, rows = min(kRows, p.group - h % p.row_tiles * kRows), dim = p.c.dim;
+  __shared__ int64_t sums[2][kWarps];
+  __shared__ float weight[kMaxPieces], reduced[2][kWarps];
+  const int b = blockIdx.x / p.heads, head = blockIdx.x % p.heads, g = head / p.group, in_group = head % p.group;
+  const int heads = p.c.kv_heads * p.row_tiles, h = g * p.row_tiles + in_group / kRows, row = in_group % kRows, dim = p.c.dim;
+  const int warp = threadIdx.x / 32;
   // the units before sequence b, and all of them
   int64_t before = 0, total = 0;
   for (int i = threadIdx.x; i < p.c.sequences; i += kWarps * 32) {
@@ -510,39 +516,54 @@ __global__ void __launch_bounds__(kWarps * 32) join_kernel(const __grid_constant
     before += __shfl_xor_sync(0xffffffffu, before, o);
     total += __shfl_xor_sync(0xffffffffu, total, o);
   }
-  __shared__ int64_t sums[2][kWarps];
-  if ((threadIdx.x & 31) == 0) sums[0][threadIdx.x / 32] = before, sums[1][threadIdx.x / 32] = total;
+  if ((threadIdx.x & 31) == 0) sums[0][warp] = before, sums[1][warp] = total;
   __syncthreads();
   before = total = 0;
 #pragma unroll
   for (int i = 0; i < kWarps; ++i) before += sums[0][i], total += sums[1][i];
   const int64_t units = (length_of(p, b) + (int64_t)unit - 1) / unit;
-  T *out = static_cast<T *>(p.out) + ((int64_t)b * p.heads + head0) * dim;
+  T *const out = static_cast<T *>(p.out) + ((int64_t)b * p.heads + head) * dim;
   // in every block: this kernel's end stands for the first one's too
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (units == 0) {
-    for (int e = threadIdx.x; e < rows * dim; e += kWarps * 32) out[e] = from_f32<T>(0.f);
+    for (int col = threadIdx.x; col < dim; col += kWarps * 32) out[col] = from_f32<T>(0.f);
     return;
   }
   before = before * heads + h * units;
   total *= heads;
   // CTA i of n has the places from total * i / n on
   const int64_t n = line_ctas(p, total);
-  const int first = (int)(((before + 1) * n - 1) / total), last = (int)(((before + units) * n - 1) / total);
-  if (first == last) return;
+  const int first = (int)(((before + 1) * n - 1) / total), pieces = (int)(((before + units) * n - 1) / total) - first + 1;
+  if (pieces == 1) return;
   const int64_t size = (int64_t)p.part_rows * (dim + 2);
-  for (int e = threadIdx.x; e < rows * dim; e += kWarps * 32) {
-    const int row = e / dim, col = e - row * dim;
-    float top = -INFINITY, o = 0.f, l = 0.f;
-    for (int i = first; i <= last; ++i) {
-      const float *part = p.parts + (2 * i + (i == first)) * size + row * (dim + 2);
-      const float m = part[dim], to = fmaxf(top, m), ref = to == -INFINITY ? 0.f : to;
-      const float down = sm100::ex2_approx(top - ref), f = sm100::ex2_approx(m - ref);
-      o = o * down + f * part[col];
-      l = l * down + f * part[dim + 1];
-      top = to;
+  auto part = [&](int i) { return p.parts + (2 * (first + i) + (i == 0)) * size + (int64_t)row * (dim + 2); };
+  auto all = [&](float v, bool largest, int which) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const float u = __shfl_xor_sync(0xffffffffu, v, o);
+      v = largest ? fmaxf(v, u) : v + u;
     }
-    out[e] = from_f32<T>(o / l);
+    if ((threadIdx.x & 31) == 0) reduced[which][warp] = v;
+    __syncthreads();
+    v = reduced[which][0];
+#pragma unroll
+    for (int i = 1; i < kWarps; ++i) v = largest ? fmaxf(v, reduced[which][i]) : v + reduced[which][i];
+    return v;
+  };
+  float top = -INFINITY, l = 0.f;
+  for (int i = threadIdx.x; i < pieces; i += kWarps * 32) top = fmaxf(top, weight[i] = part(i)[dim]);
+  top = all(top, true, 0);
+  const float ref = top == -INFINITY ? 0.f : top;
+  for (int i = threadIdx.x; i < pieces; i += kWarps * 32) {
+    weight[i] = sm100::ex2_approx(weight[i] - ref);
+    l += weight[i] * part(i)[dim + 1];
+  }
+  l = all(l, false, 1);   // and the weights are there
+  for (int col = threadIdx.x; col < dim; col += kWarps * 32) {
+    float o = 0.f;
+#pragma unroll 8
+    for (int i = 0; i < pieces; ++i) o = fmaf(weight[i], part(i)[col], o);
+    out[col] = from_f32<T>(o / l);
   }
 }
 
@@ -562,7 +583,7 @@ int plan(const p3d_cache *c, int heads, Plan *out) {
   // as far as the tables reach: a few units a head are done by one CTA, which costs less than a second kernel
   const int64_t unit = unit_of(*c), most = ((int64_t)c->table_width * c->page_size + unit - 1) / unit;
   const int64_t all = most * c->sequences * c->kv_heads * out->row_tiles;
-  out->ctas = most <= 4 ? 0 : (int)std::min<int64_t>(all, (int64_t)info.sm_count * per_sm(c->dtype == P3D_E4M3, padded(c->dim)));
+  out->ctas = most <= 4 ? 0 : (int)std::min<int64_t>(std::min<int64_t>(all, kMaxPieces), (int64_t)info.sm_count * per_sm(c->dtype == P3D_E4M3, padded(c->dim)));
   return P3D_OK;
 }
 
@@ -577,7 +598,7 @@ int launch(const Params &p, cudaStream_t s) {
   if (!p.ctas) return P3D_OK;
   // starts while the first kernel still runs, and waits in the kernel for what it wrote
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(p.c.sequences * heads);
+  cfg.gridDim = dim3(p.c.sequences * p.heads);
   cfg.blockDim = dim3(kWarps * 32);
   cfg.stream = s;
   cudaLaunchAttribute attr = {};
@@ -585,7 +606,7 @@ int launch(const Params &p, cudaStream_t s) {
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  P3D_CUDA_TRY(cudaLaunchKernelEx(&cfg, join_kernel<T, DP>, p, (int)(Tile<T, k8, DP>::TT * kWarps)));
+  P3D_CUDA_TRY(cudaLaunchKernelEx(&cfg, join_kernel<T>, p, (int)(Tile<T, k8, DP>::TT * kWarps)));
   return P3D_OK;
 }
 
