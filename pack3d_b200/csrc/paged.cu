@@ -46,6 +46,7 @@ struct Params {
   int row_tiles;        // tiles of 16 query heads that a group takes
   int ctas;             // that the line is cut for; 0: a CTA for each head
   int wide;             // 8-bit rows are 16-byte aligned
+  int exact;            // the head dim is the padded one: no piece of a row is cut
   float *parts;         // [2 * ctas][part_rows][dim + 2]
   int part_rows;
 };
@@ -95,7 +96,8 @@ struct Tile {
   uint32_t q[KC * (k8 ? 4 : 2)][4];   // A operands, a step of 16 columns each
   float q_scale[2];                   // of rows lane / 4 and + 8: scale and, for 8 bits, the query's power of two
   uint32_t k[NT][KC][4], v[KT][4][VC][VW];
-  float o[CT][4], m[2], l[2];
+  float o[CT][4], m[2];
+  float2 l[2];                        // of the even and odd columns that a lane has
 
   __device__ __forceinline__ static uint4 load16(const uint8_t *p, int at, int bytes, int wide) {
     uint4 w = make_uint4(0, 0, 0, 0);
@@ -177,8 +179,22 @@ struct Tile {
     return static_cast<const uint8_t *>(pages) + (uint64_t)row * (uint32_t)bytes;
   }
 
-  __device__ __forceinline__ void load_k(const Params &p, uint32_t rows, int lane) {
+  // `all`: every token of the tile is there and rows are whole, as in all tiles but a sequence's last: loads without conditions.
+  __device__ __forceinline__ void load_k(const Params &p, uint32_t rows, bool all, int lane) {
     const int bytes = p.c.dim * (k8 ? 1 : 2);
+    if (all) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const uint4 *from = reinterpret_cast<const uint4 *>(
+            row_of(p.c.k, __shfl_sync(0xffffffffu, rows, t * 8 + lane / 4), DP * (k8 ? 1 : 2)) + lane % 4 * 16);
+#pragma unroll
+        for (int s = 0; s < KC; ++s) {
+          const uint4 w = __ldg(from + 4 * s);
+          k[t][s][0] = w.x, k[t][s][1] = w.y, k[t][s][2] = w.z, k[t][s][3] = w.w;
+        }
+      }
+      return;
+    }
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       const uint32_t row = __shfl_sync(0xffffffffu, rows, t * 8 + lane / 4);
@@ -191,8 +207,28 @@ struct Tile {
     }
   }
 
-  __device__ __forceinline__ void load_v(const Params &p, uint32_t rows, int lane) {
+  __device__ __forceinline__ void load_v(const Params &p, uint32_t rows, bool all, int lane) {
     const int bytes = p.c.dim * (k8 ? 1 : 2);
+    if (all) {
+#pragma unroll
+      for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint8_t *from = row_of(p.c.v, __shfl_sync(0xffffffffu, rows, t * 16 + lane % 4 * 2 + i % 2 + i / 2 * 8),
+                                       DP * (k8 ? 1 : 2)) + lane / 4 * VB;
+#pragma unroll
+          for (int s = 0; s < VC; ++s) {
+            if constexpr (VW == 4) {
+              const uint4 w = __ldg(reinterpret_cast<const uint4 *>(from + s * 128));
+              v[t][i][s][0] = w.x, v[t][i][s][1] = w.y, v[t][i][s][2] = w.z, v[t][i][s][3] = w.w;
+            } else {
+              const uint2 w = __ldg(reinterpret_cast<const uint2 *>(from));
+              v[t][i][s][0] = w.x, v[t][i][s][1] = w.y;
+            }
+          }
+        }
+      return;
+    }
 #pragma unroll
     for (int t = 0; t < KT; ++t)
 #pragma unroll
@@ -234,28 +270,41 @@ struct Tile {
     }
   }
 
-  // Weights from scores, running maximum and sum, and the weighted values.  `kb`, `vb`: the lane's token's scale bytes.
-  __device__ __forceinline__ void add(float (&s)[NT][4], uint32_t rows, uint32_t kb, uint32_t vb, int lane) {
+  // Weights from scores, running maximum and sum, and the weighted values.  Of the lane's token: ks, vs its scales 2^e, e the value's.
+  __device__ __forceinline__ void add(float (&s)[NT][4], uint32_t rows, bool all, float ks, float vs, float e, int lane) {
+    using sm100::add2;
+    using sm100::mul2;
     const int c = lane % 4;
-    float e[NT][2], top[2] = {m[0], m[1]};
+    float2 y[NT][2], scale[NT];   // scores of rows r, r + 8; the values' scales
+    float top[2] = {m[0], m[1]};
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+    for (int t = 0; t < NT; ++t) {
+      const int from = t * 8 + c * 2;
+      float2 key = make_float2(1.f, 1.f), ev = make_float2(0.f, 0.f);
+      if constexpr (k8) {
+        key = make_float2(__shfl_sync(0xffffffffu, ks, from), __shfl_sync(0xffffffffu, ks, from + 1));
+        scale[t] = make_float2(__shfl_sync(0xffffffffu, vs, from), __shfl_sync(0xffffffffu, vs, from + 1));
+        ev = make_float2(__shfl_sync(0xffffffffu, e, from), __shfl_sync(0xffffffffu, e, from + 1));
+      }
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const int from = t * 8 + c * 2 + x;
-        const uint32_t row = __shfl_sync(0xffffffffu, rows, from);
-        const float ks = k8 ? two_to(__shfl_sync(0xffffffffu, kb, from)) : 1.f;
-        e[t][x] = k8 ? (float)(int)__shfl_sync(0xffffffffu, vb, from) - 127.f : 0.f;
+      for (int i = 0; i < 2; ++i) {
+        y[t][i] = mul2(make_float2(s[t][2 * i], s[t][2 * i + 1]), make_float2(q_scale[i], q_scale[i]));
+        if constexpr (k8) y[t][i] = mul2(y[t][i], key);
+      }
+      if (!all) {
+        const uint32_t r0 = __shfl_sync(0xffffffffu, rows, from), r1 = __shfl_sync(0xffffffffu, rows, from + 1);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          float y = s[t][2 * i + x] * q_scale[i];
-          if constexpr (k8) y *= ks;
-          y = row == kNone ? -INFINITY : row == kBad ? NAN : y;
-          s[t][2 * i + x] = y;
-          // a scale below 2^-96 does not set the reference, so that the sum of weights stays finite
-          top[i] = fmaxf(top[i], k8 ? y + fmaxf(e[t][x], -96.f) : y);
+          y[t][i].x = r0 == kNone ? -INFINITY : r0 == kBad ? NAN : y[t][i].x;
+          y[t][i].y = r1 == kNone ? -INFINITY : r1 == kBad ? NAN : y[t][i].y;
         }
       }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float2 u = k8 ? add2(y[t][i], ev) : y[t][i];
+        top[i] = fmaxf(top[i], fmaxf(u.x, u.y));
+      }
+    }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
@@ -265,7 +314,7 @@ struct Tile {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const float down = m[i] == -INFINITY ? 0.f : sm100::ex2_approx(m[i] - top[i]);
-        l[i] *= down;
+        l[i] = mul2(l[i], make_float2(down, down));
 #pragma unroll
         for (int j = 0; j < CT; ++j) {
           o[j][2 * i] *= down;
@@ -274,7 +323,8 @@ struct Tile {
         m[i] = top[i];
       }
     }
-    const float ref[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
+    const float2 minus[2] = {m[0] == -INFINITY ? make_float2(0.f, 0.f) : make_float2(-m[0], -m[0]),
+                             m[1] == -INFINITY ? make_float2(0.f, 0.f) : make_float2(-m[1], -m[1])};
 #pragma unroll
     for (int t = 0; t < KT; ++t) {
       uint32_t w[4];   // A operand: rows r, r + 8; tokens 2c, 2c + 1 and + 8
@@ -282,30 +332,26 @@ struct Tile {
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          float p[2];
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            const float y = s[2 * t + h][2 * i + x] - ref[i];
-            p[x] = sm100::ex2_approx(y);
-            l[i] += p[x];
-            if constexpr (k8) p[x] = sm100::ex2_approx(y + e[2 * t + h][x]);
-          }
-          w[2 * h + i] = pack<M>(p[0], p[1]);
+          const float2 x = add2(y[2 * t + h][i], minus[i]);
+          float2 p = make_float2(sm100::ex2_approx(x.x), sm100::ex2_approx(x.y));
+          l[i] = add2(l[i], p);
+          if constexpr (k8) p = mul2(p, scale[2 * t + h]);
+          w[2 * h + i] = pack<M>(p.x, p.y);
         }
 #pragma unroll
       for (int s4 = 0; s4 < VC; ++s4)
 #pragma unroll
         for (int x = 0; x < VW; ++x) {
           if constexpr (k8) {
-            // four columns of rows 2c, 2c + 1, 2c + 8, 2c + 9
+            // bytes of rows 2c and 2c + 1 (2c + 8 and 2c + 9) side by side, two columns a word
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-              uint32_t f[4];
-#pragma unroll
-              for (int i = 0; i < 4; ++i) f[i] = e4m3x2(half ? v[t][i][s4][x] >> 16 : v[t][i][s4][x]);
+              const uint32_t order = half ? 0x7362 : 0x5140;
+              const uint32_t lo = __byte_perm(v[t][0][s4][x], v[t][1][s4][x], order);
+              const uint32_t hi = __byte_perm(v[t][2][s4][x], v[t][3][s4][x], order);
               const int j = 4 * x + 2 * half;
-              mma<M>(o[j], w, __byte_perm(f[0], f[1], 0x5410), __byte_perm(f[2], f[3], 0x5410));
-              mma<M>(o[j + 1], w, __byte_perm(f[0], f[1], 0x7632), __byte_perm(f[2], f[3], 0x7632));
+              mma<M>(o[j], w, e4m3x2(lo), e4m3x2(hi));
+              mma<M>(o[j + 1], w, e4m3x2(lo >> 16), e4m3x2(hi >> 16));
             }
           } else {
             const int j = s4 * 8 + 2 * x;
@@ -336,37 +382,46 @@ __device__ __forceinline__ void attend(const Params &p, Shared<DP> &sh, int b, i
   W w;
   w.load_q(p, b, head0, rows, lane);
 #pragma unroll
-  for (int i = 0; i < 2; ++i) w.m[i] = -INFINITY, w.l[i] = 0.f;
+  for (int i = 0; i < 2; ++i) w.m[i] = -INFINITY, w.l[i] = make_float2(0.f, 0.f);
 #pragma unroll
   for (int j = 0; j < W::CT; ++j) w.o[j][0] = w.o[j][1] = w.o[j][2] = w.o[j][3] = 0.f;
   constexpr int64_t kStep = W::TT * kWarps;
   const int64_t first = unit0 * kStep + warp * W::TT, last = unit1 * kStep;
-  auto scale_bytes = [&](uint32_t row, uint32_t &kb, uint32_t &vb) {
+  // a lane's token's scales; a value's exponent below -96 does not set the reference, so that the sum of weights stays finite
+  float ks = 1.f, vs = 1.f, e = 0.f;
+  auto scales = [&](uint32_t row, uint32_t &kb, uint32_t &vb) {
     kb = vb = 127;
     if (k8 && row < kBad) kb = __ldg(p.c.k_scales + row), vb = __ldg(p.c.v_scales + row);
   };
+  auto all_there = [&](uint32_t row) { return p.exact && __all_sync(0xffffffffu, row < kBad || lane >= W::TT); };
   uint32_t now = W::resolve(p, b, g, n, first, lane), next = W::resolve(p, b, g, last > first + kStep ? n : 0, first + kStep, lane);
   uint32_t kb, vb;
-  w.load_k(p, now, lane);
-  w.load_v(p, now, lane);
-  scale_bytes(now, kb, vb);
+  bool all = all_there(now);
+  w.load_k(p, now, all, lane);
+  w.load_v(p, now, all, lane);
+  scales(now, kb, vb);
   for (int64_t at = first; at < last; at += kStep) {
     float s[W::NT][4];
     w.scores(s);
-    uint32_t kb2, vb2;
-    w.load_k(p, next, lane);
-    scale_bytes(next, kb2, vb2);
+    if constexpr (k8) {
+      ks = two_to(kb), vs = two_to(vb);
+      e = fmaxf((float)(int)vb - 127.f, -96.f);
+    }
+    const bool next_all = all_there(next);
+    w.load_k(p, next, next_all, lane);
+    scales(next, kb, vb);
     const uint32_t after = W::resolve(p, b, g, at + 2 * kStep < last ? n : 0, at + 2 * kStep, lane);
-    w.add(s, now, kb, vb, lane);
-    w.load_v(p, next, lane);
-    now = next, next = after, kb = kb2, vb = vb2;
+    w.add(s, now, all, ks, vs, e, lane);
+    w.load_v(p, next, next_all, lane);
+    now = next, next = after, all = next_all;
   }
   const int r = lane / 4, c = lane % 4;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    w.l[i] += __shfl_xor_sync(0xffffffffu, w.l[i], 1);
-    w.l[i] += __shfl_xor_sync(0xffffffffu, w.l[i], 2);
-    if (c == 0) sh.m[warp][r + 8 * i] = w.m[i], sh.l[warp][r + 8 * i] = w.l[i];
+    float l = w.l[i].x + w.l[i].y;
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    if (c == 0) sh.m[warp][r + 8 * i] = w.m[i], sh.l[warp][r + 8 * i] = l;
 #pragma unroll
     for (int j = 0; j < W::CT; ++j)
 #pragma unroll
@@ -671,6 +726,7 @@ int p3d_paged_attention(const p3d_cache *c, const void *q, const int64_t q_strid
   p.scale = scale * 1.4426950408889634f;
   p.heads = heads, p.group = heads / c->kv_heads, p.row_tiles = pl.row_tiles, p.ctas = pl.ctas, p.part_rows = pl.part_rows;
   p.wide = c->dtype != P3D_E4M3 || c->dim % 16 == 0;
+  p.exact = c->dim == padded(c->dim);
   p.parts = static_cast<float *>(workspace);
   return dtype == P3D_F16 ? launch_t<__half>(p, (cudaStream_t)stream) : launch_t<__nv_bfloat16>(p, (cudaStream_t)stream);
 }
