@@ -9,8 +9,8 @@
 //   key are the columns that it contributes to two (8-bit: four) products, and 16 consecutive bytes of a value row are its
 //   column in eight (sixteen) of them. The heads of a group are the products' 16 rows (padded: the tensor pipe has time to
 //   spare at this intensity).
-// * The next tile's keys are asked for as soon as this one's are used, and its values likewise: one memory latency a tile, with both
-//   under way (values asked for at a tile's start instead: two, 0.23 ms for 0.16). The page table is read a tile further ahead.
+// * The next tile's keys and values are asked for as soon as this one's scores are there, before its softmax and its values' products.
+//   For the registers that takes, the queries stay in shared memory. The page table is read a tile further ahead.
 // * 8 bits: e4m3 goes to f16 exactly. A query is brought below 2 by a power of two, the keys' scales multiply the scores. The
 //   values' scales 2^e go into the weights, which are held relative to the largest weighted scale, m = max(s_t + e_t), so that they
 //   fit f16 whatever the scales; the sum of weights without them stays in fp32.
@@ -93,9 +93,12 @@ struct Tile {
     else return j / 8 * 64 + x * 8 + j % 8;
   }
 
-  uint32_t q[KC * (k8 ? 4 : 2)][4];   // A operands, a step of 16 columns each
+  static constexpr int kSteps = KC * (k8 ? 4 : 2);                     // of 16 columns
   float q_scale[2];                   // of rows lane / 4 and + 8: scale and, for 8 bits, the query's power of two
-  uint32_t k[NT][KC][4], v[KT][4][VC][VW];
+  uint32_t k[NT][KC][4];
+  struct Values {
+    uint32_t w[KT][4][VC][VW];
+  };
   float o[CT][4], m[2];
   float2 l[2];                        // of the even and odd columns that a lane has
 
@@ -113,7 +116,9 @@ struct Tile {
     return w;
   }
 
-  __device__ __forceinline__ void load_q(const Params &p, int b, int head0, int rows, int lane) {
+  // The queries as A operands, in shared memory: [step][lane], written by one warp.
+  __device__ __forceinline__ void load_q(const Params &p, uint4 *to, bool write, int b, int head0, int rows, int lane) {
+    uint32_t q[kSteps][4];
     const int r = lane / 4, c = lane % 4, dim = p.c.dim;
     float top[2] = {0.f, 0.f};
     const T *row[2];
@@ -161,6 +166,9 @@ struct Tile {
         }
       }
     }
+    if (write)
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) to[s * 32 + lane] = make_uint4(q[s][0], q[s][1], q[s][2], q[s][3]);
   }
 
   // What a lane resolves for its tile: the row of token base + lane.
@@ -207,7 +215,7 @@ struct Tile {
     }
   }
 
-  __device__ __forceinline__ void load_v(const Params &p, uint32_t rows, bool all, int lane) {
+  __device__ __forceinline__ void load_v(const Params &p, Values &v, uint32_t rows, bool all, int lane) {
     const int bytes = p.c.dim * (k8 ? 1 : 2);
     if (all) {
 #pragma unroll
@@ -220,10 +228,10 @@ struct Tile {
           for (int s = 0; s < VC; ++s) {
             if constexpr (VW == 4) {
               const uint4 w = __ldg(reinterpret_cast<const uint4 *>(from + s * 128));
-              v[t][i][s][0] = w.x, v[t][i][s][1] = w.y, v[t][i][s][2] = w.z, v[t][i][s][3] = w.w;
+              v.w[t][i][s][0] = w.x, v.w[t][i][s][1] = w.y, v.w[t][i][s][2] = w.z, v.w[t][i][s][3] = w.w;
             } else {
               const uint2 w = __ldg(reinterpret_cast<const uint2 *>(from));
-              v[t][i][s][0] = w.x, v[t][i][s][1] = w.y;
+              v.w[t][i][s][0] = w.x, v.w[t][i][s][1] = w.y;
             }
           }
         }
@@ -240,38 +248,34 @@ struct Tile {
           if constexpr (VW == 4) {
             uint4 w = make_uint4(0, 0, 0, 0);
             if (row < kBad) w = load16(row_of(p.c.v, row, bytes), at, bytes, p.wide);
-            v[t][i][s][0] = w.x, v[t][i][s][1] = w.y, v[t][i][s][2] = w.z, v[t][i][s][3] = w.w;
+            v.w[t][i][s][0] = w.x, v.w[t][i][s][1] = w.y, v.w[t][i][s][2] = w.z, v.w[t][i][s][3] = w.w;
           } else {
             uint2 w = make_uint2(0, 0);
             if (row < kBad && at < bytes) w = __ldg(reinterpret_cast<const uint2 *>(row_of(p.c.v, row, bytes) + at));
-            v[t][i][s][0] = w.x, v[t][i][s][1] = w.y;
+            v.w[t][i][s][0] = w.x, v.w[t][i][s][1] = w.y;
           }
         }
       }
   }
 
   // Scores of the tile's tokens: columns 2c, 2c + 1 of each eight in rows r and r + 8.
-  __device__ __forceinline__ void scores(float (&s)[NT][4]) const {
+  __device__ __forceinline__ void scores(float (&s)[NT][4], const uint4 *queries, int lane) const {
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
+    for (int t = 0; t < NT; ++t) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s[t][i] = 0.f;
+    for (int a = 0; a < kSteps; ++a) {
+      const uint4 w = queries[a * 32 + lane];
+      const uint32_t q[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-      for (int a = 0; a < KC; ++a) {
-        if constexpr (k8) {
-#pragma unroll
-          for (int w = 0; w < 4; ++w)
-            mma<M>(s[t], q[4 * a + w], e4m3x2(k[t][a][w]), e4m3x2(k[t][a][w] >> 16));
-        } else {
-          mma<M>(s[t], q[2 * a], k[t][a][0], k[t][a][1]);
-          mma<M>(s[t], q[2 * a + 1], k[t][a][2], k[t][a][3]);
-        }
+      for (int t = 0; t < NT; ++t) {
+        if constexpr (k8) mma<M>(s[t], q, e4m3x2(k[t][a / 4][a % 4]), e4m3x2(k[t][a / 4][a % 4] >> 16));
+        else mma<M>(s[t], q, k[t][a / 2][a % 2 * 2], k[t][a / 2][a % 2 * 2 + 1]);
       }
     }
   }
 
   // Weights from scores, running maximum and sum, and the weighted values.  Of the lane's token: ks, vs its scales 2^e, e the value's.
-  __device__ __forceinline__ void add(float (&s)[NT][4], uint32_t rows, bool all, float ks, float vs, float e, int lane) {
+  __device__ __forceinline__ void add(float (&s)[NT][4], const Values &v, uint32_t rows, bool all, float ks, float vs, float e, int lane) {
     using sm100::add2;
     using sm100::mul2;
     const int c = lane % 4;
@@ -347,18 +351,18 @@ struct Tile {
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
               const uint32_t order = half ? 0x7362 : 0x5140;
-              const uint32_t lo = __byte_perm(v[t][0][s4][x], v[t][1][s4][x], order);
-              const uint32_t hi = __byte_perm(v[t][2][s4][x], v[t][3][s4][x], order);
+              const uint32_t lo = __byte_perm(v.w[t][0][s4][x], v.w[t][1][s4][x], order);
+              const uint32_t hi = __byte_perm(v.w[t][2][s4][x], v.w[t][3][s4][x], order);
               const int j = 4 * x + 2 * half;
               mma<M>(o[j], w, e4m3x2(lo), e4m3x2(hi));
               mma<M>(o[j + 1], w, e4m3x2(lo >> 16), e4m3x2(hi >> 16));
             }
           } else {
             const int j = s4 * 8 + 2 * x;
-            mma<M>(o[j], w, __byte_perm(v[t][0][s4][x], v[t][1][s4][x], 0x5410),
-                   __byte_perm(v[t][2][s4][x], v[t][3][s4][x], 0x5410));
-            mma<M>(o[j + 1], w, __byte_perm(v[t][0][s4][x], v[t][1][s4][x], 0x7632),
-                   __byte_perm(v[t][2][s4][x], v[t][3][s4][x], 0x7632));
+            mma<M>(o[j], w, __byte_perm(v.w[t][0][s4][x], v.w[t][1][s4][x], 0x5410),
+                   __byte_perm(v.w[t][2][s4][x], v.w[t][3][s4][x], 0x5410));
+            mma<M>(o[j + 1], w, __byte_perm(v.w[t][0][s4][x], v.w[t][1][s4][x], 0x7632),
+                   __byte_perm(v.w[t][2][s4][x], v.w[t][3][s4][x], 0x7632));
           }
         }
     }
@@ -367,6 +371,7 @@ struct Tile {
 
 template <int DP>
 struct Shared {
+  uint4 q[8 * 32];
   float m[kWarps][kRows], l[kWarps][kRows], o[kWarps][kRows][DP + 4];
   int64_t sums[kWarps];
   int64_t total, before;
@@ -380,7 +385,8 @@ __device__ __forceinline__ void attend(const Params &p, Shared<DP> &sh, int b, i
   const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
   const int head0 = g * p.group + row_tile * kRows, rows = min(kRows, p.group - row_tile * kRows);
   W w;
-  w.load_q(p, b, head0, rows, lane);
+  w.load_q(p, sh.q, warp == 0, b, head0, rows, lane);
+  __syncthreads();
 #pragma unroll
   for (int i = 0; i < 2; ++i) w.m[i] = -INFINITY, w.l[i] = make_float2(0.f, 0.f);
 #pragma unroll
@@ -398,22 +404,35 @@ __device__ __forceinline__ void attend(const Params &p, Shared<DP> &sh, int b, i
   uint32_t kb, vb;
   bool all = all_there(now);
   w.load_k(p, now, all, lane);
-  w.load_v(p, now, all, lane);
+  typename W::Values even, odd;
+  w.load_v(p, even, now, all, lane);
   scales(now, kb, vb);
-  for (int64_t at = first; at < last; at += kStep) {
+  int64_t at = first;
+  auto tile = [&](const typename W::Values &v, typename W::Values &coming) {
     float s[W::NT][4];
-    w.scores(s);
+    w.scores(s, sh.q, lane);
     if constexpr (k8) {
       ks = two_to(kb), vs = two_to(vb);
       e = fmaxf((float)(int)vb - 127.f, -96.f);
     }
     const bool next_all = all_there(next);
     w.load_k(p, next, next_all, lane);
+    w.load_v(p, coming, next, next_all, lane);
     scales(next, kb, vb);
     const uint32_t after = W::resolve(p, b, g, at + 2 * kStep < last ? n : 0, at + 2 * kStep, lane);
-    w.add(s, now, all, ks, vs, e, lane);
-    w.load_v(p, next, next_all, lane);
+    w.add(s, v, now, all, ks, vs, e, lane);
     now = next, next = after, all = next_all;
+    at += kStep;
+  };
+  while (at < last) {
+    tile(even, odd);
+    if constexpr (k8) {
+      // a copy, which waits for the values: twice the code instead costs more (140 -> 184 us), as it leaves the instruction cache
+      even = odd;
+    } else {
+      if (at >= last) break;
+      tile(odd, even);   // 205 -> 156 us
+    }
   }
   const int r = lane / 4, c = lane % 4;
 #pragma unroll
