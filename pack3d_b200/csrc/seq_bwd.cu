@@ -90,9 +90,11 @@ struct LayoutQ {
   static constexpr int kK = 3, kV = 2;   // stages
   static constexpr size_t kBytes = 1024 + (2 + kK + kV) * (size_t)kTileBytes;
 };
-// Parity waits: each waiter of a barrier that completes many times has seen every completion before. Border tiles have barriers of
-// their own: kSeen (their S is complete), kClean (K cleared).
-enum { kQFull, kSFull, kDPFull = kSFull + 2, kDPFree, kDSFull, kDQDone, kDone, kDrainQ, kSeen, kClean = kSeen + kBorders,
+// Parity waits: each waiter of a barrier that completes many times has seen every completion before, and the one after its own needs a
+// step of the waiter: so dS has a barrier for each of its two buffers (with one, dS of the next keys could be there while the wait for
+// this one's begins, as S and dP of those are made ahead of it). Border tiles have barriers of their own: kSeen (their S is complete),
+// kClean (K cleared).
+enum { kQFull, kSFull, kDPFull = kSFull + 2, kDPFree, kDSFull, kDQDone = kDSFull + 2, kDone, kDrainQ, kSeen, kClean = kSeen + kBorders,
        kKFull = kClean + kBorders, kKEmpty = kKFull + 3, kVFull = kKEmpty + 3, kVEmpty = kVFull + 2, kBarsQ = kVEmpty + 2 };
 
 template <typename T, int DP>
@@ -126,7 +128,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t k_ring = base + 2 * TB, v_ring = k_ring + L::kK * TB;
   auto bar = [&](int i) { return smem_u32(&bar_mem[i]); };
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kBarsQ; ++i) mbar_init(bar(i), i == kDPFree || i == kDSFull ? kSoftmaxWarps : 1);
+    for (int i = 0; i < kBarsQ; ++i) mbar_init(bar(i), i >= kDPFree && i < kDQDone ? kSoftmaxWarps : 1);
     fence_mbar_init();
   }
   if (warp == kMmaWarp) {
@@ -192,32 +194,28 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_wait(bar(kVFull + i % L::kV), (i / L::kV) & 1, &g_seq_bwd_errors, kWaitNs, kErrTeardown);
     }
   } else if (warp == kMmaWarp) {
-    if (lane == 0) {
+    {   // warp-wide, as in the forward kernel
       const uint32_t idesc_s = idesc_f16(128, 128, std::is_same<T, __nv_bfloat16>::value, false);
       const uint64_t d_q = desc_rows(base), d_do = desc_rows(base + TB), d_k = desc_rows(k_ring), d_v = desc_rows(v_ring),
                      d_kc = desc_cols(k_ring);
       int n_s = 0, n_dp = 0, n_dq = 0, n_seen = 0;
       bool done = false;
-      auto wait = [&](int b, uint32_t parity) {
-        if (!mbar_wait(bar(b), parity, &g_seq_bwd_errors, kWaitNs, kErrMma)) return false;
-        tc_fence_after();
-        return true;
-      };
+      auto wait = [&](int b, uint32_t parity) { return wait_warp(bar(b), parity, &g_seq_bwd_errors, kErrMma); };
       auto issue_s = [&](int c) {
         const uint64_t k = d_k + ((uint32_t)(c % L::kK) * TB >> 4);
-        for (int j = 0; j < p.steps; ++j) mma_ss(tmem + 128 * (c & 1), d_q + step_rows(j), k + step_rows(j), idesc_s, j > 0);
-        mma_commit(bar(kSFull + (c & 1)));
+        for (int j = 0; j < p.steps; ++j) mma_ss_warp(tmem + 128 * (c & 1), d_q + step_rows(j), k + step_rows(j), idesc_s, j > 0);
+        mma_commit_warp(bar(kSFull + (c & 1)));
         ++n_s;
         if (c >= border) {
-          mma_commit(bar(kSeen + c - border));
+          mma_commit_warp(bar(kSeen + c - border));
           ++n_seen;
         }
       };
       auto issue_dp = [&](int c) {
         const uint64_t v = d_v + ((uint32_t)(c % L::kV) * TB >> 4);
-        for (int j = 0; j < p.steps; ++j) mma_ss(t_dp, d_do + step_rows(j), v + step_rows(j), idesc_s, j > 0);
-        mma_commit(bar(kDPFull));
-        mma_commit(bar(kVEmpty + c % L::kV));
+        for (int j = 0; j < p.steps; ++j) mma_ss_warp(t_dp, d_do + step_rows(j), v + step_rows(j), idesc_s, j > 0);
+        mma_commit_warp(bar(kDPFull));
+        mma_commit_warp(bar(kVEmpty + c % L::kV));
         ++n_dp;
       };
       bool ok = wait(kQFull, 0) && wait(kKFull, 0);
@@ -236,21 +234,21 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!ok) break;
           issue_dp(c + 1);
         }
-        ok = (c < border || wait(kClean + c - border, 0)) && wait(kDSFull, c & 1);
+        ok = (c < border || wait(kClean + c - border, 0)) && wait(kDSFull + (c & 1), (c >> 1) & 1);
         if (!ok) break;
         const uint64_t k = d_kc + ((uint32_t)(c % L::kK) * TB >> 4);
 #pragma unroll
         for (int j = 0; j < kTile / 16; ++j)   // each softmax group's dS lies over its own half of S
-          mma_ts(t_dq, tmem + 128 * (c & 1) + j / 4 * 64 + j % 4 * 8, k + step_cols(j), p.idesc_out, c > 0 || j > 0);
-        mma_commit(bar(kDQDone));
-        mma_commit(bar(kKEmpty + c % L::kK));
+          mma_ts_warp(t_dq, tmem + 128 * (c & 1) + j / 4 * 64 + j % 4 * 8, k + step_cols(j), p.idesc_out, c > 0 || j > 0);
+        mma_commit_warp(bar(kDQDone));
+        mma_commit_warp(bar(kKEmpty + c % L::kK));
         ++n_dq;
       }
       if (ok) {
-        mma_commit(bar(kDone));
+        mma_commit_warp(bar(kDone));
         done = true;
       }
-      mma_commit(bar(kDrainQ));
+      mma_commit_warp(bar(kDrainQ));
       auto drained = [&](int b, int times) {
         if (times > 0) mbar_wait(bar(b), (times - 1) & 1, &g_seq_bwd_errors, kWaitNs, kErrTeardown);
       };
@@ -313,7 +311,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(bar(kDSFull));
+      if (lane == 0) mbar_arrive(bar(kDSFull + (c & 1)));
     }
     if (ok) ok = wait_warp(bar(kDone), 0, &g_seq_bwd_errors, kErrSoftmax);
     if (ok) {
@@ -485,36 +483,32 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_wait(full(i % NS), (i / NS) & 1, &g_seq_bwd_errors, kWaitNs, kErrTeardown);
     }
   } else if (warp == kMmaWarp) {
-    if (lane == 0) {
+    {   // warp-wide, as in the forward kernel
       const uint32_t idesc_s = idesc_f16(128, 128, std::is_same<T, __nv_bfloat16>::value, false);
       const uint64_t d_k = desc_rows(base), d_v = desc_rows(base + TB), d_ring = desc_rows(ring), d_ringc = desc_cols(ring);
       int n_s = 0, n_dp = 0, n_dv = 0, n_dk = 0, n_seen = 0, borders = 0;
       bool done = false;
-      auto wait = [&](uint32_t b, uint32_t parity) {
-        if (!mbar_wait(b, parity, &g_seq_bwd_errors, kWaitNs, kErrMma)) return false;
-        tc_fence_after();
-        return true;
-      };
+      auto wait = [&](uint32_t b, uint32_t parity) { return wait_warp(b, parity, &g_seq_bwd_errors, kErrMma); };
       auto stage = [&](int i) { return (uint32_t)(i % NS) * L::kStageBytes >> 4; };
       auto issue_s = [&](int i) {
-        for (int j = 0; j < p.steps; ++j) mma_ss(tmem, d_k + step_rows(j), d_ring + stage(i) + step_rows(j), idesc_s, j > 0);
-        mma_commit(bar(kSTFull));
+        for (int j = 0; j < p.steps; ++j) mma_ss_warp(tmem, d_k + step_rows(j), d_ring + stage(i) + step_rows(j), idesc_s, j > 0);
+        mma_commit_warp(bar(kSTFull));
         ++n_s;
       };
       auto issue_dp = [&](int i) {
         const uint64_t o = d_ring + stage(i) + (TB >> 4);
-        for (int j = 0; j < p.steps; ++j) mma_ss(t_dp, d_v + step_rows(j), o + step_rows(j), idesc_s, j > 0);
-        mma_commit(bar(kDPTFull));
+        for (int j = 0; j < p.steps; ++j) mma_ss_warp(t_dp, d_v + step_rows(j), o + step_rows(j), idesc_s, j > 0);
+        mma_commit_warp(bar(kDPTFull));
         ++n_dp;
         if (is_border(i)) {   // covers S too
-          mma_commit(bar(kSeenKV));
+          mma_commit_warp(bar(kSeenKV));
           ++n_seen;
         }
       };
       auto sum = [&](uint32_t to, uint32_t from, uint64_t b, bool more) {
 #pragma unroll
         for (int j = 0; j < kTile / 16; ++j)
-          mma_ts(to, from + j / 4 * 64 + j % 4 * 8, b + step_cols(j), p.idesc_out, more || j > 0);
+          mma_ts_warp(to, from + j / 4 * 64 + j % 4 * 8, b + step_cols(j), p.idesc_out, more || j > 0);
       };
       bool ok = wait(bar(kKVFull), 0) && wait(full(0), 0);
       if (ok) {
@@ -526,7 +520,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = ok && wait(bar(kPFull), i & 1);
         if (!ok) break;
         sum(t_dv, tmem, d_ringc + stage(i) + (TB >> 4), i > 0);
-        mma_commit(bar(kDVDone));
+        mma_commit_warp(bar(kDVDone));
         ++n_dv;
         if (i + 1 < steps) {
           ok = wait(full((i + 1) % NS), ((i + 1) / NS) & 1) && wait(bar(kDVDone), i & 1);
@@ -536,8 +530,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = wait(bar(kDSTFull), i & 1);
         if (!ok) break;
         sum(t_dk, t_dp, d_ringc + stage(i), i > 0);
-        mma_commit(bar(kDKDone));
-        mma_commit(empty(i % NS));
+        mma_commit_warp(bar(kDKDone));
+        mma_commit_warp(empty(i % NS));
         ++n_dk;
         if (i + 1 < steps) {
           ok = wait(bar(kDKDone), i & 1);
@@ -546,10 +540,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       if (ok) {
-        mma_commit(bar(kAllDone));
+        mma_commit_warp(bar(kAllDone));
         done = true;
       }
-      mma_commit(bar(kDrainKV));
+      mma_commit_warp(bar(kDrainKV));
       auto drained = [&](uint32_t b, int times) {
         if (times > 0) mbar_wait(b, (times - 1) & 1, &g_seq_bwd_errors, kWaitNs, kErrTeardown);
       };

@@ -180,15 +180,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp == kMmaWarp) {
     // ------------------------------------------------------------------ products
-    if (lane == 0) {
+    // the whole warp runs this, with the same operands in every lane; one elected lane issues (30 cycles a product instead of 75)
+    {
       const uint32_t idesc_s = idesc_f16(128, 128, std::is_same<T, __nv_bfloat16>::value, false);
       const uint64_t desc_q = desc_rows(base), desc_k = desc_rows(ring), desc_v = desc_cols(ring);
       int n_s[2] = {0, 0}, n_o[2] = {0, 0}, items = 0, landed = 0;
-      auto wait = [&](uint32_t b, uint32_t parity) {
-        if (!mbar_wait(b, parity, &g_seq_fwd_errors, kWaitNs, kErrMma)) return false;
-        tc_fence_after();
-        return true;
-      };
+      auto wait = [&](uint32_t b, uint32_t parity) { return wait_warp(b, parity, &g_seq_fwd_errors, kErrMma); };
       // item i is there (and, for values of a border tile, cleared); items are waited for in order, once
       auto wait_item = [&](int i) {
         while (landed <= i) {
@@ -202,16 +199,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       auto issue_s = [&](int t, int c) {
         const uint64_t q = desc_q + (t * L::kTileBytes >> 4), k = desc_k + ((uint32_t)(2 * c % NS) * L::kTileBytes >> 4);
         for (int j = 0; j < p.steps; ++j)
-          mma_ss(tmem + kColS + 128 * t, q + step_rows(j), k + step_rows(j), idesc_s, j > 0);
-        mma_commit(bar(kSFull + t));
+          mma_ss_warp(tmem + kColS + 128 * t, q + step_rows(j), k + step_rows(j), idesc_s, j > 0);
+        mma_commit_warp(bar(kSFull + t));
         ++n_s[t];
       };
       auto issue_o = [&](int t, int c) {
         const uint64_t v = desc_v + ((uint32_t)((2 * c + 1) % NS) * L::kTileBytes >> 4);
 #pragma unroll
         for (int j = 0; j < kTile / 16; ++j)
-          mma_ts(tmem + kColO + 128 * t, tmem + kColS + 128 * t + 8 * j, v + step_cols(j), p.idesc_o, c > 0 || j > 0);
-        mma_commit(bar(kODone + t));
+          mma_ts_warp(tmem + kColO + 128 * t, tmem + kColS + 128 * t + 8 * j, v + step_cols(j), p.idesc_o, c > 0 || j > 0);
+        mma_commit_warp(bar(kODone + t));
         ++n_o[t];
       };
       bool ok = wait(bar(kQFull), 0) && wait_item(0);
@@ -219,7 +216,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int t = 0; t < 2; ++t)
           if (w.chunks[t]) issue_s(t, 0);
-        mma_commit(empty(0));
+        mma_commit_warp(empty(0));
         items = 1;
       }
       for (int c = 0; ok && c < chunks; ++c) {
@@ -235,12 +232,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         if (!ok) break;
-        mma_commit(empty((2 * c + 1) % NS));
-        if (c + 1 < chunks) mma_commit(empty((2 * c + 2) % NS));
+        mma_commit_warp(empty((2 * c + 1) % NS));
+        if (c + 1 < chunks) mma_commit_warp(empty((2 * c + 2) % NS));
         items += 1 + (c + 1 < chunks);
       }
       // every product completed and every commit arrived before tensor memory and barriers are given up
-      mma_commit(bar(kDrain));
+      mma_commit_warp(bar(kDrain));
       mbar_wait(bar(kDrain), 0, &g_seq_fwd_errors, kWaitNs, kErrTeardown);
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
