@@ -44,15 +44,27 @@ struct Params {
   float sc;                // scale * log2(e)
 };
 
-// 64 columns of scores to weights: 2^(s sc - shift), a quarter of them by polynomial where none is masked.
-__device__ __forceinline__ float2 weight(float2 s, float2 sc, float2 minus, bool poly) {
+// 2^(s sc + minus) of a pair of scores.
+template <bool kPoly>
+__device__ __forceinline__ float2 weight(float2 s, float2 sc, float2 minus) {
   const float2 x = fma2(s, sc, minus);
-  if (poly) {
+  if constexpr (kPoly) {
     // NaN would not come through
     const float2 e = exp2_poly2(x);
     return make_float2(x.x == x.x ? e.x : x.x, x.y == x.y ? e.y : x.y);
+  } else {
+    return make_float2(ex2_approx(x.x), ex2_approx(x.y));
   }
-  return make_float2(ex2_approx(x.x), ex2_approx(x.y));
+}
+// 64 columns, a quarter of them by polynomials where none is masked; minus(k): of columns 2 k, 2 k + 1.
+template <bool kPoly, typename F>
+__device__ __forceinline__ void weights(float (&s)[64], float2 sc, F minus) {
+#pragma unroll
+  for (int k = 0; k < 32; ++k) {
+    const float2 x = make_float2(s[2 * k], s[2 * k + 1]);
+    const float2 w = kPoly && k % 4 == 3 ? weight<true>(x, sc, minus(k)) : weight<false>(x, sc, minus(k));
+    s[2 * k] = w.x, s[2 * k + 1] = w.y;
+  }
 }
 
 template <int N>
@@ -279,11 +291,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       tmem_wait_ld();
       const int limit = seen - c * kTile - half * 64;
       const bool masked = __any_sync(0xffffffffu, limit < 64);
-#pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        const float2 w = weight(make_float2(s[2 * i], s[2 * i + 1]), sc, shift, i % 4 == 3 && !masked);
-        s[2 * i] = w.x, s[2 * i + 1] = w.y;
-      }
+      auto lse = [&](int) { return shift; };
+      if (masked) weights<false>(s, sc, lse);
+      else weights<true>(s, sc, lse);
       ok = wait_warp(bar(kDPFull), c & 1, &g_seq_bwd_errors, kErrSoftmax);
       if (!ok) break;
       float d[64];
@@ -572,12 +582,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       float s[64];
       load_columns<64>(t_s, s);
       tmem_wait_ld();
-#pragma unroll
-      for (int k = 0; k < 32; ++k) {
+      auto lse = [&](int k) {
         const float4 q = st[k];
-        const float2 w = weight(make_float2(s[2 * k], s[2 * k + 1]), sc, make_float2(-q.x, -q.z), k % 4 == 3 && !masked);
-        s[2 * k] = w.x, s[2 * k + 1] = w.y;
-      }
+        return make_float2(-q.x, -q.z);
+      };
+      if (masked) weights<false>(s, sc, lse);
+      else weights<true>(s, sc, lse);
       if (masked) {
 #pragma unroll
         for (int k = 0; k < 64; ++k) s[k] = k >= lo && k < hi ? s[k] : 0.f;

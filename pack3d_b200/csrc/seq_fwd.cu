@@ -31,6 +31,7 @@ __device__ unsigned g_seq_fwd_errors = 0;
 constexpr int kMmaWarp = 8, kCopyWarp = 9, kThreads = 320;
 constexpr uint32_t kColS = 0, kColO = 256;   // tensor memory: S of tile t at 128 t, O at 256 + 128 t
 constexpr float kSlack = 8.f;                // the maximum may lag by 2^8
+constexpr int kPoly = 2;                     // exponentials of eight that are polynomials
 
 template <int DP>
 struct Layout {
@@ -84,6 +85,34 @@ __device__ __forceinline__ Work work_of(const Params &p) {
   }
   w.kv = w.head[0] / group;
   return w;
+}
+
+// P = 2^(s sc + shift) of a row's 128 scores, rounded to T and written over them; returns the row's sum.  kPoly of every eight pairs are
+// polynomials (scores are not NaN there: the row's maximum, and with it shift, would be).
+template <typename T, int kPoly>
+__device__ __forceinline__ float weights(const float (&s)[kTile], float sc, float shift, uint32_t t_s) {
+  const float2 sc2 = make_float2(sc, sc), shift2 = make_float2(shift, shift);
+  float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+  for (int i = 0; i < kTile; i += 32) {
+    uint32_t pk[16];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      const float2 x = fma2(make_float2(s[i + 2 * k], s[i + 2 * k + 1]), sc2, shift2);
+      float2 e;
+      if ((k * kPoly & 7) + kPoly > 7) {
+        e = exp2_poly2(x);
+      } else {
+        e.x = ex2_approx(x.x);
+        e.y = ex2_approx(x.y);
+      }
+      sum[k & 1] = add2(sum[k & 1], e);
+      pk[k] = pack<T>(e.x, e.y);
+    }
+    tmem_st16(t_s + i / 2, pk);
+  }
+  const float2 both = add2(sum[0], sum[1]);
+  return both.x + both.y;
 }
 
 template <typename T, int DP>
@@ -272,13 +301,15 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int i = 0; i < kTile; ++i) s[i] = i < limit ? s[i] : -INFINITY;
       }
-      float top[4];
+      float top[8];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) top[i] = max_nan(s[2 * i], s[2 * i + 1]);
+      for (int i = 0; i < 8; ++i) top[i] = max_nan(s[2 * i], s[2 * i + 1]);
 #pragma unroll
-      for (int i = 8; i < kTile; i += 8)
+      for (int i = 16; i < kTile; i += 16)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) top[k] = max3_nan(top[k], s[i + 2 * k], s[i + 2 * k + 1]);
+        for (int k = 0; k < 8; ++k) top[k] = max3_nan(top[k], s[i + 2 * k], s[i + 2 * k + 1]);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) top[k] = max_nan(top[k], top[k + 4]);
       const float now = max3_nan(m, max_nan(top[0], top[1]), max_nan(top[2], top[3]));
       // a row that has seen nothing yet has an empty O: its first maximum rescales nothing
       const bool moves = !((now - m) * sc <= kSlack) && !(now == -INFINITY);
@@ -302,27 +333,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       const float shift = m == -INFINITY ? 0.f : -m * sc;
-      const float2 sc2 = make_float2(sc, sc), shift2 = make_float2(shift, shift);
-      float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll
-      for (int i = 0; i < kTile; i += 32) {
-        uint32_t pk[16];
-#pragma unroll
-        for (int k = 0; k < 16; ++k) {
-          const float2 x = fma2(make_float2(s[i + 2 * k], s[i + 2 * k + 1]), sc2, shift2);
-          float2 e;
-          if (k % 4 == 3 && !masked) {
-            e = exp2_poly2(x);
-          } else {
-            e.x = ex2_approx(x.x);
-            e.y = ex2_approx(x.y);
-          }
-          sum[k & 1] = add2(sum[k & 1], e);
-          pk[k] = pack<T>(e.x, e.y);
-        }
-        tmem_st16(t_s + i / 2, pk);
-      }
-      l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+      // a border's masked scores have weight 0, which the polynomial does not give
+      l += masked ? weights<T, 0>(s, sc, shift, t_s) : weights<T, kPoly>(s, sc, shift, t_s);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
