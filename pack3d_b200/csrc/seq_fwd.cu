@@ -3,14 +3,16 @@
 // A CTA has two tiles of 128 query rows that read the same keys: one place in a sequence for two heads of a group (where groups are
 // even: equal work and masks), else two neighbouring places of one head. Keys and values come in tiles of 128 through a
 // ring; S and O of both tiles are in tensor memory, P is written over its S. Two groups of four softmax warps (a row a thread)
-// take a tile each, one warp issues the products, one the copies.
+// take a tile each, two warps issue the products, one the copies.
 //
 // What bounds it: at dim 128 a tile of 128 x 128 costs the tensor pipe 1024 cycles and, at 16 exponentials a clock, the
 // special-function units as many, so a quarter of the exponentials go to the FMA pipe as polynomials; at dim 64 and below
-// the exponentials are the bound. The tiles take turns: while one's softmax runs, the pipe works for the other. S of the
-// next keys is issued when the product that reads P has completed, as it overwrites P and only products of one
-// accumulator are ordered among themselves; so a softmax warp that sees S also knows that O rests, and may rescale it. That it
-// does only where the row's maximum has grown by more than 2^8: weights up to 2^8 cost no precision.
+// the exponentials are the bound. What counts is that neither waits for the other: the softmax goes by 64 keys, and each tile has two
+// buffers of S (64 columns; P of 16 bits goes over its own S), so that S of the next 64 keys is made while the softmax works on
+// these (one buffer of 128 columns, S waiting for the product that reads P: 350 us for the figure below). S of 64 keys costs a
+// third more of the pipe than half of 128, as its operands come from shared memory.
+// O is rescaled only where a row's maximum has grown by more than 2^8 (weights up to 2^8 cost no precision), after the product before
+// has completed.
 //
 // Masks: key j counts for row i where j < seen(i); tiles of keys that some row does not see whole ("border" tiles, the last ones) are masked
 // by columns. A masked weight is 0, but 0 times an infinity or NaN of a value that the row does not see is NaN. So in border tiles the copying
@@ -28,8 +30,9 @@ namespace {
 
 __device__ unsigned g_seq_fwd_errors = 0;
 
-constexpr int kMmaWarp = 8, kCopyWarp = 9, kThreads = 320;
-constexpr uint32_t kColS = 0, kColO = 256;   // tensor memory: S of tile t at 128 t, O at 256 + 128 t
+constexpr int kMmaWarp = 8, kCopyWarp = 10, kThreads = 352;   // a warp of products for each tile
+constexpr int kKeys = 64;                    // of one softmax step
+constexpr uint32_t kColS = 0, kColO = 256;   // tensor memory: S of tile t at 128 t and 128 t + 64, O at 256 + 128 t
 constexpr float kSlack = 8.f;                // the maximum may lag by 2^8
 constexpr int kPoly = 2;                     // exponentials of eight that are polynomials
 
@@ -44,7 +47,7 @@ struct Layout {
 // one after needs. Border tiles, at most kBorders of them (the rows of a CTA see the same keys but for 255), are cleared ahead
 // of that order: each has a barrier of its own.
 constexpr int kBorders = 3;
-enum { kQFull, kSFull, kPFull = kSFull + 2, kODone = kPFull + 2, kClean = kODone + 2, kDrain = kClean + kBorders, kFull };
+enum { kQFull, kSFull, kPFull = kSFull + 4, kODone = kPFull + 2, kClean = kODone + 2, kDrain = kClean + kBorders, kFull = kDrain + 2 };
 template <int DP> constexpr int bars() { return kFull + 2 * Layout<DP>::kStages; }
 
 struct Params {
@@ -62,8 +65,8 @@ struct Params {
 struct Work {
   Range r;
   int row[2], head[2], kv;
-  int chunks[2];   // tiles of keys that each tile sees any of
-  int border;      // the first that some row does not see whole
+  int units[2];    // 64 keys that each tile sees any of
+  int border;      // the first tile of keys that some row does not see whole
 };
 __device__ __forceinline__ Work work_of(const Params &p) {
   const int slot = (int)(gridDim.x / p.units - 1 - blockIdx.x / p.units), unit = blockIdx.x % p.units;   // the longest first
@@ -77,24 +80,24 @@ __device__ __forceinline__ Work work_of(const Params &p) {
   for (int t = 0; t < 2; ++t) {
     w.head[t] = p.two_heads ? 2 * unit + t : unit;
     w.row[t] = s.group * per_slot + (p.two_heads ? 0 : t * kTile);
-    w.chunks[t] = 0;
+    w.units[t] = 0;
     if (s.group >= 0 && w.row[t] < w.r.nq) {
-      w.chunks[t] = (seen_by(w.r, min(w.row[t] + kTile, w.r.nq) - 1, p.a.causal) + kTile - 1) / kTile;
-      if (w.chunks[t]) w.border = min(w.border, seen_by(w.r, w.row[t], p.a.causal) / kTile);
+      w.units[t] = (seen_by(w.r, min(w.row[t] + kTile, w.r.nq) - 1, p.a.causal) + kKeys - 1) / kKeys;
+      if (w.units[t]) w.border = min(w.border, seen_by(w.r, w.row[t], p.a.causal) / kTile);
     }
   }
   w.kv = w.head[0] / group;
   return w;
 }
 
-// P = 2^(s sc + shift) of a row's 128 scores, rounded to T and written over them; returns the row's sum.  kPoly of every eight pairs are
+// P = 2^(s sc + shift) of a row's 64 scores, rounded to T and written over them; returns the row's sum.  kPoly of every eight pairs are
 // polynomials (scores are not NaN there: the row's maximum, and with it shift, would be).
 template <typename T, int kPoly>
-__device__ __forceinline__ float weights(const float (&s)[kTile], float sc, float shift, uint32_t t_s) {
+__device__ __forceinline__ float weights(const float (&s)[kKeys], float sc, float shift, uint32_t t_s) {
   const float2 sc2 = make_float2(sc, sc), shift2 = make_float2(shift, shift);
   float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-  for (int i = 0; i < kTile; i += 32) {
+  for (int i = 0; i < kKeys; i += 32) {
     uint32_t pk[16];
 #pragma unroll
     for (int k = 0; k < 16; ++k) {
@@ -127,7 +130,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ int not_finite;   // border tiles hold values that are not
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Work w = work_of(p);
-  const int chunks = max(w.chunks[0], w.chunks[1]);
+  const int units = max(w.units[0], w.units[1]), chunks = (units + 1) / 2;   // chunks: tiles of keys
   if (chunks == 0) {
     // rows that see no key, or none at all
     if (threadIdx.x < 256) {
@@ -149,7 +152,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto empty = [&](int s) { return bar(kFull + NS + s); };
   if (threadIdx.x == 0) {
     not_finite = 0;
-    for (int i = 0; i < bars<DP>(); ++i) mbar_init(bar(i), i == kPFull || i == kPFull + 1 ? 4 : 1);
+    for (int i = 0; i < bars<DP>(); ++i)
+      mbar_init(bar(i), i == kPFull || i == kPFull + 1 ? 4 : i >= kFull + NS ? 2 : 1);   // a stage is empty when both tiles are done with it
     fence_mbar_init();
   }
   if (warp == kMmaWarp) {
@@ -207,80 +211,84 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int i = max(0, issued - NS); i < issued; ++i)
         mbar_wait(full(i % NS), (i / NS) & 1, &g_seq_fwd_errors, kWaitNs, kErrTeardown);
     }
-  } else if (warp == kMmaWarp) {
-    // ------------------------------------------------------------------ products
-    // the whole warp runs this, with the same operands in every lane; one elected lane issues (30 cycles a product instead of 75)
-    {
-      const uint32_t idesc_s = idesc_f16(128, 128, std::is_same<T, __nv_bfloat16>::value, false);
-      const uint64_t desc_q = desc_rows(base), desc_k = desc_rows(ring), desc_v = desc_cols(ring);
-      int n_s[2] = {0, 0}, n_o[2] = {0, 0}, items = 0, landed = 0;
-      auto wait = [&](uint32_t b, uint32_t parity) { return wait_warp(b, parity, &g_seq_fwd_errors, kErrMma); };
-      // item i is there (and, for values of a border tile, cleared); items are waited for in order, once
-      auto wait_item = [&](int i) {
-        while (landed <= i) {
-          const int c = landed / 2;
-          if (!wait(full(landed % NS), (landed / NS) & 1)) return false;
-          if (landed % 2 && c >= w.border && !wait(bar(kClean + c - w.border), 0)) return false;
-          ++landed;
+  } else if (warp >= kMmaWarp) {
+    // ------------------------------------------------------------------ products, of one tile
+    // The whole warp runs this, with the same operands in every lane; one elected lane issues (30 cycles a product instead of 75). The
+    // pipe takes four products ahead and a wait costs 70 cycles even where there is nothing to wait for: with one warp for both
+    // tiles the pipe ran dry at each of them.
+    const int t = warp - kMmaWarp, mine = t ? w.units[1] : w.units[0];
+    const uint32_t idesc_s = idesc_f16(128, kKeys, std::is_same<T, __nv_bfloat16>::value, false);
+    const uint64_t desc_q = desc_rows(base + t * L::kTileBytes), desc_k = desc_rows(ring), desc_v = desc_cols(ring);
+    const uint32_t t_s = tmem + kColS + 128 * t, t_o = tmem + kColO + 128 * t;
+    int n_s = 0, n_o = 0, n_k = 0, n_v = 0, landed = 0;
+    auto wait = [&](uint32_t b, uint32_t parity) { return wait_warp(b, parity, &g_seq_fwd_errors, kErrMma); };
+    // item i is there (and, for values of a border tile, cleared); items are waited for in order, once
+    auto wait_item = [&](int i) {
+      while (landed <= i) {
+        const int c = landed / 2;
+        if (!wait(full(landed % NS), (landed / NS) & 1)) return false;
+        if (landed % 2 && c >= w.border && !wait(bar(kClean + c - w.border), 0)) return false;
+        ++landed;
+      }
+      return true;
+    };
+    auto issue_s = [&](int u) {
+      const uint64_t k = desc_k + (((uint32_t)(u / 2 * 2 % NS) * L::kTileBytes + (u & 1) * kKeys * 128) >> 4);
+#pragma unroll
+      for (int j = 0; j < DP / 16; ++j)
+        if (j < p.steps) mma_ss_warp(t_s + 64 * (u & 1), desc_q + step_rows(j), k + step_rows(j), idesc_s, j > 0);
+      mma_commit_warp(bar(kSFull + 2 * t + (u & 1)));
+      ++n_s;
+    };
+    auto issue_o = [&](int u) {
+      const uint64_t v = desc_v + ((uint32_t)((u / 2 * 2 + 1) % NS) * L::kTileBytes >> 4) + step_cols((u & 1) * (kKeys / 16));
+#pragma unroll
+      for (int j = 0; j < kKeys / 16; ++j)
+        mma_ts_warp(t_o, t_s + 64 * (u & 1) + 8 * j, v + step_cols(j), p.idesc_o, u > 0 || j > 0);
+      mma_commit_warp(bar(kODone + t));
+      ++n_o;
+    };
+    // A stage is given back after its second half's product, or the first half's where that is all; by both tiles, once it has landed
+    auto last_half = [&](int u) { return u & 1 || u == units - 1; };
+    bool ok = wait(bar(kQFull), 0) && wait_item(0);
+    if (ok) {
+      if (mine) issue_s(0);
+      if (last_half(0)) mma_commit_warp(empty(0)), ++n_k;
+    }
+    for (int u = 0; ok && u < units; ++u) {
+      if (u + 1 < units) {
+        ok = wait_item((u + 1) / 2 * 2);
+        if (ok && u + 1 < mine) {
+          ok = u == 0 || wait(bar(kODone + t), (u - 1) & 1);   // its buffer held P(u - 1)
+          if (ok) issue_s(u + 1);
         }
-        return true;
-      };
-      auto issue_s = [&](int t, int c) {
-        const uint64_t q = desc_q + (t * L::kTileBytes >> 4), k = desc_k + ((uint32_t)(2 * c % NS) * L::kTileBytes >> 4);
-        for (int j = 0; j < p.steps; ++j)
-          mma_ss_warp(tmem + kColS + 128 * t, q + step_rows(j), k + step_rows(j), idesc_s, j > 0);
-        mma_commit_warp(bar(kSFull + t));
-        ++n_s[t];
-      };
-      auto issue_o = [&](int t, int c) {
-        const uint64_t v = desc_v + ((uint32_t)((2 * c + 1) % NS) * L::kTileBytes >> 4);
-#pragma unroll
-        for (int j = 0; j < kTile / 16; ++j)
-          mma_ts_warp(tmem + kColO + 128 * t, tmem + kColS + 128 * t + 8 * j, v + step_cols(j), p.idesc_o, c > 0 || j > 0);
-        mma_commit_warp(bar(kODone + t));
-        ++n_o[t];
-      };
-      bool ok = wait(bar(kQFull), 0) && wait_item(0);
-      if (ok) {
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-          if (w.chunks[t]) issue_s(t, 0);
-        mma_commit_warp(empty(0));
-        items = 1;
+        if (ok && last_half(u + 1)) mma_commit_warp(empty((u + 1) / 2 * 2 % NS)), ++n_k;
       }
-      for (int c = 0; ok && c < chunks; ++c) {
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          if (!ok || c >= w.chunks[t]) continue;
-          ok = wait_item(2 * c + 1) && wait(bar(kPFull + t), c & 1);
-          if (!ok) continue;
-          issue_o(t, c);
-          if (c + 1 < w.chunks[t]) {
-            ok = wait_item(2 * c + 2) && wait(bar(kODone + t), c & 1);
-            if (ok) issue_s(t, c + 1);
-          }
-        }
-        if (!ok) break;
-        mma_commit_warp(empty((2 * c + 1) % NS));
-        if (c + 1 < chunks) mma_commit_warp(empty((2 * c + 2) % NS));
-        items += 1 + (c + 1 < chunks);
+      ok = ok && wait_item(u / 2 * 2 + 1);
+      if (ok && u < mine) {
+        ok = wait(bar(kPFull + t), u & 1);
+        if (ok) issue_o(u);
       }
-      // every product completed and every commit arrived before tensor memory and barriers are given up
-      mma_commit_warp(bar(kDrain));
-      mbar_wait(bar(kDrain), 0, &g_seq_fwd_errors, kWaitNs, kErrTeardown);
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        if (n_s[t]) mbar_wait(bar(kSFull + t), (n_s[t] - 1) & 1, &g_seq_fwd_errors, kWaitNs, kErrTeardown);
-        if (n_o[t]) mbar_wait(bar(kODone + t), (n_o[t] - 1) & 1, &g_seq_fwd_errors, kWaitNs, kErrTeardown);
-      }
-      for (int s = 0; s < NS; ++s) {
-        const int times = items / NS + (s < items % NS);
-        if (times) mbar_wait(empty(s), (times - 1) & 1, &g_seq_fwd_errors, kWaitNs, kErrTeardown);
-      }
+      if (ok && last_half(u)) mma_commit_warp(empty((u / 2 * 2 + 1) % NS)), ++n_v;
+    }
+    // every product completed and every commit arrived before tensor memory and barriers are given up
+    mma_commit_warp(bar(kDrain + t));
+    auto drained = [&](uint32_t b, int times) {
+      if (times > 0) mbar_wait(b, (times - 1) & 1, &g_seq_fwd_errors, kWaitNs, kErrTeardown);
+    };
+    drained(bar(kDrain + t), 1);
+    drained(bar(kSFull + 2 * t), (n_s + 1) / 2);
+    drained(bar(kSFull + 2 * t + 1), n_s / 2);
+    drained(bar(kODone + t), n_o);
+    // the stages' barriers complete when both tiles' warps have come this far; a warp that gave up leaves them to time out
+    for (int s = 0; s < NS; ++s) {
+      int times = 0;
+      for (int i = s; i < 2 * chunks; i += NS) times += i / 2 < (i % 2 ? n_v : n_k);
+      drained(empty(s), times);
     }
   } else {
     // ------------------------------------------------------------------ softmax, a row a thread
-    const int t = warp / 4, mine = t ? w.chunks[1] : w.chunks[0], head = t ? w.head[1] : w.head[0];
+    const int t = warp / 4, mine = t ? w.units[1] : w.units[0], head = t ? w.head[1] : w.head[0];
     const int row = (t ? w.row[1] : w.row[0]) + (warp % 4) * 32 + lane;
     const int seen = row < w.r.nq ? seen_by(w.r, row, p.a.causal) : 0;
     const uint32_t lanes = (uint32_t)((warp % 4) * 32) << 16;
@@ -288,61 +296,65 @@ __global__ void __launch_bounds__(kThreads, 1)
     const float sc = p.sc;
     float m = -INFINITY, l = 0.f;
     bool ok = true;
-    for (int c = 0; c < mine; ++c) {
-      ok = wait_warp(bar(kSFull + t), c & 1, &g_seq_fwd_errors, kErrSoftmax);
+    for (int u = 0; u < mine; ++u) {
+      const uint32_t t_u = t_s + 64 * (u & 1);
+      ok = wait_warp(bar(kSFull + 2 * t + (u & 1)), (u >> 1) & 1, &g_seq_fwd_errors, kErrSoftmax);
       if (!ok) break;
-      float s[kTile];
+      float s[kKeys];
 #pragma unroll
-      for (int i = 0; i < kTile; i += 32) tmem_ld32(t_s + i, reinterpret_cast<uint32_t *>(s) + i);
+      for (int i = 0; i < kKeys; i += 32) tmem_ld32(t_u + i, reinterpret_cast<uint32_t *>(s) + i);
       tmem_wait_ld();
-      const int limit = seen - c * kTile;
-      const bool masked = __any_sync(0xffffffffu, limit < kTile);
+      const int limit = seen - u * kKeys;
+      const bool masked = __any_sync(0xffffffffu, limit < kKeys);
       if (masked) {
 #pragma unroll
-        for (int i = 0; i < kTile; ++i) s[i] = i < limit ? s[i] : -INFINITY;
+        for (int i = 0; i < kKeys; ++i) s[i] = i < limit ? s[i] : -INFINITY;
       }
       float top[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) top[i] = max_nan(s[2 * i], s[2 * i + 1]);
 #pragma unroll
-      for (int i = 16; i < kTile; i += 16)
+      for (int i = 16; i < kKeys; i += 16)
 #pragma unroll
         for (int k = 0; k < 8; ++k) top[k] = max3_nan(top[k], s[i + 2 * k], s[i + 2 * k + 1]);
 #pragma unroll
       for (int k = 0; k < 4; ++k) top[k] = max_nan(top[k], top[k + 4]);
       const float now = max3_nan(m, max_nan(top[0], top[1]), max_nan(top[2], top[3]));
       // a row that has seen nothing yet has an empty O: its first maximum rescales nothing
-      const bool moves = !((now - m) * sc <= kSlack) && !(now == -INFINITY);
-      if (__any_sync(0xffffffffu, moves)) {
-        const float down = moves ? (m == -INFINITY ? 0.f : ex2_approx((m - now) * sc)) : 1.f;
-        if (moves) m = now;
-        l *= down;
-        if (c > 0) {
+      const bool moves = !((now - m) * sc <= kSlack) && !(now == -INFINITY), rescale = __any_sync(0xffffffffu, moves) && u > 0;
+      const float down = moves ? (m == -INFINITY ? 0.f : ex2_approx((m - now) * sc)) : 1.f;
+      if (moves) m = now;
+      l *= down;
+      const float shift = m == -INFINITY ? 0.f : -m * sc;
+      // a border's masked scores have weight 0, which the polynomial does not give
+      l += masked ? weights<T, 0>(s, sc, shift, t_u) : weights<T, kPoly>(s, sc, shift, t_u);
+      // O rests once the product before has completed (waited for at every step, so that the parity is exact)
+      if (u > 0) {
+        ok = wait_warp(bar(kODone + t), (u - 1) & 1, &g_seq_fwd_errors, kErrSoftmax);
+        if (!ok) break;
+      }
+      if (rescale) {
 #pragma unroll
-          for (int i = 0; i < DP; i += 32) {
-            if (i < p.a.dim) {
-              uint32_t o[32];
-              tmem_ld32(t_o + i, o);
-              tmem_wait_ld();
+        for (int i = 0; i < DP; i += 32) {
+          if (i < p.a.dim) {
+            uint32_t o[32];
+            tmem_ld32(t_o + i, o);
+            tmem_wait_ld();
 #pragma unroll
-              for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * down);
-              tmem_st16(t_o + i, o);
-              tmem_st16(t_o + i + 16, o + 16);
-            }
+            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * down);
+            tmem_st16(t_o + i, o);
+            tmem_st16(t_o + i + 16, o + 16);
           }
         }
       }
-      const float shift = m == -INFINITY ? 0.f : -m * sc;
-      // a border's masked scores have weight 0, which the polynomial does not give
-      l += masked ? weights<T, 0>(s, sc, shift, t_s) : weights<T, kPoly>(s, sc, shift, t_s);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(kPFull + t));
     }
     if (ok && mine) ok = wait_warp(bar(kODone + t), (mine - 1) & 1, &g_seq_fwd_errors, kErrSoftmax);
-    if (ok && mine > w.border)   // for what the copying warp says of the values
-      ok = wait_warp(bar(kClean + mine - 1 - w.border), 0, &g_seq_fwd_errors, kErrSoftmax);
+    if (ok && (mine + 1) / 2 > w.border)   // for what the copying warp says of the values
+      ok = wait_warp(bar(kClean + (mine + 1) / 2 - 1 - w.border), 0, &g_seq_fwd_errors, kErrSoftmax);
     if (ok) {
       const float inv = seen > 0 ? 1.f / l : 0.f;
       const int64_t at = (int64_t)(w.r.q0 + row) * p.a.heads + head;
