@@ -227,7 +227,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint64_t v = d_v + ((uint32_t)(c % L::kV) * TB >> 4);
         for (int j = 0; j < p.steps; ++j) mma_ss_warp(t_dp, d_do + step_rows(j), v + step_rows(j), idesc_s, j > 0);
         mma_commit_warp(bar(kDPFull));
-        mma_commit_warp(bar(kVEmpty + c % L::kV));
         ++n_dp;
       };
       bool ok = wait(kQFull, 0) && wait(kKFull, 0);
@@ -239,7 +238,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int c = 0; ok && c < chunks; ++c) {
         if (c + 1 < chunks) {
           // the buffer of S(c + 1) held dS(c - 1)
-          ok = wait(kKFull + (c + 1) % L::kK, ((c + 1) / L::kK) & 1) && (c == 0 || wait(kDQDone, (c - 1) & 1));
+          ok = c == 0 || wait(kDQDone, (c - 1) & 1);
+          if (!ok) break;
+          // keys whose dQ is there may go; by a plain arrival, as a second commit would wait until the pipe has run dry
+          if (c > 0 && lane == 0) mbar_arrive(bar(kKEmpty + (c - 1) % L::kK));
+          ok = wait(kKFull + (c + 1) % L::kK, ((c + 1) / L::kK) & 1);
           if (!ok) break;
           issue_s(c + 1);
           ok = wait(kVFull + (c + 1) % L::kV, ((c + 1) / L::kV) & 1) && wait(kDPFree, c & 1);
@@ -253,7 +256,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int j = 0; j < kTile / 16; ++j)   // each softmax group's dS lies over its own half of S
           mma_ts_warp(t_dq, tmem + 128 * (c & 1) + j / 4 * 64 + j % 4 * 8, k + step_cols(j), p.idesc_out, c > 0 || j > 0);
         mma_commit_warp(bar(kDQDone));
-        mma_commit_warp(bar(kKEmpty + c % L::kK));
         ++n_dq;
       }
       if (ok) {
@@ -271,8 +273,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       drained(kDQDone, n_dq);
       drained(kDone, done);
       for (int i = 0; i < n_seen; ++i) drained(kSeen + i, 1);
-      for (int s = 0; s < L::kK; ++s) drained(kKEmpty + s, n_dq / L::kK + (s < n_dq % L::kK));
-      for (int s = 0; s < L::kV; ++s) drained(kVEmpty + s, n_dp / L::kV + (s < n_dp % L::kV));
     }
   } else {
     const int half = warp / 4, row = row0 + (warp % 4) * 32 + lane;
@@ -301,7 +301,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       tmem_wait_ld();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(bar(kDPFree));
+      if (lane == 0) {
+        mbar_arrive(bar(kDPFree));
+        if (warp == 0) mbar_arrive(bar(kVEmpty + c % L::kV));   // dP is complete: its values may go
+      }
 #pragma unroll
       for (int i = 0; i < 32; ++i) {
         const float2 v = mul2(make_float2(s[2 * i], s[2 * i + 1]), fma2(make_float2(d[2 * i], d[2 * i + 1]), scale, minus));
@@ -541,11 +544,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
         sum(t_dk, t_dp, d_ringc + stage(i), i > 0);
         mma_commit_warp(bar(kDKDone));
-        mma_commit_warp(empty(i % NS));
         ++n_dk;
         if (i + 1 < steps) {
           ok = wait(bar(kDKDone), i & 1);
           if (!ok) break;
+          if (lane == 0) mbar_arrive(empty(i % NS));   // a plain arrival: a second commit would wait until the pipe has run dry
           issue_dp(i + 1);
         }
       }
@@ -564,7 +567,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       drained(bar(kDKDone), n_dk);
       drained(bar(kSeenKV), n_seen);
       drained(bar(kAllDone), done);
-      for (int s = 0; s < NS; ++s) drained(empty(s), n_dk / NS + (s < n_dk % NS));
     }
   } else {
     const int half = warp / 4;

@@ -220,7 +220,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t idesc_s = idesc_f16(128, kKeys, std::is_same<T, __nv_bfloat16>::value, false);
     const uint64_t desc_q = desc_rows(base + t * L::kTileBytes), desc_k = desc_rows(ring), desc_v = desc_cols(ring);
     const uint32_t t_s = tmem + kColS + 128 * t, t_o = tmem + kColO + 128 * t;
-    int n_s = 0, n_o = 0, n_k = 0, n_v = 0, landed = 0;
+    int n_s = 0, n_o = 0, landed = 0;
     auto wait = [&](uint32_t b, uint32_t parity) { return wait_warp(b, parity, &g_seq_fwd_errors, kErrMma); };
     // item i is there (and, for values of a border tile, cleared); items are waited for in order, once
     auto wait_item = [&](int i) {
@@ -248,28 +248,28 @@ __global__ void __launch_bounds__(kThreads, 1)
       mma_commit_warp(bar(kODone + t));
       ++n_o;
     };
-    // A stage is given back after its second half's product, or the first half's where that is all; by both tiles, once it has landed
-    auto last_half = [&](int u) { return u & 1 || u == units - 1; };
     bool ok = wait(bar(kQFull), 0) && wait_item(0);
-    if (ok) {
-      if (mine) issue_s(0);
-      if (last_half(0)) mma_commit_warp(empty(0)), ++n_k;
-    }
+    if (ok && mine) issue_s(0);
     for (int u = 0; ok && u < units; ++u) {
-      if (u + 1 < units) {
-        ok = wait_item((u + 1) / 2 * 2);
-        if (ok && u + 1 < mine) {
-          ok = u == 0 || wait(bar(kODone + t), (u - 1) & 1);   // its buffer held P(u - 1)
-          if (ok) issue_s(u + 1);
+      if (u > 0) {
+        // O(u - 1) is there, and with it S(u - 1): their keys and values may go. By a plain arrival: a commit after another one's
+        // waits until the pipe has run dry. A tile that is done, or has no rows, arrives for what has landed.
+        ok = u - 1 < mine ? wait(bar(kODone + t), (u - 1) & 1) : wait_item((u - 1) / 2 * 2 + 1);
+        if (!ok) break;
+        if ((u & 1) == 0 && lane == 0) {
+          mbar_arrive(empty((u - 2) % NS));
+          mbar_arrive(empty((u - 1) % NS));
         }
-        if (ok && last_half(u + 1)) mma_commit_warp(empty((u + 1) / 2 * 2 % NS)), ++n_k;
       }
-      ok = ok && wait_item(u / 2 * 2 + 1);
-      if (ok && u < mine) {
-        ok = wait(bar(kPFull + t), u & 1);
+      if (u + 1 < mine) {   // into the buffer that held P(u - 1)
+        ok = wait_item((u + 1) / 2 * 2);
+        if (!ok) break;
+        issue_s(u + 1);
+      }
+      if (u < mine) {
+        ok = wait_item(u / 2 * 2 + 1) && wait(bar(kPFull + t), u & 1);
         if (ok) issue_o(u);
       }
-      if (ok && last_half(u)) mma_commit_warp(empty((u / 2 * 2 + 1) % NS)), ++n_v;
     }
     // every product completed and every commit arrived before tensor memory and barriers are given up
     mma_commit_warp(bar(kDrain + t));
@@ -280,12 +280,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     drained(bar(kSFull + 2 * t), (n_s + 1) / 2);
     drained(bar(kSFull + 2 * t + 1), n_s / 2);
     drained(bar(kODone + t), n_o);
-    // the stages' barriers complete when both tiles' warps have come this far; a warp that gave up leaves them to time out
-    for (int s = 0; s < NS; ++s) {
-      int times = 0;
-      for (int i = s; i < 2 * chunks; i += NS) times += i / 2 < (i % 2 ? n_v : n_k);
-      drained(empty(s), times);
-    }
   } else {
     // ------------------------------------------------------------------ softmax, a row a thread
     const int t = warp / 4, mine = t ? w.units[1] : w.units[0], head = t ? w.head[1] : w.head[0];
