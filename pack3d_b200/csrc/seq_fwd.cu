@@ -14,6 +14,10 @@
 // O is rescaled only where a row's maximum has grown by more than 2^8 (weights up to 2^8 cost no precision), after the product before
 // has completed.
 //
+// A CTA goes through several such pairs (two thousand keys take 12 us, and setting a CTA up and taking it down 6): the next pair's
+// queries, keys and first S come while this one's softmax ends and O is written. Pairs are launched the longest first and taken
+// over as CTAs get done. All waits go by counts that run on over the pairs.
+//
 // Masks: key j counts for row i where j < seen(i); tiles of keys that some row does not see whole ("border" tiles, the last ones) are masked
 // by columns. A masked weight is 0, but 0 times an infinity or NaN of a value that the row does not see is NaN. So in border tiles the copying
 // warp, which has nothing else to do by then, sets values that are not finite to 0 before the product, and the epilogue adds them back
@@ -44,10 +48,11 @@ struct Layout {
 };
 
 // Every wait on a barrier that completes more than once is by someone who has seen the completion before, and whose own next step the
-// one after needs. Border tiles, at most kBorders of them (the rows of a CTA see the same keys but for 255), are cleared ahead
-// of that order: each has a barrier of its own.
+// one after needs. Border tiles, at most kBorders of them (the rows of a pair see the same keys but for 255), are cleared ahead of
+// that order: each has a barrier of its own, and the next pair's are cleared only once both products' warps have passed these.
 constexpr int kBorders = 3;
-enum { kQFull, kSFull, kPFull = kSFull + 4, kODone = kPFull + 2, kClean = kODone + 2, kDrain = kClean + kBorders, kFull = kDrain + 2 };
+enum { kQFull, kQEmpty, kSFull, kPFull = kSFull + 4, kODone = kPFull + 2, kNext = kODone + 2, kClean = kNext + 2, kDrain = kClean + kBorders,
+       kFull = kDrain + 2 };
 template <int DP> constexpr int bars() { return kFull + 2 * Layout<DP>::kStages; }
 
 struct Params {
@@ -57,25 +62,28 @@ struct Params {
   int units;       // of heads: pairs, or single ones
   int two_heads;   // a CTA's tiles are two heads
   int steps;       // of 16 columns
+  int works;       // pairs of tiles
   uint32_t idesc_o;
   float sc;        // scale * log2(e)
 };
 
-// What a CTA does: rows i0 (+ 128 for the second tile where the tiles are of one head) of sequence `r`.
+// A pair of tiles: rows i0 (+ 128 for the second tile where the tiles are of one head) of sequence `r`.
 struct Work {
   Range r;
   int row[2], head[2], kv;
   int units[2];    // 64 keys that each tile sees any of
   int border;      // the first tile of keys that some row does not see whole
+  __device__ __forceinline__ int most() const { return max(units[0], units[1]); }
+  __device__ __forceinline__ int chunks() const { return (most() + 1) / 2; }   // tiles of keys
 };
-__device__ __forceinline__ Work work_of(const Params &p) {
-  const int slot = (int)(gridDim.x / p.units - 1 - blockIdx.x / p.units), unit = blockIdx.x % p.units;   // the longest first
+__device__ __forceinline__ Work work_of(const Params &p, int index) {
+  const int slot = p.works / p.units - 1 - index / p.units, unit = index % p.units;   // the longest first
   const int per_slot = p.two_heads ? kTile : 2 * kTile;
   const Slot s = find_slot(p.a.q_offsets, p.a.sequences, (int)p.a.q_rows, per_slot, slot);
   Work w;
   w.r = slot_range(p.a, s.sequence);
   const int group = p.a.heads / p.a.kv_heads;
-  w.border = 1 << 30;
+  w.border = 1 << 28;   // beyond any tile
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
     w.head[t] = p.two_heads ? 2 * unit + t : unit;
@@ -127,23 +135,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t bar_mem[bars<DP>()];
   __shared__ uint32_t tmem_holder;
-  __shared__ int not_finite;   // border tiles hold values that are not
+  __shared__ int not_finite[2];   // border tiles of a pair (by its number's last bit) hold values that are not
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const Work w = work_of(p);
-  const int units = max(w.units[0], w.units[1]), chunks = (units + 1) / 2;   // chunks: tiles of keys
-  if (chunks == 0) {
-    // rows that see no key, or none at all
-    if (threadIdx.x < 256) {
-      const int t = threadIdx.x / 128, row = w.row[t] + threadIdx.x % 128;
-      if (w.row[t] >= 0 && row < w.r.nq) {
-        const int64_t at = (int64_t)(w.r.q0 + row) * p.a.heads + w.head[t];
-        uint4 *out = reinterpret_cast<uint4 *>(static_cast<T *>(p.out) + at * p.a.dim);
-        for (int i = 0; i < p.a.dim / 8; ++i) out[i] = make_uint4(0, 0, 0, 0);
-        if (p.lse) p.lse[(int64_t)w.head[t] * p.a.q_rows + w.r.q0 + row] = -INFINITY;
-      }
-    }
-    return;
-  }
+  __shared__ __align__(16) uint4 answer[2];
+  Work w = work_of(p, blockIdx.x);
   const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
   uint8_t *const smem = smem_raw + (base - raw);
   const uint32_t ring = base + 2 * L::kTileBytes;
@@ -151,9 +146,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto full = [&](int s) { return bar(kFull + s); };
   auto empty = [&](int s) { return bar(kFull + NS + s); };
   if (threadIdx.x == 0) {
-    not_finite = 0;
+    not_finite[0] = not_finite[1] = 0;
     for (int i = 0; i < bars<DP>(); ++i)
-      mbar_init(bar(i), i == kPFull || i == kPFull + 1 ? 4 : i >= kFull + NS ? 2 : 1);   // a stage is empty when both tiles are done with it
+      mbar_init(bar(i), i == kQEmpty ? 10 : i == kPFull || i == kPFull + 1 ? 4 : i >= kFull + NS ? 2 : 1);
     fence_mbar_init();
   }
   if (warp == kMmaWarp) {
@@ -170,44 +165,69 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = tmem_holder;
 
+  int done = 0;   // pairs before this one
+  // The number of the pair after this one, or -1 (asked for by the copying warp when it began this one): by whole warps.
+  auto next_work = [&](unsigned role) {
+    if (!wait_warp(bar(kNext + (done & 1)), (done >> 1) & 1, &g_seq_fwd_errors, role)) return -1;
+    const int index = work_given(smem_u32(&answer[done & 1]));
+    fence_proxy_async_smem();   // read before the next answer is written there
+    return index;
+  };
   if (warp == kCopyWarp) {
-    // ------------------------------------------------------------------ copies; items K0, V0, K1, V1, ..
+    // ------------------------------------------------------------------ copies; items K0, V0, K1, V1, .. of one pair after another
     bool ok = true;
-    int issued = 0;
-    if (lane == 0) {
-      mbar_expect_tx(bar(kQFull), 2 * L::kTileBytes);
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-        for (int c = 0; c < DP / 64; ++c)
-          tma_load_3d(base + t * L::kTileBytes + c * kBox, &tq, bar(kQFull), 64 * c, w.head[t], w.r.q0 + w.row[t]);
-      for (int i = 0; i < 2 * chunks; ++i) {
-        const int s = i % NS;
-        if (i >= NS && !mbar_wait(empty(s), (i / NS - 1) & 1, &g_seq_fwd_errors, kWaitNs, kErrProducer)) {
-          ok = false;
-          break;
-        }
-        mbar_expect_tx(full(s), L::kTileBytes);
-        for (int c = 0; c < DP / 64; ++c)
-          tma_load_3d(ring + s * L::kTileBytes + c * kBox, i % 2 ? &tv : &tk, full(s), 64 * c, w.kv, w.r.k0 + i / 2 * kTile);
-        issued = i + 1;
-      }
-    }
-    ok = __all_sync(0xffffffffu, ok);
-    // values of the border tiles that are not finite
-    for (int c = min(w.border, chunks); ok && c < chunks; ++c) {
-      const int i = 2 * c + 1, s = i % NS;
-      ok = __all_sync(0xffffffffu, mbar_wait(full(s), (i / NS) & 1, &g_seq_fwd_errors, kWaitNs, kErrProducer));
+    int item0 = 0, issued = 0;
+    for (int index = blockIdx.x; index >= 0;) {
+      const Work now = w;
+      const int chunks = now.chunks();
+      // the last pair's queries have had their last product and its clearing has been seen; the pair before it is written
+      if (done) ok = __all_sync(0xffffffffu, mbar_wait(bar(kQEmpty), (done - 1) & 1, &g_seq_fwd_errors, kWaitNs, kErrProducer));
       if (!ok) break;
-      if (clear_not_finite<T>(smem + (2 + s) * L::kTileBytes, L::kTileBytes)) {
-        fence_proxy_async_smem();
-        if (lane == 0) not_finite = 1;
+      if (lane == 0) {
+        ask_for_work(smem_u32(&answer[done & 1]), bar(kNext + (done & 1)));
+        not_finite[done & 1] = 0;
+        if (chunks) mbar_expect_tx(bar(kQFull), 2 * L::kTileBytes);
+        else mbar_arrive(bar(kQFull));
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          for (int c = 0; chunks && c < DP / 64; ++c)
+            tma_load_3d(base + t * L::kTileBytes + c * kBox, &tq, bar(kQFull), 64 * c, now.head[t], now.r.q0 + now.row[t]);
+        for (int i = item0; i < item0 + 2 * chunks; ++i) {
+          const int s = i % NS, c = (i - item0) / 2;
+          if (i >= NS && !mbar_wait(empty(s), (i / NS - 1) & 1, &g_seq_fwd_errors, kWaitNs, kErrProducer)) {
+            ok = false;
+            break;
+          }
+          mbar_expect_tx(full(s), L::kTileBytes);
+          for (int k = 0; k < DP / 64; ++k)
+            tma_load_3d(ring + s * L::kTileBytes + k * kBox, (i - item0) % 2 ? &tv : &tk, full(s), 64 * k, now.kv, now.r.k0 + c * kTile);
+          issued = i + 1;
+        }
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(kClean + c - w.border));
+      ok = __all_sync(0xffffffffu, ok);
+      // values of the border tiles that are not finite
+#pragma unroll
+      for (int b = 0; b < kBorders; ++b) {
+        const int c = now.border + b, i = item0 + 2 * c + 1, s = i % NS;
+        if (!ok || c >= chunks) continue;
+        ok = __all_sync(0xffffffffu, mbar_wait(full(s), (i / NS) & 1, &g_seq_fwd_errors, kWaitNs, kErrProducer));
+        if (!ok) continue;
+        if (clear_not_finite<T>(smem + (2 + s) * L::kTileBytes, L::kTileBytes)) {
+          fence_proxy_async_smem();
+          if (lane == 0) not_finite[done & 1] = 1;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(kClean + b));
+      }
+      item0 += 2 * chunks;
+      index = next_work(kErrProducer);
+      ++done;
+      if (!ok) break;
+      if (index >= 0) w = work_of(p, index);
     }
     // no copy in flight into memory that is about to be given up
     if (lane == 0) {
-      mbar_wait(bar(kQFull), 0, &g_seq_fwd_errors, kWaitNs, kErrTeardown);
+      if (done) mbar_wait(bar(kQFull), (done - 1) & 1, &g_seq_fwd_errors, kWaitNs, kErrTeardown);
       for (int i = max(0, issued - NS); i < issued; ++i)
         mbar_wait(full(i % NS), (i / NS) & 1, &g_seq_fwd_errors, kWaitNs, kErrTeardown);
     }
@@ -216,60 +236,84 @@ __global__ void __launch_bounds__(kThreads, 1)
     // The whole warp runs this, with the same operands in every lane; one elected lane issues (30 cycles a product instead of 75). The
     // pipe takes four products ahead and a wait costs 70 cycles even where there is nothing to wait for: with one warp for both
     // tiles the pipe ran dry at each of them.
-    const int t = warp - kMmaWarp, mine = t ? w.units[1] : w.units[0];
+    const int t = warp - kMmaWarp;
     const uint32_t idesc_s = idesc_f16(128, kKeys, std::is_same<T, __nv_bfloat16>::value, false);
     const uint64_t desc_q = desc_rows(base + t * L::kTileBytes), desc_k = desc_rows(ring), desc_v = desc_cols(ring);
     const uint32_t t_s = tmem + kColS + 128 * t, t_o = tmem + kColO + 128 * t;
-    int n_s = 0, n_o = 0, landed = 0;
+    int n_s = 0, n_o = 0;                  // products of this tile so far
+    int item0 = 0, landed = 0, cleared[kBorders] = {};
+    int give_back = -1;                    // the items whose last readers are under way: this one and the next
+    bool waited = true;                    // the last O has been waited for
     auto wait = [&](uint32_t b, uint32_t parity) { return wait_warp(b, parity, &g_seq_fwd_errors, kErrMma); };
-    // item i is there (and, for values of a border tile, cleared); items are waited for in order, once
-    auto wait_item = [&](int i) {
-      while (landed <= i) {
-        const int c = landed / 2;
-        if (!wait(full(landed % NS), (landed / NS) & 1)) return false;
-        if (landed % 2 && c >= w.border && !wait(bar(kClean + c - w.border), 0)) return false;
-        ++landed;
-      }
-      return true;
-    };
-    auto issue_s = [&](int u) {
-      const uint64_t k = desc_k + (((uint32_t)(u / 2 * 2 % NS) * L::kTileBytes + (u & 1) * kKeys * 128) >> 4);
-#pragma unroll
-      for (int j = 0; j < DP / 16; ++j)
-        if (j < p.steps) mma_ss_warp(t_s + 64 * (u & 1), desc_q + step_rows(j), k + step_rows(j), idesc_s, j > 0);
-      mma_commit_warp(bar(kSFull + 2 * t + (u & 1)));
-      ++n_s;
-    };
-    auto issue_o = [&](int u) {
-      const uint64_t v = desc_v + ((uint32_t)((u / 2 * 2 + 1) % NS) * L::kTileBytes >> 4) + step_cols((u & 1) * (kKeys / 16));
-#pragma unroll
-      for (int j = 0; j < kKeys / 16; ++j)
-        mma_ts_warp(t_o, t_s + 64 * (u & 1) + 8 * j, v + step_cols(j), p.idesc_o, u > 0 || j > 0);
-      mma_commit_warp(bar(kODone + t));
-      ++n_o;
-    };
-    bool ok = wait(bar(kQFull), 0) && wait_item(0);
-    if (ok && mine) issue_s(0);
-    for (int u = 0; ok && u < units; ++u) {
-      if (u > 0) {
-        // O(u - 1) is there, and with it S(u - 1): their keys and values may go. By a plain arrival: a commit after another one's
-        // waits until the pipe has run dry. A tile that is done, or has no rows, arrives for what has landed.
-        ok = u - 1 < mine ? wait(bar(kODone + t), (u - 1) & 1) : wait_item((u - 1) / 2 * 2 + 1);
-        if (!ok) break;
-        if ((u & 1) == 0 && lane == 0) {
-          mbar_arrive(empty((u - 2) % NS));
-          mbar_arrive(empty((u - 1) % NS));
+    bool ok = true;
+    for (int index = blockIdx.x; index >= 0;) {
+      const Work now = w;
+      const int units = now.most(), mine = t ? now.units[1] : now.units[0], chunks = now.chunks();
+      // item i is there (and, for values of a border tile, cleared); items are waited for in order, once
+      auto wait_item = [&](int i) {
+        for (; landed <= i; ++landed) {
+          if (!wait(full(landed % NS), (landed / NS) & 1)) return false;
+          const int b = (landed - item0) / 2 - now.border;
+          if ((landed - item0) % 2 && b >= 0) {
+            const int phase = b == 0 ? cleared[0] : b == 1 ? cleared[1] : cleared[2];
+            if (!wait(bar(kClean + b), phase & 1)) return false;
+          }
         }
-      }
-      if (u + 1 < mine) {   // into the buffer that held P(u - 1)
-        ok = wait_item((u + 1) / 2 * 2);
+        return true;
+      };
+      // S of unit u: into the buffer that S two before was in
+      auto issue_s = [&](int u) {
+        const uint64_t k = desc_k + (((uint32_t)((item0 + u / 2 * 2) % NS) * L::kTileBytes + (u & 1) * kKeys * 128) >> 4);
+#pragma unroll
+        for (int j = 0; j < DP / 16; ++j)
+          if (j < p.steps) mma_ss_warp(t_s + 64 * (n_s & 1), desc_q + step_rows(j), k + step_rows(j), idesc_s, j > 0);
+        mma_commit_warp(bar(kSFull + 2 * t + (n_s & 1)));
+        ++n_s;
+      };
+      auto issue_o = [&](int u) {
+        const uint64_t v = desc_v + ((uint32_t)((item0 + u / 2 * 2 + 1) % NS) * L::kTileBytes >> 4) + step_cols((u & 1) * (kKeys / 16));
+#pragma unroll
+        for (int j = 0; j < kKeys / 16; ++j)
+          mma_ts_warp(t_o, t_s + 64 * (n_o & 1) + 8 * j, v + step_cols(j), p.idesc_o, u > 0 || j > 0);
+        mma_commit_warp(bar(kODone + t));
+        ++n_o;
+        waited = false;
+      };
+      ok = wait(bar(kQFull), done & 1) && (!units || wait_item(item0));
+      if (ok && mine) issue_s(0);
+      index = next_work(kErrMma);
+      if (index >= 0) w = work_of(p, index);
+      for (int u = 0; ok && u < units; ++u) {
+        // The last O is there, and with it its S: their keys and values may go. By a plain arrival: a commit after another one's
+        // waits until the pipe has run dry. A tile that is done, or has no rows, arrives for what has landed.
+        if (!waited) ok = wait(bar(kODone + t), (n_o - 1) & 1);
+        waited = true;
         if (!ok) break;
-        issue_s(u + 1);
+        if (give_back >= 0 && lane == 0) {
+          mbar_arrive(empty(give_back % NS));
+          mbar_arrive(empty((give_back + 1) % NS));
+        }
+        give_back = -1;
+        if (u + 1 < mine) {
+          ok = wait_item(item0 + (u + 1) / 2 * 2);
+          if (!ok) break;
+          issue_s(u + 1);
+        }
+        ok = wait_item(item0 + u / 2 * 2 + 1);
+        if (!ok) break;
+        if (u < mine) {
+          ok = wait(bar(kPFull + t), n_o & 1);
+          if (!ok) break;
+          issue_o(u);
+        }
+        if (u & 1 || u == units - 1) give_back = item0 + u / 2 * 2;
       }
-      if (u < mine) {
-        ok = wait_item(u / 2 * 2 + 1) && wait(bar(kPFull + t), u & 1);
-        if (ok) issue_o(u);
-      }
+      if (!ok) break;
+      if (lane == 0) mbar_arrive(bar(kQEmpty));
+#pragma unroll
+      for (int b = 0; b < kBorders; ++b) cleared[b] += now.border + b < chunks;
+      item0 += 2 * chunks;
+      ++done;
     }
     // every product completed and every commit arrived before tensor memory and barriers are given up
     mma_commit_warp(bar(kDrain + t));
@@ -282,78 +326,96 @@ __global__ void __launch_bounds__(kThreads, 1)
     drained(bar(kODone + t), n_o);
   } else {
     // ------------------------------------------------------------------ softmax, a row a thread
-    const int t = warp / 4, mine = t ? w.units[1] : w.units[0], head = t ? w.head[1] : w.head[0];
-    const int row = (t ? w.row[1] : w.row[0]) + (warp % 4) * 32 + lane;
-    const int seen = row < w.r.nq ? seen_by(w.r, row, p.a.causal) : 0;
+    const int t = warp / 4;
     const uint32_t lanes = (uint32_t)((warp % 4) * 32) << 16;
     const uint32_t t_s = tmem + kColS + 128 * t + lanes, t_o = tmem + kColO + 128 * t + lanes;
     const float sc = p.sc;
-    float m = -INFINITY, l = 0.f;
+    int n = 0;   // steps of this tile so far
     bool ok = true;
-    for (int u = 0; u < mine; ++u) {
-      const uint32_t t_u = t_s + 64 * (u & 1);
-      ok = wait_warp(bar(kSFull + 2 * t + (u & 1)), (u >> 1) & 1, &g_seq_fwd_errors, kErrSoftmax);
+    for (int index = blockIdx.x; index >= 0;) {
+      const Work now = w;
+      const int mine = t ? now.units[1] : now.units[0], head = t ? now.head[1] : now.head[0], row0 = t ? now.row[1] : now.row[0];
+      const int row = row0 + (warp % 4) * 32 + lane;
+      const bool there = row0 >= 0 && row < now.r.nq;
+      const int seen = there ? seen_by(now.r, row, p.a.causal) : 0;
+      // The pair before is written. After the wait for this one's queries, which come only when every warp has said so for the
+      // pair before: no warp, with rows or without, is a pair ahead.
+      ok = wait_warp(bar(kQFull), done & 1, &g_seq_fwd_errors, kErrSoftmax);
       if (!ok) break;
-      float s[kKeys];
-#pragma unroll
-      for (int i = 0; i < kKeys; i += 32) tmem_ld32(t_u + i, reinterpret_cast<uint32_t *>(s) + i);
-      tmem_wait_ld();
-      const int limit = seen - u * kKeys;
-      const bool masked = __any_sync(0xffffffffu, limit < kKeys);
-      if (masked) {
-#pragma unroll
-        for (int i = 0; i < kKeys; ++i) s[i] = i < limit ? s[i] : -INFINITY;
-      }
-      float top[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) top[i] = max_nan(s[2 * i], s[2 * i + 1]);
-#pragma unroll
-      for (int i = 16; i < kKeys; i += 16)
-#pragma unroll
-        for (int k = 0; k < 8; ++k) top[k] = max3_nan(top[k], s[i + 2 * k], s[i + 2 * k + 1]);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) top[k] = max_nan(top[k], top[k + 4]);
-      const float now = max3_nan(m, max_nan(top[0], top[1]), max_nan(top[2], top[3]));
-      // a row that has seen nothing yet has an empty O: its first maximum rescales nothing
-      const bool moves = !((now - m) * sc <= kSlack) && !(now == -INFINITY), rescale = __any_sync(0xffffffffu, moves) && u > 0;
-      const float down = moves ? (m == -INFINITY ? 0.f : ex2_approx((m - now) * sc)) : 1.f;
-      if (moves) m = now;
-      l *= down;
-      const float shift = m == -INFINITY ? 0.f : -m * sc;
-      // a border's masked scores have weight 0, which the polynomial does not give
-      l += masked ? weights<T, 0>(s, sc, shift, t_u) : weights<T, kPoly>(s, sc, shift, t_u);
-      // O rests once the product before has completed (waited for at every step, so that the parity is exact)
-      if (u > 0) {
-        ok = wait_warp(bar(kODone + t), (u - 1) & 1, &g_seq_fwd_errors, kErrSoftmax);
+      if (lane == 0) mbar_arrive(bar(kQEmpty));
+      index = next_work(kErrSoftmax);
+      if (index >= 0) w = work_of(p, index);
+      float m = -INFINITY, l = 0.f;
+      for (int u = 0; u < mine; ++u, ++n) {
+        const uint32_t t_u = t_s + 64 * (n & 1);
+        ok = wait_warp(bar(kSFull + 2 * t + (n & 1)), (n >> 1) & 1, &g_seq_fwd_errors, kErrSoftmax);
         if (!ok) break;
-      }
-      if (rescale) {
+        float s[kKeys];
 #pragma unroll
-        for (int i = 0; i < DP; i += 32) {
-          if (i < p.a.dim) {
-            uint32_t o[32];
-            tmem_ld32(t_o + i, o);
-            tmem_wait_ld();
+        for (int i = 0; i < kKeys; i += 32) tmem_ld32(t_u + i, reinterpret_cast<uint32_t *>(s) + i);
+        tmem_wait_ld();
+        const int limit = seen - u * kKeys;
+        const bool masked = __any_sync(0xffffffffu, limit < kKeys);
+        if (masked) {
 #pragma unroll
-            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * down);
-            tmem_st16(t_o + i, o);
-            tmem_st16(t_o + i + 16, o + 16);
+          for (int i = 0; i < kKeys; ++i) s[i] = i < limit ? s[i] : -INFINITY;
+        }
+        float top[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top[i] = max_nan(s[2 * i], s[2 * i + 1]);
+#pragma unroll
+        for (int i = 16; i < kKeys; i += 16)
+#pragma unroll
+          for (int k = 0; k < 8; ++k) top[k] = max3_nan(top[k], s[i + 2 * k], s[i + 2 * k + 1]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) top[k] = max_nan(top[k], top[k + 4]);
+        const float best = max3_nan(m, max_nan(top[0], top[1]), max_nan(top[2], top[3]));
+        // a row that has seen nothing yet has an empty O: its first maximum rescales nothing
+        const bool moves = !((best - m) * sc <= kSlack) && !(best == -INFINITY);
+        const bool any_moves = __any_sync(0xffffffffu, moves);
+        float down = 1.f;
+        if (any_moves) {
+          if (moves) {
+            down = m == -INFINITY ? 0.f : ex2_approx((m - best) * sc);
+            m = best;
+          }
+          l *= down;
+        }
+        const float shift = m == -INFINITY ? 0.f : -m * sc;
+        // a border's masked scores have weight 0, which the polynomial does not give
+        l += masked ? weights<T, 0>(s, sc, shift, t_u) : weights<T, kPoly>(s, sc, shift, t_u);
+        // O rests once the product before has completed (waited for at every step, so that the parity is exact)
+        if (u > 0) {
+          ok = wait_warp(bar(kODone + t), (n - 1) & 1, &g_seq_fwd_errors, kErrSoftmax);
+          if (!ok) break;
+          if (any_moves) {
+#pragma unroll
+            for (int i = 0; i < DP; i += 32) {
+              if (i < p.a.dim) {
+                uint32_t o[32];
+                tmem_ld32(t_o + i, o);
+                tmem_wait_ld();
+#pragma unroll
+                for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * down);
+                tmem_st16(t_o + i, o);
+                tmem_st16(t_o + i + 16, o + 16);
+              }
+            }
           }
         }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(kPFull + t));
       }
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(kPFull + t));
-    }
-    if (ok && mine) ok = wait_warp(bar(kODone + t), (mine - 1) & 1, &g_seq_fwd_errors, kErrSoftmax);
-    if (ok && (mine + 1) / 2 > w.border)   // for what the copying warp says of the values
-      ok = wait_warp(bar(kClean + (mine + 1) / 2 - 1 - w.border), 0, &g_seq_fwd_errors, kErrSoftmax);
-    if (ok) {
+      if (!ok) break;
+      if (mine) ok = wait_warp(bar(kODone + t), (n - 1) & 1, &g_seq_fwd_errors, kErrSoftmax);
+      if (!ok) break;
       const float inv = seen > 0 ? 1.f / l : 0.f;
-      const int64_t at = (int64_t)(w.r.q0 + row) * p.a.heads + head;
+      const int64_t at = (int64_t)(now.r.q0 + row) * p.a.heads + head;
       T *out = static_cast<T *>(p.out) + at * p.a.dim;
-      const bool add_back = not_finite != 0;
+      // what the copying warp says of this pair's values: written before the last O was made
+      const bool add_back = (mine + 1) / 2 > now.border && *reinterpret_cast<volatile int *>(&not_finite[done & 1]) != 0;
 #pragma unroll
       for (int i = 0; i < DP; i += 32) {
         if (i >= p.a.dim) continue;
@@ -365,8 +427,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int k = 0; k < 32; ++k) o[k] = seen > 0 ? __float_as_uint(__uint_as_float(o[k]) * inv) : 0u;
         if (add_back && seen > 0) {
-          for (int j = w.border * kTile; j < seen; ++j) {
-            const T *v = static_cast<const T *>(p.a.v) + (int64_t)(w.r.k0 + j) * p.a.v_stride[0] + w.kv * p.a.v_stride[1];
+          for (int j = now.border * kTile; j < seen; ++j) {
+            const T *v = static_cast<const T *>(p.a.v) + (int64_t)(now.r.k0 + j) * p.a.v_stride[0] + now.kv * p.a.v_stride[1];
 #pragma unroll
             for (int k = 0; k < 32; ++k) {
               const float x = i + k < p.a.dim ? to_f32<T>(v[i + k]) : 0.f;
@@ -374,7 +436,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         }
-        if (row < w.r.nq) {
+        if (there) {
 #pragma unroll
           for (int k = 0; k < 32; k += 8)
             if (i + k < p.a.dim)
@@ -385,8 +447,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                              pack<T>(__uint_as_float(o[k + 6]), __uint_as_float(o[k + 7])));
         }
       }
-      if (p.lse && row < w.r.nq)
-        p.lse[(int64_t)head * p.a.q_rows + w.r.q0 + row] = seen > 0 ? (m * sc + log2f(l)) * 0.6931471805599453f : -INFINITY;
+      if (p.lse && there)
+        p.lse[(int64_t)head * p.a.q_rows + now.r.q0 + row] = seen > 0 ? (m * sc + log2f(l)) * 0.6931471805599453f : -INFINITY;
+      tc_fence_before();   // O is read before the next pair's P lets a product write it
+      ++done;
     }
     tmem_wait_st();
   }
@@ -404,10 +468,10 @@ __global__ void fill_kernel(float *p, int64_t n, float v) {
 }
 
 template <typename T, int DP>
-int launch_t(const Params &p, int64_t grid, const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv, cudaStream_t s) {
+int launch_t(const Params &p, int grid, const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv, cudaStream_t s) {
   static size_t seen[kMaxDevices] = {};
   if (int st = smem_optin(sequence_fwd_kernel<T, DP>, Layout<DP>::kBytes, seen)) return st;
-  sequence_fwd_kernel<T, DP><<<(unsigned)grid, kThreads, Layout<DP>::kBytes, s>>>(tq, tk, tv, p);
+  sequence_fwd_kernel<T, DP><<<grid, kThreads, Layout<DP>::kBytes, s>>>(tq, tk, tv, p);
   P3D_LAUNCH_CHECK();
   return P3D_OK;
 }
@@ -430,8 +494,10 @@ int launch_fwd(const p3d_sequence &a, void *out, float *lse, cudaStream_t s) {
   p.steps = (a.dim + 15) / 16;
   p.idesc_o = idesc_f16(128, p.steps * 16, a.dtype == P3D_BF16, true);
   p.sc = a.scale * 1.4426950408889634f;
-  const int64_t grid = slots_of(a.q_rows, a.sequences, p.two_heads ? kTile : 2 * kTile) * p.units;
-  if (grid > 0x7fffffff) return fail(P3D_ERR_UNSUPPORTED, "p3d_sequence_fwd: too many tiles");
+  const int64_t works = slots_of(a.q_rows, a.sequences, p.two_heads ? kTile : 2 * kTile) * p.units;
+  if (works > 0x7fffffff - 4096) return fail(P3D_ERR_UNSUPPORTED, "p3d_sequence_fwd: too many tiles");
+  p.works = (int)works;
+  const int grid = p.works;
   CUtensorMap tq, tk, tv;
   if (int st = encode_heads(&tq, a.dtype, a.q, a.dim, a.heads, a.q_rows, a.q_stride)) return st;
   if (int st = encode_heads(&tk, a.dtype, a.k, a.dim, a.kv_heads, a.k_rows, a.k_stride)) return st;

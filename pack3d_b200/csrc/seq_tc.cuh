@@ -66,6 +66,28 @@ __device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, unsigne
   return all;
 }
 
+// Work beyond a CTA's own: a CTA that is about to be done takes over one that the grid has not launched yet (cluster launch control), so
+// that long and short pieces even out as they would by separate launches, without setting a CTA up for each. The answer, 16 bytes,
+// arrives at `slot` and completes on the barrier (which expects them); after a -1 nothing may be asked any more.
+__device__ __forceinline__ void ask_for_work(uint32_t slot, uint32_t bar) {
+  mbar_expect_tx(bar, 16);
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(slot), "r"(bar)
+               : "memory");
+}
+__device__ __forceinline__ int work_given(uint32_t slot) {
+  int index;
+  asm volatile(
+      "{\n\t.reg .b128 answer;\n\t.reg .pred given;\n\t"
+      "ld.shared.b128 answer, [%1];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 given, answer;\n\t"
+      "mov.s32 %0, -1;\n\t"
+      "@given clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %0, answer;\n\t}"
+      : "=r"(index)
+      : "r"(slot)
+      : "memory");
+  return index;
+}
+
 template <typename T> __device__ __forceinline__ uint32_t pack(float a, float b) {
   return std::is_same<T, __half>::value ? pack_f16(a, b) : pack_bf16(a, b);
 }
