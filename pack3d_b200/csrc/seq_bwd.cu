@@ -9,10 +9,10 @@
 // 512 cycles a product), the exponentials at dim 64 and below.
 //
 // dQ: a CTA has 128 queries of a head; S in two buffers, dP and dQ fill the tensor memory (512 columns). dS (16-bit) goes over S. The pipe makes S
-//   and dP of the next keys while the softmax warps, in two groups of 64 columns, work on these.
+//   and dP of the next keys while the softmax warps, in two groups of 64 columns, work on these. One warp issues S, one dP and dQ: with one for
+//   all, S waited for dQ with nothing else under way (383 us for the figure below).
 // dK, dV: a CTA has 128 keys of a KV head and goes over the queries that see them of all heads of its group: S^T = K Q^T and dP^T = V dO^T (keys
-//   on the lanes), P^T over S^T, dS^T over dP^T, both read from tensor memory by dV += P^T dO and dK += dS^T Q. Order: dV(i), S(i + 1), dK(i), dP(i + 1),
-//   so that the exponentials of the next step run beside two products. Where there are few key tiles, a group's heads are shared among
+//   on the lanes), P^T over S^T, dS^T over dP^T, both read from tensor memory by dV += P^T dO and dK += dS^T Q. Where there are few key tiles, a group's heads are shared among
 //   several CTAs, whose sums in fp32 are added by a last kernel.
 //
 // Masks and values that are not finite: as in the forward kernel, operands of border tiles are cleared of infinities and NaN before the
@@ -30,7 +30,7 @@ namespace {
 
 __device__ unsigned g_seq_bwd_errors = 0;
 
-constexpr int kMmaWarp = 8, kCopyWarp = 9, kThreads = 320, kSoftmaxWarps = 8, kBorders = 3;
+constexpr int kMmaWarp = 8, kCopyWarp = 10, kThreads = 352, kSoftmaxWarps = 8, kBorders = 3;   // two warps of products
 
 struct Params {
   p3d_sequence a;
@@ -103,10 +103,10 @@ struct LayoutQ {
   static constexpr size_t kBytes = 1024 + (2 + kK + kV) * (size_t)kTileBytes;
 };
 // Parity waits: each waiter of a barrier that completes many times has seen every completion before, and the one after its own needs a
-// step of the waiter: so dS has a barrier for each of its two buffers (with one, dS of the next keys could be there while the wait for
-// this one's begins, as S and dP of those are made ahead of it). Border tiles have barriers of their own: kSeen (their S is complete),
+// step of the waiter: so dS and dQ have a barrier for each of the two buffers (with one, those of the next keys could be there while the wait for
+// these begins, as S and dP of those are made ahead of it). Border tiles have barriers of their own: kSeen (their S is complete),
 // kClean (K cleared).
-enum { kQFull, kSFull, kDPFull = kSFull + 2, kDPFree, kDSFull, kDQDone = kDSFull + 2, kDone, kDrainQ, kSeen, kClean = kSeen + kBorders,
+enum { kQFull, kSFull, kDPFull = kSFull + 2, kDPFree, kDSFull, kDQDone = kDSFull + 2, kDone = kDQDone + 2, kDrainQ, kSeen = kDrainQ + 2, kClean = kSeen + kBorders,
        kKFull = kClean + kBorders, kKEmpty = kKFull + 3, kVFull = kKEmpty + 3, kVEmpty = kVFull + 2, kBarsQ = kVEmpty + 2 };
 
 template <typename T, int DP>
@@ -205,46 +205,59 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int i = max(0, n_v - L::kV); i < n_v; ++i)
         mbar_wait(bar(kVFull + i % L::kV), (i / L::kV) & 1, &g_seq_bwd_errors, kWaitNs, kErrTeardown);
     }
-  } else if (warp == kMmaWarp) {
-    {   // warp-wide, as in the forward kernel
-      const uint32_t idesc_s = idesc_f16(128, 128, std::is_same<T, __nv_bfloat16>::value, false);
-      const uint64_t d_q = desc_rows(base), d_do = desc_rows(base + TB), d_k = desc_rows(k_ring), d_v = desc_rows(v_ring),
-                     d_kc = desc_cols(k_ring);
-      int n_s = 0, n_dp = 0, n_dq = 0, n_seen = 0;
-      bool done = false;
-      auto wait = [&](int b, uint32_t parity) { return wait_warp(bar(b), parity, &g_seq_bwd_errors, kErrMma); };
-      auto issue_s = [&](int c) {
+  } else if (warp >= kMmaWarp) {
+    // Products, warp-wide as in the forward kernel, by two warps that need not wait for one another's: S of the keys ahead, dP and dQ.
+    const uint32_t idesc_s = idesc_f16(128, 128, std::is_same<T, __nv_bfloat16>::value, false);
+    auto wait = [&](int b, uint32_t parity) { return wait_warp(bar(b), parity, &g_seq_bwd_errors, kErrMma); };
+    auto drained = [&](int b, int times) {
+      if (times > 0) mbar_wait(bar(b), (times - 1) & 1, &g_seq_bwd_errors, kWaitNs, kErrTeardown);
+    };
+    bool ok = wait(kQFull, 0);
+    if (warp == kMmaWarp) {
+      const uint64_t d_q = desc_rows(base), d_k = desc_rows(k_ring);
+      int n = 0, n_seen = 0;
+      for (int c = 0; ok && c < chunks; ++c) {
+        if (c >= 2) {
+          // The buffer held dS(c - 2), and its dQ was the last that its keys were for. They go by a plain arrival: a commit after
+          // another one's waits until the pipe has run dry.
+          ok = wait(kDQDone + (c & 1), ((c - 2) >> 1) & 1);
+          if (!ok) break;
+          if (lane == 0) mbar_arrive(bar(kKEmpty + (c - 2) % L::kK));
+        }
+        ok = wait(kKFull + c % L::kK, (c / L::kK) & 1);
+        if (!ok) break;
         const uint64_t k = d_k + ((uint32_t)(c % L::kK) * TB >> 4);
-        for (int j = 0; j < p.steps; ++j) mma_ss_warp(tmem + 128 * (c & 1), d_q + step_rows(j), k + step_rows(j), idesc_s, j > 0);
+#pragma unroll
+        for (int j = 0; j < DP / 16; ++j)
+          if (j < p.steps) mma_ss_warp(tmem + 128 * (c & 1), d_q + step_rows(j), k + step_rows(j), idesc_s, j > 0);
         mma_commit_warp(bar(kSFull + (c & 1)));
-        ++n_s;
+        ++n;
         if (c >= border) {
           mma_commit_warp(bar(kSeen + c - border));
           ++n_seen;
         }
-      };
+      }
+      mma_commit_warp(bar(kDrainQ));
+      drained(kDrainQ, 1);
+      drained(kSFull, (n + 1) / 2);
+      drained(kSFull + 1, n / 2);
+      for (int i = 0; i < n_seen; ++i) drained(kSeen + i, 1);
+    } else {
+      const uint64_t d_do = desc_rows(base + TB), d_v = desc_rows(v_ring), d_kc = desc_cols(k_ring);
+      int n_dp = 0, n_dq = 0;
+      bool done = false;
       auto issue_dp = [&](int c) {
         const uint64_t v = d_v + ((uint32_t)(c % L::kV) * TB >> 4);
-        for (int j = 0; j < p.steps; ++j) mma_ss_warp(t_dp, d_do + step_rows(j), v + step_rows(j), idesc_s, j > 0);
+#pragma unroll
+        for (int j = 0; j < DP / 16; ++j)
+          if (j < p.steps) mma_ss_warp(t_dp, d_do + step_rows(j), v + step_rows(j), idesc_s, j > 0);
         mma_commit_warp(bar(kDPFull));
         ++n_dp;
       };
-      bool ok = wait(kQFull, 0) && wait(kKFull, 0);
-      if (ok) {
-        issue_s(0);
-        ok = wait(kVFull, 0);
-        if (ok) issue_dp(0);
-      }
+      ok = ok && wait(kVFull, 0);
+      if (ok) issue_dp(0);
       for (int c = 0; ok && c < chunks; ++c) {
         if (c + 1 < chunks) {
-          // the buffer of S(c + 1) held dS(c - 1)
-          ok = c == 0 || wait(kDQDone, (c - 1) & 1);
-          if (!ok) break;
-          // keys whose dQ is there may go; by a plain arrival, as a second commit would wait until the pipe has run dry
-          if (c > 0 && lane == 0) mbar_arrive(bar(kKEmpty + (c - 1) % L::kK));
-          ok = wait(kKFull + (c + 1) % L::kK, ((c + 1) / L::kK) & 1);
-          if (!ok) break;
-          issue_s(c + 1);
           ok = wait(kVFull + (c + 1) % L::kV, ((c + 1) / L::kV) & 1) && wait(kDPFree, c & 1);
           if (!ok) break;
           issue_dp(c + 1);
@@ -255,24 +268,19 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int j = 0; j < kTile / 16; ++j)   // each softmax group's dS lies over its own half of S
           mma_ts_warp(t_dq, tmem + 128 * (c & 1) + j / 4 * 64 + j % 4 * 8, k + step_cols(j), p.idesc_out, c > 0 || j > 0);
-        mma_commit_warp(bar(kDQDone));
+        mma_commit_warp(bar(kDQDone + (c & 1)));
         ++n_dq;
       }
       if (ok) {
         mma_commit_warp(bar(kDone));
         done = true;
       }
-      mma_commit_warp(bar(kDrainQ));
-      auto drained = [&](int b, int times) {
-        if (times > 0) mbar_wait(bar(b), (times - 1) & 1, &g_seq_bwd_errors, kWaitNs, kErrTeardown);
-      };
-      drained(kDrainQ, 1);
-      drained(kSFull, (n_s + 1) / 2);
-      drained(kSFull + 1, n_s / 2);
+      mma_commit_warp(bar(kDrainQ + 1));
+      drained(kDrainQ + 1, 1);
       drained(kDPFull, n_dp);
-      drained(kDQDone, n_dq);
+      drained(kDQDone, (n_dq + 1) / 2);
+      drained(kDQDone + 1, n_dq / 2);
       drained(kDone, done);
-      for (int i = 0; i < n_seen; ++i) drained(kSeen + i, 1);
     }
   } else {
     const int half = warp / 4, row = row0 + (warp % 4) * 32 + lane;
@@ -353,7 +361,7 @@ struct LayoutKV {
   static constexpr uint32_t kStageBytes = 2 * kTileBytes;   // Q, dO
   static constexpr size_t kBytes = 1024 + 2 * kTileBytes + kStages * (size_t)(kStageBytes + kTile * sizeof(float2));
 };
-enum { kKVFull, kSTFull, kDPTFull, kPFull, kDSTFull, kDVDone, kDKDone, kAllDone, kDrainKV, kSeenKV, kCleanKV, kFullKV };
+enum { kKVFull, kSTFull, kDPTFull, kPFull, kDSTFull, kDVDone, kDKDone, kAllDone, kDrainKV, kSeenKV = kDrainKV + 2, kCleanKV, kFullKV };
 template <int DP> constexpr int bars_kv() { return kFullKV + 2 * LayoutKV<DP>::kStages; }
 
 template <typename T, int DP>
@@ -424,7 +432,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto empty = [&](int s) { return bar(kFullKV + NS + s); };
   if (threadIdx.x == 0) {
     not_finite = 0;
-    for (int i = 0; i < bars_kv<DP>(); ++i) mbar_init(bar(i), i == kPFull || i == kDSTFull ? kSoftmaxWarps : 1);
+    // S and dP are complete, all is, a stage is empty: when both warps of products say so
+    for (int i = 0; i < bars_kv<DP>(); ++i)
+      mbar_init(bar(i), i == kPFull || i == kDSTFull ? kSoftmaxWarps : i == kSeenKV || i == kAllDone || i >= kFullKV + NS ? 2 : 1);
     fence_mbar_init();
   }
   if (warp == kMmaWarp) {
@@ -495,79 +505,61 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int i = max(0, issued - NS); i < issued; ++i)
         mbar_wait(full(i % NS), (i / NS) & 1, &g_seq_bwd_errors, kWaitNs, kErrTeardown);
     }
-  } else if (warp == kMmaWarp) {
-    {   // warp-wide, as in the forward kernel
-      const uint32_t idesc_s = idesc_f16(128, 128, std::is_same<T, __nv_bfloat16>::value, false);
-      const uint64_t d_k = desc_rows(base), d_v = desc_rows(base + TB), d_ring = desc_rows(ring), d_ringc = desc_cols(ring);
-      int n_s = 0, n_dp = 0, n_dv = 0, n_dk = 0, n_seen = 0, borders = 0;
-      bool done = false;
-      auto wait = [&](uint32_t b, uint32_t parity) { return wait_warp(b, parity, &g_seq_bwd_errors, kErrMma); };
-      auto stage = [&](int i) { return (uint32_t)(i % NS) * L::kStageBytes >> 4; };
-      auto issue_s = [&](int i) {
-        for (int j = 0; j < p.steps; ++j) mma_ss_warp(tmem, d_k + step_rows(j), d_ring + stage(i) + step_rows(j), idesc_s, j > 0);
-        mma_commit_warp(bar(kSTFull));
-        ++n_s;
-      };
-      auto issue_dp = [&](int i) {
-        const uint64_t o = d_ring + stage(i) + (TB >> 4);
-        for (int j = 0; j < p.steps; ++j) mma_ss_warp(t_dp, d_v + step_rows(j), o + step_rows(j), idesc_s, j > 0);
-        mma_commit_warp(bar(kDPTFull));
-        ++n_dp;
-        if (is_border(i)) {   // covers S too
-          mma_commit_warp(bar(kSeenKV));
-          ++n_seen;
-        }
-      };
-      auto sum = [&](uint32_t to, uint32_t from, uint64_t b, bool more) {
+  } else if (warp >= kMmaWarp) {
+    // Products, warp-wide as in the forward kernel: two chains that meet only in the softmax, a warp each, so that each fills the other's
+    // waits: dV(i), then S(i + 1) over the P that it read; dK(i), then dP(i + 1) over the dS that it read.
+    const bool second = warp != kMmaWarp;
+    const uint32_t idesc_s = idesc_f16(128, 128, std::is_same<T, __nv_bfloat16>::value, false);
+    const uint32_t t_in = second ? t_dp : tmem, t_out = second ? t_dk : t_dv;
+    const uint64_t d_a = desc_rows(second ? base + TB : base);                        // V, K
+    const uint64_t d_b = desc_rows(second ? ring + TB : ring), d_c = desc_cols(second ? ring : ring + TB);   // dO, Q; then Q, dO
+    const int in_full = second ? kDPTFull : kSTFull, weights_full = second ? kDSTFull : kPFull, out_done = second ? kDKDone : kDVDone;
+    int n_in = 0, n_out = 0, n_seen = 0, borders = 0;
+    bool done = false;
+    auto wait = [&](uint32_t b, uint32_t parity) { return wait_warp(b, parity, &g_seq_bwd_errors, kErrMma); };
+    auto stage = [&](int i) { return (uint32_t)(i % NS) * L::kStageBytes >> 4; };
+    auto issue_in = [&](int i) {
 #pragma unroll
-        for (int j = 0; j < kTile / 16; ++j)
-          mma_ts_warp(to, from + j / 4 * 64 + j % 4 * 8, b + step_cols(j), p.idesc_out, more || j > 0);
-      };
-      bool ok = wait(bar(kKVFull), 0) && wait(full(0), 0);
-      if (ok) {
-        issue_s(0);
-        issue_dp(0);
+      for (int j = 0; j < DP / 16; ++j)
+        if (j < p.steps) mma_ss_warp(t_in, d_a + step_rows(j), d_b + stage(i) + step_rows(j), idesc_s, j > 0);
+      mma_commit_warp(bar(in_full));
+      ++n_in;
+      if (is_border(i)) {
+        mma_commit_warp(bar(kSeenKV));
+        ++n_seen;
       }
-      for (int i = 0; ok && i < steps; ++i) {
-        if (is_border(i)) ok = wait(bar(kCleanKV), borders++ & 1);
-        ok = ok && wait(bar(kPFull), i & 1);
+    };
+    bool ok = wait(bar(kKVFull), 0) && wait(full(0), 0);
+    if (ok) issue_in(0);
+    for (int i = 0; ok && i < steps; ++i) {
+      if (is_border(i)) ok = wait(bar(kCleanKV), borders++ & 1);
+      ok = ok && wait(bar(weights_full), i & 1);
+      if (!ok) break;
+#pragma unroll
+      for (int j = 0; j < kTile / 16; ++j)
+        mma_ts_warp(t_out, t_in + j / 4 * 64 + j % 4 * 8, d_c + stage(i) + step_cols(j), p.idesc_out, i > 0 || j > 0);
+      mma_commit_warp(bar(out_done));
+      ++n_out;
+      if (i + 1 < steps) {
+        ok = wait(full((i + 1) % NS), ((i + 1) / NS) & 1) && wait(bar(out_done), i & 1);
         if (!ok) break;
-        sum(t_dv, tmem, d_ringc + stage(i) + (TB >> 4), i > 0);
-        mma_commit_warp(bar(kDVDone));
-        ++n_dv;
-        if (i + 1 < steps) {
-          ok = wait(full((i + 1) % NS), ((i + 1) / NS) & 1) && wait(bar(kDVDone), i & 1);
-          if (!ok) break;
-          issue_s(i + 1);
-        }
-        ok = wait(bar(kDSTFull), i & 1);
-        if (!ok) break;
-        sum(t_dk, t_dp, d_ringc + stage(i), i > 0);
-        mma_commit_warp(bar(kDKDone));
-        ++n_dk;
-        if (i + 1 < steps) {
-          ok = wait(bar(kDKDone), i & 1);
-          if (!ok) break;
-          if (lane == 0) mbar_arrive(empty(i % NS));   // a plain arrival: a second commit would wait until the pipe has run dry
-          issue_dp(i + 1);
-        }
+        if (lane == 0) mbar_arrive(empty(i % NS));   // a plain arrival: a second commit would wait until the pipe has run dry
+        issue_in(i + 1);
       }
-      if (ok) {
-        mma_commit_warp(bar(kAllDone));
-        done = true;
-      }
-      mma_commit_warp(bar(kDrainKV));
-      auto drained = [&](uint32_t b, int times) {
-        if (times > 0) mbar_wait(b, (times - 1) & 1, &g_seq_bwd_errors, kWaitNs, kErrTeardown);
-      };
-      drained(bar(kDrainKV), 1);
-      drained(bar(kSTFull), n_s);
-      drained(bar(kDPTFull), n_dp);
-      drained(bar(kDVDone), n_dv);
-      drained(bar(kDKDone), n_dk);
-      drained(bar(kSeenKV), n_seen);
-      drained(bar(kAllDone), done);
     }
+    if (ok) {
+      mma_commit_warp(bar(kAllDone));
+      done = true;
+    }
+    mma_commit_warp(bar(kDrainKV + second));
+    auto drained = [&](uint32_t b, int times) {
+      if (times > 0) mbar_wait(b, (times - 1) & 1, &g_seq_bwd_errors, kWaitNs, kErrTeardown);
+    };
+    drained(bar(kDrainKV + second), 1);
+    drained(bar(in_full), n_in);
+    drained(bar(out_done), n_out);
+    drained(bar(kSeenKV), n_seen);
+    drained(bar(kAllDone), done);
   } else {
     const int half = warp / 4;
     const uint32_t lanes = (uint32_t)((warp % 4) * 32) << 16, t_s = tmem + 64 * half + lanes, t_d = t_dp + 64 * half + lanes;
