@@ -4,20 +4,15 @@
 //
 // (dS with its scale, so that in f16 it stays in range where the gradients do.)
 //
-// Two kernels, so that each gradient is a sum in one fixed order without atomics: dQ by tiles of queries, dK and dV by tiles of keys. They make
-// S and dP both, seven products of which five are the mathematics' own; the tensor pipe bounds both at dim 128 (a tile of 128 x 128 is
-// 512 cycles a product), the exponentials at dim 64 and below.
+// Two kernels, so that each gradient is a sum in one fixed order without atomics: dQ by tiles of queries, dK and dV by tiles of keys.
+// They make S and dP both, seven products of which five are the mathematics' own (a tile of 128 x 128 is 512 cycles a product).
 //
-// dQ: a CTA has 128 queries of a head; S in two buffers, dP and dQ fill the tensor memory (512 columns). dS (16-bit) goes over S. The pipe makes S
-//   and dP of the next keys while the softmax warps, in two groups of 64 columns, work on these. One warp issues S, one dP and dQ: with one for
-//   all, S waited for dQ with nothing else under way (383 us for the figure below).
-// dK, dV: a CTA has 128 keys of a KV head and goes over the queries that see them of all heads of its group: S^T = K Q^T and dP^T = V dO^T (keys
-//   on the lanes), P^T over S^T, dS^T over dP^T, both read from tensor memory by dV += P^T dO and dK += dS^T Q. Where there are few key tiles, a group's heads are shared among
-//   several CTAs, whose sums in fp32 are added by a last kernel.
+// dQ: a CTA has 128 queries of a head; S in two buffers, dP and dQ fill the tensor memory (512 columns). dS (16-bit) goes over S. The
+//   pipe makes S and dP of the next keys while the softmax warps, in two groups of 64 columns, work on these.
+// dK, dV: a CTA has 128 keys of a KV head and goes over the queries that see them of all heads of its group: S^T = K Q^T and
+//   dP^T = V dO^T (keys on the lanes), P^T over S^T, dS^T over dP^T, both read from tensor memory by dV += P^T dO and dK += dS^T Q.
+//   Where there are few key tiles, a group's heads are shared among several CTAs, whose sums in fp32 are added by a last kernel.
 //
-// Masks and values that are not finite: as in the forward kernel, operands of border tiles are cleared of infinities and NaN before the
-// product whose weights are 0 for rows that do not see them (K for dQ; dO and Q for dV and dK), once the products that need them
-// as they are have completed. A row that sees such a value is NaN through lse or delta; only dO's in dV are added back.
 #include <math.h>
 
 #include <algorithm>
@@ -30,11 +25,11 @@ namespace {
 
 __device__ unsigned g_seq_bwd_errors = 0;
 
-constexpr int kMmaWarp = 8, kCopyWarp = 10, kThreads = 352, kSoftmaxWarps = 8, kBorders = 3;   // two warps of products
+constexpr int kMmaWarp = 8, kCopyWarp = 10, kThreads = 352, kSoftmaxWarps = 8;   // two warps of products
 
 struct Params {
   p3d_sequence a;
-  const float2 *stats;     // [heads][q_rows]: lse * log2(e), scale * delta
+  const float2 *stats;     // [heads][q_rows]: -lse * log2(e), -scale * delta
   const void *dout;        // contiguous
   void *dq, *dk, *dv;
   float *part;             // [2][parts][k_rows * kv_heads * dim] where parts > 1
@@ -44,26 +39,14 @@ struct Params {
   float sc;                // scale * log2(e)
 };
 
-// 2^(s sc + minus) of a pair of scores.
-template <bool kPoly>
-__device__ __forceinline__ float2 weight(float2 s, float2 sc, float2 minus) {
-  const float2 x = fma2(s, sc, minus);
-  if constexpr (kPoly) {
-    // NaN would not come through
-    const float2 e = exp2_poly2(x);
-    return make_float2(x.x == x.x ? e.x : x.x, x.y == x.y ? e.y : x.y);
-  } else {
-    return make_float2(ex2_approx(x.x), ex2_approx(x.y));
-  }
-}
-// 64 columns, a quarter of them by polynomials where none is masked; minus(k): of columns 2 k, 2 k + 1.
-template <bool kPoly, typename F>
+// 2^(s sc + minus) of 64 scores; minus(k): of columns 2 k, 2 k + 1. All on the special-function units: a pair is 16 cycles there, and
+// as many on the FMA pipe as polynomials, which has the products' other arithmetic to do.
+template <typename F>
 __device__ __forceinline__ void weights(float (&s)[64], float2 sc, F minus) {
 #pragma unroll
   for (int k = 0; k < 32; ++k) {
-    const float2 x = make_float2(s[2 * k], s[2 * k + 1]);
-    const float2 w = kPoly && k % 4 == 3 ? weight<true>(x, sc, minus(k)) : weight<false>(x, sc, minus(k));
-    s[2 * k] = w.x, s[2 * k + 1] = w.y;
+    const float2 x = fma2(make_float2(s[2 * k], s[2 * k + 1]), sc, minus(k));
+    s[2 * k] = ex2_approx(x.x), s[2 * k + 1] = ex2_approx(x.y);
   }
 }
 
@@ -73,26 +56,63 @@ __device__ __forceinline__ void load_columns(uint32_t t, float *v) {
   for (int i = 0; i < N; i += 32) tmem_ld32(t + i, reinterpret_cast<uint32_t *>(v) + i);
 }
 
-// 32 columns of an accumulator into a row of T, or of fp32.
+// 64 columns of an accumulator in 16 bits (zeros unless `write`); returns NaN where any of those below dim is not finite.
 template <typename T>
-__device__ __forceinline__ void store_columns(uint32_t t, int col, int dim, T *row, float *wide) {
-  uint32_t o[32];
-  tmem_ld32(t + col, o);
-  tmem_wait_ld();
+__device__ __forceinline__ float pack_columns(uint32_t t, int col, int dim, bool write, uint32_t (&packed)[32]) {
+  float odd = 0.f;
 #pragma unroll
-  for (int k = 0; k < 32; k += 8) {
-    if (col + k >= dim) continue;
-    float v[8];
+  for (int h = 0; h < 64; h += 32) {
+    uint32_t o[32];
+    tmem_ld32(t + h, o);
+    tmem_wait_ld();
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(o[k + i]);
-    if (wide) {
-      reinterpret_cast<float4 *>(wide + col + k)[0] = make_float4(v[0], v[1], v[2], v[3]);
-      reinterpret_cast<float4 *>(wide + col + k)[1] = make_float4(v[4], v[5], v[6], v[7]);
-    } else if (row) {
-      *reinterpret_cast<uint4 *>(row + col + k) =
-          make_uint4(pack<T>(v[0], v[1]), pack<T>(v[2], v[3]), pack<T>(v[4], v[5]), pack<T>(v[6], v[7]));
+    for (int k = 0; k < 32; k += 2) {
+      const float a = write ? __uint_as_float(o[k]) : 0.f, b = write ? __uint_as_float(o[k + 1]) : 0.f;
+      if (col + h + k < dim) odd = fmaf(a, 0.f, fmaf(b, 0.f, odd));
+      packed[(h + k) / 2] = pack<T>(a, b);
     }
   }
+  return odd;
+}
+
+// One row of dQ by the definition (a warp); columns of the half that found it.
+template <typename T>
+__device__ __noinline__ void redo_dq(const Params &p, const Range &r, int head, int row, int seen, int half, T *out) {
+  const p3d_sequence &a = p.a;
+  const int kv = head / (a.heads / a.kv_heads), dim = a.dim, lane = threadIdx.x & 31;
+  float q[4], d[4], k[4], v[4], sum[4] = {0.f, 0.f, 0.f, 0.f};
+  load4(static_cast<const T *>(a.q) + (int64_t)(r.q0 + row) * a.q_stride[0] + head * a.q_stride[1], dim, q);
+  load4(static_cast<const T *>(p.dout) + ((int64_t)(r.q0 + row) * a.heads + head) * dim, dim, d);
+  const float2 stat = p.stats[(int64_t)head * a.q_rows + r.q0 + row];
+  for (int j = 0; j < seen; ++j) {
+    load4(static_cast<const T *>(a.k) + (int64_t)(r.k0 + j) * a.k_stride[0] + kv * a.k_stride[1], dim, k);
+    load4(static_cast<const T *>(a.v) + (int64_t)(r.k0 + j) * a.v_stride[0] + kv * a.v_stride[1], dim, v);
+    const float ds = exp2f(dot4(q, k) * p.sc + stat.x) * fmaf(dot4(d, v), a.scale, stat.y);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum[i] = fmaf(ds, k[i], sum[i]);
+  }
+  // 64 columns each for the two groups of warps
+  if (lane / 16 == half) mend4(out, dim, sum);
+}
+
+// One key's row of dK (or dV) from the queries of `heads` heads that see it, by the definition (a warp): added up in four columns a lane.
+template <typename T>
+__device__ __noinline__ void redo_dkv(const Params &p, const Range &r, int kv, int head0, int heads, int key, int from, bool values,
+                                      float (&sum)[4]) {
+  const p3d_sequence &a = p.a;
+  float q[4], d[4], k[4], v[4];
+  load4(static_cast<const T *>(a.k) + (int64_t)(r.k0 + key) * a.k_stride[0] + kv * a.k_stride[1], a.dim, k);
+  load4(static_cast<const T *>(a.v) + (int64_t)(r.k0 + key) * a.v_stride[0] + kv * a.v_stride[1], a.dim, v);
+  sum[0] = sum[1] = sum[2] = sum[3] = 0.f;
+  for (int head = head0; head < head0 + heads; ++head)
+    for (int i = from; i < r.nq; ++i) {
+      load4(static_cast<const T *>(a.q) + (int64_t)(r.q0 + i) * a.q_stride[0] + head * a.q_stride[1], a.dim, q);
+      load4(static_cast<const T *>(p.dout) + ((int64_t)(r.q0 + i) * a.heads + head) * a.dim, a.dim, d);
+      const float2 stat = p.stats[(int64_t)head * a.q_rows + r.q0 + i];
+      const float w = exp2f(dot4(q, k) * p.sc + stat.x), ds = w * fmaf(dot4(d, v), a.scale, stat.y);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) sum[c] = values ? fmaf(w, d[c], sum[c]) : fmaf(ds, q[c], sum[c]);
+    }
 }
 
 // ------------------------------------------------------------------------------- dQ
@@ -100,14 +120,13 @@ template <int DP>
 struct LayoutQ {
   static constexpr uint32_t kTileBytes = DP / 64 * kBox;
   static constexpr int kK = 3, kV = 2;   // stages
-  static constexpr size_t kBytes = 1024 + (2 + kK + kV) * (size_t)kTileBytes;
+  static constexpr size_t kBytes = 1024 + (2 + kK + kV) * (size_t)kTileBytes;   // O's way out is over the queries
 };
 // Parity waits: each waiter of a barrier that completes many times has seen every completion before, and the one after its own needs a
 // step of the waiter: so dS and dQ have a barrier for each of the two buffers (with one, those of the next keys could be there while the wait for
-// these begins, as S and dP of those are made ahead of it). Border tiles have barriers of their own: kSeen (their S is complete),
-// kClean (K cleared).
-enum { kQFull, kSFull, kDPFull = kSFull + 2, kDPFree, kDSFull, kDQDone = kDSFull + 2, kDone = kDQDone + 2, kDrainQ, kSeen = kDrainQ + 2, kClean = kSeen + kBorders,
-       kKFull = kClean + kBorders, kKEmpty = kKFull + 3, kVFull = kKEmpty + 3, kVEmpty = kVFull + 2, kBarsQ = kVEmpty + 2 };
+// these begins, as S and dP of those are made ahead of it).
+enum { kQFull, kSFull, kDPFull = kSFull + 2, kDPFree, kDSFull, kDQDone = kDSFull + 2, kDone = kDQDone + 2, kLanded, kDrainQ, kKFull = kDrainQ + 2,
+       kKEmpty = kKFull + 3, kVFull = kKEmpty + 3, kVEmpty = kVFull + 2, kBarsQ = kVEmpty + 2 };
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -122,12 +141,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int slot = (int)(gridDim.x / p.a.heads - 1 - blockIdx.x / p.a.heads), head = blockIdx.x % p.a.heads;   // the longest first
   const int kv = head / (p.a.heads / p.a.kv_heads);
-  const Slot at = find_slot(p.a.q_offsets, p.a.sequences, (int)p.a.q_rows, kTile, slot);
-  const Range r = slot_range(p.a, at.sequence);
+  const Place at = place_of<false>(p.a, 7, slot);
+  const Range r = at.r;
   const int row0 = at.group * kTile;
   if (at.group < 0 || row0 >= r.nq) return;
   const int chunks = (seen_by(r, min(row0 + kTile, r.nq) - 1, p.a.causal) + kTile - 1) / kTile;
-  const int border = seen_by(r, row0, p.a.causal) / kTile;
   if (chunks == 0) {
     const int row = row0 + threadIdx.x;
     if (threadIdx.x < kTile && row < r.nq) {
@@ -159,7 +177,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = tmem_holder, t_dp = tmem + 256, t_dq = tmem + 384;   // S at 0 and 128
 
   if (warp == kCopyWarp) {
-    bool ok = true;
     int n_k = 0, n_v = 0;
     if (lane == 0) {
       auto tile = [&](uint32_t dst, const CUtensorMap *map, uint32_t full, int h, int row) {
@@ -173,30 +190,23 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       for (int c = 0; c < chunks; ++c) {
         int s = c % L::kK;
-        if (c >= L::kK && !mbar_wait(bar(kKEmpty + s), (c / L::kK - 1) & 1, &g_seq_bwd_errors, kWaitNs, kErrProducer)) {
-          ok = false;
-          break;
-        }
-        tile(k_ring + s * TB, &tk, bar(kKFull + s), kv, r.k0 + c * kTile);
+        if (c >= L::kK && !mbar_wait(bar(kKEmpty + s), (c / L::kK - 1) & 1, &g_seq_bwd_errors, kWaitNs, kErrProducer)) break;
+        // the last keys, where their tile goes past the sequence's end, land on a barrier of their own
+        tile(k_ring + s * TB, &tk, bar((c + 1) * kTile > r.nk ? kLanded : kKFull + s), kv, r.k0 + c * kTile);
         n_k = c + 1;
         s = c % L::kV;
-        if (c >= L::kV && !mbar_wait(bar(kVEmpty + s), (c / L::kV - 1) & 1, &g_seq_bwd_errors, kWaitNs, kErrProducer)) {
-          ok = false;
-          break;
-        }
+        if (c >= L::kV && !mbar_wait(bar(kVEmpty + s), (c / L::kV - 1) & 1, &g_seq_bwd_errors, kWaitNs, kErrProducer)) break;
         tile(v_ring + s * TB, &tv, bar(kVFull + s), kv, r.k0 + c * kTile);
         n_v = c + 1;
       }
     }
-    ok = __all_sync(0xffffffffu, ok);
-    for (int c = min(border, chunks); ok && c < chunks; ++c) {
-      ok = __all_sync(0xffffffffu, mbar_wait(bar(kSeen + c - border), 0, &g_seq_bwd_errors, kWaitNs, kErrProducer));
-      ok = ok && __all_sync(0xffffffffu, mbar_wait(bar(kKFull + c % L::kK), (c / L::kK) & 1, &g_seq_bwd_errors, kWaitNs, kErrProducer));
-      if (!ok) break;
-      tc_fence_after();
-      if (clear_not_finite<T>(smem_raw + (k_ring - raw) + (c % L::kK) * TB, TB)) fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(kClean + c - border));
+    n_k = __shfl_sync(0xffffffffu, n_k, 0);
+    if (n_k == chunks && chunks * kTile > r.nk) {
+      const int s = (chunks - 1) % L::kK;
+      if (wait_warp(bar(kLanded), 0, &g_seq_bwd_errors, kErrProducer)) {
+        clear_rows<DP / 64>(smem_raw + (k_ring - raw) + s * TB, r.nk - (chunks - 1) * kTile);
+        if (lane == 0) mbar_arrive(bar(kKFull + s));
+      }
     }
     if (lane == 0) {
       mbar_wait(bar(kQFull), 0, &g_seq_bwd_errors, kWaitNs, kErrTeardown);
@@ -215,7 +225,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = wait(kQFull, 0);
     if (warp == kMmaWarp) {
       const uint64_t d_q = desc_rows(base), d_k = desc_rows(k_ring);
-      int n = 0, n_seen = 0;
+      int n = 0;
       for (int c = 0; ok && c < chunks; ++c) {
         if (c >= 2) {
           // The buffer held dS(c - 2), and its dQ was the last that its keys were for. They go by a plain arrival: a commit after
@@ -232,16 +242,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (j < p.steps) mma_ss_warp(tmem + 128 * (c & 1), d_q + step_rows(j), k + step_rows(j), idesc_s, j > 0);
         mma_commit_warp(bar(kSFull + (c & 1)));
         ++n;
-        if (c >= border) {
-          mma_commit_warp(bar(kSeen + c - border));
-          ++n_seen;
-        }
       }
       mma_commit_warp(bar(kDrainQ));
       drained(kDrainQ, 1);
       drained(kSFull, (n + 1) / 2);
       drained(kSFull + 1, n / 2);
-      for (int i = 0; i < n_seen; ++i) drained(kSeen + i, 1);
     } else {
       const uint64_t d_do = desc_rows(base + TB), d_v = desc_rows(v_ring), d_kc = desc_cols(k_ring);
       int n_dp = 0, n_dq = 0;
@@ -262,7 +267,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!ok) break;
           issue_dp(c + 1);
         }
-        ok = (c < border || wait(kClean + c - border, 0)) && wait(kDSFull + (c & 1), (c >> 1) & 1);
+        ok = wait(kDSFull + (c & 1), (c >> 1) & 1);
         if (!ok) break;
         const uint64_t k = d_kc + ((uint32_t)(c % L::kK) * TB >> 4);
 #pragma unroll
@@ -287,7 +292,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const bool there = row < r.nq;
     const int seen = there ? seen_by(r, row, p.a.causal) : 0;
     const float2 stat = there ? p.stats[(int64_t)head * p.a.q_rows + r.q0 + row] : make_float2(0.f, 0.f);
-    const float2 sc = make_float2(p.sc, p.sc), shift = make_float2(-stat.x, -stat.x), minus = make_float2(-stat.y, -stat.y), scale = make_float2(p.a.scale, p.a.scale);
+    const float2 sc = make_float2(p.sc, p.sc), shift = make_float2(stat.x, stat.x), minus = make_float2(stat.y, stat.y), scale = make_float2(p.a.scale, p.a.scale);
     const uint32_t lanes = (uint32_t)((warp % 4) * 32) << 16;
     bool ok = true;
     for (int c = 0; c < chunks; ++c) {
@@ -299,9 +304,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       tmem_wait_ld();
       const int limit = seen - c * kTile - half * 64;
       const bool masked = __any_sync(0xffffffffu, limit < 64);
-      auto lse = [&](int) { return shift; };
-      if (masked) weights<false>(s, sc, lse);
-      else weights<true>(s, sc, lse);
+      weights(s, sc, [&](int) { return shift; });
       ok = wait_warp(bar(kDPFull), c & 1, &g_seq_bwd_errors, kErrSoftmax);
       if (!ok) break;
       float d[64];
@@ -336,11 +339,27 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (ok) ok = wait_warp(bar(kDone), 0, &g_seq_bwd_errors, kErrSoftmax);
     if (ok) {
-      T *to = there ? static_cast<T *>(p.dq) + ((int64_t)(r.q0 + row) * p.a.heads + head) * p.a.dim : nullptr;
-#pragma unroll
-      for (int i = 0; i < DP / 2; i += 32) store_columns<T>(t_dq + lanes, half * (DP / 2) + i, seen > 0 ? p.a.dim : 0, to, nullptr);
-      if (there && seen <= 0)   // a row that sees no key beside rows that do
-        for (int i = half; i < p.a.dim / 8; i += 2) reinterpret_cast<uint4 *>(to)[i] = make_uint4(0, 0, 0, 0);
+      // dQ, by way of the queries' memory: every product has been made
+      uint8_t *const stage = smem_raw + (base - raw) + warp * 4096;
+      const int64_t to = there ? ((int64_t)(r.q0 + row) * p.a.heads + head) * p.a.dim : -1;
+      T *const dq = static_cast<T *>(p.dq);
+      float odd = 0.f;
+      if (DP == 128 || half == 0) {
+        const int col = DP == 128 ? half * 64 : 0;
+        uint32_t packed[32];
+        odd = pack_columns<T>(t_dq + lanes + col, col, p.a.dim, seen > 0, packed);
+        store_rows(stage, packed, dq, to, col, p.a.dim);
+      }
+      // rows beside keys that they do not see; with a NaN lse or delta they are NaN by right. Either group may find the row.
+      const int past = min(chunks * kTile, r.nk);
+      const bool look = there && odd != odd && seen > 0 && seen < past && stat.x == stat.x && stat.y == stat.y;
+      for (unsigned rows = __ballot_sync(0xffffffffu, look); rows; rows &= rows - 1) {
+        const int from = __ffs(rows) - 1, first = __shfl_sync(0xffffffffu, seen, from);
+        if (!rows_not_finite(static_cast<const T *>(p.a.k) + (int64_t)(r.k0 + first) * p.a.k_stride[0] + kv * p.a.k_stride[1],
+                             p.a.k_stride[0], past - first, p.a.dim))
+          continue;
+        redo_dq<T>(p, r, head, __shfl_sync(0xffffffffu, row, from), first, half, dq + __shfl_sync(0xffffffffu, to, from));
+      }
     }
     tmem_wait_st();
   }
@@ -361,7 +380,7 @@ struct LayoutKV {
   static constexpr uint32_t kStageBytes = 2 * kTileBytes;   // Q, dO
   static constexpr size_t kBytes = 1024 + 2 * kTileBytes + kStages * (size_t)(kStageBytes + kTile * sizeof(float2));
 };
-enum { kKVFull, kSTFull, kDPTFull, kPFull, kDSTFull, kDVDone, kDKDone, kAllDone, kDrainKV, kSeenKV = kDrainKV + 2, kCleanKV, kFullKV };
+enum { kKVFull, kSTFull, kDPTFull, kPFull, kDSTFull, kDVDone, kDKDone, kAllDone, kLandedKV, kDrainKV, kFullKV = kDrainKV + 2 };
 template <int DP> constexpr int bars_kv() { return kFullKV + 2 * LayoutKV<DP>::kStages; }
 
 template <typename T, int DP>
@@ -375,20 +394,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t bar_mem[bars_kv<DP>()];
   __shared__ uint32_t tmem_holder;
-  __shared__ int not_finite;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // keys at a sequence's start are seen by the most queries: in order
   const int per_slot = p.a.kv_heads * p.parts, slot = blockIdx.x / per_slot, kv = blockIdx.x % per_slot / p.parts,
             part = blockIdx.x % p.parts;
-  const Slot at = find_slot(p.a.k_offsets, p.a.sequences, (int)p.a.k_rows, kTile, slot);
-  Range r;
-  if (at.sequence < p.a.sequences) {
-    r = range_of(p.a, at.sequence);
-  } else {
-    r = {};
-    r.k0 = cache::offset_at(p.a.k_offsets, at.sequence, (int)p.a.k_rows);
-    r.nk = (int)p.a.k_rows - r.k0;
-  }
+  const Place at = place_of<true>(p.a, 7, slot);
+  const Range r = at.r;
   const int key0 = at.group * kTile;
   if (at.group < 0 || key0 >= r.nk) return;
   const int group = p.a.heads / p.a.kv_heads, head0 = kv * group + group * part / p.parts,
@@ -396,12 +407,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   // query i sees key j where i >= j - (nk - nq)
   const int shift = r.nk - r.nq, first = p.a.causal ? max(0, key0 - shift) : 0;
   const int tiles = first < r.nq ? (r.nq - first + kTile - 1) / kTile : 0, steps = tiles * heads;
-  // a tile of queries from row i on with a pair of query and key that is masked
-  const int whole = p.a.causal ? min(key0 + kTile, r.nk) - 1 - shift : 0;
-  auto is_border = [&](int step) {
-    const int i = first + step % tiles * kTile;
-    return i < whole || i + kTile > r.nq;
-  };
   const int key = key0 + (warp % 4) * 32 + lane;   // of a softmax thread
   const bool there = key < r.nk;
   const int64_t out_row = ((int64_t)(r.k0 + key) * p.a.kv_heads + kv) * p.a.dim;
@@ -426,15 +431,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
   uint8_t *const smem = smem_raw + (base - raw);
   const uint32_t ring = base + 2 * TB;
-  float2 *const stats = reinterpret_cast<float2 *>(smem + 2 * TB + NS * L::kStageBytes);   // [stage][128]
+  float *const stats = reinterpret_cast<float *>(smem + 2 * TB + NS * L::kStageBytes);   // [stage][2][128]: both of 128 queries
   auto bar = [&](int i) { return smem_u32(&bar_mem[i]); };
   auto full = [&](int s) { return bar(kFullKV + s); };
   auto empty = [&](int s) { return bar(kFullKV + NS + s); };
   if (threadIdx.x == 0) {
-    not_finite = 0;
-    // S and dP are complete, all is, a stage is empty: when both warps of products say so
+    // all is complete, a stage is empty: when both warps of products say so
     for (int i = 0; i < bars_kv<DP>(); ++i)
-      mbar_init(bar(i), i == kPFull || i == kDSTFull ? kSoftmaxWarps : i == kSeenKV || i == kAllDone || i >= kFullKV + NS ? 2 : 1);
+      mbar_init(bar(i), i == kPFull || i == kDSTFull ? kSoftmaxWarps : i == kAllDone || i >= kFullKV + NS ? 2 : 1);
     fence_mbar_init();
   }
   if (warp == kMmaWarp) {
@@ -454,7 +458,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp == kCopyWarp) {
     bool ok = true;
-    int issued = 0, borders = 0;
+    int issued = 0, cleared = 0;
     if (lane == 0) {
       mbar_expect_tx(bar(kKVFull), 2 * TB);
       for (int c = 0; c < DP / 64; ++c) {
@@ -462,43 +466,43 @@ __global__ void __launch_bounds__(kThreads, 1)
         tma_load_3d(base + TB + c * kBox, &tv, bar(kKVFull), 64 * c, kv, r.k0 + key0);
       }
     }
-    // step n's copies, then what step n - 1 has to have cleared
-    for (int n = 0; n <= steps; ++n) {
-      if (n < steps) {
-        const int s = n % NS, head = head0 + n / tiles, i0 = first + n % tiles * kTile;
-        float2 v[4];
+    for (int n = 0, head = head0, i0 = first; n < steps; ++n) {
+      const int s = n % NS;
+      float2 v[4];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int i = i0 + lane + 32 * u;
-          v[u] = i < r.nq ? p.stats[(int64_t)head * p.a.q_rows + r.q0 + i] : make_float2(0.f, 0.f);
-        }
-        if (n >= NS) ok = __all_sync(0xffffffffu, mbar_wait(empty(s), (n / NS - 1) & 1, &g_seq_bwd_errors, kWaitNs, kErrProducer));
-        if (!ok) break;
+      for (int u = 0; u < 4; ++u) {
+        const int i = i0 + lane + 32 * u;
+        v[u] = i < r.nq ? p.stats[(int64_t)head * p.a.q_rows + r.q0 + i] : make_float2(0.f, 0.f);
+      }
+      if (n >= NS) ok = __all_sync(0xffffffffu, mbar_wait(empty(s), (n / NS - 1) & 1, &g_seq_bwd_errors, kWaitNs, kErrProducer));
+      if (!ok) break;
 #pragma unroll
-        for (int u = 0; u < 4; ++u) stats[s * kTile + lane + 32 * u] = v[u];
-        __syncwarp();
-        if (lane == 0) {
-          mbar_expect_tx(full(s), 2 * TB);
-          for (int c = 0; c < DP / 64; ++c) {
-            tma_load_3d(ring + s * L::kStageBytes + c * kBox, &tq, full(s), 64 * c, head, r.q0 + i0);
-            tma_load_3d(ring + s * L::kStageBytes + TB + c * kBox, &tdo, full(s), 64 * c, head, r.q0 + i0);
-          }
+      for (int u = 0; u < 4; ++u) {
+        stats[s * 256 + lane + 32 * u] = v[u].x;
+        stats[s * 256 + 128 + lane + 32 * u] = v[u].y;
+      }
+      __syncwarp();
+      // a head's last queries, where their tile goes past the sequence's end, land on a barrier of their own
+      const bool past = i0 + kTile > r.nq;
+      if (lane == 0) {
+        const uint32_t on = past ? bar(kLandedKV) : full(s);
+        mbar_expect_tx(on, 2 * TB);
+        for (int c = 0; c < DP / 64; ++c) {
+          tma_load_3d(ring + s * L::kStageBytes + c * kBox, &tq, on, 64 * c, head, r.q0 + i0);
+          tma_load_3d(ring + s * L::kStageBytes + TB + c * kBox, &tdo, on, 64 * c, head, r.q0 + i0);
         }
-        issued = n + 1;
       }
-      if (n >= 1 && is_border(n - 1)) {
-        ok = __all_sync(0xffffffffu, mbar_wait(bar(kSeenKV), borders & 1, &g_seq_bwd_errors, kWaitNs, kErrProducer));
-        ok = ok && __all_sync(0xffffffffu, mbar_wait(full((n - 1) % NS), ((n - 1) / NS) & 1, &g_seq_bwd_errors, kWaitNs, kErrProducer));
+      issued = n + 1;
+      if (past) {
+        ok = wait_warp(bar(kLandedKV), cleared++ & 1, &g_seq_bwd_errors, kErrProducer);
         if (!ok) break;
-        tc_fence_after();
-        uint8_t *const stage = smem + 2 * TB + (n - 1) % NS * L::kStageBytes;
-        const bool q_odd = clear_not_finite<T>(stage, TB), do_odd = clear_not_finite<T>(stage + TB, TB);
-        if (q_odd || do_odd) fence_proxy_async_smem();
-        if (do_odd && lane == 0) not_finite = 1;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(kCleanKV));
-        ++borders;
+        uint8_t *const tile = smem + 2 * TB + s * L::kStageBytes;
+        clear_rows<DP / 64>(tile, r.nq - i0);
+        clear_rows<DP / 64>(tile + TB, r.nq - i0);
+        if (lane == 0) mbar_arrive(full(s));
       }
+      i0 += kTile;
+      if (i0 >= r.nq) i0 = first, ++head;
     }
     if (lane == 0) {
       mbar_wait(bar(kKVFull), 0, &g_seq_bwd_errors, kWaitNs, kErrTeardown);
@@ -514,7 +518,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint64_t d_a = desc_rows(second ? base + TB : base);                        // V, K
     const uint64_t d_b = desc_rows(second ? ring + TB : ring), d_c = desc_cols(second ? ring : ring + TB);   // dO, Q; then Q, dO
     const int in_full = second ? kDPTFull : kSTFull, weights_full = second ? kDSTFull : kPFull, out_done = second ? kDKDone : kDVDone;
-    int n_in = 0, n_out = 0, n_seen = 0, borders = 0;
+    int n_in = 0, n_out = 0;
     bool done = false;
     auto wait = [&](uint32_t b, uint32_t parity) { return wait_warp(b, parity, &g_seq_bwd_errors, kErrMma); };
     auto stage = [&](int i) { return (uint32_t)(i % NS) * L::kStageBytes >> 4; };
@@ -524,16 +528,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (j < p.steps) mma_ss_warp(t_in, d_a + step_rows(j), d_b + stage(i) + step_rows(j), idesc_s, j > 0);
       mma_commit_warp(bar(in_full));
       ++n_in;
-      if (is_border(i)) {
-        mma_commit_warp(bar(kSeenKV));
-        ++n_seen;
-      }
     };
     bool ok = wait(bar(kKVFull), 0) && wait(full(0), 0);
     if (ok) issue_in(0);
     for (int i = 0; ok && i < steps; ++i) {
-      if (is_border(i)) ok = wait(bar(kCleanKV), borders++ & 1);
-      ok = ok && wait(bar(weights_full), i & 1);
+      ok = wait(bar(weights_full), i & 1);
       if (!ok) break;
 #pragma unroll
       for (int j = 0; j < kTile / 16; ++j)
@@ -558,7 +557,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     drained(bar(kDrainKV + second), 1);
     drained(bar(in_full), n_in);
     drained(bar(out_done), n_out);
-    drained(bar(kSeenKV), n_seen);
     drained(bar(kAllDone), done);
   } else {
     const int half = warp / 4;
@@ -566,22 +564,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     const float2 sc = make_float2(p.sc, p.sc), scale = make_float2(p.a.scale, p.a.scale);
     const int from = p.a.causal ? key - shift : 0;   // the first query that sees this key
     bool ok = true;
-    for (int i = 0; i < steps; ++i) {
-      const int i0 = first + i % tiles * kTile + half * 64, lo = from - i0, hi = r.nq - i0;
+    for (int i = 0, row = first; i < steps; ++i, row = row + kTile < r.nq ? row + kTile : first) {
+      const int i0 = row + half * 64, lo = from - i0, hi = r.nq - i0;
       const bool masked = __any_sync(0xffffffffu, lo > 0 || hi < 64);
-      const float4 *st = reinterpret_cast<const float4 *>(stats + i % NS * kTile + half * 64);   // two queries each
+      const float4 *st = reinterpret_cast<const float4 *>(stats + i % NS * 256 + half * 64);   // of four queries each
       ok = wait_warp(full(i % NS), (i / NS) & 1, &g_seq_bwd_errors, kErrSoftmax) &&
            wait_warp(bar(kSTFull), i & 1, &g_seq_bwd_errors, kErrSoftmax);
       if (!ok) break;
       float s[64];
       load_columns<64>(t_s, s);
       tmem_wait_ld();
-      auto lse = [&](int k) {
-        const float4 q = st[k];
-        return make_float2(-q.x, -q.z);
-      };
-      if (masked) weights<false>(s, sc, lse);
-      else weights<true>(s, sc, lse);
+      weights(s, sc, [&](int k) {
+        const float4 q = st[k / 2];
+        return k % 2 ? make_float2(q.z, q.w) : make_float2(q.x, q.y);
+      });
       if (masked) {
 #pragma unroll
         for (int k = 0; k < 64; ++k) s[k] = k >= lo && k < hi ? s[k] : 0.f;
@@ -604,8 +600,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       tmem_wait_ld();
 #pragma unroll
       for (int k = 0; k < 32; ++k) {
-        const float4 q = st[k];
-        const float2 v = mul2(make_float2(s[2 * k], s[2 * k + 1]), fma2(make_float2(d[2 * k], d[2 * k + 1]), scale, make_float2(-q.y, -q.w)));
+        const float4 q = st[32 + k / 2];
+        const float2 minus = k % 2 ? make_float2(q.z, q.w) : make_float2(q.x, q.y);
+        const float2 v = mul2(make_float2(s[2 * k], s[2 * k + 1]), fma2(make_float2(d[2 * k], d[2 * k + 1]), scale, minus));
         s[2 * k] = v.x, s[2 * k + 1] = v.y;
       }
       if (masked) {
@@ -626,28 +623,57 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (ok) ok = wait_warp(bar(kAllDone), 0, &g_seq_bwd_errors, kErrSoftmax);
     if (ok) {
-      // a half of the warps writes dK, the other dV
-      const int dim = there ? p.a.dim : 0;
+      // a half of the warps writes dK, the other dV; in 16 bits by way of the keys' memory: every product has been made
+      uint8_t *const stage = smem + warp * 4096;
       T *const narrow = half ? static_cast<T *>(p.dv) : static_cast<T *>(p.dk);
       float *const wide = half ? wide_v : wide_k;
+      const uint32_t t_out = (half ? t_dv : t_dk) + lanes;
+      float odd = 0.f;
 #pragma unroll
-      for (int i = 0; i < DP; i += 32)
-        store_columns<T>((half ? t_dv : t_dk) + lanes, i, dim, narrow ? narrow + out_row : nullptr, wide ? wide + out_row : nullptr);
-      if (half && there && *reinterpret_cast<volatile int *>(&not_finite) && (wide || narrow)) {
-        // dO's infinities and NaN that this key's queries have in border tiles
-        for (int n = 0; n < steps; ++n) {
-          if (!is_border(n)) continue;
-          const int i0 = first + n % tiles * kTile;
-          for (int i = max(i0, from); i < min(i0 + kTile, r.nq); ++i) {
-            const T *o = static_cast<const T *>(p.dout) + ((int64_t)(r.q0 + i) * p.a.heads + head0 + n / tiles) * p.a.dim;
-            for (int c = 0; c < p.a.dim; ++c) {
-              const float v = to_f32<T>(o[c]);
-              if (isfinite(v)) continue;
-              if (wide) wide[out_row + c] += v;
-              else narrow[out_row + c] = from_f32<T>(to_f32<T>(narrow[out_row + c]) + v);
+      for (int i = 0; i < DP; i += 64) {
+        uint32_t packed[32];
+        if (!wide) {
+          odd += pack_columns<T>(t_out + i, i, p.a.dim, true, packed);
+          if (narrow) store_rows(stage, packed, narrow, there ? out_row : -1, i, p.a.dim);
+        } else {
+#pragma unroll
+          for (int h = 0; h < 64; h += 32) {
+            uint32_t o[32];
+            tmem_ld32(t_out + i + h, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int k = 0; k < 32; k += 4) {
+              if (i + h + k >= p.a.dim) continue;
+#pragma unroll
+              for (int c = 0; c < 4; ++c) odd = fmaf(__uint_as_float(o[k + c]), 0.f, odd);
+              if (there)
+                *reinterpret_cast<float4 *>(wide + out_row + i + h + k) =
+                    make_float4(__uint_as_float(o[k]), __uint_as_float(o[k + 1]), __uint_as_float(o[k + 2]), __uint_as_float(o[k + 3]));
             }
           }
         }
+      }
+      __syncwarp();
+      // Keys beside queries that do not see them: those of the tiles before `from`. A key whose first query has a NaN lse is NaN by right.
+      const int begin = max(from, 0);
+      const bool look = there && odd != odd && begin < r.nq && (narrow || wide);
+      for (unsigned rows = __ballot_sync(0xffffffffu, look); rows; rows &= rows - 1) {
+        const int lane_of = __ffs(rows) - 1, at_row = __shfl_sync(0xffffffffu, begin, lane_of), key_of = __shfl_sync(0xffffffffu, key, lane_of);
+        const float lse = p.stats[(int64_t)head0 * p.a.q_rows + r.q0 + at_row].x;
+        if (lse != lse) continue;
+        bool found = false;
+        for (int h = head0; h < head0 + heads && !found; ++h) {
+          const T *q = static_cast<const T *>(p.a.q) + (int64_t)r.q0 * p.a.q_stride[0] + h * p.a.q_stride[1];
+          const T *d = static_cast<const T *>(p.dout) + ((int64_t)r.q0 * p.a.heads + h) * p.a.dim;
+          const int64_t qs = p.a.q_stride[0], ds = (int64_t)p.a.heads * p.a.dim;
+          found = rows_not_finite(half ? d + first * ds : q + first * qs, half ? ds : qs, at_row - first, p.a.dim);
+        }
+        if (!found) continue;
+        float sum[4];
+        redo_dkv<T>(p, r, kv, head0, heads, key_of, at_row, half, sum);
+        const int64_t to = __shfl_sync(0xffffffffu, out_row, lane_of);
+        if (wide) mend4(wide + to, p.a.dim, sum);
+        else mend4(narrow + to, p.a.dim, sum);
       }
     }
     tmem_wait_st();
@@ -661,7 +687,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// lse * log2(e) and scale * delta of every row: a row is `lanes` lanes of 16 bytes.
+// -lse * log2(e) and -scale * delta of every row: a row is `lanes` lanes of 16 bytes.
 template <typename T>
 __global__ void __launch_bounds__(256) stats_kernel(const T *out, const T *dout, const float *lse, float2 *stats, int64_t rows,
                                                     int heads, int64_t tokens, int dim, int lanes, float scale) {
@@ -684,7 +710,7 @@ __global__ void __launch_bounds__(256) stats_kernel(const T *out, const T *dout,
     if (row < rows && lane % lanes == 0) {
       const int64_t t = row / heads;
       const int64_t to = (row - t * heads) * tokens + t;
-      stats[to] = make_float2(lse[to] * 1.4426950408889634f, sum * scale);
+      stats[to] = make_float2(lse[to] * -1.4426950408889634f, sum * -scale);
     }
   }
 }

@@ -18,10 +18,7 @@
 // queries, keys and first S come while this one's softmax ends and O is written. Pairs are launched the longest first and taken
 // over as CTAs get done. All waits go by counts that run on over the pairs.
 //
-// Masks: key j counts for row i where j < seen(i); tiles of keys that some row does not see whole ("border" tiles, the last ones) are masked
-// by columns. A masked weight is 0, but 0 times an infinity or NaN of a value that the row does not see is NaN. So in border tiles the copying
-// warp, which has nothing else to do by then, sets values that are not finite to 0 before the product, and the epilogue adds them back
-// for the rows that see them.
+// Masks: key j counts for row i where j < seen(i); units of keys that some row of a warp does not see whole are masked by columns.
 #include <math.h>
 
 #include <algorithm>
@@ -43,16 +40,14 @@ constexpr int kPoly = 2;                     // exponentials of eight that are p
 template <int DP>
 struct Layout {
   static constexpr uint32_t kTileBytes = DP / 64 * kBox;
-  static constexpr int kStages = DP == 128 ? 5 : 8;
-  static constexpr size_t kBytes = 1024 + (2 + kStages) * (size_t)kTileBytes;
+  static constexpr int kStages = DP == 128 ? 4 : 8;
+  static constexpr uint32_t kStageOut = 8 * 4096;   // of the softmax warps, for O on its way out
+  static constexpr size_t kBytes = 1024 + (2 + kStages) * (size_t)kTileBytes + kStageOut;
 };
 
 // Every wait on a barrier that completes more than once is by someone who has seen the completion before, and whose own next step the
-// one after needs. Border tiles, at most kBorders of them (the rows of a pair see the same keys but for 255), are cleared ahead of
-// that order: each has a barrier of its own, and the next pair's are cleared only once both products' warps have passed these.
-constexpr int kBorders = 3;
-enum { kQFull, kQEmpty, kSFull, kPFull = kSFull + 4, kODone = kPFull + 2, kNext = kODone + 2, kClean = kNext + 2, kDrain = kClean + kBorders,
-       kFull = kDrain + 2 };
+// one after needs.
+enum { kQFull, kQEmpty, kSFull, kPFull = kSFull + 4, kODone = kPFull + 2, kNext = kODone + 2, kLanded, kDrain, kFull = kDrain + 2 };
 template <int DP> constexpr int bars() { return kFull + 2 * Layout<DP>::kStages; }
 
 struct Params {
@@ -72,27 +67,25 @@ struct Work {
   Range r;
   int row[2], head[2], kv;
   int units[2];    // 64 keys that each tile sees any of
-  int border;      // the first tile of keys that some row does not see whole
+  int index;       // in the order of launches; -1: none
   __device__ __forceinline__ int most() const { return max(units[0], units[1]); }
   __device__ __forceinline__ int chunks() const { return (most() + 1) / 2; }   // tiles of keys
 };
 __device__ __forceinline__ Work work_of(const Params &p, int index) {
   const int slot = p.works / p.units - 1 - index / p.units, unit = index % p.units;   // the longest first
-  const int per_slot = p.two_heads ? kTile : 2 * kTile;
-  const Slot s = find_slot(p.a.q_offsets, p.a.sequences, (int)p.a.q_rows, per_slot, slot);
+  const int shift = p.two_heads ? 7 : 8;   // 128 or 256 rows a slot
+  const Place s = place_of<false>(p.a, shift, slot);
   Work w;
-  w.r = slot_range(p.a, s.sequence);
+  w.r = s.r;
   const int group = p.a.heads / p.a.kv_heads;
-  w.border = 1 << 28;   // beyond any tile
+  w.index = index;
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
     w.head[t] = p.two_heads ? 2 * unit + t : unit;
-    w.row[t] = s.group * per_slot + (p.two_heads ? 0 : t * kTile);
+    w.row[t] = (s.group << shift) + (p.two_heads ? 0 : t * kTile);
     w.units[t] = 0;
-    if (s.group >= 0 && w.row[t] < w.r.nq) {
+    if (s.group >= 0 && w.row[t] < w.r.nq)
       w.units[t] = (seen_by(w.r, min(w.row[t] + kTile, w.r.nq) - 1, p.a.causal) + kKeys - 1) / kKeys;
-      if (w.units[t]) w.border = min(w.border, seen_by(w.r, w.row[t], p.a.causal) / kTile);
-    }
   }
   w.kv = w.head[0] / group;
   return w;
@@ -126,6 +119,27 @@ __device__ __forceinline__ float weights(const float (&s)[kKeys], float sc, floa
   return both.x + both.y;
 }
 
+// One row by the definition (a warp).
+template <typename T>
+__device__ __noinline__ void redo_row(const p3d_sequence &a, const Range &r, int head, int row, int seen, T *out) {
+  const int kv = head / (a.heads / a.kv_heads);
+  float q[4], k[4], v[4], o[4] = {0.f, 0.f, 0.f, 0.f}, m = -INFINITY, l = 0.f;
+  load4(static_cast<const T *>(a.q) + (int64_t)(r.q0 + row) * a.q_stride[0] + head * a.q_stride[1], a.dim, q);
+  for (int j = 0; j < seen; ++j) {
+    load4(static_cast<const T *>(a.k) + (int64_t)(r.k0 + j) * a.k_stride[0] + kv * a.k_stride[1], a.dim, k);
+    load4(static_cast<const T *>(a.v) + (int64_t)(r.k0 + j) * a.v_stride[0] + kv * a.v_stride[1], a.dim, v);
+    const float s = dot4(q, k) * a.scale * 1.4426950408889634f, top = max_nan(m, s);
+    const float down = m == -INFINITY ? 0.f : exp2f(m - top), w = top == -INFINITY ? 0.f : exp2f(s - top);
+    l = l * down + w;
+    m = top;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = fmaf(w, v[i], o[i] * down);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[i] /= l;
+  mend4(out, a.dim, o);
+}
+
 template <typename T, int DP>
 __global__ void __launch_bounds__(kThreads, 1)
     sequence_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
@@ -135,10 +149,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t bar_mem[bars<DP>()];
   __shared__ uint32_t tmem_holder;
-  __shared__ int not_finite[2];   // border tiles of a pair (by its number's last bit) hold values that are not
+  __shared__ Work works[2];   // of a pair (by its number's last bit), as the copying warp found it
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  __shared__ __align__(16) uint4 answer[2];
-  Work w = work_of(p, blockIdx.x);
+  __shared__ __align__(16) uint4 answer;
   const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
   uint8_t *const smem = smem_raw + (base - raw);
   const uint32_t ring = base + 2 * L::kTileBytes;
@@ -146,7 +159,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto full = [&](int s) { return bar(kFull + s); };
   auto empty = [&](int s) { return bar(kFull + NS + s); };
   if (threadIdx.x == 0) {
-    not_finite[0] = not_finite[1] = 0;
     for (int i = 0; i < bars<DP>(); ++i)
       mbar_init(bar(i), i == kQEmpty ? 10 : i == kPFull || i == kPFull + 1 ? 4 : i >= kFull + NS ? 2 : 1);
     fence_mbar_init();
@@ -166,28 +178,21 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = tmem_holder;
 
   int done = 0;   // pairs before this one
-  // The number of the pair after this one, or -1 (asked for by the copying warp when it began this one): by whole warps.
-  auto next_work = [&](unsigned role) {
-    if (!wait_warp(bar(kNext + (done & 1)), (done >> 1) & 1, &g_seq_fwd_errors, role)) return -1;
-    const int index = work_given(smem_u32(&answer[done & 1]));
-    fence_proxy_async_smem();   // read before the next answer is written there
-    return index;
-  };
   if (warp == kCopyWarp) {
     // ------------------------------------------------------------------ copies; items K0, V0, K1, V1, .. of one pair after another
     bool ok = true;
-    int item0 = 0, issued = 0;
-    for (int index = blockIdx.x; index >= 0;) {
-      const Work now = w;
-      const int chunks = now.chunks();
-      // the last pair's queries have had their last product and its clearing has been seen; the pair before it is written
+    int item0 = 0, issued = 0, cleared = 0;
+    Work now = work_of(p, blockIdx.x);
+    for (;; ++done) {
+      // the last pair's queries have had their last product, and everybody knows of it
       if (done) ok = __all_sync(0xffffffffu, mbar_wait(bar(kQEmpty), (done - 1) & 1, &g_seq_fwd_errors, kWaitNs, kErrProducer));
       if (!ok) break;
+      const int chunks = now.index < 0 ? 0 : now.chunks();
       if (lane == 0) {
-        ask_for_work(smem_u32(&answer[done & 1]), bar(kNext + (done & 1)));
-        not_finite[done & 1] = 0;
+        works[done & 1] = now;
         if (chunks) mbar_expect_tx(bar(kQFull), 2 * L::kTileBytes);
         else mbar_arrive(bar(kQFull));
+        if (now.index >= 0) ask_for_work(smem_u32(&answer), bar(kNext));
 #pragma unroll
         for (int t = 0; t < 2; ++t)
           for (int c = 0; chunks && c < DP / 64; ++c)
@@ -198,36 +203,34 @@ __global__ void __launch_bounds__(kThreads, 1)
             ok = false;
             break;
           }
-          mbar_expect_tx(full(s), L::kTileBytes);
+          // the last values, where their tile goes past the sequence's end, land on a barrier of their own
+          const uint32_t on = (i - item0) % 2 && (c + 1) * kTile > now.r.nk ? bar(kLanded) : full(s);
+          mbar_expect_tx(on, L::kTileBytes);
           for (int k = 0; k < DP / 64; ++k)
-            tma_load_3d(ring + s * L::kTileBytes + k * kBox, (i - item0) % 2 ? &tv : &tk, full(s), 64 * k, now.kv, now.r.k0 + c * kTile);
+            tma_load_3d(ring + s * L::kTileBytes + k * kBox, (i - item0) % 2 ? &tv : &tk, on, 64 * k, now.kv, now.r.k0 + c * kTile);
           issued = i + 1;
         }
       }
       ok = __all_sync(0xffffffffu, ok);
-      // values of the border tiles that are not finite
-#pragma unroll
-      for (int b = 0; b < kBorders; ++b) {
-        const int c = now.border + b, i = item0 + 2 * c + 1, s = i % NS;
-        if (!ok || c >= chunks) continue;
-        ok = __all_sync(0xffffffffu, mbar_wait(full(s), (i / NS) & 1, &g_seq_fwd_errors, kWaitNs, kErrProducer));
-        if (!ok) continue;
-        if (clear_not_finite<T>(smem + (2 + s) * L::kTileBytes, L::kTileBytes)) {
-          fence_proxy_async_smem();
-          if (lane == 0) not_finite[done & 1] = 1;
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(kClean + b));
+      if (ok && chunks * kTile > now.r.nk && chunks) {
+        const int s = (item0 + 2 * chunks - 1) % NS;
+        ok = wait_warp(bar(kLanded), cleared++ & 1, &g_seq_fwd_errors, kErrProducer);
+        if (!ok) break;
+        clear_rows<DP / 64>(smem + (2 + s) * L::kTileBytes, now.r.nk - (chunks - 1) * kTile);
+        if (lane == 0) mbar_arrive(full(s));
       }
       item0 += 2 * chunks;
-      index = next_work(kErrProducer);
-      ++done;
+      if (now.index < 0) break;
+      ok = wait_warp(bar(kNext), done & 1, &g_seq_fwd_errors, kErrProducer) && ok;
       if (!ok) break;
-      if (index >= 0) w = work_of(p, index);
+      const int index = work_given(smem_u32(&answer));
+      fence_proxy_async_smem();   // read before the next answer is written there
+      if (index >= 0) now = work_of(p, index);
+      else now.index = -1;
     }
     // no copy in flight into memory that is about to be given up
     if (lane == 0) {
-      if (done) mbar_wait(bar(kQFull), (done - 1) & 1, &g_seq_fwd_errors, kWaitNs, kErrTeardown);
+      if (issued) mbar_wait(bar(kQFull), done & 1, &g_seq_fwd_errors, kWaitNs, kErrTeardown);
       for (int i = max(0, issued - NS); i < issued; ++i)
         mbar_wait(full(i % NS), (i / NS) & 1, &g_seq_fwd_errors, kWaitNs, kErrTeardown);
     }
@@ -241,24 +244,21 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint64_t desc_q = desc_rows(base + t * L::kTileBytes), desc_k = desc_rows(ring), desc_v = desc_cols(ring);
     const uint32_t t_s = tmem + kColS + 128 * t, t_o = tmem + kColO + 128 * t;
     int n_s = 0, n_o = 0;                  // products of this tile so far
-    int item0 = 0, landed = 0, cleared[kBorders] = {};
+    int item0 = 0, landed = 0;
     int give_back = -1;                    // the items whose last readers are under way: this one and the next
     bool waited = true;                    // the last O has been waited for
     auto wait = [&](uint32_t b, uint32_t parity) { return wait_warp(b, parity, &g_seq_fwd_errors, kErrMma); };
     bool ok = true;
-    for (int index = blockIdx.x; index >= 0;) {
-      const Work now = w;
-      const int units = now.most(), mine = t ? now.units[1] : now.units[0], chunks = now.chunks();
-      // item i is there (and, for values of a border tile, cleared); items are waited for in order, once
+    for (;; ++done) {
+      ok = wait(bar(kQFull), done & 1);
+      if (!ok) break;
+      const Work &now = works[done & 1];
+      if (now.index < 0) break;
+      const int units = now.most(), mine = now.units[t];
+      // item i is there; items are waited for in order, once
       auto wait_item = [&](int i) {
-        for (; landed <= i; ++landed) {
+        for (; landed <= i; ++landed)
           if (!wait(full(landed % NS), (landed / NS) & 1)) return false;
-          const int b = (landed - item0) / 2 - now.border;
-          if ((landed - item0) % 2 && b >= 0) {
-            const int phase = b == 0 ? cleared[0] : b == 1 ? cleared[1] : cleared[2];
-            if (!wait(bar(kClean + b), phase & 1)) return false;
-          }
-        }
         return true;
       };
       // S of unit u: into the buffer that S two before was in
@@ -279,10 +279,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         ++n_o;
         waited = false;
       };
-      ok = wait(bar(kQFull), done & 1) && (!units || wait_item(item0));
+      ok = !units || wait_item(item0);
       if (ok && mine) issue_s(0);
-      index = next_work(kErrMma);
-      if (index >= 0) w = work_of(p, index);
       for (int u = 0; ok && u < units; ++u) {
         // The last O is there, and with it its S: their keys and values may go. By a plain arrival: a commit after another one's
         // waits until the pipe has run dry. A tile that is done, or has no rows, arrives for what has landed.
@@ -309,11 +307,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (u & 1 || u == units - 1) give_back = item0 + u / 2 * 2;
       }
       if (!ok) break;
+      item0 += (units + 1) / 2 * 2;
       if (lane == 0) mbar_arrive(bar(kQEmpty));
-#pragma unroll
-      for (int b = 0; b < kBorders; ++b) cleared[b] += now.border + b < chunks;
-      item0 += 2 * chunks;
-      ++done;
     }
     // every product completed and every commit arrived before tensor memory and barriers are given up
     mma_commit_warp(bar(kDrain + t));
@@ -332,19 +327,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     const float sc = p.sc;
     int n = 0;   // steps of this tile so far
     bool ok = true;
-    for (int index = blockIdx.x; index >= 0;) {
-      const Work now = w;
+    uint8_t *const stage = smem + (2 + NS) * L::kTileBytes + warp * 4096;
+    for (;; ++done) {
+      // After the wait for a pair's queries, which come only when every warp has said that it knows of the pair before: no warp, with
+      // rows or without, is a pair ahead.
+      ok = wait_warp(bar(kQFull), done & 1, &g_seq_fwd_errors, kErrSoftmax);
+      if (!ok) break;
+      const Work now = works[done & 1];
+      if (now.index < 0) break;
       const int mine = t ? now.units[1] : now.units[0], head = t ? now.head[1] : now.head[0], row0 = t ? now.row[1] : now.row[0];
       const int row = row0 + (warp % 4) * 32 + lane;
       const bool there = row0 >= 0 && row < now.r.nq;
       const int seen = there ? seen_by(now.r, row, p.a.causal) : 0;
-      // The pair before is written. After the wait for this one's queries, which come only when every warp has said so for the
-      // pair before: no warp, with rows or without, is a pair ahead.
-      ok = wait_warp(bar(kQFull), done & 1, &g_seq_fwd_errors, kErrSoftmax);
-      if (!ok) break;
+      __syncwarp();
       if (lane == 0) mbar_arrive(bar(kQEmpty));
-      index = next_work(kErrSoftmax);
-      if (index >= 0) w = work_of(p, index);
       float m = -INFINITY, l = 0.f;
       for (int u = 0; u < mine; ++u, ++n) {
         const uint32_t t_u = t_s + 64 * (n & 1);
@@ -412,45 +408,43 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (mine) ok = wait_warp(bar(kODone + t), (n - 1) & 1, &g_seq_fwd_errors, kErrSoftmax);
       if (!ok) break;
       const float inv = seen > 0 ? 1.f / l : 0.f;
-      const int64_t at = (int64_t)(now.r.q0 + row) * p.a.heads + head;
-      T *out = static_cast<T *>(p.out) + at * p.a.dim;
-      // what the copying warp says of this pair's values: written before the last O was made
-      const bool add_back = (mine + 1) / 2 > now.border && *reinterpret_cast<volatile int *>(&not_finite[done & 1]) != 0;
+      const int64_t at = there ? ((int64_t)(now.r.q0 + row) * p.a.heads + head) * p.a.dim : -1;
+      T *const out = static_cast<T *>(p.out);
+      float odd = 0.f;   // NaN where any of the row is not finite
 #pragma unroll
-      for (int i = 0; i < DP; i += 32) {
+      for (int i = 0; i < DP; i += 64) {
         if (i >= p.a.dim) continue;
-        uint32_t o[32];
-        if (mine) {
-          tmem_ld32(t_o + i, o);
-          tmem_wait_ld();
-        }
+        uint32_t packed[32];
 #pragma unroll
-        for (int k = 0; k < 32; ++k) o[k] = seen > 0 ? __float_as_uint(__uint_as_float(o[k]) * inv) : 0u;
-        if (add_back && seen > 0) {
-          for (int j = now.border * kTile; j < seen; ++j) {
-            const T *v = static_cast<const T *>(p.a.v) + (int64_t)(now.r.k0 + j) * p.a.v_stride[0] + now.kv * p.a.v_stride[1];
+        for (int h = 0; h < 64; h += 32) {
+          uint32_t o[32];
+          if (mine) {
+            tmem_ld32(t_o + i + h, o);
+            tmem_wait_ld();
+          }
 #pragma unroll
-            for (int k = 0; k < 32; ++k) {
-              const float x = i + k < p.a.dim ? to_f32<T>(v[i + k]) : 0.f;
-              if (!isfinite(x)) o[k] = __float_as_uint(__uint_as_float(o[k]) + x);
-            }
+          for (int k = 0; k < 32; k += 2) {
+            const float a = seen > 0 ? __uint_as_float(o[k]) * inv : 0.f, b = seen > 0 ? __uint_as_float(o[k + 1]) * inv : 0.f;
+            if (i + h + k < p.a.dim) odd = fmaf(a, 0.f, fmaf(b, 0.f, odd));
+            packed[(h + k) / 2] = pack<T>(a, b);
           }
         }
-        if (there) {
-#pragma unroll
-          for (int k = 0; k < 32; k += 8)
-            if (i + k < p.a.dim)
-              *reinterpret_cast<uint4 *>(out + i + k) =
-                  make_uint4(pack<T>(__uint_as_float(o[k]), __uint_as_float(o[k + 1])),
-                             pack<T>(__uint_as_float(o[k + 2]), __uint_as_float(o[k + 3])),
-                             pack<T>(__uint_as_float(o[k + 4]), __uint_as_float(o[k + 5])),
-                             pack<T>(__uint_as_float(o[k + 6]), __uint_as_float(o[k + 7])));
-        }
+        store_rows(stage, packed, out, at, i, p.a.dim);
       }
       if (p.lse && there)
         p.lse[(int64_t)head * p.a.q_rows + now.r.q0 + row] = seen > 0 ? (m * sc + log2f(l)) * 0.6931471805599453f : -INFINITY;
+      // rows with an infinity or NaN, in a unit with keys that they do not see; where the last key that they see is NaN they are right
+      const int past = min(mine * kKeys, now.r.nk);
+      for (unsigned rows = __ballot_sync(0xffffffffu, there && odd != odd && seen > 0 && seen < past); rows; rows &= rows - 1) {
+        const int from = __ffs(rows) - 1, first = __shfl_sync(0xffffffffu, seen, from);
+        const T *v = static_cast<const T *>(p.a.v) + (int64_t)(now.r.k0 + first) * p.a.v_stride[0] + now.kv * p.a.v_stride[1];
+        float last[4];
+        load4(v - p.a.v_stride[0], p.a.dim, last);
+        const bool right = last[0] != last[0] && last[1] != last[1] && last[2] != last[2] && last[3] != last[3];
+        if (__all_sync(0xffffffffu, right || lane * 4 >= p.a.dim) || !rows_not_finite(v, p.a.v_stride[0], past - first, p.a.dim)) continue;
+        redo_row<T>(p.a, now.r, head, __shfl_sync(0xffffffffu, row, from), first, out + __shfl_sync(0xffffffffu, at, from));
+      }
       tc_fence_before();   // O is read before the next pair's P lets a product write it
-      ++done;
     }
     tmem_wait_st();
   }

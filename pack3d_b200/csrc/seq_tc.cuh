@@ -16,6 +16,10 @@ constexpr int kTile = 128;                       // rows of an operand tile
 constexpr uint32_t kBox = kTile * 128;           // bytes of one TMA box: 128 rows of 64 columns, SWIZZLE_128B
 constexpr uint64_t kWaitNs = 2000000000ull;      // every wait is bounded: 2 s
 
+template <typename T> __device__ __forceinline__ uint32_t pack(float a, float b) {
+  return std::is_same<T, __half>::value ? pack_f16(a, b) : pack_bf16(a, b);
+}
+
 // Columns of a head rounded up to whole boxes; a box's columns past dim are zero-filled by the copy.
 constexpr int padded(int dim) { return dim <= 64 ? 64 : 128; }
 
@@ -30,32 +34,35 @@ __device__ __forceinline__ uint64_t desc_cols(uint32_t tile) {
 }
 __device__ __forceinline__ uint32_t step_cols(int k) { return (uint32_t)(k * 16 * 128) >> 4; }
 
-// Which sequence a slot belongs to, and which of its groups of `rows` rows: a sequence b that begins at row o_b has the slots from
-// o_b / rows + b on, one more than it can need; the rows behind the last sequence are sequence `sequences`. All lanes of a warp
-// take part and search 32 ways at a time.
-struct Slot {
-  int sequence, group;
+// Which sequence a slot belongs to, its rows, and which of its groups of 2^shift rows the slot is: a sequence b that begins at row o_b
+// has the slots from o_b / 2^shift + b on, one more than it can need; the rows behind the last sequence are sequence
+// `sequences`, without rows on the other side. By queries, or by keys. All lanes of a warp take part and search 32 ways at a
+// time; the last round brings both sides' offsets, so that up to 30 sequences cost one memory latency.
+struct Place {
+  Range r;
+  int group;
 };
-__device__ __forceinline__ Slot find_slot(const int32_t *offsets, int sequences, int total, int rows, int slot) {
-  int lo = 0, n = sequences + 1;   // the answer is one of lo .. lo + n - 1; the one at lo qualifies
+template <bool kByKeys>
+__device__ __forceinline__ Place place_of(const p3d_sequence &a, int shift, int slot) {
+  const int32_t *const mine = kByKeys ? a.k_offsets : a.q_offsets, *const other = kByKeys ? a.q_offsets : a.k_offsets;
+  const int total = (int)(kByKeys ? a.k_rows : a.q_rows), other_total = (int)(kByKeys ? a.q_rows : a.k_rows);
+  int lo = 0, n = a.sequences + 1;   // the answer is one of lo .. lo + n - 1; the one at lo qualifies
   const int lane = threadIdx.x & 31;
-  while (n > 1) {
+  while (n > 31) {
     const int step = (n + 31) / 32, at = lane * step;
-    const bool in = at < n && (lane == 0 || cache::offset_at(offsets, lo + at, total) / rows + lo + at <= slot);
+    const bool in = at < n && (lane == 0 || (cache::offset_at(mine, lo + at, total) >> shift) + lo + at <= slot);
     const int last = 31 - __clz(__ballot_sync(0xffffffffu, in));
     lo += last * step;
     n = min(step, n - last * step);
   }
-  return {lo, slot - (cache::offset_at(offsets, lo, total) / rows + lo)};
-}
-// Its rows; those of the last, empty one see no keys.
-__device__ __forceinline__ Range slot_range(const p3d_sequence &a, int b) {
-  if (b < a.sequences) return range_of(a, b);
-  Range r = {};
-  r.q0 = cache::offset_at(a.q_offsets, b, (int)a.q_rows);
-  r.nq = (int)a.q_rows - r.q0;
-  r.k0 = cache::offset_at(a.k_offsets, b, (int)a.k_rows);
-  return r;
+  const int at = min(lo + lane, a.sequences);
+  const int m = cache::offset_at(mine, at, total), o = cache::offset_at(other, at, other_total);
+  const bool in = lane < n && (lane == 0 || (m >> shift) + lo + lane <= slot);
+  const int last = 31 - __clz(__ballot_sync(0xffffffffu, in)), b = lo + last;
+  const int m0 = __shfl_sync(0xffffffffu, m, last), m1 = b < a.sequences ? __shfl_sync(0xffffffffu, m, last + 1) : total;
+  const int o0 = __shfl_sync(0xffffffffu, o, last), o1 = b < a.sequences ? __shfl_sync(0xffffffffu, o, last + 1) : o0;
+  const int mn = max(m1 - m0, 0), on = max(o1 - o0, 0);
+  return {kByKeys ? Range{o0, on, m0, mn} : Range{m0, mn, o0, on}, slot - ((m0 >> shift) + b)};
 }
 inline int64_t slots_of(int64_t rows, int sequences, int per_slot) { return rows / per_slot + sequences + 1; }
 
@@ -88,9 +95,6 @@ __device__ __forceinline__ int work_given(uint32_t slot) {
   return index;
 }
 
-template <typename T> __device__ __forceinline__ uint32_t pack(float a, float b) {
-  return std::is_same<T, __half>::value ? pack_f16(a, b) : pack_bf16(a, b);
-}
 
 // The larger, NaN if either is: a NaN score makes its row's maximum NaN, and with it all that the row gives.
 __device__ __forceinline__ float max_nan(float a, float b) {
@@ -104,32 +108,77 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   return d;
 }
 
-// Elements of a tile that are not finite become 0 (a warp; `bytes` of it). A product with a weight of 0 would make them NaN in rows
-// that do not see them. Returns whether there were any. Bits: the exponent is all ones where adding one to its last place
-// carries into the sign's place.
+// Masked weights and values that are not finite.  A masked weight is 0, but 0 times an infinity or NaN is NaN: a product over a whole tile
+// would pass on what a row does not see.
+// * Rows of a tile behind the end of its sequence (another sequence's, or memory that nobody filled) are set to 0 before the products
+//   read the tile: by the copying warp, which has it land on a barrier of its own (clear_rows).
+// * Within a sequence, what lies behind a row's last key shows in the result. Rows whose result is not finite, and beside whose keys
+//   (queries) in the tile there is such a value that they do not see, have those columns made again by their definition, a warp to a
+//   row (rows_not_finite, mend4, and the redo functions of each kernel). Nothing is paid for that where all is finite.
+template <int kBoxes>
+__device__ __forceinline__ void clear_rows(uint8_t *tile, int first) {
+  for (int i = threadIdx.x & 31; i < (kTile - first) * 8; i += 32)
+#pragma unroll
+    for (int b = 0; b < kBoxes; ++b) *reinterpret_cast<uint4 *>(tile + b * kBox + first * 128 + i * 16) = make_uint4(0, 0, 0, 0);
+  fence_proxy_async_smem();
+  __syncwarp();
+}
+__device__ __forceinline__ bool not_finite(float v) { return (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u; }
+
+// Four columns of a row for each lane.
 template <typename T>
-__device__ __forceinline__ bool clear_not_finite(uint8_t *tile, int bytes) {
-  constexpr uint32_t one = std::is_same<T, __half>::value ? 0x04000400u : 0x00800080u;
-  const int lane = threadIdx.x & 31;
+__device__ __forceinline__ void load4(const T *row, int dim, float (&v)[4]) {
+  const int c = (threadIdx.x & 31) * 4;
+  if (c < dim) {   // dim is a multiple of 8, rows are 16-byte aligned
+    const uint2 w = *reinterpret_cast<const uint2 *>(row + c);
+    const float2 a = unpack2<T>(w.x), b = unpack2<T>(w.y);
+    v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
+  } else {
+    v[0] = v[1] = v[2] = v[3] = 0.f;
+  }
+}
+__device__ __forceinline__ float dot4(const float (&a)[4], const float (&b)[4]) {
+  return warp_sum(a[0] * b[0] + a[1] * b[1] + a[2] * b[2] + a[3] * b[3]);
+}
+// Into the places of a row whose value is not finite.
+template <typename T>
+__device__ __forceinline__ void mend4(T *row, int dim, const float (&v)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int c = (threadIdx.x & 31) * 4 + i;
+    if (c < dim && not_finite(to_f32<T>(row[c]))) row[c] = from_f32<T>(v[i]);
+  }
+}
+// Whether any of `rows` rows from `from` on, `stride` elements apart, is not finite (by a warp).
+template <typename T>
+__device__ __forceinline__ bool rows_not_finite(const T *from, int64_t stride, int rows, int dim) {
   bool found = false;
-  for (int i = lane; i < bytes / 16; i += 32 * 4) {
-    uint4 w[4];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) w[u] = reinterpret_cast<const uint4 *>(tile)[i + 32 * u];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const uint32_t m[4] = {(w[u].x & 0x7fff7fffu) + one, (w[u].y & 0x7fff7fffu) + one, (w[u].z & 0x7fff7fffu) + one,
-                             (w[u].w & 0x7fff7fffu) + one};
-      if ((m[0] | m[1] | m[2] | m[3]) & 0x80008000u) {
-        found = true;
-        auto keep = [](uint32_t v, uint32_t odd) {
-          return v & ((odd & 0x8000u ? 0u : 0xffffu) | (odd & 0x80000000u ? 0u : 0xffff0000u));
-        };
-        reinterpret_cast<uint4 *>(tile)[i + 32 * u] = make_uint4(keep(w[u].x, m[0]), keep(w[u].y, m[1]), keep(w[u].z, m[2]), keep(w[u].w, m[3]));
-      }
-    }
+  for (int j = 0; j < rows; ++j) {
+    float v[4];
+    load4(from + j * stride, dim, v);
+    found |= not_finite(v[0]) || not_finite(v[1]) || not_finite(v[2]) || not_finite(v[3]);
   }
   return __any_sync(0xffffffffu, found);
+}
+
+// A warp's 32 rows (a row a lane, 64 columns of 16 bits as 32 words) to memory by way of shared memory, whole lines at a time: `stage` is
+// the warp's own 4 KB. Lane i's row is at `row` elements from `out` where it is not negative; columns from `dim` on are left out.
+template <typename T>
+__device__ __forceinline__ void store_rows(uint8_t *stage, const uint32_t (&w)[32], T *out, int64_t row, int col, int dim) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    *reinterpret_cast<uint4 *>(stage + lane * 128 + ((i ^ (lane & 7)) * 16)) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+  __syncwarp();
+  const int chunk = lane & 7;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = i * 4 + lane / 8;
+    const int64_t to = __shfl_sync(0xffffffffu, row, r);
+    const uint4 v = *reinterpret_cast<const uint4 *>(stage + r * 128 + ((chunk ^ (r & 7)) * 16));
+    if (to >= 0 && col + chunk * 8 < dim) *reinterpret_cast<uint4 *>(out + to + col + chunk * 8) = v;
+  }
+  __syncwarp();
 }
 
 // The tensor map of [rows, heads, dim] with strides in elements: boxes of 64 columns of 128 rows of one head.

@@ -9,6 +9,14 @@ pytestmark = pytest.mark.gpu
 BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
 
 
+@pytest.fixture(autouse=True)
+def no_wait_ran_out():
+    """No bounded wait of a kernel gave up."""
+    yield
+    from pack3d_b200 import _native
+    assert _native.device_errors() == 0
+
+
 def half_step(dtype):
     return torch.finfo(dtype).eps / 2
 
@@ -217,38 +225,56 @@ def test_what_nobody_sees_changes_nothing(cuda_device, value, dim):
 @pytest.mark.parametrize("which", ["k", "v"])
 @pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
 @pytest.mark.parametrize("at", [0, 100, 127, 128, 290])
-def test_what_comes_later_is_not_seen(cuda_device, which, value, at):
-    """Causal: a key or value that is not finite reaches the queries from its own on, and none before."""
+@pytest.mark.parametrize("dim", [64, 128])
+def test_what_comes_later_is_not_seen(cuda_device, which, value, at, dim):
+    """Causal: a key or value that is not finite reaches the queries from its own on, and none before: bit for bit, but in the value's own
+    column of the queries whose tile of keys it lies in, which is made another way."""
     n = 300
-    q, k, v, dout = make([n], [n], 2, 1, 64, BF16, cuda_device)
+    q, k, v, dout = make([n], [n], 2, 1, dim, BF16, cuda_device)
     clean, _ = run(q, k, v, dout, [n], [n], True)
+    want, tol, _, _ = reference(q, k, v, [n], [n], True, dim ** -0.5)
     (k if which == "k" else v)[at, 0, 3] = value
     out, _ = run(q, k, v, dout, [n], [n], True)
-    assert torch.equal(out[:at], clean[:at])
+    keep = torch.arange(dim, device=cuda_device) != 3
+    assert torch.equal(out[:at][..., keep], clean[:at][..., keep])
+    check(out[:at], want[:at], tol[:at], "out")
     if which == "v":
-        want = torch.full_like(out[at:, :, 3], value)
-        assert torch.equal(out[at:, :, 3].isnan(), want.isnan())
-        assert math.isnan(value) or torch.equal(out[at:, :, 3], want)
-        keep = torch.arange(64, device=cuda_device) != 3
+        filled = torch.full_like(out[at:, :, 3], value)
+        assert torch.equal(out[at:, :, 3].isnan(), filled.isnan())
+        assert math.isnan(value) or torch.equal(out[at:, :, 3], filled)
         assert torch.equal(out[at:][..., keep], clean[at:][..., keep])
-    elif math.isnan(value):
-        assert out[at:].isnan().all()
+    else:
+        assert torch.equal(out[:at], clean[:at])
+        assert not math.isnan(value) or out[at:].isnan().all()
 
 
 @pytest.mark.parametrize("which", ["q", "k", "v", "dout"])
 @pytest.mark.parametrize("at", [0, 100, 255])
-def test_gradients_of_queries_before_a_nan(cuda_device, which, at):
+@pytest.mark.parametrize("heads,kv,dim", [(2, 1, 64), (2, 2, 128)])
+def test_gradients_of_queries_before_a_nan(cuda_device, which, at, heads, kv, dim):
     n = 300
-    tensors = dict(zip(("q", "k", "v", "dout"), make([n], [n], 2, 1, 64, BF16, cuda_device)))
+    tensors = dict(zip(("q", "k", "v", "dout"), make([n], [n], heads, kv, dim, BF16, cuda_device)))
     _, clean = run(*tensors.values(), [n], [n], True)
+    _, _, want, tol = reference(tensors["q"], tensors["k"], tensors["v"], [n], [n], True, dim ** -0.5, tensors["dout"])
     tensors[which][at] = math.nan
     _, grads = run(*tensors.values(), [n], [n], True)
-    assert torch.equal(grads[0][:at], clean[0][:at])
+    tile = at // 128 * 128
+    assert torch.equal(grads[0][:tile], clean[0][:tile])
+    check(grads[0][:at], want[0][:at], tol[0][:at], "dq")
     # keys after a query's own see nothing of it; those up to it get NaN
     if which in ("q", "dout"):
         for i in (1, 2):
-            assert torch.equal(grads[i][at + 1:], clean[i][at + 1:])
+            assert torch.equal(grads[i][tile + 128:], clean[i][tile + 128:])
+            check(grads[i][at + 1:], want[i][at + 1:], tol[i][at + 1:], "dk, dv")
             assert grads[i][:at + 1].isnan().any(-1).all()
+
+
+def test_all_nan(cuda_device):
+    """Nothing but NaN: quick, and NaN."""
+    n = 3000
+    q, k, v, dout = (torch.full_like(t, math.nan) for t in make([n], [n], 4, 2, 64, BF16, cuda_device))
+    out, grads = run(q, k, v, dout, [n], [n], True)
+    assert out.isnan().all() and all(g.isnan().all() for g in grads)
 
 
 def test_gradients_against_differences(cuda_device):
