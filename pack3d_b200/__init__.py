@@ -16,9 +16,10 @@ from .ops import pack3d_streamed
 from .residual import NormSpec, dropout, norm, residual_norm
 from .rope import balanced_pairs, rotate_projections
 from .sequence import norm_rotate, sequence_attention
+from .sequence_layer import SequenceAttention
 
 __version__ = "0.1.0"
-__all__ = ["FeedForward", "Fp8Matrix", "NormSpec", "PACK3DAttention", "Pack3DGeometry", "PagedCache", "TokenLayout",
-           "balanced_pairs", "build_layout", "dropout", "fp8_linear", "fp8_matmul", "grid_coordinates", "norm",
-           "norm_rotate", "pack3d_streamed", "paged_attention", "prepare_geometry", "quantize", "quantize_weight",
-           "residual_norm", "rotate_projections", "sequence_attention"]
+__all__ = ["FeedForward", "Fp8Matrix", "NormSpec", "PACK3DAttention", "Pack3DGeometry", "PagedCache",
+           "SequenceAttention", "TokenLayout", "balanced_pairs", "build_layout", "dropout", "fp8_linear", "fp8_matmul",
+           "grid_coordinates", "norm", "norm_rotate", "pack3d_streamed", "paged_attention", "prepare_geometry",
+           "quantize", "quantize_weight", "residual_norm", "rotate_projections", "sequence_attention"]
