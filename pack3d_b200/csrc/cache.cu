@@ -7,9 +7,14 @@
 // token is written once and its neighbours in the page never change.
 //
 // Bound by HBM: each value is read once and written once. A row (token, head, key or value) is S = dim / 8 lanes (up to a power
-// of two), 32 / S rows a pass, four passes of loads in flight. What page a token goes to is a chain of loads (offsets, start,
-// table), so a warp takes up to 32 consecutive tokens, each lane follows the chain for one of them, and the places are handed
-// round by shuffles.
+// of two), and a pass is 32 / S rows. What page a token goes to is a chain of loads (offsets, start, table), so a warp takes up to
+// 32 consecutive tokens, each lane follows the chain for one of them, and the places are handed round by shuffles. Tokens and
+// heads are cut so that the warps that the device holds have about one item each.
+//
+// A kernel reads in the order in which its input lies: append takes the heads of one token (four passes in flight), read takes
+// consecutive tokens of one head, which are neighbours in a page (eight). At 45,000 tokens of 8
+// heads of 128 between bf16 and 8 bits (277 MB each) append takes 54 us, 5.1 TB/s (by tokens of one head 107), and read 66 us,
+// 4.2 TB/s (by heads of one token 83). What is left in both is the wait for loads: 64 registers leave an SM 32 warps.
 #include "cache.cuh"
 
 #include <cuda_fp8.h>
@@ -24,7 +29,8 @@ namespace {
 
 __device__ unsigned g_cache_errors = 0;
 
-constexpr int kWarps = 8, kPasses = 4;
+constexpr int kWarps = 8, kAppendPasses = 4;
+constexpr int read_passes(int s) { return s < 8 ? s : 8; }
 
 struct Params {
   p3d_cache c;
@@ -34,7 +40,7 @@ struct Params {
   const int32_t *starts, *offsets;
   int rows;          // packed rows
   int run;           // tokens of a warp's item
-  int chunks;        // groups of kPasses passes that a token's 2 * kv_heads rows take
+  int group, groups; // its rows of each of them, and how many such groups the 2 * kv_heads rows make
   int shift;         // log2 of the lanes of a row
 };
 
@@ -53,58 +59,62 @@ __device__ __forceinline__ cache::Place find(const Params &p, int t) {
   return place;
 }
 
-// Row (token's place, head, key or value) of the pages.
-__device__ __forceinline__ int64_t page_row(const Params &p, int page, int row, int head) {
-  return ((int64_t)page * p.c.kv_heads + head) * p.c.page_size + row;
-}
-
-template <typename T, bool k8>
-__global__ void __launch_bounds__(kWarps * 32) append_kernel(const __grid_constant__ Params p) {
-  const int lane = threadIdx.x & 31, col = (lane & ((1 << p.shift) - 1)) * 8, rows = 2 * p.c.kv_heads;
-  const int per_pass = 32 >> p.shift;
-  const int64_t items = (int64_t)((p.rows + p.run - 1) / p.run) * p.chunks;
+// S: lanes of a row.
+template <typename T, bool k8, int S>
+__global__ void __launch_bounds__(kWarps * 32, 4) append_kernel(const __grid_constant__ Params p) {
+  constexpr int U = kAppendPasses, kPerPass = 32 / S;
+  const int lane = threadIdx.x & 31, col = lane % S * 8, rows = 2 * p.c.kv_heads;
+  const int64_t items = (int64_t)((p.rows + p.run - 1) / p.run) * p.groups;
   for (int64_t item = (int64_t)blockIdx.x * kWarps + threadIdx.x / 32; item < items; item += (int64_t)gridDim.x * kWarps) {
-    const int run = (int)(item / p.chunks), t0 = run * p.run;
-    const int first = (int)(item - (int64_t)run * p.chunks) * kPasses * per_pass + (lane >> p.shift);
+    const int run = (int)(item / p.groups), t0 = run * p.run;
+    const int first = (int)(item - (int64_t)run * p.groups) * U * kPerPass + lane / S;
     const cache::Place mine = find(p, lane < p.run ? t0 + lane : p.rows);
+    // a lane's rows of every token of the run: the same heads
+    const T *in[U];
+    int64_t to[U];   // row of the pages, less the page and the place in it
+    bool on[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int r = first + u * kPerPass, which = r >= p.c.kv_heads, head = r - which * p.c.kv_heads;
+      on[u] = r < rows && col < p.c.dim;
+      to[u] = (int64_t)head * p.c.page_size;
+      in[u] = static_cast<const T *>(which ? p.in[1] : p.in[0]) + (int64_t)t0 * (which ? p.token_stride[1] : p.token_stride[0]) +
+              head * (which ? p.head_stride[1] : p.head_stride[0]) + col;
+    }
     for (int i = 0; i < p.run && t0 + i < p.rows; ++i) {
       const int page = __shfl_sync(0xffffffffu, mine.page, i), at = __shfl_sync(0xffffffffu, mine.row, i);
-      if (page < 0) continue;
-      quant::Raw<T> raw[kPasses];
+      quant::Raw<T> raw[U];
 #pragma unroll
-      for (int u = 0; u < kPasses; ++u) {
-        const int r = first + u * per_pass, which = r >= p.c.kv_heads, head = r - which * p.c.kv_heads;
-        const T *row = static_cast<const T *>(which ? p.in[1] : p.in[0]) +
-                       (int64_t)(t0 + i) * (which ? p.token_stride[1] : p.token_stride[0]) +
-                       head * (which ? p.head_stride[1] : p.head_stride[0]);
-        raw[u] = quant::load8<T, true>(row, col, r < rows ? p.c.dim : 0);
+      for (int u = 0; u < U; ++u) {
+        raw[u] = quant::load8<T, true>(in[u], 0, on[u] && page >= 0 ? 8 : 0);
+        in[u] += first + u * kPerPass >= p.c.kv_heads ? p.token_stride[1] : p.token_stride[0];
       }
+      if (page < 0) continue;
+      const int64_t place = (int64_t)page * p.c.kv_heads * p.c.page_size + at;
 #pragma unroll
-      for (int u = 0; u < kPasses; ++u) {
-        const int r = first + u * per_pass, which = r >= p.c.kv_heads, head = r - which * p.c.kv_heads;
-        const int64_t to = page_row(p, page, at, head);
-        const bool write = r < rows && col < p.c.dim;
+      for (int u = 0; u < U; ++u) {
+        const bool values = first + u * kPerPass >= p.c.kv_heads;
         if constexpr (k8) {
           uint32_t m = quant::largest8<T>(raw[u]);
 #pragma unroll
-          for (int o = 16; o > 0; o >>= 1)
-            if (o < 1 << p.shift) m = quant::larger<T>(m, __shfl_xor_sync(0xffffffffu, m, o));
-          if (__any_sync(0xffffffffu, quant::infinite<T>(m))) {
+          for (int o = S / 2; o > 0; o >>= 1) m = quant::larger<T>(m, __shfl_xor_sync(0xffffffffu, m, o));
+          const bool odd = __any_sync(0xffffffffu, quant::infinite<T>(m));   // infinities or NaN among the warp's rows
+          if (odd) {
             m = quant::finite_largest8<T>(raw[u]);
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1)
-              if (o < 1 << p.shift) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+            for (int o = S / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
           } else {
             m = quant::widest<T>(m);
           }
           const uint32_t byte = m ? quant::scale_byte(m) : 1u;
-          if (write) {
-            *reinterpret_cast<uint2 *>(static_cast<uint8_t *>(which ? p.c.v : p.c.k) + to * p.c.dim + col) =
-                quant::quantize8<true, T>(raw[u], quant::inverse_scale(byte));
-            if (col == 0) (which ? p.c.v_scales : p.c.k_scales)[to] = (uint8_t)byte;
+          const float inv = quant::inverse_scale(byte);
+          const uint2 w = odd ? quant::quantize8<true, T>(raw[u], inv) : quant::quantize8<false, T>(raw[u], inv);
+          if (on[u]) {
+            *reinterpret_cast<uint2 *>(static_cast<uint8_t *>(values ? p.c.v : p.c.k) + (place + to[u]) * p.c.dim + col) = w;
+            if (col == 0) (values ? p.c.v_scales : p.c.k_scales)[place + to[u]] = (uint8_t)byte;
           }
-        } else if (write) {
-          T *dst = static_cast<T *>(which ? p.c.v : p.c.k) + to * p.c.dim + col;
+        } else if (on[u]) {
+          T *dst = static_cast<T *>(values ? p.c.v : p.c.k) + (place + to[u]) * p.c.dim + col;
 #pragma unroll
           for (int q = 0; q < quant::Raw<T>::kWords / 4; ++q)
             reinterpret_cast<uint4 *>(dst)[q] =
@@ -121,90 +131,121 @@ template <> struct Stored<E4m3> {
   struct Raw { uint2 w; };
 };
 
-template <typename C, typename T>
-__global__ void __launch_bounds__(kWarps * 32) read_kernel(const __grid_constant__ Params p) {
+template <typename C, typename T, int S>
+__global__ void __launch_bounds__(kWarps * 32, 4) read_kernel(const __grid_constant__ Params p) {
   constexpr bool k8 = std::is_same<C, E4m3>::value;
-  const int lane = threadIdx.x & 31, col = (lane & ((1 << p.shift) - 1)) * 8, rows = 2 * p.c.kv_heads;
-  const int per_pass = 32 >> p.shift;
-  const int64_t items = (int64_t)((p.rows + p.run - 1) / p.run) * p.chunks;
+  constexpr int U = read_passes(S), kTokens = 32 / S;
+  const int lane = threadIdx.x & 31, col = lane % S * 8;
+  const bool on = col < p.c.dim;
+  const int64_t items = (int64_t)((p.rows + p.run - 1) / p.run) * p.groups;
   for (int64_t item = (int64_t)blockIdx.x * kWarps + threadIdx.x / 32; item < items; item += (int64_t)gridDim.x * kWarps) {
-    const int run = (int)(item / p.chunks), t0 = run * p.run;
-    const int first = (int)(item - (int64_t)run * p.chunks) * kPasses * per_pass + (lane >> p.shift);
-    const cache::Place mine = find(p, lane < p.run ? t0 + lane : p.rows);
-    for (int i = 0; i < p.run && t0 + i < p.rows; ++i) {
-      const int page = __shfl_sync(0xffffffffu, mine.page, i), at = __shfl_sync(0xffffffffu, mine.row, i);
-      typename Stored<C>::Raw raw[kPasses];
-      float scale[kPasses];
+    const int run = (int)(item / p.groups), t0 = run * p.run, n = min(p.run, p.rows - t0), r0 = (int)(item - (int64_t)run * p.groups) * p.group;
+    const cache::Place place = find(p, lane < n ? t0 + lane : p.rows);
+    // the token's row of the pages' first head, or why it has none
+    const int64_t mine = place.page < 0 ? place.page : (int64_t)place.page * p.c.kv_heads * p.c.page_size + place.row;
+    for (int r = r0; r < min(r0 + p.group, 2 * p.c.kv_heads); ++r) {
+      const bool values = r >= p.c.kv_heads;
+      const int head = values ? r - p.c.kv_heads : r;
+      using Element = std::conditional_t<k8, uint8_t, C>;
+      const Element *const from = static_cast<const Element *>(values ? p.c.v : p.c.k) + (int64_t)head * p.c.page_size * p.c.dim + col;
+      const uint8_t *const scales = (values ? p.c.v_scales : p.c.k_scales) + (int64_t)head * p.c.page_size;
+      T *dst = static_cast<T *>(values ? p.out[1] : p.out[0]) + ((int64_t)(t0 + lane / S) * p.c.kv_heads + head) * p.c.dim + col;
+      const int64_t step = (int64_t)kTokens * p.c.kv_heads * p.c.dim;
+      for (int i0 = 0; i0 < n; i0 += U * kTokens) {
+        typename Stored<C>::Raw raw[U];
+        uint32_t byte[U];
+        int state[U];
 #pragma unroll
-      for (int u = 0; u < kPasses; ++u) {
-        const int r = first + u * per_pass, which = r >= p.c.kv_heads, head = r - which * p.c.kv_heads;
-        const bool there = page >= 0 && r < rows && col < p.c.dim;
-        const int64_t from = page_row(p, page, at, head);
-        if constexpr (k8) {
-          raw[u].w = make_uint2(0, 0);
-          uint32_t byte = 127;
-          if (there) {
-            raw[u].w = *reinterpret_cast<const uint2 *>(static_cast<const uint8_t *>(which ? p.c.v : p.c.k) + from * p.c.dim + col);
-            byte = (which ? p.c.v_scales : p.c.k_scales)[from];
+        for (int u = 0; u < U; ++u) {
+          const int i = i0 + u * kTokens + lane / S;
+          const int64_t at = __shfl_sync(0xffffffffu, mine, i & 31);
+          const bool there = at >= 0 && i < n && on;
+          state[u] = at < 0 ? (int)at : 0;
+          if constexpr (k8) {
+            raw[u].w = make_uint2(0, 0);
+            byte[u] = 127;
+            if (there) {
+              raw[u].w = *reinterpret_cast<const uint2 *>(from + at * p.c.dim);
+              byte[u] = scales[at];
+            }
+          } else {
+            raw[u] = quant::load8<C, true>(from + (there ? at : 0) * p.c.dim, 0, there ? 8 : 0);
           }
-          // 2^(byte - 127); byte 0 would be 2^-127
-          scale[u] = __uint_as_float(byte ? byte << 23 : 0x400000u);
-        } else {
-          raw[u] = quant::load8<C, true>(static_cast<const C *>(which ? p.c.v : p.c.k) + (there ? from * p.c.dim : 0), col,
-                                         there ? p.c.dim : 0);
         }
-      }
 #pragma unroll
-      for (int u = 0; u < kPasses; ++u) {
-        const int r = first + u * per_pass, which = r >= p.c.kv_heads, head = r - which * p.c.kv_heads;
-        if (r >= rows || col >= p.c.dim) continue;
-        float v[8];
-        if constexpr (k8) {
+        for (int u = 0; u < U; ++u) {
+          const int i = i0 + u * kTokens + lane / S;
+          T *const to = dst;
+          dst += step;
+          if (i >= n || !on) continue;
+          float v[8];
+          if constexpr (k8) {
+            const float scale = __uint_as_float(byte[u] ? byte[u] << 23 : 0x400000u);   // 2^(byte - 127); byte 0 is 2^-127
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const uint32_t w = q < 2 ? raw[u].w.x : raw[u].w.y;
-            const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> 16 * (q % 2)), __NV_E4M3);
-            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h));
-            v[2 * q] = f.x * scale[u];
-            v[2 * q + 1] = f.y * scale[u];
+            for (int q = 0; q < 4; ++q) {
+              const uint32_t w = q < 2 ? raw[u].w.x : raw[u].w.y;
+              const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> 16 * (q % 2)), __NV_E4M3);
+              const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h));
+              v[2 * q] = f.x * scale;
+              v[2 * q + 1] = f.y * scale;
+            }
+          } else {
+#pragma unroll
+            for (int q = 0; q < 8; ++q) v[q] = quant::value(raw[u], q);
           }
-        } else {
+          if (state[u] == kBad)
 #pragma unroll
-          for (int q = 0; q < 8; ++q) v[q] = quant::value(raw[u], q);
+            for (int q = 0; q < 8; ++q) v[q] = __uint_as_float(0x7fffffffu);
+          alignas(16) T packed[8];
+#pragma unroll
+          for (int q = 0; q < 8; ++q) packed[q] = from_f32<T>(v[q]);
+#pragma unroll
+          for (int q = 0; q < (int)sizeof(T) / 2; ++q)
+            reinterpret_cast<uint4 *>(to)[q] = reinterpret_cast<const uint4 *>(packed)[q];
         }
-        if (page == kBad)
-#pragma unroll
-          for (int q = 0; q < 8; ++q) v[q] = __uint_as_float(0x7fffffffu);
-        T *dst = static_cast<T *>(which ? p.out[1] : p.out[0]) + ((int64_t)(t0 + i) * p.c.kv_heads + head) * p.c.dim + col;
-        alignas(16) T packed[8];
-#pragma unroll
-        for (int q = 0; q < 8; ++q) packed[q] = from_f32<T>(v[q]);
-#pragma unroll
-        for (int q = 0; q < (int)sizeof(T) / 2; ++q)
-          reinterpret_cast<uint4 *>(dst)[q] = reinterpret_cast<const uint4 *>(packed)[q];
       }
     }
   }
 }
 
-// Tokens of a warp's item: as many as leave the device's warps one item each, so that the chain of loads is followed seldom.
-int fill(Params *p, const p3d_cache *c, int64_t rows) {
+// Cuts tokens and rows into items. Append: the rows of four passes each, and as many tokens as leave the warps that the device
+// holds one item each. Read: one pass of tokens and one row, and while there are more items than warps, more tokens up to 32,
+// then more rows.
+int fill(Params *p, const p3d_cache *c, int64_t rows, bool read) {
   p->c = *c;
   p->rows = (int)rows;
   p->shift = 0;
   while (8 << p->shift < c->dim) ++p->shift;
-  const int per_pass = 32 >> p->shift;
-  p->chunks = (2 * c->kv_heads + per_pass * kPasses - 1) / (per_pass * kPasses);
   DeviceInfo info;
   if (int st = device_info(&info)) return st;
-  const int64_t warps = (int64_t)info.sm_count * 32;
-  p->run = 1;
-  while (p->run < 32 && rows * p->chunks / (2 * p->run) >= warps) p->run *= 2;
+  const int64_t warps = (int64_t)info.sm_count * 32, heads = 2 * (int64_t)c->kv_heads;
+  const int per_pass = 32 >> p->shift;
+  if (read) {
+    p->run = per_pass;
+    while (p->run < 32 && (rows + p->run - 1) / p->run * heads > warps) p->run *= 2;
+    const int64_t runs = (rows + p->run - 1) / p->run;
+    p->group = (int)std::min(heads, std::max<int64_t>(1, (runs * heads + warps - 1) / warps));
+  } else {
+    p->group = per_pass * kAppendPasses;
+  }
+  p->groups = (int)((heads + p->group - 1) / p->group);
+  if (!read) p->run = (int)std::min<int64_t>(32, std::max<int64_t>(1, (rows * p->groups + warps - 1) / warps));
   return P3D_OK;
 }
 int blocks_of(const Params &p) {
-  const int64_t items = (int64_t)((p.rows + p.run - 1) / p.run) * p.chunks;
+  const int64_t items = (int64_t)((p.rows + p.run - 1) / p.run) * p.groups;
   return (int)std::min<int64_t>((items + kWarps - 1) / kWarps, 1 << 20);
+}
+template <typename F>
+void by_lanes(int shift, F go) {
+  switch (shift) {
+    case 0: return go(std::integral_constant<int, 1>());
+    case 1: return go(std::integral_constant<int, 2>());
+    case 2: return go(std::integral_constant<int, 4>());
+    case 3: return go(std::integral_constant<int, 8>());
+    case 4: return go(std::integral_constant<int, 16>());
+    default: return go(std::integral_constant<int, 32>());
+  }
 }
 
 bool aligned(const void *q) { return (uintptr_t)q % 16 == 0; }
@@ -259,7 +300,7 @@ int p3d_cache_append(const p3d_cache *c, const void *new_k, const int64_t k_stri
                     v_stride[0] % unit == 0 && v_stride[1] % unit == 0,
                 "p3d_cache_append: rows must be 16-byte aligned");
   Params p = {};
-  if (int st = fill(&p, c, rows)) return st;
+  if (int st = fill(&p, c, rows, false)) return st;
   p.in[0] = new_k, p.in[1] = new_v;
   for (int i = 0; i < 2; ++i) {
     p.token_stride[i] = (i ? v_stride : k_stride)[0];
@@ -270,8 +311,11 @@ int p3d_cache_append(const p3d_cache *c, const void *new_k, const int64_t k_stri
   const cudaStream_t s = (cudaStream_t)stream;
   auto go = [&](auto type) {
     using T = decltype(type);
-    if (c->dtype == P3D_E4M3) append_kernel<T, true><<<blocks, kWarps * 32, 0, s>>>(p);
-    else append_kernel<T, false><<<blocks, kWarps * 32, 0, s>>>(p);
+    by_lanes(p.shift, [&](auto lanes) {
+      constexpr int S = decltype(lanes)::value;
+      if (c->dtype == P3D_E4M3) append_kernel<T, true, S><<<blocks, kWarps * 32, 0, s>>>(p);
+      else append_kernel<T, false, S><<<blocks, kWarps * 32, 0, s>>>(p);
+    });
   };
   dtype == P3D_F32 ? go(float()) : dtype == P3D_F16 ? go(__half()) : go(__nv_bfloat16());
   P3D_LAUNCH_CHECK();
@@ -288,19 +332,22 @@ int p3d_cache_read(const p3d_cache *c, const int32_t *starts, const int32_t *off
   P3D_CHECK_ARG(out_k && out_v && offsets, "p3d_cache_read: null argument");
   P3D_CHECK_ARG(aligned(out_k) && aligned(out_v), "p3d_cache_read: outputs must be 16-byte aligned");
   Params p = {};
-  if (int st = fill(&p, c, rows)) return st;
+  if (int st = fill(&p, c, rows, true)) return st;
   p.out[0] = out_k, p.out[1] = out_v;
   p.starts = starts, p.offsets = offsets;
   const int blocks = blocks_of(p);
   const cudaStream_t s = (cudaStream_t)stream;
   auto go = [&](auto type) {
     using T = decltype(type);
-    switch (c->dtype) {
-      case P3D_F32: read_kernel<float, T><<<blocks, kWarps * 32, 0, s>>>(p); break;
-      case P3D_F16: read_kernel<__half, T><<<blocks, kWarps * 32, 0, s>>>(p); break;
-      case P3D_BF16: read_kernel<__nv_bfloat16, T><<<blocks, kWarps * 32, 0, s>>>(p); break;
-      default: read_kernel<E4m3, T><<<blocks, kWarps * 32, 0, s>>>(p);
-    }
+    by_lanes(p.shift, [&](auto lanes) {
+      constexpr int S = decltype(lanes)::value;
+      switch (c->dtype) {
+        case P3D_F32: read_kernel<float, T, S><<<blocks, kWarps * 32, 0, s>>>(p); break;
+        case P3D_F16: read_kernel<__half, T, S><<<blocks, kWarps * 32, 0, s>>>(p); break;
+        case P3D_BF16: read_kernel<__nv_bfloat16, T, S><<<blocks, kWarps * 32, 0, s>>>(p); break;
+        default: read_kernel<E4m3, T, S><<<blocks, kWarps * 32, 0, s>>>(p);
+      }
+    });
   };
   dtype == P3D_F32 ? go(float()) : dtype == P3D_F16 ? go(__half()) : go(__nv_bfloat16());
   P3D_LAUNCH_CHECK();
