@@ -58,7 +58,7 @@ class PagedCache:
         sequence b, for ``i < offsets[b + 1] - offsets[b]``.  Other rows are not read and other places stay as they are; the
         caller advances ``lengths``.  Into 8 bits each token and head is scaled by the smallest power of two that brings its
         largest finite magnitude to at most 448 and rounded to nearest even (infinities and NaN become NaN).  Two rows for
-        one place leave one of them.  No gradients."""
+        one place leave a mixture of them.  No gradients."""
         _native.host().cache_append(self.k, self.v, self.k_scales, self.v_scales, table, k, v, lengths, offsets)
 
     def read(self, table, offsets, rows, *, starts=None, dtype=None):

@@ -171,6 +171,20 @@ inline void refuse_tangents(std::initializer_list<const Tensor *> tensors) {
                                 "forward-mode derivatives of this operator are not implemented");
 }
 
+// While a graph of a leaf that was recorded on the default stream lives, its gradient is added up on that stream, which a backward
+// pass under capture cannot reach: PyTorch then fails outside of any exception handler. So the forward pass is refused.
+inline void refuse_live_graph(std::initializer_list<const Tensor *> tensors) {
+  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
+  for (const Tensor *t : tensors) {
+    if (!t->defined() || !t->is_leaf() || !t->requires_grad()) continue;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+    const auto stream = node ? node->stream() : std::nullopt;
+    TORCH_CHECK_VALUE(!stream || *stream != c10::cuda::getDefaultCUDAStream(stream->device_index()).unwrap(),
+                      "a graph recorded on the default stream still holds this input's gradient: drop its results before "
+                      "the capture, or record it on another stream");
+  }
+}
+
 // host_sequence.cpp
 extern PyMethodDef g_sequence_methods[];
 

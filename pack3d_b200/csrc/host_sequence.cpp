@@ -219,6 +219,7 @@ PyObject *py_norm_rotate(PyObject *, PyObject *const *args, Py_ssize_t count) {
     grad = grad || wants_grad({&w, &b});
   }
   variable_list y;
+  if (grad) refuse_live_graph({&q, &k, &qs.weight, &qs.bias, &ks.weight, &ks.bias});
   if (grad)
     y = NormRotate::apply(a, r.positions, optional(r.t[kQ]), optional(r.t[kK]), optional(r.t[kQW]), optional(r.t[kQB]),
                           optional(r.t[kKW]), optional(r.t[kKB]));
@@ -324,6 +325,7 @@ PyObject *py_sequence_attention(PyObject *, PyObject *const *args, Py_ssize_t co
   a.heads = (int32_t)s.q.size(1), a.kv_heads = (int32_t)s.k.size(1), a.dim = (int32_t)dim;
   a.dtype = dtype_code(s.q.scalar_type());
   const bool grad = wants_grad({&s.q, &s.k, &s.v});
+  if (grad) refuse_live_graph({&s.q, &s.k, &s.v});
   s.q = rows16(s.q), s.k = rows16(s.k), s.v = rows16(s.v);
   if (grad) return THPVariable_Wrap(SequenceAttention::apply(a, s.q, s.k, s.v, s.q_offsets, s.k_offsets));
   return THPVariable_Wrap(run_sequence(s, nullptr));

@@ -573,3 +573,41 @@ def test_norm_rotate_refusals(cuda_device):
                              ((q.cpu(), None, p), {}, "CUDA"), ((q[0], None, p), {}, "shape")):
         with pytest.raises(ValueError, match=text):
             norm_rotate(*args, **more)
+
+
+def test_capture_behind_a_living_graph(cuda_device):
+    """While a graph from the default stream holds a leaf, a captured step over it is refused; without it the step is captured,
+    and its replay follows its inputs."""
+    from pack3d_b200 import NormSpec, norm_rotate, sequence_attention
+    torch.manual_seed(12)
+    x = torch.randn(40, 2, 64, device=cuda_device, dtype=BF16, requires_grad=True)
+    w = torch.randn(64, device=cuda_device, requires_grad=True)
+    at = torch.arange(40, device=cuda_device)
+    offsets = torch.tensor([0, 11, 40], dtype=torch.int32, device=cuda_device)
+
+    def step(x, w):
+        q, k = norm_rotate(x, x, at, q_norm=NormSpec(w, None, "rms", 1e-6))
+        y = sequence_attention(q, k, x, offsets)
+        return y, torch.autograd.grad(y.float().square().sum(), (x, w))
+
+    alive = step(x, w)[0]
+    for call in (lambda: norm_rotate(x, None, at), lambda: norm_rotate(x.detach(), None, at, q_norm=NormSpec(w, None, "rms", 1e-6)),
+                 lambda: sequence_attention(x.detach(), x.detach(), x, offsets)):
+        with pytest.raises(ValueError, match="before the capture"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                call()
+    del alive
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        other = step(x, w)                        # lives on, from another stream than the default one
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, grads = step(x, w)
+    with torch.no_grad():
+        x.mul_(-0.5).add_(0.25)
+    graph.replay()
+    want, ref = step(x.detach().requires_grad_(), w.detach().requires_grad_())
+    assert torch.equal(out, want) and all(torch.equal(a, b) for a, b in zip(grads, ref))
+    assert not torch.equal(other[0], want)
