@@ -363,6 +363,24 @@ def test_many_sequences(cuda_device):
         check(g, w, t, "gradients")
 
 
+@pytest.mark.parametrize("count", [31, 32, 126, 127, 128])
+@pytest.mark.parametrize("heads,kv", [(2, 1), (3, 3)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_order_of_tiles(cuda_device, count, heads, kv, causal):
+    """Sequences of none to three tiles, more keys or more queries, on both sides of the count up to which tiles are sorted, and rows
+    behind them all."""
+    q_len = [(37 * i) % 301 if i % 4 else 0 for i in range(count)]
+    k_len = [max(0, n + (53 * i) % 200 - 60) for i, n in enumerate(q_len)]
+    q, k, v, dout = make(q_len, k_len, heads, kv, 16, BF16, cuda_device, extra=200)
+    out, grads = run(q, k, v, dout, q_len, k_len, causal)
+    want, tol, want_grads, grad_tols = reference(q, k, v, q_len, k_len, causal, 0.25, dout)
+    check(out, want, tol, "out")
+    for g, w, t in zip(grads, want_grads, grad_tols):
+        check(g, w, t, "gradients")
+    assert not out[sum(q_len):].any() and not grads[0][sum(q_len):].any()
+    assert not grads[1][sum(k_len):].any() and not grads[2][sum(k_len):].any()
+
+
 def test_some_gradients_only(cuda_device):
     from pack3d_b200 import sequence_attention
     lengths = [200, 40]
