@@ -34,6 +34,7 @@ struct Params {
   void *dq, *dk, *dv;
   float *part;             // [2][parts][k_rows * kv_heads * dim] where parts > 1
   int parts;
+  int falling;             // the order of key tiles
   int steps;               // of 16 columns
   uint32_t idesc_out;
   float sc;                // scale * log2(e)
@@ -399,7 +400,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   // keys at a sequence's start are seen by the most queries
   const int per_slot = p.a.kv_heads * p.parts, slot = blockIdx.x / per_slot, kv = blockIdx.x % per_slot / p.parts,
             part = blockIdx.x % p.parts;
-  const Place at = falling(p.a) ? place_falling<true>(p.a, 7, slot) : place_of<true>(p.a, 7, slot);
+  const Place at = p.falling ? place_falling<true>(p.a, 7, slot) : place_of<true>(p.a, 7, slot);
   const Range r = at.r;
   const int key0 = at.group * kTile;
   if (at.group < 0 || key0 >= r.nk) return;
@@ -817,6 +818,7 @@ int launch_bwd(const p3d_sequence &a, const void *out, const float *lse, const v
   float2 *const stats = static_cast<float2 *>(workspace);
   p.stats = stats;
   p.parts = parts_of(a, info.sm_count);
+  p.falling = falling(a, slots_of(a.k_rows, a.sequences, kTile) * a.kv_heads * p.parts, info.sm_count);
   p.part = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + stats_bytes(a));
   p.steps = (a.dim + 15) / 16;
   p.idesc_out = idesc_f16(128, p.steps * 16, a.dtype == P3D_BF16, true);

@@ -9,14 +9,13 @@
 // special-function units as many, so a quarter of the exponentials go to the FMA pipe as polynomials; at dim 64 and below
 // the exponentials are the bound. What counts is that neither waits for the other: the softmax goes by 64 keys, and each tile has two
 // buffers of S (64 columns; P of 16 bits goes over its own S), so that S of the next 64 keys is made while the softmax works on
-// these. S of 64 keys costs a
-// third more of the pipe than half of 128, as its operands come from shared memory.
+// these. S of 64 keys costs a third more of the pipe than half of 128, as its operands come from shared memory.
 // O is rescaled only where a row's maximum has grown by more than 2^8 (weights up to 2^8 cost no precision), after the product before
 // has completed.
 //
 // A CTA goes through several such pairs (two thousand keys take 12 us, and setting a CTA up and taking it down 6): the next pair's
-// queries, keys and first S come while this one's softmax ends and O is written. Pairs are launched the longest first, over all sequences, and taken
-// over as CTAs get done. All waits go by counts that run on over the pairs.
+// queries, keys and first S come while this one's softmax ends and O is written. Pairs are launched the longest first, over all
+// sequences, and taken over as CTAs get done. All waits go by counts that run on over the pairs.
 //
 // Masks: key j counts for row i where j < seen(i); units of keys that some row of a warp does not see whole are masked by columns.
 #include <math.h>
@@ -58,6 +57,7 @@ struct Params {
   int two_heads;   // a CTA's tiles are two heads
   int steps;       // of 16 columns
   int works;       // pairs of tiles
+  int falling;     // their order
   uint32_t idesc_o;
   float sc;        // scale * log2(e)
 };
@@ -74,7 +74,7 @@ struct Work {
 __device__ __forceinline__ Work work_of(const Params &p, int index) {
   const int slot = index / p.units, unit = index % p.units;
   const int shift = p.two_heads ? 7 : 8;   // 128 or 256 rows a slot
-  const Place s = falling(p.a) ? place_falling<false>(p.a, shift, slot)
+  const Place s = p.falling ? place_falling<false>(p.a, shift, slot)
                                : place_of<false>(p.a, shift, p.works / p.units - 1 - slot);   // the longest of each sequence first
   Work w;
   w.r = s.r;
@@ -492,6 +492,9 @@ int launch_fwd(const p3d_sequence &a, void *out, float *lse, cudaStream_t s) {
   const int64_t works = slots_of(a.q_rows, a.sequences, p.two_heads ? kTile : 2 * kTile) * p.units;
   if (works > 0x7fffffff - 4096) return fail(P3D_ERR_UNSUPPORTED, "p3d_sequence_fwd: too many tiles");
   p.works = (int)works;
+  DeviceInfo info;
+  if (int st = device_info(&info)) return st;
+  p.falling = falling(a, works, info.sm_count);
   const int grid = p.works;
   CUtensorMap tq, tk, tv;
   if (int st = encode_heads(&tq, a.dtype, a.q, a.dim, a.heads, a.q_rows, a.q_stride)) return st;
