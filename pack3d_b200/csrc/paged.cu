@@ -18,6 +18,10 @@
 //   every CTA takes an equal stretch of it: one long sequence or many uneven ones fill the device alike. A head's pieces
 //   are joined by a second kernel, in order; a stretch holds at most one head that began before it and one that goes on
 //   after it, so two slots a CTA keep all pieces. Where no sequence can be longer than a few units, a CTA takes a whole head.
+//
+// Measured, 32 heads over 8 of 128, with the join: one sequence of 200,003 tokens in bf16 153 us, 5.3 TB/s (loads in flight: 255 registers
+// a thread leave eight warps an SM); 64 sequences, 262,144 tokens, in 8 bits 139 us, 3.9 TB/s (the conversions' instructions, at a
+// third of the issue slots, between two loads of a warp).
 #include <cuda_fp8.h>
 #include <math.h>
 
@@ -427,11 +431,12 @@ __device__ __forceinline__ void attend(const Params &p, Shared<DP> &sh, int b, i
   while (at < last) {
     tile(even, odd);
     if constexpr (k8) {
-      // a copy, which waits for the values: twice the code instead costs more (140 -> 184 us), as it leaves the instruction cache
+      // a copy, which waits for the values: twice the code instead costs more (the 64 sequences: 140 -> 184 us), as it leaves the
+      // instruction cache
       even = odd;
     } else {
       if (at >= last) break;
-      tile(odd, even);   // 205 -> 156 us
+      tile(odd, even);   // the long sequence: 205 -> 156 us
     }
   }
   const int r = lane / 4, c = lane % 4;

