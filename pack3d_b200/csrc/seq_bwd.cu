@@ -2,7 +2,9 @@
 //
 //     P = 2^(S c - lse),  dS = scale P (dO V^T - delta),  dQ = dS K,  dK = dS^T Q,  dV = P^T dO
 //
-// (dS with its scale, so that in f16 it stays in range where the gradients do.)
+// (dS with its scale, so that in f16 it stays in range where the gradients do.) Where a query sees a single key, P is 1 and dS is 0;
+// dP - delta, two sums of the same products, would leave the rounding of their orders: scale and delta are 0 there (in dK: where a sequence
+// has one key. Among more keys, whose gradients are sums over many queries, that rounding is as small as any).
 //
 // Two kernels, so that each gradient is a sum in one fixed order without atomics: dQ by tiles of queries, dK and dV by tiles of keys.
 // They make S and dP both, seven products of which five are the mathematics' own (a tile of 128 x 128 is 512 cycles a product).
@@ -91,7 +93,7 @@ __device__ __noinline__ void redo_dq(const Params &p, const Range &r, int head, 
   for (int j = 0; j < seen; ++j) {
     load4(static_cast<const T *>(a.k) + (int64_t)(r.k0 + j) * a.k_stride[0] + kv * a.k_stride[1], dim, k);
     load4(static_cast<const T *>(a.v) + (int64_t)(r.k0 + j) * a.v_stride[0] + kv * a.v_stride[1], dim, v);
-    const float ds = exp2f(dot4(q, k) * p.sc + stat.x) * fmaf(dot4(d, v), a.scale, stat.y);
+    const float ds = exp2f(dot4(q, k) * p.sc + stat.x) * (seen == 1 ? 0.f * dot4(d, v) : fmaf(dot4(d, v), a.scale, stat.y));
 #pragma unroll
     for (int i = 0; i < 4; ++i) sum[i] = fmaf(ds, k[i], sum[i]);
   }
@@ -113,7 +115,7 @@ __device__ __noinline__ void redo_dkv(const Params &p, const Range &r, int kv, i
       load4(static_cast<const T *>(a.q) + (int64_t)(r.q0 + i) * a.q_stride[0] + head * a.q_stride[1], a.dim, q);
       load4(static_cast<const T *>(p.dout) + ((int64_t)(r.q0 + i) * a.heads + head) * a.dim, a.dim, d);
       const float2 stat = p.stats[(int64_t)head * a.q_rows + r.q0 + i];
-      const float w = exp2f(dot4(q, k) * p.sc + stat.x), ds = w * fmaf(dot4(d, v), a.scale, stat.y);
+      const float w = exp2f(dot4(q, k) * p.sc + stat.x), ds = w * (r.nk == 1 ? 0.f * dot4(d, v) : fmaf(dot4(d, v), a.scale, stat.y));
 #pragma unroll
       for (int c = 0; c < 4; ++c) sum[c] = values ? fmaf(w, d[c], sum[c]) : fmaf(ds, q[c], sum[c]);
     }
@@ -297,7 +299,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const bool there = row < r.nq;
     const int seen = there ? seen_by(r, row, p.a.causal) : 0;
     const float2 stat = there ? p.stats[(int64_t)head * p.a.q_rows + r.q0 + row] : make_float2(0.f, 0.f);
-    const float2 sc = make_float2(p.sc, p.sc), shift = make_float2(stat.x, stat.x), minus = make_float2(stat.y, stat.y), scale = make_float2(p.a.scale, p.a.scale);
+    const float one = seen == 1 ? 0.f : p.a.scale, less = seen == 1 ? 0.f : stat.y;
+    const float2 sc = make_float2(p.sc, p.sc), shift = make_float2(stat.x, stat.x), minus = make_float2(less, less), scale = make_float2(one, one);
     const uint32_t lanes = (uint32_t)((warp % 4) * 32) << 16;
     bool ok = true;
     for (int c = 0; c < chunks; ++c) {
@@ -484,7 +487,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         stats[s * 256 + lane + 32 * u] = v[u].x;
-        stats[s * 256 + 128 + lane + 32 * u] = v[u].y;
+        stats[s * 256 + 128 + lane + 32 * u] = r.nk == 1 ? 0.f : v[u].y;
       }
       __syncwarp();
       // a head's last queries, where their tile goes past the sequence's end, land on a barrier of their own
@@ -566,7 +569,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else {
     const int half = warp / 4;
     const uint32_t lanes = (uint32_t)((warp % 4) * 32) << 16, t_s = tmem + 64 * half + lanes, t_d = t_dp + 64 * half + lanes;
-    const float2 sc = make_float2(p.sc, p.sc), scale = make_float2(p.a.scale, p.a.scale);
+    const float one = r.nk == 1 ? 0.f : p.a.scale;
+    const float2 sc = make_float2(p.sc, p.sc), scale = make_float2(one, one);
     const int from = p.a.causal ? key - shift : 0;   // the first query that sees this key
     bool ok = true;
     for (int i = 0, row = first; i < steps; ++i, row = row + kTile < r.nq ? row + kTile : first) {

@@ -381,6 +381,24 @@ def test_order_of_tiles(cuda_device, count, heads, kv, causal):
     assert not grads[1][sum(k_len):].any() and not grads[2][sum(k_len):].any()
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("heads,kv,dim", [(2, 1, 64), (5, 1, 128), (3, 3, 48)])
+def test_single_keys_have_no_score_gradient(cuda_device, dtype, heads, kv, dim):
+    """Where a query sees one key its weight is 1 whatever the score: its gradient is 0 exactly, and a key's of a sequence of one."""
+    for q_len, k_len, causal in (([1, 0, 1, 1], None, True), ([4, 300, 1], [1, 1, 1], False), ([4, 300, 1], [1, 1, 1], True),
+                                 ([1, 2], [1, 2], True)):
+        k_len = q_len if k_len is None else k_len
+        q, k, v, dout = make(q_len, k_len, heads, kv, dim, dtype, cuda_device)
+        out, (dq, dk, dv) = run(q, k, v, dout, q_len, k_len, causal)
+        want, tol, want_grads, grad_tols = reference(q, k, v, q_len, k_len, causal, dim ** -0.5, dout)
+        check(out, want, tol, "out")
+        check(dv, want_grads[2], grad_tols[2], "dv")
+        if k_len[-1] == 1:
+            assert not dq.any() and not dk.any()
+        else:   # the second sequence's first query sees one key, its second two
+            assert not dq[:2].any() and not dk[:1].any() and dq[2].any()
+
+
 def test_some_gradients_only(cuda_device):
     from pack3d_b200 import sequence_attention
     lengths = [200, 40]
