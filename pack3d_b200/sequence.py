@@ -3,6 +3,8 @@
 * :func:`norm_rotate` -- norms of queries and keys for each head and the rotation of their positions, one kernel a direction.
 * :func:`sequence_attention` -- attention over sequences packed one behind the other, grouped heads, both directions.
 
+Steps of both may be captured in CUDA graphs; a leaf that a living graph from the default stream still holds is refused there.
+
 For serving, :mod:`pack3d_b200.cache` keeps keys and values in pages.  No counterpart in the reference, whose attention is
 over a geometry (``reference.py:8-31``) and whose rotation stands alone (``rope.py:15-48``).
 """
