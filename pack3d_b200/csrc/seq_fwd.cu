@@ -97,7 +97,8 @@ __device__ __forceinline__ Work work_of(const Params &p, int index) {
 }
 
 // P = 2^(s sc + shift) of a row's 64 scores, rounded to T and written over them; returns the row's sum.  kPoly of every eight pairs are
-// polynomials (scores are not NaN there: the row's maximum, and with it shift, would be).
+// polynomials, which make a finite number of a NaN and of -inf. A NaN score makes the row's maximum NaN; a score
+// of +inf makes it infinite, as scores that are all -inf do. Such rows have no softmax: they become NaN at their end, whatever they held.
 template <typename T, int kPoly>
 __device__ __forceinline__ float weights(const float (&s)[kKeys], float sc, float shift, uint32_t t_s) {
   const float2 sc2 = make_float2(sc, sc), shift2 = make_float2(shift, shift);
@@ -412,6 +413,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!ok) break;
       if (mine) ok = wait_warp(bar(kODone + t), (n - 1) & 1, &g_seq_fwd_errors, kErrSoftmax);
       if (!ok) break;
+      if (not_finite(m)) l = NAN;   // of no row whose softmax exists
       const float inv = seen > 0 ? 1.f / l : 0.f;
       const int64_t at = there ? ((int64_t)(now.r.q0 + row) * p.a.heads + head) * p.a.dim : -1;
       T *const out = static_cast<T *>(p.out);

@@ -1,0 +1,90 @@
+"""Packed-sequence attention and the norms with rotation over values that are not finite, small gradients and long sums, against
+their definitions in 64 bits."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+NAN, INF = math.nan, math.inf
+
+
+@pytest.fixture(autouse=True)
+def no_wait_ran_out():
+    """No bounded wait of a kernel gave up."""
+    yield
+    from pack3d_b200 import _native
+    assert _native.device_errors() == 0
+
+
+def offsets_of(lengths, device):
+    at = [0]
+    for n in lengths:
+        at.append(at[-1] + n)
+    return torch.tensor(at, dtype=torch.int32, device=device)
+
+
+def randn(*shape, device, seed, dtype, scale=1.0):
+    gen = torch.Generator(device=device).manual_seed(seed)
+    return (torch.randn(*shape, generator=gen, device=device) * scale).to(dtype)
+
+
+# ------------------------------------------------------------------------------- scores that are infinite
+@pytest.mark.parametrize("dtype,dim", [(BF16, 64), (F16, 128), (BF16, 128), (F16, 48)])
+@pytest.mark.parametrize("keys", [64, 128, 256])
+@pytest.mark.parametrize("causal", [False, True])
+def test_infinite_scores(cuda_device, dtype, dim, keys, causal):
+    """A key with an infinity in one column, at every place of the last 64, one to a sequence: queries with a positive, a negative or both
+    signs in that column. NaN exactly where the 64-bit softmax is, and its value elsewhere."""
+    from pack3d_b200 import sequence_attention
+    rows, heads, last = 160, 2, 64
+    q = randn(last, rows, heads, dim, device=cuda_device, seed=1, dtype=dtype)
+    k = randn(last, keys, 1, dim, device=cuda_device, seed=2, dtype=dtype)
+    v = randn(last, keys, 1, dim, device=cuda_device, seed=3, dtype=dtype)
+    at = torch.arange(last, device=cuda_device)
+    k[at, keys - last + at, 0, 3] = INF
+    for sign in (1, -1, 0):
+        x = q.clone()
+        x[..., 3] = q[..., 3].abs() * sign if sign else q[..., 3]
+        x[..., 3] += 0.125 * torch.where(x[..., 3] < 0, -1, 1)    # not 0
+        got = sequence_attention(x.flatten(0, 1), k.flatten(0, 1), v.flatten(0, 1), offsets_of([rows] * last, cuda_device),
+                                 offsets_of([keys] * last, cuda_device), causal=causal).view(last, rows, heads, dim)
+        s = torch.einsum("bihd,bjd->bhij", x.double(), k[:, :, 0].double()) * dim ** -0.5
+        if causal:
+            s = torch.where(torch.ones(rows, keys, dtype=torch.bool, device=cuda_device).tril(keys - rows), s, -INF)
+        p = torch.softmax(s, -1)
+        nothing = s.new_zeros(rows, dtype=torch.bool)
+        if causal and rows > keys:
+            nothing[:rows - keys] = True
+            p = torch.where(nothing[:, None], 0.0, p)
+        want = torch.einsum("bhij,bjd->bihd", p, v[:, :, 0].double())
+        assert torch.equal(got.isnan(), want.isnan())
+        # weights and results rounded (half a step each), exponentials to 2^-13, sums in fp32
+        u = torch.finfo(dtype).eps / 2
+        tol = (2 * u + 2.0 ** -13 + 2.0 ** -15) * torch.einsum("bhij,bjd->bihd", p, v[:, :, 0].double().abs()) + 2.0 ** -24
+        there = ~want.isnan()
+        assert there.any() or sign == 1
+        assert ((got.double() - want).abs() <= tol)[there].all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("keys", [64, 128, 192])
+def test_every_score_minus_infinity(cuda_device, dtype, keys):
+    """The softmax of nothing but -inf is NaN, and so are the gradients that come of it; the sequence beside it keeps its own."""
+    from pack3d_b200 import sequence_attention
+    rows, dim = 128, 64
+    q = randn(2 * rows, 1, dim, device=cuda_device, seed=1, dtype=dtype)
+    k, v = (randn(2 * keys, 1, dim, device=cuda_device, seed=s, dtype=dtype) for s in (2, 3))
+    q[:rows, :, 3] = 1
+    qo, ko = offsets_of([rows, rows], cuda_device), offsets_of([keys, keys], cuda_device)
+
+    def run():
+        leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+        out = sequence_attention(*leaves, qo, ko, causal=False)
+        return [out.detach(), *torch.autograd.grad(out, leaves, torch.ones_like(out))]
+    clean = run()
+    k[:keys, :, 3] = -INF
+    for got, before, n in zip(run(), clean, (rows, rows, keys, keys)):
+        assert got[:n].isnan().all() and torch.equal(got[n:], before[n:])
