@@ -50,7 +50,7 @@ struct Layout {
 
 // Every wait on a barrier that completes more than once is by someone who has seen the completion before, and whose own next step the
 // one after needs.
-enum { kQFull, kQEmpty, kSFull, kPFull = kSFull + 4, kODone = kPFull + 2, kNext = kODone + 2, kLanded, kDrain, kFull = kDrain + 2 };
+enum { kQFull, kQEmpty, kSFull, kPFull = kSFull + 4, kODone = kPFull + 2, kNext = kODone + 2, kDrain, kFull = kDrain + 2 };
 template <int DP> constexpr int bars() { return kFull + 2 * Layout<DP>::kStages; }
 
 struct Params {
@@ -71,6 +71,7 @@ struct Work {
   Range r;
   int row[2], head[2], kv;
   int units[2];    // 64 keys that each tile sees any of
+  int whole;       // of those, the first ones that every row of both tiles sees all of
   int index;       // in the order of launches; -1: none
   __device__ __forceinline__ int most() const { return max(units[0], units[1]); }
   __device__ __forceinline__ int chunks() const { return (most() + 1) / 2; }   // tiles of keys
@@ -92,6 +93,7 @@ __device__ __forceinline__ Work work_of(const Params &p, int index) {
     if (s.group >= 0 && w.row[t] < w.r.nq)
       w.units[t] = (seen_by(w.r, min(w.row[t] + kTile, w.r.nq) - 1, p.a.causal) + kKeys - 1) / kKeys;
   }
+  w.whole = w.units[0] ? seen_by(w.r, w.row[0], p.a.causal) / kKeys : 0;
   w.kv = w.head[0] / group;
   return w;
 }
@@ -125,25 +127,26 @@ __device__ __forceinline__ float weights(const float (&s)[kKeys], float sc, floa
   return both.x + both.y;
 }
 
-// One row by the definition (a warp).
+// Adds what clear_not_finite took out of the values from key j on to a warp's rows that see it: rows see the more keys the further down they
+// are, so one pass over the keys serves all of them. `at` (a row's place in out, -1 for none) and `seen` are of a lane's row.
 template <typename T>
-__device__ __noinline__ void redo_row(const p3d_sequence &a, const Range &r, int head, int row, int seen, T *out) {
-  const int kv = head / (a.heads / a.kv_heads);
-  float q[4], k[4], v[4], o[4] = {0.f, 0.f, 0.f, 0.f}, m = -INFINITY, l = 0.f;
-  load4(static_cast<const T *>(a.q) + (int64_t)(r.q0 + row) * a.q_stride[0] + head * a.q_stride[1], a.dim, q);
-  for (int j = 0; j < seen; ++j) {
-    load4(static_cast<const T *>(a.k) + (int64_t)(r.k0 + j) * a.k_stride[0] + kv * a.k_stride[1], a.dim, k);
-    load4(static_cast<const T *>(a.v) + (int64_t)(r.k0 + j) * a.v_stride[0] + kv * a.v_stride[1], a.dim, v);
-    const float s = dot4(q, k) * a.scale * 1.4426950408889634f, top = max_nan(m, s);
-    const float down = m == -INFINITY ? 0.f : exp2f(m - top), w = top == -INFINITY ? 0.f : exp2f(s - top);
-    l = l * down + w;
-    m = top;
+__device__ __noinline__ void add_not_finite(const p3d_sequence &a, const Range &r, int kv, int j, int64_t at, int seen, T *out) {
+  const int c = (threadIdx.x & 31) * 4;
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int from = 0; from < 32; ++from) {
+    const int64_t to = __shfl_sync(0xffffffffu, at, from);
+    const int upto = __shfl_sync(0xffffffffu, seen, from);
+    if (to < 0) break;
+    for (; j < upto; ++j) {
+      float v[4];
+      load4(static_cast<const T *>(a.v) + (int64_t)(r.k0 + j) * a.v_stride[0] + kv * a.v_stride[1], a.dim, v);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = fmaf(w, v[i], o[i] * down);
+      for (int i = 0; i < 4; ++i) sum[i] += not_finite(v[i]) ? v[i] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (sum[i] != 0.f) out[to + c + i] = from_f32<T>(to_f32<T>(out[to + c + i]) + sum[i]);
   }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) o[i] /= l;
-  mend4(out, a.dim, o);
 }
 
 template <typename T, int DP>
@@ -156,6 +159,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ __align__(8) uint64_t bar_mem[bars<DP>()];
   __shared__ uint32_t tmem_holder;
   __shared__ Work works[2];   // of a pair (by its number's last bit), as the copying warp found it
+  __shared__ int odd_pair[2][2];   // by the same bit and the tile: the number + 1 of the last pair whose values were not all finite
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   __shared__ __align__(16) uint4 answer;
   const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
@@ -168,6 +172,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0; i < bars<DP>(); ++i)
       mbar_init(bar(i), i == kQEmpty ? 10 : i == kPFull || i == kPFull + 1 ? 4 : i >= kFull + NS ? 2 : 1);
     fence_mbar_init();
+    for (int i = 0; i < 4; ++i) odd_pair[i / 2][i % 2] = 0;
   }
   if (warp == kMmaWarp) {
     tmem_alloc(smem_u32(&tmem_holder), 512);
@@ -187,7 +192,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == kCopyWarp) {
     // ------------------------------------------------------------------ copies; items K0, V0, K1, V1, .. of one pair after another
     bool ok = true;
-    int item0 = 0, issued = 0, cleared = 0;
+    int item0 = 0, issued = 0;
     Work now = work_of(p, blockIdx.x);
     for (;; ++done) {
       // the last pair's queries have had their last product, and everybody knows of it
@@ -209,22 +214,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             ok = false;
             break;
           }
-          // the last values, where their tile goes past the sequence's end, land on a barrier of their own
-          const uint32_t on = (i - item0) % 2 && (c + 1) * kTile > now.r.nk ? bar(kLanded) : full(s);
-          mbar_expect_tx(on, L::kTileBytes);
+          mbar_expect_tx(full(s), L::kTileBytes);
           for (int k = 0; k < DP / 64; ++k)
-            tma_load_3d(ring + s * L::kTileBytes + k * kBox, (i - item0) % 2 ? &tv : &tk, on, 64 * k, now.kv, now.r.k0 + c * kTile);
+            tma_load_3d(ring + s * L::kTileBytes + k * kBox, (i - item0) % 2 ? &tv : &tk, full(s), 64 * k, now.kv, now.r.k0 + c * kTile);
           issued = i + 1;
         }
       }
       ok = __all_sync(0xffffffffu, ok);
-      if (ok && chunks * kTile > now.r.nk && chunks) {
-        const int s = (item0 + 2 * chunks - 1) % NS;
-        ok = wait_warp(bar(kLanded), cleared++ & 1, &g_seq_fwd_errors, kErrProducer);
-        if (!ok) break;
-        clear_rows<DP / 64>(smem + (2 + s) * L::kTileBytes, now.r.nk - (chunks - 1) * kTile);
-        if (lane == 0) mbar_arrive(full(s));
-      }
       item0 += 2 * chunks;
       if (now.index < 0) break;
       ok = wait_warp(bar(kNext), done & 1, &g_seq_fwd_errors, kErrProducer) && ok;
@@ -331,7 +327,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lanes = (uint32_t)((warp % 4) * 32) << 16;
     const uint32_t t_s = tmem + kColS + 128 * t + lanes, t_o = tmem + kColO + 128 * t + lanes;
     const float sc = p.sc;
-    int n = 0;   // steps of this tile so far
+    int n = 0;       // steps of this tile so far
+    int item0 = 0;   // of this pair
     bool ok = true;
     uint8_t *const stage = smem + (2 + NS) * L::kTileBytes + warp * 4096;
     for (;; ++done) {
@@ -405,6 +402,16 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         }
+        // Keys that some row does not see: its weights are 0, and 0 times an infinity or NaN is not. The four warps clear their quarters
+        // of the 64 values before this tile's product may read them. (The other tile's may be under way: its own warps have cleared
+        // them, and what is written here is what is there.) The item before this one in its stage has long landed.
+        if (u >= now.whole) {
+          const int item = item0 + u / 2 * 2 + 1;
+          ok = wait_warp(full(item % NS), (item / NS) & 1, &g_seq_fwd_errors, kErrSoftmax);
+          if (!ok) break;
+          const bool odd = clear_not_finite<T, DP / 64, kKeys / 4>(smem + (2 + item % NS) * L::kTileBytes + ((u & 1) * 4 + warp % 4) * (kKeys / 4 * 128));
+          if (odd && lane == 0) *const_cast<volatile int *>(&odd_pair[done & 1][t]) = done + 1;
+        }
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -417,7 +424,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       const float inv = seen > 0 ? 1.f / l : 0.f;
       const int64_t at = there ? ((int64_t)(now.r.q0 + row) * p.a.heads + head) * p.a.dim : -1;
       T *const out = static_cast<T *>(p.out);
-      float odd = 0.f;   // NaN where any of the row is not finite
 #pragma unroll
       for (int i = 0; i < DP; i += 64) {
         if (i >= p.a.dim) continue;
@@ -432,7 +438,6 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int k = 0; k < 32; k += 2) {
             const float a = seen > 0 ? __uint_as_float(o[k]) * inv : 0.f, b = seen > 0 ? __uint_as_float(o[k + 1]) * inv : 0.f;
-            if (i + h + k < p.a.dim) odd = fmaf(a, 0.f, fmaf(b, 0.f, odd));
             packed[(h + k) / 2] = pack<T>(a, b);
           }
         }
@@ -440,17 +445,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (p.lse && there)
         p.lse[(int64_t)head * p.a.q_rows + now.r.q0 + row] = seen > 0 ? (m * sc + log2f(l)) * 0.6931471805599453f : -INFINITY;
-      // rows with an infinity or NaN, in a unit with keys that they do not see; where the last key that they see is NaN they are right
-      const int past = min(mine * kKeys, now.r.nk);
-      for (unsigned rows = __ballot_sync(0xffffffffu, there && odd != odd && seen > 0 && seen < past); rows; rows &= rows - 1) {
-        const int from = __ffs(rows) - 1, first = __shfl_sync(0xffffffffu, seen, from);
-        const T *v = static_cast<const T *>(p.a.v) + (int64_t)(now.r.k0 + first) * p.a.v_stride[0] + now.kv * p.a.v_stride[1];
-        float last[4];
-        load4(v - p.a.v_stride[0], p.a.dim, last);
-        const bool right = last[0] != last[0] && last[1] != last[1] && last[2] != last[2] && last[3] != last[3];
-        if (__all_sync(0xffffffffu, right || lane * 4 >= p.a.dim) || !rows_not_finite(v, p.a.v_stride[0], past - first, p.a.dim)) continue;
-        redo_row<T>(p.a, now.r, head, __shfl_sync(0xffffffffu, row, from), first, out + __shfl_sync(0xffffffffu, at, from));
-      }
+      // what was cleared, for the rows that see it: written before the arrival that the last product waited for
+      if (mine && *const_cast<volatile int *>(&odd_pair[done & 1][t]) == done + 1)
+        add_not_finite<T>(p.a, now.r, now.kv, now.whole * kKeys, at, seen, out);
+      item0 += 2 * now.chunks();
       tc_fence_before();   // O is read before the next pair's P lets a product write it
     }
     tmem_wait_st();

@@ -167,12 +167,14 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
 }
 
 // Masked weights and values that are not finite.  A masked weight is 0, but 0 times an infinity or NaN is NaN: a product over a whole tile
-// would pass on what a row does not see.
-// * Rows of a tile behind the end of its sequence (another sequence's, or memory that nobody filled) are set to 0 before the products
-//   read the tile: by the copying warp, which has it land on a barrier of its own (clear_rows).
-// * Within a sequence, what lies behind a row's last key shows in the result. Rows whose result is not finite, and beside whose keys
-//   (queries) in the tile there is such a value that they do not see, have those columns made again by their definition, a warp to a
-//   row (rows_not_finite, mend4, and the redo functions of each kernel). Nothing is paid for that where all is finite.
+// would pass on what a row does not see. So in tiles that some row does not see whole, such values are set to 0 before the product reads
+// them, and added again to the rows that see them once the sum is there: an infinity whose weight is positive makes the sum that infinity, two
+// that meet make it NaN. Each such value is looked at once for 32 rows, so the work is bounded by what is read anyway.
+// * Forward: the softmax warps look through the values of those tiles (clear_not_finite) before they hand over their weights; rows behind the end
+//   of a sequence (another sequence's, or memory that nobody filled) are among them.
+// * Backward: rows of a tile behind the end of its sequence are cleared by the copying warp, which has it land on a barrier of its own (clear_rows).
+//   Within a sequence, rows whose result is not finite, beside values that they do not see, have those columns made again by their
+//   definition, a warp to a row (rows_not_finite, mend4, and the redo functions of each kernel).
 template <int kBoxes>
 __device__ __forceinline__ void clear_rows(uint8_t *tile, int first) {
   for (int i = threadIdx.x & 31; i < (kTile - first) * 8; i += 32)
@@ -180,6 +182,36 @@ __device__ __forceinline__ void clear_rows(uint8_t *tile, int first) {
     for (int b = 0; b < kBoxes; ++b) *reinterpret_cast<uint4 *>(tile + b * kBox + first * 128 + i * 16) = make_uint4(0, 0, 0, 0);
   fence_proxy_async_smem();
   __syncwarp();
+}
+// `kRows` rows of each box from `tile` on (shared memory, by a warp): infinities and NaN become 0; whether there were any. All finite, it
+// costs a load and four additions of zeros for 16 bytes.
+template <typename T, int kBoxes, int kRows>
+__device__ __forceinline__ bool clear_not_finite(uint8_t *tile) {
+  constexpr int kEach = kRows * 128 / 512;   // loads of a lane in a box
+  constexpr uint32_t kExp = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+  uint4 w[kBoxes * kEach];
+  uint32_t sum = 0;
+  auto add = [&](uint32_t v) {   // v * 0 + sum, each half: 0, or NaN for ever
+    if constexpr (std::is_same<T, __half>::value) asm("fma.rn.f16x2 %0, %1, %2, %0;" : "+r"(sum) : "r"(v), "r"(0u));
+    else asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(sum) : "r"(v), "r"(0u));
+  };
+#pragma unroll
+  for (int i = 0; i < kBoxes * kEach; ++i)
+    w[i] = *reinterpret_cast<const uint4 *>(tile + i / kEach * kBox + i % kEach * 512 + (threadIdx.x & 31) * 16);
+#pragma unroll
+  for (int i = 0; i < kBoxes * kEach; ++i) add(w[i].x), add(w[i].y), add(w[i].z), add(w[i].w);
+  if (!__any_sync(0xffffffffu, (sum & 0x7fff7fffu) != 0)) return false;
+  auto clean = [&](uint32_t &v) {
+    if ((v & kExp) == kExp) v &= 0xffff0000u;
+    if ((v & kExp << 16) == kExp << 16) v &= 0xffffu;
+  };
+#pragma unroll
+  for (int i = 0; i < kBoxes * kEach; ++i) {
+    clean(w[i].x), clean(w[i].y), clean(w[i].z), clean(w[i].w);
+    *reinterpret_cast<uint4 *>(tile + i / kEach * kBox + i % kEach * 512 + (threadIdx.x & 31) * 16) = w[i];
+  }
+  fence_proxy_async_smem();
+  return true;
 }
 __device__ __forceinline__ bool not_finite(float v) { return (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u; }
 

@@ -88,3 +88,39 @@ def test_every_score_minus_infinity(cuda_device, dtype, keys):
     k[:keys, :, 3] = -INF
     for got, before, n in zip(run(), clean, (rows, rows, keys, keys)):
         assert got[:n].isnan().all() and torch.equal(got[n:], before[n:])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("value", [NAN, INF, -INF])
+@pytest.mark.parametrize("heads,kv,dim", [(8, 2, 128), (3, 3, 64)])
+def test_a_channel_of_values_that_are_not_finite(cuda_device, dtype, value, heads, kv, dim):
+    """One column of every value: the other columns keep their bits, and it takes no longer than a few times the usual (below 1 ms)."""
+    from pack3d_b200 import sequence_attention
+    n = 8192
+    offsets = offsets_of([n - 900, 900], cuda_device)
+    q, k, v = (randn(n, h, dim, device=cuda_device, seed=s, dtype=dtype) for s, h in enumerate((heads, kv, kv)))
+    clean = sequence_attention(q, k, v, offsets)
+    v[:, :, 9] = value
+    start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+    start.record()
+    out = sequence_attention(q, k, v, offsets)
+    end.record()
+    end.synchronize()
+    assert start.elapsed_time(end) < 15
+    keep = torch.arange(dim, device=cuda_device) != 9
+    assert torch.equal(out[..., keep], clean[..., keep])
+    assert out[..., 9].isnan().all() if math.isnan(value) else (out[..., 9] == value).all()
+
+
+@pytest.mark.parametrize("heads,kv", [(2, 1), (1, 1)])
+def test_infinite_value_at_the_end_of_a_long_sequence(cuda_device, heads, kv):
+    """200,000 tokens, the last ones' values infinite: the rows before keep their bits, as do sequences behind it, in bounded time."""
+    from pack3d_b200 import sequence_attention
+    lengths = [200000, 5, 700]
+    offsets = offsets_of(lengths, cuda_device)
+    q, k, v = (randn(sum(lengths), h, 64, device=cuda_device, seed=s, dtype=BF16) for s, h in enumerate((heads, kv, kv)))
+    clean = sequence_attention(q, k, v, offsets)
+    v[199990:200000] = INF
+    out = sequence_attention(q, k, v, offsets)
+    assert torch.equal(out[:199990], clean[:199990]) and torch.equal(out[200000:], clean[200000:])
+    assert (out[199990:200000] == INF).all()
