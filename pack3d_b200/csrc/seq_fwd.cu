@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ __align__(8) uint64_t bar_mem[bars<DP>()];
   __shared__ uint32_t tmem_holder;
   __shared__ Work works[2];   // of a pair (by its number's last bit), as the copying warp found it
-  __shared__ int odd_pair[2][2];   // by the same bit and the tile: the number + 1 of the last pair whose values were not all finite
+  __shared__ int odd_pair[2];   // by the same bit: the number + 1 of the last pair whose values were not all finite
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   __shared__ __align__(16) uint4 answer;
   const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
@@ -172,7 +172,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0; i < bars<DP>(); ++i)
       mbar_init(bar(i), i == kQEmpty ? 10 : i == kPFull || i == kPFull + 1 ? 4 : i >= kFull + NS ? 2 : 1);
     fence_mbar_init();
-    for (int i = 0; i < 4; ++i) odd_pair[i / 2][i % 2] = 0;
+    odd_pair[0] = odd_pair[1] = 0;
   }
   if (warp == kMmaWarp) {
     tmem_alloc(smem_u32(&tmem_holder), 512);
@@ -403,14 +403,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         // Keys that some row does not see: its weights are 0, and 0 times an infinity or NaN is not. The four warps clear their quarters
-        // of the 64 values before this tile's product may read them. (The other tile's may be under way: its own warps have cleared
-        // them, and what is written here is what is there.) The item before this one in its stage has long landed.
+        // of the 64 values before this tile's product may read them. (The other tile's product may be under way: its own warps have
+        // cleared them, and what is written here is what is there.) The item before this one in its stage has long landed.
         if (u >= now.whole) {
           const int item = item0 + u / 2 * 2 + 1;
           ok = wait_warp(full(item % NS), (item / NS) & 1, &g_seq_fwd_errors, kErrSoftmax);
           if (!ok) break;
-          const bool odd = clear_not_finite<T, DP / 64, kKeys / 4>(smem + (2 + item % NS) * L::kTileBytes + ((u & 1) * 4 + warp % 4) * (kKeys / 4 * 128));
-          if (odd && lane == 0) *const_cast<volatile int *>(&odd_pair[done & 1][t]) = done + 1;
+          clear_not_finite<T, DP / 64, kKeys / 4>(smem + (2 + item % NS) * L::kTileBytes + ((u & 1) * 4 + warp % 4) * (kKeys / 4 * 128),
+                                                  &odd_pair[done & 1], done + 1);
         }
         tmem_wait_st();
         tc_fence_before();
@@ -445,8 +445,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (p.lse && there)
         p.lse[(int64_t)head * p.a.q_rows + now.r.q0 + row] = seen > 0 ? (m * sc + log2f(l)) * 0.6931471805599453f : -INFINITY;
-      // what was cleared, for the rows that see it: written before the arrival that the last product waited for
-      if (mine && *const_cast<volatile int *>(&odd_pair[done & 1][t]) == done + 1)
+      // what was cleared, by this tile's warps or the other's, for the rows that see it
+      if (mine && *const_cast<volatile int *>(&odd_pair[done & 1]) == done + 1)
         add_not_finite<T>(p.a, now.r, now.kv, now.whole * kKeys, at, seen, out);
       item0 += 2 * now.chunks();
       tc_fence_before();   // O is read before the next pair's P lets a product write it

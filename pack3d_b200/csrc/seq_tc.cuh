@@ -183,10 +183,11 @@ __device__ __forceinline__ void clear_rows(uint8_t *tile, int first) {
   fence_proxy_async_smem();
   __syncwarp();
 }
-// `kRows` rows of each box from `tile` on (shared memory, by a warp): infinities and NaN become 0; whether there were any. All finite, it
-// costs a load and four additions of zeros for 16 bytes.
+// `kRows` rows of each box from `tile` on (shared memory, by a warp): infinities and NaN become 0. Where there are any, *flag becomes `value`, and
+// it does before they go: another warp that finds them cleared finds the flag. All finite, it costs a load and four additions of zeros
+// for 16 bytes.
 template <typename T, int kBoxes, int kRows>
-__device__ __forceinline__ bool clear_not_finite(uint8_t *tile) {
+__device__ __forceinline__ void clear_not_finite(uint8_t *tile, volatile int *flag, int value) {
   constexpr int kEach = kRows * 128 / 512;   // loads of a lane in a box
   constexpr uint32_t kExp = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
   uint4 w[kBoxes * kEach];
@@ -200,7 +201,13 @@ __device__ __forceinline__ bool clear_not_finite(uint8_t *tile) {
     w[i] = *reinterpret_cast<const uint4 *>(tile + i / kEach * kBox + i % kEach * 512 + (threadIdx.x & 31) * 16);
 #pragma unroll
   for (int i = 0; i < kBoxes * kEach; ++i) add(w[i].x), add(w[i].y), add(w[i].z), add(w[i].w);
-  if (!__any_sync(0xffffffffu, (sum & 0x7fff7fffu) != 0)) return false;
+  if (!__any_sync(0xffffffffu, (sum & 0x7fff7fffu) != 0)) {
+    if (*flag == value) fence_proxy_async_smem();   // what another warp has written, for this one's product
+    return;
+  }
+  if ((threadIdx.x & 31) == 0) *flag = value;
+  __threadfence_block();
+  __syncwarp();
   auto clean = [&](uint32_t &v) {
     if ((v & kExp) == kExp) v &= 0xffff0000u;
     if ((v & kExp << 16) == kExp << 16) v &= 0xffffu;
@@ -211,7 +218,6 @@ __device__ __forceinline__ bool clear_not_finite(uint8_t *tile) {
     *reinterpret_cast<uint4 *>(tile + i / kEach * kBox + i % kEach * 512 + (threadIdx.x & 31) * 16) = w[i];
   }
   fence_proxy_async_smem();
-  return true;
 }
 __device__ __forceinline__ bool not_finite(float v) { return (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u; }
 

@@ -90,6 +90,25 @@ def test_every_score_minus_infinity(cuda_device, dtype, keys):
         assert got[:n].isnan().all() and torch.equal(got[n:], before[n:])
 
 
+@pytest.mark.parametrize("value", [NAN, INF, -INF])
+@pytest.mark.parametrize("heads,kv,dim", [(2, 1, 64), (3, 3, 128), (8, 1, 48), (16, 4, 128)])
+def test_a_value_reaches_every_row_that_sees_it(cuda_device, value, heads, kv, dim):
+    """Two tiles of queries share what is cleared of their values, in any order: at every place of a tile, over many sequences."""
+    from pack3d_b200 import sequence_attention
+    n, count = 256, 64
+    offsets = offsets_of([n] * count, cuda_device)
+    q, k, v = (randn(n * count, h, dim, device=cuda_device, seed=s, dtype=BF16) for s, h in enumerate((heads, kv, kv)))
+    clean = sequence_attention(q, k, v, offsets).view(count, n, heads, dim)
+    at = torch.arange(count, device=cuda_device) * 4 + 1
+    v.view(count, n, kv, dim)[torch.arange(count, device=cuda_device), at, 0, 3] = value
+    sees = (torch.arange(n, device=cuda_device) >= at[:, None])[..., None]
+    want = clean.clone()
+    want[..., :heads // kv, 3] = torch.where(sees, value, want[..., :heads // kv, 3])
+    for _ in range(5):
+        out = sequence_attention(q, k, v, offsets).view(count, n, heads, dim)
+        assert torch.equal(out.nan_to_num(3.25), want.nan_to_num(3.25))
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("value", [NAN, INF, -INF])
 @pytest.mark.parametrize("heads,kv,dim", [(8, 2, 128), (3, 3, 64)])
