@@ -62,63 +62,44 @@ __device__ __forceinline__ void load_columns(uint32_t t, float *v) {
   for (int i = 0; i < N; i += 32) tmem_ld32(t + i, reinterpret_cast<uint32_t *>(v) + i);
 }
 
-// 64 columns of an accumulator in 16 bits (zeros unless `write`); returns NaN where any of those below dim is not finite.
+// 64 columns of an accumulator in 16 bits (zeros unless `write`).
 template <typename T>
-__device__ __forceinline__ float pack_columns(uint32_t t, int col, int dim, bool write, uint32_t (&packed)[32]) {
-  float odd = 0.f;
+__device__ __forceinline__ void pack_columns(uint32_t t, bool write, uint32_t (&packed)[32]) {
 #pragma unroll
   for (int h = 0; h < 64; h += 32) {
     uint32_t o[32];
     tmem_ld32(t + h, o);
     tmem_wait_ld();
 #pragma unroll
-    for (int k = 0; k < 32; k += 2) {
-      const float a = write ? __uint_as_float(o[k]) : 0.f, b = write ? __uint_as_float(o[k + 1]) : 0.f;
-      if (col + h + k < dim) odd = fmaf(a, 0.f, fmaf(b, 0.f, odd));
-      packed[(h + k) / 2] = pack<T>(a, b);
-    }
+    for (int k = 0; k < 32; k += 2)
+      packed[(h + k) / 2] = pack<T>(write ? __uint_as_float(o[k]) : 0.f, write ? __uint_as_float(o[k + 1]) : 0.f);
   }
-  return odd;
 }
 
-// One row of dQ by the definition (a warp); columns of the half that found it.
-template <typename T>
-__device__ __noinline__ void redo_dq(const Params &p, const Range &r, int head, int row, int seen, int half, T *out) {
-  const p3d_sequence &a = p.a;
-  const int kv = head / (a.heads / a.kv_heads), dim = a.dim, lane = threadIdx.x & 31;
-  float q[4], d[4], k[4], v[4], sum[4] = {0.f, 0.f, 0.f, 0.f};
-  load4(static_cast<const T *>(a.q) + (int64_t)(r.q0 + row) * a.q_stride[0] + head * a.q_stride[1], dim, q);
-  load4(static_cast<const T *>(p.dout) + ((int64_t)(r.q0 + row) * a.heads + head) * dim, dim, d);
-  const float2 stat = p.stats[(int64_t)head * a.q_rows + r.q0 + row];
-  for (int j = 0; j < seen; ++j) {
-    load4(static_cast<const T *>(a.k) + (int64_t)(r.k0 + j) * a.k_stride[0] + kv * a.k_stride[1], dim, k);
-    load4(static_cast<const T *>(a.v) + (int64_t)(r.k0 + j) * a.v_stride[0] + kv * a.v_stride[1], dim, v);
-    const float ds = exp2f(dot4(q, k) * p.sc + stat.x) * (seen == 1 ? 0.f * dot4(d, v) : fmaf(dot4(d, v), a.scale, stat.y));
+// The same for dV from gradient rows of the queries [first, i) of `heads` heads: a warp's keys see the fewer of them the further down they
+// are. `at` (-1 for none) and `from` (it sees the rows from there on) are of a lane's key.
+template <typename T, typename Out>
+__device__ __noinline__ void add_gradients_not_finite(const T *dout, int64_t stride, int heads, int dim, int first, int i, int64_t at, int from,
+                                                       Out *out) {
+  const int c = (threadIdx.x & 31) * 4;
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int key = 31; key >= 0; --key) {
+    const int64_t to = __shfl_sync(0xffffffffu, at, key);
+    const int down = max(first, __shfl_sync(0xffffffffu, from, key));
+    if (to < 0) continue;
+    while (i > down) {
+      --i;
+      for (int h = 0; h < heads; ++h) {
+        float v[4];
+        load4(dout + i * stride + h * dim, dim, v);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) sum[i] = fmaf(ds, k[i], sum[i]);
-  }
-  // 64 columns each for the two groups of warps
-  if (lane / 16 == half) mend4(out, dim, sum);
-}
-
-// One key's row of dK (or dV) from the queries of `heads` heads that see it, by the definition (a warp): added up in four columns a lane.
-template <typename T>
-__device__ __noinline__ void redo_dkv(const Params &p, const Range &r, int kv, int head0, int heads, int key, int from, bool values,
-                                      float (&sum)[4]) {
-  const p3d_sequence &a = p.a;
-  float q[4], d[4], k[4], v[4];
-  load4(static_cast<const T *>(a.k) + (int64_t)(r.k0 + key) * a.k_stride[0] + kv * a.k_stride[1], a.dim, k);
-  load4(static_cast<const T *>(a.v) + (int64_t)(r.k0 + key) * a.v_stride[0] + kv * a.v_stride[1], a.dim, v);
-  sum[0] = sum[1] = sum[2] = sum[3] = 0.f;
-  for (int head = head0; head < head0 + heads; ++head)
-    for (int i = from; i < r.nq; ++i) {
-      load4(static_cast<const T *>(a.q) + (int64_t)(r.q0 + i) * a.q_stride[0] + head * a.q_stride[1], a.dim, q);
-      load4(static_cast<const T *>(p.dout) + ((int64_t)(r.q0 + i) * a.heads + head) * a.dim, a.dim, d);
-      const float2 stat = p.stats[(int64_t)head * a.q_rows + r.q0 + i];
-      const float w = exp2f(dot4(q, k) * p.sc + stat.x), ds = w * (r.nk == 1 ? 0.f * dot4(d, v) : fmaf(dot4(d, v), a.scale, stat.y));
-#pragma unroll
-      for (int c = 0; c < 4; ++c) sum[c] = values ? fmaf(w, d[c], sum[c]) : fmaf(ds, q[c], sum[c]);
+        for (int k = 0; k < 4; ++k) sum[k] += not_finite(v[k]) ? v[k] : 0.f;
+      }
     }
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (sum[k] != 0.f) out[to + c + k] = from_f32<Out>(to_f32<Out>(out[to + c + k]) + sum[k]);
+  }
 }
 
 // ------------------------------------------------------------------------------- dQ
@@ -144,6 +125,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t bar_mem[kBarsQ];
   __shared__ uint32_t tmem_holder;
+  __shared__ int odd_keys;   // keys have been cleared
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int slot = blockIdx.x / p.a.heads, head = blockIdx.x % p.a.heads;
   const int kv = head / (p.a.heads / p.a.kv_heads);
@@ -167,6 +149,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < kBarsQ; ++i) mbar_init(bar(i), i >= kDPFree && i < kDQDone ? kSoftmaxWarps : 1);
     fence_mbar_init();
+    odd_keys = 0;
   }
   if (warp == kMmaWarp) {
     tmem_alloc(smem_u32(&tmem_holder), 512);
@@ -312,6 +295,18 @@ __global__ void __launch_bounds__(kThreads, 1)
       tmem_wait_ld();
       const int limit = seen - c * kTile - half * 64;
       const bool masked = __any_sync(0xffffffffu, limit < 64);
+      if (masked) {
+        // Scores that are not finite where some row does not see the key: these 64 keys are cleared. Every warp that needs it does so, by
+        // now S has been made of them and dQ waits for all warps; what one has cleared another leaves as it is.
+        float2 odd = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) odd = fma2(make_float2(s[2 * i], s[2 * i + 1]), make_float2(0.f, 0.f), odd);
+        if (__any_sync(0xffffffffu, odd.x != odd.x || odd.y != odd.y)) {
+#pragma unroll 1
+          for (int i = 0; i < 4; ++i)
+            clear_not_finite<T, DP / 64, 16>(smem_raw + (k_ring - raw) + c % L::kK * TB + half * 8192 + i * 2048, &odd_keys, 1);
+        }
+      }
       weights(s, sc, [&](int) { return shift; });
       ok = wait_warp(bar(kDPFull), c & 1, &g_seq_bwd_errors, kErrSoftmax);
       if (!ok) break;
@@ -351,22 +346,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint8_t *const stage = smem_raw + (base - raw) + warp * 4096;
       const int64_t to = there ? ((int64_t)(r.q0 + row) * p.a.heads + head) * p.a.dim : -1;
       T *const dq = static_cast<T *>(p.dq);
-      float odd = 0.f;
       if (DP == 128 || half == 0) {
         const int col = DP == 128 ? half * 64 : 0;
         uint32_t packed[32];
-        odd = pack_columns<T>(t_dq + lanes + col, col, p.a.dim, seen > 0, packed);
+        pack_columns<T>(t_dq + lanes + col, seen > 0, packed);
         store_rows(stage, packed, dq, to, col, p.a.dim);
-      }
-      // rows beside keys that they do not see; with a NaN lse or delta they are NaN by right. Either group may find the row.
-      const int past = min(chunks * kTile, r.nk);
-      const bool look = there && odd != odd && seen > 0 && seen < past && stat.x == stat.x && stat.y == stat.y;
-      for (unsigned rows = __ballot_sync(0xffffffffu, look); rows; rows &= rows - 1) {
-        const int from = __ffs(rows) - 1, first = __shfl_sync(0xffffffffu, seen, from);
-        if (!rows_not_finite(static_cast<const T *>(p.a.k) + (int64_t)(r.k0 + first) * p.a.k_stride[0] + kv * p.a.k_stride[1],
-                             p.a.k_stride[0], past - first, p.a.dim))
-          continue;
-        redo_dq<T>(p, r, head, __shfl_sync(0xffffffffu, row, from), first, half, dq + __shfl_sync(0xffffffffu, to, from));
+        // written before an arrival that the last product waited for
+        if (*const_cast<volatile int *>(&odd_keys))
+          add_not_finite(static_cast<const T *>(p.a.k) + (int64_t)r.k0 * p.a.k_stride[0] + kv * p.a.k_stride[1], p.a.k_stride[0],
+                         seen_by(r, row0, p.a.causal) / kTile * kTile, col, min(col + 64, p.a.dim), true, to, seen, dq);
       }
     }
     tmem_wait_st();
@@ -402,6 +390,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t bar_mem[bars_kv<DP>()];
   __shared__ uint32_t tmem_holder;
+  __shared__ int odd_queries[NS];   // a stage has a query whose lse or delta is not finite
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // keys at a sequence's start are seen by the most queries
   const int per_slot = p.a.kv_heads * p.parts, slot = blockIdx.x / per_slot, kv = blockIdx.x % per_slot / p.parts,
@@ -489,6 +478,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         stats[s * 256 + lane + 32 * u] = v[u].x;
         stats[s * 256 + 128 + lane + 32 * u] = r.nk == 1 ? 0.f : v[u].y;
       }
+      const bool odd = __any_sync(0xffffffffu, not_finite(v[0].x + v[0].y) || not_finite(v[1].x + v[1].y) || not_finite(v[2].x + v[2].y) ||
+                                                 not_finite(v[3].x + v[3].y));
+      if (lane == 0) odd_queries[s] = odd;
       __syncwarp();
       // a head's last queries, where their tile goes past the sequence's end, land on a barrier of their own
       const bool past = i0 + kTile > r.nq;
@@ -572,7 +564,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const float one = r.nk == 1 ? 0.f : p.a.scale;
     const float2 sc = make_float2(p.sc, p.sc), scale = make_float2(one, one);
     const int from = p.a.causal ? key - shift : 0;   // the first query that sees this key
-    bool ok = true;
+    const int all_from = p.a.causal ? min(key0 + kTile, r.nk) - 1 - shift : 0;   // and that sees all of the tile's
+    bool ok = true, cleared = false;
     for (int i = 0, row = first; i < steps; ++i, row = row + kTile < r.nq ? row + kTile : first) {
       const int i0 = row + half * 64, lo = from - i0, hi = r.nq - i0;
       const bool masked = __any_sync(0xffffffffu, lo > 0 || hi < 64);
@@ -580,6 +573,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       ok = wait_warp(full(i % NS), (i / NS) & 1, &g_seq_bwd_errors, kErrSoftmax) &&
            wait_warp(bar(kSTFull), i & 1, &g_seq_bwd_errors, kErrSoftmax);
       if (!ok) break;
+      if (row < all_from && *const_cast<volatile int *>(&odd_queries[i % NS])) {
+        // Queries that some key is not seen by, one of them not finite: cleared, by each warp 16 rows, once S and dP have been made of
+        // them; dK and dV wait for all warps.
+        ok = wait_warp(bar(kDPTFull), i & 1, &g_seq_bwd_errors, kErrSoftmax);
+        if (!ok) break;
+        uint8_t *const tile = smem + 2 * TB + i % NS * L::kStageBytes + warp * 2048;
+        clear_not_finite<T, DP / 64, 16>(tile, &odd_queries[i % NS], 1);
+        clear_not_finite<T, DP / 64, 16>(tile + TB, &odd_queries[i % NS], 1);
+        cleared = true;
+      }
       float s[64];
       load_columns<64>(t_s, s);
       tmem_wait_ld();
@@ -637,12 +640,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       T *const narrow = half ? static_cast<T *>(p.dv) : static_cast<T *>(p.dk);
       float *const wide = half ? wide_v : wide_k;
       const uint32_t t_out = (half ? t_dv : t_dk) + lanes;
-      float odd = 0.f;
 #pragma unroll
       for (int i = 0; i < DP; i += 64) {
         uint32_t packed[32];
         if (!wide) {
-          odd += pack_columns<T>(t_out + i, i, p.a.dim, true, packed);
+          pack_columns<T>(t_out + i, true, packed);
           if (narrow) store_rows(stage, packed, narrow, there ? out_row : -1, i, p.a.dim);
         } else {
 #pragma unroll
@@ -652,10 +654,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             tmem_wait_ld();
 #pragma unroll
             for (int k = 0; k < 32; k += 4) {
-              if (i + h + k >= p.a.dim) continue;
-#pragma unroll
-              for (int c = 0; c < 4; ++c) odd = fmaf(__uint_as_float(o[k + c]), 0.f, odd);
-              if (there)
+              if (there && i + h + k < p.a.dim)
                 *reinterpret_cast<float4 *>(wide + out_row + i + h + k) =
                     make_float4(__uint_as_float(o[k]), __uint_as_float(o[k + 1]), __uint_as_float(o[k + 2]), __uint_as_float(o[k + 3]));
             }
@@ -663,26 +662,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       __syncwarp();
-      // Keys beside queries that do not see them: those of the tiles before `from`. A key whose first query has a NaN lse is NaN by right.
-      const int begin = max(from, 0);
-      const bool look = there && odd != odd && begin < r.nq && (narrow || wide);
-      for (unsigned rows = __ballot_sync(0xffffffffu, look); rows; rows &= rows - 1) {
-        const int lane_of = __ffs(rows) - 1, at_row = __shfl_sync(0xffffffffu, begin, lane_of), key_of = __shfl_sync(0xffffffffu, key, lane_of);
-        const float lse = p.stats[(int64_t)head0 * p.a.q_rows + r.q0 + at_row].x;
-        if (lse != lse) continue;
-        bool found = false;
-        for (int h = head0; h < head0 + heads && !found; ++h) {
-          const T *q = static_cast<const T *>(p.a.q) + (int64_t)r.q0 * p.a.q_stride[0] + h * p.a.q_stride[1];
-          const T *d = static_cast<const T *>(p.dout) + ((int64_t)r.q0 * p.a.heads + h) * p.a.dim;
-          const int64_t qs = p.a.q_stride[0], ds = (int64_t)p.a.heads * p.a.dim;
-          found = rows_not_finite(half ? d + first * ds : q + first * qs, half ? ds : qs, at_row - first, p.a.dim);
-        }
-        if (!found) continue;
-        float sum[4];
-        redo_dkv<T>(p, r, kv, head0, heads, key_of, at_row, half, sum);
-        const int64_t to = __shfl_sync(0xffffffffu, out_row, lane_of);
-        if (wide) mend4(wide + to, p.a.dim, sum);
-        else mend4(narrow + to, p.a.dim, sum);
+      if (cleared && half && (narrow || wide)) {   // all in the heads' first tiles
+        const T *const d = static_cast<const T *>(p.dout) + ((int64_t)r.q0 * p.a.heads + head0) * p.a.dim;
+        const int64_t to = there ? out_row : -1;
+        if (wide) add_gradients_not_finite(d, (int64_t)p.a.heads * p.a.dim, heads, p.a.dim, first, min(first + kTile, r.nq), to, from, wide);
+        else add_gradients_not_finite(d, (int64_t)p.a.heads * p.a.dim, heads, p.a.dim, first, min(first + kTile, r.nq), to, from, narrow);
       }
     }
     tmem_wait_st();

@@ -127,28 +127,6 @@ __device__ __forceinline__ float weights(const float (&s)[kKeys], float sc, floa
   return both.x + both.y;
 }
 
-// Adds what clear_not_finite took out of the values from key j on to a warp's rows that see it: rows see the more keys the further down they
-// are, so one pass over the keys serves all of them. `at` (a row's place in out, -1 for none) and `seen` are of a lane's row.
-template <typename T>
-__device__ __noinline__ void add_not_finite(const p3d_sequence &a, const Range &r, int kv, int j, int64_t at, int seen, T *out) {
-  const int c = (threadIdx.x & 31) * 4;
-  float sum[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int from = 0; from < 32; ++from) {
-    const int64_t to = __shfl_sync(0xffffffffu, at, from);
-    const int upto = __shfl_sync(0xffffffffu, seen, from);
-    if (to < 0) break;
-    for (; j < upto; ++j) {
-      float v[4];
-      load4(static_cast<const T *>(a.v) + (int64_t)(r.k0 + j) * a.v_stride[0] + kv * a.v_stride[1], a.dim, v);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) sum[i] += not_finite(v[i]) ? v[i] : 0.f;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (sum[i] != 0.f) out[to + c + i] = from_f32<T>(to_f32<T>(out[to + c + i]) + sum[i]);
-  }
-}
-
 template <typename T, int DP>
 __global__ void __launch_bounds__(kThreads, 1)
     sequence_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
@@ -447,7 +425,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         p.lse[(int64_t)head * p.a.q_rows + now.r.q0 + row] = seen > 0 ? (m * sc + log2f(l)) * 0.6931471805599453f : -INFINITY;
       // what was cleared, by this tile's warps or the other's, for the rows that see it
       if (mine && *const_cast<volatile int *>(&odd_pair[done & 1]) == done + 1)
-        add_not_finite<T>(p.a, now.r, now.kv, now.whole * kKeys, at, seen, out);
+        add_not_finite(static_cast<const T *>(p.a.v) + (int64_t)now.r.k0 * p.a.v_stride[0] + now.kv * p.a.v_stride[1], p.a.v_stride[0],
+                       now.whole * kKeys, 0, p.a.dim, false, at, seen, out);
       item0 += 2 * now.chunks();
       tc_fence_before();   // O is read before the next pair's P lets a product write it
     }

@@ -168,13 +168,16 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
 
 // Masked weights and values that are not finite.  A masked weight is 0, but 0 times an infinity or NaN is NaN: a product over a whole tile
 // would pass on what a row does not see. So in tiles that some row does not see whole, such values are set to 0 before the product reads
-// them, and added again to the rows that see them once the sum is there: an infinity whose weight is positive makes the sum that infinity, two
-// that meet make it NaN. Each such value is looked at once for 32 rows, so the work is bounded by what is read anyway.
-// * Forward: the softmax warps look through the values of those tiles (clear_not_finite) before they hand over their weights; rows behind the end
-//   of a sequence (another sequence's, or memory that nobody filled) are among them.
-// * Backward: rows of a tile behind the end of its sequence are cleared by the copying warp, which has it land on a barrier of its own (clear_rows).
-//   Within a sequence, rows whose result is not finite, beside values that they do not see, have those columns made again by their
-//   definition, a warp to a row (rows_not_finite, mend4, and the redo functions of each kernel).
+// them (clear_not_finite), and added again to the rows that see them once the sum is there (add_not_finite): an infinity whose weight is
+// positive makes the sum that infinity, two that meet make it NaN. Each such value is looked at once for 32 rows, so the work is bounded
+// by what is read anyway, whatever the values are.
+// * Forward: the softmax warps look through the values of those tiles before they hand over their weights.
+// * dQ: a key that is not finite makes the scores of its column not finite, also of the rows that do not see it: the softmax warps have them.
+//   A query that sees the key has no score gradient there (its score is -inf: 0 times the infinity) or nowhere: NaN.
+// * dK, dV: a query or a gradient row that is not finite has an lse or a delta that is not. A key that such a query sees gets NaN from its
+//   weight; a gradient row's value is added to dV.
+// * Backward, rows of a tile behind the end of its sequence (another sequence's, or memory that nobody filled): cleared by the copying warp,
+//   which has the tile land on a barrier of its own (clear_rows). In the forward pass they are among what the softmax warps look at.
 template <int kBoxes>
 __device__ __forceinline__ void clear_rows(uint8_t *tile, int first) {
   for (int i = threadIdx.x & 31; i < (kTile - first) * 8; i += 32)
@@ -233,28 +236,28 @@ __device__ __forceinline__ void load4(const T *row, int dim, float (&v)[4]) {
     v[0] = v[1] = v[2] = v[3] = 0.f;
   }
 }
-__device__ __forceinline__ float dot4(const float (&a)[4], const float (&b)[4]) {
-  return warp_sum(a[0] * b[0] + a[1] * b[1] + a[2] * b[2] + a[3] * b[3]);
-}
-// Into the places of a row whose value is not finite.
+
+// Adds what is not finite in the rows from j on of `rows` (`stride` elements apart), from column lo up to hi, to a warp's rows of out that see
+// them. These see the more of them the further down they are, so one pass serves all. `at` (a row's place in out, -1 for none, which come
+// last) and `seen` (it sees the rows below) are of a lane's row. `as_nan`: whatever is not finite counts as NaN.
 template <typename T>
-__device__ __forceinline__ void mend4(T *row, int dim, const float (&v)[4]) {
+__device__ __noinline__ void add_not_finite(const T *rows, int64_t stride, int j, int lo, int hi, bool as_nan, int64_t at, int seen, T *out) {
+  const int c = (threadIdx.x & 31) * 4;
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int from = 0; from < 32; ++from) {
+    const int64_t to = __shfl_sync(0xffffffffu, at, from);
+    const int upto = __shfl_sync(0xffffffffu, seen, from);
+    if (to < 0) break;
+    for (; j < upto; ++j) {
+      float v[4];
+      load4(rows + j * stride, c < lo ? 0 : hi, v);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int c = (threadIdx.x & 31) * 4 + i;
-    if (c < dim && not_finite(to_f32<T>(row[c]))) row[c] = from_f32<T>(v[i]);
+      for (int i = 0; i < 4; ++i) sum[i] += not_finite(v[i]) ? as_nan ? NAN : v[i] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (sum[i] != 0.f) out[to + c + i] = from_f32<T>(to_f32<T>(out[to + c + i]) + sum[i]);
   }
-}
-// Whether any of `rows` rows from `from` on, `stride` elements apart, is not finite (by a warp).
-template <typename T>
-__device__ __forceinline__ bool rows_not_finite(const T *from, int64_t stride, int rows, int dim) {
-  bool found = false;
-  for (int j = 0; j < rows; ++j) {
-    float v[4];
-    load4(from + j * stride, dim, v);
-    found |= not_finite(v[0]) || not_finite(v[1]) || not_finite(v[2]) || not_finite(v[3]);
-  }
-  return __any_sync(0xffffffffu, found);
 }
 
 // A warp's 32 rows (a row a lane, 64 columns of 16 bits as 32 words) to memory by way of shared memory, whole lines at a time: `stage` is

@@ -90,6 +90,139 @@ def test_every_score_minus_infinity(cuda_device, dtype, keys):
         assert got[:n].isnan().all() and torch.equal(got[n:], before[n:])
 
 
+# ------------------------------------------------------------------------------- values that nobody before them sees
+def step(q, k, v, dout, offsets, causal=True, k_offsets=None):
+    """(out, dq, dk, dv) and the milliseconds that they took."""
+    from pack3d_b200 import sequence_attention
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+    start.record()
+    out = sequence_attention(*leaves, offsets, k_offsets, causal=causal)
+    grads = torch.autograd.grad(out, leaves, dout)
+    end.record()
+    end.synchronize()
+    return [out.detach(), *grads], start.elapsed_time(end)
+
+
+@pytest.mark.parametrize("value", [NAN, INF, -INF])
+@pytest.mark.parametrize("at", [0, 63, 64, 100, 255, 290])
+@pytest.mark.parametrize("heads,kv,dim", [(2, 1, 64), (3, 3, 128), (8, 1, 48)])
+def test_later_values_keep_out_of_earlier_rows(cuda_device, value, at, heads, kv, dim):
+    """A value, key, query or gradient row that is not finite: what does not see it keeps its bits, in every column."""
+    n = 300
+    offsets = offsets_of([n], cuda_device)
+    clean = [randn(n, h, dim, device=cuda_device, seed=s, dtype=BF16) for s, h in enumerate((heads, kv, kv, heads))]
+    want, _ = step(*clean, offsets)
+    for which in range(4):
+        tensors = [t.clone() for t in clean]
+        tensors[which][at, 0, 3] = value
+        got, _ = step(*tensors, offsets)
+        assert torch.equal(got[0][:at], want[0][:at]) and torch.equal(got[1][:at], want[1][:at])
+        if which in (0, 3):
+            assert all(torch.equal(got[i][at + 1:], want[i][at + 1:]) for i in (2, 3))
+        if which == 2:
+            # weights are positive: the column of every query that sees it, and no other
+            column = torch.full_like(got[0][at:, :heads // kv, 3], value)
+            assert torch.equal(got[0][at:, :heads // kv, 3].nan_to_num(7.0), column.nan_to_num(7.0))
+            keep = torch.arange(dim, device=cuda_device) != 3
+            assert torch.equal(got[0][at:][..., keep], want[0][at:][..., keep])
+        if which == 3:
+            # dv of every key that the row sees has the weight's sign in that column; the row's own score gradient is not finite
+            seen = got[3][:at + 1, 0, 3]
+            assert seen.isnan().all() if math.isnan(value) else (seen == value).all()
+            keep = torch.arange(dim, device=cuda_device) != 3
+            assert torch.equal(got[3][..., keep], want[3][..., keep])
+            assert (at == 0 or got[1][at, 0].isnan().any()) and not got[2][:at + 1, 0].isfinite().all()
+
+
+def test_signs_that_meet(cuda_device):
+    """A column with infinities of both signs is NaN from the second on, and the first one's sign in between; the same of gradients, from
+    the other end."""
+    n, dim = 400, 64
+    offsets = offsets_of([n], cuda_device)
+    q, k, v, dout = (randn(n, 1, dim, device=cuda_device, seed=s, dtype=BF16) for s in range(4))
+    for first, second in ((10, 50), (130, 140), (130, 300), (383, 390)):
+        x, d = v.clone(), dout.clone()
+        x[first, 0, 5], x[second, 0, 5], x[second, 0, 6] = INF, -INF, -INF
+        out = step(q, k, x, dout, offsets)[0][0][:, 0]
+        assert out[:first].isfinite().all() and (out[first:second, 5] == INF).all() and out[second:, 5].isnan().all()
+        assert out[:second, 6].isfinite().all() and (out[second:, 6] == -INF).all() and out[:, 7:].isfinite().all()
+        d[first, 0, 5], d[second, 0, 5], d[first, 0, 6] = INF, -INF, -INF
+        dv = step(q, k, v, d, offsets)[0][3][:, 0]
+        assert dv[second + 1:].isfinite().all() and (dv[first + 1:second + 1, 5] == -INF).all() and dv[:first + 1, 5].isnan().all()
+        assert dv[first + 1:, 6].isfinite().all() and (dv[:first + 1, 6] == -INF).all() and dv[:, 7:].isfinite().all()
+
+
+@pytest.mark.parametrize("prefix", [0, 70, -40])
+@pytest.mark.parametrize("heads,kv", [(4, 1), (3, 3)])
+def test_prefix_with_values_that_are_not_finite(cuda_device, prefix, heads, kv):
+    """Keys of other lengths than the queries: masks that begin anywhere in a tile, and rows that see nothing."""
+    lengths = [129, 1, 64, 200]
+    keys = [max(0, n + prefix) for n in lengths]
+    offsets, k_offsets = offsets_of(lengths, cuda_device), offsets_of(keys, cuda_device)
+    clean = [randn(sum(r), h, 80, device=cuda_device, seed=s, dtype=F16) for s, (h, r) in enumerate(((heads, lengths), (kv, keys), (kv, keys), (heads, lengths)))]
+    want, _ = step(*clean, offsets, k_offsets=k_offsets)
+    at = sum(lengths[:3]) + 100
+    key = sum(keys[:3]) + 100 + prefix            # what query 100 of the last sequence sees last
+    for which in range(4):
+        tensors = [t.clone() for t in clean]
+        tensors[which][at if which in (0, 3) else key, 0, 2] = NAN if which == 1 else INF   # -inf scores would have no weight
+        got, _ = step(*tensors, offsets, k_offsets=k_offsets)
+        if which in (1, 2):                        # earlier queries, and all of the other sequences
+            assert torch.equal(got[0][:at], want[0][:at]) and torch.equal(got[1][:at], want[1][:at])
+            assert not got[0][at, 0].isfinite().all()
+        else:                                      # later keys, and the other sequences' ones
+            for i in (2, 3):
+                assert torch.equal(got[i][key + 1:], want[i][key + 1:])
+                assert torch.equal(got[i][:sum(keys[:3])], want[i][:sum(keys[:3])])
+                assert not got[i][key, 0].isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("what", ["dout nan", "dout inf", "dout one inf a row", "v channel", "v nan", "k channel", "q nan"])
+def test_many_that_are_not_finite(cuda_device, what, dtype):
+    """A step whose values have overflown, at a length where work that grows with its square would show: as every value is looked at a
+    bounded number of times, it stays within 30 ms (all finite: about one)."""
+    n, heads, kv, dim = 8192, 8, 2, 128
+    offsets = offsets_of([n], cuda_device)
+    q, k, v, dout = (randn(n, h, dim, device=cuda_device, seed=s, dtype=dtype) for s, h in enumerate((heads, kv, kv, heads)))
+    clean, _ = step(q, k, v, dout, offsets)
+    if what == "dout nan":
+        dout[:] = NAN
+    elif what == "dout inf":
+        dout[:] = INF
+    elif what == "dout one inf a row":
+        dout[:, :, 9] = INF
+    elif what == "v channel":
+        v[:, :, 9] = INF
+    elif what == "v nan":
+        v[:] = NAN
+    elif what == "k channel":
+        k[:, :, 9] = INF
+    else:
+        q[:] = NAN
+    (out, dq, dk, dv), ms = step(q, k, v, dout, offsets)
+    assert ms < 30
+    keep = torch.arange(dim, device=cuda_device) != 9
+    if what.startswith("dout"):
+        assert torch.equal(out, clean[0])
+        if what == "dout one inf a row":
+            assert (dv[..., 9] == INF).all() and torch.equal(dv[..., keep], clean[3][..., keep])
+        elif what == "dout nan":
+            assert dv.isnan().all() and dq.isnan().all() and dk.isnan().all()
+        else:
+            assert (dv == INF).all()
+    elif what == "v channel":
+        assert (out[..., 9] == INF).all() and torch.equal(out[..., keep], clean[0][..., keep])
+    elif what == "v nan":
+        assert out.isnan().all()
+    elif what == "q nan":
+        assert out.isnan().all() and dq.isnan().all() and dk.isnan().all() and dv.isnan().all()
+    else:
+        # queries see an infinite key of either sign: NaN where any score is +inf, and where all are -inf
+        assert out.isnan().all() and dq.isnan().all()
+
+
 @pytest.mark.parametrize("value", [NAN, INF, -INF])
 @pytest.mark.parametrize("heads,kv,dim", [(2, 1, 64), (3, 3, 128), (8, 1, 48), (16, 4, 128)])
 def test_a_value_reaches_every_row_that_sees_it(cuda_device, value, heads, kv, dim):
