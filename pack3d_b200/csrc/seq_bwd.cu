@@ -2,9 +2,14 @@
 //
 //     P = 2^(S c - lse),  dS = scale P (dO V^T - delta),  dQ = dS K,  dK = dS^T Q,  dV = P^T dO
 //
-// (dS with its scale, so that in f16 it stays in range where the gradients do.) Where a query sees a single key, P is 1 and dS is 0;
-// dP - delta, two sums of the same products, would leave the rounding of their orders: scale and delta are 0 there (in dK: where a sequence
-// has one key. Among more keys, whose gradients are sums over many queries, that rounding is as small as any).
+// In f16 neither P nor dS fits as it is: both get small as keys get many, while the sums over them do not (4,096 keys and a dO of 1e-4: dQ and
+// dK off by a tenth), and a large dO overflows dS. So P is held 2^10 times as large for dV, and dS by the power of two that brings the
+// largest that it can be, scale |dO_i| max |V_j| + |scale delta_i|, to 2^11 .. 2^12: of a query in dQ, of the whole tile's queries and keys in
+// dK, of its own sequence in any case. Sums are brought back in fp32. The norms come from the kernel that makes delta.
+//
+// Where a query sees a single key, P is 1 and dS is 0; dP - delta, two sums of the same products, would leave the rounding of their orders:
+// scale and delta are 0 there (in dK: where a sequence has one key. Among more keys, whose gradients are sums over many queries, that
+// rounding is as small as any).
 //
 // Two kernels, so that each gradient is a sum in one fixed order without atomics: dQ by tiles of queries, dK and dV by tiles of keys.
 // They make S and dP both, seven products of which five are the mathematics' own (a tile of 128 x 128 is 512 cycles a product).
@@ -35,6 +40,8 @@ constexpr int kMmaWarp = 8, kCopyWarp = 10, kThreads = 352, kSoftmaxWarps = 8;  
 struct Params {
   p3d_sequence a;
   const float2 *stats;     // [heads][q_rows]: -lse * log2(e), -scale * delta
+  const float *dout_norm;  // [heads][q_rows], f16 only
+  const float *v_norm;     // [kv_heads][k_rows], f16 only
   const void *dout;        // contiguous
   void *dq, *dk, *dv;
   float *part;             // [2][parts][k_rows * kv_heads * dim] where parts > 1
@@ -62,17 +69,32 @@ __device__ __forceinline__ void load_columns(uint32_t t, float *v) {
   for (int i = 0; i < N; i += 32) tmem_ld32(t + i, reinterpret_cast<uint32_t *>(v) + i);
 }
 
-// 64 columns of an accumulator in 16 bits (zeros unless `write`).
+template <typename T> constexpr bool kScaled = std::is_same<T, __half>::value;   // P and dS are
+constexpr int kWeightUp = 10;
+__device__ __forceinline__ float two_to(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
+// The power of two that brings `most` (not negative) to 2^11 .. 2^12, as far as 2^+-100.
+__device__ __forceinline__ int exponent_for(float most) {
+  return min(max(138 - (int)(__float_as_uint(most) >> 23 & 255u), -100), 100);
+}
+__device__ __forceinline__ float finite_or_0(float v) { return not_finite(v) ? 0.f : v; }
+__device__ __forceinline__ float warp_most(float v) {   // of values that are not negative
+  return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v)));
+}
+
+// 64 columns of an accumulator, times `factor` (f16), in 16 bits (zeros unless `write`).
 template <typename T>
-__device__ __forceinline__ void pack_columns(uint32_t t, bool write, uint32_t (&packed)[32]) {
+__device__ __forceinline__ void pack_columns(uint32_t t, bool write, float factor, uint32_t (&packed)[32]) {
 #pragma unroll
   for (int h = 0; h < 64; h += 32) {
     uint32_t o[32];
     tmem_ld32(t + h, o);
     tmem_wait_ld();
 #pragma unroll
-    for (int k = 0; k < 32; k += 2)
-      packed[(h + k) / 2] = pack<T>(write ? __uint_as_float(o[k]) : 0.f, write ? __uint_as_float(o[k + 1]) : 0.f);
+    for (int k = 0; k < 32; k += 2) {
+      float2 v = make_float2(__uint_as_float(o[k]), __uint_as_float(o[k + 1]));
+      if constexpr (kScaled<T>) v = mul2(v, make_float2(factor, factor));
+      packed[(h + k) / 2] = pack<T>(write ? v.x : 0.f, write ? v.y : 0.f);
+    }
   }
 }
 
@@ -126,6 +148,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ __align__(8) uint64_t bar_mem[kBarsQ];
   __shared__ uint32_t tmem_holder;
   __shared__ int odd_keys;   // keys have been cleared
+  __shared__ float most_v[kThreads / 32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int slot = blockIdx.x / p.a.heads, head = blockIdx.x % p.a.heads;
   const int kv = head / (p.a.heads / p.a.kv_heads);
@@ -160,6 +183,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     prefetch_tmap(&tdo);
     prefetch_tmap(&tk);
     prefetch_tmap(&tv);
+  }
+  if constexpr (kScaled<T>) {
+    const float *norm = p.v_norm + kv * p.a.k_rows + r.k0;
+    float most = 0.f;
+#pragma unroll 4
+    for (int j = threadIdx.x; j < min(chunks * kTile, r.nk); j += kThreads) most = fmaxf(most, finite_or_0(norm[j]));
+    most_v[warp] = warp_most(most);
   }
   tc_fence_before();
   __syncthreads();
@@ -282,7 +312,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     const bool there = row < r.nq;
     const int seen = there ? seen_by(r, row, p.a.causal) : 0;
     const float2 stat = there ? p.stats[(int64_t)head * p.a.q_rows + r.q0 + row] : make_float2(0.f, 0.f);
-    const float one = seen == 1 ? 0.f : p.a.scale, less = seen == 1 ? 0.f : stat.y;
+    int up = 0;   // dS is 2^up times as large
+    if constexpr (kScaled<T>) {
+      float v = most_v[0];
+      for (int i = 1; i < kThreads / 32; ++i) v = fmaxf(v, most_v[i]);
+      if (there) up = exponent_for(fmaf(p.dout_norm[(int64_t)head * p.a.q_rows + r.q0 + row], p.a.scale * v, fabsf(stat.y)));
+    }
+    const float one = seen == 1 ? 0.f : p.a.scale * two_to(up), less = seen == 1 ? 0.f : stat.y * two_to(up);
     const float2 sc = make_float2(p.sc, p.sc), shift = make_float2(stat.x, stat.x), minus = make_float2(less, less), scale = make_float2(one, one);
     const uint32_t lanes = (uint32_t)((warp % 4) * 32) << 16;
     bool ok = true;
@@ -349,7 +385,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (DP == 128 || half == 0) {
         const int col = DP == 128 ? half * 64 : 0;
         uint32_t packed[32];
-        pack_columns<T>(t_dq + lanes + col, seen > 0, packed);
+        pack_columns<T>(t_dq + lanes + col, seen > 0, two_to(-up), packed);
         store_rows(stage, packed, dq, to, col, p.a.dim);
         // written before an arrival that the last product waited for
         if (*const_cast<volatile int *>(&odd_keys))
@@ -391,6 +427,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ __align__(8) uint64_t bar_mem[bars_kv<DP>()];
   __shared__ uint32_t tmem_holder;
   __shared__ int odd_queries[NS];   // a stage has a query whose lse or delta is not finite
+  __shared__ float most[3][kThreads / 32];   // of the queries' |dO| and |scale delta|, the keys' |V|
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // keys at a sequence's start are seen by the most queries
   const int per_slot = p.a.kv_heads * p.parts, slot = blockIdx.x / per_slot, kv = blockIdx.x % per_slot / p.parts,
@@ -448,14 +485,37 @@ __global__ void __launch_bounds__(kThreads, 1)
     prefetch_tmap(&tk);
     prefetch_tmap(&tv);
   }
+  if constexpr (kScaled<T>) {
+    float n = 0.f, y = 0.f;
+    for (int64_t at = (int64_t)head0 * p.a.q_rows + r.q0, h = 0; h < heads; ++h, at += p.a.q_rows)
+#pragma unroll 4
+      for (int i = first + threadIdx.x; i < r.nq; i += kThreads) {
+        n = fmaxf(n, finite_or_0(p.dout_norm[at + i]));
+        y = fmaxf(y, finite_or_0(fabsf(p.stats[at + i].y)));
+      }
+    const int mine = key0 + threadIdx.x;
+    const float v = threadIdx.x < kTile && mine < r.nk ? finite_or_0(p.v_norm[kv * p.a.k_rows + r.k0 + mine]) : 0.f;
+    most[0][warp] = warp_most(n), most[1][warp] = warp_most(y), most[2][warp] = warp_most(v);
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_holder, t_dp = tmem + 128, t_dk = tmem + 256, t_dv = tmem + 384;
+  auto exponent = [&] {   // dS is that power of two times as large
+    if constexpr (kScaled<T>) {
+      float n = 0.f, y = 0.f, v = 0.f;
+      for (int i = 0; i < kThreads / 32; ++i) n = fmaxf(n, most[0][i]), y = fmaxf(y, most[1][i]), v = fmaxf(v, most[2][i]);
+      return exponent_for(fmaf(n, p.a.scale * v, y));
+    } else {
+      return 0;
+    }
+  };
+  constexpr int kUp = kScaled<T> ? kWeightUp : 0;   // and P
 
   if (warp == kCopyWarp) {
     bool ok = true;
     int issued = 0, cleared = 0;
+    const float times = two_to(exponent() - kUp);
     if (lane == 0) {
       mbar_expect_tx(bar(kKVFull), 2 * TB);
       for (int c = 0; c < DP / 64; ++c) {
@@ -475,8 +535,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!ok) break;
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        stats[s * 256 + lane + 32 * u] = v[u].x;
-        stats[s * 256 + 128 + lane + 32 * u] = r.nk == 1 ? 0.f : v[u].y;
+        stats[s * 256 + lane + 32 * u] = v[u].x + kUp;
+        stats[s * 256 + 128 + lane + 32 * u] = r.nk == 1 ? 0.f : v[u].y * times;
       }
       const bool odd = __any_sync(0xffffffffu, not_finite(v[0].x + v[0].y) || not_finite(v[1].x + v[1].y) || not_finite(v[2].x + v[2].y) ||
                                                  not_finite(v[3].x + v[3].y));
@@ -561,7 +621,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else {
     const int half = warp / 4;
     const uint32_t lanes = (uint32_t)((warp % 4) * 32) << 16, t_s = tmem + 64 * half + lanes, t_d = t_dp + 64 * half + lanes;
-    const float one = r.nk == 1 ? 0.f : p.a.scale;
+    const float one = r.nk == 1 ? 0.f : p.a.scale * two_to(exponent() - kUp);
     const float2 sc = make_float2(p.sc, p.sc), scale = make_float2(one, one);
     const int from = p.a.causal ? key - shift : 0;   // the first query that sees this key
     const int all_from = p.a.causal ? min(key0 + kTile, r.nk) - 1 - shift : 0;   // and that sees all of the tile's
@@ -640,11 +700,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       T *const narrow = half ? static_cast<T *>(p.dv) : static_cast<T *>(p.dk);
       float *const wide = half ? wide_v : wide_k;
       const uint32_t t_out = (half ? t_dv : t_dk) + lanes;
+      const float back = two_to(half ? -kUp : -exponent());
 #pragma unroll
       for (int i = 0; i < DP; i += 64) {
         uint32_t packed[32];
         if (!wide) {
-          pack_columns<T>(t_out + i, true, packed);
+          pack_columns<T>(t_out + i, true, back, packed);
           if (narrow) store_rows(stage, packed, narrow, there ? out_row : -1, i, p.a.dim);
         } else {
 #pragma unroll
@@ -656,7 +717,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int k = 0; k < 32; k += 4) {
               if (there && i + h + k < p.a.dim)
                 *reinterpret_cast<float4 *>(wide + out_row + i + h + k) =
-                    make_float4(__uint_as_float(o[k]), __uint_as_float(o[k + 1]), __uint_as_float(o[k + 2]), __uint_as_float(o[k + 3]));
+                    make_float4(__uint_as_float(o[k]) * back, __uint_as_float(o[k + 1]) * back, __uint_as_float(o[k + 2]) * back,
+                                __uint_as_float(o[k + 3]) * back);
             }
           }
         }
@@ -680,30 +742,53 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// -lse * log2(e) and -scale * delta of every row: a row is `lanes` lanes of 16 bytes.
+// Eight columns of a row as pairs; a lane past the row's end has zeros.
 template <typename T>
-__global__ void __launch_bounds__(256) stats_kernel(const T *out, const T *dout, const float *lse, float2 *stats, int64_t rows,
-                                                    int heads, int64_t tokens, int dim, int lanes, float scale) {
-  const int lane = threadIdx.x & 31, per_warp = 32 / lanes, col = lane % lanes * 8;
-  const int64_t stride = (int64_t)gridDim.x * 8 * per_warp;
+__device__ __forceinline__ void load8(const T *from, bool there, float2 (&v)[4]) {
+  const uint4 w = there ? __ldcs(reinterpret_cast<const uint4 *>(from)) : make_uint4(0, 0, 0, 0);
+  v[0] = unpack2<T>(w.x), v[1] = unpack2<T>(w.y), v[2] = unpack2<T>(w.z), v[3] = unpack2<T>(w.w);
+}
+// -lse * log2(e) and -scale * delta of every row, in f16 its |dO| and each value's norm too: a row is `lanes` lanes of 16 bytes.
+template <typename T>
+__global__ void __launch_bounds__(256) stats_kernel(const T *out, const float *lse, const __grid_constant__ Params p, float2 *stats,
+                                                    float *dout_norm, float *v_norm, int lanes) {
+  const T *const dout = static_cast<const T *>(p.dout);
+  const int lane = threadIdx.x & 31, per_warp = 32 / lanes, col = lane % lanes * 8, dim = p.a.dim;
+  const int64_t row_first = ((int64_t)blockIdx.x * 8 + threadIdx.x / 32) * per_warp, stride = (int64_t)gridDim.x * 8 * per_warp;
   // whole warps take part in the sums: rows past the last are zeros
-  for (int64_t row0 = ((int64_t)blockIdx.x * 8 + threadIdx.x / 32) * per_warp; row0 < rows; row0 += stride) {
+  for (int64_t row0 = row_first; row0 < p.a.q_rows * p.a.heads; row0 += stride) {
     const int64_t row = row0 + lane / lanes;
-    float sum = 0.f;
-    if (row < rows && col < dim) {
-      const uint4 a = __ldcs(reinterpret_cast<const uint4 *>(out + row * dim + col)), b = __ldcs(reinterpret_cast<const uint4 *>(dout + row * dim + col));
-      const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+    const bool there = row < p.a.q_rows * p.a.heads;
+    float2 a[4], b[4];
+    load8(out + row * dim + col, there && col < dim, a);
+    load8(dout + row * dim + col, there && col < dim, b);
+    float sum = 0.f, square = 0.f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 u = unpack2<T>(x[i]), v = unpack2<T>(y[i]);
-        sum = fmaf(u.x, v.x, fmaf(u.y, v.y, sum));
-      }
+    for (int i = 0; i < 4; ++i) {
+      sum = fmaf(a[i].x, b[i].x, fmaf(a[i].y, b[i].y, sum));
+      if constexpr (kScaled<T>) square = fmaf(b[i].x, b[i].x, fmaf(b[i].y, b[i].y, square));
     }
-    for (int o = lanes / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (row < rows && lane % lanes == 0) {
-      const int64_t t = row / heads;
-      const int64_t to = (row - t * heads) * tokens + t;
-      stats[to] = make_float2(lse[to] * -1.4426950408889634f, sum * -scale);
+    for (int o = lanes / 2; o > 0; o >>= 1) {
+      sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if constexpr (kScaled<T>) square += __shfl_xor_sync(0xffffffffu, square, o);
+    }
+    if (there && lane % lanes == 0) {
+      const int64_t t = row / p.a.heads, to = (row - t * p.a.heads) * p.a.q_rows + t;
+      stats[to] = make_float2(lse[to] * -1.4426950408889634f, sum * -p.a.scale);
+      if constexpr (kScaled<T>) dout_norm[to] = sqrtf(square);
+    }
+  }
+  if constexpr (kScaled<T>) {
+    for (int64_t row0 = row_first; row0 < p.a.k_rows * p.a.kv_heads; row0 += stride) {
+      const int64_t row = row0 + lane / lanes, t = row / p.a.kv_heads, head = row - t * p.a.kv_heads;
+      const bool there = row < p.a.k_rows * p.a.kv_heads;
+      float2 v[4];
+      load8(static_cast<const T *>(p.a.v) + t * p.a.v_stride[0] + head * p.a.v_stride[1] + col, there && col < dim, v);
+      float square = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) square = fmaf(v[i].x, v[i].x, fmaf(v[i].y, v[i].y, square));
+      for (int o = lanes / 2; o > 0; o >>= 1) square += __shfl_xor_sync(0xffffffffu, square, o);
+      if (there && lane % lanes == 0) v_norm[head * p.a.k_rows + t] = sqrtf(square);
     }
   }
 }
@@ -738,8 +823,8 @@ int launch_t(const Params &p, const void *out, const float *lse, float2 *stats, 
     int lanes = 1;
     while (lanes * 8 < a.dim) lanes *= 2;
     const int64_t blocks = std::min<int64_t>((rows * lanes + 255) / 256, 148 * 16);
-    stats_kernel<T><<<(unsigned)blocks, 256, 0, s>>>((const T *)out, (const T *)p.dout, lse, stats, rows, a.heads, a.q_rows, a.dim, lanes,
-                                                        a.scale);
+    stats_kernel<T><<<(unsigned)blocks, 256, 0, s>>>((const T *)out, lse, p, stats, const_cast<float *>(p.dout_norm),
+                                                        const_cast<float *>(p.v_norm), lanes);
     P3D_LAUNCH_CHECK();
     const int64_t dense[2] = {(int64_t)a.heads * a.dim, a.dim};
     if (int st = encode_heads(&tq, a.dtype, a.q, a.dim, a.heads, a.q_rows, a.q_stride)) return st;
@@ -782,7 +867,11 @@ int launch_t(const Params &p, const void *out, const float *lse, float2 *stats, 
   return P3D_OK;
 }
 
-size_t stats_bytes(const p3d_sequence &a) { return ((size_t)a.q_rows * a.heads * sizeof(float2) + 255) / 256 * 256; }
+size_t whole(size_t bytes) { return (bytes + 255) / 256 * 256; }
+size_t stats_bytes(const p3d_sequence &a) { return whole((size_t)a.q_rows * a.heads * sizeof(float2)); }
+size_t norm_bytes(const p3d_sequence &a) {   // of dO, then of V
+  return a.dtype == P3D_F16 ? whole(((size_t)a.q_rows * a.heads + (size_t)a.k_rows * a.kv_heads) * sizeof(float)) : 0;
+}
 
 }  // namespace
 
@@ -790,7 +879,7 @@ int bwd_workspace(const p3d_sequence &a, size_t *bytes) {
   DeviceInfo info;
   if (int st = device_info(&info)) return st;
   const int parts = parts_of(a, info.sm_count);
-  *bytes = stats_bytes(a) + (parts > 1 ? 2 * sizeof(float) * (size_t)parts * a.k_rows * a.kv_heads * a.dim : 0);
+  *bytes = stats_bytes(a) + norm_bytes(a) + (parts > 1 ? 2 * sizeof(float) * (size_t)parts * a.k_rows * a.kv_heads * a.dim : 0);
   return P3D_OK;
 }
 
@@ -810,7 +899,12 @@ int launch_bwd(const p3d_sequence &a, const void *out, const float *lse, const v
   p.stats = stats;
   p.parts = parts_of(a, info.sm_count);
   p.falling = falling(a, slots_of(a.k_rows, a.sequences, kTile) * a.kv_heads * p.parts, info.sm_count);
-  p.part = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + stats_bytes(a));
+  uint8_t *const after = static_cast<uint8_t *>(workspace) + stats_bytes(a);
+  if (a.dtype == P3D_F16) {
+    p.dout_norm = reinterpret_cast<float *>(after);
+    p.v_norm = p.dout_norm + a.q_rows * a.heads;
+  }
+  p.part = reinterpret_cast<float *>(after + norm_bytes(a));
   p.steps = (a.dim + 15) / 16;
   p.idesc_out = idesc_f16(128, p.steps * 16, a.dtype == P3D_BF16, true);
   p.sc = a.scale * 1.4426950408889634f;

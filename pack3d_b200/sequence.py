@@ -42,9 +42,10 @@ def sequence_attention(q, k, v, q_offsets, k_offsets=None, *, causal=True, scale
     A query that sees no key gives 0 and sends no gradient, as do rows behind the last sequence, whatever they hold.  An
     infinity or NaN reaches the queries that see it, and no other sequence.
 
-    fp16 or bf16, head_dim a multiple of 8 up to 128; rows that are not 16-byte aligned are copied first.  Scores, sums and
-    gradients in fp32, weights of the products rounded to the inputs' dtype.  Every sum has a fixed order, so the
-    gradients are bitwise repeatable.  Differentiable once, in reverse mode; second and forward-mode derivatives are
+    fp16 or bf16, head_dim a multiple of 8 up to 128; rows that are not 16-byte aligned are copied first.  Scores and sums in
+    fp32; what goes into a product (weights, and score gradients from the rounded output) is rounded to the inputs' dtype, in
+    fp16 times powers of two that bring it into range.  Every sum has a fixed order, so the gradients are bitwise
+    repeatable.  Differentiable once, in reverse mode; second and forward-mode derivatives are
     refused.
     """
     return _native.host().sequence_attention(q, k, v, q_offsets, k_offsets, causal, scale)

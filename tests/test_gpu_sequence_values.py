@@ -276,3 +276,90 @@ def test_infinite_value_at_the_end_of_a_long_sequence(cuda_device, heads, kv):
     out = sequence_attention(q, k, v, offsets)
     assert torch.equal(out[:199990], clean[:199990]) and torch.equal(out[200000:], clean[200000:])
     assert (out[199990:200000] == INF).all()
+
+
+# ------------------------------------------------------------------------------- gradients and weights of any size
+def coherent(n, heads, kv, dim, up, device, small=1.0):
+    """Queries, keys, values and upstream gradients whose score gradients are about 1 / n each and add up to results of the order of
+    `up`: V_j and K_j have a common sign each, dO one direction for all rows, and scores are near 0."""
+    def noise(h, s):
+        return randn(n, h, dim, device=device, seed=s, dtype=F32) * 0.1
+    gen = torch.Generator(device=device).manual_seed(9)
+    sign = torch.randint(0, 2, (n, kv, 1), generator=gen, device=device) * 2.0 - 1
+    g = torch.randint(0, 2, (dim,), generator=gen, device=device) * 2.0 - 1
+    half = torch.ones(dim, device=device)
+    half[dim // 2:] = -1
+    q = (0.5 * half + noise(heads, 1)) * small
+    k = (sign + noise(kv, 2)) * small
+    return q.half(), k.half(), (sign * g + noise(kv, 3)).half(), ((g + noise(heads, 4)) * up).half()
+
+
+def definition(q, k, v, dout, causal, scale):
+    """(out, dq, dk, dv) in 64 bits of one sequence, and how far a kernel may be off: weights p and score gradients ds are rounded to the
+    dtype before a product, half a step u relative, or half of the smallest f16 number beside 2^10 for p and beside 2^11 for the
+    largest that a row's (a key's) ds can be; exponentials are off by 2^-13, sums in fp32 by 2^-15 of magnitudes, out (which delta
+    comes from) by what its own rounding and its weights' make, results by half a step, or half of the smallest number."""
+    u, e, least = torch.finfo(q.dtype).eps / 2, 2.0 ** -13 + 2.0 ** -15, 2.0 ** -25
+    q, k, v, d = (t.double() for t in (q, k, v, dout))
+    n, h, g = q.shape[0], q.shape[1], k.shape[1]
+    out, grads, tols = torch.zeros_like(q), [torch.zeros_like(t) for t in (q, k, v)], [torch.zeros_like(t) for t in (q, k, v)]
+    for i in range(h):
+        j = i // (h // g)
+        s = q[:, i] @ k[:, j].t() * scale
+        if causal:
+            s = torch.where(torch.ones_like(s, dtype=torch.bool).tril(), s, -INF)
+        p = torch.softmax(s, -1)
+        o = p @ v[:, j]
+        out[:, i] = o
+        out_tol = u * o.abs() + (u + e) * (p @ v[:, j].abs())
+        dp = d[:, i] @ v[:, j].t()
+        delta = (d[:, i] * o).sum(-1, keepdim=True)
+        ds = p * (dp - delta) * scale
+        # the largest that ds of a row can be, by Cauchy and Schwarz, for the power of two that it is held in
+        most = scale * (d[:, i].norm(dim=-1, keepdim=True) * v[:, j].norm(dim=-1).max() + delta.abs())
+        wrong = scale * p * (e * (dp.abs() + delta.abs() + d[:, i].abs() @ v[:, j].abs().t()) + (d[:, i].abs() * out_tol).sum(-1, keepdim=True)) + u * ds.abs()
+        floor = least * 2.0 ** -11
+        grads[0][:, i] = ds @ k[:, j]
+        tols[0][:, i] = (wrong + e * ds.abs()) @ k[:, j].abs() + floor * most * k[:, j].abs().sum(0)
+        grads[1][:, j] += ds.t() @ q[:, i]
+        tols[1][:, j] += (wrong + e * ds.abs()).t() @ q[:, i].abs() + floor * most.max() * q[:, i].abs().sum(0)
+        grads[2][:, j] += p.t() @ d[:, i]
+        tols[2][:, j] += (u + 2 * e) * (p.t() @ d[:, i].abs()) + least * 2.0 ** -10 * d[:, i].abs().sum(0)
+        del s, p, dp, ds, wrong
+    return out, grads, [t + u * x.abs() + least for t, x in zip(tols, grads)]
+
+
+@pytest.mark.parametrize("causal,n", [(False, 12000), (True, 9001)])
+@pytest.mark.parametrize("heads,kv,dim", [(2, 1, 64), (1, 1, 128)])
+@pytest.mark.parametrize("up,small", [(2e-5, 1.0), (1e-3, 1.0), (2e4, 0.01)])
+def test_f16_gradients_of_any_size(cuda_device, causal, n, heads, kv, dim, up, small):
+    """Score gradients below what f16 holds that add up to results well within it, and above it with results that are not."""
+    q, k, v, dout = coherent(n, heads, kv, dim, up, cuda_device, small)
+    got, _ = step(q, k, v, dout, offsets_of([n], cuda_device), causal=causal)
+    _, want, tols = definition(q, k, v, dout, causal, dim ** -0.5)
+    for name, g, w, t in zip("qkv", got[1:], want, tols):
+        # the first keys' values have gradients of up to 2 * 2e4 * (1 + 1/2 + ..), past the largest f16 number: infinite, as rounded;
+        # where the error may carry them over that border, either
+        past = w.abs() >= 65520 + t
+        assert (g.double() == w.sign() * INF)[past].all() and (name == "v" or not past.any())
+        past |= (w.abs() > 65520 - t) & (g.double() == w.sign() * INF)
+        off = torch.where(past, 0.0, (g.double() - w).abs())
+        assert (off <= t).all(), f"d{name}: {float((off / t).max()):.2f} x the tolerance, {float(off.norm() / w.norm()):.2e} of the norm"
+
+
+@pytest.mark.parametrize("causal", [False, True])
+def test_f16_value_gradients_of_small_weights(cuda_device, causal):
+    """One key has nearly all of each query's weight, the others 2^-26 each, and their values' gradients are sums over many queries."""
+    n, dim = 9000, 64
+    q = torch.zeros(n, 1, dim, device=cuda_device, dtype=F16)
+    k, v = torch.zeros_like(q), randn(n, 1, dim, device=cuda_device, seed=1, dtype=F16)
+    q[..., 0] = 1
+    k[0, 0, 0] = 18.0                      # e^18 is 2^26
+    dout = (randn(n, 1, dim, device=cuda_device, seed=2, dtype=F32) * 0.1 + 1).half()
+    from pack3d_b200 import sequence_attention
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    out = sequence_attention(*leaves, offsets_of([n], cuda_device), causal=causal, scale=1.0)
+    got = torch.autograd.grad(out, leaves, dout)
+    _, want, tols = definition(q, k, v, dout, causal, 1.0)
+    for g, w, t in zip(got, want, tols):
+        assert ((g.double() - w).abs() <= t).all()
