@@ -325,6 +325,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       float m = -INFINITY, l = 0.f;
       for (int u = 0; u < mine; ++u, ++n) {
         const uint32_t t_u = t_s + 64 * (n & 1);
+        // Keys that some row does not see: its weights are 0, and 0 times an infinity or NaN is not. The four warps clear their quarters
+        // of the 64 values before this tile's product may read them. (The other tile's product may be under way: its own warps have
+        // cleared them, and what is written here is what is there.) Here, as S is still being made. The wait is exact: the stage's item before
+        // this one has landed, as a product of this tile that has been waited for came after it, or it was of a pair that is done.
+        if (u >= now.whole) {
+          const int item = item0 + u / 2 * 2 + 1;
+          ok = wait_warp(full(item % NS), (item / NS) & 1, &g_seq_fwd_errors, kErrSoftmax);
+          if (!ok) break;
+          clear_not_finite<T, DP / 64, kKeys / 4>(smem + (2 + item % NS) * L::kTileBytes + ((u & 1) * 4 + warp % 4) * (kKeys / 4 * 128),
+                                                  &odd_pair[done & 1], done + 1);
+        }
         ok = wait_warp(bar(kSFull + 2 * t + (n & 1)), (n >> 1) & 1, &g_seq_fwd_errors, kErrSoftmax);
         if (!ok) break;
         float s[kKeys];
@@ -379,16 +390,6 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
             }
           }
-        }
-        // Keys that some row does not see: its weights are 0, and 0 times an infinity or NaN is not. The four warps clear their quarters
-        // of the 64 values before this tile's product may read them. (The other tile's product may be under way: its own warps have
-        // cleared them, and what is written here is what is there.) The item before this one in its stage has long landed.
-        if (u >= now.whole) {
-          const int item = item0 + u / 2 * 2 + 1;
-          ok = wait_warp(full(item % NS), (item / NS) & 1, &g_seq_fwd_errors, kErrSoftmax);
-          if (!ok) break;
-          clear_not_finite<T, DP / 64, kKeys / 4>(smem + (2 + item % NS) * L::kTileBytes + ((u & 1) * 4 + warp % 4) * (kKeys / 4 * 128),
-                                                  &odd_pair[done & 1], done + 1);
         }
         tmem_wait_st();
         tc_fence_before();
