@@ -10,7 +10,7 @@
 // the exponentials are the bound. What counts is that neither waits for the other: the softmax goes by 64 keys, and each tile has two
 // buffers of S (64 columns; P of 16 bits goes over its own S), so that S of the next 64 keys is made while the softmax works on
 // these. S of 64 keys costs a third more of the pipe than half of 128, as its operands come from shared memory.
-// O is rescaled only where a row's maximum has grown by more than 2^8 (weights up to 2^8 cost no precision), after the product before
+// O is rescaled only where a row's maximum has grown by more than a slack (larger weights cost no precision), after the product before
 // has completed.
 //
 // A CTA goes through several such pairs (two thousand keys take 12 us, and setting a CTA up and taking it down 6): the next pair's
@@ -37,7 +37,11 @@ __device__ unsigned g_seq_fwd_errors = 0;
 constexpr int kMmaWarp = 8, kCopyWarp = 10, kThreads = 352;   // a warp of products for each tile
 constexpr int kKeys = 64;                    // of one softmax step
 constexpr uint32_t kColS = 0, kColO = 256;   // tensor memory: S of tile t at 128 t and 128 t + 64, O at 256 + 128 t
-constexpr float kSlack = 8.f;                // the maximum may lag by 2^8
+// The maximum may lag by 2^slack, and weights are 2^up times as large. bf16: 2^8, and as they are. f16 has no numbers below 2^-24, so the largest
+// weight is between 2^10 and 2^14 (its largest number is 2^16, what is left is for the rounding of large scores): what is lost below
+// 2^-35 of it, against 2^-25, is under half a step of the result for a million keys.
+template <typename T> constexpr float kSlack = std::is_same<T, __half>::value ? 4.f : 8.f;
+template <typename T> constexpr float kWeightUp = std::is_same<T, __half>::value ? 10.f : 0.f;
 constexpr int kPoly = 2;                     // pairs of exponentials of eight that are polynomials
 
 template <int DP>
@@ -359,7 +363,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int k = 0; k < 4; ++k) top[k] = max_nan(top[k], top[k + 4]);
         const float best = max3_nan(m, max_nan(top[0], top[1]), max_nan(top[2], top[3]));
         // a row that has seen nothing yet has an empty O: its first maximum rescales nothing
-        const bool moves = !((best - m) * sc <= kSlack) && !(best == -INFINITY);
+        const bool moves = !((best - m) * sc <= kSlack<T>) && !(best == -INFINITY);
         const bool any_moves = __any_sync(0xffffffffu, moves);
         float down = 1.f;
         if (any_moves) {
@@ -369,7 +373,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           l *= down;
         }
-        const float shift = m == -INFINITY ? 0.f : -m * sc;
+        float shift = m == -INFINITY ? 0.f : -m * sc;
+        if constexpr (kWeightUp<T> != 0.f) shift += kWeightUp<T>;
         // a border's masked scores have weight 0, which the polynomial does not give
         l += masked ? weights<T, 0>(s, sc, shift, t_u) : weights<T, kPoly>(s, sc, shift, t_u);
         // O rests once the product before has completed (waited for at every step, so that the parity is exact)
@@ -423,7 +428,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         store_rows(stage, packed, out, at, i, p.a.dim);
       }
       if (p.lse && there)
-        p.lse[(int64_t)head * p.a.q_rows + now.r.q0 + row] = seen > 0 ? (m * sc + log2f(l)) * 0.6931471805599453f : -INFINITY;
+        p.lse[(int64_t)head * p.a.q_rows + now.r.q0 + row] = seen > 0 ? (m * sc + log2f(l) - kWeightUp<T>) * 0.6931471805599453f : -INFINITY;
       // what was cleared, by this tile's warps or the other's, for the rows that see it
       if (mine && *const_cast<volatile int *>(&odd_pair[done & 1]) == done + 1)
         add_not_finite(static_cast<const T *>(p.a.v) + (int64_t)now.r.k0 * p.a.v_stride[0] + now.kv * p.a.v_stride[1], p.a.v_stride[0],

@@ -363,3 +363,24 @@ def test_f16_value_gradients_of_small_weights(cuda_device, causal):
     _, want, tols = definition(q, k, v, dout, causal, 1.0)
     for g, w, t in zip(got, want, tols):
         assert ((g.double() - w).abs() <= t).all()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("first", [True, False])
+def test_many_small_weights(cuda_device, dtype, first):
+    """One loud key whose value is 0 and 65,536 of 2^-26 of its weight: what they add up to is not lost."""
+    from pack3d_b200 import sequence_attention
+    n, rows, dim = 65537, 130, 64
+    at = 0 if first else n - 1
+    q, k = torch.zeros(rows, 2, dim, device=cuda_device, dtype=dtype), torch.zeros(n, 1, dim, device=cuda_device, dtype=dtype)
+    q[..., 0] = 1
+    k[at, 0, 0] = 18.0
+    v = (randn(n, 1, dim, device=cuda_device, seed=1, dtype=F32) * 0.25 + 1).to(dtype)
+    v[at] = 0
+    out = sequence_attention(q, k, v, offsets_of([rows], cuda_device), offsets_of([n], cuda_device), causal=False, scale=1.0)
+    p = torch.softmax(k[:, 0, 0].double(), 0)
+    want = (p[:, None] * v[:, 0].double()).sum(0)
+    # weights: half a step, and for f16 half its smallest number beside 2^10 for the largest; exponentials and sums as everywhere
+    u = torch.finfo(dtype).eps / 2
+    tol = (2 * u + 2.0 ** -13 + 2.0 ** -15) * want.abs() + (2.0 ** -35 * v[:, 0].double().abs().sum(0) if dtype is F16 else 0)
+    assert ((out.double() - want).abs() <= tol).all()
