@@ -597,8 +597,8 @@ P3D_API int p3d_sequence_bwd(const p3d_sequence *args, const void *out, const fl
  *   (contiguous, `dtype`); rows outside the sequences are set to 0, rows of bad pages to NaN.
  * p3d_paged_attention: q [sequences, heads, dim] (f16 or bf16, the cache's dtype where that is 16-bit; strides as above),
  *   out contiguous: attention of each sequence's one query over the tokens 0 .. lengths[b] of the cache; 0 where that is none,
- *   NaN where it meets a bad page.  dim up to 128.  A value's weight over 8 bits is held in f16 relative to the largest
- *   weight times 2^e.  workspace: p3d_paged_attention_workspace() bytes, 16-byte aligned.
+ *   NaN where it meets a bad page.  dim up to 128.  Weights are held in the pages' 16-bit type, over 8 bits in
+ *   f16 and times 2^e; in f16 2^10 stands for the largest.  workspace: p3d_paged_attention_workspace() bytes, 16-byte aligned.
  */
 #define P3D_E4M3 3
 typedef struct {

@@ -13,7 +13,8 @@
 //   For the registers that takes, the queries stay in shared memory. The page table is read a tile further ahead.
 // * 8 bits: e4m3 goes to f16 exactly. A query is brought below 2 by a power of two, the keys' scales multiply the scores. The
 //   values' scales 2^e go into the weights, which are held relative to the largest weighted scale, m = max(s_t + e_t), so that they
-//   fit f16 whatever the scales; the sum of weights without them stays in fp32.
+//   fit f16 whatever the scales; the sum of weights without them stays in fp32. In f16 (of either kind of page) the largest is 2^10,
+//   so that what is below 2^-35 of it is lost, against 2^-25: tens of thousands of quiet tokens behind a loud one count.
 // * Work is cut into units of four tiles (one for each warp of a CTA), laid out in one line over all sequences and KV heads, and
 //   every CTA takes an equal stretch of it: one long sequence or many uneven ones fill the device alike. A head's pieces
 //   are joined by a second kernel, in order; a stretch holds at most one head that began before it and one that goes on
@@ -85,6 +86,7 @@ __host__ __device__ constexpr int per_sm(bool k8, int dp) { return k8 && dp == 6
 template <typename T, bool k8, int DP>
 struct Tile {
   using M = typename std::conditional<k8, __half, T>::type;            // what the products take
+  static constexpr float kWeightUp = std::is_same<M, __half>::value ? 10.f : 0.f;
   static constexpr int KT = DP == 128 && !k8 ? 1 : 2, TT = 16 * KT, NT = 2 * KT;
   static constexpr int KC = k8 ? DP / 64 : DP / 32;                    // 16-byte pieces of a key that a lane holds
   static constexpr int VC = k8 ? 1 : DP / 64, VW = k8 && DP == 64 ? 2 : 4;   // pieces of a value row, words of each
@@ -331,8 +333,12 @@ struct Tile {
         m[i] = top[i];
       }
     }
-    const float2 minus[2] = {m[0] == -INFINITY ? make_float2(0.f, 0.f) : make_float2(-m[0], -m[0]),
-                             m[1] == -INFINITY ? make_float2(0.f, 0.f) : make_float2(-m[1], -m[1])};
+    float2 minus[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float by = m[i] == -INFINITY ? 0.f : kWeightUp - m[i];
+      minus[i] = make_float2(by, by);
+    }
 #pragma unroll
     for (int t = 0; t < KT; ++t) {
       uint32_t w[4];   // A operand: rows r, r + 8; tokens 2c, 2c + 1 and + 8
@@ -397,7 +403,8 @@ __device__ __forceinline__ void attend(const Params &p, Shared<DP> &sh, int b, i
   for (int j = 0; j < W::CT; ++j) w.o[j][0] = w.o[j][1] = w.o[j][2] = w.o[j][3] = 0.f;
   constexpr int64_t kStep = W::TT * kWarps;
   const int64_t first = unit0 * kStep + warp * W::TT, last = unit1 * kStep;
-  // a lane's token's scales; a value's exponent below -96 does not set the reference, so that the sum of weights stays finite
+  // a lane's token's scales; a value's exponent below -80 does not set the reference, so that the sum of weights (2^(80 + 10) of up to 2^31
+  // tokens) stays finite
   float ks = 1.f, vs = 1.f, e = 0.f;
   auto scales = [&](uint32_t row, uint32_t &kb, uint32_t &vb) {
     kb = vb = 127;
@@ -417,7 +424,7 @@ __device__ __forceinline__ void attend(const Params &p, Shared<DP> &sh, int b, i
     w.scores(s, sh.q, lane);
     if constexpr (k8) {
       ks = two_to(kb), vs = two_to(vb);
-      e = fmaxf((float)(int)vb - 127.f, -96.f);
+      e = fmaxf((float)(int)vb - 127.f, -80.f);
     }
     const bool next_all = all_there(next);
     w.load_k(p, next, next_all, lane);

@@ -347,3 +347,32 @@ def test_no_sequences_and_no_rows(cuda_device):
     assert paged_attention(empty.expand(0, 2, 64), cache, none, ints([], cuda_device)).shape == (0, 2, 64)
     assert not paged_attention(torch.ones(1, 2, 64, dtype=BF16, device=cuda_device), cache, ints([[0]], cuda_device)[:, :0],
                                ints([0], cuda_device)).any()
+
+
+@pytest.mark.parametrize("stored,dtype", [(F16, F16), (E4M3, F16), (E4M3, BF16), (BF16, BF16)])
+@pytest.mark.parametrize("first", [True, False])
+def test_many_small_weights(cuda_device, stored, dtype, first):
+    """One loud token whose values are 0 but for one and 65,535 of 2^-26 of its weight: what they add up to is not lost.  400 sequences over
+    the same pages, so that a block has whole sequences."""
+    from pack3d_b200 import PagedCache, paged_attention
+    n, dim, page, sequences = 65536, 64, 64, 400
+    at = 0 if first else n - 1
+    cache = PagedCache(n // page, 1, page, dim, dtype=stored, device=cuda_device)
+    table = torch.arange(n // page, dtype=torch.int32, device=cuda_device)[None]
+    k = torch.zeros(n, 1, dim, dtype=dtype, device=cuda_device)
+    v = (torch.randn(n, 1, dim, generator=torch.Generator(device=cuda_device).manual_seed(1), device=cuda_device) * 0.25 + 1).to(dtype)
+    k[at, 0, 0], v[at], v[at, 0, 0] = 18.0, 0, 1     # e^18 is 2^26; a value of about the others' scale
+    cache.append(k, v, table, ints([0], cuda_device), ints([0, n], cuda_device))
+    held = cache.read(table, ints([0, n], cuda_device), n, dtype=F32)
+    q = torch.zeros(sequences, 3, dim, dtype=dtype, device=cuda_device)
+    q[..., 0] = 1
+    out = paged_attention(q, cache, table.expand(sequences, -1), ints([n] * sequences, cuda_device), scale=1.0)
+    assert held[0][at, 0, 0] == 18
+    p = torch.softmax(held[0][:, 0, 0].double(), 0)
+    values = held[1][:, 0].double()
+    want = (p[:, None] * values).sum(0)
+    # weights and results: half a step each; f16 weights half of its smallest number, beside 2^10 for the largest weight times scale
+    # (values lie below 4, their scales below 2^-6); exponentials to 2^-13, fp32 sums of a thread's thousands of tokens to 2^-13
+    u = torch.finfo(dtype).eps / 2
+    tol = (2 * u + 2 * 2.0 ** -13) * want.abs() + (0 if stored is BF16 else 2.0 ** -35 * n * 448 * 2.0 ** -6)
+    assert ((out.double() - want).abs() <= tol).all()
