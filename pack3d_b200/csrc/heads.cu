@@ -145,13 +145,14 @@ struct Phases {
   }
   struct Angles {
     float c[4], s[4];
-    // R(pos), or R(-pos) for kBack, of the four pairs
+    // R(pos), or R(-pos) for kBack, of the four pairs, of which only the first `turned` turn: columns past them stand alone, whatever is
+    // beside them
     template <bool kBack>
-    __device__ __forceinline__ void turn4(float2 (&v)[4]) const {
+    __device__ __forceinline__ void turn4(int turned, float2 (&v)[4]) const {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float a = v[i].x, b = v[i].y, t = kBack ? -s[i] : s[i];
-        v[i] = make_float2(fmaf(-b, t, a * c[i]), fmaf(a, t, b * c[i]));
+        if (i < turned) v[i] = make_float2(fmaf(-b, t, a * c[i]), fmaf(a, t, b * c[i]));
       }
     }
   };
@@ -226,6 +227,7 @@ __global__ void __launch_bounds__(kWarps * 32, sizeof(T) == 2 && kVec && !kBias 
   const uint32_t token0 = warp / p.chunks;
   const float inv_dim = 1.f / p.dim;
   const bool any_layer = p.kind0 == P3D_NORM_LAYER || p.kind1 == P3D_NORM_LAYER;
+  const int turned = p.end2 - lane % S * 4;
   Phases<S> ph;
   ph.init(p, lane);
   Row row[U];
@@ -275,14 +277,16 @@ __global__ void __launch_bounds__(kWarps * 32, sizeof(T) == 2 && kVec && !kBias 
         if constexpr (kBias) v[i] = sm100::fma2(v[i], w[u][i], b[u][i]);
         else v[i] = sm100::mul2(v[i], w[u][i]);
       }
-      turn.template turn4<false>(v);
+      turn.template turn4<false>(turned, v);
       store8<T, kVec>(out[u], row[u].on ? n : 0, v);
       out[u] += row[u].out_step;
     }
   }
 }
 
-template <typename T, int S, bool kVec, bool kParams>
+// kAll: every pair of columns turns. A kernel of its own, as the choice costs a tenth here (registers; nothing in the forward). Without it the
+// parameters' sums are made whether or not anybody wants them.
+template <typename T, int S, bool kVec, bool kParams, bool kAll>
 __global__ void __launch_bounds__(kWarps * 32, sizeof(T) == 2 && kVec ? 4 : 3)
     norm_rotate_bwd_kernel(const __grid_constant__ RotateParams p) {
   constexpr int R = 32 / S;
@@ -335,7 +339,7 @@ __global__ void __launch_bounds__(kWarps * 32, sizeof(T) == 2 && kVec ? 4 : 3)
     for (int k = 0; k < 2; ++k) {
       // zeros stand for a token that is not there: its norm has to be finite
       dev[k] = normalise<S>(v[k], n, kind, there[k] ? eps : 1.f, inv_dim, any_layer);
-      turn[k].template turn4<true>(g[k]);
+      turn[k].template turn4<true>(kAll ? 4 : p.end2 - lane % S * 4, g[k]);
     }
     if constexpr (kParams) {
 #pragma unroll
@@ -376,7 +380,7 @@ __global__ void __launch_bounds__(kWarps * 32, sizeof(T) == 2 && kVec ? 4 : 3)
       out += row.out_step;
     }
   }
-  if constexpr (kParams) {
+  if (kParams && (kAll || p.partial)) {
     // the rows of a warp (each of the first or the second input), then the warps of the block, each in a fixed order
     __shared__ float2 joined[kWarps][S][4];
 #pragma unroll
@@ -527,16 +531,17 @@ int launch_s(Plan pl, bool backward, bool params, int blocks, int u, cudaStream_
   auto fwd = [&](auto vec, auto passes, auto with_bias) {
     norm_rotate_kernel<T, S, decltype(passes)::value, decltype(vec)::value, decltype(with_bias)::value><<<blocks, kWarps * 32, 0, s>>>(p);
   };
-  auto bwd = [&](auto vec, auto with_params) {
-    norm_rotate_bwd_kernel<T, S, decltype(vec)::value, decltype(with_params)::value><<<blocks, kWarps * 32, 0, s>>>(p);
+  auto bwd = [&](auto vec, auto with_params, auto all) {
+    norm_rotate_bwd_kernel<T, S, decltype(vec)::value, decltype(with_params)::value, decltype(all)::value><<<blocks, kWarps * 32, 0, s>>>(p);
   };
   using One = std::integral_constant<int, 1>;
   using Two = std::integral_constant<int, 2>;
   using Yes = std::true_type;
   using No = std::false_type;
   if (backward) {
-    if (pl.vec) params ? bwd(Yes(), Yes()) : bwd(Yes(), No());
-    else params ? bwd(No(), Yes()) : bwd(No(), No());
+    if (2 * p.end2 != p.dim) pl.vec ? bwd(Yes(), Yes(), No()) : bwd(No(), Yes(), No());
+    else if (pl.vec) params ? bwd(Yes(), Yes(), Yes()) : bwd(Yes(), No(), Yes());
+    else params ? bwd(No(), Yes(), Yes()) : bwd(No(), No(), Yes());
   } else if (!pl.vec) {
     fwd(No(), One(), Yes());
   } else if (u == 2) {
@@ -609,7 +614,7 @@ int p3d_norm_rotate_bwd(const p3d_norm_rotate *args, const void *const dy[2], vo
   pl.vec = pl.vec && aligned(dy[0]) && aligned(dy[1]) && aligned(dx[0]) && aligned(dx[1]);
   pl.p.dy0 = dy[0], pl.p.dy1 = dy[1], pl.p.y0 = dx[0], pl.p.y1 = dx[1];
   const int blocks = set_items(&pl, 1, kPerSmBackward);
-  pl.p.partial = static_cast<float *>(workspace);
+  pl.p.partial = params ? static_cast<float *>(workspace) : nullptr;
   if (params && (!workspace || workspace_bytes < sizeof(float) * 4 * (size_t)blocks * pl.p.dim))
     return fail(P3D_ERR_WORKSPACE, "p3d_norm_rotate_bwd: workspace of %zu bytes needed",
                 sizeof(float) * 4 * (size_t)blocks * pl.p.dim);

@@ -384,3 +384,30 @@ def test_many_small_weights(cuda_device, dtype, first):
     u = torch.finfo(dtype).eps / 2
     tol = (2 * u + 2.0 ** -13 + 2.0 ** -15) * want.abs() + (2.0 ** -35 * v[:, 0].double().abs().sum(0) if dtype is F16 else 0)
     assert ((out.double() - want).abs() <= tol).all()
+
+
+# ------------------------------------------------------------------------------- norms with rotation
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("dim,pairs", [(64, (5,)), (48, (3, 0, 2)), (10, (2,)), (16, (0,))])
+@pytest.mark.parametrize("value", [NAN, INF])
+def test_columns_past_the_last_pair_stand_alone(cuda_device, dtype, dim, pairs, value):
+    """They are not rotated: what is not finite in one of them reaches no other, nor does a gradient."""
+    from pack3d_b200 import norm_rotate
+    axes = len(pairs)
+    positions = torch.arange(40, device=cuda_device) if axes == 1 else torch.arange(40 * axes, device=cuda_device).view(40, axes)
+    x = randn(40, 3, dim, device=cuda_device, seed=1, dtype=dtype)
+    up = randn(40, 3, dim, device=cuda_device, seed=2, dtype=dtype)
+
+    def run(x, up):
+        leaf = x.clone().requires_grad_()
+        y, _ = norm_rotate(leaf, None, positions, pairs=pairs)
+        return y.detach(), torch.autograd.grad(y, leaf, up)[0]
+    clean = run(x, up)
+    for column in (2 * sum(pairs), dim - 1):
+        bad = [x.clone(), up.clone()]
+        for t in bad:
+            t[7, 1, column] = value
+        for got, want, given in zip(run(*bad), clean, bad):
+            expected = want.clone()
+            expected[7, 1, column] = given[7, 1, column]
+            assert torch.equal(got.nan_to_num(3.25), expected.nan_to_num(3.25))
