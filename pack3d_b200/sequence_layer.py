@@ -5,6 +5,8 @@
 :func:`~pack3d_b200.residual_norm` together.  No counterpart in the reference, whose layer attends over a geometry
 (``src/pack3d/attention.py:12-89``).
 """
+import math
+
 import torch
 from torch import nn
 
@@ -86,13 +88,16 @@ class SequenceAttention(nn.Module):
         """:meth:`forward` for the new tokens of each sequence, which go into the cache behind ``lengths`` [sequences] tokens.
 
         ``cached_rows``: the number of tokens that all sequences have with these, where any had some before: keys and values are
-        then read back from the cache (as it holds them, the new ones too).  Without it every length is taken to be 0.  No
-        gradients.
+        then read back from the cache (as it holds them, the new ones too).  Without it the sequences that have new tokens
+        have to begin with them: where one of those has a length, its first tokens would be missing, and all results are
+        NaN.  No gradients.
         """
         q, k, v = self._qkv(x, positions, normed)
         cache.append(k, v, table, lengths, offsets)
         if cached_rows is None:
             a = sequence_attention(q, k, v, offsets, causal=self.causal)
+            # lengths are on the device: a refusal would wait for it
+            a.masked_fill_(((lengths != 0) & (offsets.diff() != 0)).any(), math.nan)
         else:
             all_offsets = torch.nn.functional.pad((lengths + offsets.diff()).cumsum(0, dtype=torch.int32), (1, 0))
             k, v = cache.read(table, all_offsets, cached_rows, dtype=q.dtype)

@@ -184,3 +184,17 @@ def test_layer_refusals(cuda_device):
         table, pages = table_of(1, 2, cuda_device)
         m.decode(torch.zeros(1, 256, device=cuda_device, dtype=BF16), torch.zeros(1, dtype=torch.long, device=cuda_device),
                  m.new_cache(pages, 16), table, torch.zeros(1, dtype=torch.int32, device=cuda_device))
+
+
+@pytest.mark.parametrize("had,n", [([3, 0], [30, 9]), ([0, 1], [30, 9]), ([0, 0], [30, 9]), ([7, 0], [0, 9]), ([0, 5], [30, 0])])
+def test_a_second_prompt_needs_the_cached_rows(cuda_device, had, n):
+    """Without `cached_rows` a sequence begins with its new tokens: where one that has some had others already, the results say so."""
+    m = layer(cuda_device, BF16)
+    x = torch.randn(sum(n), 256, device=cuda_device, dtype=BF16)
+    table, pages = table_of(2, 4, cuda_device)
+    offsets, lengths = offsets_of(n, cuda_device), torch.tensor(had, dtype=torch.int32, device=cuda_device)
+    cache = m.new_cache(pages, 16)
+    with torch.no_grad():
+        got, _ = m.prefill(x, positions_of(n, cuda_device), offsets, cache, table, lengths)
+        want, _ = m(x, positions_of(n, cuda_device), offsets)
+    assert got.isnan().all() if any(a and b for a, b in zip(had, n)) else torch.equal(got, want)
