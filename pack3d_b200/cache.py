@@ -72,8 +72,10 @@ def paged_attention(q, cache, table, lengths, *, scale=None):
     its pages (the new token's own among them, once appended); 0 for a sequence without any.
 
     fp16 or bf16 queries, of the cache's dtype where that is 16-bit, or any of the two over 8 bits; head_dim up to 128; heads
-    a multiple of the cache's.  Scores and sums in fp32; what 8 bits hold enters exactly.  The order of a sum depends on the
-    lengths alone.  No gradients.
+    a multiple of the cache's.  Scores and sums in fp32, weights rounded to the pages' 16-bit type; over 8 bits, which enter
+    exactly, to fp16, as queries are relative to their largest column.  The same call gives the same bits: the order of a
+    sum depends on the batch's lengths, the heads, the device, and on whether the table is wider than four units of 128 tokens
+    (of 64, over 16-bit pages with a head_dim above 64), not on how much wider.  No gradients.
     """
     if not isinstance(cache, PagedCache):
         raise ValueError("paged_attention takes a PagedCache")

@@ -376,3 +376,26 @@ def test_many_small_weights(cuda_device, stored, dtype, first):
     u = torch.finfo(dtype).eps / 2
     tol = (2 * u + 2 * 2.0 ** -13) * want.abs() + (0 if stored is BF16 else 2.0 ** -35 * n * 448 * 2.0 ** -6)
     assert ((out.double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("stored,dim", [(BF16, 64), (BF16, 128), (E4M3, 128)])
+def test_wider_tables(cuda_device, stored, dim):
+    """The same lengths under tables of any width, on both sides of the one from which work is cut over sequences: the same result up to the
+    order of its sums, whatever the columns that no token reaches hold."""
+    from pack3d_b200 import paged_attention
+    lengths, page = [100, 0, 256, 1, 200], 16
+    cache, table, held, q = filled(lengths, 2, dim, page, stored, cuda_device, heads=4)
+    want, tol = decode_reference(q, held, lengths, dim ** -0.5)
+    n = ints(lengths, cuda_device)
+    seen = {}
+    unit = 4 * (16 if dim == 128 and stored is not E4M3 else 32)
+    for width in (table.shape[1], 4 * unit // page, 4 * unit // page + 1, 10 * unit // page, 2000):
+        more = width - table.shape[1]
+        wide = torch.cat([table, torch.full((len(lengths), max(more, 0)), -7, dtype=torch.int32, device=cuda_device)], 1)
+        got = paged_attention(q, cache, wide, n)
+        assert torch.equal(got, paged_attention(q, cache, wide, n))
+        assert ((got.double() - want).abs() <= tol).all()
+        # the order depends on which side of four units the table is, and on no more of its width
+        side = wide.shape[1] * page > 4 * unit
+        assert torch.equal(got, seen.setdefault(side, got))
+    assert len(seen) == 2
