@@ -592,7 +592,7 @@ P3D_API int p3d_sequence_bwd(const p3d_sequence *args, const void *out, const fl
  *   written; it sets bit 6 (64) of p3d_device_errors.  The same holds for places past table_width pages.
  * p3d_cache_append: row offsets[b] + i of new_k, new_v (of `dtype`; [rows, kv_heads, dim], strides in elements) becomes
  *   token starts[b] + i of sequence b.  Rows outside the sequences are not read; two rows for one place leave
- *   either of them.
+ *   a mixture of them.
  * p3d_cache_read: token starts[b] + i (starts NULL: i) of sequence b into row offsets[b] + i of out_k, out_v [rows, kv_heads, dim]
  *   (contiguous, `dtype`); rows outside the sequences are set to 0, rows of bad pages to NaN.
  * p3d_paged_attention: q [sequences, heads, dim] (f16 or bf16, the cache's dtype where that is 16-bit; strides as above),
