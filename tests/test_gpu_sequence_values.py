@@ -411,3 +411,45 @@ def test_columns_past_the_last_pair_stand_alone(cuda_device, dtype, dim, pairs, 
             expected = want.clone()
             expected[7, 1, column] = given[7, 1, column]
             assert torch.equal(got.nan_to_num(3.25), expected.nan_to_num(3.25))
+
+
+@pytest.mark.parametrize("tokens,heads,kv,dim,kind", [(4097, 3, 1, 64, "rms"), (1000, 32, 8, 128, "layer"), (263, 4, 4, 48, "layer"), (1, 1, 1, 8, "rms"),
+                                                      (5000, 1, 7, 250, "rms")])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_every_row_counts_in_the_parameters_gradients(cuda_device, tokens, heads, kv, dim, kind, dtype):
+    """Upstream gradients in one row alone (the first and last token, head, of each input), and in all: sums to 2^-18 of their magnitudes."""
+    from pack3d_b200 import NormSpec, norm_rotate
+    x = [randn(tokens, h, dim, device=cuda_device, seed=s, dtype=dtype, scale=2.0) for s, h in enumerate((heads, kv))]
+    positions = torch.arange(tokens, device=cuda_device) * 7 + 100000
+    params = [[(1 + 0.2 * randn(dim, device=cuda_device, seed=5 + i, dtype=F32)).requires_grad_(), randn(dim, device=cuda_device, seed=7 + i, dtype=F32).requires_grad_()]
+              for i in range(2)]
+    spec = [NormSpec(*p, kind, 1e-5) for p in params]
+    leaves = [t for p in params for t in p]
+    y = norm_rotate(*x, positions, q_norm=spec[0], k_norm=spec[1])
+    angle = positions.double()[:, None] * 10000.0 ** (-torch.arange(dim // 2, device=cuda_device).double() / (dim // 2))
+    cos, sin = angle.cos()[:, None], angle.sin()[:, None]
+    for where in [None] + [(i, t, h) for i, n in enumerate((heads, kv)) for t in sorted({0, tokens - 1}) for h in sorted({0, n - 1})]:
+        up = [randn(tokens, h, dim, device=cuda_device, seed=20 + i, dtype=dtype) for i, h in enumerate((heads, kv))]
+        if where is not None:
+            i, t, h = where
+            kept = up[i][t, h].clone()
+            for u in up:
+                u.zero_()
+            up[i][t, h] = kept
+        got = torch.autograd.grad(y, leaves, up, retain_graph=True)
+        for i in range(2):
+            z = x[i].double()
+            top = z.abs().amax(-1, keepdim=True)
+            if kind == "layer":
+                z = z - z.mean(-1, keepdim=True)
+            r = 1 / torch.sqrt(z.square().mean(-1, keepdim=True) + 1e-5)
+            z, own = z * r, top * r if kind == "layer" else 0
+            a, b = up[i].double()[..., 0::2], up[i].double()[..., 1::2]
+            g = torch.stack((a * cos + b * sin, b * cos - a * sin), -1).flatten(-2)
+            # sine and cosine to 2^-21 and a product in fp32, of both columns of a pair; the deviation and sums in fp32
+            size = torch.stack((a.abs() + b.abs(),) * 2, -1).flatten(-2)
+            # a mean in fp32 is off by 2^-21 of the row's largest magnitude (eight levels of additions, the division), however near
+            # to it the column lies: z is off by as much of that over the deviation
+            wrong = size * (2.0 ** -18 * z.abs() + 2.0 ** -21 * own)
+            for have, want, most in ((got[2 * i], (g * z).sum((0, 1)), wrong.sum((0, 1))), (got[2 * i + 1], g.sum((0, 1)), 2.0 ** -18 * size.sum((0, 1)))):
+                assert ((have.double() - want).abs() <= most + 2.0 ** -24 * want.abs()).all()
