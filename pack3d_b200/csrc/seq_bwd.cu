@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ __align__(8) uint64_t bar_mem[kBarsQ];
   __shared__ uint32_t tmem_holder;
   __shared__ int odd_keys;   // keys have been cleared
-  __shared__ float most_v[kThreads / 32];
+  __shared__ float most_v[kSoftmaxWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int slot = blockIdx.x / p.a.heads, head = blockIdx.x % p.a.heads;
   const int kv = head / (p.a.heads / p.a.kv_heads);
@@ -183,13 +183,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     prefetch_tmap(&tdo);
     prefetch_tmap(&tk);
     prefetch_tmap(&tv);
-  }
-  if constexpr (kScaled<T>) {
-    const float *norm = p.v_norm + kv * p.a.k_rows + r.k0;
-    float most = 0.f;
-#pragma unroll 4
-    for (int j = threadIdx.x; j < min(chunks * kTile, r.nk); j += kThreads) most = fmaxf(most, finite_or_0(norm[j]));
-    most_v[warp] = warp_most(most);
   }
   tc_fence_before();
   __syncthreads();
@@ -314,9 +307,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     const float2 stat = there ? p.stats[(int64_t)head * p.a.q_rows + r.q0 + row] : make_float2(0.f, 0.f);
     int up = 0;   // dS is 2^up times as large
     if constexpr (kScaled<T>) {
-      float v = most_v[0];
-      for (int i = 1; i < kThreads / 32; ++i) v = fmaxf(v, most_v[i]);
-      if (there) up = exponent_for(fmaf(p.dout_norm[(int64_t)head * p.a.q_rows + r.q0 + row], p.a.scale * v, fabsf(stat.y)));
+      // while the first tiles are on their way; all eight warps come by here, before any wait that could end early
+      const float own = there ? p.dout_norm[(int64_t)head * p.a.q_rows + r.q0 + row] : 0.f, *const norm = p.v_norm + kv * p.a.k_rows + r.k0;
+      float v = 0.f;
+#pragma unroll 4
+      for (int j = threadIdx.x; j < min(chunks * kTile, r.nk); j += kSoftmaxWarps * 32) v = fmaxf(v, finite_or_0(norm[j]));
+      most_v[warp] = warp_most(v);
+      asm volatile("bar.sync 1, %0;" ::"n"(kSoftmaxWarps * 32) : "memory");
+#pragma unroll
+      for (int i = 0; i < kSoftmaxWarps; ++i) v = fmaxf(v, most_v[i]);
+      up = exponent_for(fmaf(own, p.a.scale * v, fabsf(stat.y)));
     }
     const float one = seen == 1 ? 0.f : p.a.scale * two_to(up), less = seen == 1 ? 0.f : stat.y * two_to(up);
     const float2 sc = make_float2(p.sc, p.sc), shift = make_float2(stat.x, stat.x), minus = make_float2(less, less), scale = make_float2(one, one);
@@ -462,6 +462,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     return;
   }
+  // of the queries of every head: the first ones' norms are asked for before the set-up
+  const int64_t stat0 = (int64_t)head0 * p.a.q_rows + r.q0;
+  float early_n = 0.f, early_y = 0.f, early_v = 0.f;
+  if constexpr (kScaled<T>) {
+    const int i = first + threadIdx.x;
+    if (i < r.nq) early_n = p.dout_norm[stat0 + i], early_y = p.stats[stat0 + i].y;
+    if (threadIdx.x < min(kTile, r.nk - key0)) early_v = p.v_norm[kv * p.a.k_rows + r.k0 + key0 + threadIdx.x];
+  }
   const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
   uint8_t *const smem = smem_raw + (base - raw);
   const uint32_t ring = base + 2 * TB;
@@ -486,25 +494,25 @@ __global__ void __launch_bounds__(kThreads, 1)
     prefetch_tmap(&tv);
   }
   if constexpr (kScaled<T>) {
-    float n = 0.f, y = 0.f;
-    for (int64_t at = (int64_t)head0 * p.a.q_rows + r.q0, h = 0; h < heads; ++h, at += p.a.q_rows)
+    float n = finite_or_0(early_n), y = finite_or_0(fabsf(early_y));
+    for (int h = 0; h < heads; ++h) {
+      const int64_t to = stat0 + h * p.a.q_rows;
 #pragma unroll 4
-      for (int i = first + threadIdx.x; i < r.nq; i += kThreads) {
-        n = fmaxf(n, finite_or_0(p.dout_norm[at + i]));
-        y = fmaxf(y, finite_or_0(fabsf(p.stats[at + i].y)));
+      for (int i = first + threadIdx.x + (h ? 0 : kThreads); i < r.nq; i += kThreads) {
+        n = fmaxf(n, finite_or_0(p.dout_norm[to + i]));
+        y = fmaxf(y, finite_or_0(fabsf(p.stats[to + i].y)));
       }
-    const int mine = key0 + threadIdx.x;
-    const float v = threadIdx.x < kTile && mine < r.nk ? finite_or_0(p.v_norm[kv * p.a.k_rows + r.k0 + mine]) : 0.f;
-    most[0][warp] = warp_most(n), most[1][warp] = warp_most(y), most[2][warp] = warp_most(v);
+    }
+    most[0][warp] = warp_most(n), most[1][warp] = warp_most(y), most[2][warp] = warp_most(finite_or_0(early_v));
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_holder, t_dp = tmem + 128, t_dk = tmem + 256, t_dv = tmem + 384;
-  auto exponent = [&] {   // dS is that power of two times as large
+  auto exponent = [&] {   // dS is that power of two times as large (by a warp)
     if constexpr (kScaled<T>) {
-      float n = 0.f, y = 0.f, v = 0.f;
-      for (int i = 0; i < kThreads / 32; ++i) n = fmaxf(n, most[0][i]), y = fmaxf(y, most[1][i]), v = fmaxf(v, most[2][i]);
+      const int i = min(lane, kThreads / 32 - 1);
+      const float n = warp_most(most[0][i]), y = warp_most(most[1][i]), v = warp_most(most[2][i]);
       return exponent_for(fmaf(n, p.a.scale * v, y));
     } else {
       return 0;
@@ -515,7 +523,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == kCopyWarp) {
     bool ok = true;
     int issued = 0, cleared = 0;
-    const float times = two_to(exponent() - kUp);
     if (lane == 0) {
       mbar_expect_tx(bar(kKVFull), 2 * TB);
       for (int c = 0; c < DP / 64; ++c) {
@@ -523,6 +530,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         tma_load_3d(base + TB + c * kBox, &tv, bar(kKVFull), 64 * c, kv, r.k0 + key0);
       }
     }
+    __syncwarp();
+    const float times = two_to(exponent() - kUp);
     for (int n = 0, head = head0, i0 = first; n < steps; ++n) {
       const int s = n % NS;
       float2 v[4];
@@ -755,41 +764,41 @@ __global__ void __launch_bounds__(256) stats_kernel(const T *out, const float *l
   const T *const dout = static_cast<const T *>(p.dout);
   const int lane = threadIdx.x & 31, per_warp = 32 / lanes, col = lane % lanes * 8, dim = p.a.dim;
   const int64_t row_first = ((int64_t)blockIdx.x * 8 + threadIdx.x / 32) * per_warp, stride = (int64_t)gridDim.x * 8 * per_warp;
+  const int64_t q_rows = p.a.q_rows * p.a.heads, v_rows = kScaled<T> ? p.a.k_rows * p.a.kv_heads : 0;
   // whole warps take part in the sums: rows past the last are zeros
-  for (int64_t row0 = row_first; row0 < p.a.q_rows * p.a.heads; row0 += stride) {
+  for (int64_t row0 = row_first; row0 < max(q_rows, v_rows); row0 += stride) {
     const int64_t row = row0 + lane / lanes;
-    const bool there = row < p.a.q_rows * p.a.heads;
-    float2 a[4], b[4];
+    const bool there = row < q_rows, value = row < v_rows;
+    float2 a[4], b[4], v[4];
     load8(out + row * dim + col, there && col < dim, a);
     load8(dout + row * dim + col, there && col < dim, b);
-    float sum = 0.f, square = 0.f;
+    const int64_t key = row / p.a.kv_heads, kv = row - key * p.a.kv_heads;
+    if constexpr (kScaled<T>)
+      load8(static_cast<const T *>(p.a.v) + key * p.a.v_stride[0] + kv * p.a.v_stride[1] + col, value && col < dim, v);
+    float sum = 0.f, square = 0.f, square_v = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       sum = fmaf(a[i].x, b[i].x, fmaf(a[i].y, b[i].y, sum));
-      if constexpr (kScaled<T>) square = fmaf(b[i].x, b[i].x, fmaf(b[i].y, b[i].y, square));
+      if constexpr (kScaled<T>) {
+        square = fmaf(b[i].x, b[i].x, fmaf(b[i].y, b[i].y, square));
+        square_v = fmaf(v[i].x, v[i].x, fmaf(v[i].y, v[i].y, square_v));
+      }
     }
     for (int o = lanes / 2; o > 0; o >>= 1) {
       sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      if constexpr (kScaled<T>) square += __shfl_xor_sync(0xffffffffu, square, o);
+      if constexpr (kScaled<T>) {
+        square += __shfl_xor_sync(0xffffffffu, square, o);
+        square_v += __shfl_xor_sync(0xffffffffu, square_v, o);
+      }
     }
-    if (there && lane % lanes == 0) {
+    if (lane % lanes) continue;
+    if (there) {
       const int64_t t = row / p.a.heads, to = (row - t * p.a.heads) * p.a.q_rows + t;
       stats[to] = make_float2(lse[to] * -1.4426950408889634f, sum * -p.a.scale);
       if constexpr (kScaled<T>) dout_norm[to] = sqrtf(square);
     }
-  }
-  if constexpr (kScaled<T>) {
-    for (int64_t row0 = row_first; row0 < p.a.k_rows * p.a.kv_heads; row0 += stride) {
-      const int64_t row = row0 + lane / lanes, t = row / p.a.kv_heads, head = row - t * p.a.kv_heads;
-      const bool there = row < p.a.k_rows * p.a.kv_heads;
-      float2 v[4];
-      load8(static_cast<const T *>(p.a.v) + t * p.a.v_stride[0] + head * p.a.v_stride[1] + col, there && col < dim, v);
-      float square = 0.f;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) square = fmaf(v[i].x, v[i].x, fmaf(v[i].y, v[i].y, square));
-      for (int o = lanes / 2; o > 0; o >>= 1) square += __shfl_xor_sync(0xffffffffu, square, o);
-      if (there && lane % lanes == 0) v_norm[head * p.a.k_rows + t] = sqrtf(square);
-    }
+    if constexpr (kScaled<T>)
+      if (value) v_norm[kv * p.a.k_rows + key] = sqrtf(square_v);
   }
 }
 
@@ -819,7 +828,7 @@ int launch_t(const Params &p, const void *out, const float *lse, float2 *stats, 
   const p3d_sequence &a = p.a;
   CUtensorMap tq, tdo, tk, tv;
   if (a.q_rows && a.k_rows) {
-    const int64_t rows = a.q_rows * a.heads;
+    const int64_t rows = std::max(a.q_rows * a.heads, kScaled<T> ? a.k_rows * a.kv_heads : 0);
     int lanes = 1;
     while (lanes * 8 < a.dim) lanes *= 2;
     const int64_t blocks = std::min<int64_t>((rows * lanes + 255) / 256, 148 * 16);

@@ -335,7 +335,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // this one has landed, as a product of this tile that has been waited for came after it, or it was of a pair that is done.
         if (u >= now.whole) {
           const int item = item0 + u / 2 * 2 + 1;
-          ok = wait_warp(full(item % NS), (item / NS) & 1, &g_seq_fwd_errors, kErrSoftmax);
+          if (u == now.whole || u % 2 == 0) ok = wait_warp(full(item % NS), (item / NS) & 1, &g_seq_fwd_errors, kErrSoftmax);
           if (!ok) break;
           clear_not_finite<T, DP / 64, kKeys / 4>(smem + (2 + item % NS) * L::kTileBytes + ((u & 1) * 4 + warp % 4) * (kKeys / 4 * 128),
                                                   &odd_pair[done & 1], done + 1);

@@ -202,10 +202,11 @@ __device__ __forceinline__ void clear_not_finite(uint8_t *tile, volatile int *fl
 #pragma unroll
   for (int i = 0; i < kBoxes * kEach; ++i)
     w[i] = *reinterpret_cast<const uint4 *>(tile + i / kEach * kBox + i % kEach * 512 + (threadIdx.x & 31) * 16);
+  const int set = *flag;
 #pragma unroll
   for (int i = 0; i < kBoxes * kEach; ++i) add(w[i].x), add(w[i].y), add(w[i].z), add(w[i].w);
   if (!__any_sync(0xffffffffu, (sum & 0x7fff7fffu) != 0)) {
-    if (*flag == value) fence_proxy_async_smem();   // what another warp has written, for this one's product
+    if (set == value) fence_proxy_async_smem();   // what another warp has written, for this one's product
     return;
   }
   if ((threadIdx.x & 31) == 0) *flag = value;
