@@ -331,9 +331,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       tmem_wait_ld();
       const int limit = seen - c * kTile - half * 64;
       const bool masked = __any_sync(0xffffffffu, limit < 64);
-      if (masked) {
-        // Scores that are not finite where some row does not see the key: these 64 keys are cleared. Every warp that needs it does so, by
-        // now S has been made of them and dQ waits for all warps; what one has cleared another leaves as it is.
+      if (masked && __any_sync(0xffffffffu, there && limit < 64)) {
+        // Scores that are not finite where some row of the sequence does not see the key (rows behind its end count for nothing: what is
+        // cleared has to lie among the keys that add_not_finite goes over): these 64 keys are cleared. Every warp that needs it does
+        // so, by now S has been made of them and dQ waits for all warps; what one has cleared another leaves as it is.
         float2 odd = make_float2(0.f, 0.f);
 #pragma unroll
         for (int i = 0; i < 32; ++i) odd = fma2(make_float2(s[2 * i], s[2 * i + 1]), make_float2(0.f, 0.f), odd);

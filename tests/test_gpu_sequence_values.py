@@ -135,6 +135,37 @@ def test_later_values_keep_out_of_earlier_rows(cuda_device, value, at, heads, kv
             assert (at == 0 or got[1][at, 0].isnan().any()) and not got[2][:at + 1, 0].isfinite().all()
 
 
+@pytest.mark.parametrize("n", [130, 256, 300])
+@pytest.mark.parametrize("at", [0, 1, 63, 64, 127, 129])
+@pytest.mark.parametrize("heads,kv,dim,dtype", [(2, 1, 64, BF16), (3, 3, 128, F16)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_a_key_without_weight_that_is_infinite(cuda_device, n, at, heads, kv, dim, dtype, causal):
+    """A key whose score is -inf for every query has no weight, and its score gradient is 0: times the infinity, NaN in that column of dq for
+    every query that sees it, whole tile or not; all else as if the key were not seen."""
+    offsets = offsets_of([n], cuda_device)
+    q, k, v, dout = (randn(n, h, dim, device=cuda_device, seed=s, dtype=dtype) for s, h in enumerate((heads, kv, kv, heads)))
+    q[:, :, 3] = 1
+    k[at, :, 3] = -INF
+    (out, dq, dk, dv), _ = step(q, k, v, dout, offsets, causal=causal)
+    sees = torch.ones(n, dtype=torch.bool, device=cuda_device)
+    if causal:
+        sees[:at] = False
+    nothing = sees.clone()
+    nothing[1 if causal and at == 0 else 0:] = False        # a query that sees that key alone
+    keep = torch.arange(dim, device=cuda_device) != 3
+    assert dq[sees][..., 3].isnan().all() and dq[~sees].isfinite().all()
+    assert out[~nothing].isfinite().all() and dq[~nothing][..., keep].isfinite().all()
+    if not nothing.any():
+        assert not dk[at].any() and not dv[at].any() and dk.isfinite().all() and dv.isfinite().all()
+    other = torch.arange(n, device=cuda_device) != at
+    if not causal:
+        want, _ = step(q, k[other], v[other], dout, offsets, causal=False, k_offsets=offsets_of([n - 1], cuda_device))
+        u = torch.finfo(dtype).eps / 2
+        # the same sums in another order of tiles: weights and score gradients round alike, the accumulations in fp32 do not
+        for a, b in ((out, want[0]), (dq[..., keep], want[1][..., keep]), (dk[other], want[2]), (dv[other], want[3])):
+            assert (a.double() - b.double()).norm() <= 8 * u * b.double().norm()
+
+
 def test_signs_that_meet(cuda_device):
     """A column with infinities of both signs is NaN from the second on, and the first one's sign in between; the same of gradients, from
     the other end."""
