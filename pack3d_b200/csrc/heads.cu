@@ -17,7 +17,8 @@
 //
 // Measured, bf16: 16,384 tokens of 32 + 8 heads of 128, forward 70 us (4.8 TB/s), backward 110 (4.6); 262,144 tokens of 4 + 4 heads of
 // 48 on three axes, 91 (4.4) and 145 (4.2), where two lanes of eight are idle. Issue slots are 60 % used at 30 and 23 % occupancy: the
-// registers of the rows ahead and of the sums are what more warps would need.
+// registers of the rows ahead and of the sums are what more warps would need. At those dims the forward spills nothing up to 64 columns and 32
+// bytes of two passes of 128, the backward 12; above 128 columns 124 and up to 196 (not measured).
 #include <math.h>
 
 #include <algorithm>

@@ -20,8 +20,8 @@ def norm_rotate(q, k, positions, *, q_norm=None, k_norm=None, pairs=None, base=1
     ``positions``: int32 or int64, [tokens], or [tokens, axes] for up to three axes, shared by the leading dimensions.  The
     axes own the pairs of columns (2 i, 2 i + 1) in turn, ``pairs`` of them each (default: all of them, dealt evenly, as
     :func:`~pack3d_b200.balanced_pairs`); columns past the last pair are not rotated.  Pair i of n of an axis turns by
-    ``position * base**(-i / n)`` radians.  Angles are exact at any position: unlike
-    :func:`~pack3d_b200.rotate_projections`, which has the reference's fp32 angles bit for bit.
+    ``position * base**(-i / n)`` radians.  A frequency is that power in fp64, to 2^-64 turns, and its product with the position
+    is exact, unlike in :func:`~pack3d_b200.rotate_projections`, which has the reference's fp32 angles bit for bit.
 
     fp32, fp16 or bf16, an even head_dim up to 256, any strides; statistics in fp32, one rounding at the end.  Results are
     contiguous.  Differentiable once in q, k and the norms' parameters, whose gradients are summed in fp32 in a fixed
@@ -40,11 +40,12 @@ def sequence_attention(q, k, v, q_offsets, k_offsets=None, *, causal=True, scale
     last key, each query before it one key less.  ``scale``: default ``head_dim ** -0.5``.
 
     A query that sees no key gives 0 and sends no gradient, as do rows behind the last sequence, whatever they hold.  An
-    infinity or NaN reaches the queries that see it, and no other sequence.
+    infinity or NaN reaches the queries that see it and nothing else: no earlier query, no other sequence.  A query with a score
+    of +inf, or with none but -inf, has no softmax: NaN.
 
     fp16 or bf16, head_dim a multiple of 8 up to 128; rows that are not 16-byte aligned are copied first.  Scores and sums in
     fp32; what goes into a product (weights, and score gradients from the rounded output) is rounded to the inputs' dtype, in
-    fp16 times powers of two that bring it into range.  Every sum has a fixed order, so the gradients are bitwise
+    fp16 times powers of two that bring it into range; exponentials are good to 2^-13.  Every sum has a fixed order, so the gradients are bitwise
     repeatable.  Differentiable once, in reverse mode; second and forward-mode derivatives are
     refused.
     """
