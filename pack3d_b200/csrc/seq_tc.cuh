@@ -169,8 +169,8 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
 // Masked weights and values that are not finite.  A masked weight is 0, but 0 times an infinity or NaN is NaN: a product over a whole tile
 // would pass on what a row does not see. So in tiles that some row does not see whole, such values are set to 0 before the product reads
 // them (clear_not_finite), and added again to the rows that see them once the sum is there (add_not_finite): an infinity whose weight is
-// positive makes the sum that infinity, two that meet make it NaN. Each such value is looked at once for 32 rows, so the work is bounded
-// by what is read anyway, whatever the values are.
+// positive makes the sum that infinity, two that meet make it NaN (a value whose key has a score of -inf counts by its sign). Each such
+// value is looked at once for 32 rows, so the work is bounded by what is read anyway, whatever the values are.
 // * Forward: the softmax warps look through the values of those tiles before they hand over their weights.
 // * dQ: a key that is not finite makes the scores of its column not finite, also of the rows that do not see it: the softmax warps have them.
 //   A query that sees the key has no score gradient there (its score is -inf: 0 times the infinity) or nowhere: NaN.
